@@ -1,0 +1,641 @@
+// The 4-bit cache (kv4.cuh): writing rows to it, reading them back, and causal attention over it.
+//
+// Rows of one segment are consecutive rows of q (cu_rows); row r of segment i stands at key index p = seg_pos[i] + r and
+// reads the keys max(0, p - window + 1) .. p (no window: 0 .. p).  A row with no key (p < 0) gives zeros.
+#include "kv4.cuh"
+
+// ------------------------------------------------------------------ write and read
+// A thread takes 8 consecutive values of a group; the lanes of a group (8, or 4) find its range together.
+__device__ __forceinline__ float kv4_min_nan(float a, float b) { float d; asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
+__device__ __forceinline__ float kv4_max_nan(float a, float b) { float d; asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void kv4_load8(float (&v)[8], const T* p) {
+    if (VEC && sizeof(T) == 2) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else if (VEC) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f32(p[i]);
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+kv4_write_kernel(const T* __restrict__ k, long long ldk, const T* __restrict__ v, long long ldv, unsigned char* __restrict__ pages,
+                 const int* __restrict__ slot_map, long long n_slots, int n, int ps, int G, int hd, int gs) {
+    kp_pdl_begin();
+    const int per_row = G * hd / 8;                        // threads a row of k (and of v)
+    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long unit = idx / per_row;                  // (row, k or v)
+    const int within = (int)(idx - unit * per_row);
+    const bool live = unit < 2LL * n;
+    const int row = live ? (int)(unit >> 1) : 0;
+    const bool is_v = unit & 1;
+    const int head = within / (hd / 8), d8 = within - head * (hd / 8);
+    const int lanes = gs / 8;                              // of a group
+    const long long slot = live ? slot_map[row] : -1;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = 0.f;
+    if (slot >= 0 && slot < n_slots) kv4_load8<T, VEC>(x, (is_v ? v + row * ldv : k + row * ldk) + (size_t)head * hd + d8 * 8);
+    // a range that holds a NaN, or an infinity, is none: the group reads as NaN
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) { lo = kv4_min_nan(lo, x[i]); hi = kv4_max_nan(hi, x[i]); }
+    for (int d = 1; d < lanes; d <<= 1) {
+        lo = kv4_min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+        hi = kv4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    }
+    if (slot < 0 || slot >= n_slots) return;
+    const bf16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.0f)), zb = __float2bfloat16_rn(lo);
+    const float s = __bfloat162float(sb), z = __bfloat162float(zb);
+    uint32_t w = 0;
+    if (s > 0.f) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) w |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i] - z, s)), 0.f), 15.f) << (4 * i);
+    }
+    const int page = (int)(slot / ps), off = (int)(slot - (long long)page * ps), ng = hd / gs;
+    unsigned char* rec = pages + ((size_t)page * G + head) * kv4_page_bytes(ps, hd);
+    unsigned char* codes = rec + (is_v ? (size_t)ps * (hd / 2) : 0) + (size_t)off * (hd / 2);
+    *reinterpret_cast<uint32_t*>(codes + d8 * 4) = w;
+    if (d8 % lanes == 0) {
+        unsigned char* ranges = rec + (size_t)ps * hd + (is_v ? (size_t)ps * 4 * ng : 0);
+        reinterpret_cast<uint32_t*>(ranges)[off * ng + d8 / lanes] =
+            (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+kv4_read_kernel(const unsigned char* __restrict__ pages, const int* __restrict__ slot_map, long long n_slots, T* __restrict__ k, T* __restrict__ v,
+                int n, int ps, int G, int hd, int gs) {
+    kp_pdl_begin();
+    const int per_row = G * hd / 8;
+    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long unit = idx / per_row;
+    if (unit >= 2LL * n) return;
+    const int within = (int)(idx - unit * per_row);
+    const int row = (int)(unit >> 1);
+    const bool is_v = unit & 1;
+    const int head = within / (hd / 8), d8 = within - head * (hd / 8), ng = hd / gs;
+    const long long slot = slot_map[row];
+    float x[8];
+    if (slot >= 0 && slot < n_slots) {
+        const int page = (int)(slot / ps), off = (int)(slot - (long long)page * ps);
+        const unsigned char* rec = pages + ((size_t)page * G + head) * kv4_page_bytes(ps, hd);
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + (is_v ? (size_t)ps * (hd / 2) : 0) + (size_t)off * (hd / 2) + d8 * 4);
+        const uint32_t r = reinterpret_cast<const uint32_t*>(rec + (size_t)ps * hd + (is_v ? (size_t)ps * 4 * ng : 0))[off * ng + d8 / (gs / 8)];
+        const float s = kv4_scale(r), z = kv4_least(r);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = fmaf(s, (float)((w >> (4 * i)) & 15u), z);       // (s c is exact)
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = 0.f;            // a row without a slot reads as zeros
+    }
+    T* dst = (is_v ? v : k) + (size_t)row * G * hd + within * 8;
+    if (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+    } else {
+        reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
+
+// ------------------------------------------------------------------ attention
+struct Kv4Args {
+    const void* q; long long ldq;
+    void* out; long long ldo;
+    const unsigned char* pages;
+    const int* block_table; int max_blocks;
+    const int* cu_rows; const int* seg_pos;
+    float scale; int window; int ps; int H, G;
+    // split form, [place] = [segment][row of it, of max_rows][head]: results of chunks [place][chunk][hd], (shift, sum of p)
+    // [place][chunk][2]; with mass, or else null: scores [place][key], shift + log2(sum of p) [place]
+    float* part_o; float* part_ml; float* scores; int ld_scores; float* lse_split;
+    float* lse;                                            // tiled form with mass: shift + log2(sum of p) (base 2) [row][head], or null
+    float* mass;                                           // [page][G][ps], or null
+    int n_chunks, chunk;                                   // split form: chunks of `chunk` keys
+    int max_rows;                                          // split form: segments of more rows are not its own
+    int min_rows;                                          // tiled form: nor are segments of fewer rows this form's
+    int n_seg;
+};
+
+// What a warp knows of its columns: column c of a segment stands for row c / R and head kvh R + c % R.
+template <int NT>
+struct Kv4Cols { int hi[NT][2], lo[NT][2]; };
+
+template <int NT>
+__device__ __forceinline__ void kv4_columns(Kv4Cols<NT>& C, int col0, int n_cols, int R, int pos0, int window, int lane) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int c = col0 + nt * 8 + 2 * (lane & 3) + i;
+            const int hi = c < n_cols ? pos0 + c / R : -1;
+            C.hi[nt][i] = hi;
+            C.lo[nt][i] = window > 0 ? max(0, hi - window + 1) : 0;
+        }
+}
+
+// ---- split form: few rows a segment (decode).  One CTA per (chunk of keys, kv head and 8 of its columns, segment): its four warps take the
+// chunk's tiles in turn, each with a ring of its own in shared memory that cp.async fills, and are joined at the end.  Many
+// small CTAs on an SM keep enough loads in flight; nothing but the end waits for another warp.
+template <int HD, int PARTS>
+struct Kv4Split {
+    static constexpr int TB = HD <= 64 ? 4 : (HD <= 128 ? 2 : 1), STAGES = 3, NW = 4;
+    static constexpr int TILE = TB * 16, STAGE = TB * Kv4<HD>::BLOCK;
+    static constexpr size_t RING = (size_t)NW * STAGES * STAGE, JOIN = sizeof(float) * NW * 8 * (HD + 2);
+    static constexpr size_t SMEM = RING > JOIN ? RING : JOIN;
+};
+
+template <int HD, int PARTS, bool KEEP, typename T>
+__global__ void __launch_bounds__(128)
+kv4_split_kernel(const Kv4Args p) {
+    using F = Kv4<HD>;
+    using S = Kv4Split<HD, PARTS>;
+    constexpr bool CENTRE = KEEP || PARTS > 1;
+    kp_pdl_begin();
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int R = p.H / p.G, kvh = blockIdx.y % p.G, seg = blockIdx.z, chunk = blockIdx.x;
+    const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg];
+    const int col0 = (blockIdx.y / p.G) * 8, n_cols = n_rows * R;
+    if (n_rows > p.max_rows || col0 >= n_cols) return;
+    const int col1 = min(col0 + 8, n_cols) - 1;
+    // the last key that the columns read in the chunk (and none that the block table has no page for)
+    const int k_hi = min(min(pos0 + col1 / R, (chunk + 1) * p.chunk - 1), p.max_blocks * p.ps - 1);
+    const int k_first = p.window > 0 ? max(0, pos0 + col0 / R - p.window + 1) : 0;
+    const int k_lo = max(k_first, chunk * p.chunk);
+    const int t_lo = k_lo / S::TILE, n_tiles = k_hi >= k_lo ? k_hi / S::TILE - t_lo + 1 : 0;
+    if (p.n_chunks > 1 && n_tiles == 0) return;            // (a single chunk writes its rows also where they read nothing)
+    const int* bt = p.block_table + (size_t)seg * p.max_blocks;
+    const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);
+    unsigned char* ring = smem + (size_t)warp * S::STAGES * S::STAGE;
+
+    auto load = [&](int i) {                               // the warp's i-th tile
+        const int tile = warp + i * S::NW;
+        if (tile < n_tiles) {
+            unsigned char* dst = ring + (i % S::STAGES) * S::STAGE;
+#pragma unroll
+            for (int b = 0; b < S::TB; b++) {
+                const int key = (t_lo + tile) * S::TILE + b * 16;
+                if (key <= k_hi && key + 15 >= k_lo) {
+                    const int page = key / p.ps;
+                    kv4_load_block<HD>(dst + b * F::BLOCK, p.pages + ((size_t)bt[page] * p.G + kvh) * rec, key - page * p.ps, p.ps, lane);
+                }
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; i++) load(i);
+
+    Kv4Cols<1> C;
+    kv4_columns<1>(C, col0, n_cols, R, pos0, p.window, lane);
+    Kv4Q<HD, PARTS, 1> Q;
+    {
+        const int c = col0 + (lane >> 2);
+        const T* src = c < n_cols ? (const T*)p.q + (size_t)(row0 + c / R) * p.ldq + (size_t)(kvh * R + c % R) * HD : nullptr;
+        kv4_load_q<HD, PARTS, 1, CENTRE, T>(Q, 0, src, p.scale, lane);
+    }
+    float* sc[1][2] = {{nullptr, nullptr}};
+    if (KEEP) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int c = col0 + 2 * (lane & 3) + i;
+            if (c < n_cols) sc[0][i] = p.scores + (((size_t)seg * p.max_rows + c / R) * p.H + kvh * R + c % R) * p.ld_scores;
+        }
+    }
+    Kv4Acc<HD, PARTS, 1> A;
+    A.clear();
+    // no key at all is masked between these
+    const int safe_lo = p.window > 0 ? max(0, pos0 + col1 / R - p.window + 1) : 0, safe_hi = min(k_hi, pos0 + col0 / R);
+#pragma unroll 1
+    for (int i = 0; warp + i * S::NW < n_tiles; i++) {
+        load(i + S::STAGES - 1);
+        cp_async_wait<S::STAGES - 1>();
+        __syncwarp();
+        const int key0 = (t_lo + warp + i * S::NW) * S::TILE;
+        const unsigned char* tile = ring + (i % S::STAGES) * S::STAGE;
+        if (key0 >= max(k_lo, safe_lo) && key0 + S::TILE - 1 <= safe_hi)
+            kv4_tile<HD, PARTS, 1, S::TB, CENTRE, false, KEEP>(A, Q, tile, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+        else
+            kv4_tile<HD, PARTS, 1, S::TB, CENTRE, true, KEEP>(A, Q, tile, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+        __syncwarp();
+    }
+    cp_async_wait<0>();
+    A.finish();
+    __syncthreads();                                       // the rings are done with: the warps' results take their place
+    float* jo = reinterpret_cast<float*>(smem);            // [warp][column][HD]
+    float* jm = jo + S::NW * 8 * HD;                       // [warp][column]: shift
+    float* jl = jm + S::NW * 8;                            // sum of p
+#pragma unroll
+    for (int y = 0; y < F::NG; y++)
+#pragma unroll
+        for (int j = 0; j < F::MT; j++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<float2*>(jo + (size_t)(warp * 8 + 2 * (lane & 3) + i) * HD + A.dim(y, j, lane)) = A.value(0, y, j, i);
+    if (lane < 4) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) { jm[warp * 8 + 2 * lane + i] = A.shift[0][i]; jl[warp * 8 + 2 * lane + i] = A.l[0][i]; }
+    }
+    __syncthreads();
+    const int live = col1 - col0 + 1;
+    for (int e = threadIdx.x; e < live * HD; e += 128) {
+        const int c = e / HD, d = e - c * HD;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < S::NW; w++) M = fmaxf(M, jm[w * 8 + c]);
+        float acc = 0.f, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < S::NW; w++) {
+            const float f = jm[w * 8 + c] == -INFINITY ? 0.f : kv4_exp2(jm[w * 8 + c] - M);
+            if (jm[w * 8 + c] != -INFINITY) acc = fmaf(jo[(size_t)(w * 8 + c) * HD + d], f, acc);
+            L = fmaf(jl[w * 8 + c], f, L);
+        }
+        const int col = col0 + c;
+        const size_t rh = ((size_t)seg * p.max_rows + col / R) * p.H + kvh * R + col % R;
+        if (p.n_chunks == 1) {
+            ((T*)p.out)[(size_t)(row0 + col / R) * p.ldo + (size_t)(kvh * R + col % R) * HD + d] = from_f32<T>(M == -INFINITY ? 0.f : acc / L);
+            if (KEEP && d == 0) p.lse_split[rh] = M == -INFINITY ? INFINITY : M + log2f(L);
+        } else {
+            p.part_o[(rh * p.n_chunks + chunk) * HD + d] = acc;
+            if (d == 0) { p.part_ml[(rh * p.n_chunks + chunk) * 2] = M; p.part_ml[(rh * p.n_chunks + chunk) * 2 + 1] = L; }
+        }
+    }
+}
+
+// ---- joins the chunks of a (row, head): one CTA each, in the order of the chunks
+template <typename T>
+__global__ void __launch_bounds__(128)
+kv4_merge_kernel(const Kv4Args p, int hd) {
+    kp_pdl_begin();
+    const int seg = blockIdx.x / p.max_rows, r = blockIdx.x % p.max_rows, h = blockIdx.y;
+    const int row = p.cu_rows[seg] + r, n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg];
+    if (r >= n_rows || n_rows > p.max_rows) return;
+    const int hi = p.seg_pos[seg] + r;
+    const int lo = p.window > 0 ? max(0, hi - p.window + 1) : 0;
+    const size_t rh = (size_t)blockIdx.x * p.H + h;
+    const float* ml = p.part_ml + rh * p.n_chunks * 2;
+    const float* po = p.part_o + rh * p.n_chunks * hd;
+    const int c_lo = lo / p.chunk, c_hi = hi < 0 ? -1 : min(hi / p.chunk, p.n_chunks - 1);
+    float M = -INFINITY, L = 0.f;
+    for (int c = c_lo; c <= c_hi; c++) M = fmaxf(M, ml[2 * c]);
+    for (int c = c_lo; c <= c_hi; c++)
+        if (ml[2 * c] != -INFINITY) L = fmaf(ml[2 * c + 1], kv4_exp2(ml[2 * c] - M), L);
+    for (int d = threadIdx.x; d < hd; d += 128) {
+        float acc = 0.f;
+        for (int c = c_lo; c <= c_hi; c++)
+            if (ml[2 * c] != -INFINITY) acc = fmaf(po[(size_t)c * hd + d], kv4_exp2(ml[2 * c] - M), acc);
+        ((T*)p.out)[(size_t)row * p.ldo + (size_t)h * hd + d] = from_f32<T>(M == -INFINITY ? 0.f : acc / L);
+    }
+    if (p.lse_split && threadIdx.x == 0) p.lse_split[rh] = M == -INFINITY ? INFINITY : M + log2f(L);
+}
+
+// ---- adds the weights of the split form's rows to their keys' mass: a thread a key, rows and heads in order
+__global__ void __launch_bounds__(128)
+kv4_split_mass_kernel(const Kv4Args p) {
+    kp_pdl_begin();
+    const int seg = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 128 + threadIdx.x;
+    const int n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg], pos0 = p.seg_pos[seg], R = p.H / p.G;
+    // (in front of the first row's window nothing is read, and the pages may be somebody else's by now)
+    if (n_rows > p.max_rows || key > pos0 + n_rows - 1 || key >= p.max_blocks * p.ps || key >= p.ld_scores ||
+        (p.window > 0 && key <= pos0 - p.window)) return;
+    float sum = 0.f;
+    for (int r = 0; r < n_rows; r++) {
+        const int hi = pos0 + r;
+        if (key > hi || (p.window > 0 && key <= hi - p.window)) continue;
+        for (int j = 0; j < R; j++) {
+            const size_t rh = ((size_t)seg * p.max_rows + r) * p.H + kvh * R + j;
+            sum += kv4_exp2(p.scores[rh * p.ld_scores + key] - p.lse_split[rh]);
+        }
+    }
+    const int page = p.block_table[(size_t)seg * p.max_blocks + key / p.ps];
+    p.mass[((size_t)page * p.G + kvh) * p.ps + key % p.ps] += sum;
+}
+
+// ---- tiled form: many rows a segment (portions of prompts).  A CTA takes 32 NT columns of a kv head (8 NT a warp) and walks
+// their keys in tiles of 64 that its warps bring and share.
+template <int HD, int PARTS>
+struct Kv4Tiled {
+    static constexpr int NT = PARTS == 1 ? (HD <= 64 ? 4 : (HD <= 128 ? 2 : 1)) : (HD <= 64 ? 2 : 1);
+    static constexpr int COLS = 32 * NT, TILE = 64, STAGE = 4 * Kv4<HD>::BLOCK;
+    static constexpr size_t SMEM = 2 * STAGE;
+};
+
+// The tile'th of the tiles that the segments of at least min_rows rows make of `per` columns each: its segment and first column
+// (found by one warp; segment -1: there is none).
+__device__ __forceinline__ void kv4_find_tile(const Kv4Args& p, int tile, int per, int R, int lane, int& seg, int& col0) {
+    seg = -1;
+    int before = 0;
+    for (int base = 0; base < p.n_seg; base += 32) {
+        const int i = base + lane;
+        int rows = 0;
+        if (i < p.n_seg) rows = p.cu_rows[i + 1] - p.cu_rows[i];
+        const int mine = rows >= p.min_rows ? (rows * R + per - 1) / per : 0;
+        int run = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
+        const unsigned hit = __ballot_sync(0xffffffffu, tile < before + run);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            seg = base + src;
+            const int all = __shfl_sync(0xffffffffu, mine, src), end = before + __shfl_sync(0xffffffffu, run, src);
+            col0 = (all - 1 - (tile - (end - all))) * per;     // (the last columns of a segment, which read the most keys, first)
+            return;
+        }
+        before += __shfl_sync(0xffffffffu, run, 31);
+    }
+}
+
+template <int HD, int PARTS, bool CENTRE, typename T>
+__global__ void __launch_bounds__(128)
+kv4_tiled_kernel(const Kv4Args p) {
+    using F = Kv4<HD>;
+    using S = Kv4Tiled<HD, PARTS>;
+    constexpr int NT = S::NT;
+    kp_pdl_begin();
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int R = p.H / p.G, kvh = blockIdx.y;
+    int seg, cta_col0 = 0;
+    kv4_find_tile(p, blockIdx.x, S::COLS, R, lane, seg, cta_col0);
+    if (seg < 0) return;
+    const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg], n_cols = n_rows * R;
+    const int cta_col1 = min(cta_col0 + S::COLS, n_cols) - 1;
+    const int k_hi = min(pos0 + cta_col1 / R, p.max_blocks * p.ps - 1), k_lo = p.window > 0 ? max(0, pos0 + cta_col0 / R - p.window + 1) : 0;
+    const int t_lo = k_lo / S::TILE, n_tiles = k_hi >= k_lo ? k_hi / S::TILE - t_lo + 1 : 0;
+    const int* bt = p.block_table + (size_t)seg * p.max_blocks;
+    const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);
+    auto load = [&](int i) {                               // every warp a block of the tile
+        const int key = (t_lo + i) * S::TILE + warp * 16;
+        if (i < n_tiles && key <= k_hi && key + 15 >= k_lo) {
+            const int page = key / p.ps;
+            kv4_load_block<HD>(smem + (size_t)(i & 1) * S::STAGE + warp * F::BLOCK, p.pages + ((size_t)bt[page] * p.G + kvh) * rec, key - page * p.ps, p.ps, lane);
+        }
+        cp_async_commit();
+    };
+    load(0);
+    const int col0 = cta_col0 + warp * 8 * NT;
+    Kv4Cols<NT> C;
+    kv4_columns<NT>(C, col0, n_cols, R, pos0, p.window, lane);
+    Kv4Q<HD, PARTS, NT> Q;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int c = col0 + nt * 8 + (lane >> 2);
+        const T* src = c < n_cols ? (const T*)p.q + (size_t)(row0 + c / R) * p.ldq + (size_t)(kvh * R + c % R) * HD : nullptr;
+        kv4_load_q<HD, PARTS, NT, CENTRE, T>(Q, nt, src, p.scale, lane);
+    }
+    float* sc[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) sc[nt][0] = sc[nt][1] = nullptr;
+    Kv4Acc<HD, PARTS, NT> A;
+    A.clear();
+    const int col1 = min(col0 + 8 * NT, n_cols) - 1;       // the warp's last column (it has none where col1 < col0)
+    const int w_hi = min(pos0 + col1 / R, k_hi), w_lo = p.window > 0 ? max(0, pos0 + col0 / R - p.window + 1) : 0;
+    const int safe_hi = pos0 + col0 / R, safe_lo = p.window > 0 ? max(0, pos0 + col1 / R - p.window + 1) : 0;
+#pragma unroll 1
+    for (int i = 0; i < n_tiles; i++) {
+        load(i + 1);
+        cp_async_wait<1>();
+        __syncthreads();
+        const unsigned char* tile = smem + (size_t)(i & 1) * S::STAGE;
+#pragma unroll 1
+        for (int b = 0; b < 4; b++) {
+            const int key0 = (t_lo + i) * S::TILE + b * 16;
+            if (col1 < col0 || key0 > w_hi || key0 + 15 < w_lo) continue;
+            if (key0 >= max(k_lo, safe_lo) && key0 + 15 <= safe_hi && col0 + 8 * NT <= n_cols)
+                kv4_tile<HD, PARTS, NT, 1, CENTRE, false, false>(A, Q, tile + b * F::BLOCK, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+            else
+                kv4_tile<HD, PARTS, NT, 1, CENTRE, true, false>(A, Q, tile + b * F::BLOCK, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+        }
+        __syncthreads();                                   // the next tile but one takes this one's place
+    }
+    cp_async_wait<0>();
+    A.finish();
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int c = col0 + nt * 8 + 2 * (lane & 3) + i;
+            if (c >= n_cols) continue;
+            const size_t row = row0 + c / R;
+            const int h = kvh * R + c % R;
+            const bool none = A.m[nt][i] == -INFINITY;
+            const float inv = none ? 0.f : 1.0f / A.l[nt][i];
+            T* dst = (T*)p.out + row * p.ldo + (size_t)h * HD;
+#pragma unroll
+            for (int y = 0; y < F::NG; y++)
+#pragma unroll
+                for (int j = 0; j < F::MT; j++) {
+                    float2 o = A.value(nt, y, j, i);
+                    if (none) o = make_float2(0.f, 0.f);
+                    dst[A.dim(y, j, lane)] = from_f32<T>(o.x * inv);
+                    dst[A.dim(y, j, lane) + 1] = from_f32<T>(o.y * inv);
+                }
+            if (p.lse && lane < 4) p.lse[row * p.H + h] = none ? INFINITY : A.shift[nt][i] + log2f(A.l[nt][i]);
+        }
+}
+
+// ---- the tiled form's mass: one CTA per (64 keys, kv head, segment).  Its warps take the columns that read the keys, 8 at a
+// time, compute the scores again and add up 2^(score - lse); the warps' sums are added in their order.
+template <int HD, int PARTS, typename T>
+__global__ void __launch_bounds__(128)
+kv4_mass_kernel(const Kv4Args p) {
+    using F = Kv4<HD>;
+    constexpr int NB = HD <= 128 ? 4 : 2, KEYS = NB * 16;
+    kp_pdl_begin();
+    __shared__ __align__(16) unsigned char smem[NB * F::BLOCK];
+    __shared__ float part[4][KEYS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int seg = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x * KEYS, R = p.H / p.G;
+    const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg];
+    // keys that any row reads (in front of them the pages may be somebody else's by now)
+    const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+    if (n_rows < p.min_rows || k0 > last || k0 + KEYS - 1 < first) return;
+    // rows that read any of the keys
+    const int r_lo = max(0, k0 - pos0), r_hi = p.window > 0 ? min(n_rows - 1, k0 + KEYS - 1 + p.window - 1 - pos0) : n_rows - 1;
+    if (r_hi < r_lo) return;
+    const int* bt = p.block_table + (size_t)seg * p.max_blocks;
+    for (int b = warp; b < NB; b += 4) {
+        const int key = k0 + b * 16;
+        if (key <= last && key + 15 >= first) {
+            const int page = key / p.ps;
+            kv4_load_block<HD>(smem + b * F::BLOCK, p.pages + ((size_t)bt[page] * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key - page * p.ps, p.ps, lane);
+        }
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    float sum[NB][2];
+#pragma unroll
+    for (int b = 0; b < NB; b++) sum[b][0] = sum[b][1] = 0.f;
+    const int c_end = (r_hi + 1) * R, key = kv4_key_of(lane >> 2);
+#pragma unroll 1
+    for (int col0 = r_lo * R + warp * 8; col0 < c_end; col0 += 32) {
+        Kv4Q<HD, PARTS, 1> Q;
+        const int cq = col0 + (lane >> 2);
+        kv4_load_q<HD, PARTS, 1, true, T>(Q, 0, cq < c_end ? (const T*)p.q + (size_t)(row0 + cq / R) * p.ldq + (size_t)(kvh * R + cq % R) * HD : nullptr,
+                                    p.scale, lane);
+        float lse[2];
+        int hi[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int c = col0 + 2 * (lane & 3) + i;
+            hi[i] = c < c_end ? pos0 + c / R : -1;
+            lse[i] = c < c_end ? p.lse[(size_t)(row0 + c / R) * p.H + kvh * R + c % R] : 0.f;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float s[1][4];
+            kv4_scores<HD, PARTS, 1, true>(s, smem + b * F::BLOCK, Q, lane);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int k = k0 + b * 16 + key + (e >> 1) * 8, h = hi[e & 1];
+                const bool sees = k <= h && (p.window <= 0 || k > h - p.window);
+                sum[b][e >> 1] += sees ? kv4_exp2(s[0][e] - lse[e & 1]) : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float v = sum[b][e];
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            if ((lane & 3) == 0) part[warp][b * 16 + key + e * 8] = v;
+        }
+    __syncthreads();
+    const int k = threadIdx.x;
+    if (k < KEYS && k0 + k <= last && k0 + k >= first) {
+        const int page = bt[(k0 + k) / p.ps];
+        p.mass[((size_t)page * p.G + kvh) * p.ps + (k0 + k) % p.ps] += (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
+    }
+}
+
+// ------------------------------------------------------------------ launchers
+#define KV4_DISPATCH_HD(hd, HD, ...)                                   \
+    switch (hd) {                                                      \
+        case 32: { constexpr int HD = 32; __VA_ARGS__; } break;        \
+        case 64: { constexpr int HD = 64; __VA_ARGS__; } break;        \
+        case 96: { constexpr int HD = 96; __VA_ARGS__; } break;        \
+        case 128: { constexpr int HD = 128; __VA_ARGS__; } break;      \
+        case 192: { constexpr int HD = 192; __VA_ARGS__; } break;      \
+        case 256: { constexpr int HD = 256; __VA_ARGS__; } break;      \
+        default: return KP_ERR_UNSUPPORTED;                            \
+    }
+
+template <typename Kern>
+static int kv4_launch(Kern kern, dim3 grid, size_t smem, std::atomic<unsigned long long>& ready, cudaStream_t st, const Kv4Args& a) {
+    if (smem > 48 * 1024) {
+        const int e = kp_smem_limit(kern, smem, ready);
+        if (e) return e;
+    }
+    const cudaError_t e = kp_launch_pdl(kern, grid, dim3(128), smem, st, a);
+    return e ? (int)e : kp_launch_status();
+}
+
+template <int HD, int PARTS, typename T>
+static int kv4_run(const Kv4Args& a, int n_rows, int long_tiles, int long_keys, cudaStream_t st) {
+    const int R = a.H / a.G;
+    if (a.max_rows > 0) {
+        using S = Kv4Split<HD, PARTS>;
+        static std::atomic<unsigned long long> ready{0}, ready_keep{0};
+        const dim3 grid(a.n_chunks, a.G * ((a.max_rows * R + 7) / 8), a.n_seg);
+        const int e = a.mass ? kv4_launch(kv4_split_kernel<HD, PARTS, true, T>, grid, S::SMEM, ready_keep, st, a)
+                             : kv4_launch(kv4_split_kernel<HD, PARTS, false, T>, grid, S::SMEM, ready, st, a);
+        if (e) return e;
+        if (a.n_chunks > 1) {
+            const cudaError_t c = kp_launch_pdl(kv4_merge_kernel<T>, dim3(a.n_seg * a.max_rows, a.H), dim3(128), 0, st, a, HD);
+            if (c) return (int)c;
+        }
+        if (a.mass) {
+            const cudaError_t c = kp_launch_pdl(kv4_split_mass_kernel, dim3((a.n_chunks * a.chunk + 127) / 128, a.G, a.n_seg), dim3(128), 0, st, a);
+            if (c) return (int)c;
+        }
+    }
+    if (long_tiles > 0) {
+        using S = Kv4Tiled<HD, PARTS>;
+        static std::atomic<unsigned long long> ready{0}, ready_mass{0};
+        const int tiles = (n_rows * R + S::COLS - 1) / S::COLS + a.n_seg;
+        // (with mass the scores are those that the mass is computed from again)
+        int e = a.mass ? kv4_launch(kv4_tiled_kernel<HD, PARTS, true, T>, dim3(tiles, a.G), S::SMEM, ready, st, a)
+                       : kv4_launch(kv4_tiled_kernel<HD, PARTS, (PARTS > 1), T>, dim3(tiles, a.G), S::SMEM, ready, st, a);
+        if (e) return e;
+        if (a.mass) {
+            constexpr int KEYS = HD <= 128 ? 64 : 32;
+            e = kv4_launch(kv4_mass_kernel<HD, PARTS, T>, dim3((long_keys + KEYS - 1) / KEYS, a.G, a.n_seg), 0, ready_mass, st, a);
+            if (e) return e;
+        }
+    }
+    return kp_launch_status();
+}
+
+extern "C" {
+
+int kp_kv4_write(const void* k, long long ldk, const void* v, long long ldv, void* pages, long long n_pages, const int* slot_map, int n, int ps,
+                 int G, int hd, int dtype, void* stream) {
+    if (n <= 0) return 0;
+    if (hd < 32 || hd % 32 || ps < 16 || ps % 16 || G < 1 || ((uintptr_t)pages & 15)) return KP_ERR_BAD_ARG;
+    const int gs = hd % 64 == 0 ? 64 : 32;
+    const long long blocks = (2LL * n * G * (hd / 8) + 255) / 256;
+    if (blocks > 2147483647LL) return KP_ERR_UNSUPPORTED;
+    KP_DISPATCH_DTYPE(dtype, T, {
+        const long long a = 16 / sizeof(T);
+        const bool vec = !(((uintptr_t)k | (uintptr_t)v) & 15) && ldk % a == 0 && ldv % a == 0;
+        cudaError_t e = vec ? kp_launch_pdl(kv4_write_kernel<T, true>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const T*)k, ldk,
+                                            (const T*)v, ldv, (unsigned char*)pages, slot_map, n_pages * ps, n, ps, G, hd, gs)
+                            : kp_launch_pdl(kv4_write_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const T*)k, ldk,
+                                            (const T*)v, ldv, (unsigned char*)pages, slot_map, n_pages * ps, n, ps, G, hd, gs);
+        if (e) return (int)e;
+    });
+    return kp_launch_status();
+}
+
+int kp_kv4_read(const void* pages, long long n_pages, const int* slot_map, void* k, void* v, int n, int ps, int G, int hd, int dtype, void* stream) {
+    if (n <= 0) return 0;
+    if (hd < 32 || hd % 32 || ps < 16 || ps % 16 || G < 1 || (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15)) return KP_ERR_BAD_ARG;
+    const long long blocks = (2LL * n * G * (hd / 8) + 255) / 256;
+    if (blocks > 2147483647LL) return KP_ERR_UNSUPPORTED;
+    KP_DISPATCH_DTYPE(dtype, T, {
+        const cudaError_t e = kp_launch_pdl(kv4_read_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const unsigned char*)pages,
+                                            slot_map, n_pages * ps, (T*)k, (T*)v, n, ps, G, hd, hd % 64 == 0 ? 64 : 32);
+        if (e) return (int)e;
+    });
+    return kp_launch_status();
+}
+
+// Segments of at most `short_rows` rows go to the split form (0: none), the others to the tiled form if `long_rows` is not 0.
+// Scratch: see Kv4Args; lse_split and scores where there is mass and a split form, lse where there is mass and a tiled one.
+int kp_kv4_attention(const void* q, long long ldq, const void* pages, const int* block_table, int max_blocks, const int* cu_rows, const int* seg_pos,
+                     int n_seg, void* out, long long ldo, float scale, int window, int ps, int H, int G, int hd, int n_rows, int short_rows,
+                     int long_rows, int n_chunks, int chunk, int max_context, float* part_o, float* part_ml, float* scores, int ld_scores,
+                     float* lse_split, float* lse, float* mass, int dtype, void* stream) {
+    if (n_rows <= 0 || n_seg <= 0) return 0;
+    if (G < 1 || H < 1 || H % G || ps < 16 || ps % 16 || window < 0 || n_chunks < 1 || chunk < 64 || chunk % 64 || n_seg > 65535 || H > 65535 ||
+        ((uintptr_t)pages & 15) || (mass && ((long_rows && !lse) || (short_rows > 0 && (!scores || !lse_split)))) || (n_chunks > 1 && short_rows > 0 && (!part_o || !part_ml)))
+        return KP_ERR_BAD_ARG;
+    Kv4Args a = {};
+    a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.pages = (const unsigned char*)pages;
+    a.block_table = block_table; a.max_blocks = max_blocks; a.cu_rows = cu_rows; a.seg_pos = seg_pos;
+    a.scale = scale; a.window = window; a.ps = ps; a.H = H; a.G = G;
+    a.part_o = part_o; a.part_ml = part_ml; a.scores = mass ? scores : nullptr; a.ld_scores = ld_scores;
+    a.lse_split = mass ? lse_split : nullptr; a.lse = mass ? lse : nullptr; a.mass = mass;
+    a.n_chunks = n_chunks; a.chunk = chunk; a.max_rows = short_rows; a.min_rows = short_rows + 1; a.n_seg = n_seg;
+    if (dtype == KP_DTYPE_BF16) {
+        KV4_DISPATCH_HD(hd, HD, return (kv4_run<HD, 1, bf16>(a, n_rows, long_rows, max_context, (cudaStream_t)stream)));
+    } else if (dtype == KP_DTYPE_F32) {
+        KV4_DISPATCH_HD(hd, HD, return (kv4_run<HD, 2, float>(a, n_rows, long_rows, max_context, (cudaStream_t)stream)));
+    }
+    return KP_ERR_BAD_ARG;
+}
+
+}  // extern "C"
