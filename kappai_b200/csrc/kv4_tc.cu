@@ -1,0 +1,720 @@
+// Attention of many rows (portions of prompts) over the 4-bit cache on the 5th-generation tensor cores: bfloat16 rows, heads
+// of 64 or 128 values.  Formulas and bytes as in kv4.cuh.
+//
+// Columns.  The rows of a segment and the R query heads that share a kv head are one list of columns, c = row R + head: a tile of
+// 128 columns reads the same keys once for all of them.  A CTA takes 256 columns of a kv head, two groups of 128, and walks
+// their keys in tiles of 128:
+//   4 warps turn the codes of a tile into fp16 operands in shared memory, a thread a key;
+//   1 warp issues  S = Q K^T  and  O += P V  (tcgen05.mma, kind::f16; S and O in tensor memory);
+//   2 x 4 warps have a thread a column: S from tensor memory, softmax, P (fp16) to shared memory.
+// While one group is at its exponentials the tensor core works for the other.
+//
+// Exactness.  K's operand is s (c - 8): an 8-bit times a 4-bit number, exact in fp16's 11 bits.  The rest, (z + 8 s) times the
+// query's sum over the group, is 16 more columns of the same product: both factors in two fp16 parts.  So S is off by float32
+// rounding only, and the weights added up as mass are those of the definition to 1e-6.  V's operand s (c - 8) + (z + 8 s) is
+// rounded to fp16 once (2^-12; the output's own rounding to bfloat16 is 2^-9), and so is P.
+// Ranges.  Queries are scaled by a power of two a column, K by one a tile of keys, V by one that only grows from tile to tile
+// (O is rescaled when it does): fp16 then holds whatever bfloat16 did.  P is taken against a reference that follows the row's maximum
+// in steps of at least 2^8 (O is rescaled in tensor memory only then), P <= 2^15.
+// Every mbarrier wait is bounded; one that gives up sets the status word, and the CTA frees its tensor memory and returns.
+#include <type_traits>
+
+#include "kv4.cuh"
+#include "tcgen05.cuh"
+
+KP_STATUS_WORD(g_kv4_tc_status, kv4_tc)               // 0 ok; 1: a bounded wait gave up
+
+#define KT_ROWS 128                                    // columns a group, and keys a tile
+#define KT_EXT 4096                                    // 128 rows of 16 fp16 beside a tile: the parts of the second term
+
+struct Kv4TcArgs {
+    const bf16* q; long long ldq;
+    bf16* out; long long ldo;
+    const unsigned char* pages;
+    const int* block_table; int max_blocks;
+    const int* cu_rows; const int* seg_pos;
+    float scale; int window; int ps; int H, G;
+    unsigned char* q_image; float2* col;               // with mass: the groups' Q operands and (factor, lse) of their columns
+    float* mass;
+    int min_rows, n_seg, n_tiles;                      // n_tiles: an upper bound of the CTAs' tiles
+};
+
+template <int HD>
+struct Kt {
+    static constexpr int NG = HD / 64, TILE = NG * 16384, OPER = TILE + KT_EXT, ST = HD == 64 ? 2 : 1;
+    static constexpr int PV = 2 * 16384;               // P of a group: keys 0..63 | keys 64..127
+    static constexpr size_t SMEM = 1024 + 2 * OPER + ST * OPER + ST * TILE + 2 * PV + 512;
+    static constexpr int THREADS = 416;
+    // the pass that adds up the mass: one K tile, a ring of Q images
+    static constexpr int QST = 3, IMAGE = OPER + 1024; // an image in shared memory, and (factor, lse) of its columns
+    static constexpr size_t MASS_SMEM = 1024 + OPER + QST * IMAGE + 512;
+};
+
+// tcgen05 instruction descriptor with fp16 operands (the helper's are bfloat16)
+__host__ __device__ constexpr uint32_t kt_idesc(int M, int N, bool b_mn) { return kp_umma_idesc(M, N, b_mn) & ~((1u << 7) | (1u << 10)); }
+// K-major operand of 16 columns: rows of 32 bytes with the 32-byte swizzle, 8-row groups 256 bytes apart
+__device__ __forceinline__ uint64_t kt_desc_ext(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr >> 4) & 0x3FFF);
+    d |= (uint64_t)1 << 16;
+    d |= (uint64_t)(256 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)6 << 61;
+    return d;
+}
+__device__ __forceinline__ int kt_ext_at(int row, int chunk) { return row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4); }
+__device__ __forceinline__ int kt_at(int row, int chunk) { return (chunk >> 3) * 16384 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
+
+__device__ __forceinline__ float kt_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
+__device__ __forceinline__ float kt_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t kt_h2(float lo, float hi) { return pack_f16(lo, hi); }
+
+// eight codes as fp16 pairs (0, 4), (1, 5), (2, 6), (3, 7), times s (s16: s / 16), plus z
+__device__ __forceinline__ uint4 kt_codes(uint32_t w, __half2 s, __half2 s16, __half2 z, bool add) {
+    uint32_t x[4] = {w & 0x000f000fu, w & 0x00f000f0u, (w >> 8) & 0x000f000fu, (w >> 8) & 0x00f000f0u};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t y = x[i] | 0x64006400u, c = (i & 1) ? 0x64806480u : 0x64086408u;
+        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&y), *reinterpret_cast<const __half2*>(&c));
+        const __half2 v = add ? __hfma2(d, (i & 1) ? s16 : s, z) : __hmul2(d, (i & 1) ? s16 : s);
+        r[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+// the power of two above a group's largest magnitude (nothing for one that is not finite)
+__device__ __forceinline__ int kt_exponent(uint32_t range) {
+    const float s = kv4_scale(range), z = kv4_least(range), top = fmaxf(fabsf(z), fabsf(fmaf(15.0f, s, z)));
+    return top < INFINITY ? (int)(__float_as_uint(top) >> 23) - 126 : -126;
+}
+// One row of an operand of the score product: K's codes of a key
+template <int HD>
+__device__ __forceinline__ void kt_write_key(unsigned char* tile, int row, const uint4 (&codes)[HD / 32], const uint32_t (&ranges)[HD / 64], int e) {
+    const float f = kt_pow2(7 - e);
+    uint32_t ext[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int y = 0; y < HD / 64; y++) {
+        const float s = kv4_scale(ranges[y]) * f, z = fmaf(8.0f, kv4_scale(ranges[y]), kv4_least(ranges[y])) * f;
+        const __half2 s2 = __float2half2_rn(s), s16 = __float2half2_rn(s * 0.0625f);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint4 c = codes[2 * y + i];
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *reinterpret_cast<uint4*>(tile + kt_at(row, y * 8 + i * 4 + j)) = kt_codes(w[j], s2, s16, s2, false);
+        }
+        const __half zh = __float2half_rn(z), zl = __float2half_rn(z - __half2float(zh));
+        const __half2 h2 = __halves2half2(zh, zh), l2 = __halves2half2(zl, zl);
+        ext[2 * y] = *reinterpret_cast<const uint32_t*>(&h2);
+        ext[2 * y + 1] = *reinterpret_cast<const uint32_t*>(&l2);
+    }
+    *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 0)) = make_uint4(ext[0], ext[1], ext[2], ext[3]);
+    *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 1)) = make_uint4(0u, 0u, 0u, 0u);
+}
+// and a query (null: zeros).  Returns the factor that makes scores (base 2) of the product with a tile scaled by 2^(7 - e): factor 2^(e - 7).
+template <int HD>
+__device__ __forceinline__ float kt_write_query(unsigned char* tile, int row, const bf16* src, float scale) {
+    float v[HD], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 8; i++) {
+        const uint4 x = src ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) { v[8 * i + 2 * j] = __uint_as_float(w[j] << 16); v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
+    }
+#pragma unroll
+    for (int i = 0; i < HD; i++) top = fmaxf(top, fabsf(v[i]));
+    int e = 0;
+    if (top > 0.f && top < INFINITY) e = min(6 - ilogbf(top), 100);          // the largest value to [2^6, 2^7): a sum of 64 then fits fp16
+    const float up = kt_pow2(e);
+    uint32_t ext[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int y = 0; y < HD / 64; y++) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float* x = v + y * 64 + i * 8;
+            uint32_t r[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                r[j] = kt_h2(x[j] * up, x[j + 4] * up);
+                const __half2 h = *reinterpret_cast<const __half2*>(&r[j]);
+                sum += __low2float(h) + __high2float(h);
+            }
+            *reinterpret_cast<uint4*>(tile + kt_at(row, y * 8 + i)) = make_uint4(r[0], r[1], r[2], r[3]);
+        }
+        const __half sh = __float2half_rn(sum), sl = __float2half_rn(sum - __half2float(sh));
+        const __half2 both = __halves2half2(sh, sl);
+        ext[2 * y] = ext[2 * y + 1] = *reinterpret_cast<const uint32_t*>(&both);
+    }
+    *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 0)) = make_uint4(ext[0], ext[1], ext[2], ext[3]);
+    *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 1)) = make_uint4(0u, 0u, 0u, 0u);
+    return scale * KV4_LOG2E * kt_pow2(-e);
+}
+// S of 128 x 128 (one thread issues)
+template <int HD>
+__device__ __forceinline__ void kt_issue_s(uint32_t tmem, const unsigned char* a, const unsigned char* b) {
+    constexpr uint32_t idesc = kt_idesc(128, 128, false);
+#pragma unroll
+    for (int y = 0; y < HD / 64; y++) {
+        const uint64_t ad = kp_umma_desc(kp_smem_u32(a + y * 16384)), bd = kp_umma_desc(kp_smem_u32(b + y * 16384));
+#pragma unroll
+        for (int k = 0; k < 4; k++) kp_umma_bf16(tmem, ad + 2 * k, bd + 2 * k, idesc, (y | k) ? 1u : 0u);
+    }
+    kp_umma_bf16(tmem, kt_desc_ext(kp_smem_u32(a + Kt<HD>::TILE)), kt_desc_ext(kp_smem_u32(b + Kt<HD>::TILE)), idesc, 1u);
+}
+
+// What a thread of the code warps has of its key
+template <int HD>
+struct KtKey {
+    uint4 k[HD / 32], v[HD / 32];
+    uint32_t kr[HD / 64], vr[HD / 64];
+    __device__ __forceinline__ void load(const unsigned char* rec, int off, int ps, bool there, bool values) {
+        constexpr int NG = HD / 64;
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int y = 0; y < NG; y++) kr[y] = vr[y] = 0u;
+        if (!there) return;                            // a key that is not there: zeros, whatever lies in its place
+        const uint4* kc = reinterpret_cast<const uint4*>(rec + (size_t)off * (HD / 2));
+        const uint4* vc = reinterpret_cast<const uint4*>(rec + (size_t)(ps + off) * (HD / 2));
+        const uint32_t* r = reinterpret_cast<const uint32_t*>(rec + (size_t)ps * HD);
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) { k[i] = kc[i]; if (values) v[i] = vc[i]; }
+#pragma unroll
+        for (int y = 0; y < NG; y++) { kr[y] = r[off * NG + y]; if (values) vr[y] = r[(ps + off) * NG + y]; }
+    }
+};
+
+// segment and first column of a tile of 256 columns (kv4.cu's tiles: the last columns of a segment first); -1: none
+__device__ __forceinline__ void kt_find(const Kv4TcArgs& p, int tile, int R, int lane, int& seg, int& col0) {
+    seg = -1; col0 = 0;
+    int before = 0;
+    for (int base = 0; base < p.n_seg; base += 32) {
+        const int i = base + lane;
+        const int rows = i < p.n_seg ? p.cu_rows[i + 1] - p.cu_rows[i] : 0;
+        const int mine = rows >= p.min_rows ? (rows * R + 255) / 256 : 0;
+        int run = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
+        const unsigned hit = __ballot_sync(0xffffffffu, tile < before + run);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            const int end = before + __shfl_sync(0xffffffffu, run, src);
+            seg = base + src;
+            col0 = (end - 1 - tile) * 256;
+            return;
+        }
+        before += __shfl_sync(0xffffffffu, run, 31);
+    }
+}
+// the tile of segment `seg`'s first 256 columns (its tiles run downwards from there)
+__device__ __forceinline__ int kt_first_tile(const Kv4TcArgs& p, int seg, int R, int lane) {
+    int sum = 0;
+    for (int i = lane; i <= seg; i += 32) {
+        const int rows = p.cu_rows[i + 1] - p.cu_rows[i];
+        sum += rows >= p.min_rows ? (rows * R + 255) / 256 : 0;
+    }
+    return __reduce_add_sync(0xffffffffu, sum) - 1;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(Kt<HD>::THREADS, 1)
+kv4_tc_kernel(const Kv4TcArgs p) {
+    using S = Kt<HD>;
+    constexpr int ST = S::ST;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+    unsigned char* Qs = sm;                            // [2] OPER
+    unsigned char* Ks = Qs + 2 * S::OPER;              // [ST] OPER
+    unsigned char* Vs = Ks + ST * S::OPER;             // [ST] TILE
+    unsigned char* Ps = Vs + ST * S::TILE;             // [2] PV
+    uint64_t* bars = reinterpret_cast<uint64_t*>(Ps + 2 * S::PV);
+    uint64_t* q_full = bars;                           // [2] each, by group or by stage
+    uint64_t* k_full = bars + 2; uint64_t* k_empty = bars + 4;
+    uint64_t* v_full = bars + 6; uint64_t* v_empty = bars + 8;
+    uint64_t* s_full = bars + 10; uint64_t* s_free = bars + 12;
+    uint64_t* p_full = bars + 14; uint64_t* o_done = bars + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* meta = abort_flag + 1;               // [4 tiles][2]: exponents of K's and V's scales
+    volatile int* tops = meta + 8;                     // [2][4 warps][2]
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; i++) {
+            kp_mbar_init(&q_full[i], 128);
+            kp_mbar_init(&k_full[i], 128); kp_mbar_init(&k_empty[i], 1);
+            kp_mbar_init(&v_full[i], 128); kp_mbar_init(&v_empty[i], 1);
+            kp_mbar_init(&s_full[i], 1); kp_mbar_init(&s_free[i], 128);
+            kp_mbar_init(&p_full[i], 128); kp_mbar_init(&o_done[i], 1);
+        }
+        *abort_flag = 0;
+        kp_mbar_init_fence();
+    }
+    if (warp == 12) kp_tmem_alloc(tmem_slot, 512);
+    kp_tc_fence_before();
+    __syncthreads();
+    kp_tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;             // S of the groups: 2 x 128 columns; then O: 2 x HD
+    kp_pdl_begin();
+
+    const int R = p.H / p.G, kvh = blockIdx.y;
+    int seg, cta_col0;
+    kt_find(p, blockIdx.x, R, lane, seg, cta_col0);
+    int row0 = 0, n_cols = 0, pos0 = 0;
+    if (seg >= 0) { row0 = p.cu_rows[seg]; n_cols = (p.cu_rows[seg + 1] - row0) * R; pos0 = p.seg_pos[seg]; }
+    const int n_here = min(256, n_cols - cta_col0);    // columns of this CTA
+    const int k_hi = seg < 0 ? -1 : min(pos0 + (cta_col0 + n_here - 1) / R, p.max_blocks * p.ps - 1);
+    const int k_lo = p.window > 0 ? max(0, pos0 + cta_col0 / R - p.window + 1) : 0;
+    const int kt_lo = k_lo / KT_ROWS, n_kt = k_hi >= k_lo ? k_hi / KT_ROWS - kt_lo + 1 : 0;
+
+    if (warp >= 8 && warp < 12) {
+        // ---- codes to operands: thread d has key d of every tile
+        const int d = threadIdx.x - 256;
+        const int* bt = p.block_table + (size_t)max(seg, 0) * p.max_blocks;
+        const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);
+        auto page_of = [&](int i) {
+            const int key = (kt_lo + i) * KT_ROWS + d;
+            return i < n_kt && key >= k_lo && key <= k_hi ? bt[key / p.ps] : -1;
+        };
+        auto fetch = [&](KtKey<HD>& x, int i, int page) {
+            const int key = (kt_lo + i) * KT_ROWS + d;
+            x.load(p.pages + ((size_t)max(page, 0) * p.G + kvh) * rec, key % p.ps, p.ps, page >= 0, true);
+        };
+        bool ok = true;
+        KtKey<HD> now;
+        int page = page_of(1), ev_run = -100;
+        fetch(now, 0, page_of(0));
+#pragma unroll 1
+        for (int i = 0; i < n_kt; i++) {
+            const int st = i % ST, use = i / ST;
+            KtKey<HD> next;
+            fetch(next, i + 1, page);
+            page = page_of(i + 2);
+            int ek = -100, ev = ev_run;
+#pragma unroll
+            for (int y = 0; y < S::NG; y++) { ek = max(ek, kt_exponent(now.kr[y])); ev = max(ev, kt_exponent(now.vr[y])); }
+            ek = __reduce_max_sync(0xffffffffu, ek);
+            ev = __reduce_max_sync(0xffffffffu, ev);
+            volatile int* t = tops + (i & 1) * 8;
+            if (lane == 0) { t[(warp & 3) * 2] = ek; t[(warp & 3) * 2 + 1] = ev; }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            ek = max(max(t[0], t[2]), max(t[4], t[6]));
+            ev_run = max(max(t[1], t[3]), max(t[5], t[7]));
+            if (d == 0) { meta[(i & 3) * 2] = ek; meta[(i & 3) * 2 + 1] = ev_run; }
+            if (ok && (*abort_flag || !kp_mbar_wait_bounded(&k_empty[st], (use & 1) ^ 1))) ok = false;
+            kt_write_key<HD>(Ks + st * S::OPER, d, now.k, now.kr, ek);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            kp_mbar_arrive(&k_full[st]);
+            if (ok && !kp_mbar_wait_bounded(&v_empty[st], (use & 1) ^ 1)) ok = false;
+            const float f = kt_pow2(14 - ev_run);
+#pragma unroll
+            for (int y = 0; y < S::NG; y++) {
+                const float s = kv4_scale(now.vr[y]) * f, z = fmaf(8.0f, kv4_scale(now.vr[y]), kv4_least(now.vr[y])) * f;
+                const __half2 s2 = __float2half2_rn(s), s16 = __float2half2_rn(s * 0.0625f), z2 = __float2half2_rn(z);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const uint4 c = now.v[2 * y + j];
+                    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        *reinterpret_cast<uint4*>(Vs + st * S::TILE + kt_at(d, y * 8 + j * 4 + e)) = kt_codes(w[e], s2, s16, z2, true);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            kp_mbar_arrive(&v_full[st]);
+            now = next;
+        }
+        if (__builtin_expect(!ok, 0)) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+    } else if (warp == 12) {
+        // ---- the tensor core's work
+        if (lane == 0 && n_kt > 0) {
+            constexpr uint32_t idesc_pv = kt_idesc(128, HD, true);
+            bool ok = kp_mbar_wait_bounded(&q_full[0], 0) && kp_mbar_wait_bounded(&q_full[1], 0);
+            auto issue_s_both = [&](int i) {
+                if (!kp_mbar_wait_bounded(&k_full[i % ST], (i / ST) & 1)) return false;
+                for (int g = 0; g < 2; g++) {
+                    if (i > 0 && !kp_mbar_wait_bounded(&s_free[g], (i - 1) & 1)) return false;
+                    kp_tc_fence_after();
+                    kt_issue_s<HD>(tmem_base + 128 * g, Qs + g * S::OPER, Ks + (i % ST) * S::OPER);
+                    kp_umma_commit(&s_full[g]);
+                }
+                kp_umma_commit(&k_empty[i % ST]);
+                return true;
+            };
+            if (ok) ok = issue_s_both(0);
+            for (int i = 0; i < n_kt && ok; i++) {
+                if (i + 1 < n_kt && !issue_s_both(i + 1)) { ok = false; break; }
+                if (!kp_mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1)) { ok = false; break; }
+                const uint32_t va = kp_smem_u32(Vs + (i % ST) * S::TILE);
+                for (int g = 0; g < 2 && ok; g++) {
+                    if (!kp_mbar_wait_bounded(&p_full[g], i & 1)) { ok = false; break; }
+                    kp_tc_fence_after();
+                    const uint32_t pa = kp_smem_u32(Ps + g * S::PV);
+#pragma unroll
+                    for (int kk = 0; kk < KT_ROWS / 16; kk++)
+                        kp_umma_bf16(tmem_base + 256 + HD * g, kp_umma_desc(pa + (kk >> 2) * 16384) + 2 * (kk & 3),
+                                     HD == 64 ? kp_umma_desc(va + kk * 2048) : kp_umma_desc_mn(va + kk * 2048, 16384), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+                    kp_umma_commit(&o_done[g]);
+                }
+                if (ok) kp_umma_commit(&v_empty[i % ST]);
+            }
+            if (!ok) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+        }
+    } else {
+        // ---- the columns: warps 0-3 group 0, warps 4-7 group 1; thread r of a group has column r
+        const int g = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;
+        const int c = cta_col0 + g * 128 + r;
+        const bool live = c < n_cols;
+        const int pos = live ? min(pos0 + c / R, k_hi) : -1;
+        const size_t row = (size_t)(row0 + (live ? c / R : 0));
+        const int h = kvh * R + (live ? c % R : 0);
+        const float f = kt_write_query<HD>(Qs + g * S::OPER, r, live ? p.q + row * p.ldq + (size_t)h * HD : nullptr, p.scale);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        kp_mbar_arrive(&q_full[g]);
+        const size_t tile_id = ((size_t)blockIdx.y * p.n_tiles + blockIdx.x) * 2 + g;
+        if (p.mass && seg >= 0) {
+            // the pass that adds up the mass takes the same operand; this thread's row of it, as it lies
+            unsigned char* im = p.q_image + tile_id * S::OPER;
+            const unsigned char* from = Qs + g * S::OPER;
+#pragma unroll
+            for (int y = 0; y < S::NG; y++)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    *reinterpret_cast<uint4*>(im + y * 16384 + r * 128 + e * 16) = *reinterpret_cast<const uint4*>(from + y * 16384 + r * 128 + e * 16);
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                *reinterpret_cast<uint4*>(im + S::TILE + r * 32 + e * 16) = *reinterpret_cast<const uint4*>(from + S::TILE + r * 32 + e * 16);
+        }
+        const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+        // keys that every column of the group reads
+        const int g_first = min(cta_col0 + g * 128, max(n_cols - 1, 0)), g_last = min(cta_col0 + g * 128 + 127, max(n_cols - 1, 0));
+        const int all_hi = cta_col0 + g * 128 + 127 < n_cols ? min(pos0 + g_first / R, k_hi) : -1;
+        const int all_lo = p.window > 0 ? max(0, pos0 + g_last / R - p.window + 1) : 0;
+        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+        const uint32_t tmem_s = tmem_base + 128 * g + lane_off, tmem_o = tmem_base + 256 + HD * g + lane_off;
+        unsigned char* Pg = Ps + g * S::PV + r * 128;
+        bool ok = true;
+        float m = -INFINITY, l = 0.f;
+        int ev = -100;
+#pragma unroll 1
+        for (int i = 0; i < n_kt; i++) {
+            if (ok && (*abort_flag || !kp_mbar_wait_bounded(&s_full[g], i & 1))) ok = false;
+            kp_tc_fence_after();
+            uint32_t s0[32], s1[32];
+            kp_tmem_ld32_issue(tmem_s, s0);
+            kp_tmem_ld32_issue(tmem_s + 32, s1);
+            const int key0 = (kt_lo + i) * KT_ROWS;
+            const bool masked = !(key0 + KT_ROWS - 1 <= all_hi && key0 >= all_lo);
+            const float fk = f * kt_pow2(meta[(i & 3) * 2] - 7);
+            const int ev_now = meta[(i & 3) * 2 + 1];
+            float tmax = -INFINITY;
+            auto max32 = [&](const uint32_t (&s)[32], int at) {
+                if (masked) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (key0 + at + j >= lo && key0 + at + j <= pos) tmax = fmaxf(tmax, __uint_as_float(s[j]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) tmax = kt_max3(tmax, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                }
+            };
+            kp_tmem_ld_wait();
+            max32(s0, 0); max32(s1, 32);
+            kp_tmem_ld32_issue(tmem_s + 64, s0);
+            kp_tmem_ld32_issue(tmem_s + 96, s1);
+            kp_tmem_ld_wait();
+            max32(s0, 64); max32(s1, 96);
+            const float top = tmax * fk;
+            const float m_new = top > m + 8.0f ? top : m;                        // (the first: m = -inf)
+            const float corr_l = m_new == m ? 1.0f : kv4_exp2(m - m_new);
+            const float corr_o = corr_l * kt_pow2(ev - ev_now);
+            const float sub = m_new == -INFINITY ? 0.f : m_new - 7.0f;
+            if (i > 0) {
+                // the product of the tile before has read P and added to O
+                if (ok && !kp_mbar_wait_bounded(&o_done[g], (i - 1) & 1)) ok = false;
+                if (__any_sync(0xffffffffu, corr_o != 1.0f)) {
+                    kp_tc_fence_after();
+#pragma unroll 1
+                    for (int e = 0; e < HD; e += 16) {
+                        uint32_t v[16];
+                        kp_tmem_ld16_issue(tmem_o + e, v);
+                        kp_tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr_o);
+                        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                                     ::"r"(tmem_o + e), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+                                     "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+                    }
+                    kp_tmem_st_wait();
+                }
+            }
+            float lsum = 0.f;
+            auto p32 = [&](const uint32_t (&s)[32], int at, auto masked_c) {
+                constexpr bool MASKED = decltype(masked_c)::value;
+#pragma unroll
+                for (int j8 = 0; j8 < 4; j8++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j2 = 0; j2 < 4; j2++) {
+                        float pv[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int j = j8 * 8 + j2 * 2 + e;
+                            pv[e] = kv4_exp2(fmaf(__uint_as_float(s[j]), fk, -sub));
+                            if (MASKED && !(key0 + at + j >= lo && key0 + at + j <= pos)) pv[e] = 0.f;
+                        }
+                        lsum += pv[0] + pv[1];
+                        w[j2] = pack_f16(pv[0], pv[1]);
+                    }
+                    *reinterpret_cast<uint4*>(Pg + (at >> 6) * 16384 + (((((at & 63) >> 3) + j8) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            };
+            if (masked) { p32(s0, 64, std::true_type{}); p32(s1, 96, std::true_type{}); }
+            else { p32(s0, 64, std::false_type{}); p32(s1, 96, std::false_type{}); }
+            kp_tmem_ld32_issue(tmem_s, s0);
+            kp_tmem_ld32_issue(tmem_s + 32, s1);
+            kp_tmem_ld_wait();
+            kp_tc_fence_before();
+            kp_mbar_arrive(&s_free[g]);                                          // the next tile's S may be computed
+            if (masked) { p32(s0, 0, std::true_type{}); p32(s1, 32, std::true_type{}); }
+            else { p32(s0, 0, std::false_type{}); p32(s1, 32, std::false_type{}); }
+            l = l * corr_l + lsum;
+            m = m_new;
+            ev = ev_now;
+            kp_tc_fence_before();                                                // O (if rescaled) is written
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // P is read by the tensor core
+            kp_mbar_arrive(&p_full[g]);
+        }
+        if (n_kt > 0 && ok && !kp_mbar_wait_bounded(&o_done[g], (n_kt - 1) & 1)) ok = false;
+        kp_tc_fence_after();
+        const bool none = m == -INFINITY;
+        const float inv = none ? 0.f : kt_pow2(ev - 14) / l;
+        if (p.mass && seg >= 0) p.col[tile_id * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
+        bf16* dst = p.out + row * p.ldo + (size_t)h * HD;
+#pragma unroll 1
+        for (int e = 0; e < HD; e += 32) {
+            uint32_t v[32];
+            if (n_kt > 0) kp_tmem_ld32(tmem_o + e, v);
+            if (ok && live) {
+#pragma unroll
+                for (int d = 0; d < 32; d += 8) {
+                    // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[(j >> 1) + (j & 1) * 4] = none ? 0.f : __uint_as_float(v[d + j]) * inv;
+                    *reinterpret_cast<uint4*>(dst + e + d) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                }
+            }
+        }
+        kp_tc_fence_before();
+        if (__builtin_expect(!ok, 0)) { if (lane == 0) atomicExch(&g_kv4_tc_status, 1); }
+    }
+    kp_tc_fence_before();
+    __syncthreads();
+    if (warp == 12) kp_tmem_dealloc(tmem_base, 512);
+}
+
+// ---- mass.  One CTA per (128 keys, kv head, segment): S^T = K Q^T with a thread a key, so that a key's weights add up in its
+// thread.  The operands of Q and the columns' (factor, lse) are those that the kernel above left, brought by bulk copies into a
+// ring; the two groups of 128 threads take the tiles of 128 columns in turn, two S each under way, and are added at the end.
+template <int HD>
+__global__ void __launch_bounds__(Kt<HD>::THREADS, 1)
+kv4_tc_mass_kernel(const Kv4TcArgs p) {
+    using S = Kt<HD>;
+    constexpr int QST = S::QST;
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+    unsigned char* Ks = sm;                            // OPER
+    unsigned char* Qs = Ks + S::OPER;                  // [QST] IMAGE
+    uint64_t* bars = reinterpret_cast<uint64_t*>(Qs + QST * S::IMAGE);
+    uint64_t* k_full = bars;
+    uint64_t* q_full = bars + 1; uint64_t* q_empty = bars + 4;                   // [QST]
+    uint64_t* s_full = bars + 7; uint64_t* s_free = bars + 11;                   // [group][2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* tops = abort_flag + 1;               // [4]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        kp_mbar_init(k_full, 128);
+        for (int i = 0; i < QST; i++) { kp_mbar_init(&q_full[i], 1); kp_mbar_init(&q_empty[i], 1 + 128); }
+        for (int i = 0; i < 4; i++) { kp_mbar_init(&s_full[i], 1); kp_mbar_init(&s_free[i], 128); }
+        *abort_flag = 0;
+        kp_mbar_init_fence();
+    }
+    if (warp == 12) kp_tmem_alloc(tmem_slot, 512);
+    kp_tc_fence_before();
+    __syncthreads();
+    kp_tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    kp_pdl_begin();
+
+    const int seg = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x * KT_ROWS, R = p.H / p.G;
+    const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg], n_cols = n_rows * R;
+    const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+    const bool work = n_rows >= p.min_rows && k0 <= last && k0 + KT_ROWS - 1 >= first;
+    // columns that read any of the keys, in tiles of 128 from column 0
+    const int c_lo = max(0, k0 - pos0) * R;
+    const int c_hi = (p.window > 0 ? min(n_rows - 1, k0 + KT_ROWS - 1 + p.window - 1 - pos0) : n_rows - 1) * R + R - 1;
+    const int j_lo = c_lo / 128, n_j = work && c_hi >= c_lo ? c_hi / 128 - j_lo + 1 : 0;
+    const int top_tile = kt_first_tile(p, seg, R, lane);
+    float sum = 0.f;
+
+    if (warp >= 8 && warp < 12) {
+        const int d = threadIdx.x - 256, key = k0 + d;
+        const bool there = work && key >= first && key <= last;
+        const int page = there ? p.block_table[(size_t)seg * p.max_blocks + key / p.ps] : 0;
+        KtKey<HD> x;
+        x.load(p.pages + ((size_t)page * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key % p.ps, p.ps, there, false);
+        int ek = -100;
+#pragma unroll
+        for (int y = 0; y < S::NG; y++) ek = max(ek, kt_exponent(x.kr[y]));
+        ek = __reduce_max_sync(0xffffffffu, ek);
+        if (lane == 0) tops[warp & 3] = ek;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        ek = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+        kt_write_key<HD>(Ks, d, x.k, x.kr, ek);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        kp_mbar_arrive(k_full);
+        if (d == 0) {
+            bool ok = true;
+            for (int i = 0; i < n_j && ok; i++) {
+                const int st = i % QST, j = j_lo + i;
+                if (*abort_flag || !kp_mbar_wait_bounded(&q_empty[st], ((i / QST) & 1) ^ 1)) { ok = false; break; }
+                const size_t tile_id = ((size_t)kvh * p.n_tiles + top_tile - (j >> 1)) * 2 + (j & 1);
+                kp_mbar_expect_tx(&q_full[st], S::IMAGE);
+                kp_bulk_g2s(Qs + st * S::IMAGE, p.q_image + tile_id * S::OPER, S::OPER, &q_full[st]);
+                kp_bulk_g2s(Qs + st * S::IMAGE + S::OPER, p.col + tile_id * 128, 1024, &q_full[st]);
+            }
+            if (!ok) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+            if (*abort_flag) kp_linger_after_failure();      // copies may still be under way
+        }
+    } else if (warp == 12) {
+        if (lane == 0 && n_j > 0) {
+            bool ok = kp_mbar_wait_bounded(k_full, 0);
+            for (int i = 0; i < n_j && ok; i++) {
+                const int st = i % QST, g = i & 1, b = (i >> 1) & 1, use = i >> 2;       // S buffer (g, b) for the use-th time
+                ok = kp_mbar_wait_bounded(&q_full[st], (i / QST) & 1) && kp_mbar_wait_bounded(&s_free[2 * g + b], (use & 1) ^ 1);
+                if (!ok) break;
+                kp_tc_fence_after();
+                kt_issue_s<HD>(tmem_base + (2 * g + b) * 128, Ks, Qs + st * S::IMAGE);
+                kp_umma_commit(&s_full[2 * g + b]);
+                kp_umma_commit(&q_empty[st]);
+            }
+            if (!ok) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+        }
+    } else {
+        const int g = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane, key = k0 + r;
+        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
+        // columns that read this key
+        const bool there = key >= first && key <= last;
+        const int mine_lo = max(0, key - pos0) * R;
+        const int mine_hi = !there ? -1 : (p.window > 0 ? min(n_cols, (key + p.window - pos0) * R) : n_cols) - 1;
+        bool ok = n_j == 0 || kp_mbar_wait_bounded(k_full, 0);
+        const float kappa = kt_pow2(max(max(tops[0], tops[1]), max(tops[2], tops[3])) - 7);
+#pragma unroll 1
+        for (int i = g; i < n_j; i += 2) {
+            const int st = i % QST, b = (i >> 1) & 1, use = i >> 2;
+            if (ok && (*abort_flag || !kp_mbar_wait_bounded(&s_full[2 * g + b], use & 1))) ok = false;
+            // (the copies of the columns' factors arrived before the product that this waits for was issued; the wait makes them visible)
+            if (ok && !kp_mbar_wait_bounded(&q_full[st], (i / QST) & 1)) ok = false;
+            kp_tc_fence_after();
+            const float4* col = reinterpret_cast<const float4*>(Qs + st * S::IMAGE + S::OPER);
+            const int c0 = (j_lo + i) * 128;
+            const bool masked = __any_sync(0xffffffffu, c0 < mine_lo || c0 + 127 > mine_hi);
+            float part = 0.f;
+#pragma unroll 1
+            for (int e = 0; e < 128; e += 32) {
+                uint32_t s[32];
+                kp_tmem_ld32(tmem_base + (2 * g + b) * 128 + lane_off + e, s);
+                float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    const float4 f = col[(e + j) >> 1];                          // (factor, lse) of two columns
+                    float p0 = kv4_exp2(fmaf(__uint_as_float(s[j]) * kappa, f.x, -f.y));
+                    float p1 = kv4_exp2(fmaf(__uint_as_float(s[j + 1]) * kappa, f.z, -f.w));
+                    if (masked) {
+                        if (!(c0 + e + j >= mine_lo && c0 + e + j <= mine_hi)) p0 = 0.f;
+                        if (!(c0 + e + j + 1 >= mine_lo && c0 + e + j + 1 <= mine_hi)) p1 = 0.f;
+                    }
+                    a0 += p0; a1 += p1;
+                }
+                part += a0 + a1;
+            }
+            kp_tc_fence_before();
+            kp_mbar_arrive(&s_free[2 * g + b]);
+            kp_mbar_arrive(&q_empty[st]);
+            sum += part;
+        }
+        if (__builtin_expect(!ok, 0)) { if (lane == 0) atomicExch(&g_kv4_tc_status, 1); sum = 0.f; }
+    }
+    kp_tc_fence_before();
+    __syncthreads();
+    if (warp == 12) kp_tmem_dealloc(tmem_base, 512);
+    float* join = reinterpret_cast<float*>(Ks);
+    if (warp >= 4 && warp < 8) join[threadIdx.x - 128] = sum;
+    __syncthreads();
+    if (warp < 4 && n_j > 0) {
+        const int key = k0 + threadIdx.x;
+        if (key >= first && key <= last) {
+            const int page = p.block_table[(size_t)seg * p.max_blocks + key / p.ps];
+            p.mass[((size_t)page * p.G + kvh) * p.ps + key % p.ps] += sum + join[threadIdx.x];
+        }
+    }
+}
+
+template <int HD>
+static int kt_run(const Kv4TcArgs& a, int max_context, cudaStream_t st) {
+    using S = Kt<HD>;
+    static std::atomic<unsigned long long> ready{0}, ready_mass{0};
+    int e = kp_smem_limit(kv4_tc_kernel<HD>, S::SMEM, ready);
+    if (e) return e;
+    cudaError_t c = kp_launch_pdl(kv4_tc_kernel<HD>, dim3(a.n_tiles, a.G), dim3(S::THREADS), S::SMEM, st, a);
+    if (c) return (int)c;
+    if (a.mass) {
+        e = kp_smem_limit(kv4_tc_mass_kernel<HD>, S::MASS_SMEM, ready_mass);
+        if (e) return e;
+        c = kp_launch_pdl(kv4_tc_mass_kernel<HD>, dim3((max_context + KT_ROWS - 1) / KT_ROWS, a.G, a.n_seg), dim3(S::THREADS), S::MASS_SMEM, st, a);
+        if (c) return (int)c;
+    }
+    return kp_launch_status();
+}
+
+extern "C" {
+
+// Bytes of the operand image and of the columns' factors that a call with mass needs beside each other (16-byte aligned).
+long long kp_kv4_tc_scratch(int n_rows, int n_seg, int H, int G, int hd) {
+    const long long tiles = ((long long)n_rows * (H / G) + 255) / 256 + n_seg;
+    return tiles * G * 2 * ((hd / 64) * 16384 + KT_EXT + 1024);
+}
+
+// The segments of at least min_rows rows (bfloat16, head size 64 or 128); scratch (with mass): kp_kv4_tc_scratch bytes.
+int kp_kv4_attention_tc(const void* q, long long ldq, const void* pages, const int* block_table, int max_blocks, const int* cu_rows,
+                        const int* seg_pos, int n_seg, void* out, long long ldo, float scale, int window, int ps, int H, int G, int hd, int n_rows,
+                        int min_rows, int max_context, float* mass, void* scratch, void* stream) {
+    if (n_rows <= 0 || n_seg <= 0) return 0;
+    if (G < 1 || H < 1 || H % G || ps < 16 || ps % 16 || window < 0 || n_seg > 65535 || G > 65535 || min_rows < 1 || !(scale > 0.f) ||
+        (((uintptr_t)pages | (uintptr_t)q | (uintptr_t)out | (uintptr_t)scratch) & 15) || (ldq & 7) || (ldo & 7) || (mass && !scratch))
+        return KP_ERR_BAD_ARG;
+    const int R = H / G;
+    const long long tiles = ((long long)n_rows * R + 255) / 256 + n_seg;
+    Kv4TcArgs a = {};
+    a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo; a.pages = (const unsigned char*)pages;
+    a.block_table = block_table; a.max_blocks = max_blocks; a.cu_rows = cu_rows; a.seg_pos = seg_pos;
+    a.scale = scale; a.window = window; a.ps = ps; a.H = H; a.G = G; a.mass = mass; a.min_rows = min_rows; a.n_seg = n_seg; a.n_tiles = (int)tiles;
+    if (mass) {
+        a.q_image = (unsigned char*)scratch;
+        a.col = (float2*)((unsigned char*)scratch + (size_t)tiles * G * 2 * ((hd / 64) * 16384 + KT_EXT));
+    }
+    if (hd == 64) return kt_run<64>(a, max_context, (cudaStream_t)stream);
+    if (hd == 128) return kt_run<128>(a, max_context, (cudaStream_t)stream);
+    return KP_ERR_UNSUPPORTED;
+}
+
+}  // extern "C"

@@ -17,6 +17,7 @@ from .kernels import STREAM, KernelError, _need, _ptr, _rows_2d, _run, dtype_cod
 
 KV4_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 KV4_SHORT_ROWS = 8         # segments of at most this many rows share their keys out over many CTAs
+USE_TC_KV4 = True          # longer ones of bfloat16 rows with heads of 64 or 128 run on the tcgen05 tensor cores
 _CTAS = 148 * 4            # CTAs of the split form that an even spread over the SMs wants
 
 
@@ -82,6 +83,12 @@ def kv4_chunks(n_seg: int, max_rows: int, max_context: int, window: Optional[int
     return -(-max_context // chunk), chunk
 
 
+def kv4_tc_ok(q: torch.Tensor, out: torch.Tensor, hd: int, scale: float) -> bool:
+    """Does the tcgen05 form take these rows (bfloat16, heads of 64 or 128, rows on 16-byte boundaries)?"""
+    return (USE_TC_KV4 and q.dtype == torch.bfloat16 and hd in (64, 128) and scale > 0 and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0
+            and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
+
+
 def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tensor, cu_rows: torch.Tensor, seg_pos: torch.Tensor,
                   out: torch.Tensor, scale: float, window: Optional[int], page_size: int, H: int, G: int, hd: int, max_rows: int,
                   max_context: int, min_rows: int = 1, mass: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -110,18 +117,30 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd)
     part_o = part_ml = scores = lse_split = lse = None
     floats = lambda count: torch.empty(count, dtype=torch.float32, device=q.device)  # noqa: E731
-    places, tiled = n_seg * short * H, max_rows > KV4_SHORT_ROWS
+    places = n_seg * short * H
+    tiled = max_rows > KV4_SHORT_ROWS
+    tc = tiled and kv4_tc_ok(q, out, hd, scale)
     if short and n_chunks > 1:
         part_o, part_ml = floats(places * n_chunks * hd), floats(places * n_chunks * 2)
     if mass is not None:
         if short:
             scores, lse_split = floats(places * n_chunks * chunk), floats(places)
-        if tiled:
+        if tiled and not tc:
             lse = floats(n * H)
-    _run("kv4_attention", load_library("kv4").kp_kv4_attention, _ptr(q), ctypes.c_longlong(_rows_2d(q, "q")), _ptr(pages), _ptr(block_table),
-         block_table.shape[1], _ptr(cu_rows), _ptr(seg_pos), n_seg, _ptr(out), ctypes.c_longlong(_rows_2d(out, "out")), ctypes.c_float(scale),
-         int(window or 0), page_size, H, G, hd, n, short, int(tiled), n_chunks, chunk, max_context, _ptr(part_o), _ptr(part_ml),
-         _ptr(scores), n_chunks * chunk, _ptr(lse_split), _ptr(lse), _ptr(mass), dtype_code(q.dtype), STREAM)
+    ldq, ldo = ctypes.c_longlong(_rows_2d(q, "q")), ctypes.c_longlong(_rows_2d(out, "out"))
+    if short or (tiled and not tc):
+        _run("kv4_attention", load_library("kv4").kp_kv4_attention, _ptr(q), ldq, _ptr(pages), _ptr(block_table), block_table.shape[1], _ptr(cu_rows),
+             _ptr(seg_pos), n_seg, _ptr(out), ldo, ctypes.c_float(scale), int(window or 0), page_size, H, G, hd, n, short, int(tiled and not tc),
+             n_chunks, chunk, max_context, _ptr(part_o), _ptr(part_ml), _ptr(scores), n_chunks * chunk, _ptr(lse_split), _ptr(lse), _ptr(mass),
+             dtype_code(q.dtype), STREAM)
+    if tc:
+        lib, scratch = load_library("kv4_tc"), None
+        if mass is not None:
+            lib.kp_kv4_tc_scratch.restype = ctypes.c_longlong
+            scratch = torch.empty(lib.kp_kv4_tc_scratch(n, n_seg, H, G, hd), dtype=torch.uint8, device=q.device)
+        _run("kv4_attention_tc", lib.kp_kv4_attention_tc, _ptr(q), ldq, _ptr(pages), _ptr(block_table), block_table.shape[1], _ptr(cu_rows),
+             _ptr(seg_pos), n_seg, _ptr(out), ldo, ctypes.c_float(scale), int(window or 0), page_size, H, G, hd, n, short + 1, max_context,
+             _ptr(mass), _ptr(scratch), STREAM)
     return out
 
 
