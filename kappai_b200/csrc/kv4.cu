@@ -25,85 +25,106 @@ __device__ __forceinline__ void kv4_load8(float (&v)[8], const T* p) {
     }
 }
 
-template <typename T, bool VEC>
+// Thread idx of a launch of `n_threads`: place `idx % per_row` of the rows idx / per_row + u (n_threads / per_row), u < U.  With
+// U rows a thread their loads are under way together: one row a thread leaves a CTA waiting for its slot, then for its values
+// (6,007 rows of 8 heads of 128 float32 values written: 29 us with one, 20 with four).
+struct Kv4Rows { int n, ps_log2, G, hd, gs; long long n_slots; };
+
+template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(256)
 kv4_write_kernel(const T* __restrict__ k, long long ldk, const T* __restrict__ v, long long ldv, unsigned char* __restrict__ pages,
-                 const int* __restrict__ slot_map, long long n_slots, int n, int ps, int G, int hd, int gs) {
+                 const int* __restrict__ slot_map, const Kv4Rows p) {
     kp_pdl_begin();
-    const int per_row = G * hd / 8;                        // threads a row of k (and of v)
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long unit = idx / per_row;                  // (row, k or v)
-    const int within = (int)(idx - unit * per_row);
-    const bool live = unit < 2LL * n;
-    const int row = live ? (int)(unit >> 1) : 0;
-    const bool is_v = unit & 1;
-    const int head = within / (hd / 8), d8 = within - head * (hd / 8);
-    const int lanes = gs / 8;                              // of a group
-    const long long slot = live ? slot_map[row] : -1;
-    float x[8];
+    const int half = p.G * p.hd / 8, per_row = 2 * half;   // threads a row: its keys, then its values
+    const unsigned idx = blockIdx.x * 256u + threadIdx.x;
+    const int row0 = idx / per_row, place = idx - (unsigned)row0 * per_row, step = (p.n + U - 1) / U;
+    const bool is_v = place >= half;
+    const int within = is_v ? place - half : place, head = within / (p.hd / 8), d8 = within - head * (p.hd / 8);
+    const int lanes = p.gs / 8, ng = p.hd / p.gs;          // lanes of a group, groups of a head
+    const T* src = (is_v ? v : k) + within * 8;
+    const long long ld = is_v ? ldv : ldk;
+    int slot[U];
+    float x[U][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = 0.f;
-    if (slot >= 0 && slot < n_slots) kv4_load8<T, VEC>(x, (is_v ? v + row * ldv : k + row * ldk) + (size_t)head * hd + d8 * 8);
-    // a range that holds a NaN, or an infinity, is none: the group reads as NaN
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int i = 1; i < 8; i++) { lo = kv4_min_nan(lo, x[i]); hi = kv4_max_nan(hi, x[i]); }
-    for (int d = 1; d < lanes; d <<= 1) {
-        lo = kv4_min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-        hi = kv4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    for (int u = 0; u < U; u++) {
+        const int row = row0 + u * step;
+        slot[u] = row0 < step && row < p.n ? slot_map[row] : -1;
+        if (slot[u] >= p.n_slots) slot[u] = -1;
     }
-    if (slot < 0 || slot >= n_slots) return;
-    const bf16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.0f)), zb = __float2bfloat16_rn(lo);
-    const float s = __bfloat162float(sb), z = __bfloat162float(zb);
-    uint32_t w = 0;
-    if (s > 0.f) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) w |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i] - z, s)), 0.f), 15.f) << (4 * i);
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[u][i] = 0.f;
+        if (slot[u] >= 0) kv4_load8<T, VEC>(x[u], src + (row0 + u * step) * ld);
     }
-    const int page = (int)(slot / ps), off = (int)(slot - (long long)page * ps), ng = hd / gs;
-    unsigned char* rec = pages + ((size_t)page * G + head) * kv4_page_bytes(ps, hd);
-    unsigned char* codes = rec + (is_v ? (size_t)ps * (hd / 2) : 0) + (size_t)off * (hd / 2);
-    *reinterpret_cast<uint32_t*>(codes + d8 * 4) = w;
-    if (d8 % lanes == 0) {
-        unsigned char* ranges = rec + (size_t)ps * hd + (is_v ? (size_t)ps * 4 * ng : 0);
-        reinterpret_cast<uint32_t*>(ranges)[off * ng + d8 / lanes] =
-            (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        // a range that holds a NaN, or an infinity, is none: the group reads as NaN
+        float lo = x[u][0], hi = x[u][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) { lo = kv4_min_nan(lo, x[u][i]); hi = kv4_max_nan(hi, x[u][i]); }
+        for (int d = 1; d < lanes; d <<= 1) {
+            lo = kv4_min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+            hi = kv4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+        }
+        if (slot[u] < 0) continue;
+        const bf16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.0f)), zb = __float2bfloat16_rn(lo);
+        const float s = __bfloat162float(sb), z = __bfloat162float(zb);
+        uint32_t w = 0;
+        if (s > 0.f) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) w |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[u][i] - z, s)), 0.f), 15.f) << (4 * i);
+        }
+        const int ps = 1 << p.ps_log2, page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);
+        unsigned char* rec = pages + ((size_t)page * p.G + head) * kv4_page_bytes(ps, p.hd);
+        reinterpret_cast<uint32_t*>(rec + (size_t)((is_v ? ps : 0) + off) * (p.hd / 2))[d8] = w;
+        if (d8 % lanes == 0)
+            reinterpret_cast<uint32_t*>(rec + (size_t)ps * p.hd)[((is_v ? ps : 0) + off) * ng + d8 / lanes] =
+                (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
     }
 }
 
-template <typename T>
+template <typename T, int U>
 __global__ void __launch_bounds__(256)
-kv4_read_kernel(const unsigned char* __restrict__ pages, const int* __restrict__ slot_map, long long n_slots, T* __restrict__ k, T* __restrict__ v,
-                int n, int ps, int G, int hd, int gs) {
+kv4_read_kernel(const unsigned char* __restrict__ pages, const int* __restrict__ slot_map, T* __restrict__ k, T* __restrict__ v, const Kv4Rows p) {
     kp_pdl_begin();
-    const int per_row = G * hd / 8;
-    const long long idx = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long unit = idx / per_row;
-    if (unit >= 2LL * n) return;
-    const int within = (int)(idx - unit * per_row);
-    const int row = (int)(unit >> 1);
-    const bool is_v = unit & 1;
-    const int head = within / (hd / 8), d8 = within - head * (hd / 8), ng = hd / gs;
-    const long long slot = slot_map[row];
-    float x[8];
-    if (slot >= 0 && slot < n_slots) {
-        const int page = (int)(slot / ps), off = (int)(slot - (long long)page * ps);
-        const unsigned char* rec = pages + ((size_t)page * G + head) * kv4_page_bytes(ps, hd);
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + (is_v ? (size_t)ps * (hd / 2) : 0) + (size_t)off * (hd / 2) + d8 * 4);
-        const uint32_t r = reinterpret_cast<const uint32_t*>(rec + (size_t)ps * hd + (is_v ? (size_t)ps * 4 * ng : 0))[off * ng + d8 / (gs / 8)];
-        const float s = kv4_scale(r), z = kv4_least(r);
+    const int half = p.G * p.hd / 8, per_row = 2 * half;
+    const unsigned idx = blockIdx.x * 256u + threadIdx.x;
+    const int row0 = idx / per_row, place = idx - (unsigned)row0 * per_row, step = (p.n + U - 1) / U;
+    if (row0 >= step) return;
+    const bool is_v = place >= half;
+    const int within = is_v ? place - half : place, head = within / (p.hd / 8), d8 = within - head * (p.hd / 8), ng = p.hd / p.gs, g = d8 / (p.gs / 8);
+    int slot[U];
+    uint32_t w[U], r[U];
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = fmaf(s, (float)((w >> (4 * i)) & 15u), z);       // (s c is exact)
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = 0.f;            // a row without a slot reads as zeros
+    for (int u = 0; u < U; u++) {
+        const int row = row0 + u * step;
+        slot[u] = row < p.n ? slot_map[row] : -1;
     }
-    T* dst = (is_v ? v : k) + (size_t)row * G * hd + within * 8;
-    if (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-    } else {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        w[u] = r[u] = 0u;                                  // a row without a slot reads as zeros
+        if (slot[u] < 0 || slot[u] >= p.n_slots) continue;
+        const int ps = 1 << p.ps_log2, page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);
+        const unsigned char* rec = pages + ((size_t)page * p.G + head) * kv4_page_bytes(ps, p.hd);
+        w[u] = reinterpret_cast<const uint32_t*>(rec + (size_t)((is_v ? ps : 0) + off) * (p.hd / 2))[d8];
+        r[u] = reinterpret_cast<const uint32_t*>(rec + (size_t)ps * p.hd)[((is_v ? ps : 0) + off) * ng + g];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int row = row0 + u * step;
+        if (row >= p.n) break;
+        const float s = kv4_scale(r[u]), z = kv4_least(r[u]);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = fmaf(s, (float)((w[u] >> (4 * i)) & 15u), z);       // (s c is exact)
+        T* dst = (is_v ? v : k) + (size_t)row * p.G * p.hd + within * 8;
+        if (sizeof(T) == 2) {
+            *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+        } else {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        }
     }
 }
 
@@ -114,7 +135,7 @@ struct Kv4Args {
     const unsigned char* pages;
     const int* block_table; int max_blocks;
     const int* cu_rows; const int* seg_pos;
-    float scale; int window; int ps; int H, G;
+    float scale; int window; int ps, ps_log2; int H, G;
     // split form, [place] = [segment][row of it, of max_rows][head]: results of chunks [place][chunk][hd], (shift, sum of p)
     // [place][chunk][2]; with mass, or else null: scores [place][key], shift + log2(sum of p) [place]
     float* part_o; float* part_ml; float* scores; int ld_scores; float* lse_split;
@@ -143,26 +164,37 @@ __device__ __forceinline__ void kv4_columns(Kv4Cols<NT>& C, int col0, int n_cols
         }
 }
 
-// ---- split form: few rows a segment (decode).  One CTA per (chunk of keys, kv head and 8 of its columns, segment): its four warps take the
-// chunk's tiles in turn, each with a ring of its own in shared memory that cp.async fills, and are joined at the end.  Many
-// small CTAs on an SM keep enough loads in flight; nothing but the end waits for another warp.
+// ---- split form: few rows a segment (decode).  One CTA per (chunk of keys, kv head and 8 of its columns, segment).  Its tiles of KEYS
+// keys come by the TMA into a ring of three stages, asked for two tiles ahead by the warps in turn; each of the four warps takes a
+// quarter of a tile, with the softmax and output of its own keys, and the four are joined at the end.  What bounds it is the issue of
+// instructions, 170 a block of 16 keys of 64 values (1,152 bytes; 192 slots would pass while those come at the copy rate): hence the TMA and
+// not cp.async (97 instructions a block), tiles asked for by one warp and not by each (65 against 15), four CTAs an SM.
+KP_STATUS_WORD(g_kv4_status, kv4)                     // 0 ok; 1: a bounded wait gave up
+
 template <int HD, int PARTS>
 struct Kv4Split {
-    static constexpr int TB = HD <= 64 ? 4 : (HD <= 128 ? 2 : 1), STAGES = 3, NW = 4;
-    static constexpr int TILE = TB * 16, STAGE = TB * Kv4<HD>::BLOCK;
-    static constexpr size_t RING = (size_t)NW * STAGES * STAGE, JOIN = sizeof(float) * NW * 8 * (HD + 2);
-    static constexpr size_t SMEM = RING > JOIN ? RING : JOIN;
+    static constexpr int TILE = HD <= 64 ? 64 : (HD <= 128 ? 32 : 16), TB = TILE / 16, STAGES = 3, NW = 4, KEYS = NW * TILE;
+    static constexpr int STAGE = (Kv4<HD>::bytes(KEYS) + 1023) / 1024 * 1024;
+    static constexpr size_t RING = (size_t)STAGES * STAGE, JOIN = sizeof(float) * NW * 8 * (HD + 2);
+    static constexpr size_t SMEM = 1024 + (RING > JOIN ? RING : JOIN);
 };
 
 template <int HD, int PARTS, bool KEEP, typename T>
-__global__ void __launch_bounds__(128)
-kv4_split_kernel(const Kv4Args p) {
+__global__ void __launch_bounds__(128, PARTS == 1 && HD <= 128 ? 4 : 2)
+kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
     using F = Kv4<HD>;
     using S = Kv4Split<HD, PARTS>;
     constexpr bool CENTRE = KEEP || PARTS > 1;
+    extern __shared__ unsigned char smem_dyn[];
+    __shared__ uint64_t full[S::STAGES], empty[S::STAGES];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the warp's number in a uniform register)
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; i++) { kp_mbar_init(&full[i], 1); kp_mbar_init(&empty[i], S::NW); }
+        kp_mbar_init_fence();
+    }
+    __syncthreads();
     kp_pdl_begin();
-    extern __shared__ __align__(16) unsigned char smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int R = p.H / p.G, kvh = blockIdx.y % p.G, seg = blockIdx.z, chunk = blockIdx.x;
     const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg];
     const int col0 = (blockIdx.y / p.G) * 8, n_cols = n_rows * R;
@@ -172,37 +204,50 @@ kv4_split_kernel(const Kv4Args p) {
     const int k_hi = min(min(pos0 + col1 / R, (chunk + 1) * p.chunk - 1), p.max_blocks * p.ps - 1);
     const int k_first = p.window > 0 ? max(0, pos0 + col0 / R - p.window + 1) : 0;
     const int k_lo = max(k_first, chunk * p.chunk);
-    const int t_lo = k_lo / S::TILE, n_tiles = k_hi >= k_lo ? k_hi / S::TILE - t_lo + 1 : 0;
+    const int t_lo = k_lo / S::KEYS, n_tiles = k_hi >= k_lo ? k_hi / S::KEYS - t_lo + 1 : 0;
     if (p.n_chunks > 1 && n_tiles == 0) return;            // (a single chunk writes its rows also where they read nothing)
     const int* bt = p.block_table + (size_t)seg * p.max_blocks;
-    const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);
-    unsigned char* ring = smem + (size_t)warp * S::STAGES * S::STAGE;
 
-    auto load = [&](int i) {                               // the warp's i-th tile
-        const int tile = warp + i * S::NW;
-        if (tile < n_tiles) {
-            unsigned char* dst = ring + (i % S::STAGES) * S::STAGE;
-#pragma unroll
-            for (int b = 0; b < S::TB; b++) {
-                const int key = (t_lo + tile) * S::TILE + b * 16;
-                if (key <= k_hi && key + 15 >= k_lo) {
-                    const int page = key / p.ps;
-                    kv4_load_block<HD>(dst + b * F::BLOCK, p.pages + ((size_t)bt[page] * p.G + kvh) * rec, key - page * p.ps, p.ps, lane);
-                }
-            }
-        }
-        cp_async_commit();
+    // Lane j has piece j of a tile: the keys of one page (at most 16 pieces).
+    const int piece = min(p.ps, S::KEYS);
+    auto page_of = [&](int i) {                            // piece's page of tile i, or -1 if nothing of it is read
+        const int key = (t_lo + i) * S::KEYS + lane * piece;
+        return i < n_tiles && lane * piece < S::KEYS && key <= k_hi && key + piece - 1 >= k_lo ? bt[key >> p.ps_log2] : -1;
     };
-#pragma unroll
-    for (int i = 0; i < S::STAGES - 1; i++) load(i);
+    auto load = [&](int i, int page) {
+        unsigned char* dst = smem + (i % S::STAGES) * S::STAGE;
+        uint64_t* bar = &full[i % S::STAGES];
+        const unsigned need = __ballot_sync(0xffffffffu, page >= 0);
+        kp_mbar_expect_tx_warp(bar, (uint32_t)(__popc(need) * F::bytes(piece)));
+        const int off = (t_lo + i) * S::KEYS & (p.ps - 1);
+        // (piece by piece and by an elected lane, so that the copies' operands are uniform)
+        for (int j = 0; j * piece < S::KEYS; j++) {
+            const int rec = __shfl_sync(0xffffffffu, page, j) * p.G + kvh, at = j * piece;
+            if (!(need >> j & 1)) continue;
+            kp_tma_load_3d_warp(dst + at * F::ROW, &codes, 0, off, rec, bar);
+            kp_tma_load_3d_warp(dst + (S::KEYS + at) * F::ROW, &codes, 0, p.ps + off, rec, bar);
+            // (64 bytes of ranges a piece where pages have 16 keys: less than a tensor copy's destination is aligned to)
+            const unsigned char* from = p.pages + (size_t)rec * kv4_page_bytes(p.ps, HD) + (size_t)p.ps * HD + off * 4 * F::NG;
+            unsigned char* r = dst + S::KEYS * HD + at * 4 * F::NG;
+            kp_bulk_g2s_warp(r, from, piece * 4 * F::NG, bar);
+            kp_bulk_g2s_warp(r + S::KEYS * 4 * F::NG, from + (size_t)p.ps * 4 * F::NG, piece * 4 * F::NG, bar);
+        }
+    };
+    // warp w asks for tiles w, w + 4, ...; the first two before anything else
+    int page = page_of(warp);
+    if (warp < S::STAGES - 1 && warp < n_tiles) {
+        load(warp, page);
+        page = page_of(warp + S::NW);
+    }
 
+    const Kv4Block<HD, S::KEYS> B(lane);
     Kv4Cols<1> C;
     kv4_columns<1>(C, col0, n_cols, R, pos0, p.window, lane);
     Kv4Q<HD, PARTS, 1> Q;
     {
         const int c = col0 + (lane >> 2);
-        const T* src = c < n_cols ? (const T*)p.q + (size_t)(row0 + c / R) * p.ldq + (size_t)(kvh * R + c % R) * HD : nullptr;
-        kv4_load_q<HD, PARTS, 1, CENTRE, T>(Q, 0, src, p.scale, lane);
+        const T* const src[1] = {c < n_cols ? (const T*)p.q + (size_t)(row0 + c / R) * p.ldq + (size_t)(kvh * R + c % R) * HD : nullptr};
+        kv4_load_q<HD, PARTS, 1, CENTRE, T>(Q, src, p.scale, lane);
     }
     float* sc[1][2] = {{nullptr, nullptr}};
     if (KEEP) {
@@ -216,20 +261,36 @@ kv4_split_kernel(const Kv4Args p) {
     A.clear();
     // no key at all is masked between these
     const int safe_lo = p.window > 0 ? max(0, pos0 + col1 / R - p.window + 1) : 0, safe_hi = min(k_hi, pos0 + col0 / R);
+    bool ok = true;
+    int stage = 0, phase = 0;
 #pragma unroll 1
-    for (int i = 0; warp + i * S::NW < n_tiles; i++) {
-        load(i + S::STAGES - 1);
-        cp_async_wait<S::STAGES - 1>();
+    for (int i = 0; i < n_tiles; i++) {
+        const int ahead = i + S::STAGES - 1;
+        if (ahead < n_tiles && warp == ahead % S::NW) {
+            // its stage is that of tile i - 1, which every warp has to be through with
+            if (i > 0) ok = __all_sync(0xffffffffu, kp_mbar_wait_bounded(&empty[ahead % S::STAGES], ((ahead / S::STAGES) & 1) ^ 1));
+            if (!ok) break;
+            load(ahead, page);
+            page = page_of(ahead + S::NW);
+        }
+        ok = __all_sync(0xffffffffu, kp_mbar_wait_bounded(&full[stage], phase));      // (a warp gives up as one)
+        if (!ok) break;
+        const int key0 = (t_lo + i) * S::KEYS + warp * S::TILE;
+        const unsigned char* tile = smem + stage * S::STAGE;
+        if (key0 <= k_hi && key0 + S::TILE - 1 >= k_lo) {
+            if (key0 >= max(k_lo, safe_lo) && key0 + S::TILE - 1 <= safe_hi)
+                kv4_tile<HD, S::KEYS, PARTS, 1, S::TB, CENTRE, false, KEEP>(A, Q, B, tile, warp * S::TILE, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+            else
+                kv4_tile<HD, S::KEYS, PARTS, 1, S::TB, CENTRE, true, KEEP>(A, Q, B, tile, warp * S::TILE, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+        }
         __syncwarp();
-        const int key0 = (t_lo + warp + i * S::NW) * S::TILE;
-        const unsigned char* tile = ring + (i % S::STAGES) * S::STAGE;
-        if (key0 >= max(k_lo, safe_lo) && key0 + S::TILE - 1 <= safe_hi)
-            kv4_tile<HD, PARTS, 1, S::TB, CENTRE, false, KEEP>(A, Q, tile, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
-        else
-            kv4_tile<HD, PARTS, 1, S::TB, CENTRE, true, KEEP>(A, Q, tile, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
-        __syncwarp();
+        if (lane == 0) kp_mbar_arrive(&empty[stage]);
+        if (++stage == S::STAGES) { stage = 0; phase ^= 1; }
     }
-    cp_async_wait<0>();
+    if (__builtin_expect(!ok, 0)) {
+        if (lane == 0) atomicExch(&g_kv4_status, 1);
+        kp_linger_after_failure();
+    }
     A.finish();
     __syncthreads();                                       // the rings are done with: the warps' results take their place
     float* jo = reinterpret_cast<float*>(smem);            // [warp][column][HD]
@@ -272,53 +333,104 @@ kv4_split_kernel(const Kv4Args p) {
     }
 }
 
-// ---- joins the chunks of a (row, head): one CTA each, in the order of the chunks
-template <typename T>
-__global__ void __launch_bounds__(128)
-kv4_merge_kernel(const Kv4Args p, int hd) {
-    kp_pdl_begin();
-    const int seg = blockIdx.x / p.max_rows, r = blockIdx.x % p.max_rows, h = blockIdx.y;
-    const int row = p.cu_rows[seg] + r, n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg];
-    if (r >= n_rows || n_rows > p.max_rows) return;
-    const int hi = p.seg_pos[seg] + r;
-    const int lo = p.window > 0 ? max(0, hi - p.window + 1) : 0;
-    const size_t rh = (size_t)blockIdx.x * p.H + h;
-    const float* ml = p.part_ml + rh * p.n_chunks * 2;
-    const float* po = p.part_o + rh * p.n_chunks * hd;
-    const int c_lo = lo / p.chunk, c_hi = hi < 0 ? -1 : min(hi / p.chunk, p.n_chunks - 1);
+// ---- joins the chunks and adds up the mass: a warp a (segment, row, head), in the order of the chunks; behind those CTAs, where
+// there is mass, a CTA a (128 keys, kv head, segment) with a thread a key, rows and heads in order.  Both find a (row, head)'s shift and sum from
+// the chunks' (at most a few dozen), so that neither waits for the other.
+// Largest shift and sum of p of the chunks c_lo .. c_hi of a place; every lane gets them.
+__device__ __forceinline__ float2 kv4_total(const float* ml, int c_lo, int c_hi, int lane) {
     float M = -INFINITY, L = 0.f;
-    for (int c = c_lo; c <= c_hi; c++) M = fmaxf(M, ml[2 * c]);
-    for (int c = c_lo; c <= c_hi; c++)
-        if (ml[2 * c] != -INFINITY) L = fmaf(ml[2 * c + 1], kv4_exp2(ml[2 * c] - M), L);
-    for (int d = threadIdx.x; d < hd; d += 128) {
-        float acc = 0.f;
-        for (int c = c_lo; c <= c_hi; c++)
-            if (ml[2 * c] != -INFINITY) acc = fmaf(po[(size_t)c * hd + d], kv4_exp2(ml[2 * c] - M), acc);
-        ((T*)p.out)[(size_t)row * p.ldo + (size_t)h * hd + d] = from_f32<T>(M == -INFINITY ? 0.f : acc / L);
+    for (int c0 = c_lo; c0 <= c_hi; c0 += 32) {
+        const int c = c0 + lane;
+        const float2 x = c <= c_hi ? reinterpret_cast<const float2*>(ml)[c] : make_float2(-INFINITY, 0.f);
+        const float top = fmaxf(M, warp_max(x.x));
+        const float part = warp_sum(x.x == -INFINITY ? 0.f : x.y * kv4_exp2(x.x - top));
+        L = (M == -INFINITY ? 0.f : L * kv4_exp2(M - top)) + part;
+        M = top;
     }
-    if (p.lse_split && threadIdx.x == 0) p.lse_split[rh] = M == -INFINITY ? INFINITY : M + log2f(L);
+    return make_float2(M, L);
 }
 
-// ---- adds the weights of the split form's rows to their keys' mass: a thread a key, rows and heads in order
+template <typename T>
 __global__ void __launch_bounds__(128)
-kv4_split_mass_kernel(const Kv4Args p) {
+kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
     kp_pdl_begin();
-    const int seg = blockIdx.z, kvh = blockIdx.y, key = blockIdx.x * 128 + threadIdx.x;
-    const int n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg], pos0 = p.seg_pos[seg], R = p.H / p.G;
+    const int lane = threadIdx.x & 31;
+    if ((int)blockIdx.x < n_join) {
+        const int place = blockIdx.x * 4 + (threadIdx.x >> 5);
+        const int h = place % p.H, r = (place / p.H) % p.max_rows, seg = place / p.H / p.max_rows;
+        if (seg >= p.n_seg) return;
+        const int row = p.cu_rows[seg] + r, n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg];
+        if (r >= n_rows || n_rows > p.max_rows) return;
+        const int hi = p.seg_pos[seg] + r;
+        const int lo = p.window > 0 ? max(0, hi - p.window + 1) : 0;
+        const float* ml = p.part_ml + (size_t)place * p.n_chunks * 2;
+        const float* po = p.part_o + (size_t)place * p.n_chunks * hd;
+        const int c_lo = lo / p.chunk, c_hi = hi < 0 ? -1 : min(hi / p.chunk, p.n_chunks - 1);
+        const float2 t = kv4_total(ml, c_lo, c_hi, lane);
+        const float inv = t.x == -INFINITY ? 0.f : 1.0f / t.y;
+        for (int d = lane * 2; d < hd; d += 64) {
+            float2 acc = make_float2(0.f, 0.f);
+            for (int c0 = c_lo; c0 <= c_hi; c0 += 8) {
+                float2 v[8];
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool in = c0 + e <= c_hi;
+                    w[e] = in ? ml[2 * (c0 + e)] : -INFINITY;
+                    v[e] = in ? *reinterpret_cast<const float2*>(po + (size_t)(c0 + e) * hd + d) : make_float2(0.f, 0.f);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (w[e] != -INFINITY) {
+                        const float f = kv4_exp2(w[e] - t.x);
+                        acc.x = fmaf(v[e].x, f, acc.x);
+                        acc.y = fmaf(v[e].y, f, acc.y);
+                    }
+            }
+            T* dst = (T*)p.out + (size_t)row * p.ldo + (size_t)h * hd + d;
+            dst[0] = from_f32<T>(acc.x * inv);
+            dst[1] = from_f32<T>(acc.y * inv);
+        }
+        return;
+    }
+    __shared__ float lse[64];                              // of 64 (row, head)s at a time
+    const int b = blockIdx.x - n_join, key = (b % mass_blocks) * 128 + threadIdx.x, kvh = b / mass_blocks % p.G, seg = b / mass_blocks / p.G;
+    const int n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg], pos0 = p.seg_pos[seg], R = p.H / p.G, n_cols = n_rows * R;
+    const int k0 = key - threadIdx.x;
+    if (n_rows > p.max_rows || k0 > pos0 + n_rows - 1 || (p.window > 0 && k0 + 127 <= pos0 - p.window)) return;
     // (in front of the first row's window nothing is read, and the pages may be somebody else's by now)
-    if (n_rows > p.max_rows || key > pos0 + n_rows - 1 || key >= p.max_blocks * p.ps || key >= p.ld_scores ||
-        (p.window > 0 && key <= pos0 - p.window)) return;
+    const bool there = key <= pos0 + n_rows - 1 && key < p.max_blocks * p.ps && key < p.ld_scores && !(p.window > 0 && key <= pos0 - p.window);
     float sum = 0.f;
-    for (int r = 0; r < n_rows; r++) {
-        const int hi = pos0 + r;
-        if (key > hi || (p.window > 0 && key <= hi - p.window)) continue;
-        for (int j = 0; j < R; j++) {
-            const size_t rh = ((size_t)seg * p.max_rows + r) * p.H + kvh * R + j;
-            sum += kv4_exp2(p.scores[rh * p.ld_scores + key] - p.lse_split[rh]);
+    for (int c0 = 0; c0 < n_cols; c0 += 64) {
+        __syncthreads();
+        for (int i = threadIdx.x >> 5; i < min(64, n_cols - c0); i += 4) {
+            const int r = (c0 + i) / R, h = kvh * R + (c0 + i) % R, hi = pos0 + r;
+            const size_t place = ((size_t)seg * p.max_rows + r) * p.H + h;
+            float v;
+            if (p.n_chunks == 1) {
+                v = p.lse_split[place];
+            } else {
+                const int c_lo = p.window > 0 ? max(0, hi - p.window + 1) / p.chunk : 0, c_hi = hi < 0 ? -1 : min(hi / p.chunk, p.n_chunks - 1);
+                const float2 t = kv4_total(p.part_ml + place * p.n_chunks * 2, c_lo, c_hi, lane);
+                v = t.x == -INFINITY ? INFINITY : t.x + log2f(t.y);
+            }
+            if (lane == 0) lse[i] = v;
+        }
+        __syncthreads();
+        if (there) {
+            const int n = min(64, n_cols - c0);
+            for (int i = 0; i < n; i++) {
+                const int r = (c0 + i) / R, hi = pos0 + r;
+                if (key > hi || (p.window > 0 && key <= hi - p.window)) continue;
+                const size_t place = ((size_t)seg * p.max_rows + r) * p.H + kvh * R + (c0 + i) % R;
+                sum += kv4_exp2(p.scores[place * p.ld_scores + key] - lse[i]);
+            }
         }
     }
-    const int page = p.block_table[(size_t)seg * p.max_blocks + key / p.ps];
-    p.mass[((size_t)page * p.G + kvh) * p.ps + key % p.ps] += sum;
+    if (there) {
+        const int page = p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)];
+        p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += sum;
+    }
 }
 
 // ---- tiled form: many rows a segment (portions of prompts).  A CTA takes 32 NT columns of a kv head (8 NT a warp) and walks
@@ -326,7 +438,7 @@ kv4_split_mass_kernel(const Kv4Args p) {
 template <int HD, int PARTS>
 struct Kv4Tiled {
     static constexpr int NT = PARTS == 1 ? (HD <= 64 ? 4 : (HD <= 128 ? 2 : 1)) : (HD <= 64 ? 2 : 1);
-    static constexpr int COLS = 32 * NT, TILE = 64, STAGE = 4 * Kv4<HD>::BLOCK;
+    static constexpr int COLS = 32 * NT, TILE = 64, STAGE = Kv4<HD>::bytes(64);
     static constexpr size_t SMEM = 2 * STAGE;
 };
 
@@ -362,8 +474,8 @@ kv4_tiled_kernel(const Kv4Args p) {
     using S = Kv4Tiled<HD, PARTS>;
     constexpr int NT = S::NT;
     kp_pdl_begin();
-    extern __shared__ __align__(16) unsigned char smem[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the warp's number in a uniform register)
     const int R = p.H / p.G, kvh = blockIdx.y;
     int seg, cta_col0 = 0;
     kv4_find_tile(p, blockIdx.x, S::COLS, R, lane, seg, cta_col0);
@@ -377,22 +489,24 @@ kv4_tiled_kernel(const Kv4Args p) {
     auto load = [&](int i) {                               // every warp a block of the tile
         const int key = (t_lo + i) * S::TILE + warp * 16;
         if (i < n_tiles && key <= k_hi && key + 15 >= k_lo) {
-            const int page = key / p.ps;
-            kv4_load_block<HD>(smem + (size_t)(i & 1) * S::STAGE + warp * F::BLOCK, p.pages + ((size_t)bt[page] * p.G + kvh) * rec, key - page * p.ps, p.ps, lane);
+            const int page = key >> p.ps_log2;
+            kv4_load_block<HD, S::TILE>(smem + (size_t)(i & 1) * S::STAGE, warp * 16, p.pages + ((size_t)bt[page] * p.G + kvh) * rec, key & (p.ps - 1), p.ps, lane);
         }
         cp_async_commit();
     };
     load(0);
     const int col0 = cta_col0 + warp * 8 * NT;
+    const Kv4Block<HD, S::TILE> B(lane);
     Kv4Cols<NT> C;
     kv4_columns<NT>(C, col0, n_cols, R, pos0, p.window, lane);
     Kv4Q<HD, PARTS, NT> Q;
+    const T* src[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const int c = col0 + nt * 8 + (lane >> 2);
-        const T* src = c < n_cols ? (const T*)p.q + (size_t)(row0 + c / R) * p.ldq + (size_t)(kvh * R + c % R) * HD : nullptr;
-        kv4_load_q<HD, PARTS, NT, CENTRE, T>(Q, nt, src, p.scale, lane);
+        src[nt] = c < n_cols ? (const T*)p.q + (size_t)(row0 + c / R) * p.ldq + (size_t)(kvh * R + c % R) * HD : nullptr;
     }
+    kv4_load_q<HD, PARTS, NT, CENTRE, T>(Q, src, p.scale, lane);
     float* sc[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) sc[nt][0] = sc[nt][1] = nullptr;
@@ -412,9 +526,9 @@ kv4_tiled_kernel(const Kv4Args p) {
             const int key0 = (t_lo + i) * S::TILE + b * 16;
             if (col1 < col0 || key0 > w_hi || key0 + 15 < w_lo) continue;
             if (key0 >= max(k_lo, safe_lo) && key0 + 15 <= safe_hi && col0 + 8 * NT <= n_cols)
-                kv4_tile<HD, PARTS, NT, 1, CENTRE, false, false>(A, Q, tile + b * F::BLOCK, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+                kv4_tile<HD, S::TILE, PARTS, NT, 1, CENTRE, false, false>(A, Q, B, tile, b * 16, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
             else
-                kv4_tile<HD, PARTS, NT, 1, CENTRE, true, false>(A, Q, tile + b * F::BLOCK, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
+                kv4_tile<HD, S::TILE, PARTS, NT, 1, CENTRE, true, false>(A, Q, B, tile, b * 16, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
         }
         __syncthreads();                                   // the next tile but one takes this one's place
     }
@@ -452,9 +566,9 @@ kv4_mass_kernel(const Kv4Args p) {
     using F = Kv4<HD>;
     constexpr int NB = HD <= 128 ? 4 : 2, KEYS = NB * 16;
     kp_pdl_begin();
-    __shared__ __align__(16) unsigned char smem[NB * F::BLOCK];
+    __shared__ __align__(128) unsigned char smem[F::bytes(KEYS)];
     __shared__ float part[4][KEYS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the warp's number in a uniform register)
     const int seg = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x * KEYS, R = p.H / p.G;
     const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg];
     // keys that any row reads (in front of them the pages may be somebody else's by now)
@@ -467,8 +581,8 @@ kv4_mass_kernel(const Kv4Args p) {
     for (int b = warp; b < NB; b += 4) {
         const int key = k0 + b * 16;
         if (key <= last && key + 15 >= first) {
-            const int page = key / p.ps;
-            kv4_load_block<HD>(smem + b * F::BLOCK, p.pages + ((size_t)bt[page] * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key - page * p.ps, p.ps, lane);
+            const int page = key >> p.ps_log2;
+            kv4_load_block<HD, KEYS>(smem, b * 16, p.pages + ((size_t)bt[page] * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key & (p.ps - 1), p.ps, lane);
         }
     }
     cp_async_commit();
@@ -477,13 +591,14 @@ kv4_mass_kernel(const Kv4Args p) {
     float sum[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; b++) sum[b][0] = sum[b][1] = 0.f;
-    const int c_end = (r_hi + 1) * R, key = kv4_key_of(lane >> 2);
+    const Kv4Block<HD, KEYS> B(lane);
+    const int c_end = (r_hi + 1) * R, key = F::key_of(lane >> 2);
 #pragma unroll 1
     for (int col0 = r_lo * R + warp * 8; col0 < c_end; col0 += 32) {
         Kv4Q<HD, PARTS, 1> Q;
         const int cq = col0 + (lane >> 2);
-        kv4_load_q<HD, PARTS, 1, true, T>(Q, 0, cq < c_end ? (const T*)p.q + (size_t)(row0 + cq / R) * p.ldq + (size_t)(kvh * R + cq % R) * HD : nullptr,
-                                    p.scale, lane);
+        const T* const src[1] = {cq < c_end ? (const T*)p.q + (size_t)(row0 + cq / R) * p.ldq + (size_t)(kvh * R + cq % R) * HD : nullptr};
+        kv4_load_q<HD, PARTS, 1, true, T>(Q, src, p.scale, lane);
         float lse[2];
         int hi[2];
 #pragma unroll
@@ -495,7 +610,7 @@ kv4_mass_kernel(const Kv4Args p) {
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             float s[1][4];
-            kv4_scores<HD, PARTS, 1, true>(s, smem + b * F::BLOCK, Q, lane);
+            kv4_scores<HD, KEYS, PARTS, 1, true>(s, smem, b * 16, B, Q);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int k = k0 + b * 16 + key + (e >> 1) * 8, h = hi[e & 1];
@@ -516,8 +631,8 @@ kv4_mass_kernel(const Kv4Args p) {
     __syncthreads();
     const int k = threadIdx.x;
     if (k < KEYS && k0 + k <= last && k0 + k >= first) {
-        const int page = bt[(k0 + k) / p.ps];
-        p.mass[((size_t)page * p.G + kvh) * p.ps + (k0 + k) % p.ps] += (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
+        const int page = bt[(k0 + k) >> p.ps_log2];
+        p.mass[((size_t)page * p.G + kvh) * p.ps + ((k0 + k) & (p.ps - 1))] += (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
     }
 }
 
@@ -533,6 +648,18 @@ kv4_mass_kernel(const Kv4Args p) {
         default: return KP_ERR_UNSUPPORTED;                            \
     }
 
+static int kv4_log2(int v) { int l = 0; while ((1 << l) < v) l++; return l; }
+
+// CTAs of the writing and reading kernels with one row a thread, and with four
+#define KV4_ONE_ROW (148 * 8)                              // more CTAs than that are more than fit at once: four rows a thread
+static int kv4_row_blocks(const Kv4Rows& p, unsigned (&blocks)[2]) {
+    const long long per_row = 2LL * p.G * p.hd / 8;
+    if (p.n * per_row >= (1LL << 32) - 256) return KP_ERR_UNSUPPORTED;
+    blocks[0] = (unsigned)((p.n * per_row + 255) / 256);
+    blocks[1] = (unsigned)(((p.n + 3) / 4 * per_row + 255) / 256);
+    return 0;
+}
+
 template <typename Kern>
 static int kv4_launch(Kern kern, dim3 grid, size_t smem, std::atomic<unsigned long long>& ready, cudaStream_t st, const Kv4Args& a) {
     if (smem > 48 * 1024) {
@@ -543,22 +670,47 @@ static int kv4_launch(Kern kern, dim3 grid, size_t smem, std::atomic<unsigned lo
     return e ? (int)e : kp_launch_status();
 }
 
+// The pages' codes as the TMA sees them: one record a (page, kv head), rows of codes (keys', then values').  A box has the keys of one page that lie
+// in one tile.
+template <int HD>
+static int kv4_codes_map(CUtensorMap* codes, const Kv4Args& a, long long n_pages, int tile) {
+    using F = Kv4<HD>;
+    const KpEncodeTiledFn fn = kp_encode_tiled_fn();
+    const cuuint64_t records = (cuuint64_t)n_pages * a.G, bytes = (cuuint64_t)kv4_page_bytes(a.ps, HD);
+    if (!fn || n_pages < 1 || records > 2147483647ull) return KP_ERR_UNSUPPORTED;
+    const cuuint32_t one[3] = {1, 1, 1}, box[3] = {F::ROW, (cuuint32_t)(a.ps < tile ? a.ps : tile), 1};
+    const cuuint64_t dims[3] = {F::ROW, 2ull * a.ps, records}, strides[2] = {F::ROW, bytes};
+    const CUresult r = fn(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<unsigned char*>(a.pages), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          F::ROW == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : (F::ROW == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE),
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : KP_ERR_UNSUPPORTED;
+}
+
+template <int HD, int PARTS, bool KEEP, typename T>
+static int kv4_run_split(const Kv4Args& a, long long n_pages, cudaStream_t st) {
+    using S = Kv4Split<HD, PARTS>;
+    static std::atomic<unsigned long long> ready{0};
+    alignas(64) CUtensorMap codes;
+    int e = kv4_codes_map<HD>(&codes, a, n_pages, S::KEYS);
+    if (e) return e;
+    if ((e = kp_smem_limit(kv4_split_kernel<HD, PARTS, KEEP, T>, S::SMEM, ready))) return e;
+    const cudaError_t c = kp_launch_pdl(kv4_split_kernel<HD, PARTS, KEEP, T>, dim3(a.n_chunks, a.G * ((a.max_rows * (a.H / a.G) + 7) / 8), a.n_seg), dim3(128),
+                                        S::SMEM, st, codes, a);
+    return c ? (int)c : kp_launch_status();
+}
+
 template <int HD, int PARTS, typename T>
-static int kv4_run(const Kv4Args& a, int n_rows, int long_tiles, int long_keys, cudaStream_t st) {
+static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_tiles, int long_keys, cudaStream_t st) {
     const int R = a.H / a.G;
     if (a.max_rows > 0) {
-        using S = Kv4Split<HD, PARTS>;
-        static std::atomic<unsigned long long> ready{0}, ready_keep{0};
-        const dim3 grid(a.n_chunks, a.G * ((a.max_rows * R + 7) / 8), a.n_seg);
-        const int e = a.mass ? kv4_launch(kv4_split_kernel<HD, PARTS, true, T>, grid, S::SMEM, ready_keep, st, a)
-                             : kv4_launch(kv4_split_kernel<HD, PARTS, false, T>, grid, S::SMEM, ready, st, a);
+        const int e = a.mass ? kv4_run_split<HD, PARTS, true, T>(a, n_pages, st) : kv4_run_split<HD, PARTS, false, T>(a, n_pages, st);
         if (e) return e;
-        if (a.n_chunks > 1) {
-            const cudaError_t c = kp_launch_pdl(kv4_merge_kernel<T>, dim3(a.n_seg * a.max_rows, a.H), dim3(128), 0, st, a, HD);
-            if (c) return (int)c;
-        }
-        if (a.mass) {
-            const cudaError_t c = kp_launch_pdl(kv4_split_mass_kernel, dim3((a.n_chunks * a.chunk + 127) / 128, a.G, a.n_seg), dim3(128), 0, st, a);
+        if (a.n_chunks > 1 || a.mass) {
+            const long long join = a.n_chunks > 1 ? ((long long)a.n_seg * a.max_rows * a.H + 3) / 4 : 0;
+            const int mass_blocks = a.mass ? (a.n_chunks * a.chunk + 127) / 128 : 0;
+            const long long blocks = join + (long long)mass_blocks * a.G * a.n_seg;
+            if (blocks > 2147483647LL) return KP_ERR_UNSUPPORTED;
+            const cudaError_t c = kp_launch_pdl(kv4_join_kernel<T>, dim3((unsigned)blocks), dim3(128), 0, st, a, HD, (int)join, mass_blocks);
             if (c) return (int)c;
         }
     }
@@ -584,56 +736,60 @@ extern "C" {
 int kp_kv4_write(const void* k, long long ldk, const void* v, long long ldv, void* pages, long long n_pages, const int* slot_map, int n, int ps,
                  int G, int hd, int dtype, void* stream) {
     if (n <= 0) return 0;
-    if (hd < 32 || hd % 32 || ps < 16 || ps % 16 || G < 1 || ((uintptr_t)pages & 15)) return KP_ERR_BAD_ARG;
-    const int gs = hd % 64 == 0 ? 64 : 32;
-    const long long blocks = (2LL * n * G * (hd / 8) + 255) / 256;
-    if (blocks > 2147483647LL) return KP_ERR_UNSUPPORTED;
+    if (hd < 32 || hd % 32 || ps < 16 || (ps & (ps - 1)) || G < 1 || ((uintptr_t)pages & 15)) return KP_ERR_BAD_ARG;
+    const Kv4Rows p = {n, kv4_log2(ps), G, hd, hd % 64 == 0 ? 64 : 32, n_pages * ps};
+    unsigned blocks[2];
+    const int e = kv4_row_blocks(p, blocks);
+    if (e) return e;
+    const bool many = blocks[0] > KV4_ONE_ROW;
     KP_DISPATCH_DTYPE(dtype, T, {
         const long long a = 16 / sizeof(T);
         const bool vec = !(((uintptr_t)k | (uintptr_t)v) & 15) && ldk % a == 0 && ldv % a == 0;
-        cudaError_t e = vec ? kp_launch_pdl(kv4_write_kernel<T, true>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const T*)k, ldk,
-                                            (const T*)v, ldv, (unsigned char*)pages, slot_map, n_pages * ps, n, ps, G, hd, gs)
-                            : kp_launch_pdl(kv4_write_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const T*)k, ldk,
-                                            (const T*)v, ldv, (unsigned char*)pages, slot_map, n_pages * ps, n, ps, G, hd, gs);
-        if (e) return (int)e;
+        auto kern = vec ? (many ? kv4_write_kernel<T, true, 4> : kv4_write_kernel<T, true, 1>) : (many ? kv4_write_kernel<T, false, 4> : kv4_write_kernel<T, false, 1>);
+        const cudaError_t c = kp_launch_pdl(kern, dim3(blocks[many]), dim3(256), 0, (cudaStream_t)stream, (const T*)k, ldk, (const T*)v, ldv,
+                                            (unsigned char*)pages, slot_map, p);
+        if (c) return (int)c;
     });
     return kp_launch_status();
 }
 
 int kp_kv4_read(const void* pages, long long n_pages, const int* slot_map, void* k, void* v, int n, int ps, int G, int hd, int dtype, void* stream) {
     if (n <= 0) return 0;
-    if (hd < 32 || hd % 32 || ps < 16 || ps % 16 || G < 1 || (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15)) return KP_ERR_BAD_ARG;
-    const long long blocks = (2LL * n * G * (hd / 8) + 255) / 256;
-    if (blocks > 2147483647LL) return KP_ERR_UNSUPPORTED;
+    if (hd < 32 || hd % 32 || ps < 16 || (ps & (ps - 1)) || G < 1 || (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15)) return KP_ERR_BAD_ARG;
+    const Kv4Rows p = {n, kv4_log2(ps), G, hd, hd % 64 == 0 ? 64 : 32, n_pages * ps};
+    unsigned blocks[2];
+    const int e = kv4_row_blocks(p, blocks);
+    if (e) return e;
+    const bool many = blocks[0] > KV4_ONE_ROW;
     KP_DISPATCH_DTYPE(dtype, T, {
-        const cudaError_t e = kp_launch_pdl(kv4_read_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, (const unsigned char*)pages,
-                                            slot_map, n_pages * ps, (T*)k, (T*)v, n, ps, G, hd, hd % 64 == 0 ? 64 : 32);
-        if (e) return (int)e;
+        const cudaError_t c = kp_launch_pdl(many ? kv4_read_kernel<T, 4> : kv4_read_kernel<T, 1>, dim3(blocks[many]), dim3(256), 0, (cudaStream_t)stream,
+                                            (const unsigned char*)pages, slot_map, (T*)k, (T*)v, p);
+        if (c) return (int)c;
     });
     return kp_launch_status();
 }
 
 // Segments of at most `short_rows` rows go to the split form (0: none), the others to the tiled form if `long_rows` is not 0.
 // Scratch: see Kv4Args; lse_split and scores where there is mass and a split form, lse where there is mass and a tiled one.
-int kp_kv4_attention(const void* q, long long ldq, const void* pages, const int* block_table, int max_blocks, const int* cu_rows, const int* seg_pos,
+int kp_kv4_attention(const void* q, long long ldq, const void* pages, long long n_pages, const int* block_table, int max_blocks, const int* cu_rows, const int* seg_pos,
                      int n_seg, void* out, long long ldo, float scale, int window, int ps, int H, int G, int hd, int n_rows, int short_rows,
                      int long_rows, int n_chunks, int chunk, int max_context, float* part_o, float* part_ml, float* scores, int ld_scores,
                      float* lse_split, float* lse, float* mass, int dtype, void* stream) {
     if (n_rows <= 0 || n_seg <= 0) return 0;
-    if (G < 1 || H < 1 || H % G || ps < 16 || ps % 16 || window < 0 || n_chunks < 1 || chunk < 64 || chunk % 64 || n_seg > 65535 || H > 65535 ||
+    if (G < 1 || H < 1 || H % G || ps < 16 || (ps & (ps - 1)) || window < 0 || n_chunks < 1 || chunk < 64 || chunk % 64 || n_seg > 65535 || H > 65535 ||
         ((uintptr_t)pages & 15) || (mass && ((long_rows && !lse) || (short_rows > 0 && (!scores || !lse_split)))) || (n_chunks > 1 && short_rows > 0 && (!part_o || !part_ml)))
         return KP_ERR_BAD_ARG;
     Kv4Args a = {};
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.pages = (const unsigned char*)pages;
     a.block_table = block_table; a.max_blocks = max_blocks; a.cu_rows = cu_rows; a.seg_pos = seg_pos;
-    a.scale = scale; a.window = window; a.ps = ps; a.H = H; a.G = G;
+    a.scale = scale; a.window = window; a.ps = ps; a.ps_log2 = kv4_log2(ps); a.H = H; a.G = G;
     a.part_o = part_o; a.part_ml = part_ml; a.scores = mass ? scores : nullptr; a.ld_scores = ld_scores;
     a.lse_split = mass ? lse_split : nullptr; a.lse = mass ? lse : nullptr; a.mass = mass;
     a.n_chunks = n_chunks; a.chunk = chunk; a.max_rows = short_rows; a.min_rows = short_rows + 1; a.n_seg = n_seg;
     if (dtype == KP_DTYPE_BF16) {
-        KV4_DISPATCH_HD(hd, HD, return (kv4_run<HD, 1, bf16>(a, n_rows, long_rows, max_context, (cudaStream_t)stream)));
+        KV4_DISPATCH_HD(hd, HD, return (kv4_run<HD, 1, bf16>(a, n_pages, n_rows, long_rows, max_context, (cudaStream_t)stream)));
     } else if (dtype == KP_DTYPE_F32) {
-        KV4_DISPATCH_HD(hd, HD, return (kv4_run<HD, 2, float>(a, n_rows, long_rows, max_context, (cudaStream_t)stream)));
+        KV4_DISPATCH_HD(hd, HD, return (kv4_run<HD, 2, float>(a, n_pages, n_rows, long_rows, max_context, (cudaStream_t)stream)));
     }
     return KP_ERR_BAD_ARG;
 }

@@ -1,6 +1,6 @@
 // A cache of keys and values held in 4 bits: its bytes, and the warp-level attention over it that the kernels share.
 //
-// A page holds, for every kv head, one record of bytes about its `ps` keys (ps a multiple of 16):
+// A page holds, for every kv head, one record of bytes about its `ps` keys (ps a power of two, at least 16):
 //     key codes [ps][HD/2] | value codes [ps][HD/2] | key ranges [ps][NG] | value ranges [ps][NG]
 // A row of HD values is cut into NG groups of GS = 64 values (32 where 64 does not divide HD).  A group has a scale s and
 // a minimum z, both bfloat16 (a range in the low and the high half of 4 bytes), and 4-bit codes c (value 2i of the row in
@@ -11,11 +11,12 @@
 // The arithmetic.  With q the query and k = s c + z,   q.k = sum over groups  s (q.c) + z (sum of q),
 // so the codes themselves enter the matrix instructions and a scale is one multiplication a (key, group), not one a value.
 // A code is an fp16 operand without any arithmetic: the bits 0000 0000 0000 cccc are the subnormal c 2^-24, and
-// 0000 0000 cccc 0000 are c 2^-20, so eight codes of a word need four ANDs and one shift.  Queries enter as fp16 too, each
-// scaled by a power of two of its own that brings its largest value to [2^14, 2^15): a bfloat16 query loses nothing that
-// is above 2^-38 of its largest value.  float32 queries enter as two fp16 parts (22 bits).  The softmax weights p are
+// 0000 0000 cccc 0000 are c 2^-20, so eight codes of a word need four ANDs and one shift.  Queries enter as fp16 too,
+// scaled by a power of two that brings the largest value of the warp's queries to [2^14, 2^15): a bfloat16 query loses nothing
+// that is above 2^-38 of that value.  float32 queries enter as two fp16 parts (22 bits).  The softmax weights p are
 // multiplied with the values' scales and enter as fp16 (as two parts in the float32 form), with the running maximum in
-// units that hold p s at or below 2^15: fp16's whole range, 39 binary orders, lies below the largest weight of a row.
+// units that hold p s at or below 2^15 (it follows the maxima in steps of 2^8 and more): at least 31 binary orders of fp16 lie
+// below the largest weight of a row.
 // Scores, maxima, sums and accumulators are float32.
 //
 // Keys are the rows of the score product (m16n8k16: 16 keys x 8 queries), so that no row of the instruction is wasted where
@@ -36,20 +37,23 @@ struct Kv4 {
     static constexpr int PP = ROW / 16;                     // 16-byte pieces of it
     static constexpr int KS = GS / 16;                      // steps of 16 values in a group
     static constexpr int MT = GS / 16;                      // tiles of 16 dimensions in a group
-    // a block of 16 keys in shared memory: the four parts of the record, one behind the other
-    static constexpr int V_OFF = 16 * ROW, KR_OFF = 32 * ROW, VR_OFF = KR_OFF + 64 * NG, BLOCK = VR_OFF + 64 * NG;
-    // where a 16-byte piece of a key's row lies: rows whose length is a power of two have their pieces turned, so that the
-    // rows read together do not meet in the same banks
-    static __device__ __forceinline__ int piece(int key, int p) {
-        if (PP == 4) return key * 4 + (p ^ (((key >> 1) & 1) << 1));
-        if (PP == 8) return key * 8 + (p ^ ((key & 3) << 1));
-        return key * PP + p;
-    }
+    // A tile of KEYS keys in shared memory: rows of key codes, rows of value codes, key ranges, value ranges.  Rows of 64 and 128 bytes
+    // lie as the TMA's 64- and 128-byte swizzles put them (the tile on such a boundary), others as they are.
+    static constexpr int bytes(int keys) { return keys * (HD + 8 * NG); }
+    static __device__ __forceinline__ int turn(int key) { return PP == 4 ? (key >> 1) & 3 : (PP == 8 ? key & 7 : 0); }
+    // Which of a block's 8 keys stands in row (or slot) g of the products' operands: in these orders neither the key words (rows
+    // 0..3, rows 4..7) nor the value words (slots 0, 2, 4, 6, slots 1, 3, 5, 7) meet in a bank.
+    static __device__ __forceinline__ int key_of(int g) { return (PP == 4 ? 0x32547160 : (PP == 8 ? 0x57136420 : 0x53427160)) >> (4 * g) & 7; }
 };
 __host__ __device__ constexpr long long kv4_page_bytes(int page_size, int hd) {
     return (long long)page_size * (hd + 8 * (hd / (hd % 64 == 0 ? 64 : 32)));
 }
 
+__device__ __forceinline__ float kv4_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float kv4_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -79,97 +83,154 @@ __device__ __forceinline__ uint32_t pack_f16_part(float& a, float& b) {
 __device__ __forceinline__ float kv4_scale(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float kv4_least(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
 
-// The key of a block's half that stands in row (or slot) g of the products' operands: with this order neither the key words
-// (rows 0..3 and 4..7 together) nor the value words (slots 0, 2, 4, 6, then 1, 3, 5, 7) meet in a bank.
-__device__ __forceinline__ int kv4_key_of(int g) { return (g & 1) ? 4 + (((g >> 1) + 2) & 3) : g >> 1; }
-
-// ---- a block of 16 keys from its page's record to shared memory, by one warp (`rec`: record of (page, kv head), `off`: the
-// block's first key in the page)
-template <int HD>
-__device__ __forceinline__ void kv4_load_block(unsigned char* dst, const unsigned char* __restrict__ rec, int off, int ps, int lane) {
+// ---- a block of 16 keys from its page's record to shared memory by a warp's cp.async: row `at` of a tile of KEYS keys (`rec`:
+// record of (page, kv head), `off`: the block's first key in the page)
+template <int HD, int KEYS>
+__device__ __forceinline__ void kv4_load_block(unsigned char* tile, int at, const unsigned char* __restrict__ rec, int off, int ps, int lane) {
     using F = Kv4<HD>;
     const unsigned char* kc = rec + (size_t)off * F::ROW;
     const unsigned char* vc = kc + (size_t)ps * F::ROW;
     const unsigned char* kr = rec + (size_t)ps * HD + (size_t)off * 4 * F::NG;
     const unsigned char* vr = kr + (size_t)ps * 4 * F::NG;
     constexpr int N = F::ROW;                              // 16-byte pieces of 16 rows of codes
+    unsigned char* dst = tile + at * F::ROW;
 #pragma unroll
     for (int i = 0; i < (N + 31) / 32; i++) {
         const int j = i * 32 + lane;
         if (N % 32 == 0 || j < N) {
-            const int at = F::piece(j / F::PP, j % F::PP) * 16;
-            cp_async16(dst + at, kc + j * 16, true);
-            cp_async16(dst + F::V_OFF + at, vc + j * 16, true);
+            const int to = j / F::PP * F::ROW + ((j % F::PP) ^ F::turn(j / F::PP)) * 16;
+            cp_async16(dst + to, kc + j * 16, true);
+            cp_async16(dst + KEYS * F::ROW + to, vc + j * 16, true);
         }
     }
     static_assert(8 * F::NG <= 32, "the ranges of a block are at most a piece a lane");
-    if (lane < 4 * F::NG) cp_async16(dst + F::KR_OFF + lane * 16, kr + lane * 16, true);
-    else if (lane < 8 * F::NG) cp_async16(dst + F::VR_OFF + (lane - 4 * F::NG) * 16, vr + (lane - 4 * F::NG) * 16, true);
+    unsigned char* r = tile + KEYS * HD + at * 4 * F::NG;
+    if (lane < 4 * F::NG) cp_async16(r + lane * 16, kr + lane * 16, true);
+    else if (lane < 8 * F::NG) cp_async16(r + KEYS * 4 * F::NG + (lane - 4 * F::NG) * 16, vr + (lane - 4 * F::NG) * 16, true);
 }
+// Where a lane finds its part of a block of 16 keys of a tile of KEYS keys (the tile on a 128-byte boundary): offsets from the tile, for
+// its first block.
+template <int HD, int KEYS>
+struct Kv4Block {
+    int k, va, vb, r;                                      // its key words, its value words of slots 2t and 2t + 1, its key's ranges
+    __device__ __forceinline__ explicit Kv4Block(int lane) {
+        using F = Kv4<HD>;
+        const int g = lane >> 2, t = lane & 3, key = F::key_of(g), ka = F::key_of(2 * t), kb = F::key_of(2 * t + 1);
+        const int v = KEYS * F::ROW;
+        if (F::GS == 64) {
+            k = key * F::ROW + ((t >> 1) ^ F::turn(key)) * 16 + (t & 1) * 8;
+            va = v + ka * F::ROW + ((g >> 2) ^ F::turn(ka)) * 16 + (g & 3) * 4;
+            vb = v + kb * F::ROW + ((g >> 2) ^ F::turn(kb)) * 16 + (g & 3) * 4;
+        } else {
+            k = key * F::ROW + t * 4;
+            va = v + ka * F::ROW + g * 2;
+            vb = v + kb * F::ROW + g * 2;
+        }
+        r = KEYS * HD + key * 4 * F::NG;
+    }
+    // an offset of group 0, moved to group y (in rows whose pieces are turned the group's bits of the piece's number are exchanged)
+    static __device__ __forceinline__ int group(int off, int y) {
+        using F = Kv4<HD>;
+        return F::PP == 4 || F::PP == 8 ? off ^ (y * 32) : off + y * (F::GS / 2);
+    }
+};
+
+template <typename W>
+__device__ __forceinline__ W kv4_at(const unsigned char* p) { return *reinterpret_cast<const W*>(p); }
 
 // ---- queries of a warp: 8 NT columns as B operands of the score product
 template <int HD, int PARTS, int NT>
 struct Kv4Q {
     uint32_t b[NT][PARTS][HD / 16][2];
-    // for this thread's queries 2t and 2t + 1: the factors of s (q.(c - 8)) and of z + 8 s, and what the product starts from
-    // (- 8 times the sum of q in the codes' unit; 0 where the operand is c - 8 itself)
-    float fs[NT][2], fz[NT][Kv4<HD>::NG][2], init[NT][Kv4<HD>::NG][2];
+    float fs;                                              // factor of s (q.c), the same for all columns
+    float fz[NT][Kv4<HD>::NG][2];                          // factor of z for this thread's queries 2t and 2t + 1
 };
 
-// Loads column n-tile `nt`: `src` is the query of column lane / 4 (null: none).
+// Loads the warp's columns: src[nt] is the query of column 8 nt + lane / 4 (null: none).
+// N consecutive values, 16 bytes at a time where they lie so
+template <int N>
+__device__ __forceinline__ void kv4_values(float (&v)[N], const bf16* p) {
+    if (((uintptr_t)p & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 8; i++) {
+            const uint4 x = reinterpret_cast<const uint4*>(p)[i];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) { v[8 * i + 2 * j] = kv4_scale(w[j]); v[8 * i + 2 * j + 1] = kv4_least(w[j]); }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = to_f32(p[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void kv4_values(float (&v)[N], const float* p) {
+    if (((uintptr_t)p & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const float4 x = reinterpret_cast<const float4*>(p)[i];
+            v[4 * i] = x.x; v[4 * i + 1] = x.y; v[4 * i + 2] = x.z; v[4 * i + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = p[i];
+    }
+}
 template <int HD, int PARTS, int NT, bool CENTRE, typename T>
-__device__ __forceinline__ void kv4_load_q(Kv4Q<HD, PARTS, NT>& Q, int nt, const T* src, float scale, int lane) {
+__device__ __forceinline__ void kv4_load_q(Kv4Q<HD, PARTS, NT>& Q, const T* const (&src)[NT], float scale, int lane) {
     using F = Kv4<HD>;
     const int t = lane & 3;
     constexpr int W = F::GS / 4;                           // values of a group that a lane holds: 16 or 8 consecutive ones
-    float v[F::NG][W];
+    // One power of two for all the columns brings their largest value to [2^14, 2^15): what fp16 cannot hold of a smaller column is
+    // below 2^-39 of that value.  A column that is not finite has no say.
     float top = 0.f;
 #pragma unroll
-    for (int y = 0; y < F::NG; y++)
+    for (int nt = 0; nt < NT; nt++) {
+        float mine = 0.f;
+        if (src[nt]) {
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            v[y][i] = src ? to_f32(src[y * F::GS + t * W + i]) : 0.f;
-            top = fmaxf(top, fabsf(v[y][i]));
-        }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^e brings the largest value to [2^14, 2^15); a query of zeros, or one that is not finite, stays as it is
-    int e = 0;
-    if (top > 0.f && top < INFINITY) e = min(14 - ilogbf(top), 100);
-    const float up = ldexpf(1.0f, e);
-    float sum[F::NG];
+            for (int y = 0; y < F::NG; y++) {
+                float v[W];
+                kv4_values<W>(v, src[nt] + y * F::GS + t * W);
 #pragma unroll
-    for (int y = 0; y < F::NG; y++) {
-        sum[y] = 0.f;
-#pragma unroll
-        for (int k = 0; k < F::KS; k++) {                  // step k: values (0, 4), (1, 5) of a word, then (2, 6), (3, 7), then the next word
-            const int d = (k >> 1) * 8 + (k & 1) * 2;
-            float x[4] = {v[y][d] * up, v[y][d + 4] * up, v[y][d + 1] * up * 0.0625f, v[y][d + 5] * up * 0.0625f};
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) {
-                const float w0 = x[0], w1 = x[1], w2 = x[2], w3 = x[3];
-                Q.b[nt][p][y * F::KS + k][0] = pack_f16_part(x[0], x[1]);
-                Q.b[nt][p][y * F::KS + k][1] = pack_f16_part(x[2], x[3]);
-                // (an infinite value leaves NaN behind: the sum must not see more than what the operand holds)
-                sum[y] += ((w0 - x[0]) + (w1 - x[1])) + 16.0f * ((w2 - x[2]) + (w3 - x[3]));
+                for (int i = 0; i < W; i++) mine = fmaxf(mine, fabsf(v[i]));
             }
         }
-        sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
-        sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
+        top = mine < INFINITY ? fmaxf(top, mine) : top;
     }
-    const float f = ldexpf(scale * KV4_LOG2E, -e);
+    top = warp_max(top);
+    const int e = top > 0.f ? min(14 - ilogbf(top), 100) : 0;
+    const float up = ldexpf(1.0f, e), f = ldexpf(scale * KV4_LOG2E, -e);
+    Q.fs = CENTRE ? f : f * 16777216.0f;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int from = (2 * t + i) * 4;                  // a lane whose column this is
-        const float fi = __shfl_sync(0xffffffffu, f, from);
-        Q.fs[nt][i] = CENTRE ? fi : fi * 16777216.0f;
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int y = 0; y < F::NG; y++) {
-            const float qs = __shfl_sync(0xffffffffu, sum[y], from);
-            Q.fz[nt][y][i] = fi * qs;
-            Q.init[nt][y][i] = CENTRE ? 0.f : qs * (-8.0f / 16777216.0f);
+            float v[W], sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; i++) v[i] = 0.f;
+            if (src[nt]) kv4_values<W>(v, src[nt] + y * F::GS + t * W);
+#pragma unroll
+            for (int i = 0; i < W; i++) v[i] *= up;
+#pragma unroll
+            for (int k = 0; k < F::KS; k++) {              // step k: values (0, 4), (1, 5) of a word, then (2, 6), (3, 7), then the next word
+                const int d = (k >> 1) * 8 + (k & 1) * 2;
+                float x[4] = {v[d], v[d + 4], v[d + 1] * 0.0625f, v[d + 5] * 0.0625f};
+#pragma unroll
+                for (int p = 0; p < PARTS; p++) {
+                    const float w0 = x[0], w1 = x[1], w2 = x[2], w3 = x[3];
+                    Q.b[nt][p][y * F::KS + k][0] = pack_f16_part(x[0], x[1]);
+                    Q.b[nt][p][y * F::KS + k][1] = pack_f16_part(x[2], x[3]);
+                    sum += ((w0 - x[0]) + (w1 - x[1])) + 16.0f * ((w2 - x[2]) + (w3 - x[3]));      // of what the operand holds
+                }
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                Q.fz[nt][y][i] = f * __shfl_sync(0xffffffffu, sum, (2 * t + i) * 4);                // (from a lane whose column this is)
+            }
         }
-    }
 }
 
 // Two codes as an fp16 operand: as they are (CENTRE: about their middle, c - 8, exactly; what the sums of s c and of z have in
@@ -186,18 +247,18 @@ __device__ __forceinline__ uint32_t kv4_code(uint32_t w) {
 }
 
 // the A operand of the score product: codes of group y of the keys in rows g and g + 8
-template <int HD, bool CENTRE>
-__device__ __forceinline__ void kv4_key_operand(uint32_t (&a)[Kv4<HD>::KS][4], const unsigned char* blk, int y, int lane) {
+template <int HD, int KEYS, bool CENTRE>
+__device__ __forceinline__ void kv4_key_operand(uint32_t (&a)[Kv4<HD>::KS][4], const unsigned char* tile, int at, const Kv4Block<HD, KEYS>& B, int y) {
     using F = Kv4<HD>;
-    const int key = kv4_key_of(lane >> 2), t = lane & 3;
+    const unsigned char* p = tile + B.group(B.k, y) + at * F::ROW;
     uint32_t w[2][F::GS / 32];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         if (F::GS == 64) {
-            const uint2 x = *reinterpret_cast<const uint2*>(blk + F::piece(key + 8 * h, 2 * y + (t >> 1)) * 16 + (t & 1) * 8);
+            const uint2 x = kv4_at<uint2>(p + 8 * h * F::ROW);
             w[h][0] = x.x; w[h][F::GS / 32 - 1] = x.y;
         } else {
-            w[h][0] = *reinterpret_cast<const uint32_t*>(blk + F::piece(key + 8 * h, y) * 16 + t * 4);
+            w[h][0] = kv4_at<uint32_t>(p + 8 * h * F::ROW);
         }
     }
 #pragma unroll
@@ -211,33 +272,38 @@ __device__ __forceinline__ void kv4_key_operand(uint32_t (&a)[Kv4<HD>::KS][4], c
 }
 
 // Scores of a block's 16 keys, times scale and log2 e: s[nt][0, 1] of the key in row g and queries 2t, 2t + 1, s[nt][2, 3] of row g + 8.
-template <int HD, int PARTS, int NT, bool CENTRE>
-__device__ __forceinline__ void kv4_scores(float (&s)[NT][4], const unsigned char* blk, const Kv4Q<HD, PARTS, NT>& Q, int lane) {
+template <int HD, int KEYS, int PARTS, int NT, bool CENTRE>
+__device__ __forceinline__ void kv4_scores(float (&s)[NT][4], const unsigned char* tile, int at, const Kv4Block<HD, KEYS>& B,
+                                           const Kv4Q<HD, PARTS, NT>& Q) {
     using F = Kv4<HD>;
-    const int key = kv4_key_of(lane >> 2);
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) s[nt][i] = 0.f;
 #pragma unroll
     for (int y = 0; y < F::NG; y++) {
         uint32_t a[F::KS][4];
-        kv4_key_operand<HD, CENTRE>(a, blk, y, lane);
-        const uint32_t r0 = *reinterpret_cast<const uint32_t*>(blk + F::KR_OFF + (key * F::NG + y) * 4);
-        const uint32_t r1 = *reinterpret_cast<const uint32_t*>(blk + F::KR_OFF + ((key + 8) * F::NG + y) * 4);
-        const float s0 = kv4_scale(r0), z0 = fmaf(8.0f, s0, kv4_least(r0)), s1 = kv4_scale(r1), z1 = fmaf(8.0f, s1, kv4_least(r1));
+        kv4_key_operand<HD, KEYS, CENTRE>(a, tile, at, B, y);
+        const unsigned char* r = tile + B.r + at * 4 * F::NG + y * 4;
+        const uint32_t r0 = kv4_at<uint32_t>(r), r1 = kv4_at<uint32_t>(r + 32 * F::NG);
+        float z0 = kv4_least(r0), s0 = kv4_scale(r0), z1 = kv4_least(r1), s1 = kv4_scale(r1);
+        if (CENTRE) { z0 = fmaf(8.0f, s0, z0); z1 = fmaf(8.0f, s1, z1); }
+        s0 *= Q.fs; s1 *= Q.fs;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float acc[4] = {Q.init[nt][y][0], Q.init[nt][y][1], Q.init[nt][y][0], Q.init[nt][y][1]};
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int p = PARTS - 1; p >= 0; p--)           // (the small part first)
 #pragma unroll
                 for (int k = 0; k < F::KS; k++)
                     mma_f16(acc, a[k][0], a[k][1], a[k][2], a[k][3], Q.b[nt][p][y * F::KS + k][0], Q.b[nt][p][y * F::KS + k][1]);
-            s[nt][0] += fmaf(acc[0] * s0, Q.fs[nt][0], z0 * Q.fz[nt][y][0]);
-            s[nt][1] += fmaf(acc[1] * s0, Q.fs[nt][1], z0 * Q.fz[nt][y][1]);
-            s[nt][2] += fmaf(acc[2] * s1, Q.fs[nt][0], z1 * Q.fz[nt][y][0]);
-            s[nt][3] += fmaf(acc[3] * s1, Q.fs[nt][1], z1 * Q.fz[nt][y][1]);
+            if (y == 0) {
+                s[nt][0] = fmaf(acc[0], s0, z0 * Q.fz[nt][y][0]);
+                s[nt][1] = fmaf(acc[1], s0, z0 * Q.fz[nt][y][1]);
+                s[nt][2] = fmaf(acc[2], s1, z1 * Q.fz[nt][y][0]);
+                s[nt][3] = fmaf(acc[3], s1, z1 * Q.fz[nt][y][1]);
+            } else {
+                s[nt][0] = fmaf(acc[0], s0, fmaf(z0, Q.fz[nt][y][0], s[nt][0]));
+                s[nt][1] = fmaf(acc[1], s0, fmaf(z0, Q.fz[nt][y][1], s[nt][1]));
+                s[nt][2] = fmaf(acc[2], s1, fmaf(z1, Q.fz[nt][y][0], s[nt][2]));
+                s[nt][3] = fmaf(acc[3], s1, fmaf(z1, Q.fz[nt][y][1], s[nt][3]));
+            }
         }
     }
 }
@@ -267,35 +333,37 @@ struct Kv4Acc {
         // of keys.  (Values of 2^-56 and less lose their last bits.)
         top_s = 8.673617379884035e-19f;
     }
-    // After the scores' maxima: moves the shift, and with it what has been added up.
-    __device__ __forceinline__ void rescale(const float (&mx)[NT][2], float ts) {
-        top_s = fmaxf(top_s, ts);
-        const float lg = (float)((int)(__float_as_uint(top_s) >> 23) - 126 - 15);      // 2^(lg + 15) >= top_s: p s <= 2^15
-        bool moved = false;
-        float corr[NT][2];
+    // Before a tile's weights: `mx` are the thread's largest scores of it, `ts` its largest scale of a value.  The shift follows
+    // the maxima in steps: only a score above the last one's by 8, or a larger scale, moves it (and what has been added up).
+    __device__ __forceinline__ void follow(float (&mx)[NT][2], float ts) {
+        bool above = ts > top_s;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) above = above || mx[nt][0] > m[nt][0] + 8.0f || mx[nt][1] > m[nt][1] + 8.0f;
+        if (!__any_sync(0xffffffffu, above)) return;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) mx[nt][i] = fmaxf(mx[nt][i], __shfl_xor_sync(0xffffffffu, mx[nt][i], d));
+        // (the bound of the scales is a power of two, up to four times the largest: the next tiles' need not move it again)
+        ts = warp_max(ts);
+        if (ts > top_s) top_s = __uint_as_float(min((__float_as_uint(ts) >> 23) + 2u, 254u) << 23);
+        const float lg = (float)((int)(__float_as_uint(top_s) >> 23) - 127 - 7);       // 2^(lg + 7) = top_s: p s <= 2^7, and 2^15 with the step
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 m[nt][i] = fmaxf(m[nt][i], mx[nt][i]);
                 const float ns = m[nt][i] == -INFINITY ? -INFINITY : m[nt][i] + lg;
-                corr[nt][i] = ns == shift[nt][i] ? 1.0f : kv4_exp2(shift[nt][i] - ns);
-                moved = moved || ns != shift[nt][i];
+                const float corr = ns == shift[nt][i] ? 1.0f : kv4_exp2(shift[nt][i] - ns);
                 shift[nt][i] = ns;
+                l[nt][i] *= corr;
+#pragma unroll
+                for (int y = 0; y < Kv4<HD>::NG; y++) z[nt][y][i] *= corr;
+#pragma unroll
+                for (int j = 0; j < HD / 16; j++) { o[nt][j][i] *= corr; o[nt][j][2 + i] *= corr; }
             }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    l[nt][i] *= corr[nt][i];
-#pragma unroll
-                    for (int y = 0; y < Kv4<HD>::NG; y++) z[nt][y][i] *= corr[nt][i];
-#pragma unroll
-                    for (int j = 0; j < HD / 16; j++) { o[nt][j][i] *= corr[nt][i]; o[nt][j][2 + i] *= corr[nt][i]; }
-                }
-            }
-        }
     }
     // Behind the last key: the threads' shares of the sums are added up (all get them).
     __device__ __forceinline__ void finish() {
@@ -320,29 +388,15 @@ struct Kv4Acc {
     }
 };
 
-// the values' ranges of the keys in rows g and g + 8, of group y (a key that is not there counts as zeros: whatever lies in
-// its place must not reach a sum)
-template <int HD>
-__device__ __forceinline__ void kv4_value_ranges(uint32_t (&r)[2], const unsigned char* blk, int y, bool there0, bool there1, int lane) {
+// Adds a block of 16 keys: p [nt][4] are its weights, laid out as the scores; the values' ranges of group y in ranges[y].
+template <int HD, int KEYS, int PARTS, int NT>
+__device__ __forceinline__ void kv4_add_block(Kv4Acc<HD, PARTS, NT>& A, const float (&p)[NT][4], const unsigned char* tile, int at,
+                                              const Kv4Block<HD, KEYS>& B, const uint32_t (&ranges)[Kv4<HD>::NG][2]) {
     using F = Kv4<HD>;
-    const int key = kv4_key_of(lane >> 2);
-    r[0] = there0 ? *reinterpret_cast<const uint32_t*>(blk + F::VR_OFF + (key * F::NG + y) * 4) : 0u;
-    r[1] = there1 ? *reinterpret_cast<const uint32_t*>(blk + F::VR_OFF + ((key + 8) * F::NG + y) * 4) : 0u;
-}
-
-// Adds a block of 16 keys: p [nt][4] are its weights, laid out as the scores.
-template <int HD, int PARTS, int NT>
-__device__ __forceinline__ void kv4_add_block(Kv4Acc<HD, PARTS, NT>& A, const float (&p)[NT][4], const unsigned char* blk, bool there0, bool there1,
-                                              int lane) {
-    using F = Kv4<HD>;
-    const int g = lane >> 2, t = lane & 3;
-    const int ka = t, kb = 4 + ((t + 2) & 3);              // the keys in slots 2t and 2t + 1
 #pragma unroll
     for (int y = 0; y < F::NG; y++) {
-        uint32_t r[2];
-        kv4_value_ranges<HD>(r, blk, y, there0, there1, lane);
-        const float s0 = kv4_scale(r[0]), s1 = kv4_scale(r[1]);
-        float z0 = kv4_least(r[0]), z1 = kv4_least(r[1]);
+        const float s0 = kv4_scale(ranges[y][0]), s1 = kv4_scale(ranges[y][1]);
+        float z0 = kv4_least(ranges[y][0]), z1 = kv4_least(ranges[y][1]);
         if (PARTS > 1) { z0 = fmaf(8.0f, s0, z0); z1 = fmaf(8.0f, s1, z1); }
         uint32_t b[NT][PARTS][2];
 #pragma unroll
@@ -357,17 +411,15 @@ __device__ __forceinline__ void kv4_add_block(Kv4Acc<HD, PARTS, NT>& A, const fl
             }
         }
         uint32_t u[2][F::GS / 32];                         // [keys 0..7, 8..15]: the codes of slots 2t and 2t + 1 side by side
+        const unsigned char *pa = tile + B.group(B.va, y) + at * F::ROW, *pb = tile + B.group(B.vb, y) + at * F::ROW;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             if (F::GS == 64) {
-                const int at = (g & 3) * 4;
-                const uint32_t wa = *reinterpret_cast<const uint32_t*>(blk + F::V_OFF + F::piece(ka + 8 * h, 2 * y + (g >> 2)) * 16 + at);
-                const uint32_t wb = *reinterpret_cast<const uint32_t*>(blk + F::V_OFF + F::piece(kb + 8 * h, 2 * y + (g >> 2)) * 16 + at);
+                const uint32_t wa = kv4_at<uint32_t>(pa + 8 * h * F::ROW), wb = kv4_at<uint32_t>(pb + 8 * h * F::ROW);
                 u[h][0] = __byte_perm(wa, wb, 0x5410);
                 u[h][F::GS / 32 - 1] = __byte_perm(wa, wb, 0x7632);
             } else {
-                const uint32_t wa = *reinterpret_cast<const uint16_t*>(blk + F::V_OFF + F::piece(ka + 8 * h, y) * 16 + g * 2);
-                const uint32_t wb = *reinterpret_cast<const uint16_t*>(blk + F::V_OFF + F::piece(kb + 8 * h, y) * 16 + g * 2);
+                const uint32_t wa = kv4_at<uint16_t>(pa + 8 * h * F::ROW), wb = kv4_at<uint16_t>(pb + 8 * h * F::ROW);
                 u[h][0] = wa | (wb << 16);
             }
         }
@@ -394,24 +446,34 @@ __device__ __forceinline__ void kv4_add_block(Kv4Acc<HD, PARTS, NT>& A, const fl
     }
 }
 
-// A tile of TB blocks (the first key's index is `key0`) against all of a warp's queries.  hi / lo: the last and the first key
+// TB blocks of a tile (from row `at` on, the first key's index is `key0`) against all of a warp's queries.  hi / lo: the last and the first key
 // of this thread's queries; k_lo .. k_hi: the keys that any query of the call reads.  MASKED: some key may lie outside.
 // KEEP: the scores of a column go to scores[nt][i] as well (null: it is none).
-template <int HD, int PARTS, int NT, int TB, bool CENTRE, bool MASKED, bool KEEP>
-__device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD, PARTS, NT>& Q, const unsigned char* tile, int key0,
+template <int HD, int KEYS, int PARTS, int NT, int TB, bool CENTRE, bool MASKED, bool KEEP>
+__device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD, PARTS, NT>& Q, const Kv4Block<HD, KEYS>& B, const unsigned char* tile, int at, int key0,
                                          const int (&hi)[NT][2], const int (&lo)[NT][2], int k_lo, int k_hi, int lane, float* const (&scores)[NT][2]) {
     using F = Kv4<HD>;
-    const int key = kv4_key_of(lane >> 2);
+    const int key = F::key_of(lane >> 2);
     float s[TB][NT][4];
+    uint32_t ranges[TB][F::NG][2];
     float mx[NT][2], ts = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
     for (int b = 0; b < TB; b++) {
-        const unsigned char* blk = tile + b * F::BLOCK;
-        kv4_scores<HD, PARTS, NT, CENTRE>(s[b], blk, Q, lane);
         const int ka = key0 + b * 16 + key, kb = ka + 8;
-        const bool t0 = !MASKED || (ka >= k_lo && ka <= k_hi), t1 = !MASKED || (kb >= k_lo && kb <= k_hi);
+#pragma unroll
+        for (int y = 0; y < F::NG; y++) {
+            const unsigned char* r = tile + B.r + (KEYS + at + b * 16) * 4 * F::NG + y * 4;
+            ranges[b][y][0] = kv4_at<uint32_t>(r);
+            ranges[b][y][1] = kv4_at<uint32_t>(r + 32 * F::NG);
+            if (MASKED) {                                  // (a key that is not there counts as zeros: whatever lies in its place must not reach a sum)
+                if (!(ka >= k_lo && ka <= k_hi)) ranges[b][y][0] = 0u;
+                if (!(kb >= k_lo && kb <= k_hi)) ranges[b][y][1] = 0u;
+            }
+            ts = kv4_max3(ts, kv4_scale(ranges[b][y][0]), kv4_scale(ranges[b][y][1]));
+        }
+        kv4_scores<HD, KEYS, PARTS, NT, CENTRE>(s[b], tile, at + b * 16, B, Q);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -421,25 +483,19 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
                     if (!(kb >= lo[nt][i] && kb <= hi[nt][i])) s[b][nt][2 + i] = -INFINITY;
                 }
                 if (KEEP && scores[nt][i]) { scores[nt][i][ka] = s[b][nt][i]; scores[nt][i][kb] = s[b][nt][2 + i]; }
-                mx[nt][i] = fmaxf(mx[nt][i], fmaxf(s[b][nt][i], s[b][nt][2 + i]));
+                mx[nt][i] = kv4_max3(mx[nt][i], s[b][nt][i], s[b][nt][2 + i]);
             }
-#pragma unroll
-        for (int y = 0; y < F::NG; y++) {
-            uint32_t r[2];
-            kv4_value_ranges<HD>(r, blk, y, t0, t1, lane);
-            const float a = kv4_scale(r[0]), c = kv4_scale(r[1]);
-            ts = fmaxf(ts, fmaxf(a < INFINITY ? a : 0.f, c < INFINITY ? c : 0.f));      // (a group that is not finite sets no scale)
-        }
     }
+    if (ts == INFINITY) {                                  // (a group that is not finite sets no scale)
+        ts = 0.f;
 #pragma unroll
-    for (int d = 4; d < 32; d <<= 1) {
-        ts = fmaxf(ts, __shfl_xor_sync(0xffffffffu, ts, d));
+        for (int b = 0; b < TB; b++)
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+            for (int y = 0; y < F::NG; y++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) mx[nt][i] = fmaxf(mx[nt][i], __shfl_xor_sync(0xffffffffu, mx[nt][i], d));
+                for (int i = 0; i < 2; i++) ts = fmaxf(ts, kv4_scale(ranges[b][y][i]) < INFINITY ? kv4_scale(ranges[b][y][i]) : 0.f);
     }
-    A.rescale(mx, ts);
+    A.follow(mx, ts);
     float sh[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
@@ -447,9 +503,6 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
         for (int i = 0; i < 2; i++) sh[nt][i] = A.shift[nt][i] == -INFINITY ? 0.f : A.shift[nt][i];
 #pragma unroll
     for (int b = 0; b < TB; b++) {
-        const unsigned char* blk = tile + b * F::BLOCK;
-        const int ka = key0 + b * 16 + key, kb = ka + 8;
-        const bool t0 = !MASKED || (ka >= k_lo && ka <= k_hi), t1 = !MASKED || (kb >= k_lo && kb <= k_hi);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -458,6 +511,6 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
                 s[b][nt][2 + i] = kv4_exp2(s[b][nt][2 + i] - sh[nt][i]);
                 A.l[nt][i] += s[b][nt][i] + s[b][nt][2 + i];
             }
-        kv4_add_block<HD, PARTS, NT>(A, s[b], blk, t0, t1, lane);
+        kv4_add_block<HD, KEYS, PARTS, NT>(A, s[b], tile, at + b * 16, B, ranges[b]);
     }
 }

@@ -148,7 +148,7 @@ extern "C" int kp_kv4_evict(const void* pages, const float* mass, const int* tab
                             const int* new_table, int new_blocks, int* kept, int n_seg, int max_keys, int keep, int recent, int first, int ps, int G,
                             int hd, void* stream) {
     if (n_seg <= 0) return 0;
-    if (hd < 32 || hd % 32 || hd > 256 || ps < 16 || ps % 16 || G < 1 || G > 65535 || n_seg > 65535 || keep < 1 || recent < 0 || first < 0 || first + recent > keep ||
+    if (hd < 32 || hd % 32 || hd > 256 || ps < 16 || (ps & (ps - 1)) || G < 1 || G > 65535 || n_seg > 65535 || keep < 1 || recent < 0 || first < 0 || first + recent > keep ||
         max_keys < 1 || (((uintptr_t)pages | (uintptr_t)new_pages) & 15))
         return KP_ERR_BAD_ARG;
     KeArgs a = {(const unsigned char*)pages, mass, table, max_blocks, (unsigned char*)new_pages, new_mass, new_table, new_blocks, n_keys, kept,

@@ -699,7 +699,7 @@ int kp_kv4_attention_tc(const void* q, long long ldq, const void* pages, const i
                         const int* seg_pos, int n_seg, void* out, long long ldo, float scale, int window, int ps, int H, int G, int hd, int n_rows,
                         int min_rows, int max_context, float* mass, void* scratch, void* stream) {
     if (n_rows <= 0 || n_seg <= 0) return 0;
-    if (G < 1 || H < 1 || H % G || ps < 16 || ps % 16 || window < 0 || n_seg > 65535 || G > 65535 || min_rows < 1 || !(scale > 0.f) ||
+    if (G < 1 || H < 1 || H % G || ps < 16 || (ps & (ps - 1)) || window < 0 || n_seg > 65535 || G > 65535 || min_rows < 1 || !(scale > 0.f) ||
         (((uintptr_t)pages | (uintptr_t)q | (uintptr_t)out | (uintptr_t)scratch) & 15) || (ldq & 7) || (ldo & 7) || (mass && !scratch))
         return KP_ERR_BAD_ARG;
     const int R = H / G;

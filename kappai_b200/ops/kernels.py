@@ -188,7 +188,7 @@ def _rows_2d(t: torch.Tensor, name: str) -> int:
 # issuing work and returns.  The engine reads the words of a step with the step's own device-to-host copy.
 
 _STATUS_LIBS = (("gemm_tc", "tc"), ("gemm_stream", "stream"), ("attention_mma", "attention_mma"),
-                ("attention_tc", "attention_tc"), ("moe", "moe_tc"), ("latent", "latent"), ("kv4_tc", "kv4_tc"))
+                ("attention_tc", "attention_tc"), ("moe", "moe_tc"), ("latent", "latent"), ("kv4", "kv4"), ("kv4_tc", "kv4_tc"))
 
 
 def read_status() -> dict:

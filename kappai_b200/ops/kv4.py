@@ -28,8 +28,8 @@ def kv4_group(hd: int) -> int:
 
 def kv4_page_bytes(page_size: int, hd: int) -> int:
     """Bytes of a page of one kv head: ``page_size`` keys and values of 4 bits, and 4 bytes a group of either."""
-    if hd not in KV4_HEAD_DIMS or page_size < 16 or page_size % 16:
-        raise KernelError(f"a 4-bit cache has heads of {KV4_HEAD_DIMS} values and pages of a multiple of 16 keys, "
+    if hd not in KV4_HEAD_DIMS or page_size < 16 or page_size & (page_size - 1):
+        raise KernelError(f"a 4-bit cache has heads of {KV4_HEAD_DIMS} values and pages of a power of two of keys, at least 16, "
                           f"got head size {hd}, page size {page_size}")
     return page_size * (hd + 8 * (hd // kv4_group(hd)))
 
@@ -129,7 +129,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
             lse = floats(n * H)
     ldq, ldo = ctypes.c_longlong(_rows_2d(q, "q")), ctypes.c_longlong(_rows_2d(out, "out"))
     if short or (tiled and not tc):
-        _run("kv4_attention", load_library("kv4").kp_kv4_attention, _ptr(q), ldq, _ptr(pages), _ptr(block_table), block_table.shape[1], _ptr(cu_rows),
+        _run("kv4_attention", load_library("kv4").kp_kv4_attention, _ptr(q), ldq, _ptr(pages), ctypes.c_longlong(pages.shape[0]), _ptr(block_table), block_table.shape[1], _ptr(cu_rows),
              _ptr(seg_pos), n_seg, _ptr(out), ldo, ctypes.c_float(scale), int(window or 0), page_size, H, G, hd, n, short, int(tiled and not tc),
              n_chunks, chunk, max_context, _ptr(part_o), _ptr(part_ml), _ptr(scores), n_chunks * chunk, _ptr(lse_split), _ptr(lse), _ptr(mass),
              dtype_code(q.dtype), STREAM)
