@@ -141,7 +141,8 @@ struct Kv4Args {
     float* part_o; float* part_ml; float* scores; int ld_scores; float* lse_split;
     float* lse;                                            // tiled form with mass: shift + log2(sum of p) (base 2) [row][head], or null
     float* mass;                                           // [page][G][ps], or null
-    int n_chunks, chunk;                                   // split form: chunks of `chunk` keys
+    int n_chunks, chunk;                                   // split form: chunks of `chunk` keys (from the first key of the segment's window on)
+    int fused;                                             // split form: a segment's chunks are the CTAs of a cluster, which join them itself
     int max_rows;                                          // split form: segments of more rows are not its own
     int min_rows;                                          // tiled form: nor are segments of fewer rows this form's
     int n_seg;
@@ -175,9 +176,28 @@ template <int HD, int PARTS>
 struct Kv4Split {
     static constexpr int TILE = HD <= 64 ? 64 : (HD <= 128 ? 32 : 16), TB = TILE / 16, STAGES = 3, NW = 4, KEYS = NW * TILE;
     static constexpr int STAGE = (Kv4<HD>::bytes(KEYS) + 1023) / 1024 * 1024;
-    static constexpr size_t RING = (size_t)STAGES * STAGE, JOIN = sizeof(float) * NW * 8 * (HD + 2);
+    static constexpr size_t RING = (size_t)STAGES * STAGE, JOIN = sizeof(float) * (NW + 1) * 8 * (HD + 2);
     static constexpr size_t SMEM = 1024 + (RING > JOIN ? RING : JOIN);
 };
+
+__device__ __forceinline__ void kv4_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+// a float at this place of the shared memory of the cluster's CTA `rank`
+__device__ __forceinline__ float kv4_peer(const float* p, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(kp_smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// The first key of a segment's chunks: that of its first row's window, down to a whole tile.
+__device__ __forceinline__ int kv4_chunk_base(int pos0, int window, int keys) {
+    const int first = pos0 - window + 1;
+    return window > 0 && first > 0 ? first / keys * keys : 0;
+}
+__host__ __device__ constexpr int kv4_tile_keys(int hd) { return hd <= 64 ? 256 : (hd <= 128 ? 128 : 64); }
 
 template <int HD, int PARTS, bool KEEP, typename T>
 __global__ void __launch_bounds__(128, PARTS == 1 && HD <= 128 ? 4 : 2)
@@ -200,13 +220,15 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
     const int col0 = (blockIdx.y / p.G) * 8, n_cols = n_rows * R;
     if (n_rows > p.max_rows || col0 >= n_cols) return;
     const int col1 = min(col0 + 8, n_cols) - 1;
+    const int c_base = kv4_chunk_base(pos0, p.window, kv4_tile_keys(HD)) + chunk * p.chunk;      // the chunk's first key
     // the last key that the columns read in the chunk (and none that the block table has no page for)
-    const int k_hi = min(min(pos0 + col1 / R, (chunk + 1) * p.chunk - 1), p.max_blocks * p.ps - 1);
+    const int k_hi = min(min(pos0 + col1 / R, c_base + p.chunk - 1), p.max_blocks * p.ps - 1);
     const int k_first = p.window > 0 ? max(0, pos0 + col0 / R - p.window + 1) : 0;
-    const int k_lo = max(k_first, chunk * p.chunk);
+    const int k_lo = max(k_first, c_base);
     const int t_lo = k_lo / S::KEYS, n_tiles = k_hi >= k_lo ? k_hi / S::KEYS - t_lo + 1 : 0;
-    if (p.n_chunks > 1 && n_tiles == 0) return;            // (a single chunk writes its rows also where they read nothing)
+    if (p.n_chunks > 1 && !p.fused && n_tiles == 0) return;      // (what joins chunks itself writes rows also where they read nothing)
     const int* bt = p.block_table + (size_t)seg * p.max_blocks;
+    const int s_base = c_base - chunk * p.chunk;           // the key of the scores' first column
 
     // Lane j has piece j of a tile: the keys of one page (at most 16 pieces).
     const int piece = min(p.ps, S::KEYS);
@@ -254,7 +276,7 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int c = col0 + 2 * (lane & 3) + i;
-            if (c < n_cols) sc[0][i] = p.scores + (((size_t)seg * p.max_rows + c / R) * p.H + kvh * R + c % R) * p.ld_scores;
+            if (c < n_cols) sc[0][i] = p.scores + (((size_t)seg * p.max_rows + c / R) * p.H + kvh * R + c % R) * p.ld_scores - s_base;
         }
     }
     Kv4Acc<HD, PARTS, 1> A;
@@ -309,6 +331,12 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
     }
     __syncthreads();
     const int live = col1 - col0 + 1;
+    float* co = jl + S::NW * 8;                            // the CTA's own: [column][HD], shift, sum of p
+    float *cm = co + 8 * HD, *cl = cm + 8;
+    auto place_of = [&](int col) { return ((size_t)seg * p.max_rows + col / R) * p.H + kvh * R + col % R; };
+    auto write = [&](int c, int d, float v) {
+        ((T*)p.out)[(size_t)(row0 + (col0 + c) / R) * p.ldo + (size_t)(kvh * R + (col0 + c) % R) * HD + d] = from_f32<T>(v);
+    };
     for (int e = threadIdx.x; e < live * HD; e += 128) {
         const int c = e / HD, d = e - c * HD;
         float M = -INFINITY;
@@ -321,16 +349,59 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
             if (jm[w * 8 + c] != -INFINITY) acc = fmaf(jo[(size_t)(w * 8 + c) * HD + d], f, acc);
             L = fmaf(jl[w * 8 + c], f, L);
         }
-        const int col = col0 + c;
-        const size_t rh = ((size_t)seg * p.max_rows + col / R) * p.H + kvh * R + col % R;
-        if (p.n_chunks == 1) {
-            ((T*)p.out)[(size_t)(row0 + col / R) * p.ldo + (size_t)(kvh * R + col % R) * HD + d] = from_f32<T>(M == -INFINITY ? 0.f : acc / L);
-            if (KEEP && d == 0) p.lse_split[rh] = M == -INFINITY ? INFINITY : M + log2f(L);
+        if (p.n_chunks > 1 && p.fused) {
+            co[e] = acc;
+            if (d == 0) { cm[c] = M; cl[c] = L; }
+        } else if (p.n_chunks == 1) {
+            write(c, d, M == -INFINITY ? 0.f : acc / L);
+            if (KEEP && d == 0) cm[c] = M == -INFINITY ? INFINITY : M + log2f(L);
+            if (KEEP && d == 0 && !p.fused) p.lse_split[place_of(col0 + c)] = cm[c];
         } else {
-            p.part_o[(rh * p.n_chunks + chunk) * HD + d] = acc;
-            if (d == 0) { p.part_ml[(rh * p.n_chunks + chunk) * 2] = M; p.part_ml[(rh * p.n_chunks + chunk) * 2 + 1] = L; }
+            const size_t at = place_of(col0 + c) * p.n_chunks + chunk;
+            p.part_o[at * HD + d] = acc;
+            if (d == 0) { p.part_ml[at * 2] = M; p.part_ml[at * 2 + 1] = L; }
         }
     }
+    if (!p.fused) return;
+    float* lse = jm;                                       // (the warps' shifts have been read) [column]
+    if (p.n_chunks > 1) {
+        // the cluster's CTAs are the chunks: each joins its share of the outputs, in the order of the chunks, from all of them
+        kv4_cluster_sync();
+        for (int e = chunk * 128 + threadIdx.x; e < live * HD; e += p.n_chunks * 128) {
+            const int c = e / HD;
+            float M = -INFINITY, acc = 0.f, L = 0.f;
+            for (int k = 0; k < p.n_chunks; k++) M = fmaxf(M, kv4_peer(cm + c, k));
+            for (int k = 0; k < p.n_chunks; k++) {
+                const float m = kv4_peer(cm + c, k);
+                if (m == -INFINITY) continue;
+                const float f = kv4_exp2(m - M);
+                acc = fmaf(kv4_peer(co + e, k), f, acc);
+                L = fmaf(kv4_peer(cl + c, k), f, L);
+            }
+            write(c, e - c * HD, M == -INFINITY ? 0.f : acc / L);
+        }
+        if (KEEP && threadIdx.x < live) {
+            float M = -INFINITY, L = 0.f;
+            for (int k = 0; k < p.n_chunks; k++) M = fmaxf(M, kv4_peer(cm + threadIdx.x, k));
+            for (int k = 0; k < p.n_chunks; k++) {
+                const float m = kv4_peer(cm + threadIdx.x, k);
+                if (m != -INFINITY) L = fmaf(kv4_peer(cl + threadIdx.x, k), kv4_exp2(m - M), L);
+            }
+            lse[threadIdx.x] = M == -INFINITY ? INFINITY : M + log2f(L);
+        }
+    }
+    if (KEEP) {
+        // the weights of the chunk's keys: a thread a key, columns in order (they are all of the segment's)
+        __syncthreads();
+        const float* sums = p.n_chunks > 1 ? lse : cm;
+        for (int key = k_lo + threadIdx.x; key <= k_hi; key += 128) {
+            float w = 0.f;
+            for (int c = 0; c < live; c++) w += kv4_exp2(p.scores[place_of(c) * p.ld_scores + key - s_base] - sums[c]);
+            const int pg = bt[key >> p.ps_log2];
+            p.mass[((size_t)pg * p.G + kvh) * p.ps + (key & (p.ps - 1))] += w;
+        }
+    }
+    if (p.n_chunks > 1) kv4_cluster_sync();                // (nobody leaves while another reads its shared memory)
 }
 
 // ---- joins the chunks and adds up the mass: a warp a (segment, row, head), in the order of the chunks; behind those CTAs, where
@@ -365,7 +436,8 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
         const int lo = p.window > 0 ? max(0, hi - p.window + 1) : 0;
         const float* ml = p.part_ml + (size_t)place * p.n_chunks * 2;
         const float* po = p.part_o + (size_t)place * p.n_chunks * hd;
-        const int c_lo = lo / p.chunk, c_hi = hi < 0 ? -1 : min(hi / p.chunk, p.n_chunks - 1);
+        const int base = kv4_chunk_base(p.seg_pos[seg], p.window, kv4_tile_keys(hd));
+        const int c_lo = (lo - base) / p.chunk, c_hi = hi < 0 ? -1 : min((hi - base) / p.chunk, p.n_chunks - 1);
         const float2 t = kv4_total(ml, c_lo, c_hi, lane);
         const float inv = t.x == -INFINITY ? 0.f : 1.0f / t.y;
         for (int d = lane * 2; d < hd; d += 64) {
@@ -394,12 +466,12 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
         return;
     }
     __shared__ float lse[64];                              // of 64 (row, head)s at a time
-    const int b = blockIdx.x - n_join, key = (b % mass_blocks) * 128 + threadIdx.x, kvh = b / mass_blocks % p.G, seg = b / mass_blocks / p.G;
+    const int b = blockIdx.x - n_join, kvh = b / mass_blocks % p.G, seg = b / mass_blocks / p.G;
     const int n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg], pos0 = p.seg_pos[seg], R = p.H / p.G, n_cols = n_rows * R;
-    const int k0 = key - threadIdx.x;
+    const int base = kv4_chunk_base(pos0, p.window, kv4_tile_keys(hd)), k0 = base + (b % mass_blocks) * 128, key = k0 + threadIdx.x;
     if (n_rows > p.max_rows || k0 > pos0 + n_rows - 1 || (p.window > 0 && k0 + 127 <= pos0 - p.window)) return;
     // (in front of the first row's window nothing is read, and the pages may be somebody else's by now)
-    const bool there = key <= pos0 + n_rows - 1 && key < p.max_blocks * p.ps && key < p.ld_scores && !(p.window > 0 && key <= pos0 - p.window);
+    const bool there = key <= pos0 + n_rows - 1 && key < p.max_blocks * p.ps && key - base < p.ld_scores && !(p.window > 0 && key <= pos0 - p.window);
     float sum = 0.f;
     for (int c0 = 0; c0 < n_cols; c0 += 64) {
         __syncthreads();
@@ -410,7 +482,8 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
             if (p.n_chunks == 1) {
                 v = p.lse_split[place];
             } else {
-                const int c_lo = p.window > 0 ? max(0, hi - p.window + 1) / p.chunk : 0, c_hi = hi < 0 ? -1 : min(hi / p.chunk, p.n_chunks - 1);
+                const int lo = p.window > 0 ? max(0, hi - p.window + 1) : 0;
+                const int c_lo = (lo - base) / p.chunk, c_hi = hi < 0 ? -1 : min((hi - base) / p.chunk, p.n_chunks - 1);
                 const float2 t = kv4_total(p.part_ml + place * p.n_chunks * 2, c_lo, c_hi, lane);
                 v = t.x == -INFINITY ? INFINITY : t.x + log2f(t.y);
             }
@@ -423,7 +496,7 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
                 const int r = (c0 + i) / R, hi = pos0 + r;
                 if (key > hi || (p.window > 0 && key <= hi - p.window)) continue;
                 const size_t place = ((size_t)seg * p.max_rows + r) * p.H + kvh * R + (c0 + i) % R;
-                sum += kv4_exp2(p.scores[place * p.ld_scores + key] - lse[i]);
+                sum += kv4_exp2(p.scores[place * p.ld_scores + key - base] - lse[i]);
             }
         }
     }
@@ -694,8 +767,21 @@ static int kv4_run_split(const Kv4Args& a, long long n_pages, cudaStream_t st) {
     int e = kv4_codes_map<HD>(&codes, a, n_pages, S::KEYS);
     if (e) return e;
     if ((e = kp_smem_limit(kv4_split_kernel<HD, PARTS, KEEP, T>, S::SMEM, ready))) return e;
-    const cudaError_t c = kp_launch_pdl(kv4_split_kernel<HD, PARTS, KEEP, T>, dim3(a.n_chunks, a.G * ((a.max_rows * (a.H / a.G) + 7) / 8), a.n_seg), dim3(128),
-                                        S::SMEM, st, codes, a);
+    static_assert(S::KEYS == kv4_tile_keys(HD), "chunks begin and end with a tile");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.n_chunks, a.G * ((a.max_rows * (a.H / a.G) + 7) / 8), a.n_seg);
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.n_chunks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.fused && a.n_chunks > 1 ? 2 : 1;
+    const cudaError_t c = cudaLaunchKernelEx(&cfg, kv4_split_kernel<HD, PARTS, KEEP, T>, codes, a);
     return c ? (int)c : kp_launch_status();
 }
 
@@ -705,7 +791,7 @@ static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_til
     if (a.max_rows > 0) {
         const int e = a.mass ? kv4_run_split<HD, PARTS, true, T>(a, n_pages, st) : kv4_run_split<HD, PARTS, false, T>(a, n_pages, st);
         if (e) return e;
-        if (a.n_chunks > 1 || a.mass) {
+        if (!a.fused && (a.n_chunks > 1 || a.mass)) {
             const long long join = a.n_chunks > 1 ? ((long long)a.n_seg * a.max_rows * a.H + 3) / 4 : 0;
             const int mass_blocks = a.mass ? (a.n_chunks * a.chunk + 127) / 128 : 0;
             const long long blocks = join + (long long)mass_blocks * a.G * a.n_seg;
@@ -773,11 +859,12 @@ int kp_kv4_read(const void* pages, long long n_pages, const int* slot_map, void*
 // Scratch: see Kv4Args; lse_split and scores where there is mass and a split form, lse where there is mass and a tiled one.
 int kp_kv4_attention(const void* q, long long ldq, const void* pages, long long n_pages, const int* block_table, int max_blocks, const int* cu_rows, const int* seg_pos,
                      int n_seg, void* out, long long ldo, float scale, int window, int ps, int H, int G, int hd, int n_rows, int short_rows,
-                     int long_rows, int n_chunks, int chunk, int max_context, float* part_o, float* part_ml, float* scores, int ld_scores,
+                     int long_rows, int n_chunks, int chunk, int fused, int max_context, float* part_o, float* part_ml, float* scores, int ld_scores,
                      float* lse_split, float* lse, float* mass, int dtype, void* stream) {
     if (n_rows <= 0 || n_seg <= 0) return 0;
     if (G < 1 || H < 1 || H % G || ps < 16 || (ps & (ps - 1)) || window < 0 || n_chunks < 1 || chunk < 64 || chunk % 64 || n_seg > 65535 || H > 65535 ||
-        ((uintptr_t)pages & 15) || (mass && ((long_rows && !lse) || (short_rows > 0 && (!scores || !lse_split)))) || (n_chunks > 1 && short_rows > 0 && (!part_o || !part_ml)))
+        ((uintptr_t)pages & 15) || (mass && ((long_rows && !lse) || (short_rows > 0 && (!scores || !lse_split)))) || (n_chunks > 1 && short_rows > 0 && !fused && (!part_o || !part_ml)) ||
+        chunk % kv4_tile_keys(hd) || (fused && (n_chunks > 8 || (mass && (long long)short_rows * (H / G) > 8))))
         return KP_ERR_BAD_ARG;
     Kv4Args a = {};
     a.q = q; a.ldq = ldq; a.out = out; a.ldo = ldo; a.pages = (const unsigned char*)pages;
@@ -785,7 +872,7 @@ int kp_kv4_attention(const void* q, long long ldq, const void* pages, long long 
     a.scale = scale; a.window = window; a.ps = ps; a.ps_log2 = kv4_log2(ps); a.H = H; a.G = G;
     a.part_o = part_o; a.part_ml = part_ml; a.scores = mass ? scores : nullptr; a.ld_scores = ld_scores;
     a.lse_split = mass ? lse_split : nullptr; a.lse = mass ? lse : nullptr; a.mass = mass;
-    a.n_chunks = n_chunks; a.chunk = chunk; a.max_rows = short_rows; a.min_rows = short_rows + 1; a.n_seg = n_seg;
+    a.n_chunks = n_chunks; a.chunk = chunk; a.fused = fused; a.max_rows = short_rows; a.min_rows = short_rows + 1; a.n_seg = n_seg;
     if (dtype == KP_DTYPE_BF16) {
         KV4_DISPATCH_HD(hd, HD, return (kv4_run<HD, 1, bf16>(a, n_pages, n_rows, long_rows, max_context, (cudaStream_t)stream)));
     } else if (dtype == KP_DTYPE_F32) {

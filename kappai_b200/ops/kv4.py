@@ -8,17 +8,40 @@ launches on the current CUDA stream and raises :class:`~kappai_b200.ops.kernels.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
 
 from .build import load_library
-from .kernels import STREAM, KernelError, _need, _ptr, _rows_2d, _run, dtype_code
+from .kernels import STREAM, KernelError, _need, _rows_2d, _run, dtype_code
 
 KV4_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 KV4_SHORT_ROWS = 8         # segments of at most this many rows share their keys out over many CTAs
 USE_TC_KV4 = True          # longer ones of bfloat16 rows with heads of 64 or 128 run on the tcgen05 tensor cores
 _CTAS = 148 * 4            # CTAs of the split form that an even spread over the SMs wants
+
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+# Argument types of the launchers: a step makes a call a layer, and plain integers that ctypes converts itself cost a third of
+# what an object an argument does.
+_LAUNCHERS = {
+    "kp_kv4_write": ("kv4", [_P, _L, _P, _L, _P, _L, _P] + [_I] * 5 + [_P]),
+    "kp_kv4_read": ("kv4", [_P, _L, _P, _P, _P] + [_I] * 5 + [_P]),
+    "kp_kv4_attention": ("kv4", [_P, _L, _P, _L, _P, _I, _P, _P, _I, _P, _L, _F] + [_I] * 12 + [_P, _P, _P, _I, _P, _P, _P, _I, _P]),
+    "kp_kv4_attention_tc": ("kv4_tc", [_P, _L, _P, _P, _I, _P, _P, _I, _P, _L, _F] + [_I] * 8 + [_P, _P, _P]),
+    "kp_kv4_evict": ("kv4_evict", [_P, _P, _P, _I, _P, _P, _P, _P, _I, _P] + [_I] * 8 + [_P]),
+}
+_fns = {}
+
+
+def _fn(name: str):
+    fn = _fns.get(name)
+    if fn is None:
+        lib, types = _LAUNCHERS[name]
+        fn = getattr(load_library(lib), name)
+        fn.argtypes = types
+        _fns[name] = fn
+    return fn
 
 
 def kv4_group(hd: int) -> int:
@@ -26,6 +49,7 @@ def kv4_group(hd: int) -> int:
     return 64 if hd % 64 == 0 else 32
 
 
+@lru_cache(maxsize=None)
 def kv4_page_bytes(page_size: int, hd: int) -> int:
     """Bytes of a page of one kv head: ``page_size`` keys and values of 4 bits, and 4 bytes a group of either."""
     if hd not in KV4_HEAD_DIMS or page_size < 16 or page_size & (page_size - 1):
@@ -34,16 +58,34 @@ def kv4_page_bytes(page_size: int, hd: int) -> int:
     return page_size * (hd + 8 * (hd // kv4_group(hd)))
 
 
-def _pages(t: torch.Tensor, name: str, page_size: int, G: int, hd: int) -> None:
-    _need(t, name, torch.uint8)
-    if t.dim() != 3 or tuple(t.shape[1:]) != (G, kv4_page_bytes(page_size, hd)):
+def _have(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+    """The address of a contiguous CUDA tensor of that type."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+        _need(t, name, dtype)
+    return t.data_ptr()
+
+
+def _have_rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, width: int) -> Tuple[int, int]:
+    """Address and row stride of a CUDA tensor [n, width] with contiguous rows."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
+        _need(t, name, dtype, contiguous=False)
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
+        raise KernelError(f"{name}: expected [{n}, {width}], got {tuple(t.shape)}")
+    return t.data_ptr(), _rows_2d(t, name)
+
+
+def _have_pages(t: torch.Tensor, name: str, page_size: int, G: int, hd: int) -> int:
+    at = _have(t, name, torch.uint8)
+    if t.dim() != 3 or t.shape[1] != G or t.shape[2] != kv4_page_bytes(page_size, hd):
         raise KernelError(f"{name}: expected [n_pages, {G}, {kv4_page_bytes(page_size, hd)}], got {tuple(t.shape)}")
+    return at
 
 
-def _mass(t: torch.Tensor, name: str, pages: torch.Tensor, page_size: int, G: int) -> None:
-    _need(t, name, torch.float32)
+def _have_mass(t: torch.Tensor, name: str, pages: torch.Tensor, page_size: int, G: int) -> int:
+    at = _have(t, name, torch.float32)
     if tuple(t.shape) != (pages.shape[0], G, page_size):
         raise KernelError(f"{name}: expected [{pages.shape[0]}, {G}, {page_size}], got {tuple(t.shape)}")
+    return at
 
 
 def kv4_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slot_map: torch.Tensor, page_size: int, G: int, hd: int) -> None:
@@ -51,36 +93,35 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slot_map: t
     (int32: page * page_size + place; -1: nowhere).  A group is cut into 16 equal steps from its smallest value on, ``s =
     bfloat16((max - min) / 15)``, ``z = bfloat16(min)``, ``c = round((x - z) / s)`` (halves to even, within 0..15; 0 where s is
     0).  A group with a value that is not finite reads as NaN."""
-    _need(k, "k", contiguous=False); _need(v, "v", k.dtype, contiguous=False); _need(slot_map, "slot_map", torch.int32)
-    _pages(pages, "pages", page_size, G, hd)
-    n = slot_map.numel()
-    if tuple(k.shape) != (n, G * hd) or tuple(v.shape) != (n, G * hd):
-        raise KernelError(f"kv4_write: expected k and v of [{n}, {G * hd}], got {tuple(k.shape)} and {tuple(v.shape)}")
-    _run("kv4_write", load_library("kv4").kp_kv4_write, _ptr(k), ctypes.c_longlong(_rows_2d(k, "k")), _ptr(v), ctypes.c_longlong(_rows_2d(v, "v")),
-         _ptr(pages), ctypes.c_longlong(pages.shape[0]), _ptr(slot_map), n, page_size, G, hd, dtype_code(k.dtype), STREAM)
+    slots = _have(slot_map, "slot_map", torch.int32)
+    at, n, code = _have_pages(pages, "pages", page_size, G, hd), slot_map.numel(), dtype_code(k.dtype)
+    pk, ldk = _have_rows(k, "k", k.dtype, n, G * hd)
+    pv, ldv = _have_rows(v, "v", k.dtype, n, G * hd)
+    _run("kv4_write", _fn("kp_kv4_write"), pk, ldk, pv, ldv, at, pages.shape[0], slots, n, page_size, G, hd, code, STREAM)
 
 
 def kv4_read(pages: torch.Tensor, slot_map: torch.Tensor, page_size: int, G: int, hd: int,
              dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values in the slots, as rows [n, G hd] of ``dtype`` (a slot of -1 reads as zeros)."""
-    _need(slot_map, "slot_map", torch.int32)
-    _pages(pages, "pages", page_size, G, hd)
-    code, n = dtype_code(dtype), slot_map.numel()
-    k = torch.empty((n, G * hd), dtype=dtype, device=pages.device)
-    v = torch.empty_like(k)
-    _run("kv4_read", load_library("kv4").kp_kv4_read, _ptr(pages), ctypes.c_longlong(pages.shape[0]), _ptr(slot_map), _ptr(k), _ptr(v), n, page_size,
-         G, hd, code, STREAM)
+    slots = _have(slot_map, "slot_map", torch.int32)
+    at, n, code = _have_pages(pages, "pages", page_size, G, hd), slot_map.numel(), dtype_code(dtype)
+    k, v = torch.empty((2, n, G * hd), dtype=dtype, device=pages.device).unbind(0)
+    _run("kv4_read", _fn("kp_kv4_read"), at, pages.shape[0], slots, k.data_ptr(), v.data_ptr(), n, page_size, G, hd, code, STREAM)
     return k, v
 
 
-def kv4_chunks(n_seg: int, max_rows: int, max_context: int, window: Optional[int], H: int, G: int, hd: int) -> Tuple[int, int]:
-    """(number of chunks, keys a chunk) of the split form: as many CTAs as fill the SMs, none with less than a tile a warp."""
-    least = 256 if hd <= 64 else (128 if hd <= 128 else 64)
-    span = max_context if not window else min(max_context, window + max_rows)
+@lru_cache(maxsize=4096)
+def kv4_chunks(n_seg: int, max_rows: int, max_context: int, window: int, H: int, G: int, hd: int) -> Tuple[int, int]:
+    """(number of chunks, keys a chunk) of the split form: as many CTAs as fill the SMs, none with less than a tile of keys.  Up to 16
+    such chunks are made 8: those are one cluster, which joins them itself and spares a launch."""
+    tile = 256 if hd <= 64 else (128 if hd <= 128 else 64)
+    span = min(max_context, window + max_rows + tile - 1) if window else max_context      # from the first tile that a row reads
     want = max(1, _CTAS // max(1, n_seg * G * -(-max_rows * (H // G) // 8)))
-    chunk = max(least, -(-span // want))
-    chunk = -(-chunk // least) * least
-    return -(-max_context // chunk), chunk
+    n = -(-span // tile)
+    if min(n, want) <= 16:
+        want = min(want, 8)
+    chunk = -(-n // want) * tile
+    return -(-span // chunk), chunk
 
 
 def kv4_tc_ok(q: torch.Tensor, out: torch.Tensor, hd: int, scale: float) -> bool:
@@ -99,49 +140,55 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     ``min_rows`` bound the rows of a sequence, ``max_context`` the keys that any row reads (host integers).  ``mass`` (float32
     [n_pages, G, page_size]): the softmax weight of every key, summed over the rows and the query heads of its kv head, is added
     to the key's entry (in a fixed order: the same call gives the same bits)."""
-    _need(q, "q", contiguous=False); _need(out, "out", q.dtype, contiguous=False)
-    _need(block_table, "block_table", torch.int32); _need(cu_rows, "cu_rows", torch.int32); _need(seg_pos, "seg_pos", torch.int32)
-    _pages(pages, "pages", page_size, G, hd)
-    n, n_seg = q.shape[0], seg_pos.numel()
-    if G < 1 or H % G or tuple(q.shape) != (n, H * hd) or tuple(out.shape) != (n, H * hd):
-        raise KernelError("kv4_attention: shape mismatch")
+    if G < 1 or H % G:
+        raise KernelError(f"kv4_attention: {H} query heads over {G} kv heads")
+    n, n_seg, code = q.shape[0], seg_pos.numel(), dtype_code(q.dtype)
+    pq, ldq = _have_rows(q, "q", q.dtype, n, H * hd)
+    po, ldo = _have_rows(out, "out", q.dtype, n, H * hd)
+    at = _have_pages(pages, "pages", page_size, G, hd)
+    table, cu, pos = _have(block_table, "block_table", torch.int32), _have(cu_rows, "cu_rows", torch.int32), _have(seg_pos, "seg_pos", torch.int32)
     if cu_rows.numel() != n_seg + 1 or block_table.dim() != 2 or block_table.shape[0] < n_seg:
         raise KernelError("kv4_attention: cu_rows has one entry more than seg_pos, block_table a row for each of them")
     if window is not None and window < 1:
         raise KernelError("kv4_attention: the window is a positive number of keys")
-    if max_context < 1 or max_context > block_table.shape[1] * page_size:
-        raise KernelError(f"kv4_attention: max_context={max_context} does not lie within the block table's {block_table.shape[1]} pages")
-    if mass is not None:
-        _mass(mass, "mass", pages, page_size, G)
+    width = block_table.shape[1]
+    if max_context < 1 or max_context > width * page_size:
+        raise KernelError(f"kv4_attention: max_context={max_context} does not lie within the block table's {width} pages")
+    pm = None if mass is None else _have_mass(mass, "mass", pages, page_size, G)
+    if not n or not n_seg:
+        return out
     short = min(max_rows, KV4_SHORT_ROWS) if min_rows <= KV4_SHORT_ROWS else 0
-    n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd)
-    part_o = part_ml = scores = lse_split = lse = None
-    floats = lambda count: torch.empty(count, dtype=torch.float32, device=q.device)  # noqa: E731
-    places = n_seg * short * H
     tiled = max_rows > KV4_SHORT_ROWS
     tc = tiled and kv4_tc_ok(q, out, hd, scale)
-    if short and n_chunks > 1:
-        part_o, part_ml = floats(places * n_chunks * hd), floats(places * n_chunks * 2)
-    if mass is not None:
-        if short:
-            scores, lse_split = floats(places * n_chunks * chunk), floats(places)
-        if tiled and not tc:
-            lse = floats(n * H)
-    ldq, ldo = ctypes.c_longlong(_rows_2d(q, "q")), ctypes.c_longlong(_rows_2d(out, "out"))
+    window = window or 0
     if short or (tiled and not tc):
-        _run("kv4_attention", load_library("kv4").kp_kv4_attention, _ptr(q), ldq, _ptr(pages), ctypes.c_longlong(pages.shape[0]), _ptr(block_table), block_table.shape[1], _ptr(cu_rows),
-             _ptr(seg_pos), n_seg, _ptr(out), ldo, ctypes.c_float(scale), int(window or 0), page_size, H, G, hd, n, short, int(tiled and not tc),
-             n_chunks, chunk, max_context, _ptr(part_o), _ptr(part_ml), _ptr(scores), n_chunks * chunk, _ptr(lse_split), _ptr(lse), _ptr(mass),
-             dtype_code(q.dtype), STREAM)
+        n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd)
+        # one allocation for what the launches hand one another: results of chunks, their (shift, sum), scores, logarithms of sums
+        fused = n_chunks <= 8 and (pm is None or short * (H // G) <= 8)
+        places, many = n_seg * short * H, n_chunks > 1 and not fused
+        sizes = (places * n_chunks * hd if many else 0, places * n_chunks * 2 if many else 0,
+                 places * n_chunks * chunk if pm else 0, places if pm and not fused else 0, n * H if pm and tiled and not tc else 0)
+        total = sum(sizes)
+        p0 = torch.empty(total, dtype=torch.float32, device=q.device).data_ptr() if total else 0
+        p1 = p0 + 4 * sizes[0]
+        p2 = p1 + 4 * sizes[1]
+        p3 = p2 + 4 * sizes[2]
+        _run("kv4_attention", _fn("kp_kv4_attention"), pq, ldq, at, pages.shape[0], table, width, cu, pos, n_seg, po, ldo, scale, window, page_size, H, G,
+             hd, n, short, int(tiled and not tc), n_chunks, chunk, fused, max_context, p0, p1, p2, n_chunks * chunk, p3, p3 + 4 * sizes[3], pm, code, STREAM)
     if tc:
-        lib, scratch = load_library("kv4_tc"), None
-        if mass is not None:
-            lib.kp_kv4_tc_scratch.restype = ctypes.c_longlong
-            scratch = torch.empty(lib.kp_kv4_tc_scratch(n, n_seg, H, G, hd), dtype=torch.uint8, device=q.device)
-        _run("kv4_attention_tc", lib.kp_kv4_attention_tc, _ptr(q), ldq, _ptr(pages), _ptr(block_table), block_table.shape[1], _ptr(cu_rows),
-             _ptr(seg_pos), n_seg, _ptr(out), ldo, ctypes.c_float(scale), int(window or 0), page_size, H, G, hd, n, short + 1, max_context,
-             _ptr(mass), _ptr(scratch), STREAM)
+        scratch = None
+        if pm:
+            size = _tc_scratch(n, n_seg, H, G, hd)
+            scratch = torch.empty(size, dtype=torch.uint8, device=q.device).data_ptr()
+        _run("kv4_attention_tc", _fn("kp_kv4_attention_tc"), pq, ldq, at, table, width, cu, pos, n_seg, po, ldo, scale, window, page_size, H, G, hd, n,
+             short + 1, max_context, pm, scratch, STREAM)
     return out
+
+
+def _tc_scratch(n: int, n_seg: int, H: int, G: int, hd: int) -> int:
+    fn = load_library("kv4_tc").kp_kv4_tc_scratch
+    fn.restype = ctypes.c_longlong
+    return fn(n, n_seg, H, G, hd)
 
 
 def kv4_evict(pages: torch.Tensor, mass: torch.Tensor, block_table: torch.Tensor, n_keys: torch.Tensor, new_pages: torch.Tensor,
@@ -151,17 +198,16 @@ def kv4_evict(pages: torch.Tensor, mass: torch.Tensor, block_table: torch.Tensor
     ``recent`` last and of the others those with the most ``mass`` (equal: the lowest index); all, where there are not more.
     They move with their mass to places 0, 1, ... of ``new_table``'s pages, in their order.  The new pages are none of the
     sequences' old ones.  ``kept`` (int32 [n, G, keep]) gets the old indices, -1 behind the last."""
-    _pages(pages, "pages", page_size, G, hd); _pages(new_pages, "new_pages", page_size, G, hd)
-    _mass(mass, "mass", pages, page_size, G); _mass(new_mass, "new_mass", new_pages, page_size, G)
-    for t, nm in ((block_table, "block_table"), (new_table, "new_table"), (n_keys, "n_keys"), (kept, "kept")):
-        _need(t, nm, torch.int32)
-    n = n_keys.numel()
+    at, new_at = _have_pages(pages, "pages", page_size, G, hd), _have_pages(new_pages, "new_pages", page_size, G, hd)
+    pm, new_pm = _have_mass(mass, "mass", pages, page_size, G), _have_mass(new_mass, "new_mass", new_pages, page_size, G)
+    table, new_t = _have(block_table, "block_table", torch.int32), _have(new_table, "new_table", torch.int32)
+    keys, pk, n = _have(n_keys, "n_keys", torch.int32), _have(kept, "kept", torch.int32), n_keys.numel()
     if keep < 1 or min(recent, first) < 0 or first + recent > keep:
         raise KernelError(f"kv4_evict: keep={keep} is positive and not less than first={first} and recent={recent} together")
     if block_table.dim() != 2 or new_table.dim() != 2 or min(block_table.shape[0], new_table.shape[0]) < n or tuple(kept.shape) != (n, G, keep):
         raise KernelError("kv4_evict: block tables with a row a sequence and kept of [sequences, kv heads, keep]")
     if max_keys < 1 or max_keys > block_table.shape[1] * page_size or min(keep, max_keys) > new_table.shape[1] * page_size:
         raise KernelError("kv4_evict: the block tables hold max_keys keys, and the ones that stay")
-    _run("kv4_evict", load_library("kv4_evict").kp_kv4_evict, _ptr(pages), _ptr(mass), _ptr(block_table), block_table.shape[1], _ptr(n_keys),
-         _ptr(new_pages), _ptr(new_mass), _ptr(new_table), new_table.shape[1], _ptr(kept), n, max_keys, keep, recent, first, page_size, G, hd, STREAM)
+    _run("kv4_evict", _fn("kp_kv4_evict"), at, pm, table, block_table.shape[1], keys, new_at, new_pm, new_t, new_table.shape[1], pk, n, max_keys, keep,
+         recent, first, page_size, G, hd, STREAM)
     return kept
