@@ -72,8 +72,16 @@ kv4_write_kernel(const T* __restrict__ k, long long ldk, const T* __restrict__ v
         const float s = __bfloat162float(sb), z = __bfloat162float(zb);
         uint32_t w = 0;
         if (s > 0.f) {
+            // round((x - z) / s): the quotient by the reciprocal is off by a few units of the last place, which matters only where it lies
+            // at a half; there (and for scales whose reciprocal is too large) it is divided.  Adding 2^23 rounds to the even integer.
+            const float inv = __frcp_rn(s);
 #pragma unroll
-            for (int i = 0; i < 8; i++) w |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[u][i] - z, s)), 0.f), 15.f) << (4 * i);
+            for (int i = 0; i < 8; i++) {
+                const float d = x[u][i] - z;
+                float t = fminf(fmaxf(d * inv, 0.f), 15.f), r = t + 8388608.0f;
+                if (s < 1e-30f || fabsf(t - (r - 8388608.0f)) > 0.4999f) r = fminf(fmaxf(__fdiv_rn(d, s), 0.f), 15.f) + 8388608.0f;
+                w |= (__float_as_uint(r) & 15u) << (4 * i);
+            }
         }
         const int ps = 1 << p.ps_log2, page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);
         unsigned char* rec = pages + ((size_t)page * p.G + head) * kv4_page_bytes(ps, p.hd);
@@ -117,7 +125,11 @@ kv4_read_kernel(const unsigned char* __restrict__ pages, const int* __restrict__
         const float s = kv4_scale(r[u]), z = kv4_least(r[u]);
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = fmaf(s, (float)((w[u] >> (4 * i)) & 15u), z);       // (s c is exact)
+        for (int i = 0; i < 8; i++) {
+            // 128 + c as float bits, without a conversion; s c is exact
+            const uint32_t c = i < 4 ? w[u] << (16 - 4 * i) : w[u] >> (4 * i - 16);
+            x[i] = fmaf(s, __uint_as_float((c & 0x000f0000u) | 0x43000000u) - 128.0f, z);
+        }
         T* dst = (is_v ? v : k) + (size_t)row * p.G * p.hd + within * 8;
         if (sizeof(T) == 2) {
             *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
@@ -404,8 +416,9 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
     if (p.n_chunks > 1) kv4_cluster_sync();                // (nobody leaves while another reads its shared memory)
 }
 
+#define KV4_MASS_KEYS 1024                              // keys of a CTA that adds weights up
 // ---- joins the chunks and adds up the mass: a warp a (segment, row, head), in the order of the chunks; behind those CTAs, where
-// there is mass, a CTA a (128 keys, kv head, segment) with a thread a key, rows and heads in order.  Both find a (row, head)'s shift and sum from
+// there is mass, a CTA a (1024 keys, kv head, segment) with a thread a key, rows and heads in order.  Both find a (row, head)'s shift and sum from
 // the chunks' (at most a few dozen), so that neither waits for the other.
 // Largest shift and sum of p of the chunks c_lo .. c_hi of a place; every lane gets them.
 __device__ __forceinline__ float2 kv4_total(const float* ml, int c_lo, int c_hi, int lane) {
@@ -468,14 +481,19 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
     __shared__ float lse[64];                              // of 64 (row, head)s at a time
     const int b = blockIdx.x - n_join, kvh = b / mass_blocks % p.G, seg = b / mass_blocks / p.G;
     const int n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg], pos0 = p.seg_pos[seg], R = p.H / p.G, n_cols = n_rows * R;
-    const int base = kv4_chunk_base(pos0, p.window, kv4_tile_keys(hd)), k0 = base + (b % mass_blocks) * 128, key = k0 + threadIdx.x;
-    if (n_rows > p.max_rows || k0 > pos0 + n_rows - 1 || (p.window > 0 && k0 + 127 <= pos0 - p.window)) return;
+    const int base = kv4_chunk_base(pos0, p.window, kv4_tile_keys(hd)), k0 = base + (b % mass_blocks) * KV4_MASS_KEYS;
     // (in front of the first row's window nothing is read, and the pages may be somebody else's by now)
-    const bool there = key <= pos0 + n_rows - 1 && key < p.max_blocks * p.ps && key - base < p.ld_scores && !(p.window > 0 && key <= pos0 - p.window);
-    float sum = 0.f;
+    const int first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+    const int last = min(min(pos0 + n_rows, p.max_blocks * p.ps), base + p.ld_scores) - 1;
+    if (n_rows > p.max_rows || k0 > last || k0 + KV4_MASS_KEYS - 1 < first) return;
+    constexpr int U = KV4_MASS_KEYS / 128;
+    float sum[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) sum[u] = 0.f;
     for (int c0 = 0; c0 < n_cols; c0 += 64) {
+        const int n = min(64, n_cols - c0);
         __syncthreads();
-        for (int i = threadIdx.x >> 5; i < min(64, n_cols - c0); i += 4) {
+        for (int i = threadIdx.x >> 5; i < n; i += 4) {
             const int r = (c0 + i) / R, h = kvh * R + (c0 + i) % R, hi = pos0 + r;
             const size_t place = ((size_t)seg * p.max_rows + r) * p.H + h;
             float v;
@@ -490,19 +508,23 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
             if (lane == 0) lse[i] = v;
         }
         __syncthreads();
-        if (there) {
-            const int n = min(64, n_cols - c0);
-            for (int i = 0; i < n; i++) {
-                const int r = (c0 + i) / R, hi = pos0 + r;
-                if (key > hi || (p.window > 0 && key <= hi - p.window)) continue;
-                const size_t place = ((size_t)seg * p.max_rows + r) * p.H + kvh * R + (c0 + i) % R;
-                sum += kv4_exp2(p.scores[place * p.ld_scores + key - base] - lse[i]);
+#pragma unroll 2
+        for (int i = 0; i < n; i++) {
+            const int r = (c0 + i) / R, hi = min(pos0 + r, last), lo = p.window > 0 ? max(0, pos0 + r - p.window + 1) : 0;
+            const float* sc = p.scores + (((size_t)seg * p.max_rows + r) * p.H + kvh * R + (c0 + i) % R) * p.ld_scores - base;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int key = k0 + u * 128 + threadIdx.x;
+                if (key >= lo && key <= hi) sum[u] += kv4_exp2(sc[key] - lse[i]);
             }
         }
     }
-    if (there) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int key = k0 + u * 128 + threadIdx.x;
+        if (key < first || key > last) continue;
         const int page = p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)];
-        p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += sum;
+        p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += sum[u];
     }
 }
 
@@ -793,7 +815,7 @@ static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_til
         if (e) return e;
         if (!a.fused && (a.n_chunks > 1 || a.mass)) {
             const long long join = a.n_chunks > 1 ? ((long long)a.n_seg * a.max_rows * a.H + 3) / 4 : 0;
-            const int mass_blocks = a.mass ? (a.n_chunks * a.chunk + 127) / 128 : 0;
+            const int mass_blocks = a.mass ? (a.n_chunks * a.chunk + KV4_MASS_KEYS - 1) / KV4_MASS_KEYS : 0;
             const long long blocks = join + (long long)mass_blocks * a.G * a.n_seg;
             if (blocks > 2147483647LL) return KP_ERR_UNSUPPORTED;
             const cudaError_t c = kp_launch_pdl(kv4_join_kernel<T>, dim3((unsigned)blocks), dim3(128), 0, st, a, HD, (int)join, mass_blocks);
