@@ -6,8 +6,9 @@
 // their keys in tiles of 128:
 //   4 warps turn the codes of a tile into fp16 operands in shared memory, a thread a key;
 //   1 warp issues  S = Q K^T  and  O += P V  (tcgen05.mma, kind::f16; S and O in tensor memory);
-//   2 x 4 warps have a thread a column: S from tensor memory, softmax, P (fp16) to shared memory.
-// While one group is at its exponentials the tensor core works for the other.
+//   2 x 4 warps have a thread a column: S from tensor memory (once for the maximum; half of it stays in registers, the other half is read
+//   again), softmax, P (fp16) to shared memory.
+// The groups run half a tile apart, so that the tensor core works for one while the other is at its exponentials.
 //
 // Exactness.  K's operand is s (c - 8): an 8-bit times a 4-bit number, exact in fp16's 11 bits.  The rest, (z + 8 s) times the
 // query's sum over the group, is 16 more columns of the same product: both factors in two fp16 parts.  So S is off by float32
@@ -33,7 +34,7 @@ struct Kv4TcArgs {
     const unsigned char* pages;
     const int* block_table; int max_blocks;
     const int* cu_rows; const int* seg_pos;
-    float scale; int window; int ps; int H, G;
+    float scale; int window; int ps, ps_log2; int H, G;
     unsigned char* q_image; float2* col;               // with mass: the groups' Q operands and (factor, lse) of their columns
     float* mass;
     int min_rows, n_seg, n_tiles;                      // n_tiles: an upper bound of the CTAs' tiles
@@ -91,9 +92,32 @@ __device__ __forceinline__ int kt_exponent(uint32_t range) {
     const float s = kv4_scale(range), z = kv4_least(range), top = fmaxf(fabsf(z), fabsf(fmaf(15.0f, s, z)));
     return top < INFINITY ? (int)(__float_as_uint(top) >> 23) - 126 : -126;
 }
+// What a thread of the code warps has of its key, or of its value: codes and ranges
+template <int HD>
+struct KtRow {
+    uint4 c[HD / 32];
+    uint32_t r[HD / 64];
+    __device__ __forceinline__ void load(const unsigned char* rec, int off, int ps, bool there, bool value) {
+        constexpr int NG = HD / 64;
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) c[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int y = 0; y < NG; y++) r[y] = 0u;
+        if (!there) return;                            // a key that is not there: zeros, whatever lies in its place
+        const int row = value ? ps + off : off;
+        const uint4* from = reinterpret_cast<const uint4*>(rec + (size_t)row * (HD / 2));
+        const uint32_t* ranges = reinterpret_cast<const uint32_t*>(rec + (size_t)ps * HD) + row * NG;
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) c[i] = from[i];
+#pragma unroll
+        for (int y = 0; y < NG; y++) r[y] = ranges[y];
+    }
+};
 // One row of an operand of the score product: K's codes of a key
 template <int HD>
-__device__ __forceinline__ void kt_write_key(unsigned char* tile, int row, const uint4 (&codes)[HD / 32], const uint32_t (&ranges)[HD / 64], int e) {
+__device__ __forceinline__ void kt_write_key(unsigned char* tile, int row, const KtRow<HD>& x, int e) {
+    const uint4 (&codes)[HD / 32] = x.c;
+    const uint32_t (&ranges)[HD / 64] = x.r;
     const float f = kt_pow2(7 - e);
     uint32_t ext[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -119,16 +143,20 @@ __device__ __forceinline__ void kt_write_key(unsigned char* tile, int row, const
 // and a query (null: zeros).  Returns the factor that makes scores (base 2) of the product with a tile scaled by 2^(7 - e): factor 2^(e - 7).
 template <int HD>
 __device__ __forceinline__ float kt_write_query(unsigned char* tile, int row, const bf16* src, float scale) {
-    float v[HD], top = 0.f;
-#pragma unroll
-    for (int i = 0; i < HD / 8; i++) {
+    auto eight = [&](float (&v)[8], int i) {
         const uint4 x = src ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int j = 0; j < 4; j++) { v[8 * i + 2 * j] = __uint_as_float(w[j] << 16); v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u); }
-    }
+        for (int j = 0; j < 4; j++) { v[2 * j] = kv4_scale(w[j]); v[2 * j + 1] = kv4_least(w[j]); }
+    };
+    float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < HD; i++) top = fmaxf(top, fabsf(v[i]));
+    for (int i = 0; i < HD / 8; i++) {
+        float v[8];
+        eight(v, i);
+#pragma unroll
+        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[j]));
+    }
     int e = 0;
     if (top > 0.f && top < INFINITY) e = min(6 - ilogbf(top), 100);          // the largest value to [2^6, 2^7): a sum of 64 then fits fp16
     const float up = kt_pow2(e);
@@ -138,7 +166,8 @@ __device__ __forceinline__ float kt_write_query(unsigned char* tile, int row, co
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            float* x = v + y * 64 + i * 8;
+            float x[8];
+            eight(x, y * 8 + i);
             uint32_t r[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -169,28 +198,19 @@ __device__ __forceinline__ void kt_issue_s(uint32_t tmem, const unsigned char* a
     kp_umma_bf16(tmem, kt_desc_ext(kp_smem_u32(a + Kt<HD>::TILE)), kt_desc_ext(kp_smem_u32(b + Kt<HD>::TILE)), idesc, 1u);
 }
 
-// What a thread of the code warps has of its key
-template <int HD>
-struct KtKey {
-    uint4 k[HD / 32], v[HD / 32];
-    uint32_t kr[HD / 64], vr[HD / 64];
-    __device__ __forceinline__ void load(const unsigned char* rec, int off, int ps, bool there, bool values) {
-        constexpr int NG = HD / 64;
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int y = 0; y < NG; y++) kr[y] = vr[y] = 0u;
-        if (!there) return;                            // a key that is not there: zeros, whatever lies in its place
-        const uint4* kc = reinterpret_cast<const uint4*>(rec + (size_t)off * (HD / 2));
-        const uint4* vc = reinterpret_cast<const uint4*>(rec + (size_t)(ps + off) * (HD / 2));
-        const uint32_t* r = reinterpret_cast<const uint32_t*>(rec + (size_t)ps * HD);
-#pragma unroll
-        for (int i = 0; i < HD / 32; i++) { k[i] = kc[i]; if (values) v[i] = vc[i]; }
-#pragma unroll
-        for (int y = 0; y < NG; y++) { kr[y] = r[off * NG + y]; if (values) vr[y] = r[(ps + off) * NG + y]; }
-    }
-};
-
+// two float32 operations at once
+__device__ __forceinline__ float2 kt_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 kt_add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
 // segment and first column of a tile of 256 columns (kv4.cu's tiles: the last columns of a segment first); -1: none
 __device__ __forceinline__ void kt_find(const Kv4TcArgs& p, int tile, int R, int lane, int& seg, int& col0) {
     seg = -1; col0 = 0;
@@ -242,8 +262,8 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     uint64_t* p_full = bars + 14; uint64_t* o_done = bars + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* meta = abort_flag + 1;               // [4 tiles][2]: exponents of K's and V's scales
-    volatile int* tops = meta + 8;                     // [2][4 warps][2]
+    volatile int* meta = abort_flag + 1;               // [K's scale, V's][4 tiles]: exponents
+    volatile int* tops = meta + 8;                     // [2][4 warps]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -275,52 +295,59 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     const int kt_lo = k_lo / KT_ROWS, n_kt = k_hi >= k_lo ? k_hi / KT_ROWS - kt_lo + 1 : 0;
 
     if (warp >= 8 && warp < 12) {
-        // ---- codes to operands: thread d has key d of every tile
+        // ---- codes to operands: thread d has key d of every tile.  Keys run two tiles ahead of the values' next: with one stage each K's is
+        // free half a tile before V's.
         const int d = threadIdx.x - 256;
         const int* bt = p.block_table + (size_t)max(seg, 0) * p.max_blocks;
         const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);
         auto page_of = [&](int i) {
             const int key = (kt_lo + i) * KT_ROWS + d;
-            return i < n_kt && key >= k_lo && key <= k_hi ? bt[key / p.ps] : -1;
+            return i < n_kt && key >= k_lo && key <= k_hi ? bt[key >> p.ps_log2] : -1;
         };
-        auto fetch = [&](KtKey<HD>& x, int i, int page) {
+        auto fetch = [&](KtRow<HD>& x, int i, int page, bool value) {
             const int key = (kt_lo + i) * KT_ROWS + d;
-            x.load(p.pages + ((size_t)max(page, 0) * p.G + kvh) * rec, key % p.ps, p.ps, page >= 0, true);
+            x.load(p.pages + ((size_t)max(page, 0) * p.G + kvh) * rec, key & (p.ps - 1), p.ps, page >= 0, value);
+        };
+        // the largest exponent of the tile's groups, of all 128 threads
+        int turn = 0;
+        auto exponent = [&](const KtRow<HD>& x, int e) {
+#pragma unroll
+            for (int y = 0; y < S::NG; y++) e = max(e, kt_exponent(x.r[y]));
+            e = __reduce_max_sync(0xffffffffu, e);
+            volatile int* t = tops + turn * 4;
+            turn ^= 1;
+            if (lane == 0) t[warp & 3] = e;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            return max(max(t[0], t[1]), max(t[2], t[3]));
         };
         bool ok = true;
-        KtKey<HD> now;
-        int page = page_of(1), ev_run = -100;
-        fetch(now, 0, page_of(0));
-#pragma unroll 1
-        for (int i = 0; i < n_kt; i++) {
-            const int st = i % ST, use = i / ST;
-            KtKey<HD> next;
-            fetch(next, i + 1, page);
-            page = page_of(i + 2);
-            int ek = -100, ev = ev_run;
-#pragma unroll
-            for (int y = 0; y < S::NG; y++) { ek = max(ek, kt_exponent(now.kr[y])); ev = max(ev, kt_exponent(now.vr[y])); }
-            ek = __reduce_max_sync(0xffffffffu, ek);
-            ev = __reduce_max_sync(0xffffffffu, ev);
-            volatile int* t = tops + (i & 1) * 8;
-            if (lane == 0) { t[(warp & 3) * 2] = ek; t[(warp & 3) * 2 + 1] = ev; }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            ek = max(max(t[0], t[2]), max(t[4], t[6]));
-            ev_run = max(max(t[1], t[3]), max(t[5], t[7]));
-            if (d == 0) { meta[(i & 3) * 2] = ek; meta[(i & 3) * 2 + 1] = ev_run; }
+        KtRow<HD> key, value;
+        int key_page = page_of(1), value_page = page_of(1), ev = -100;
+        fetch(key, 0, page_of(0), false);
+        fetch(value, 0, page_of(0), true);
+        auto do_key = [&](int i) {
+            const int st = i % ST, use = i / ST, e = exponent(key, -100);
             if (ok && (*abort_flag || !kp_mbar_wait_bounded(&k_empty[st], (use & 1) ^ 1))) ok = false;
-            kt_write_key<HD>(Ks + st * S::OPER, d, now.k, now.kr, ek);
+            if (d == 0) meta[i & 3] = e;
+            kt_write_key<HD>(Ks + st * S::OPER, d, key, e);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             kp_mbar_arrive(&k_full[st]);
-            if (ok && !kp_mbar_wait_bounded(&v_empty[st], (use & 1) ^ 1)) ok = false;
-            const float f = kt_pow2(14 - ev_run);
+            fetch(key, i + 1, key_page, false);
+            key_page = page_of(i + 2);
+        };
+        auto do_value = [&](int i) {
+            const int st = i % ST, use = i / ST;
+            ev = exponent(value, ev);
+            if (ok && (*abort_flag || !kp_mbar_wait_bounded(&v_empty[st], (use & 1) ^ 1))) ok = false;
+            if (d == 0) meta[4 + (i & 3)] = ev;
+            const float f = kt_pow2(14 - ev);
 #pragma unroll
             for (int y = 0; y < S::NG; y++) {
-                const float s = kv4_scale(now.vr[y]) * f, z = fmaf(8.0f, kv4_scale(now.vr[y]), kv4_least(now.vr[y])) * f;
+                const float s = kv4_scale(value.r[y]) * f, z = fmaf(8.0f, kv4_scale(value.r[y]), kv4_least(value.r[y])) * f;
                 const __half2 s2 = __float2half2_rn(s), s16 = __float2half2_rn(s * 0.0625f), z2 = __float2half2_rn(z);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const uint4 c = now.v[2 * y + j];
+                    const uint4 c = value.c[2 * y + j];
                     const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
                     for (int e = 0; e < 4; e++)
@@ -329,42 +356,44 @@ kv4_tc_kernel(const Kv4TcArgs p) {
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             kp_mbar_arrive(&v_full[st]);
-            now = next;
+            fetch(value, i + 1, value_page, true);
+            value_page = page_of(i + 2);
+        };
+        // keys 0, keys 1, values 0, keys 2, values 1, ...: in the order in which the products free their stages
+#pragma unroll 1
+        for (int i = -2; i < n_kt; i++) {
+            if (i + 2 < n_kt) do_key(i + 2);
+            if (i + 1 >= 0 && i + 1 < n_kt) do_value(i + 1);
         }
         if (__builtin_expect(!ok, 0)) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
     } else if (warp == 12) {
         // ---- the tensor core's work
         if (lane == 0 && n_kt > 0) {
             constexpr uint32_t idesc_pv = kt_idesc(128, HD, true);
-            bool ok = kp_mbar_wait_bounded(&q_full[0], 0) && kp_mbar_wait_bounded(&q_full[1], 0);
-            auto issue_s_both = [&](int i) {
+            auto issue_s = [&](int i, int g) {
                 if (!kp_mbar_wait_bounded(&k_full[i % ST], (i / ST) & 1)) return false;
-                for (int g = 0; g < 2; g++) {
-                    if (i > 0 && !kp_mbar_wait_bounded(&s_free[g], (i - 1) & 1)) return false;
-                    kp_tc_fence_after();
-                    kt_issue_s<HD>(tmem_base + 128 * g, Qs + g * S::OPER, Ks + (i % ST) * S::OPER);
-                    kp_umma_commit(&s_full[g]);
-                }
-                kp_umma_commit(&k_empty[i % ST]);
+                if (i > 0 && !kp_mbar_wait_bounded(&s_free[g], (i - 1) & 1)) return false;
+                kp_tc_fence_after();
+                kt_issue_s<HD>(tmem_base + 128 * g, Qs + g * S::OPER, Ks + (i % ST) * S::OPER);
+                kp_umma_commit(&s_full[g]);
+                if (g == 1) kp_umma_commit(&k_empty[i % ST]);
                 return true;
             };
-            if (ok) ok = issue_s_both(0);
-            for (int i = 0; i < n_kt && ok; i++) {
-                if (i + 1 < n_kt && !issue_s_both(i + 1)) { ok = false; break; }
-                if (!kp_mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1)) { ok = false; break; }
-                const uint32_t va = kp_smem_u32(Vs + (i % ST) * S::TILE);
-                for (int g = 0; g < 2 && ok; g++) {
-                    if (!kp_mbar_wait_bounded(&p_full[g], i & 1)) { ok = false; break; }
-                    kp_tc_fence_after();
-                    const uint32_t pa = kp_smem_u32(Ps + g * S::PV);
+            auto issue_pv = [&](int i, int g) {
+                if (!kp_mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1) || !kp_mbar_wait_bounded(&p_full[g], i & 1)) return false;
+                kp_tc_fence_after();
+                const uint32_t va = kp_smem_u32(Vs + (i % ST) * S::TILE), pa = kp_smem_u32(Ps + g * S::PV);
 #pragma unroll
-                    for (int kk = 0; kk < KT_ROWS / 16; kk++)
-                        kp_umma_bf16(tmem_base + 256 + HD * g, kp_umma_desc(pa + (kk >> 2) * 16384) + 2 * (kk & 3),
-                                     HD == 64 ? kp_umma_desc(va + kk * 2048) : kp_umma_desc_mn(va + kk * 2048, 16384), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
-                    kp_umma_commit(&o_done[g]);
-                }
-                if (ok) kp_umma_commit(&v_empty[i % ST]);
-            }
+                for (int kk = 0; kk < KT_ROWS / 16; kk++)
+                    kp_umma_bf16(tmem_base + 256 + HD * g, kp_umma_desc(pa + (kk >> 2) * 16384) + 2 * (kk & 3),
+                                 HD == 64 ? kp_umma_desc(va + kk * 2048) : kp_umma_desc_mn(va + kk * 2048, 16384), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+                kp_umma_commit(&o_done[g]);
+                if (g == 1) kp_umma_commit(&v_empty[i % ST]);
+                return true;
+            };
+            bool ok = kp_mbar_wait_bounded(&q_full[0], 0) && issue_s(0, 0) && kp_mbar_wait_bounded(&q_full[1], 0) && issue_s(0, 1);
+            for (int i = 0; i < n_kt && ok; i++)
+                for (int g = 0; g < 2 && ok; g++) ok = (i + 1 >= n_kt || issue_s(i + 1, g)) && issue_pv(i, g);
             if (!ok) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
         }
     } else {
@@ -407,90 +436,89 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         for (int i = 0; i < n_kt; i++) {
             if (ok && (*abort_flag || !kp_mbar_wait_bounded(&s_full[g], i & 1))) ok = false;
             kp_tc_fence_after();
-            uint32_t s0[32], s1[32];
-            kp_tmem_ld32_issue(tmem_s, s0);
-            kp_tmem_ld32_issue(tmem_s + 32, s1);
             const int key0 = (kt_lo + i) * KT_ROWS;
             const bool masked = !(key0 + KT_ROWS - 1 <= all_hi && key0 >= all_lo);
-            const float fk = f * kt_pow2(meta[(i & 3) * 2] - 7);
-            const int ev_now = meta[(i & 3) * 2 + 1];
-            float tmax = -INFINITY;
-            auto max32 = [&](const uint32_t (&s)[32], int at) {
+            const float fk = fmaxf(f * kt_pow2(meta[i & 3] - 7), 1.17549435e-38f);     // (not 0: a masked score stays -inf)
+            uint32_t s[2][32], w[32];
+            auto load = [&](int at) {                                            // 64 scores; one that is not there: the lowest value
+                kp_tmem_ld32_issue(tmem_s + at, s[0]);
+                kp_tmem_ld32_issue(tmem_s + at + 32, s[1]);
+                kp_tmem_ld_wait();
                 if (masked) {
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (key0 + at + j >= lo && key0 + at + j <= pos) tmax = fmaxf(tmax, __uint_as_float(s[j]));
-                } else {
+                    for (int e = 0; e < 2; e++)
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) tmax = kt_max3(tmax, __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
+                        for (int j = 0; j < 32; j++)
+                            if (!(key0 + at + e * 32 + j >= lo && key0 + at + e * 32 + j <= pos)) s[e][j] = 0xff800000u;
                 }
             };
-            kp_tmem_ld_wait();
-            max32(s0, 0); max32(s1, 32);
-            kp_tmem_ld32_issue(tmem_s + 64, s0);
-            kp_tmem_ld32_issue(tmem_s + 96, s1);
-            kp_tmem_ld_wait();
-            max32(s0, 64); max32(s1, 96);
-            const float top = tmax * fk;
+            auto largest = [&] {
+                float t[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    t[e] = fmaxf(__uint_as_float(s[e][0]), __uint_as_float(s[e][1]));
+#pragma unroll
+                    for (int j = 2; j < 32; j += 2) t[e] = kt_max3(t[e], __uint_as_float(s[e][j]), __uint_as_float(s[e][j + 1]));
+                }
+                return fmaxf(t[0], t[1]);
+            };
+            load(0);
+            float top = largest();
+            load(64);
+            top = fmaxf(top, largest()) * fk;
             const float m_new = top > m + 8.0f ? top : m;                        // (the first: m = -inf)
             const float corr_l = m_new == m ? 1.0f : kv4_exp2(m - m_new);
-            const float corr_o = corr_l * kt_pow2(ev - ev_now);
             const float sub = m_new == -INFINITY ? 0.f : m_new - 7.0f;
-            if (i > 0) {
-                // the product of the tile before has read P and added to O
-                if (ok && !kp_mbar_wait_bounded(&o_done[g], (i - 1) & 1)) ok = false;
-                if (__any_sync(0xffffffffu, corr_o != 1.0f)) {
-                    kp_tc_fence_after();
-#pragma unroll 1
-                    for (int e = 0; e < HD; e += 16) {
-                        uint32_t v[16];
-                        kp_tmem_ld16_issue(tmem_o + e, v);
-                        kp_tmem_ld_wait();
+            const float2 fk2 = make_float2(fk, fk), sub2 = make_float2(-sub, -sub);
+            float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            auto weights = [&] {                                                 // of the 64 loaded scores, packed
 #pragma unroll
-                        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr_o);
-                        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-                                     ::"r"(tmem_o + e), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-                                     "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float2 x = kt_fma2(make_float2(__uint_as_float(s[e][j]), __uint_as_float(s[e][j + 1])), fk2, sub2);
+                        x.x = kv4_exp2(x.x);
+                        x.y = kv4_exp2(x.y);
+                        sums[e] = kt_add2(sums[e], x);
+                        w[e * 16 + (j >> 1)] = pack_f16(x.x, x.y);
                     }
-                    kp_tmem_st_wait();
-                }
-            }
-            float lsum = 0.f;
-            auto p32 = [&](const uint32_t (&s)[32], int at, auto masked_c) {
-                constexpr bool MASKED = decltype(masked_c)::value;
-#pragma unroll
-                for (int j8 = 0; j8 < 4; j8++) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int j2 = 0; j2 < 4; j2++) {
-                        float pv[2];
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const int j = j8 * 8 + j2 * 2 + e;
-                            pv[e] = kv4_exp2(fmaf(__uint_as_float(s[j]), fk, -sub));
-                            if (MASKED && !(key0 + at + j >= lo && key0 + at + j <= pos)) pv[e] = 0.f;
-                        }
-                        lsum += pv[0] + pv[1];
-                        w[j2] = pack_f16(pv[0], pv[1]);
-                    }
-                    *reinterpret_cast<uint4*>(Pg + (at >> 6) * 16384 + (((((at & 63) >> 3) + j8) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
             };
-            if (masked) { p32(s0, 64, std::true_type{}); p32(s1, 96, std::true_type{}); }
-            else { p32(s0, 64, std::false_type{}); p32(s1, 96, std::false_type{}); }
-            kp_tmem_ld32_issue(tmem_s, s0);
-            kp_tmem_ld32_issue(tmem_s + 32, s1);
-            kp_tmem_ld_wait();
+            auto store = [&](int half) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    *reinterpret_cast<uint4*>(Pg + half * 16384 + ((j ^ (r & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+            };
+            weights();
+            // the product of the tile before has read P and added to O; this tile's values are there
+            if (i > 0 && ok && !kp_mbar_wait_bounded(&o_done[g], (i - 1) & 1)) ok = false;
+            if (ok && !kp_mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1)) ok = false;
+            const int ev_now = meta[4 + (i & 3)];
+            const float corr_o = corr_l * kt_pow2(ev - ev_now);
+            if (i > 0 && __any_sync(0xffffffffu, corr_o != 1.0f)) {
+                kp_tc_fence_after();
+#pragma unroll 1
+                for (int e = 0; e < HD; e += 32) {
+                    uint32_t v[32];
+                    kp_tmem_ld32(tmem_o + e, v);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr_o);
+                    kp_tmem_st32(tmem_o + e, v);
+                }
+                kp_tmem_st_wait();
+                kp_tc_fence_before();                                            // O is written
+            }
+            store(1);
+            load(0);
             kp_tc_fence_before();
             kp_mbar_arrive(&s_free[g]);                                          // the next tile's S may be computed
-            if (masked) { p32(s0, 0, std::true_type{}); p32(s1, 32, std::true_type{}); }
-            else { p32(s0, 0, std::false_type{}); p32(s1, 32, std::false_type{}); }
-            l = l * corr_l + lsum;
-            m = m_new;
-            ev = ev_now;
-            kp_tc_fence_before();                                                // O (if rescaled) is written
+            weights();
+            store(0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // P is read by the tensor core
             kp_mbar_arrive(&p_full[g]);
+            const float2 total = kt_add2(sums[0], sums[1]);
+            l = l * corr_l + (total.x + total.y);
+            m = m_new;
+            ev = ev_now;
         }
         if (n_kt > 0 && ok && !kp_mbar_wait_bounded(&o_done[g], (n_kt - 1) & 1)) ok = false;
         kp_tc_fence_after();
@@ -519,6 +547,34 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     kp_tc_fence_before();
     __syncthreads();
     if (warp == 12) kp_tmem_dealloc(tmem_base, 512);
+}
+
+// The sum of 2^(score - lse) over the 128 columns of a tile, of those from lo to hi (MASKED), for this thread's key: S of tensor memory
+// times kappa and the column's factor is the score.
+template <bool MASKED>
+__device__ __forceinline__ float kt_column_sum(uint32_t tmem_s, const float4* col, float kappa, int lo, int hi) {
+    float part = 0.f;
+    const float2 k2 = make_float2(kappa, kappa);
+#pragma unroll 1
+    for (int e = 0; e < 128; e += 32) {
+        uint32_t s[32];
+        kp_tmem_ld32(tmem_s + e, s);
+        float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+            const float4 f = col[(e + j) >> 1];            // (factor, lse) of two columns
+            float2 x = kt_fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), k2, make_float2(0.f, 0.f));
+            x = make_float2(kv4_exp2(fmaf(x.x, f.x, -f.y)), kv4_exp2(fmaf(x.y, f.z, -f.w)));
+            if (MASKED) {
+                if (e + j < lo || e + j > hi) x.x = 0.f;
+                if (e + j + 1 < lo || e + j + 1 > hi) x.y = 0.f;
+            }
+            a[(j >> 1) & 1] = kt_add2(a[(j >> 1) & 1], x);
+        }
+        const float2 t = kt_add2(a[0], a[1]);
+        part += t.x + t.y;
+    }
+    return part;
 }
 
 // ---- mass.  One CTA per (128 keys, kv head, segment): S^T = K Q^T with a thread a key, so that a key's weights add up in its
@@ -569,17 +625,17 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     if (warp >= 8 && warp < 12) {
         const int d = threadIdx.x - 256, key = k0 + d;
         const bool there = work && key >= first && key <= last;
-        const int page = there ? p.block_table[(size_t)seg * p.max_blocks + key / p.ps] : 0;
-        KtKey<HD> x;
-        x.load(p.pages + ((size_t)page * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key % p.ps, p.ps, there, false);
+        const int page = there ? p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)] : 0;
+        KtRow<HD> x;
+        x.load(p.pages + ((size_t)page * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key & (p.ps - 1), p.ps, there, false);
         int ek = -100;
 #pragma unroll
-        for (int y = 0; y < S::NG; y++) ek = max(ek, kt_exponent(x.kr[y]));
+        for (int y = 0; y < S::NG; y++) ek = max(ek, kt_exponent(x.r[y]));
         ek = __reduce_max_sync(0xffffffffu, ek);
         if (lane == 0) tops[warp & 3] = ek;
         asm volatile("bar.sync 1, 128;" ::: "memory");
         ek = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-        kt_write_key<HD>(Ks, d, x.k, x.kr, ek);
+        kt_write_key<HD>(Ks, d, x, ek);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kp_mbar_arrive(k_full);
         if (d == 0) {
@@ -628,25 +684,8 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
             const float4* col = reinterpret_cast<const float4*>(Qs + st * S::IMAGE + S::OPER);
             const int c0 = (j_lo + i) * 128;
             const bool masked = __any_sync(0xffffffffu, c0 < mine_lo || c0 + 127 > mine_hi);
-            float part = 0.f;
-#pragma unroll 1
-            for (int e = 0; e < 128; e += 32) {
-                uint32_t s[32];
-                kp_tmem_ld32(tmem_base + (2 * g + b) * 128 + lane_off + e, s);
-                float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-                for (int j = 0; j < 32; j += 2) {
-                    const float4 f = col[(e + j) >> 1];                          // (factor, lse) of two columns
-                    float p0 = kv4_exp2(fmaf(__uint_as_float(s[j]) * kappa, f.x, -f.y));
-                    float p1 = kv4_exp2(fmaf(__uint_as_float(s[j + 1]) * kappa, f.z, -f.w));
-                    if (masked) {
-                        if (!(c0 + e + j >= mine_lo && c0 + e + j <= mine_hi)) p0 = 0.f;
-                        if (!(c0 + e + j + 1 >= mine_lo && c0 + e + j + 1 <= mine_hi)) p1 = 0.f;
-                    }
-                    a0 += p0; a1 += p1;
-                }
-                part += a0 + a1;
-            }
+            const uint32_t tmem_s = tmem_base + (2 * g + b) * 128 + lane_off;
+            const float part = masked ? kt_column_sum<true>(tmem_s, col, kappa, mine_lo - c0, mine_hi - c0) : kt_column_sum<false>(tmem_s, col, kappa, 0, 127);
             kp_tc_fence_before();
             kp_mbar_arrive(&s_free[2 * g + b]);
             kp_mbar_arrive(&q_empty[st]);
@@ -663,8 +702,8 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     if (warp < 4 && n_j > 0) {
         const int key = k0 + threadIdx.x;
         if (key >= first && key <= last) {
-            const int page = p.block_table[(size_t)seg * p.max_blocks + key / p.ps];
-            p.mass[((size_t)page * p.G + kvh) * p.ps + key % p.ps] += sum + join[threadIdx.x];
+            const int page = p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)];
+            p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += sum + join[threadIdx.x];
         }
     }
 }
@@ -707,7 +746,9 @@ int kp_kv4_attention_tc(const void* q, long long ldq, const void* pages, const i
     Kv4TcArgs a = {};
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo; a.pages = (const unsigned char*)pages;
     a.block_table = block_table; a.max_blocks = max_blocks; a.cu_rows = cu_rows; a.seg_pos = seg_pos;
-    a.scale = scale; a.window = window; a.ps = ps; a.H = H; a.G = G; a.mass = mass; a.min_rows = min_rows; a.n_seg = n_seg; a.n_tiles = (int)tiles;
+    a.scale = scale; a.window = window; a.ps = ps; a.H = H;
+    while ((1 << a.ps_log2) < ps) a.ps_log2++;
+    a.G = G; a.mass = mass; a.min_rows = min_rows; a.n_seg = n_seg; a.n_tiles = (int)tiles;
     if (mass) {
         a.q_image = (unsigned char*)scratch;
         a.col = (float2*)((unsigned char*)scratch + (size_t)tiles * G * 2 * ((hd / 64) * 16384 + KT_EXT));
