@@ -185,18 +185,18 @@ __device__ __forceinline__ float kt_write_query(unsigned char* tile, int row, co
     *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 1)) = make_uint4(0u, 0u, 0u, 0u);
     return scale * KV4_LOG2E * kt_pow2(-e);
 }
-// S of 128 x 128 (one thread issues)
+// S of 128 x 128.  A warp in step issues it, by an elected lane: from inside a branch that one lane took, the operands would pass through general
+// registers, at three times the cycles an MMA.
 template <int HD>
 __device__ __forceinline__ void kt_issue_s(uint32_t tmem, const unsigned char* a, const unsigned char* b) {
     constexpr uint32_t idesc = kt_idesc(128, 128, false);
 #pragma unroll
-    for (int y = 0; y < HD / 64; y++) {
-        const uint64_t ad = kp_umma_desc(kp_smem_u32(a + y * 16384)), bd = kp_umma_desc(kp_smem_u32(b + y * 16384));
-#pragma unroll
-        for (int k = 0; k < 4; k++) kp_umma_bf16(tmem, ad + 2 * k, bd + 2 * k, idesc, (y | k) ? 1u : 0u);
-    }
-    kp_umma_bf16(tmem, kt_desc_ext(kp_smem_u32(a + Kt<HD>::TILE)), kt_desc_ext(kp_smem_u32(b + Kt<HD>::TILE)), idesc, 1u);
+    for (int y = 0; y < HD / 64; y++)
+        kp_umma_bf16_box(tmem, kp_umma_desc(kp_smem_u32(a + y * 16384)), kp_umma_desc(kp_smem_u32(b + y * 16384)), idesc, y > 0);
+    kp_umma_bf16_warp(tmem, kt_desc_ext(kp_smem_u32(a + Kt<HD>::TILE)), kt_desc_ext(kp_smem_u32(b + Kt<HD>::TILE)), idesc, 1u);
 }
+// a wait of a warp in step, which gives up as one
+__device__ __forceinline__ bool kt_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kp_mbar_wait_bounded(bar, parity)); }
 
 // two float32 operations at once
 __device__ __forceinline__ float2 kt_fma2(float2 a, float2 b, float2 c) {
@@ -368,33 +368,32 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         if (__builtin_expect(!ok, 0)) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
     } else if (warp == 12) {
         // ---- the tensor core's work
-        if (lane == 0 && n_kt > 0) {
+        if (n_kt > 0) {
             constexpr uint32_t idesc_pv = kt_idesc(128, HD, true);
             auto issue_s = [&](int i, int g) {
-                if (!kp_mbar_wait_bounded(&k_full[i % ST], (i / ST) & 1)) return false;
-                if (i > 0 && !kp_mbar_wait_bounded(&s_free[g], (i - 1) & 1)) return false;
+                if (!kt_wait(&k_full[i % ST], (i / ST) & 1) || (i > 0 && !kt_wait(&s_free[g], (i - 1) & 1))) return false;
                 kp_tc_fence_after();
                 kt_issue_s<HD>(tmem_base + 128 * g, Qs + g * S::OPER, Ks + (i % ST) * S::OPER);
-                kp_umma_commit(&s_full[g]);
-                if (g == 1) kp_umma_commit(&k_empty[i % ST]);
+                kp_umma_commit_warp(&s_full[g]);
+                if (g == 1) kp_umma_commit_warp(&k_empty[i % ST]);
                 return true;
             };
             auto issue_pv = [&](int i, int g) {
-                if (!kp_mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1) || !kp_mbar_wait_bounded(&p_full[g], i & 1)) return false;
+                if (!kt_wait(&v_full[i % ST], (i / ST) & 1) || !kt_wait(&p_full[g], i & 1)) return false;
                 kp_tc_fence_after();
                 const uint32_t va = kp_smem_u32(Vs + (i % ST) * S::TILE), pa = kp_smem_u32(Ps + g * S::PV);
 #pragma unroll
                 for (int kk = 0; kk < KT_ROWS / 16; kk++)
-                    kp_umma_bf16(tmem_base + 256 + HD * g, kp_umma_desc(pa + (kk >> 2) * 16384) + 2 * (kk & 3),
-                                 HD == 64 ? kp_umma_desc(va + kk * 2048) : kp_umma_desc_mn(va + kk * 2048, 16384), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
-                kp_umma_commit(&o_done[g]);
-                if (g == 1) kp_umma_commit(&v_empty[i % ST]);
+                    kp_umma_bf16_warp(tmem_base + 256 + HD * g, kp_umma_desc(pa + (kk >> 2) * 16384) + 2 * (kk & 3),
+                                      HD == 64 ? kp_umma_desc(va + kk * 2048) : kp_umma_desc_mn(va + kk * 2048, 16384), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+                kp_umma_commit_warp(&o_done[g]);
+                if (g == 1) kp_umma_commit_warp(&v_empty[i % ST]);
                 return true;
             };
-            bool ok = kp_mbar_wait_bounded(&q_full[0], 0) && issue_s(0, 0) && kp_mbar_wait_bounded(&q_full[1], 0) && issue_s(0, 1);
+            bool ok = kt_wait(&q_full[0], 0) && issue_s(0, 0) && kt_wait(&q_full[1], 0) && issue_s(0, 1);
             for (int i = 0; i < n_kt && ok; i++)
                 for (int g = 0; g < 2 && ok; g++) ok = (i + 1 >= n_kt || issue_s(i + 1, g)) && issue_pv(i, g);
-            if (!ok) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+            if (!ok && lane == 0) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
         }
     } else {
         // ---- the columns: warps 0-3 group 0, warps 4-7 group 1; thread r of a group has column r
@@ -652,18 +651,18 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
             if (*abort_flag) kp_linger_after_failure();      // copies may still be under way
         }
     } else if (warp == 12) {
-        if (lane == 0 && n_j > 0) {
-            bool ok = kp_mbar_wait_bounded(k_full, 0);
+        if (n_j > 0) {
+            bool ok = kt_wait(k_full, 0);
             for (int i = 0; i < n_j && ok; i++) {
                 const int st = i % QST, g = i & 1, b = (i >> 1) & 1, use = i >> 2;       // S buffer (g, b) for the use-th time
-                ok = kp_mbar_wait_bounded(&q_full[st], (i / QST) & 1) && kp_mbar_wait_bounded(&s_free[2 * g + b], (use & 1) ^ 1);
+                ok = kt_wait(&q_full[st], (i / QST) & 1) && kt_wait(&s_free[2 * g + b], (use & 1) ^ 1);
                 if (!ok) break;
                 kp_tc_fence_after();
                 kt_issue_s<HD>(tmem_base + (2 * g + b) * 128, Ks, Qs + st * S::IMAGE);
-                kp_umma_commit(&s_full[2 * g + b]);
-                kp_umma_commit(&q_empty[st]);
+                kp_umma_commit_warp(&s_full[2 * g + b]);
+                kp_umma_commit_warp(&q_empty[st]);
             }
-            if (!ok) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+            if (!ok && lane == 0) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
         }
     } else {
         const int g = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane, key = k0 + r;
