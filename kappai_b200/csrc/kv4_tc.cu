@@ -7,8 +7,10 @@
 //   4 warps turn the codes of a tile into fp16 operands in shared memory, a thread a key;
 //   1 warp issues  S = Q K^T  and  O += P V  (tcgen05.mma, kind::f16; S and O in tensor memory);
 //   2 x 4 warps have a thread a column: S from tensor memory (once for the maximum; half of it stays in registers, the other half is read
-//   again), softmax, P (fp16) to shared memory.
-// The groups run half a tile apart, so that the tensor core works for one while the other is at its exponentials.
+//   again), softmax, P (fp16) back to tensor memory, where it is the A operand of the second product.
+// The groups run half a tile apart, so that the tensor core works for one while the other is at its exponentials.  P through shared
+// memory made that memory's bandwidth the bound (a product with both operands there reads 128 bytes a cycle, all there is).  With heads
+// of 128 tensor memory has no room for P beside S and O: it takes the half of S that has been read.
 //
 // Exactness.  K's operand is s (c - 8): an 8-bit times a 4-bit number, exact in fp16's 11 bits.  The rest, (z + 8 s) times the
 // query's sum over the group, is 16 more columns of the same product: both factors in two fp16 parts.  So S is off by float32
@@ -42,9 +44,10 @@ struct Kv4TcArgs {
 
 template <int HD>
 struct Kt {
-    static constexpr int NG = HD / 64, TILE = NG * 16384, OPER = TILE + KT_EXT, ST = HD == 64 ? 2 : 1;
-    static constexpr int PV = 2 * 16384;               // P of a group: keys 0..63 | keys 64..127
-    static constexpr size_t SMEM = 1024 + 2 * OPER + ST * OPER + ST * TILE + 2 * PV + 512;
+    static constexpr int NG = HD / 64, TILE = NG * 16384, OPER = TILE + KT_EXT, ST = 2;
+    static constexpr bool ALIAS = HD == 128;           // P lies in S's columns 64..127, not in columns of its own
+    static constexpr int S_COL = 0, O_COL = 256, P_COL = ALIAS ? 64 : 256 + 2 * HD, P_STEP = ALIAS ? 128 : 64;   // columns of tensor memory (of group 0)
+    static constexpr size_t SMEM = 1024 + 2 * OPER + ST * OPER + ST * TILE + 512;
     static constexpr int THREADS = 416;
     // the pass that adds up the mass: one K tile, a ring of Q images
     static constexpr int QST = 3, IMAGE = OPER + 1024; // an image in shared memory, and (factor, lse) of its columns
@@ -195,6 +198,12 @@ __device__ __forceinline__ void kt_issue_s(uint32_t tmem, const unsigned char* a
         kp_umma_bf16_box(tmem, kp_umma_desc(kp_smem_u32(a + y * 16384)), kp_umma_desc(kp_smem_u32(b + y * 16384)), idesc, y > 0);
     kp_umma_bf16_warp(tmem, kt_desc_ext(kp_smem_u32(a + Kt<HD>::TILE)), kt_desc_ext(kp_smem_u32(b + Kt<HD>::TILE)), idesc, 1u);
 }
+// D += A B with A in tensor memory (a lane a row, a column two consecutive elements), by an elected lane of a warp in step
+__device__ __forceinline__ void kt_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
+                 ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u) : "memory");
+}
 // a wait of a warp in step, which gives up as one
 __device__ __forceinline__ bool kt_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kp_mbar_wait_bounded(bar, parity)); }
 
@@ -253,8 +262,7 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     unsigned char* Qs = sm;                            // [2] OPER
     unsigned char* Ks = Qs + 2 * S::OPER;              // [ST] OPER
     unsigned char* Vs = Ks + ST * S::OPER;             // [ST] TILE
-    unsigned char* Ps = Vs + ST * S::TILE;             // [2] PV
-    uint64_t* bars = reinterpret_cast<uint64_t*>(Ps + 2 * S::PV);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(Vs + ST * S::TILE);
     uint64_t* q_full = bars;                           // [2] each, by group or by stage
     uint64_t* k_full = bars + 2; uint64_t* k_empty = bars + 4;
     uint64_t* v_full = bars + 6; uint64_t* v_empty = bars + 8;
@@ -371,9 +379,9 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         if (n_kt > 0) {
             constexpr uint32_t idesc_pv = kt_idesc(128, HD, true);
             auto issue_s = [&](int i, int g) {
-                if (!kt_wait(&k_full[i % ST], (i / ST) & 1) || (i > 0 && !kt_wait(&s_free[g], (i - 1) & 1))) return false;
+                if (!kt_wait(&k_full[i % ST], (i / ST) & 1) || (!S::ALIAS && i > 0 && !kt_wait(&s_free[g], (i - 1) & 1))) return false;
                 kp_tc_fence_after();
-                kt_issue_s<HD>(tmem_base + 128 * g, Qs + g * S::OPER, Ks + (i % ST) * S::OPER);
+                kt_issue_s<HD>(tmem_base + S::S_COL + 128 * g, Qs + g * S::OPER, Ks + (i % ST) * S::OPER);
                 kp_umma_commit_warp(&s_full[g]);
                 if (g == 1) kp_umma_commit_warp(&k_empty[i % ST]);
                 return true;
@@ -381,18 +389,22 @@ kv4_tc_kernel(const Kv4TcArgs p) {
             auto issue_pv = [&](int i, int g) {
                 if (!kt_wait(&v_full[i % ST], (i / ST) & 1) || !kt_wait(&p_full[g], i & 1)) return false;
                 kp_tc_fence_after();
-                const uint32_t va = kp_smem_u32(Vs + (i % ST) * S::TILE), pa = kp_smem_u32(Ps + g * S::PV);
+                const uint32_t va = kp_smem_u32(Vs + (i % ST) * S::TILE);
 #pragma unroll
                 for (int kk = 0; kk < KT_ROWS / 16; kk++)
-                    kp_umma_bf16_warp(tmem_base + 256 + HD * g, kp_umma_desc(pa + (kk >> 2) * 16384) + 2 * (kk & 3),
-                                      HD == 64 ? kp_umma_desc(va + kk * 2048) : kp_umma_desc_mn(va + kk * 2048, 16384), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+                    kt_umma_ts(tmem_base + S::O_COL + HD * g, tmem_base + S::P_COL + S::P_STEP * g + 8 * kk,
+                               HD == 64 ? kp_umma_desc(va + kk * 2048) : kp_umma_desc_mn(va + kk * 2048, 16384), idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
                 kp_umma_commit_warp(&o_done[g]);
                 if (g == 1) kp_umma_commit_warp(&v_empty[i % ST]);
                 return true;
             };
             bool ok = kt_wait(&q_full[0], 0) && issue_s(0, 0) && kt_wait(&q_full[1], 0) && issue_s(0, 1);
+            // (a group's products run in the order in which they are issued: where P lies in S, the next S comes behind the product that reads it)
             for (int i = 0; i < n_kt && ok; i++)
-                for (int g = 0; g < 2 && ok; g++) ok = (i + 1 >= n_kt || issue_s(i + 1, g)) && issue_pv(i, g);
+                for (int g = 0; g < 2 && ok; g++) {
+                    const bool more = i + 1 < n_kt;
+                    ok = S::ALIAS ? issue_pv(i, g) && (!more || issue_s(i + 1, g)) : (!more || issue_s(i + 1, g)) && issue_pv(i, g);
+                }
             if (!ok && lane == 0) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
         }
     } else {
@@ -426,8 +438,8 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         const int all_hi = cta_col0 + g * 128 + 127 < n_cols ? min(pos0 + g_first / R, k_hi) : -1;
         const int all_lo = p.window > 0 ? max(0, pos0 + g_last / R - p.window + 1) : 0;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
-        const uint32_t tmem_s = tmem_base + 128 * g + lane_off, tmem_o = tmem_base + 256 + HD * g + lane_off;
-        unsigned char* Pg = Ps + g * S::PV + r * 128;
+        const uint32_t tmem_s = tmem_base + S::S_COL + 128 * g + lane_off, tmem_o = tmem_base + S::O_COL + HD * g + lane_off;
+        const uint32_t tmem_p = tmem_base + S::P_COL + S::P_STEP * g + lane_off;
         bool ok = true;
         float m = -INFINITY, l = 0.f;
         int ev = -100;
@@ -482,14 +494,9 @@ kv4_tc_kernel(const Kv4TcArgs p) {
                         w[e * 16 + (j >> 1)] = pack_f16(x.x, x.y);
                     }
             };
-            auto store = [&](int half) {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    *reinterpret_cast<uint4*>(Pg + half * 16384 + ((j ^ (r & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-            };
             weights();
-            // the product of the tile before has read P and added to O; this tile's values are there
-            if (i > 0 && ok && !kp_mbar_wait_bounded(&o_done[g], (i - 1) & 1)) ok = false;
+            // the product of the tile before has read P and added to O (known from S where P lies in it); this tile's values are there
+            if (!S::ALIAS && i > 0 && ok && !kp_mbar_wait_bounded(&o_done[g], (i - 1) & 1)) ok = false;
             if (ok && !kp_mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1)) ok = false;
             const int ev_now = meta[4 + (i & 3)];
             const float corr_o = corr_l * kt_pow2(ev - ev_now);
@@ -503,17 +510,18 @@ kv4_tc_kernel(const Kv4TcArgs p) {
                     for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * corr_o);
                     kp_tmem_st32(tmem_o + e, v);
                 }
-                kp_tmem_st_wait();
-                kp_tc_fence_before();                                            // O is written
             }
-            store(1);
+            kp_tmem_st32(tmem_p + 32, w);
             load(0);
-            kp_tc_fence_before();
-            kp_mbar_arrive(&s_free[g]);                                          // the next tile's S may be computed
+            if (!S::ALIAS) {
+                kp_tc_fence_before();
+                kp_mbar_arrive(&s_free[g]);                                      // the next tile's S may be computed
+            }
             weights();
-            store(0);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // P is read by the tensor core
-            kp_mbar_arrive(&p_full[g]);
+            kp_tmem_st32(tmem_p, w);
+            kp_tmem_st_wait();
+            kp_tc_fence_before();
+            kp_mbar_arrive(&p_full[g]);                                          // P, and O where it was rescaled, are written
             const float2 total = kt_add2(sums[0], sums[1]);
             l = l * corr_l + (total.x + total.y);
             m = m_new;
