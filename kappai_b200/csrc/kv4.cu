@@ -637,7 +637,7 @@ kv4_tiled_kernel(const Kv4Args p) {
             if (c >= n_cols) continue;
             const size_t row = row0 + c / R;
             const int h = kvh * R + c % R;
-            const bool none = A.m[nt][i] == -INFINITY;
+            const bool none = A.shift[nt][i] == -INFINITY;
             const float inv = none ? 0.f : 1.0f / A.l[nt][i];
             T* dst = (T*)p.out + row * p.ldo + (size_t)h * HD;
 #pragma unroll

@@ -365,7 +365,8 @@ struct Kv4Acc {
                 for (int j = 0; j < HD / 16; j++) { o[nt][j][i] *= corr; o[nt][j][2 + i] *= corr; }
             }
     }
-    // Behind the last key: the threads' shares of the sums are added up (all get them).
+    // Behind the last key: the threads' shares of the sums are added up (all get them).  A column without a key has the shift -inf then; one
+    // whose scores are all NaN has not.
     __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -377,6 +378,7 @@ struct Kv4Acc {
 #pragma unroll
                     for (int y = 0; y < Kv4<HD>::NG; y++) z[nt][y][i] += __shfl_xor_sync(0xffffffffu, z[nt][y][i], d);
                 }
+                if (l[nt][i] != l[nt][i] && shift[nt][i] == -INFINITY) shift[nt][i] = 0.f;
             }
     }
     // value of dimension pair (d, d + 1), d = GS y + (GS / 8) g + 2 j, for query 2t + i

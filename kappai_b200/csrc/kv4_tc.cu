@@ -529,7 +529,7 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         }
         if (n_kt > 0 && ok && !kp_mbar_wait_bounded(&o_done[g], (n_kt - 1) & 1)) ok = false;
         kp_tc_fence_after();
-        const bool none = m == -INFINITY;
+        const bool none = m == -INFINITY && l == 0.f;                            // (not: scores that are NaN)
         const float inv = none ? 0.f : kt_pow2(ev - 14) / l;
         if (p.mass && seg >= 0) p.col[tile_id * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
         bf16* dst = p.out + row * p.ldo + (size_t)h * HD;
