@@ -39,6 +39,7 @@ struct Kv4TcArgs {
     float scale; int window; int ps, ps_log2; int H, G;
     unsigned char* q_image; float2* col;               // with mass: the groups' Q operands and (factor, lse) of their columns
     float* mass;
+    int cluster;                                       // CTAs that share the columns of a tile of keys
     int min_rows, n_seg, n_tiles;                      // n_tiles: an upper bound of the CTAs' tiles
 };
 
@@ -49,8 +50,9 @@ struct Kt {
     static constexpr int S_COL = 0, O_COL = 256, P_COL = ALIAS ? 64 : 256 + 2 * HD, P_STEP = ALIAS ? 128 : 64;   // columns of tensor memory (of group 0)
     static constexpr size_t SMEM = 1024 + 2 * OPER + ST * OPER + ST * TILE + 512;
     static constexpr int THREADS = 416;
-    // the pass that adds up the mass: one K tile, a ring of Q images
-    static constexpr int QST = 3, IMAGE = OPER + 1024; // an image in shared memory, and (factor, lse) of its columns
+    // the pass that adds up the mass: one K tile, a ring of Q images; two CTAs an SM
+    static constexpr int QST = HD == 64 ? 3 : 2, IMAGE = OPER + 1024;            // an image in shared memory, and (factor, lse) of its columns
+    static constexpr int MASS_THREADS = 288;
     static constexpr size_t MASS_SMEM = 1024 + OPER + QST * IMAGE + 512;
 };
 
@@ -274,6 +276,11 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     volatile int* tops = meta + 8;                     // [2][4 warps]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    kp_pdl_begin();
+    const int R = p.H / p.G, kvh = blockIdx.y;
+    int seg, cta_col0;
+    kt_find(p, blockIdx.x, R, lane, seg, cta_col0);
+    if (seg < 0) return;                               // (the grid is an upper bound)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             kp_mbar_init(&q_full[i], 128);
@@ -290,15 +297,10 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     __syncthreads();
     kp_tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;             // S of the groups: 2 x 128 columns; then O: 2 x HD
-    kp_pdl_begin();
 
-    const int R = p.H / p.G, kvh = blockIdx.y;
-    int seg, cta_col0;
-    kt_find(p, blockIdx.x, R, lane, seg, cta_col0);
-    int row0 = 0, n_cols = 0, pos0 = 0;
-    if (seg >= 0) { row0 = p.cu_rows[seg]; n_cols = (p.cu_rows[seg + 1] - row0) * R; pos0 = p.seg_pos[seg]; }
+    const int row0 = p.cu_rows[seg], n_cols = (p.cu_rows[seg + 1] - row0) * R, pos0 = p.seg_pos[seg];
     const int n_here = min(256, n_cols - cta_col0);    // columns of this CTA
-    const int k_hi = seg < 0 ? -1 : min(pos0 + (cta_col0 + n_here - 1) / R, p.max_blocks * p.ps - 1);
+    const int k_hi = min(pos0 + (cta_col0 + n_here - 1) / R, p.max_blocks * p.ps - 1);
     const int k_lo = p.window > 0 ? max(0, pos0 + cta_col0 / R - p.window + 1) : 0;
     const int kt_lo = k_lo / KT_ROWS, n_kt = k_hi >= k_lo ? k_hi / KT_ROWS - kt_lo + 1 : 0;
 
@@ -306,7 +308,7 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         // ---- codes to operands: thread d has key d of every tile.  Keys run two tiles ahead of the values' next: with one stage each K's is
         // free half a tile before V's.
         const int d = threadIdx.x - 256;
-        const int* bt = p.block_table + (size_t)max(seg, 0) * p.max_blocks;
+        const int* bt = p.block_table + (size_t)seg * p.max_blocks;
         const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);
         auto page_of = [&](int i) {
             const int key = (kt_lo + i) * KT_ROWS + d;
@@ -419,7 +421,7 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kp_mbar_arrive(&q_full[g]);
         const size_t tile_id = ((size_t)blockIdx.y * p.n_tiles + blockIdx.x) * 2 + g;
-        if (p.mass && seg >= 0) {
+        if (p.mass) {
             // the pass that adds up the mass takes the same operand; this thread's row of it, as it lies
             unsigned char* im = p.q_image + tile_id * S::OPER;
             const unsigned char* from = Qs + g * S::OPER;
@@ -531,7 +533,7 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         kp_tc_fence_after();
         const bool none = m == -INFINITY && l == 0.f;                            // (not: scores that are NaN)
         const float inv = none ? 0.f : kt_pow2(ev - 14) / l;
-        if (p.mass && seg >= 0) p.col[tile_id * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
+        if (p.mass) p.col[tile_id * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
         bf16* dst = p.out + row * p.ldo + (size_t)h * HD;
 #pragma unroll 1
         for (int e = 0; e < HD; e += 32) {
@@ -556,6 +558,15 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     if (warp == 12) kp_tmem_dealloc(tmem_base, 512);
 }
 
+__device__ __forceinline__ void kt_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+// a float at this place of the shared memory of the cluster's CTA `rank`
+__device__ __forceinline__ float kt_peer(const float* p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(kp_cluster_addr(p, rank)) : "memory");
+    return v;
+}
 // The sum of 2^(score - lse) over the 128 columns of a tile, of those from lo to hi (MASKED), for this thread's key: S of tensor memory
 // times kappa and the column's factor is the score.
 template <bool MASKED>
@@ -584,11 +595,12 @@ __device__ __forceinline__ float kt_column_sum(uint32_t tmem_s, const float4* co
     return part;
 }
 
-// ---- mass.  One CTA per (128 keys, kv head, segment): S^T = K Q^T with a thread a key, so that a key's weights add up in its
-// thread.  The operands of Q and the columns' (factor, lse) are those that the kernel above left, brought by bulk copies into a
-// ring; the two groups of 128 threads take the tiles of 128 columns in turn, two S each under way, and are added at the end.
+// ---- mass.  A cluster of CTAs per (128 keys, kv head, segment): S^T = K Q^T with a thread a key, so that a key's weights add up in its
+// thread.  The operands of Q and the columns' (factor, lse) are those that the kernel above left, brought by bulk copies into a ring; the two groups
+// of 128 threads take the tiles of 128 columns in turn.  The CTAs of a cluster share the columns out (the first keys of a prompt are
+// read by all of it), and their sums are added in order.
 template <int HD>
-__global__ void __launch_bounds__(Kt<HD>::THREADS, 1)
+__global__ void __launch_bounds__(Kt<HD>::MASS_THREADS, 2)
 kv4_tc_mass_kernel(const Kv4TcArgs p) {
     using S = Kt<HD>;
     constexpr int QST = S::QST;
@@ -599,120 +611,119 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     uint64_t* bars = reinterpret_cast<uint64_t*>(Qs + QST * S::IMAGE);
     uint64_t* k_full = bars;
     uint64_t* q_full = bars + 1; uint64_t* q_empty = bars + 4;                   // [QST]
-    uint64_t* s_full = bars + 7; uint64_t* s_free = bars + 11;                   // [group][2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+    uint64_t* s_full = bars + 7; uint64_t* s_free = bars + 9;                    // [group]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* tops = abort_flag + 1;               // [4]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    kp_pdl_begin();
+    const int n_ctas = p.cluster, rank = blockIdx.x % n_ctas, seg = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x / n_ctas * KT_ROWS, R = p.H / p.G;
+    const int n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg], pos0 = p.seg_pos[seg], n_cols = n_rows * R;
+    // keys that any row reads, and columns that read any of this CTA's, in tiles of 128 from column 0; this CTA has every n_ctas-th tile
+    const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+    const int c_lo = max(0, k0 - pos0) * R;
+    const int c_hi = (p.window > 0 ? min(n_rows - 1, k0 + KT_ROWS - 1 + p.window - 1 - pos0) : n_rows - 1) * R + R - 1;
+    if (n_rows < p.min_rows || k0 > last || k0 + KT_ROWS - 1 < first || c_hi < c_lo) return;       // (all of a cluster or none)
+    const int j_lo = c_lo / 128 + rank, n_j = max(0, (c_hi / 128 - j_lo + n_ctas) / n_ctas);
     if (threadIdx.x == 0) {
         kp_mbar_init(k_full, 128);
         for (int i = 0; i < QST; i++) { kp_mbar_init(&q_full[i], 1); kp_mbar_init(&q_empty[i], 1 + 128); }
-        for (int i = 0; i < 4; i++) { kp_mbar_init(&s_full[i], 1); kp_mbar_init(&s_free[i], 128); }
+        for (int i = 0; i < 2; i++) { kp_mbar_init(&s_full[i], 1); kp_mbar_init(&s_free[i], 128); }
         *abort_flag = 0;
         kp_mbar_init_fence();
     }
-    if (warp == 12) kp_tmem_alloc(tmem_slot, 512);
+    if (warp == 8) kp_tmem_alloc(tmem_slot, 256);
     kp_tc_fence_before();
     __syncthreads();
     kp_tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    kp_pdl_begin();
-
-    const int seg = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x * KT_ROWS, R = p.H / p.G;
-    const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg], n_cols = n_rows * R;
-    const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
-    const bool work = n_rows >= p.min_rows && k0 <= last && k0 + KT_ROWS - 1 >= first;
-    // columns that read any of the keys, in tiles of 128 from column 0
-    const int c_lo = max(0, k0 - pos0) * R;
-    const int c_hi = (p.window > 0 ? min(n_rows - 1, k0 + KT_ROWS - 1 + p.window - 1 - pos0) : n_rows - 1) * R + R - 1;
-    const int j_lo = c_lo / 128, n_j = work && c_hi >= c_lo ? c_hi / 128 - j_lo + 1 : 0;
-    const int top_tile = kt_first_tile(p, seg, R, lane);
     float sum = 0.f;
 
-    if (warp >= 8 && warp < 12) {
-        const int d = threadIdx.x - 256, key = k0 + d;
-        const bool there = work && key >= first && key <= last;
-        const int page = there ? p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)] : 0;
-        KtRow<HD> x;
-        x.load(p.pages + ((size_t)page * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key & (p.ps - 1), p.ps, there, false);
-        int ek = -100;
-#pragma unroll
-        for (int y = 0; y < S::NG; y++) ek = max(ek, kt_exponent(x.r[y]));
-        ek = __reduce_max_sync(0xffffffffu, ek);
-        if (lane == 0) tops[warp & 3] = ek;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        ek = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
-        kt_write_key<HD>(Ks, d, x, ek);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        kp_mbar_arrive(k_full);
-        if (d == 0) {
-            bool ok = true;
-            for (int i = 0; i < n_j && ok; i++) {
-                const int st = i % QST, j = j_lo + i;
-                if (*abort_flag || !kp_mbar_wait_bounded(&q_empty[st], ((i / QST) & 1) ^ 1)) { ok = false; break; }
-                const size_t tile_id = ((size_t)kvh * p.n_tiles + top_tile - (j >> 1)) * 2 + (j & 1);
-                kp_mbar_expect_tx(&q_full[st], S::IMAGE);
-                kp_bulk_g2s(Qs + st * S::IMAGE, p.q_image + tile_id * S::OPER, S::OPER, &q_full[st]);
-                kp_bulk_g2s(Qs + st * S::IMAGE + S::OPER, p.col + tile_id * 128, 1024, &q_full[st]);
+    if (warp == 8) {
+        // ---- copies and products
+        const int top_tile = kt_first_tile(p, seg, R, lane);
+        auto load = [&](int i) {
+            const int st = i % QST, j = j_lo + i * n_ctas;
+            const size_t tile_id = ((size_t)kvh * p.n_tiles + top_tile - (j >> 1)) * 2 + (j & 1);
+            kp_mbar_expect_tx_warp(&q_full[st], S::IMAGE);
+            kp_bulk_g2s_warp(Qs + st * S::IMAGE, p.q_image + tile_id * S::OPER, S::OPER, &q_full[st]);
+            kp_bulk_g2s_warp(Qs + st * S::IMAGE + S::OPER, p.col + tile_id * 128, 1024, &q_full[st]);
+        };
+        for (int i = 0; i < QST && i < n_j; i++) load(i);
+        bool ok = n_j == 0 || kt_wait(k_full, 0);
+        for (int i = 0; i < n_j && ok; i++) {
+            const int st = i % QST, g = i & 1, use = i >> 1;                     // S of group g for the use-th time
+            ok = kt_wait(&q_full[st], (i / QST) & 1) && kt_wait(&s_free[g], (use & 1) ^ 1);
+            if (!ok) break;
+            kp_tc_fence_after();
+            kt_issue_s<HD>(tmem_base + g * 128, Ks, Qs + st * S::IMAGE);
+            kp_umma_commit_warp(&s_full[g]);
+            kp_umma_commit_warp(&q_empty[st]);
+            // the stage of the tile before is asked for again once that tile's columns have been read
+            if (i > 0 && i - 1 + QST < n_j) {
+                ok = kt_wait(&q_empty[(i - 1) % QST], ((i - 1) / QST) & 1);
+                if (ok) load(i - 1 + QST);
             }
-            if (!ok) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
-            if (*abort_flag) kp_linger_after_failure();      // copies may still be under way
         }
-    } else if (warp == 12) {
-        if (n_j > 0) {
-            bool ok = kt_wait(k_full, 0);
-            for (int i = 0; i < n_j && ok; i++) {
-                const int st = i % QST, g = i & 1, b = (i >> 1) & 1, use = i >> 2;       // S buffer (g, b) for the use-th time
-                ok = kt_wait(&q_full[st], (i / QST) & 1) && kt_wait(&s_free[2 * g + b], (use & 1) ^ 1);
-                if (!ok) break;
-                kp_tc_fence_after();
-                kt_issue_s<HD>(tmem_base + (2 * g + b) * 128, Ks, Qs + st * S::IMAGE);
-                kp_umma_commit_warp(&s_full[2 * g + b]);
-                kp_umma_commit_warp(&q_empty[st]);
-            }
-            if (!ok && lane == 0) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+        if (!ok) {
+            if (lane == 0) { *abort_flag = 1; atomicExch(&g_kv4_tc_status, 1); }
+            kp_linger_after_failure();                 // copies may still be under way
         }
     } else {
         const int g = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane, key = k0 + r;
-        const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
-        // columns that read this key
         const bool there = key >= first && key <= last;
+        if (g == 0) {
+            const int page = there ? p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)] : 0;
+            KtRow<HD> x;
+            x.load(p.pages + ((size_t)page * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key & (p.ps - 1), p.ps, there, false);
+            int ek = -100;
+#pragma unroll
+            for (int y = 0; y < S::NG; y++) ek = max(ek, kt_exponent(x.r[y]));
+            ek = __reduce_max_sync(0xffffffffu, ek);
+            if (lane == 0) tops[warp] = ek;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            kt_write_key<HD>(Ks, r, x, max(max(tops[0], tops[1]), max(tops[2], tops[3])));
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            kp_mbar_arrive(k_full);
+        }
+        const uint32_t tmem_s = tmem_base + g * 128 + ((uint32_t)(q4 * 32) << 16);
+        // columns that read this key
         const int mine_lo = max(0, key - pos0) * R;
         const int mine_hi = !there ? -1 : (p.window > 0 ? min(n_cols, (key + p.window - pos0) * R) : n_cols) - 1;
         bool ok = n_j == 0 || kp_mbar_wait_bounded(k_full, 0);
         const float kappa = kt_pow2(max(max(tops[0], tops[1]), max(tops[2], tops[3])) - 7);
 #pragma unroll 1
         for (int i = g; i < n_j; i += 2) {
-            const int st = i % QST, b = (i >> 1) & 1, use = i >> 2;
-            if (ok && (*abort_flag || !kp_mbar_wait_bounded(&s_full[2 * g + b], use & 1))) ok = false;
+            const int st = i % QST, use = i >> 1, c0 = (j_lo + i * n_ctas) * 128;
+            if (ok && (*abort_flag || !kp_mbar_wait_bounded(&s_full[g], use & 1))) ok = false;
             // (the copies of the columns' factors arrived before the product that this waits for was issued; the wait makes them visible)
             if (ok && !kp_mbar_wait_bounded(&q_full[st], (i / QST) & 1)) ok = false;
             kp_tc_fence_after();
             const float4* col = reinterpret_cast<const float4*>(Qs + st * S::IMAGE + S::OPER);
-            const int c0 = (j_lo + i) * 128;
             const bool masked = __any_sync(0xffffffffu, c0 < mine_lo || c0 + 127 > mine_hi);
-            const uint32_t tmem_s = tmem_base + (2 * g + b) * 128 + lane_off;
-            const float part = masked ? kt_column_sum<true>(tmem_s, col, kappa, mine_lo - c0, mine_hi - c0) : kt_column_sum<false>(tmem_s, col, kappa, 0, 127);
+            sum += masked ? kt_column_sum<true>(tmem_s, col, kappa, mine_lo - c0, mine_hi - c0) : kt_column_sum<false>(tmem_s, col, kappa, 0, 127);
             kp_tc_fence_before();
-            kp_mbar_arrive(&s_free[2 * g + b]);
+            kp_mbar_arrive(&s_free[g]);
             kp_mbar_arrive(&q_empty[st]);
-            sum += part;
         }
         if (__builtin_expect(!ok, 0)) { if (lane == 0) atomicExch(&g_kv4_tc_status, 1); sum = 0.f; }
     }
     kp_tc_fence_before();
     __syncthreads();
-    if (warp == 12) kp_tmem_dealloc(tmem_base, 512);
-    float* join = reinterpret_cast<float*>(Ks);
-    if (warp >= 4 && warp < 8) join[threadIdx.x - 128] = sum;
-    __syncthreads();
-    if (warp < 4 && n_j > 0) {
+    if (warp == 8) kp_tmem_dealloc(tmem_base, 256);
+    float* join = reinterpret_cast<float*>(Ks);        // [group][key]; the cluster's first CTA adds them up, in order
+    if (warp < 8) join[threadIdx.x] = sum;
+    if (n_ctas > 1) kt_cluster_sync(); else __syncthreads();
+    if (rank == 0 && warp < 4) {
         const int key = k0 + threadIdx.x;
         if (key >= first && key <= last) {
+            float all = join[threadIdx.x] + join[128 + threadIdx.x];
+            for (int r = 1; r < n_ctas; r++) all += kt_peer(join + threadIdx.x, r) + kt_peer(join + 128 + threadIdx.x, r);
             const int page = p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)];
-            p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += sum + join[threadIdx.x];
+            p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += all;
         }
     }
+    if (n_ctas > 1) kt_cluster_sync();                 // (nobody leaves while its sums are read)
 }
 
 template <int HD>
@@ -726,7 +737,25 @@ static int kt_run(const Kv4TcArgs& a, int max_context, cudaStream_t st) {
     if (a.mass) {
         e = kp_smem_limit(kv4_tc_mass_kernel<HD>, S::MASS_SMEM, ready_mass);
         if (e) return e;
-        c = kp_launch_pdl(kv4_tc_mass_kernel<HD>, dim3((max_context + KT_ROWS - 1) / KT_ROWS, a.G, a.n_seg), dim3(S::THREADS), S::MASS_SMEM, st, a);
+        // Clusters of four where that many CTAs are there at once, else one CTA a tile of keys: a CTA's start (its keys' codes, the first
+        // images) takes as long as a dozen tiles of columns.
+        const int tiles = (max_context + KT_ROWS - 1) / KT_ROWS;
+        Kv4TcArgs m = a;
+        m.cluster = (long long)tiles * a.G * a.n_seg <= 148 ? 4 : 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(tiles * m.cluster, a.G, a.n_seg);
+        cfg.blockDim = dim3(S::MASS_THREADS);
+        cfg.dynamicSmemBytes = S::MASS_SMEM;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = m.cluster;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = m.cluster > 1 ? 2 : 1;
+        c = cudaLaunchKernelEx(&cfg, kv4_tc_mass_kernel<HD>, m);
         if (c) return (int)c;
     }
     return kp_launch_status();
