@@ -8,7 +8,8 @@ kernels below.
 
 Entry points: :class:`Engine` / :class:`EngineArgs` (Python),
 ``engine_init`` / ``engine_run`` / ``engine_shutdown`` and
-``python -m kappai_b200.cli`` (command line), ``bin/trace_run`` (trace replay).
+``python -m kappai_b200.cli`` (command line), ``bin/trace_run`` (trace replay);
+:class:`Kv4Cache`, a layer's keys and values in 4 bits with eviction by attention weight.
 """
 __version__ = "0.1.0"
 
@@ -17,6 +18,7 @@ _LAZY = {
     "EngineArgs": ("kappai_b200.engine.engine", "EngineArgs"),
     "ModelRunner": ("kappai_b200.engine.runner", "ModelRunner"),
     "StepEntry": ("kappai_b200.engine.runner", "StepEntry"),
+    "Kv4Cache": ("kappai_b200.cache.kv4", "Kv4Cache"),
     "SamplingParams": ("kappai_b200.sampling.params", "SamplingParams"),
     "engine_init": ("kappai_b200.cli", "engine_init"),
     "engine_run": ("kappai_b200.cli", "engine_run"),

@@ -165,6 +165,13 @@ class PagePool:
         del self._held[req]
         del self._version[req]
 
+    def take_over(self, req: Hashable, other: Hashable) -> None:
+        """``req`` gives its pages back and gets those of ``other``, which is no more (its keys have moved to them)."""
+        t, held = self._tables[other], self._held[other]
+        self.close(req)
+        del self._tables[other], self._held[other], self._version[other]
+        self._tables[req], self._held[req], self._version[req] = t, held, self._stamp()
+
     def check(self) -> None:
         """Every page is either free or held by exactly one block table."""
         seen = {}

@@ -329,9 +329,9 @@ struct Kv4Acc {
 #pragma unroll
                 for (int i = 0; i < 4; i++) o[nt][j][i] = 0.f;
         }
-        // Scales below 2^-60 are taken for that: with p s at most 2^15 the sum of p then stays below 2^75 times the number
-        // of keys.  (Values of 2^-56 and less lose their last bits.)
-        top_s = 8.673617379884035e-19f;
+        // Scales below 2^-90 are taken for that: with p s at most 2^15 the sum of p then stays below 2^105 times the number
+        // of keys.  (Values of 2^-86 and less lose their last bits.)
+        top_s = 8.077935669463161e-28f;
     }
     // Before a tile's weights: `mx` are the thread's largest scores of it, `ts` its largest scale of a value.  The shift follows
     // the maxima in steps: only a score above the last one's by 8, or a larger scale, moves it (and what has been added up).

@@ -1,0 +1,571 @@
+"""The 4-bit cache's kernels against the definition in 64 bits.
+
+The plain implementation reads the pages' bytes with integer arithmetic in numpy and computes attention, weights and evictions in
+float64.  It shares no code with the package.
+
+Tolerances.  What the pages hold is defined bit by bit (a division, two roundings to bfloat16, a rounding to an integer), so writes,
+reads and moves are compared for equality.  Attention of float32 rows: a score is a sum of at most 256 products of numbers of a few
+units, off by a few dozen float32 roundings of values up to about 100, 1e-5 absolute; a weight is then off by 1e-5 of itself and so is an output
+of weights that sum to 1, against values of about 3: 1e-4.  bfloat16 rows: the output is rounded to bfloat16, whose 8 significant bits put it off by
+up to 2^-8 of itself, and weights, in the tcgen05 form values too, to fp16 before, 11 bits: 2^-11 of the largest value each.  Weights that are added up (float32 in every form): each is off by
+1e-5 of itself and their sum runs over all rows and heads: 1e-5 of the sum, and 1e-6 absolute for those that are next to nothing.
+"""
+import numpy as np
+import pytest
+import torch
+
+from kappai_b200.ops import kv4
+from kappai_b200.ops.kernels import KernelError, read_status
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def group(hd):
+    return 64 if hd % 64 == 0 else 32
+
+
+def bf16(x):
+    """float64 -> the nearest bfloat16, as float64 (torch rounds float32 to nearest even)."""
+    return torch.from_numpy(np.asarray(x, dtype=np.float32)).bfloat16().double().numpy()
+
+
+def quantised(x, hd):
+    """float32 [..., hd] -> (codes, scale, minimum) by the definition, in numpy float32."""
+    g = np.asarray(x, dtype=np.float32).reshape(x.shape[:-1] + (hd // group(hd), group(hd)))
+    lo, hi = g.min(-1), g.max(-1)
+    with np.errstate(all="ignore"):
+        s = bf16(((hi - lo) / np.float32(15.0)).astype(np.float32)).astype(np.float32)
+        z = bf16(lo).astype(np.float32)
+        c = np.where(s[..., None] > 0, np.clip(np.rint((g - z[..., None]) / s[..., None]), 0, 15), 0)
+    return np.nan_to_num(c).astype(np.int64), s, z
+
+
+def plain_values(x, hd):
+    c, s, z = quantised(x, hd)
+    with np.errstate(all="ignore"):
+        return (c * s[..., None].astype(np.float64) + z[..., None].astype(np.float64)).reshape(x.shape)
+
+
+class Paged:
+    """Sequences of random keys and values in shuffled pages, bytes of ones wherever nothing was written, and their values in float64."""
+
+    def __init__(self, lengths, G, hd, page, seed=0, dtype=torch.float32, scale=1.0, spare=2):
+        self.G, self.hd, self.page, self.lengths = G, hd, page, lengths
+        rng = np.random.default_rng(seed)
+        need = [-(-n // page) for n in lengths]
+        order = rng.permutation(sum(need) + spare)
+        self.table = np.zeros((len(lengths), max(1, max(need))), dtype=np.int32)
+        at = 0
+        for i, n in enumerate(need):
+            self.table[i, :n] = order[at:at + n]
+            at += n
+        count = sum(need) + spare
+        self.pages = torch.full((count, G, kv4.kv4_page_bytes(page, hd)), 255, dtype=torch.uint8, device=DEV)
+        self.k, self.v = [], []
+        for i, n in enumerate(lengths):
+            k, v = (torch.from_numpy(((rng.standard_normal((n, G, hd)) + rng.standard_normal((G, hd))) * scale).astype(np.float32)).to(dtype)
+                    for _ in range(2))
+            self.k.append(plain_values(k.float().numpy(), hd))
+            self.v.append(plain_values(v.float().numpy(), hd))
+            if n:
+                kv4.kv4_write(k.reshape(n, -1).to(DEV), v.reshape(n, -1).to(DEV), self.pages, self.slots(i, n), page, G, hd)
+        self.table_d = torch.from_numpy(self.table).to(DEV)
+
+    def slots(self, i, n):
+        key = np.arange(n)
+        return torch.from_numpy((self.table[i][key // self.page] * self.page + key % self.page).astype(np.int32)).to(DEV)
+
+    def mass(self, seed=None):
+        m = torch.zeros((self.pages.shape[0], self.G, self.page), dtype=torch.float32, device=DEV)
+        if seed is not None:
+            m.copy_(torch.from_numpy(np.random.default_rng(seed).random(m.shape).astype(np.float32)))
+        return m
+
+    def mass_of(self, mass, i):
+        n = self.lengths[i]
+        t = mass.cpu().double().numpy()[self.table[i]]                       # [blocks, G, page]
+        return t.transpose(1, 0, 2).reshape(self.G, -1)[:, :n]
+
+
+def plain_attention(q, k, v, pos0, scale, window, H):
+    """One sequence in float64: q [n, H, hd]; returns out [n, H, hd] and the weights' sums [G, keys]."""
+    n, G = q.shape[0], k.shape[1]
+    out, got = np.zeros(q.shape), np.zeros((G, k.shape[0]))
+    for r in range(n):
+        hi = pos0 + r
+        lo = max(0, hi - window + 1) if window else 0
+        if hi < 0:
+            continue
+        for h in range(H):
+            g = h // (H // G)
+            s = (k[lo:hi + 1, g] @ q[r, h]) * scale
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out[r, h] = w @ v[lo:hi + 1, g]
+            got[g, lo:hi + 1] += w
+    return out, got
+
+
+def run_and_check(lengths, rows, H, G, hd, page, dtype, window=None, mass=True, seed=1, scale=None, q_scale=1.0, strided=False, min_rows=None):
+    P = Paged(lengths, G, hd, page, seed, dtype)
+    scale = hd ** -0.5 if scale is None else scale
+    rng = np.random.default_rng(seed + 100)
+    n = sum(rows)
+    q = torch.from_numpy((rng.standard_normal((n, H * hd)) * q_scale).astype(np.float32)).to(dtype)
+    cu = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    pos = np.asarray([L - r for L, r in zip(lengths, rows)], dtype=np.int32)
+    if strided:
+        wide = torch.full((n, H * hd + 24), float("nan"), dtype=dtype, device=DEV)
+        wide[:, 8:8 + H * hd] = q.to(DEV)
+        qd, od = wide[:, 8:8 + H * hd], torch.full((n, H * hd + 40), 7.0, dtype=dtype, device=DEV)[:, 16:16 + H * hd]
+    else:
+        qd, od = q.to(DEV), torch.full((n, H * hd), float("nan"), dtype=dtype, device=DEV)
+    m0 = P.mass(5) if mass else None
+    m = m0.clone() if mass else None
+    call = lambda: kv4.kv4_attention(qd, P.pages, P.table_d, torch.from_numpy(cu).to(DEV), torch.from_numpy(pos).to(DEV), od, scale, window, page, H,  # noqa: E731
+                                     G, hd, max(rows), max(1, max(lengths)), min_rows=min(rows) if min_rows is None else min_rows, mass=m)
+    call()
+    out = od.double().cpu().numpy().reshape(n, H, hd)
+    for i in range(len(lengths)):
+        want, got = plain_attention(q[cu[i]:cu[i + 1]].double().numpy().reshape(-1, H, hd), P.k[i], P.v[i], int(pos[i]), scale, window, H)
+        have = out[cu[i]:cu[i + 1]]
+        if dtype == torch.float32:
+            np.testing.assert_allclose(have, want, rtol=0, atol=1e-4)
+        else:
+            most = np.abs(P.v[i]).max() if P.v[i].size else 0.0
+            assert (np.abs(have - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * most).all(), f"sequence {i}: {np.abs(have - want).max()}"
+        if mass:
+            np.testing.assert_allclose(P.mass_of(m, i), P.mass_of(m0, i) + got, rtol=1e-5, atol=1e-6)
+    if mass:
+        # the same call gives the same bits, and pages that are no sequence's stay as they were
+        first = m.clone()
+        m.copy_(m0)
+        before = od.clone()
+        call()
+        assert torch.equal(m, first) and torch.equal(od, before)
+        spare = sorted(set(range(P.pages.shape[0])) - {int(x) for i, L in enumerate(lengths) for x in P.table[i][:-(-L // page)]})
+        assert torch.equal(m[spare], m0[spare])
+    assert not any(read_status().values())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G,hd,page,n", [(1, 32, 16, 1), (3, 64, 16, 37), (2, 96, 32, 129), (8, 128, 64, 5), (2, 192, 16, 33), (1, 256, 128, 140),
+                                         (8, 64, 64, 5000)])
+def test_written_values_are_those_of_the_definition(dtype, G, hd, page, n):
+    rng = np.random.default_rng(n)
+    count = -(-n // page) + 2
+    pages = torch.full((count, G, kv4.kv4_page_bytes(page, hd)), 255, dtype=torch.uint8, device=DEV)
+    x = torch.from_numpy((rng.standard_normal((n, 3 * G * hd)) * 10.0 ** rng.integers(-3, 3, (n, 1))).astype(np.float32)).to(dtype)
+    slots = torch.from_numpy(rng.permutation(count * page)[:n].astype(np.int32)).to(DEV)
+    xd = x.to(DEV)
+    kv4.kv4_write(xd[:, G * hd:2 * G * hd], xd[:, 2 * G * hd:], pages, slots, page, G, hd)      # columns of a wider product
+    k, v = kv4.kv4_read(pages, slots, page, G, hd, torch.float32)
+    for have, part in ((k, 1), (v, 2)):
+        src = x[:, part * G * hd:(part + 1) * G * hd].float().numpy().reshape(n, G, hd)
+        assert np.array_equal(have.double().cpu().numpy(), plain_values(src, hd).reshape(n, G * hd).astype(np.float32).astype(np.float64))
+    rest = np.setdiff1d(np.arange(count * page), slots.cpu().numpy())[:200].astype(np.int32)
+    k, _ = kv4.kv4_read(pages, torch.from_numpy(rest).to(DEV), page, G, hd, torch.float32)
+    assert bool(torch.isnan(k).all())                                                          # (bytes of ones are not a number)
+
+
+def test_written_values_at_the_edges():
+    """Groups of equal values, halves between two codes, values that round the minimum up, denormals, the largest values, slots of -1."""
+    hd, G, page = 64, 1, 16
+    rows = [np.zeros(64), np.full(64, 3.25), np.arange(64) / 4.0, np.linspace(-1, 14, 64), np.arange(64) % 16 + 0.5 * (np.arange(64) % 2), np.full(64, 1.0039),
+            np.arange(64) * 1e-42, np.where(np.arange(64) % 2, 1.6e38, -1.6e38), 1e-30 * np.arange(64), -np.arange(64.0) ** 3, 257.0 + np.arange(64) / 64]
+    x = np.stack(rows).astype(np.float32)
+    n = len(rows)
+    pages = torch.full((2, G, kv4.kv4_page_bytes(page, hd)), 255, dtype=torch.uint8, device=DEV)
+    slots = np.arange(n).astype(np.int32)
+    slots[3] = -1
+    xd, sd = torch.from_numpy(x).to(DEV), torch.from_numpy(slots).to(DEV)
+    kv4.kv4_write(xd, xd.clone(), pages, sd, page, G, hd)
+    k, v = kv4.kv4_read(pages, sd, page, G, hd, torch.float32)
+    want = plain_values(x, hd).astype(np.float32)
+    want[3] = 0.0
+    assert np.array_equal(k.cpu().numpy(), want) and np.array_equal(v.cpu().numpy(), want)
+    held, _ = kv4.kv4_read(pages, torch.tensor([3], dtype=torch.int32, device=DEV), page, G, hd, torch.float32)
+    assert bool(torch.isnan(held).all())                                                       # the row without a slot wrote nothing
+
+
+def test_values_that_are_not_finite_spoil_their_group_only():
+    hd, G, page = 128, 2, 16
+    x = np.random.default_rng(0).standard_normal((3, G * hd)).astype(np.float32)
+    x[0, 3], x[1, 70], x[2, 200] = np.nan, np.inf, -np.inf
+    pages = torch.zeros((1, G, kv4.kv4_page_bytes(page, hd)), dtype=torch.uint8, device=DEV)
+    slots = torch.arange(3, dtype=torch.int32, device=DEV)
+    kv4.kv4_write(torch.from_numpy(x).to(DEV), torch.from_numpy(x).to(DEV), pages, slots, page, G, hd)
+    k, _ = kv4.kv4_read(pages, slots, page, G, hd, torch.float32)
+    bad = ~torch.isfinite(k.cpu()).numpy()
+    want = np.zeros_like(bad)
+    want[0, 0:64] = want[1, 64:128] = want[2, 192:256] = True
+    assert np.array_equal(bad, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", kv4.KV4_HEAD_DIMS)
+@pytest.mark.parametrize("H,G,lengths,rows", [(1, 1, [1], [1]), (4, 2, [1, 2, 15, 16, 17], [1, 1, 1, 1, 1]), (8, 8, [300, 64], [1, 1]), (12, 4, [130, 700], [3, 2]),
+                                              (16, 1, [65, 513], [1, 8])])
+def test_few_rows(dtype, hd, H, G, lengths, rows):
+    run_and_check(lengths, rows, H, G, hd, 16, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", kv4.KV4_HEAD_DIMS)
+@pytest.mark.parametrize("H,G,lengths,rows", [(2, 1, [9], [9]), (4, 1, [64, 130, 200], [64, 12, 77]), (3, 3, [127, 129], [127, 129]), (6, 2, [300], [40])])
+def test_many_rows(dtype, hd, H, G, lengths, rows):
+    run_and_check(lengths, rows, H, G, hd, 32, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 512])
+def test_pages_of_every_size(dtype, hd, page):
+    run_and_check([page - 1, page, page + 1, 3 * page + 5], [1, 2, 1, 3], 4, 2, hd, page, dtype)
+    run_and_check([page + 11, 2 * page], [11, page], 4, 2, hd, page, dtype, seed=3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("window", [1, 2, 16, 63, 200])
+def test_windows(dtype, hd, window):
+    run_and_check([700, 5, 64], [2, 1, 3], 4, 2, hd, 16, dtype, window=window)
+    run_and_check([420, 30], [170, 30], 4, 2, hd, 16, dtype, window=window, seed=4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128, 192])
+def test_rows_with_no_key(dtype, hd):
+    """Rows that stand in front of the first key give zeros; so does a sequence without any key."""
+    run_and_check([2, 3, 0, 40], [4, 3, 1, 2], 4, 2, hd, 16, dtype)
+    run_and_check([5, 100], [20, 30], 4, 2, hd, 16, dtype, seed=6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_a_mixed_step(dtype, hd):
+    """Decoded rows, drafts of a few tokens and portions of prompts in one call."""
+    run_and_check([800, 33, 150, 8, 300], [1, 3, 150, 8, 9], 8, 2, hd, 16, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd,lengths,rows", [(64, [3000], [1]), (64, [9000, 4100], [1, 1]), (128, [5000], [2]), (64, [2300], [300]), (128, [1500, 700], [260, 700])])
+def test_long_contexts(dtype, hd, lengths, rows):
+    run_and_check(lengths, rows, 4, 2, hd, 64, dtype, mass=True)
+    run_and_check(lengths, rows, 4, 2, hd, 64, dtype, mass=False, seed=9)
+
+
+@pytest.mark.parametrize("hd,rows", [(64, 1), (64, 30), (128, 30), (96, 30)])
+def test_many_chunks_are_joined(hd, rows):
+    """More chunks than a cluster has, by a context that many CTAs share out."""
+    lengths = [40000]
+    P = Paged(lengths, 1, hd, 128, 2, torch.bfloat16)
+    assert rows > 1 or kv4.kv4_chunks(1, 1, lengths[0], 0, 4, 1, hd)[0] > 8
+    run_and_check(lengths, [rows], 4, 1, hd, 128, torch.bfloat16)
+    del P
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [[1, 2], [40, 9]])
+def test_strided_rows(dtype, rows):
+    run_and_check([150, 90], rows, 4, 2, 64, 16, dtype, strided=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [[1], [20]])
+@pytest.mark.parametrize("q_scale,scale", [(30.0, None), (1e-3, None), (1.0, 1.7), (2.0 ** -60, 1e15), (2.0 ** 60, 1e-20)])
+def test_scores_of_many_sizes(dtype, rows, q_scale, scale):
+    """From one key that takes all the weight to weights that are all the same.  (Scores of 1e3 are off by 1e-4, and so are the outputs.)"""
+    hd, H, G = 64, 4, 2
+    P = Paged([200], G, hd, 16, 3, dtype)
+    q = torch.from_numpy((np.random.default_rng(8).standard_normal((rows[0], H * hd)) * q_scale).astype(np.float32)).to(dtype)
+    out = torch.empty((rows[0], H * hd), dtype=dtype, device=DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    kv4.kv4_attention(q.to(DEV), P.pages, P.table_d, i32([0, rows[0]]), i32([200 - rows[0]]), out, scale or hd ** -0.5, None, 16, H, G, hd, rows[0], 200,
+                      min_rows=rows[0])
+    want, _ = plain_attention(q.double().numpy().reshape(-1, H, hd), P.k[0], P.v[0], 200 - rows[0], scale or hd ** -0.5, None, H)
+    top = np.abs(want).max(-1, keepdims=True)
+    have = out.double().cpu().numpy().reshape(want.shape)
+    assert (np.abs(have - want) <= (2e-3 if dtype == torch.float32 else 2.0 ** -7) * top).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 24])
+@pytest.mark.parametrize("scale", [1e-25, 1e-6, 1e4, 1e30])
+def test_keys_and_values_of_many_sizes(dtype, rows, scale):
+    """Values far outside fp16's range: powers of two carry them."""
+    hd, H, G = 64, 4, 2
+    P = Paged([100], G, hd, 16, 3, dtype, scale=scale)
+    q = torch.from_numpy(np.random.default_rng(8).standard_normal((rows, H * hd)).astype(np.float32)).to(dtype)
+    out = torch.empty((rows, H * hd), dtype=dtype, device=DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    s = float(hd ** -0.5 / scale)
+    kv4.kv4_attention(q.to(DEV), P.pages, P.table_d, i32([0, rows]), i32([100 - rows]), out, s, None, 16, H, G, hd, rows, 100, min_rows=rows)
+    want, _ = plain_attention(q.double().numpy().reshape(-1, H, hd), P.k[0], P.v[0], 100 - rows, s, None, H)
+    top = np.abs(want).max(-1, keepdims=True)
+    assert (np.abs(out.double().cpu().numpy().reshape(want.shape) - want) <= (1e-3 if dtype == torch.float32 else 2.0 ** -7) * top).all()
+
+
+@pytest.mark.parametrize("rows", [1, 30])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_query_that_is_not_finite_spoils_its_own_rows_only(rows, hd, dtype):
+    H, G = 4, 2
+    P = Paged([90], G, hd, 16, 3, dtype)
+    q = torch.randn((rows, H * hd), generator=torch.Generator().manual_seed(1)).to(dtype)
+    clean = torch.empty_like(q, device=DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    call = lambda x, o: kv4.kv4_attention(x.to(DEV), P.pages, P.table_d, i32([0, rows]), i32([90 - rows]), o, hd ** -0.5, None, 16, H, G, hd, rows, 90,  # noqa: E731
+                                          min_rows=rows)
+    call(q, clean)
+    q2 = q.clone()
+    q2[0, hd + 3] = float("nan")                                             # head 1 of row 0
+    out = torch.empty_like(clean)
+    call(q2, out)
+    a, b = out.cpu().float().view(rows, H, hd), clean.cpu().float().view(rows, H, hd)
+    assert bool(torch.isnan(a[0, 1]).all())
+    a[0, 1] = b[0, 1] = 0
+    np.testing.assert_allclose(a.numpy(), b.numpy(), rtol=0, atol=1e-4 if dtype == torch.float32 else 2.0 ** -6)
+
+
+def plain_keep(mass, n, keep, recent, first):
+    """Indices that one kv head keeps, in order."""
+    if n <= keep:
+        return list(range(n))
+    sure = [j for j in range(n) if j < first or j >= n - recent]
+    rest = sorted((j for j in range(n) if first <= j < n - recent), key=lambda j: (-mass[j], j))
+    return sorted(sure + rest[:keep - len(sure)])
+
+
+@pytest.mark.parametrize("hd,G,page", [(32, 1, 16), (64, 2, 64), (96, 3, 16), (128, 2, 32), (192, 1, 16), (256, 2, 16)])
+@pytest.mark.parametrize("lengths,keep,recent,first", [([1, 40, 41, 300], 40, 8, 2), ([1000], 17, 0, 0), ([2000, 90], 64, 64, 0), ([500, 501], 100, 60, 40), ([50], 49, 1, 1)])
+def test_eviction(hd, G, page, lengths, keep, recent, first):
+    P = Paged(lengths, G, hd, page, 3)
+    rng = np.random.default_rng(0)
+    m = np.round(rng.random((P.pages.shape[0], G, page)) * 20).astype(np.float32) / 4        # (many of the same weight)
+    m[rng.random(m.shape) < 0.1] = 0.0
+    m[rng.random(m.shape) < 0.02] = np.inf
+    mass = torch.from_numpy(m).to(DEV)
+    new = Paged([min(n, keep) for n in lengths], G, hd, page, 4)
+    new_mass = torch.full((new.pages.shape[0], G, page), -1.0, device=DEV)
+    kept = torch.full((len(lengths), G, keep), 77, dtype=torch.int32, device=DEV)
+    kv4.kv4_evict(P.pages, mass, P.table_d, torch.tensor(lengths, dtype=torch.int32, device=DEV), new.pages, new_mass, new.table_d, kept, max(lengths), keep,
+                  recent, first, page, G, hd)
+    got = kept.cpu().numpy()
+    for i, n in enumerate(lengths):
+        old = P.mass_of(mass, i)
+        stay = min(n, keep)
+        k, v = (x.double().cpu().numpy().reshape(stay, G, hd) for x in kv4.kv4_read(new.pages, new.slots(i, stay), page, G, hd, torch.float32))
+        moved = new.mass_of(new_mass, i)
+        for g in range(G):
+            want = plain_keep(old[g], n, keep, recent, first)
+            assert list(got[i, g, :stay]) == want and (got[i, g, stay:] == -1).all()
+            assert np.array_equal(k[:, g], P.k[i][want, g].astype(np.float32)) and np.array_equal(v[:, g], P.v[i][want, g].astype(np.float32))
+            assert np.array_equal(moved[g], old[g][want])
+
+
+def test_eviction_of_more_keys_than_shared_memory_holds():
+    n, keep, page, hd = 70000, 5000, 128, 32
+    rng = np.random.default_rng(2)
+    count = -(-n // page)
+    pages = torch.zeros((count, 1, kv4.kv4_page_bytes(page, hd)), dtype=torch.uint8, device=DEV)
+    table = torch.from_numpy(rng.permutation(count).astype(np.int32)[None]).to(DEV)
+    weights = (rng.random(n) ** 8).astype(np.float32)
+    mass = torch.zeros((count, 1, page), device=DEV)
+    key = torch.arange(n, device=DEV)
+    mass[table[0].long()[key // page], 0, key % page] = torch.from_numpy(weights).to(DEV)
+    new_pages = torch.zeros((-(-keep // page), 1, kv4.kv4_page_bytes(page, hd)), dtype=torch.uint8, device=DEV)
+    new_mass = torch.zeros((new_pages.shape[0], 1, page), device=DEV)
+    kept = torch.empty((1, 1, keep), dtype=torch.int32, device=DEV)
+    kv4.kv4_evict(pages, mass, table, torch.tensor([n], dtype=torch.int32, device=DEV), new_pages, new_mass,
+                  torch.arange(new_pages.shape[0], dtype=torch.int32, device=DEV)[None], kept, n, keep, 100, 3, page, 1, hd)
+    assert kept.cpu().numpy()[0, 0].tolist() == plain_keep(weights, n, keep, 100, 3)
+
+
+def test_what_is_refused():
+    P = Paged([40], 2, 64, 16, 0)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    q, out = torch.zeros((1, 256), device=DEV), torch.zeros((1, 256), device=DEV)
+    ok = dict(q=q, pages=P.pages, block_table=P.table_d, cu_rows=i32([0, 1]), seg_pos=i32([39]), out=out, scale=0.1, window=None, page_size=16, H=4, G=2, hd=64,
+              max_rows=1, max_context=40)
+    kv4.kv4_attention(**ok)
+    for bad in (dict(q=q.half()), dict(q=q[:, :192]), dict(out=out.bfloat16()), dict(pages=P.pages[:, :, :-16]), dict(pages=P.pages.float()), dict(H=5),
+                dict(H=3, q=torch.zeros((1, 192), device=DEV)), dict(hd=48), dict(page_size=24), dict(window=0), dict(max_context=0), dict(max_context=1000),
+                dict(cu_rows=i32([0, 1, 1])), dict(cu_rows=torch.tensor([0, 1], device=DEV)), dict(block_table=P.table_d[0]), dict(seg_pos=torch.tensor([39.0], device=DEV)),
+                dict(mass=torch.zeros((1, 2, 16), device=DEV)), dict(q=q.cpu()), dict(G=0)):
+        with pytest.raises(KernelError):
+            kv4.kv4_attention(**{**ok, **bad})
+    k = torch.zeros((2, 128), device=DEV)
+    s = i32([0, 1])
+    for bad in (dict(k=k.half(), v=k.half()), dict(v=k.bfloat16()), dict(k=k[:1]), dict(slot_map=s.long()), dict(slot_map=i32([0])), dict(hd=40)):
+        with pytest.raises(KernelError):
+            kv4.kv4_write(**{**dict(k=k, v=k, pages=P.pages, slot_map=s, page_size=16, G=2, hd=64), **bad})
+    with pytest.raises(KernelError):
+        kv4.kv4_read(P.pages, s, 16, 2, 64, dtype=torch.float16)
+    mass = P.mass()
+    new, kept = Paged([8], 2, 64, 16, 1), torch.empty((1, 2, 8), dtype=torch.int32, device=DEV)
+    fine = dict(pages=P.pages, mass=mass, block_table=P.table_d, n_keys=i32([40]), new_pages=new.pages, new_mass=new.mass(), new_table=new.table_d, kept=kept,
+                max_keys=40, keep=8, recent=2, first=1, page_size=16, G=2, hd=64)
+    kv4.kv4_evict(**fine)
+    for bad in (dict(keep=0), dict(recent=9), dict(first=-1), dict(recent=5, first=4), dict(max_keys=0), dict(max_keys=1000), dict(kept=kept[:, :, :4]),
+                dict(mass=mass[:1]), dict(new_mass=mass.double()), dict(n_keys=torch.tensor([40], device=DEV)), dict(new_table=new.table_d[:, :0])):
+        with pytest.raises(KernelError):
+            kv4.kv4_evict(**{**fine, **bad})
+
+
+def test_calls_with_nothing_in_them():
+    P = Paged([20], 1, 32, 16, 0)
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    kv4.kv4_write(torch.empty((0, 32), device=DEV), torch.empty((0, 32), device=DEV), P.pages, none, 16, 1, 32)
+    k, v = kv4.kv4_read(P.pages, none, 16, 1, 32)
+    assert k.shape == v.shape == (0, 32)
+    out = torch.empty((0, 64), device=DEV)
+    kv4.kv4_attention(out, P.pages, P.table_d, torch.zeros(1, dtype=torch.int32, device=DEV), none, out, 1.0, None, 16, 2, 1, 32, 1, 1)
+
+
+def test_another_stream():
+    """Launches go to the current stream: work queued there before is seen, and what follows there sees the result."""
+    P = Paged([600], 2, 64, 16, 3, torch.bfloat16)
+    q = torch.randn((1, 256), device=DEV).bfloat16()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    cu, pos, want = i32([0, 1]), i32([599]), torch.empty_like(q)
+    call = lambda x, o: kv4.kv4_attention(x, P.pages, P.table_d, cu, pos, o, 0.125, None, 16, 4, 2, 64, 1, 600)  # noqa: E731
+    call(q, want)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        slow = torch.randn((4096, 4096), device=DEV)
+        for _ in range(10):
+            slow = slow @ slow / 64.0
+        late = torch.zeros_like(q)
+        late.copy_(q)
+        out = torch.empty_like(q)
+        call(late, out)
+        copy = out.clone()
+    side.synchronize()
+    assert torch.equal(copy, want)
+
+
+def test_a_captured_graph_replays():
+    P = Paged([900], 2, 64, 16, 3, torch.bfloat16)
+    q, out = torch.randn((1, 512), device=DEV).bfloat16(), torch.empty((1, 512), dtype=torch.bfloat16, device=DEV)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    cu, pos, mass = i32([0, 1]), i32([899]), P.mass()
+    call = lambda: kv4.kv4_attention(q, P.pages, P.table_d, cu, pos, out, 0.125, None, 16, 8, 2, 64, 1, 900, mass=mass)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    first, gained = out.clone(), mass.clone()
+    mass.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    out.zero_()
+    mass.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first) and torch.equal(mass, gained)
+
+
+class TestKv4Cache:
+    def cache(self, n_pages=40, mass=True):
+        from kappai_b200 import Kv4Cache
+
+        return Kv4Cache(2, 64, n_pages, page_size=16, mass=mass)
+
+    def test_sequences_grow_are_read_shrink_and_end(self):
+        from kappai_b200.cache import CacheError, OutOfPages
+
+        c = self.cache()
+        gen = torch.Generator(device=DEV).manual_seed(0)
+        rows = {"a": torch.randn((150, 2, 128), generator=gen, device=DEV), "b": torch.randn((60, 2, 128), generator=gen, device=DEV)}
+        for s in rows:
+            c.add(s)
+        c.append(torch.cat([rows["a"][:100, 0], rows["b"][:7, 0]]), torch.cat([rows["a"][:100, 1], rows["b"][:7, 1]]), ["a", "b"], [100, 7])
+        q = torch.randn((107, 512), generator=gen, device=DEV)
+        c.attend(q, ["a", "b"], [100, 7], 8, 0.125)
+        c.append(torch.cat([rows["b"][7:60, 0], rows["a"][100:, 0]]), torch.cat([rows["b"][7:60, 1], rows["a"][100:, 1]]), ["b", "a"], [53, 50])
+        assert c.length("a") == 150 and c.length("b") == 60
+        out = c.attend(q[:3], ["b", "a"], [1, 2], 8, 0.125)
+        for s in rows:
+            k, v = c.read(s, torch.float32)
+            want = [plain_values(rows[s][:, i].cpu().numpy().reshape(-1, 2, 64), 64).reshape(-1, 128).astype(np.float32) for i in (0, 1)]
+            assert np.array_equal(k.cpu().numpy(), want[0]) and np.array_equal(v.cpu().numpy(), want[1])
+        ka, va = (x.double().cpu().numpy().reshape(-1, 2, 64) for x in c.read("a", torch.float32))
+        want, _ = plain_attention(q[1:3].double().cpu().numpy().reshape(2, 8, 64), ka, va, 148, 0.125, None, 8)
+        np.testing.assert_allclose(out[1:].double().cpu().numpy().reshape(2, 8, 64), want, rtol=0, atol=1e-4)
+        # every row gave a weight of 1 a head: 100 + 2 rows of a, 7 + 1 of b, 4 heads a kv head
+        assert abs(float(c.mass_of("a").sum()) - 8 * 102) < 1e-2 and abs(float(c.mass_of("b").sum()) - 8 * 8) < 1e-2
+        mass, free = c.mass_of("a").cpu().numpy(), c.pool.n_free
+        kept = c.evict(["a", "b"], 64, recent=16, first=2).cpu().numpy()
+        for g in range(2):
+            assert kept[0, g].tolist() == plain_keep(mass[g], 150, 64, 16, 2) and kept[1, g].tolist() == list(range(60)) + [-1] * 4
+            assert np.array_equal(c.mass_of("a").cpu().numpy()[g], mass[g][kept[0, g]])
+        c.pool.check()
+        assert c.length("a") == 64 and c.length("b") == 60 and c.pool.n_free == free + 10 - 4
+        k2, _ = c.read("a", torch.float32)
+        assert np.array_equal(k2.cpu().numpy().reshape(64, 2, 64)[:, 1], ka[kept[0, 1], 1].astype(np.float32))
+        with pytest.raises(OutOfPages):
+            c.append(torch.zeros((1000, 128), device=DEV), torch.zeros((1000, 128), device=DEV), ["a"], [1000])
+        assert c.length("a") == 64
+        for call in (lambda: c.attend(q[:1], ["x"], [1], 8, 0.1), lambda: c.attend(q[:2], ["a", "a"], [1, 1], 8, 0.1), lambda: c.attend(q[:100], ["a"], [100], 8, 0.1),
+                     lambda: c.append(q[:1, :128], q[:1, :128], ["a"], [0]), lambda: c.append(q[:2, :128], q[:2, :128], ["a"], [1]), lambda: c.read("x")):
+            with pytest.raises(CacheError):
+                call()
+        with pytest.raises(CacheError):
+            self.cache(mass=False).evict([], 4)
+        c.free("a")
+        c.free("b")
+        c.pool.check()
+        assert c.pool.n_free == 40
+
+    def test_a_page_of_another_sequence_brings_no_weight(self):
+        c = self.cache(n_pages=4)
+        x = torch.randn((32, 128), device=DEV)
+        c.add("a")
+        c.append(x, x, ["a"], [32])
+        c.attend(torch.randn((32, 256), device=DEV), ["a"], [32], 4, 0.125)
+        c.free("a")
+        c.add("b")
+        c.append(x, x, ["b"], [32])
+        assert float(c.mass_of("b").abs().sum()) == 0.0
+
+    def test_an_eviction_that_finds_no_room_changes_nothing(self):
+        from kappai_b200.cache import OutOfPages
+
+        c = self.cache(n_pages=4)
+        x = torch.randn((60, 128), device=DEV)
+        c.add("a")
+        c.append(x, x, ["a"], [60])
+        with pytest.raises(OutOfPages):
+            c.evict(["a"], 32)
+        with pytest.raises(KernelError):
+            self.evict_badly()
+        assert c.length("a") == 60
+        c.pool.check()
+
+    def evict_badly(self):
+        c = self.cache()
+        x = torch.randn((60, 128), device=DEV)
+        c.add("a")
+        c.append(x, x, ["a"], [60])
+        try:
+            c.evict(["a"], 8, recent=7, first=5)
+        finally:
+            c.pool.check()
+            assert c.length("a") == 60
+
+
+def test_the_example_runs():
+    import importlib.util
+    import os
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "long_context.py")
+    spec = importlib.util.spec_from_file_location("long_context", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    got = m.main(["--tokens", "1500", "--budget", "400", "--new", "8", "--portion", "300"])
+    # 4 bits a value leave an error of about a tenth; the keys that were evicted add little to it
+    assert got["kept"] == 400 and got["evicted"] > 1000 and got["held"] < got["full"] / 10
+    assert got["error"] < 2 * got["error_4bit"] + 0.05
