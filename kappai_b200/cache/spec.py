@@ -12,7 +12,8 @@ recurrent/conv state of fixed size per layer):
   group may keep one entry for every ``every`` positions instead of one a
   position (entry e stands for the positions e every .. e every + every - 1 and
   exists once the last of them does), and one row a position instead of a key
-  and a value row (``planes`` = 1: a latent that both are made of).
+  and a value row (``planes`` = 1: a latent that both are made of).  ``bits`` = 4
+  keeps keys and values in 4 bits with a scale and a minimum a group.
 * :class:`StateSpec` — a fixed-size tensor per request; kept in a slot.
 
 A mixer that needs several of these at once (keys and values beside the last
@@ -33,6 +34,7 @@ class PagedKVSpec:
     keep_first: int = 0               # with a window: the first keys of a sequence stay readable for good
     every: int = 1                    # positions an entry stands for
     planes: int = 2                   # rows an entry: a key and a value, or one row for both
+    bits: int = 16                    # 4: codes and ranges in place of values of the compute dtype (``csrc/kv4.cuh``)
 
     @property
     def group_key(self) -> Tuple:
@@ -45,7 +47,17 @@ class PagedKVSpec:
             key += (("every", self.every),)
         if self.planes != 2:
             key += (("planes", self.planes),)
+        if self.bits != 16:
+            key += (("bits", self.bits),)
         return key
+
+    def bytes_per_entry(self, element_size: int) -> int:
+        """Bytes of an entry in all kv heads; ``element_size`` is that of the compute dtype."""
+        if self.bits == 4:
+            from ..ops.kv4 import kv4_page_bytes
+
+            return self.num_kv_heads * kv4_page_bytes(16, self.head_dim) // 16
+        return self.planes * self.num_kv_heads * self.head_dim * element_size
 
 
 @dataclass(frozen=True)

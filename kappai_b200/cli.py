@@ -59,6 +59,7 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--max-batch", type=int, default=64, help="requests that run together (default 64)")
     g.add_argument("--max-step-tokens", type=int, default=2048, help="token budget of one step (default 2048)")
     g.add_argument("--page-size", type=int, default=64, help="tokens in a cache page (default 64)")
+    g.add_argument("--kv-bits", type=int, choices=[16, 4], default=16, help="bits of a cached key or value: 16 (default) or 4")
     g.add_argument("--kv-tokens", type=int, default=0, help="tokens the cache pools hold (0 = max-batch x ctx)")
     g.add_argument("--device", default="cuda:0", help="compute device (default: cuda:0)")
     g.add_argument("--random-weights", metavar="CONFIG", help="write a model folder with random weights from this "
@@ -103,7 +104,7 @@ def engine_init(argv: Optional[Sequence[str]] = None) -> Tuple[Engine, argparse.
         logging.basicConfig(stream=sys.stderr, format="[debug] %(message)s")
         logging.getLogger("kappai_b200").setLevel(logging.DEBUG)
     eng = Engine(EngineArgs(model=a.model, dtype=a.dtype, ctx_size=a.ctx_size, max_batch=a.max_batch,
-                            max_step_tokens=a.max_step_tokens, page_size=a.page_size, kv_tokens=a.kv_tokens,
+                            max_step_tokens=a.max_step_tokens, page_size=a.page_size, kv_bits=a.kv_bits, kv_tokens=a.kv_tokens,
                             device=a.device, time_kernels=a.time, debug_forward=a.debug_forward))
     return eng, a
 

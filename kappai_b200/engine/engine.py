@@ -40,6 +40,7 @@ class EngineArgs:
     max_batch: int = 64                # requests that run together (state slots)
     max_step_tokens: int = 2048        # token budget of one step
     page_size: int = 64
+    kv_bits: int = 16                  # 4: attention keeps keys and values in 4 bits (page_size a power of two, at least 16)
     kv_tokens: int = 0                 # tokens the page pools hold (0: max_batch * ctx_size, or what fits beside the weights)
     device: str = "cuda:0"
     look_ahead: bool = True            # launch the next decode step before the last one's tokens are read
@@ -92,7 +93,7 @@ class Engine:
         # the pools hold kv_tokens, or what max_batch requests of that length need, or what fits beside the weights
         self.runner = ModelRunner(args.model, dtype=args.dtype, max_tokens=args.kv_tokens, max_requests=args.max_batch,
                                   page_size=args.page_size, max_model_len=args.ctx_size or (1 << 62), device=args.device,
-                                  max_step_tokens=args.max_step_tokens, free_memory=free_memory)
+                                  max_step_tokens=args.max_step_tokens, free_memory=free_memory, kv_bits=args.kv_bits)
         self.scheduler = Scheduler(self.runner.cache, args.max_step_tokens, args.max_batch,
                                    self.runner.max_model_len, self.runner.spec.eos_token_id)
         self.requests: Dict[Hashable, Request] = {}

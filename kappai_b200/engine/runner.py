@@ -59,7 +59,7 @@ class ModelRunner:
     def __init__(self, model_dir: str, dtype: str = "bfloat16", max_tokens: int = 4096,
                  max_requests: int = 4, page_size: int = 64, max_model_len: Optional[int] = None,
                  device="cuda:0", cuda_graphs: bool = True, max_step_tokens: Optional[int] = None,
-                 free_memory=None):
+                 free_memory=None, kv_bits: int = 16):
         """``max_tokens``: how many tokens the live requests may hold together,
         each request's count rounded up to a whole page; the page pools are
         made for exactly this many, or the runner refuses to start if the device
@@ -70,7 +70,9 @@ class ModelRunner:
         request gets in one step, if the caller keeps such a limit: pools of
         windowed page groups are then made no larger than the windows need.
         ``free_memory``: a function that returns the device's free bytes (for
-        tests; by default the device is asked)."""
+        tests; by default the device is asked).  ``kv_bits``: 4 keeps the keys and
+        values of the attention mixers in 4 bits (``page_size`` is then a power of
+        two, at least 16); a model without such a mixer is refused."""
         if dtype not in DTYPES:
             raise EngineError(f"dtype '{dtype}': expected bfloat16 or float32")
         self.device = require_cuda(device)
@@ -81,15 +83,21 @@ class ModelRunner:
             raise EngineError("page_size must be positive")
         if max_tokens < 0 or max_requests < 1:
             raise EngineError("max_tokens must not be negative and max_requests must be positive")
+        if kv_bits not in (4, 16):
+            raise EngineError(f"kv_bits={kv_bits}: expected 16 or 4")
+        if kv_bits == 4 and (page_size < 16 or page_size & (page_size - 1)):
+            raise EngineError(f"page_size={page_size}: pages in 4 bits have a power of two of tokens, at least 16")
         self.page_size = page_size
         limit = max_model_len or (-(-max_tokens // page_size) * page_size if max_tokens else self.spec.max_positions)
         self.max_model_len = min(self.spec.max_positions, limit)
         torch.cuda.set_device(self.device)
-        env = BuildEnv(self.device, self.dtype, self.max_model_len)
+        env = BuildEnv(self.device, self.dtype, self.max_model_len, kv_bits=kv_bits)
         self.model = Model(self.spec, env)
         load_weights(self.model, model_dir)
         specs = self.model.cache_specs()
         borrowing = self.model.cache_borrowing()
+        if kv_bits == 4 and not any(isinstance(leaf, PagedKVSpec) and leaf.bits == 4 for s in specs for leaf in leaf_specs(s)):
+            raise EngineError("kv_bits=4: no mixer of this model keeps keys and values that can be held in 4 bits")
         elt = torch.empty((), dtype=self.dtype).element_size()
         needs: Dict[Hashable, GroupNeed] = {}
         state_bytes = 0
@@ -97,7 +105,7 @@ class ModelRunner:
             if isinstance(s, PagedKVSpec):
                 g = needs.setdefault(s.group_key, GroupNeed(s.group_key, 0, s.window, s.keep_first if s.window is not None else 0,
                                                             s.every))
-                g.bytes_per_token += s.planes * s.num_kv_heads * s.head_dim * elt
+                g.bytes_per_token += s.bytes_per_entry(elt)
             elif isinstance(s, StateSpec):
                 n = 1
                 for d in s.shape:

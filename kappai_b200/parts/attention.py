@@ -57,6 +57,10 @@ softmax.  The means are kept in a page group of their own, an entry a block, mad
 is written; the keys themselves are given back when both the window and their own block have passed them.  ``bias`` =
 ``"qkv"``: biases on q, k and v, none on the output.
 
+Where the build asks for it (``BuildEnv.kv_bits`` = 4) keys and values are cached in 4 bits (``ops/kv4.py``): quantised as they
+would be stored, every row, its own key among them, reads what the cache holds.  Plain causal attention, with or without a window, over heads of
+32, 64, 96, 128, 192 or 256 values can be; the variants that the kernels over 4 bits do not have are refused.
+
 Sizes and constants (params): hidden_size, num_heads, num_kv_heads, head_dim,
 value_dim, scale, qk_norm_eps (None: no q/k norm), qk_norm ("per_head" |
 "projection" | "after_rotation"), window (None: all keys), cache_window, block (None), values
@@ -75,6 +79,7 @@ import torch
 from ..cache.spec import CompositeSpec, PagedKVSpec, StateSpec
 from ..config.schema import ConfigError, PartSpec
 from ..ops import kernels as K
+from ..ops import kv4 as K4
 from ..ops.linear import linear_weights as linear
 from .base import Part, WeightSpec, make_part, register_part
 
@@ -135,6 +140,7 @@ class PagedAttentionKernels:
     sink_w = None
     cap = 0.0
     kernel_scale = 1.0
+    bits = 16
 
     def _read_sink(self, what: str):
         """The parameters ``sink`` and ``keep_first`` (shared by the mixers over the paged cache)."""
@@ -172,6 +178,11 @@ class PagedAttentionKernels:
         it; ``pooled``: the means of blocks behind the window); returns the heads side by side."""
         H, G, hd = self.H, self.G, self.hd
         o = torch.empty_like(q)
+        if self.bits == 4:
+            lens = ctx.host_cu_rows
+            least = 1 if ctx.decode_only else min(b - a for a, b in zip(lens, lens[1:]))
+            return K4.kv4_attention(q, cache.tensor, view.block_table, ctx.cu_rows, ctx.seg_pos, o, self.scale, self.window, view.page_size, H, G, hd,
+                                    ctx.max_seg_len, min(ctx.max_context, view.block_table.shape[1] * view.page_size), min_rows=least)
         extra = dict(keep_first=self.keep_first, sink=self.sink_w, cap=self.cap, out_scale=self.kernel_scale, pooled=pooled)
         tiles = ctx.tables.get(self.step_tables_key)
         if self.split_ok and (tiles is None or q.dtype == torch.float32):
@@ -340,6 +351,14 @@ class Attention(PagedAttentionKernels, Part):
         if self.pool is not None and (self.pool < 1 or self.window is None or self.keep_first or self.block is not None or self.borrows):
             raise ConfigError("attention: pool (a positive number of positions) goes with a window and keys of the mixer's own, "
                               "and not with keep_first or blocks of positions")
+        self.bits = int(env.kv_bits)
+        if self.bits == 4:
+            unlike = [what for what, there in ((f"heads stored as {self.hd} values", self.hd not in K4.KV4_HEAD_DIMS), ("blocks of positions", self.block is not None),
+                                               ("kept first keys", self.keep_first), ("a sink", self.sink is not None), ("a soft cap", self.cap),
+                                               ("pooled blocks", self.pool is not None), ("an output factor", self.kernel_scale != 1.0),
+                                               ("whole softmax weights", self.exact_weights)) if there]
+            if unlike:
+                raise ConfigError(f"attention: a cache in 4 bits does not go with {', '.join(unlike)}")
         self._tile_setup()
 
     def weight_specs(self) -> Dict[str, WeightSpec]:
@@ -419,13 +438,15 @@ class Attention(PagedAttentionKernels, Part):
             self.q_w = self._pad_heads(w["q_norm.weight"].float(), 1, self.dim)
             self.k_w = self._pad_heads(w["k_norm.weight"].float(), 1, self.dim)
         self._bind_sink(w, self.w_qkv.device)
+        if self.bits == 4 and "kv4_rows" not in self.env.shared:
+            self.env.shared["kv4_rows"] = torch.arange(K.MAX_STEP_ROWS, dtype=torch.int32, device=self.w_qkv.device)
 
     def cache_spec(self):
         # (a borrower names what it reads, so that the engine can see that lender and borrower agree)
         # (a block's keys stay until its mean is made, also where the window is shorter than a block)
         window = self.cache_window if self.pool is None or self.cache_window is None else max(self.cache_window, self.pool)
         parts = [PagedKVSpec(self.G, self.hd, window, None if self.block is None else int(self.block),
-                             self.keep_first if self.cache_window is not None else 0)]
+                             self.keep_first if self.cache_window is not None else 0, bits=self.bits)]
         if self.pool is not None:
             parts.append(PagedKVSpec(self.G, self.hd, every=self.pool))
         if self.taps > 1:
@@ -466,24 +487,32 @@ class Attention(PagedAttentionKernels, Part):
         view = ctx.paged[cache.group]
         q = torch.empty((ctx.n_rows, H * hd), dtype=qkv.dtype, device=qkv.device)
         kv_out = cache.tensor if cache.writes else None
+        slots, page_size, rows4 = view.slot_map, view.page_size, None
+        if self.bits == 4 and cache.writes:
+            # this step's keys and values as they would be stored, row by row (pages of one key), to be quantised from there
+            kv_out = rows4 = torch.empty((ctx.n_rows, 2, G, 1, hd), dtype=qkv.dtype, device=qkv.device)
+            slots, page_size = self.env.shared["kv4_rows"][:ctx.n_rows], 1
         if self.borrows and cache.writes:
             raise ValueError("attention: a mixer with kv='borrowed' was given a cache of its own")
         if self.qk_norm == "projection":
             K.qk_rownorm_kv(qkv, self.k_col, self.v_col, self.q_w, self.k_w, self.qk_norm_eps, H * self.dim, G * self.dim,
-                            view.slot_map, q, kv_out, view.page_size, H, G, hd)
+                            slots, q, kv_out, page_size, H, G, hd)
         elif hasattr(self.position, "fused_rotary"):
             cos, sin, rot, inter = self.position.fused_rotary()
             K.qk_norm_rope_kv(qkv, self.q_w, self.k_w, self.qk_norm_eps or 0.0, cos, sin, rot, inter,
-                              ctx.positions, view.slot_map, q, kv_out, view.page_size, H, G, hd, self.v_col,
+                              ctx.positions, slots, q, kv_out, page_size, H, G, hd, self.v_col,
                               norm_dim=self.dim, q_temp=self.q_temp, norm_after=self.norm_after)
         else:
             # a position encoding of its own: norm in place, let it change q and k, then scatter
             if self.q_w is not None:
                 K.qk_norm_rope_kv(qkv, self.q_w, self.k_w, self.qk_norm_eps, None, None, 0, False, ctx.positions,
-                                  None, None, None, view.page_size, H, G, hd)
+                                  None, None, None, page_size, H, G, hd)
             self.position.apply(qkv[:, :H * hd], qkv[:, H * hd:(H + G) * hd], ctx)
-            K.qk_norm_rope_kv(qkv, None, None, 0.0, None, None, 0, False, ctx.positions, view.slot_map, q, kv_out,
-                              view.page_size, H, G, hd)
+            K.qk_norm_rope_kv(qkv, None, None, 0.0, None, None, 0, False, ctx.positions, slots, q, kv_out,
+                              page_size, H, G, hd)
+        if rows4 is not None:
+            kv = rows4.view(ctx.n_rows, 2 * G * hd)
+            K4.kv4_write(kv[:, :G * hd], kv[:, G * hd:], cache.tensor, view.slot_map, view.page_size, G, hd)
         pooled = None
         if means is not None:
             pv = ctx.paged[means.group]

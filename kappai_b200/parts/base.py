@@ -71,6 +71,7 @@ class BuildEnv:
     dtype: torch.dtype                  # compute dtype: torch.bfloat16 or torch.float32
     max_positions: int                  # positions 0..max_positions-1 may be run
     shared: Dict[Any, Any] = field(default_factory=dict)   # tables shared between parts (e.g. rotary)
+    kv_bits: int = 16                   # 4: attention keeps its keys and values in 4 bits
 
 
 class Part:
