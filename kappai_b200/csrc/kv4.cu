@@ -571,9 +571,9 @@ kv4_tiled_kernel(const Kv4Args p) {
     kp_pdl_begin();
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the warp's number in a uniform register)
-    const int R = p.H / p.G, kvh = blockIdx.y;
+    const int R = p.H / p.G, kvh = blockIdx.x % p.G;       // (the longest tiles first, of all heads)
     int seg, cta_col0 = 0;
-    kv4_find_tile(p, blockIdx.x, S::COLS, R, lane, seg, cta_col0);
+    kv4_find_tile(p, blockIdx.x / p.G, S::COLS, R, lane, seg, cta_col0);
     if (seg < 0) return;
     const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg], n_cols = n_rows * R;
     const int cta_col1 = min(cta_col0 + S::COLS, n_cols) - 1;
@@ -664,7 +664,8 @@ kv4_mass_kernel(const Kv4Args p) {
     __shared__ __align__(128) unsigned char smem[F::bytes(KEYS)];
     __shared__ float part[4][KEYS];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the warp's number in a uniform register)
-    const int seg = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x * KEYS, R = p.H / p.G;
+    // the first keys first, of all heads and segments: most rows read them
+    const int kvh = blockIdx.x % p.G, seg = blockIdx.x / p.G % p.n_seg, k0 = blockIdx.x / p.G / p.n_seg * KEYS, R = p.H / p.G;
     const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg];
     // keys that any row reads (in front of them the pages may be somebody else's by now)
     const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
@@ -809,7 +810,11 @@ static int kv4_run_split(const Kv4Args& a, long long n_pages, cudaStream_t st) {
 
 template <int HD, int PARTS, typename T>
 static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_tiles, int long_keys, cudaStream_t st) {
+    using S = Kv4Tiled<HD, PARTS>;
+    constexpr int KEYS = HD <= 128 ? 64 : 32;          // of the mass kernel
     const int R = a.H / a.G;
+    const long long tiles = ((long long)n_rows * R + S::COLS - 1) / S::COLS + a.n_seg, places = (long long)((long_keys + KEYS - 1) / KEYS) * a.G * a.n_seg;
+    if (long_tiles > 0 && (tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL))) return KP_ERR_UNSUPPORTED;
     if (a.max_rows > 0) {
         const int e = a.mass ? kv4_run_split<HD, PARTS, true, T>(a, n_pages, st) : kv4_run_split<HD, PARTS, false, T>(a, n_pages, st);
         if (e) return e;
@@ -823,16 +828,13 @@ static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_til
         }
     }
     if (long_tiles > 0) {
-        using S = Kv4Tiled<HD, PARTS>;
         static std::atomic<unsigned long long> ready{0}, ready_mass{0};
-        const int tiles = (n_rows * R + S::COLS - 1) / S::COLS + a.n_seg;
         // (with mass the scores are those that the mass is computed from again)
-        int e = a.mass ? kv4_launch(kv4_tiled_kernel<HD, PARTS, true, T>, dim3(tiles, a.G), S::SMEM, ready, st, a)
-                       : kv4_launch(kv4_tiled_kernel<HD, PARTS, (PARTS > 1), T>, dim3(tiles, a.G), S::SMEM, ready, st, a);
+        int e = a.mass ? kv4_launch(kv4_tiled_kernel<HD, PARTS, true, T>, dim3((unsigned)(tiles * a.G)), S::SMEM, ready, st, a)
+                       : kv4_launch(kv4_tiled_kernel<HD, PARTS, (PARTS > 1), T>, dim3((unsigned)(tiles * a.G)), S::SMEM, ready, st, a);
         if (e) return e;
         if (a.mass) {
-            constexpr int KEYS = HD <= 128 ? 64 : 32;
-            e = kv4_launch(kv4_mass_kernel<HD, PARTS, T>, dim3((long_keys + KEYS - 1) / KEYS, a.G, a.n_seg), 0, ready_mass, st, a);
+            e = kv4_launch(kv4_mass_kernel<HD, PARTS, T>, dim3((unsigned)places), 0, ready_mass, st, a);
             if (e) return e;
         }
     }

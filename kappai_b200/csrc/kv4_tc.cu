@@ -277,9 +277,9 @@ kv4_tc_kernel(const Kv4TcArgs p) {
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     kp_pdl_begin();
-    const int R = p.H / p.G, kvh = blockIdx.y;
+    const int R = p.H / p.G, kvh = blockIdx.x % p.G, tile = blockIdx.x / p.G;        // (the longest tiles first, of all heads)
     int seg, cta_col0;
-    kt_find(p, blockIdx.x, R, lane, seg, cta_col0);
+    kt_find(p, tile, R, lane, seg, cta_col0);
     if (seg < 0) return;                               // (the grid is an upper bound)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
@@ -420,7 +420,7 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         const float f = kt_write_query<HD>(Qs + g * S::OPER, r, live ? p.q + row * p.ldq + (size_t)h * HD : nullptr, p.scale);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kp_mbar_arrive(&q_full[g]);
-        const size_t tile_id = ((size_t)blockIdx.y * p.n_tiles + blockIdx.x) * 2 + g;
+        const size_t tile_id = ((size_t)kvh * p.n_tiles + tile) * 2 + g;
         if (p.mass) {
             // the pass that adds up the mass takes the same operand; this thread's row of it, as it lies
             unsigned char* im = p.q_image + tile_id * S::OPER;
@@ -617,7 +617,9 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     volatile int* tops = abort_flag + 1;               // [4]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     kp_pdl_begin();
-    const int n_ctas = p.cluster, rank = blockIdx.x % n_ctas, seg = blockIdx.z, kvh = blockIdx.y, k0 = blockIdx.x / n_ctas * KT_ROWS, R = p.H / p.G;
+    const int n_ctas = p.cluster, rank = blockIdx.x % n_ctas, R = p.H / p.G;
+    // the first keys first, of all heads and segments: most rows read them
+    const int place = blockIdx.x / n_ctas, kvh = place % p.G, seg = place / p.G % p.n_seg, k0 = place / p.G / p.n_seg * KT_ROWS;
     const int n_rows = p.cu_rows[seg + 1] - p.cu_rows[seg], pos0 = p.seg_pos[seg], n_cols = n_rows * R;
     // keys that any row reads, and columns that read any of this CTA's, in tiles of 128 from column 0; this CTA has every n_ctas-th tile
     const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
@@ -730,20 +732,24 @@ template <int HD>
 static int kt_run(const Kv4TcArgs& a, int max_context, cudaStream_t st) {
     using S = Kt<HD>;
     static std::atomic<unsigned long long> ready{0}, ready_mass{0};
+    // The mass in clusters of four where that many CTAs fit the GPU at once and each has four tiles of columns or more, else one CTA a tile of
+    // keys: a CTA's start (its keys' codes, the first images) takes as long as several tiles of columns.  Measured, attention and mass, one
+    // CTA against four: 2048 rows of 32 heads over 8 126 us against 93, 512 rows 41 against 30; 8 x 256 rows 45 against 48, 300 rows behind
+    // 4096 keys 137 against 154, 4 x 1024 behind 1024 223 against 243.
+    const int tiles = (max_context + KT_ROWS - 1) / KT_ROWS;
+    const long long places = (long long)tiles * a.n_seg * a.G;
+    if ((long long)a.n_tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL)) return KP_ERR_UNSUPPORTED;
     int e = kp_smem_limit(kv4_tc_kernel<HD>, S::SMEM, ready);
     if (e) return e;
-    cudaError_t c = kp_launch_pdl(kv4_tc_kernel<HD>, dim3(a.n_tiles, a.G), dim3(S::THREADS), S::SMEM, st, a);
+    cudaError_t c = kp_launch_pdl(kv4_tc_kernel<HD>, dim3((unsigned)a.n_tiles * a.G), dim3(S::THREADS), S::SMEM, st, a);
     if (c) return (int)c;
     if (a.mass) {
         e = kp_smem_limit(kv4_tc_mass_kernel<HD>, S::MASS_SMEM, ready_mass);
         if (e) return e;
-        // Clusters of four where that many CTAs are there at once, else one CTA a tile of keys: a CTA's start (its keys' codes, the first
-        // images) takes as long as a dozen tiles of columns.
-        const int tiles = (max_context + KT_ROWS - 1) / KT_ROWS;
         Kv4TcArgs m = a;
-        m.cluster = (long long)tiles * a.G * a.n_seg <= 148 ? 4 : 1;
+        m.cluster = places <= 148 && a.n_tiles - a.n_seg >= 8 * a.n_seg ? 4 : 1;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(tiles * m.cluster, a.G, a.n_seg);
+        cfg.gridDim = dim3((unsigned)places * m.cluster);
         cfg.blockDim = dim3(S::MASS_THREADS);
         cfg.dynamicSmemBytes = S::MASS_SMEM;
         cfg.stream = st;
