@@ -20,8 +20,6 @@
 // (O is rescaled when it does): fp16 then holds whatever bfloat16 did.  P is taken against a reference that follows the row's maximum
 // in steps of at least 2^8 (O is rescaled in tensor memory only then), P <= 2^15.
 // Every mbarrier wait is bounded; one that gives up sets the status word, and the CTA frees its tensor memory and returns.
-#include <type_traits>
-
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 
@@ -72,12 +70,6 @@ __device__ __forceinline__ int kt_ext_at(int row, int chunk) { return row * 32 +
 __device__ __forceinline__ int kt_at(int row, int chunk) { return (chunk >> 3) * 16384 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); }
 
 __device__ __forceinline__ float kt_pow2(int e) { return __uint_as_float((uint32_t)(max(-126, min(127, e)) + 127) << 23); }
-__device__ __forceinline__ float kt_max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ uint32_t kt_h2(float lo, float hi) { return pack_f16(lo, hi); }
 
 // eight codes as fp16 pairs (0, 4), (1, 5), (2, 6), (3, 7), times s (s16: s / 16), plus z
 __device__ __forceinline__ uint4 kt_codes(uint32_t w, __half2 s, __half2 s16, __half2 z, bool add) {
@@ -145,50 +137,58 @@ __device__ __forceinline__ void kt_write_key(unsigned char* tile, int row, const
     *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 0)) = make_uint4(ext[0], ext[1], ext[2], ext[3]);
     *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 1)) = make_uint4(0u, 0u, 0u, 0u);
 }
-// and a query (null: zeros).  Returns the factor that makes scores (base 2) of the product with a tile scaled by 2^(7 - e): factor 2^(e - 7).
+// and the queries of a warp's 32 columns, HD / 8 lanes a query (from memory whole lines at a time: a lane with a query of its own would ask for
+// 32 lines an instruction).  `at`: where this lane's own query lies, in elements of q; -1: none, zeros.  Returns the factor that makes its
+// scores (base 2) of the product with a tile scaled by 2^(7 - e): factor 2^(e - 7).
 template <int HD>
-__device__ __forceinline__ float kt_write_query(unsigned char* tile, int row, const bf16* src, float scale) {
-    auto eight = [&](float (&v)[8], int i) {
-        const uint4 x = src ? *reinterpret_cast<const uint4*>(src + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) { v[2 * j] = kv4_scale(w[j]); v[2 * j + 1] = kv4_least(w[j]); }
-    };
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < HD / 8; i++) {
-        float v[8];
-        eight(v, i);
-#pragma unroll
-        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[j]));
-    }
-    int e = 0;
-    if (top > 0.f && top < INFINITY) e = min(6 - ilogbf(top), 100);          // the largest value to [2^6, 2^7): a sum of 64 then fits fp16
-    const float up = kt_pow2(e);
-    uint32_t ext[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int y = 0; y < HD / 64; y++) {
-        float sum = 0.f;
+__device__ __forceinline__ float kt_write_queries(unsigned char* tile, int row0, const bf16* q, long long at, float scale, int lane) {
+    constexpr int LANES = HD / 8, STEP = 32 / LANES;
+    const int chunk = lane % LANES, sub = lane / LANES;
+    int mine = 0;
+#pragma unroll 1
+    for (int base = 0; base < 32; base += 8 * STEP) {
+        uint4 raw[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            float x[8];
-            eight(x, y * 8 + i);
+            const long long from = __shfl_sync(0xffffffffu, at, base + i * STEP + sub);
+            raw[i] = from >= 0 ? *reinterpret_cast<const uint4*>(q + from + 8 * chunk) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            float x[8], top = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) { x[2 * j] = kv4_scale(w[j]); x[2 * j + 1] = kv4_least(w[j]); }
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) top = kv4_max3(top, fabsf(x[j]), fabsf(x[j + 1]));
+#pragma unroll
+            for (int d = 1; d < LANES; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            // the largest value to [2^6, 2^7): a sum of 64 then fits fp16
+            const int e = top > 0.f && top < INFINITY ? min(133 - (int)(__float_as_uint(top) >> 23), 100) : 0;
+            const float up = kt_pow2(e);
+            const int theirs = __shfl_sync(0xffffffffu, e, lane % STEP * LANES);
+            if (lane / STEP == base / STEP + i) mine = theirs;
+            float sum = 0.f;
             uint32_t r[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                r[j] = kt_h2(x[j] * up, x[j + 4] * up);
+                r[j] = pack_f16(x[j] * up, x[j + 4] * up);
                 const __half2 h = *reinterpret_cast<const __half2*>(&r[j]);
                 sum += __low2float(h) + __high2float(h);
             }
-            *reinterpret_cast<uint4*>(tile + kt_at(row, y * 8 + i)) = make_uint4(r[0], r[1], r[2], r[3]);
+            const int row = row0 + base + i * STEP + sub;
+            *reinterpret_cast<uint4*>(tile + kt_at(row, chunk)) = make_uint4(r[0], r[1], r[2], r[3]);
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);               // of the 64 values of a group
+            const __half sh = __float2half_rn(sum), sl = __float2half_rn(sum - __half2float(sh));
+            const __half2 both = __halves2half2(sh, sl);
+            const uint32_t first = *reinterpret_cast<const uint32_t*>(&both), second = HD == 64 ? 0u : __shfl_xor_sync(0xffffffffu, first, 8);
+            if (chunk < 2)
+                *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, chunk)) =
+                    chunk == 0 ? make_uint4(first, first, second, second) : make_uint4(0u, 0u, 0u, 0u);
         }
-        const __half sh = __float2half_rn(sum), sl = __float2half_rn(sum - __half2float(sh));
-        const __half2 both = __halves2half2(sh, sl);
-        ext[2 * y] = ext[2 * y + 1] = *reinterpret_cast<const uint32_t*>(&both);
     }
-    *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 0)) = make_uint4(ext[0], ext[1], ext[2], ext[3]);
-    *reinterpret_cast<uint4*>(tile + Kt<HD>::TILE + kt_ext_at(row, 1)) = make_uint4(0u, 0u, 0u, 0u);
-    return scale * KV4_LOG2E * kt_pow2(-e);
+    return scale * KV4_LOG2E * kt_pow2(-mine);
 }
 // S of 128 x 128.  A warp in step issues it, by an elected lane: from inside a branch that one lane took, the operands would pass through general
 // registers, at three times the cycles an MMA.
@@ -417,22 +417,16 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         const int pos = live ? min(pos0 + c / R, k_hi) : -1;
         const size_t row = (size_t)(row0 + (live ? c / R : 0));
         const int h = kvh * R + (live ? c % R : 0);
-        const float f = kt_write_query<HD>(Qs + g * S::OPER, r, live ? p.q + row * p.ldq + (size_t)h * HD : nullptr, p.scale);
+        unsigned char* Qg = Qs + g * S::OPER;
+        const float f = kt_write_queries<HD>(Qg, q4 * 32, p.q, live ? (long long)row * p.ldq + h * HD : -1LL, p.scale, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kp_mbar_arrive(&q_full[g]);
         const size_t tile_id = ((size_t)kvh * p.n_tiles + tile) * 2 + g;
-        if (p.mass) {
-            // the pass that adds up the mass takes the same operand; this thread's row of it, as it lies
-            unsigned char* im = p.q_image + tile_id * S::OPER;
-            const unsigned char* from = Qs + g * S::OPER;
-#pragma unroll
-            for (int y = 0; y < S::NG; y++)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    *reinterpret_cast<uint4*>(im + y * 16384 + r * 128 + e * 16) = *reinterpret_cast<const uint4*>(from + y * 16384 + r * 128 + e * 16);
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                *reinterpret_cast<uint4*>(im + S::TILE + r * 32 + e * 16) = *reinterpret_cast<const uint4*>(from + S::TILE + r * 32 + e * 16);
+        if (p.mass && r == 0) {
+            // the pass that adds up the mass takes the same operand, as it lies
+            kp_mbar_wait_bounded(&q_full[g], 0);       // (nothing that arrives there waits)
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n cp.async.bulk.commit_group;"
+                         ::"l"(p.q_image + tile_id * S::OPER), "r"(kp_smem_u32(Qg)), "r"((uint32_t)S::OPER) : "memory");
         }
         const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         // keys that every column of the group reads
@@ -471,7 +465,7 @@ kv4_tc_kernel(const Kv4TcArgs p) {
                 for (int e = 0; e < 2; e++) {
                     t[e] = fmaxf(__uint_as_float(s[e][0]), __uint_as_float(s[e][1]));
 #pragma unroll
-                    for (int j = 2; j < 32; j += 2) t[e] = kt_max3(t[e], __uint_as_float(s[e][j]), __uint_as_float(s[e][j + 1]));
+                    for (int j = 2; j < 32; j += 2) t[e] = kv4_max3(t[e], __uint_as_float(s[e][j]), __uint_as_float(s[e][j + 1]));
                 }
                 return fmaxf(t[0], t[1]);
             };
@@ -534,21 +528,32 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         const bool none = m == -INFINITY && l == 0.f;                            // (not: scores that are NaN)
         const float inv = none ? 0.f : kt_pow2(ev - 14) / l;
         if (p.mass) p.col[tile_id * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
-        bf16* dst = p.out + row * p.ldo + (size_t)h * HD;
+        // the rows pass through the operand's place, which nothing reads any more, so that memory gets whole lines
+        if (p.mass) {
+            if (r == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");
+        }
 #pragma unroll 1
         for (int e = 0; e < HD; e += 32) {
             uint32_t v[32];
             if (n_kt > 0) kp_tmem_ld32(tmem_o + e, v);
-            if (ok && live) {
 #pragma unroll
-                for (int d = 0; d < 32; d += 8) {
-                    // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
-                    float x[8];
+            for (int d = 0; d < 32; d += 8) {
+                // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
+                float x[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[(j >> 1) + (j & 1) * 4] = none ? 0.f : __uint_as_float(v[d + j]) * inv;
-                    *reinterpret_cast<uint4*>(dst + e + d) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-                }
+                for (int j = 0; j < 8; j++) x[(j >> 1) + (j & 1) * 4] = none ? 0.f : __uint_as_float(v[d + j]) * inv;
+                *reinterpret_cast<uint4*>(Qg + kt_at(r, (e + d) / 8)) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
             }
+        }
+        __syncwarp();
+        constexpr int LANES = HD / 8, STEP = 32 / LANES;
+        const long long to = ok && live ? (long long)row * p.ldo + h * HD : -1LL;
+#pragma unroll
+        for (int i = 0; i < 32; i += STEP) {
+            const int of = i + lane / LANES;
+            const long long at = __shfl_sync(0xffffffffu, to, of);
+            if (at >= 0) *reinterpret_cast<uint4*>(p.out + at + 8 * (lane % LANES)) = *reinterpret_cast<const uint4*>(Qg + kt_at(q4 * 32 + of, lane % LANES));
         }
         kp_tc_fence_before();
         if (__builtin_expect(!ok, 0)) { if (lane == 0) atomicExch(&g_kv4_tc_status, 1); }
