@@ -222,27 +222,28 @@ __device__ __forceinline__ float2 kt_add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
-// segment and first column of a tile of 256 columns (kv4.cu's tiles: the last columns of a segment first); -1: none
-__device__ __forceinline__ void kt_find(const Kv4TcArgs& p, int tile, int R, int lane, int& seg, int& col0) {
-    seg = -1; col0 = 0;
+// segment, its first row, number of rows and position, and first column, of a tile of 256 columns (kv4.cu's tiles: the last columns of a segment
+// first); seg = -1: none
+struct KtTile { int seg, row0, n_rows, pos0, col0; };
+__device__ __forceinline__ KtTile kt_find(const Kv4TcArgs& p, int tile, int R, int lane) {
     int before = 0;
     for (int base = 0; base < p.n_seg; base += 32) {
         const int i = base + lane;
-        const int rows = i < p.n_seg ? p.cu_rows[i + 1] - p.cu_rows[i] : 0;
+        int row0 = 0, rows = 0, pos = 0;
+        if (i < p.n_seg) { row0 = p.cu_rows[i]; rows = p.cu_rows[i + 1] - row0; pos = p.seg_pos[i]; }
         const int mine = rows >= p.min_rows ? (rows * R + 255) / 256 : 0;
         int run = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) { const int o = __shfl_up_sync(0xffffffffu, run, d); if (lane >= d) run += o; }
         const unsigned hit = __ballot_sync(0xffffffffu, tile < before + run);
         if (hit) {
-            const int src = __ffs(hit) - 1;
-            const int end = before + __shfl_sync(0xffffffffu, run, src);
-            seg = base + src;
-            col0 = (end - 1 - tile) * 256;
-            return;
+            const int src = __ffs(hit) - 1, end = before + __shfl_sync(0xffffffffu, run, src);
+            return {base + src, __shfl_sync(0xffffffffu, row0, src), __shfl_sync(0xffffffffu, rows, src), __shfl_sync(0xffffffffu, pos, src),
+                    (end - 1 - tile) * 256};
         }
         before += __shfl_sync(0xffffffffu, run, 31);
     }
+    return {-1, 0, 0, 0, 0};
 }
 // the tile of segment `seg`'s first 256 columns (its tiles run downwards from there)
 __device__ __forceinline__ int kt_first_tile(const Kv4TcArgs& p, int seg, int R, int lane) {
@@ -278,9 +279,9 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     kp_pdl_begin();
     const int R = p.H / p.G, kvh = blockIdx.x % p.G, tile = blockIdx.x / p.G;        // (the longest tiles first, of all heads)
-    int seg, cta_col0;
-    kt_find(p, tile, R, lane, seg, cta_col0);
-    if (seg < 0) return;                               // (the grid is an upper bound)
+    const KtTile t = kt_find(p, tile, R, lane);
+    if (t.seg < 0) return;                             // (the grid is an upper bound)
+    const int seg = t.seg, cta_col0 = t.col0, row0 = t.row0, n_cols = t.n_rows * R, pos0 = t.pos0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             kp_mbar_init(&q_full[i], 128);
@@ -298,7 +299,6 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     kp_tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;             // S of the groups: 2 x 128 columns; then O: 2 x HD
 
-    const int row0 = p.cu_rows[seg], n_cols = (p.cu_rows[seg + 1] - row0) * R, pos0 = p.seg_pos[seg];
     const int n_here = min(256, n_cols - cta_col0);    // columns of this CTA
     const int k_hi = min(pos0 + (cta_col0 + n_here - 1) / R, p.max_blocks * p.ps - 1);
     const int k_lo = p.window > 0 ? max(0, pos0 + cta_col0 / R - p.window + 1) : 0;
