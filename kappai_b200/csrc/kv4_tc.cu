@@ -37,6 +37,7 @@ struct Kv4TcArgs {
     float scale; int window; int ps, ps_log2; int H, G;
     unsigned char* q_image; float2* col;               // with mass: the groups' Q operands and (factor, lse) of their columns
     float* mass;
+    int split;                                         // CTAs that share the keys of a tile of columns
     int cluster;                                       // CTAs that share the columns of a tile of keys
     int min_rows, n_seg, n_tiles;                      // n_tiles: an upper bound of the CTAs' tiles
 };
@@ -222,6 +223,20 @@ __device__ __forceinline__ float2 kt_add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
+__device__ __forceinline__ void kt_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+// a float at this place of the shared memory of the cluster's CTA `rank`
+__device__ __forceinline__ float kt_peer(const float* p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(kp_cluster_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 kt_peer4(const float* p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(kp_cluster_addr(p, rank)) : "memory");
+    return v;
+}
 // segment, its first row, number of rows and position, and first column, of a tile of 256 columns (kv4.cu's tiles: the last columns of a segment
 // first); seg = -1: none
 struct KtTile { int seg, row0, n_rows, pos0, col0; };
@@ -255,9 +270,69 @@ __device__ __forceinline__ int kt_first_tile(const Kv4TcArgs& p, int seg, int R,
     return __reduce_add_sync(0xffffffffu, sum) - 1;
 }
 
+// Rows of this CTA's columns from the shares of the cluster's n CTAs (at most MOST), four dimensions a thread; BATCH loads from each are under way at once
+template <int HD, int MOST, int BATCH, typename RowOf>
+__device__ __forceinline__ void kt_join(const float* part, const float* weight, int rank, int n, int n_cols, int cta_col0, RowOf row_of) {
+    constexpr int LANES = HD / 4;
+    for (int i0 = threadIdx.x; i0 < n_cols * LANES; i0 += 256 * BATCH) {
+        float4 v[BATCH][MOST];
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+            const int i = i0 + b * 256, col = rank + i / LANES * n;
+#pragma unroll
+            for (int j = 0; j < MOST; j++)
+                if (i < n_cols * LANES && j < n) v[b][j] = kt_peer4(part + col * HD + ((i % LANES ^ (col & 7)) * 4), j);
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+            const int i = i0 + b * 256, col = rank + i / LANES * n;
+            if (i >= n_cols * LANES) break;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < MOST; j++)
+                if (j < n) {
+                    const float y = weight[col * 8 + j];
+                    x = make_float4(fmaf(y, v[b][j].x, x.x), fmaf(y, v[b][j].y, x.y), fmaf(y, v[b][j].z, x.z), fmaf(y, v[b][j].w, x.w));
+                }
+            *reinterpret_cast<uint2*>(row_of(cta_col0 + col) + 4 * (i % LANES)) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+        }
+    }
+}
+
+// The shares of a tile's rows of the cluster's CTAs, each weighted by its part of the sum, added in order, by 256 threads.  The CTAs share the
+// columns out: this one has every n-th.  (A call: inlined, it costs the loop over the keys registers.)
 template <int HD>
+__device__ __noinline__ void kt_join_shares(const Kv4TcArgs& p, unsigned char* sm, int rank, int kvh, int tile, int row0, int cta_col0, int n_here) {
+    const int n = p.split, R = p.H / p.G;
+    const float* part = reinterpret_cast<const float*>(sm);
+    float* stat = reinterpret_cast<float*>(sm) + 256 * HD;
+    float* weight = stat + 768;                    // [column][8]
+    const int col = rank + threadIdx.x * n;
+    if (col < 256) {
+        float m[8], l[8], top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < n) { m[j] = kt_peer(stat + col, j); l[j] = kt_peer(stat + 256 + col, j); }
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (j < n) top = fmaxf(top, m[j]);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < n) { l[j] *= kv4_exp2(m[j] - (top == -INFINITY ? 0.f : top)); sum += l[j]; }
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (j < n) weight[col * 8 + j] = sum == 0.f ? 0.f : l[j] / sum;
+        if (p.mass) p.col[((size_t)kvh * p.n_tiles + tile) * 256 + col] = make_float2(stat[512 + col], sum == 0.f ? INFINITY : top - 7.0f + log2f(sum));
+    }
+    asm volatile("bar.sync 4, 256;" ::: "memory");
+    auto row_of = [&](int c) { return p.out + (size_t)(row0 + c / R) * p.ldo + (size_t)(kvh * R + c % R) * HD; };
+    const int n_cta = (n_here + n - 1 - rank) / n;       // this CTA's columns
+    if (n == 2) kt_join<HD, 2, 4>(part, weight, rank, n, n_cta, cta_col0, row_of);
+    else if (n <= 4) kt_join<HD, 4, 2>(part, weight, rank, n, n_cta, cta_col0, row_of);
+    else kt_join<HD, 8, 1>(part, weight, rank, n, n_cta, cta_col0, row_of);
+}
+
+template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(Kt<HD>::THREADS, 1)
-kv4_tc_kernel(const Kv4TcArgs p) {
+kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
     using S = Kt<HD>;
     constexpr int ST = S::ST;
     extern __shared__ unsigned char smem_dyn[];
@@ -278,7 +353,9 @@ kv4_tc_kernel(const Kv4TcArgs p) {
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     kp_pdl_begin();
-    const int R = p.H / p.G, kvh = blockIdx.x % p.G, tile = blockIdx.x / p.G;        // (the longest tiles first, of all heads)
+    // (the longest tiles first, of all heads)
+    const int n_split = SPLIT ? p.split : 1, rank = blockIdx.x % n_split, place = blockIdx.x / n_split;
+    const int R = p.H / p.G, kvh = place % p.G, tile = place / p.G;
     const KtTile t = kt_find(p, tile, R, lane);
     if (t.seg < 0) return;                             // (the grid is an upper bound)
     const int seg = t.seg, cta_col0 = t.col0, row0 = t.row0, n_cols = t.n_rows * R, pos0 = t.pos0;
@@ -302,7 +379,9 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     const int n_here = min(256, n_cols - cta_col0);    // columns of this CTA
     const int k_hi = min(pos0 + (cta_col0 + n_here - 1) / R, p.max_blocks * p.ps - 1);
     const int k_lo = p.window > 0 ? max(0, pos0 + cta_col0 / R - p.window + 1) : 0;
-    const int kt_lo = k_lo / KT_ROWS, n_kt = k_hi >= k_lo ? k_hi / KT_ROWS - kt_lo + 1 : 0;
+    // tiles of keys, and this CTA's of them
+    const int kt_all = k_hi >= k_lo ? k_hi / KT_ROWS - k_lo / KT_ROWS + 1 : 0;
+    const int kt_skip = kt_all * rank / n_split, kt_lo = k_lo / KT_ROWS + kt_skip, n_kt = kt_all * (rank + 1) / n_split - kt_skip;
 
     if (warp >= 8 && warp < 12) {
         // ---- codes to operands: thread d has key d of every tile.  Keys run two tiles ahead of the values' next: with one stage each K's is
@@ -415,14 +494,14 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         const int c = cta_col0 + g * 128 + r;
         const bool live = c < n_cols;
         const int pos = live ? min(pos0 + c / R, k_hi) : -1;
-        const size_t row = (size_t)(row0 + (live ? c / R : 0));
-        const int h = kvh * R + (live ? c % R : 0);
+        // where column c's row lies in q or in out; -1: nowhere
+        auto place_of = [&](int c, long long ld) { return c < n_cols ? (long long)(row0 + c / R) * ld + (kvh * R + c % R) * HD : -1LL; };
         unsigned char* Qg = Qs + g * S::OPER;
-        const float f = kt_write_queries<HD>(Qg, q4 * 32, p.q, live ? (long long)row * p.ldq + h * HD : -1LL, p.scale, lane);
+        const float f = kt_write_queries<HD>(Qg, q4 * 32, p.q, place_of(c, p.ldq), p.scale, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kp_mbar_arrive(&q_full[g]);
-        const size_t tile_id = ((size_t)kvh * p.n_tiles + tile) * 2 + g;
-        if (p.mass && r == 0) {
+        if (p.mass && rank == 0 && r == 0) {
+            const size_t tile_id = ((size_t)kvh * p.n_tiles + tile) * 2 + g;
             // the pass that adds up the mass takes the same operand, as it lies
             kp_mbar_wait_bounded(&q_full[g], 0);       // (nothing that arrives there waits)
             asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n cp.async.bulk.commit_group;"
@@ -527,33 +606,55 @@ kv4_tc_kernel(const Kv4TcArgs p) {
         kp_tc_fence_after();
         const bool none = m == -INFINITY && l == 0.f;                            // (not: scores that are NaN)
         const float inv = none ? 0.f : kt_pow2(ev - 14) / l;
-        if (p.mass) p.col[tile_id * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
-        // the rows pass through the operand's place, which nothing reads any more, so that memory gets whole lines
-        if (p.mass) {
-            if (r == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-            asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");
-        }
+        if (p.mass && r == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (SPLIT) {
+            // this CTA's share of the rows, and what it counts for: in place of the operands, once neither group's products read them
+            asm volatile("bar.sync 4, 256;" ::: "memory");
+            const int col = g * 128 + r;
+            float* part = reinterpret_cast<float*>(sm) + col * HD;
+            float* stat = reinterpret_cast<float*>(sm) + 256 * HD + col;
 #pragma unroll 1
-        for (int e = 0; e < HD; e += 32) {
-            uint32_t v[32];
-            if (n_kt > 0) kp_tmem_ld32(tmem_o + e, v);
+            for (int e = 0; e < HD; e += 32) {
+                uint32_t v[32];
+                if (n_kt > 0) kp_tmem_ld32(tmem_o + e, v);
 #pragma unroll
-            for (int d = 0; d < 32; d += 8) {
-                // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
-                float x[8];
+                for (int d = 0; d < 32; d += 4) {
+                    // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
+                    float x[4];
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[(j >> 1) + (j & 1) * 4] = none ? 0.f : __uint_as_float(v[d + j]) * inv;
-                *reinterpret_cast<uint4*>(Qg + kt_at(r, (e + d) / 8)) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                    for (int j = 0; j < 4; j++) x[j] = none ? 0.f : __uint_as_float(v[(d & ~7) + 2 * j + (d >> 2 & 1)]) * inv;
+                    *reinterpret_cast<float4*>(part + (((e + d) / 4 ^ (r & 7)) * 4)) = make_float4(x[0], x[1], x[2], x[3]);
+                }
             }
-        }
-        __syncwarp();
-        constexpr int LANES = HD / 8, STEP = 32 / LANES;
-        const long long to = ok && live ? (long long)row * p.ldo + h * HD : -1LL;
+            stat[0] = m; stat[256] = l; stat[512] = f;
+        } else {
+            if (p.mass) {
+                p.col[((size_t)kvh * p.n_tiles + tile) * 256 + g * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + g) : "memory");
+            }
+            // the rows pass through the operand's place, which nothing reads any more, so that memory gets whole lines
+#pragma unroll 1
+            for (int e = 0; e < HD; e += 32) {
+                uint32_t v[32];
+                if (n_kt > 0) kp_tmem_ld32(tmem_o + e, v);
 #pragma unroll
-        for (int i = 0; i < 32; i += STEP) {
-            const int of = i + lane / LANES;
-            const long long at = __shfl_sync(0xffffffffu, to, of);
-            if (at >= 0) *reinterpret_cast<uint4*>(p.out + at + 8 * (lane % LANES)) = *reinterpret_cast<const uint4*>(Qg + kt_at(q4 * 32 + of, lane % LANES));
+                for (int d = 0; d < 32; d += 8) {
+                    // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[(j >> 1) + (j & 1) * 4] = none ? 0.f : __uint_as_float(v[d + j]) * inv;
+                    *reinterpret_cast<uint4*>(Qg + kt_at(r, (e + d) / 8)) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
+                }
+            }
+            __syncwarp();
+            constexpr int LANES = HD / 8, STEP = 32 / LANES;
+            const long long to = ok ? place_of(c, p.ldo) : -1LL;
+#pragma unroll
+            for (int i = 0; i < 32; i += STEP) {
+                const int of = i + lane / LANES;
+                const long long at = __shfl_sync(0xffffffffu, to, of);
+                if (at >= 0) *reinterpret_cast<uint4*>(p.out + at + 8 * (lane % LANES)) = *reinterpret_cast<const uint4*>(Qg + kt_at(q4 * 32 + of, lane % LANES));
+            }
         }
         kp_tc_fence_before();
         if (__builtin_expect(!ok, 0)) { if (lane == 0) atomicExch(&g_kv4_tc_status, 1); }
@@ -561,17 +662,13 @@ kv4_tc_kernel(const Kv4TcArgs p) {
     kp_tc_fence_before();
     __syncthreads();
     if (warp == 12) kp_tmem_dealloc(tmem_base, 512);
+    if (!SPLIT) return;
+
+    kt_cluster_sync();
+    if (warp < 8) kt_join_shares<HD>(p, sm, rank, kvh, tile, row0, cta_col0, n_here);
+    kt_cluster_sync();                                 // (nobody leaves while its shares are read)
 }
 
-__device__ __forceinline__ void kt_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
-// a float at this place of the shared memory of the cluster's CTA `rank`
-__device__ __forceinline__ float kt_peer(const float* p, int rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(kp_cluster_addr(p, rank)) : "memory");
-    return v;
-}
 // The sum of 2^(score - lse) over the 128 columns of a tile, of those from lo to hi (MASKED), for this thread's key: S of tensor memory
 // times kappa and the column's factor is the score.
 template <bool MASKED>
@@ -733,40 +830,68 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     if (n_ctas > 1) kt_cluster_sync();                 // (nobody leaves while its sums are read)
 }
 
+// Launches of `places` clusters of `cluster` CTAs
+struct KtLaunch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    KtLaunch(unsigned places, int cluster, int threads, size_t smem, cudaStream_t st) {
+        cfg.gridDim = dim3(places * cluster);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = cluster > 1 ? 2 : 1;
+    }
+};
+// clusters of n CTAs of the attention kernel that the GPU holds at once (its shared memory's limit has been raised)
 template <int HD>
-static int kt_run(const Kv4TcArgs& a, int max_context, cudaStream_t st) {
+static int kt_fit(int n) {
+    static std::atomic<int> known[64][9];              // 1 more than the answer, by device
+    int dev = 0, fit = 0;
+    if (cudaGetDevice(&dev) || dev >= 64) return 0;
+    if (const int k = known[dev][n]) return k - 1;
+    KtLaunch l(1, n, Kt<HD>::THREADS, Kt<HD>::SMEM, nullptr);
+    if (cudaOccupancyMaxActiveClusters(&fit, kv4_tc_kernel<HD, true>, &l.cfg)) { cudaGetLastError(); fit = 0; }
+    known[dev][n] = fit + 1;
+    return fit;
+}
+
+template <int HD>
+static int kt_run(Kv4TcArgs a, int max_context, long long busy, cudaStream_t st) {
     using S = Kt<HD>;
-    static std::atomic<unsigned long long> ready{0}, ready_mass{0};
+    static std::atomic<unsigned long long> ready{0}, ready_split{0}, ready_mass{0};
+    int e = kp_smem_limit(kv4_tc_kernel<HD, false>, S::SMEM, ready);
+    if (!e) e = kp_smem_limit(kv4_tc_kernel<HD, true>, S::SMEM, ready_split);
+    if (e) return e;
     // The mass in clusters of four where that many CTAs fit the GPU at once and each has four tiles of columns or more, else one CTA a tile of
     // keys: a CTA's start (its keys' codes, the first images) takes as long as several tiles of columns.  Measured, attention and mass, one
     // CTA against four: 2048 rows of 32 heads over 8 126 us against 93, 512 rows 41 against 30; 8 x 256 rows 45 against 48, 300 rows behind
     // 4096 keys 137 against 154, 4 x 1024 behind 1024 223 against 243.
     const int tiles = (max_context + KT_ROWS - 1) / KT_ROWS;
     const long long places = (long long)tiles * a.n_seg * a.G;
+    // A tile's keys over as many CTAs, up to eight, as the GPU holds clusters of, where each has a tile of keys and there are three or more:
+    // the join costs less than the second tile.  Measured with 32 heads over 8, one CTA a tile against the rule's: 64 rows behind 16000 keys
+    // 249 us against 45, 300 behind 4096 111 against 47, 512 behind 1024 32 against 24, 64 behind 512 18.5 against 15; 256 rows and no
+    // more (two tiles of keys) 13.1 against 14.6, 1024 behind 4096, whose pairs would not all be there at once, 87 against 97.
+    const int reach = a.window > 0 && a.window + 256 / (a.H / a.G) < max_context ? a.window + 256 / (a.H / a.G) : max_context;
+    a.split = 1;
+    for (int n = 8; n > 1 && a.split == 1; n--)
+        if (busy * a.G <= kt_fit<HD>(n) && (reach + KT_ROWS - 1) / KT_ROWS >= max(n, 3)) a.split = n;
     if ((long long)a.n_tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL)) return KP_ERR_UNSUPPORTED;
-    int e = kp_smem_limit(kv4_tc_kernel<HD>, S::SMEM, ready);
-    if (e) return e;
-    cudaError_t c = kp_launch_pdl(kv4_tc_kernel<HD>, dim3((unsigned)a.n_tiles * a.G), dim3(S::THREADS), S::SMEM, st, a);
+    const KtLaunch l((unsigned)a.n_tiles * a.G, a.split, S::THREADS, S::SMEM, st);
+    cudaError_t c = cudaLaunchKernelEx(&l.cfg, a.split > 1 ? kv4_tc_kernel<HD, true> : kv4_tc_kernel<HD, false>, a);
     if (c) return (int)c;
     if (a.mass) {
         e = kp_smem_limit(kv4_tc_mass_kernel<HD>, S::MASS_SMEM, ready_mass);
         if (e) return e;
-        Kv4TcArgs m = a;
-        m.cluster = places <= 148 && a.n_tiles - a.n_seg >= 8 * a.n_seg ? 4 : 1;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)places * m.cluster);
-        cfg.blockDim = dim3(S::MASS_THREADS);
-        cfg.dynamicSmemBytes = S::MASS_SMEM;
-        cfg.stream = st;
-        cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = m.cluster;
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = m.cluster > 1 ? 2 : 1;
-        c = cudaLaunchKernelEx(&cfg, kv4_tc_mass_kernel<HD>, m);
+        a.cluster = places <= 148 && a.n_tiles - a.n_seg >= 8 * a.n_seg ? 4 : 1;
+        const KtLaunch l((unsigned)places, a.cluster, S::MASS_THREADS, S::MASS_SMEM, st);
+        c = cudaLaunchKernelEx(&l.cfg, kv4_tc_mass_kernel<HD>, a);
         if (c) return (int)c;
     }
     return kp_launch_status();
@@ -783,13 +908,15 @@ long long kp_kv4_tc_scratch(int n_rows, int n_seg, int H, int G, int hd) {
 // The segments of at least min_rows rows (bfloat16, head size 64 or 128); scratch (with mass): kp_kv4_tc_scratch bytes.
 int kp_kv4_attention_tc(const void* q, long long ldq, const void* pages, const int* block_table, int max_blocks, const int* cu_rows,
                         const int* seg_pos, int n_seg, void* out, long long ldo, float scale, int window, int ps, int H, int G, int hd, int n_rows,
-                        int min_rows, int max_context, float* mass, void* scratch, void* stream) {
+                        int min_rows, int max_rows, int max_context, float* mass, void* scratch, void* stream) {
     if (n_rows <= 0 || n_seg <= 0) return 0;
-    if (G < 1 || H < 1 || H % G || ps < 16 || (ps & (ps - 1)) || window < 0 || n_seg > 65535 || G > 65535 || min_rows < 1 || !(scale > 0.f) ||
+    if (G < 1 || H < 1 || H % G || max_rows < 1 || ps < 16 || (ps & (ps - 1)) || window < 0 || n_seg > 65535 || G > 65535 || min_rows < 1 || !(scale > 0.f) ||
         (((uintptr_t)pages | (uintptr_t)q | (uintptr_t)out | (uintptr_t)scratch) & 15) || (ldq & 7) || (ldo & 7) || (mass && !scratch))
         return KP_ERR_BAD_ARG;
     const int R = H / G;
     const long long tiles = ((long long)n_rows * R + 255) / 256 + n_seg;
+    // about how many tiles there are: as where each segment has max_rows rows
+    const long long busy = max(tiles - n_seg, (long long)(n_rows / max_rows) * (((long long)max_rows * R + 255) / 256));
     Kv4TcArgs a = {};
     a.q = (const bf16*)q; a.ldq = ldq; a.out = (bf16*)out; a.ldo = ldo; a.pages = (const unsigned char*)pages;
     a.block_table = block_table; a.max_blocks = max_blocks; a.cu_rows = cu_rows; a.seg_pos = seg_pos;
@@ -800,8 +927,8 @@ int kp_kv4_attention_tc(const void* q, long long ldq, const void* pages, const i
         a.q_image = (unsigned char*)scratch;
         a.col = (float2*)((unsigned char*)scratch + (size_t)tiles * G * 2 * ((hd / 64) * 16384 + KT_EXT));
     }
-    if (hd == 64) return kt_run<64>(a, max_context, (cudaStream_t)stream);
-    if (hd == 128) return kt_run<128>(a, max_context, (cudaStream_t)stream);
+    if (hd == 64) return kt_run<64>(a, max_context, busy, (cudaStream_t)stream);
+    if (hd == 128) return kt_run<128>(a, max_context, busy, (cudaStream_t)stream);
     return KP_ERR_UNSUPPORTED;
 }
 

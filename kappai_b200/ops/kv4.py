@@ -28,7 +28,7 @@ _LAUNCHERS = {
     "kp_kv4_write": ("kv4", [_P, _L, _P, _L, _P, _L, _P] + [_I] * 5 + [_P]),
     "kp_kv4_read": ("kv4", [_P, _L, _P, _P, _P] + [_I] * 5 + [_P]),
     "kp_kv4_attention": ("kv4", [_P, _L, _P, _L, _P, _I, _P, _P, _I, _P, _L, _F] + [_I] * 12 + [_P, _P, _P, _I, _P, _P, _P, _I, _P]),
-    "kp_kv4_attention_tc": ("kv4_tc", [_P, _L, _P, _P, _I, _P, _P, _I, _P, _L, _F] + [_I] * 8 + [_P, _P, _P]),
+    "kp_kv4_attention_tc": ("kv4_tc", [_P, _L, _P, _P, _I, _P, _P, _I, _P, _L, _F] + [_I] * 9 + [_P, _P, _P]),
     "kp_kv4_evict": ("kv4_evict", [_P, _P, _P, _I, _P, _P, _P, _P, _I, _P] + [_I] * 8 + [_P]),
 }
 _fns = {}
@@ -181,7 +181,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
             size = _tc_scratch(n, n_seg, H, G, hd)
             scratch = torch.empty(size, dtype=torch.uint8, device=q.device).data_ptr()
         _run("kv4_attention_tc", _fn("kp_kv4_attention_tc"), pq, ldq, at, table, width, cu, pos, n_seg, po, ldo, scale, window, page_size, H, G, hd, n,
-             short + 1, max_context, pm, scratch, STREAM)
+             short + 1, max_rows, max_context, pm, scratch, STREAM)
     return out
 
 

@@ -257,6 +257,35 @@ def test_long_contexts(dtype, hd, lengths, rows):
     run_and_check(lengths, rows, 4, 2, hd, 64, dtype, mass=False, seed=9)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lengths,rows,H,G,window", [([385], [20], 4, 1, None), ([400], [64], 4, 1, None), ([640], [70], 4, 2, None), ([700], [9], 12, 3, None),
+                                                     ([800], [40], 5, 1, None), ([2050], [130], 8, 2, None), ([600], [300], 32, 32, None),
+                                                     ([900, 40, 12, 300], [20, 20, 12, 33], 4, 2, None), ([1500, 1400], [30, 9], 4, 2, 200), ([900], [30], 4, 1, 3)])
+def test_keys_that_a_cluster_shares_out(hd, lengths, rows, H, G, window):
+    """Few rows over many keys: two to eight CTAs a tile, some of them without a key of a shorter sequence."""
+    run_and_check(lengths, rows, H, G, hd, 32, torch.bfloat16, window)
+    run_and_check(lengths, rows, H, G, hd, 32, torch.bfloat16, window, mass=False, seed=8, strided=True)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_query_that_is_not_finite_before_many_keys(hd, bad):
+    H, G, rows, n = 4, 2, 30, 1000
+    P = Paged([n], G, hd, 16, 3, torch.bfloat16)
+    q = torch.randn((rows, H * hd), generator=torch.Generator().manual_seed(1)).bfloat16()
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    out = []
+    for x in (q, q.clone()):
+        if out:
+            x[2, hd + 3] = bad                                               # head 1 of row 2
+        out.append(torch.empty_like(q, device=DEV))
+        kv4.kv4_attention(x.to(DEV), P.pages, P.table_d, i32([0, rows]), i32([n - rows]), out[-1], hd ** -0.5, None, 16, H, G, hd, rows, n, min_rows=rows)
+    b, a = (x.cpu().float().view(rows, H, hd) for x in out)
+    assert bool(torch.isnan(a[2, 1]).all())
+    a[2, 1] = b[2, 1] = 0
+    assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("hd,rows", [(64, 1), (64, 30), (128, 30), (96, 30)])
 def test_many_chunks_are_joined(hd, rows):
     """More chunks than a cluster has, by a context that many CTAs share out."""
