@@ -158,6 +158,7 @@ struct Kv4Args {
     int max_rows;                                          // split form: segments of more rows are not its own
     int min_rows;                                          // tiled form: nor are segments of fewer rows this form's
     int n_seg;
+    int split;                                             // tiled form: CTAs that share the keys of a tile of columns
 };
 
 // What a warp knows of its columns: column c of a segment stands for row c / R and head kvh R + c % R.
@@ -191,18 +192,6 @@ struct Kv4Split {
     static constexpr size_t RING = (size_t)STAGES * STAGE, JOIN = sizeof(float) * (NW + 1) * 8 * (HD + 2);
     static constexpr size_t SMEM = 1024 + (RING > JOIN ? RING : JOIN);
 };
-
-__device__ __forceinline__ void kv4_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
-// a float at this place of the shared memory of the cluster's CTA `rank`
-__device__ __forceinline__ float kv4_peer(const float* p, int rank) {
-    uint32_t at;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(kp_smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
 
 // The first key of a segment's chunks: that of its first row's window, down to a whole tile.
 __device__ __forceinline__ int kv4_chunk_base(int pos0, int window, int keys) {
@@ -534,7 +523,7 @@ template <int HD, int PARTS>
 struct Kv4Tiled {
     static constexpr int NT = PARTS == 1 ? (HD <= 64 ? 4 : (HD <= 128 ? 2 : 1)) : (HD <= 64 ? 2 : 1);
     static constexpr int COLS = 32 * NT, TILE = 64, STAGE = Kv4<HD>::bytes(64);
-    static constexpr size_t SMEM = 2 * STAGE;
+    static constexpr size_t JOIN = sizeof(float) * kv4_share_floats(COLS, HD), SMEM = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
 };
 
 // The tile'th of the tiles that the segments of at least min_rows rows make of `per` columns each: its segment and first column
@@ -571,14 +560,16 @@ kv4_tiled_kernel(const Kv4Args p) {
     kp_pdl_begin();
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the warp's number in a uniform register)
-    const int R = p.H / p.G, kvh = blockIdx.x % p.G;       // (the longest tiles first, of all heads)
+    // (the longest tiles first, of all heads)
+    const int R = p.H / p.G, rank = blockIdx.x % p.split, kvh = blockIdx.x / p.split % p.G;
     int seg, cta_col0 = 0;
-    kv4_find_tile(p, blockIdx.x / p.G, S::COLS, R, lane, seg, cta_col0);
+    kv4_find_tile(p, blockIdx.x / p.split / p.G, S::COLS, R, lane, seg, cta_col0);
     if (seg < 0) return;
     const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg], n_cols = n_rows * R;
     const int cta_col1 = min(cta_col0 + S::COLS, n_cols) - 1;
     const int k_hi = min(pos0 + cta_col1 / R, p.max_blocks * p.ps - 1), k_lo = p.window > 0 ? max(0, pos0 + cta_col0 / R - p.window + 1) : 0;
-    const int t_lo = k_lo / S::TILE, n_tiles = k_hi >= k_lo ? k_hi / S::TILE - t_lo + 1 : 0;
+    const int t_all = k_hi >= k_lo ? k_hi / S::TILE - k_lo / S::TILE + 1 : 0, t_skip = t_all * rank / p.split;
+    const int t_lo = k_lo / S::TILE + t_skip, n_tiles = t_all * (rank + 1) / p.split - t_skip;      // this CTA's
     const int* bt = p.block_table + (size_t)seg * p.max_blocks;
     const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);
     auto load = [&](int i) {                               // every warp a block of the tile
@@ -629,6 +620,35 @@ kv4_tiled_kernel(const Kv4Args p) {
     }
     cp_async_wait<0>();
     A.finish();
+    if (p.split > 1) {
+        float* part = reinterpret_cast<float*>(smem);      // (the last tile has been read by all)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int c = warp * 8 * NT + nt * 8 + 2 * (lane & 3) + i;
+                const bool none = A.shift[nt][i] == -INFINITY;
+                const float inv = none ? 0.f : 1.0f / A.l[nt][i];
+#pragma unroll
+                for (int y = 0; y < F::NG; y++)
+#pragma unroll
+                    for (int j = 0; j < F::MT; j++) {
+                        const float2 o = A.value(nt, y, j, i);
+                        *reinterpret_cast<float2*>(part + kv4_share_at(c, A.dim(y, j, lane), HD)) = none ? make_float2(0.f, 0.f) : make_float2(o.x * inv, o.y * inv);
+                    }
+                if (lane < 4) kv4_share_sums(part, S::COLS, HD, c, A.shift[nt][i], A.l[nt][i]);
+            }
+        kv4_cluster_sync();
+        kv4_join_shares<T, HD, S::COLS, 128, false>(
+            part, p.split, rank, cta_col1 - cta_col0 + 1,
+            [&](int col) { return (T*)p.out + (size_t)(row0 + (cta_col0 + col) / R) * p.ldo + (size_t)(kvh * R + (cta_col0 + col) % R) * HD; },
+            [&](int col, float top, float sum) {
+                const int c = cta_col0 + col;
+                if (p.lse && c < n_cols) p.lse[(size_t)(row0 + c / R) * p.H + kvh * R + c % R] = sum == 0.f ? INFINITY : top + log2f(sum);
+            });
+        kv4_cluster_sync();                                // (nobody leaves while its shares are read)
+        return;
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -756,14 +776,26 @@ static int kv4_row_blocks(const Kv4Rows& p, unsigned (&blocks)[2]) {
     return 0;
 }
 
-template <typename Kern>
-static int kv4_launch(Kern kern, dim3 grid, size_t smem, std::atomic<unsigned long long>& ready, cudaStream_t st, const Kv4Args& a) {
-    if (smem > 48 * 1024) {
-        const int e = kp_smem_limit(kern, smem, ready);
+template <int HD, int PARTS, bool CENTRE, typename T>
+static int kv4_run_tiled(Kv4Args a, long long tiles, long long busy, int max_context, cudaStream_t st) {
+    using S = Kv4Tiled<HD, PARTS>;
+    static std::atomic<unsigned long long> ready{0};
+    const auto kern = kv4_tiled_kernel<HD, PARTS, CENTRE, T>;
+    if (S::SMEM > 48 * 1024) {
+        const int e = kp_smem_limit(kern, S::SMEM, ready);
         if (e) return e;
     }
-    const cudaError_t e = kp_launch_pdl(kern, grid, dim3(128), smem, st, a);
-    return e ? (int)e : kp_launch_status();
+    // A tile's keys over as many CTAs, up to eight, as the GPU holds clusters of, where each has a tile of keys and there are three or more.  Measured
+    // with 32 heads over 8, one CTA a tile against the rule's: float32 rows of 64 values, 64 rows behind 4000 keys 139 us against 42, behind
+    // 500 26 against 17, 4 x 64 behind 2000 77 against 57; bfloat16 of 256 values 168 against 72, 32 against 22, 133 against 132.
+    const int reach = a.window > 0 && a.window + S::COLS / (a.H / a.G) < max_context ? a.window + S::COLS / (a.H / a.G) : max_context;
+    a.split = 1;
+    for (int n = 8; n > 1 && a.split == 1; n--)
+        if (busy * a.G <= kv4_fit<kv4_tiled_kernel<HD, PARTS, CENTRE, T>>(n, 128, S::SMEM) && (reach + S::TILE - 1) / S::TILE >= max(n, 3)) a.split = n;
+    if (tiles * a.G * a.split > 2147483647LL) return KP_ERR_UNSUPPORTED;
+    const Kv4Launch l((unsigned)(tiles * a.G), a.split, 128, S::SMEM, st);
+    const cudaError_t c = cudaLaunchKernelEx(&l.cfg, kern, a);
+    return c ? (int)c : kp_launch_status();
 }
 
 // The pages' codes as the TMA sees them: one record a (page, kv head), rows of codes (keys', then values').  A box has the keys of one page that lie
@@ -809,12 +841,12 @@ static int kv4_run_split(const Kv4Args& a, long long n_pages, cudaStream_t st) {
 }
 
 template <int HD, int PARTS, typename T>
-static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_tiles, int long_keys, cudaStream_t st) {
+static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_rows, int long_keys, cudaStream_t st) {
     using S = Kv4Tiled<HD, PARTS>;
     constexpr int KEYS = HD <= 128 ? 64 : 32;          // of the mass kernel
     const int R = a.H / a.G;
     const long long tiles = ((long long)n_rows * R + S::COLS - 1) / S::COLS + a.n_seg, places = (long long)((long_keys + KEYS - 1) / KEYS) * a.G * a.n_seg;
-    if (long_tiles > 0 && (tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL))) return KP_ERR_UNSUPPORTED;
+    if (long_rows > 0 && (tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL))) return KP_ERR_UNSUPPORTED;
     if (a.max_rows > 0) {
         const int e = a.mass ? kv4_run_split<HD, PARTS, true, T>(a, n_pages, st) : kv4_run_split<HD, PARTS, false, T>(a, n_pages, st);
         if (e) return e;
@@ -827,15 +859,15 @@ static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_til
             if (c) return (int)c;
         }
     }
-    if (long_tiles > 0) {
-        static std::atomic<unsigned long long> ready{0}, ready_mass{0};
+    if (long_rows > 0) {
+        // about how many tiles there are: as where each segment has the most rows
+        const long long busy = max(tiles - a.n_seg, (long long)(n_rows / long_rows) * (((long long)long_rows * R + S::COLS - 1) / S::COLS));
         // (with mass the scores are those that the mass is computed from again)
-        int e = a.mass ? kv4_launch(kv4_tiled_kernel<HD, PARTS, true, T>, dim3((unsigned)(tiles * a.G)), S::SMEM, ready, st, a)
-                       : kv4_launch(kv4_tiled_kernel<HD, PARTS, (PARTS > 1), T>, dim3((unsigned)(tiles * a.G)), S::SMEM, ready, st, a);
+        const int e = a.mass ? kv4_run_tiled<HD, PARTS, true, T>(a, tiles, busy, long_keys, st) : kv4_run_tiled<HD, PARTS, (PARTS > 1), T>(a, tiles, busy, long_keys, st);
         if (e) return e;
         if (a.mass) {
-            e = kv4_launch(kv4_mass_kernel<HD, PARTS, T>, dim3((unsigned)places), 0, ready_mass, st, a);
-            if (e) return e;
+            const cudaError_t c = kp_launch_pdl(kv4_mass_kernel<HD, PARTS, T>, dim3((unsigned)places), dim3(128), 0, st, a);
+            if (c) return (int)c;
         }
     }
     return kp_launch_status();

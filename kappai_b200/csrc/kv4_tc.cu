@@ -223,20 +223,6 @@ __device__ __forceinline__ float2 kt_add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
-__device__ __forceinline__ void kt_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
-// a float at this place of the shared memory of the cluster's CTA `rank`
-__device__ __forceinline__ float kt_peer(const float* p, int rank) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(kp_cluster_addr(p, rank)) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 kt_peer4(const float* p, int rank) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(kp_cluster_addr(p, rank)) : "memory");
-    return v;
-}
 // segment, its first row, number of rows and position, and first column, of a tile of 256 columns (kv4.cu's tiles: the last columns of a segment
 // first); seg = -1: none
 struct KtTile { int seg, row0, n_rows, pos0, col0; };
@@ -270,64 +256,19 @@ __device__ __forceinline__ int kt_first_tile(const Kv4TcArgs& p, int seg, int R,
     return __reduce_add_sync(0xffffffffu, sum) - 1;
 }
 
-// Rows of this CTA's columns from the shares of the cluster's n CTAs (at most MOST), four dimensions a thread; BATCH loads from each are under way at once
-template <int HD, int MOST, int BATCH, typename RowOf>
-__device__ __forceinline__ void kt_join(const float* part, const float* weight, int rank, int n, int n_cols, int cta_col0, RowOf row_of) {
-    constexpr int LANES = HD / 4;
-    for (int i0 = threadIdx.x; i0 < n_cols * LANES; i0 += 256 * BATCH) {
-        float4 v[BATCH][MOST];
-#pragma unroll
-        for (int b = 0; b < BATCH; b++) {
-            const int i = i0 + b * 256, col = rank + i / LANES * n;
-#pragma unroll
-            for (int j = 0; j < MOST; j++)
-                if (i < n_cols * LANES && j < n) v[b][j] = kt_peer4(part + col * HD + ((i % LANES ^ (col & 7)) * 4), j);
-        }
-#pragma unroll
-        for (int b = 0; b < BATCH; b++) {
-            const int i = i0 + b * 256, col = rank + i / LANES * n;
-            if (i >= n_cols * LANES) break;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int j = 0; j < MOST; j++)
-                if (j < n) {
-                    const float y = weight[col * 8 + j];
-                    x = make_float4(fmaf(y, v[b][j].x, x.x), fmaf(y, v[b][j].y, x.y), fmaf(y, v[b][j].z, x.z), fmaf(y, v[b][j].w, x.w));
-                }
-            *reinterpret_cast<uint2*>(row_of(cta_col0 + col) + 4 * (i % LANES)) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-        }
-    }
-}
-
-// The shares of a tile's rows of the cluster's CTAs, each weighted by its part of the sum, added in order, by 256 threads.  The CTAs share the
-// columns out: this one has every n-th.  (A call: inlined, it costs the loop over the keys registers.)
+// The rows of a tile from the shares of the cluster's CTAs, by 256 threads, and with mass what the pass over it needs of them.  (A call: inlined, it
+// costs the loop over the keys registers.)
 template <int HD>
 __device__ __noinline__ void kt_join_shares(const Kv4TcArgs& p, unsigned char* sm, int rank, int kvh, int tile, int row0, int cta_col0, int n_here) {
-    const int n = p.split, R = p.H / p.G;
-    const float* part = reinterpret_cast<const float*>(sm);
-    float* stat = reinterpret_cast<float*>(sm) + 256 * HD;
-    float* weight = stat + 768;                    // [column][8]
-    const int col = rank + threadIdx.x * n;
-    if (col < 256) {
-        float m[8], l[8], top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < n) { m[j] = kt_peer(stat + col, j); l[j] = kt_peer(stat + 256 + col, j); }
-#pragma unroll
-        for (int j = 0; j < 8; j++) if (j < n) top = fmaxf(top, m[j]);
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (j < n) { l[j] *= kv4_exp2(m[j] - (top == -INFINITY ? 0.f : top)); sum += l[j]; }
-#pragma unroll
-        for (int j = 0; j < 8; j++) if (j < n) weight[col * 8 + j] = sum == 0.f ? 0.f : l[j] / sum;
-        if (p.mass) p.col[((size_t)kvh * p.n_tiles + tile) * 256 + col] = make_float2(stat[512 + col], sum == 0.f ? INFINITY : top - 7.0f + log2f(sum));
-    }
-    asm volatile("bar.sync 4, 256;" ::: "memory");
-    auto row_of = [&](int c) { return p.out + (size_t)(row0 + c / R) * p.ldo + (size_t)(kvh * R + c % R) * HD; };
-    const int n_cta = (n_here + n - 1 - rank) / n;       // this CTA's columns
-    if (n == 2) kt_join<HD, 2, 4>(part, weight, rank, n, n_cta, cta_col0, row_of);
-    else if (n <= 4) kt_join<HD, 4, 2>(part, weight, rank, n, n_cta, cta_col0, row_of);
-    else kt_join<HD, 8, 1>(part, weight, rank, n, n_cta, cta_col0, row_of);
+    const int R = p.H / p.G;
+    float* part = reinterpret_cast<float*>(sm);
+    const float* factor = part + kv4_share_floats(256, HD);
+    kv4_join_shares<bf16, HD, 256, 256, true>(
+        part, p.split, rank, n_here,
+        [&](int col) { return p.out + (size_t)(row0 + (cta_col0 + col) / R) * p.ldo + (size_t)(kvh * R + (cta_col0 + col) % R) * HD; },
+        [&](int col, float top, float sum) {
+            if (p.mass) p.col[((size_t)kvh * p.n_tiles + tile) * 256 + col] = make_float2(factor[col], sum == 0.f ? INFINITY : top - 7.0f + log2f(sum));
+        });
 }
 
 template <int HD, bool SPLIT>
@@ -611,8 +552,7 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
             // this CTA's share of the rows, and what it counts for: in place of the operands, once neither group's products read them
             asm volatile("bar.sync 4, 256;" ::: "memory");
             const int col = g * 128 + r;
-            float* part = reinterpret_cast<float*>(sm) + col * HD;
-            float* stat = reinterpret_cast<float*>(sm) + 256 * HD + col;
+            float* part = reinterpret_cast<float*>(sm);
 #pragma unroll 1
             for (int e = 0; e < HD; e += 32) {
                 uint32_t v[32];
@@ -623,10 +563,11 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
                     float x[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) x[j] = none ? 0.f : __uint_as_float(v[(d & ~7) + 2 * j + (d >> 2 & 1)]) * inv;
-                    *reinterpret_cast<float4*>(part + (((e + d) / 4 ^ (r & 7)) * 4)) = make_float4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<float4*>(part + kv4_share_at(col, e + d, HD)) = make_float4(x[0], x[1], x[2], x[3]);
                 }
             }
-            stat[0] = m; stat[256] = l; stat[512] = f;
+            kv4_share_sums(part, 256, HD, col, m, l);
+            part[kv4_share_floats(256, HD) + col] = f;
         } else {
             if (p.mass) {
                 p.col[((size_t)kvh * p.n_tiles + tile) * 256 + g * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
@@ -664,9 +605,9 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
     if (warp == 12) kp_tmem_dealloc(tmem_base, 512);
     if (!SPLIT) return;
 
-    kt_cluster_sync();
+    kv4_cluster_sync();
     if (warp < 8) kt_join_shares<HD>(p, sm, rank, kvh, tile, row0, cta_col0, n_here);
-    kt_cluster_sync();                                 // (nobody leaves while its shares are read)
+    kv4_cluster_sync();                                 // (nobody leaves while its shares are read)
 }
 
 // The sum of 2^(score - lse) over the 128 columns of a tile, of those from lo to hi (MASKED), for this thread's key: S of tensor memory
@@ -817,48 +758,17 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     if (warp == 8) kp_tmem_dealloc(tmem_base, 256);
     float* join = reinterpret_cast<float*>(Ks);        // [group][key]; the cluster's first CTA adds them up, in order
     if (warp < 8) join[threadIdx.x] = sum;
-    if (n_ctas > 1) kt_cluster_sync(); else __syncthreads();
+    if (n_ctas > 1) kv4_cluster_sync(); else __syncthreads();
     if (rank == 0 && warp < 4) {
         const int key = k0 + threadIdx.x;
         if (key >= first && key <= last) {
             float all = join[threadIdx.x] + join[128 + threadIdx.x];
-            for (int r = 1; r < n_ctas; r++) all += kt_peer(join + threadIdx.x, r) + kt_peer(join + 128 + threadIdx.x, r);
+            for (int r = 1; r < n_ctas; r++) all += kv4_peer(join + threadIdx.x, r) + kv4_peer(join + 128 + threadIdx.x, r);
             const int page = p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)];
             p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += all;
         }
     }
-    if (n_ctas > 1) kt_cluster_sync();                 // (nobody leaves while its sums are read)
-}
-
-// Launches of `places` clusters of `cluster` CTAs
-struct KtLaunch {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[2];
-    KtLaunch(unsigned places, int cluster, int threads, size_t smem, cudaStream_t st) {
-        cfg.gridDim = dim3(places * cluster);
-        cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = st;
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = cluster;
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = cluster > 1 ? 2 : 1;
-    }
-};
-// clusters of n CTAs of the attention kernel that the GPU holds at once (its shared memory's limit has been raised)
-template <int HD>
-static int kt_fit(int n) {
-    static std::atomic<int> known[64][9];              // 1 more than the answer, by device
-    int dev = 0, fit = 0;
-    if (cudaGetDevice(&dev) || dev >= 64) return 0;
-    if (const int k = known[dev][n]) return k - 1;
-    KtLaunch l(1, n, Kt<HD>::THREADS, Kt<HD>::SMEM, nullptr);
-    if (cudaOccupancyMaxActiveClusters(&fit, kv4_tc_kernel<HD, true>, &l.cfg)) { cudaGetLastError(); fit = 0; }
-    known[dev][n] = fit + 1;
-    return fit;
+    if (n_ctas > 1) kv4_cluster_sync();                 // (nobody leaves while its sums are read)
 }
 
 template <int HD>
@@ -881,16 +791,16 @@ static int kt_run(Kv4TcArgs a, int max_context, long long busy, cudaStream_t st)
     const int reach = a.window > 0 && a.window + 256 / (a.H / a.G) < max_context ? a.window + 256 / (a.H / a.G) : max_context;
     a.split = 1;
     for (int n = 8; n > 1 && a.split == 1; n--)
-        if (busy * a.G <= kt_fit<HD>(n) && (reach + KT_ROWS - 1) / KT_ROWS >= max(n, 3)) a.split = n;
+        if (busy * a.G <= kv4_fit<kv4_tc_kernel<HD, true>>(n, S::THREADS, S::SMEM) && (reach + KT_ROWS - 1) / KT_ROWS >= max(n, 3)) a.split = n;
     if ((long long)a.n_tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL)) return KP_ERR_UNSUPPORTED;
-    const KtLaunch l((unsigned)a.n_tiles * a.G, a.split, S::THREADS, S::SMEM, st);
+    const Kv4Launch l((unsigned)a.n_tiles * a.G, a.split, S::THREADS, S::SMEM, st);
     cudaError_t c = cudaLaunchKernelEx(&l.cfg, a.split > 1 ? kv4_tc_kernel<HD, true> : kv4_tc_kernel<HD, false>, a);
     if (c) return (int)c;
     if (a.mass) {
         e = kp_smem_limit(kv4_tc_mass_kernel<HD>, S::MASS_SMEM, ready_mass);
         if (e) return e;
         a.cluster = places <= 148 && a.n_tiles - a.n_seg >= 8 * a.n_seg ? 4 : 1;
-        const KtLaunch l((unsigned)places, a.cluster, S::MASS_THREADS, S::MASS_SMEM, st);
+        const Kv4Launch l((unsigned)places, a.cluster, S::MASS_THREADS, S::MASS_SMEM, st);
         c = cudaLaunchKernelEx(&l.cfg, kv4_tc_mass_kernel<HD>, a);
         if (c) return (int)c;
     }

@@ -17,7 +17,11 @@ from .build import load_library
 from .kernels import STREAM, KernelError, _need, _rows_2d, _run, dtype_code
 
 KV4_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
-KV4_SHORT_ROWS = 8         # segments of at most this many rows share their keys out over many CTAs
+# Segments of few columns (rows times the query heads of a kv head) take the split form, where eight columns share a block of keys.  Measured against
+# the tcgen05 form, 32 heads over 8 of 64 values, 64 columns: 8 x 4000 keys 51 us against 67, 1 x 32000 52 against 122; 96 columns: 73 against
+# 67, 88 against 122.  With mass, whose scores it keeps in memory: 32 columns, 8 x 4000 keys 66 against 106, 1 x 500 29 against 20; 64 columns
+# 136 against 106.
+KV4_SHORT_COLS, KV4_SHORT_COLS_MASS, KV4_SHORT_ROWS_MASS = 64, 32, 16
 USE_TC_KV4 = True          # longer ones of bfloat16 rows with heads of 64 or 128 run on the tcgen05 tensor cores
 _CTAS = 148 * 4            # CTAs of the split form that an even spread over the SMs wants
 
@@ -111,17 +115,23 @@ def kv4_read(pages: torch.Tensor, slot_map: torch.Tensor, page_size: int, G: int
 
 
 @lru_cache(maxsize=4096)
-def kv4_chunks(n_seg: int, max_rows: int, max_context: int, window: int, H: int, G: int, hd: int) -> Tuple[int, int]:
+def kv4_chunks(n_seg: int, max_rows: int, max_context: int, window: int, H: int, G: int, hd: int, usual_rows: Optional[int] = None) -> Tuple[int, int]:
     """(number of chunks, keys a chunk) of the split form: as many CTAs as fill the SMs, none with less than a tile of keys.  Up to 16
-    such chunks are made 8: those are one cluster, which joins them itself and spares a launch."""
+    such chunks are made 8: those are one cluster, which joins them itself and spares a launch.  ``usual_rows`` (None: the most): the rows
+    that most segments have (beside portions of prompts that is the fewest: decoded tokens')."""
     tile = 256 if hd <= 64 else (128 if hd <= 128 else 64)
     span = min(max_context, window + max_rows + tile - 1) if window else max_context      # from the first tile that a row reads
-    want = max(1, _CTAS // max(1, n_seg * G * -(-max_rows * (H // G) // 8)))
+    want = max(1, _CTAS // max(1, n_seg * G * -(-(usual_rows or max_rows) * (H // G) // 8)))
     n = -(-span // tile)
     if min(n, want) <= 16:
         want = min(want, 8)
     chunk = -(-n // want) * tile
     return -(-span // chunk), chunk
+
+
+def kv4_short_rows(R: int, mass: bool) -> int:
+    """The most rows of a segment that the split form takes, with R query heads a kv head (one row it always takes)."""
+    return max(1, min(KV4_SHORT_COLS_MASS // R, KV4_SHORT_ROWS_MASS) if mass else KV4_SHORT_COLS // R)
 
 
 def kv4_tc_ok(q: torch.Tensor, out: torch.Tensor, hd: int, scale: float) -> bool:
@@ -157,12 +167,13 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     pm = None if mass is None else _have_mass(mass, "mass", pages, page_size, G)
     if not n or not n_seg:
         return out
-    short = min(max_rows, KV4_SHORT_ROWS) if min_rows <= KV4_SHORT_ROWS else 0
-    tiled = max_rows > KV4_SHORT_ROWS
+    most = kv4_short_rows(H // G, pm is not None)
+    short = min(max_rows, most) if min_rows <= most else 0
+    tiled = max_rows > most
     tc = tiled and kv4_tc_ok(q, out, hd, scale)
     window = window or 0
     if short or (tiled and not tc):
-        n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd)
+        n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd, min_rows if short and tiled else None)
         # one allocation for what the launches hand one another: results of chunks, their (shift, sum), scores, logarithms of sums
         fused = n_chunks <= 8 and (pm is None or short * (H // G) <= 8)
         places, many = n_seg * short * H, n_chunks > 1 and not fused
@@ -174,7 +185,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
         p2 = p1 + 4 * sizes[1]
         p3 = p2 + 4 * sizes[2]
         _run("kv4_attention", _fn("kp_kv4_attention"), pq, ldq, at, pages.shape[0], table, width, cu, pos, n_seg, po, ldo, scale, window, page_size, H, G,
-             hd, n, short, int(tiled and not tc), n_chunks, chunk, fused, max_context, p0, p1, p2, n_chunks * chunk, p3, p3 + 4 * sizes[3], pm, code, STREAM)
+             hd, n, short, max_rows if tiled and not tc else 0, n_chunks, chunk, fused, max_context, p0, p1, p2, n_chunks * chunk, p3, p3 + 4 * sizes[3], pm, code, STREAM)
     if tc:
         scratch = None
         if pm:

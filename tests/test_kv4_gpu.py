@@ -257,22 +257,23 @@ def test_long_contexts(dtype, hd, lengths, rows):
     run_and_check(lengths, rows, 4, 2, hd, 64, dtype, mass=False, seed=9)
 
 
-@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 96), (torch.bfloat16, 256), (torch.float32, 32), (torch.float32, 64),
+                                      (torch.float32, 128), (torch.float32, 192)])
 @pytest.mark.parametrize("lengths,rows,H,G,window", [([385], [20], 4, 1, None), ([400], [64], 4, 1, None), ([640], [70], 4, 2, None), ([700], [9], 12, 3, None),
                                                      ([800], [40], 5, 1, None), ([2050], [130], 8, 2, None), ([600], [300], 32, 32, None),
                                                      ([900, 40, 12, 300], [20, 20, 12, 33], 4, 2, None), ([1500, 1400], [30, 9], 4, 2, 200), ([900], [30], 4, 1, 3)])
-def test_keys_that_a_cluster_shares_out(hd, lengths, rows, H, G, window):
+def test_keys_that_a_cluster_shares_out(dtype, hd, lengths, rows, H, G, window):
     """Few rows over many keys: two to eight CTAs a tile, some of them without a key of a shorter sequence."""
-    run_and_check(lengths, rows, H, G, hd, 32, torch.bfloat16, window)
-    run_and_check(lengths, rows, H, G, hd, 32, torch.bfloat16, window, mass=False, seed=8, strided=True)
+    run_and_check(lengths, rows, H, G, hd, 32, dtype, window)
+    run_and_check(lengths, rows, H, G, hd, 32, dtype, window, mass=False, seed=8, strided=True)
 
 
-@pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_a_query_that_is_not_finite_before_many_keys(hd, bad):
-    H, G, rows, n = 4, 2, 30, 1000
-    P = Paged([n], G, hd, 16, 3, torch.bfloat16)
-    q = torch.randn((rows, H * hd), generator=torch.Generator().manual_seed(1)).bfloat16()
+@pytest.mark.parametrize("dtype,hd,rows", [(torch.bfloat16, 64, 30), (torch.bfloat16, 64, 60), (torch.bfloat16, 128, 60), (torch.bfloat16, 96, 60), (torch.float32, 64, 60)])
+def test_a_query_that_is_not_finite_before_many_keys(hd, bad, dtype, rows):
+    H, G, n = 4, 2, 1000
+    P = Paged([n], G, hd, 16, 3, dtype)
+    q = torch.randn((rows, H * hd), generator=torch.Generator().manual_seed(1)).to(dtype)
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
     out = []
     for x in (q, q.clone()):
