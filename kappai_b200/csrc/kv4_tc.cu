@@ -210,6 +210,11 @@ __device__ __forceinline__ void kt_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uin
 // a wait of a warp in step, which gives up as one
 __device__ __forceinline__ bool kt_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kp_mbar_wait_bounded(bar, parity)); }
 
+// bits lo .. hi of 32 (lo may lie below, hi above them)
+__device__ __forceinline__ uint32_t kt_bits(int lo, int hi) {
+    const uint32_t upto = hi >= 31 ? 0xffffffffu : (hi < 0 ? 0u : (2u << hi) - 1u), from = lo <= 0 ? 0xffffffffu : (lo > 31 ? 0u : 0xffffffffu << lo);
+    return upto & from;
+}
 // two float32 operations at once
 __device__ __forceinline__ float2 kt_fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -433,8 +438,7 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
         // ---- the columns: warps 0-3 group 0, warps 4-7 group 1; thread r of a group has column r
         const int g = warp >> 2, q4 = warp & 3, r = q4 * 32 + lane;
         const int c = cta_col0 + g * 128 + r;
-        const bool live = c < n_cols;
-        const int pos = live ? min(pos0 + c / R, k_hi) : -1;
+        const int pos = min(pos0 + min(c, n_cols - 1) / R, k_hi);                // (a column that is not there reads what the last one does)
         // where column c's row lies in q or in out; -1: nowhere
         auto place_of = [&](int c, long long ld) { return c < n_cols ? (long long)(row0 + c / R) * ld + (kvh * R + c % R) * HD : -1LL; };
         unsigned char* Qg = Qs + g * S::OPER;
@@ -450,8 +454,8 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
         }
         const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
         // keys that every column of the group reads
-        const int g_first = min(cta_col0 + g * 128, max(n_cols - 1, 0)), g_last = min(cta_col0 + g * 128 + 127, max(n_cols - 1, 0));
-        const int all_hi = cta_col0 + g * 128 + 127 < n_cols ? min(pos0 + g_first / R, k_hi) : -1;
+        const int g_first = min(cta_col0 + g * 128, n_cols - 1), g_last = min(cta_col0 + g * 128 + 127, n_cols - 1);
+        const int all_hi = min(pos0 + g_first / R, k_hi);
         const int all_lo = p.window > 0 ? max(0, pos0 + g_last / R - p.window + 1) : 0;
         const uint32_t lane_off = (uint32_t)(q4 * 32) << 16;
         const uint32_t tmem_s = tmem_base + S::S_COL + 128 * g + lane_off, tmem_o = tmem_base + S::O_COL + HD * g + lane_off;
@@ -473,10 +477,12 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
                 kp_tmem_ld_wait();
                 if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 2; e++)
+                    for (int e = 0; e < 2; e++) {
+                        const uint32_t there = kt_bits(lo - key0 - at - e * 32, pos - key0 - at - e * 32);
 #pragma unroll
                         for (int j = 0; j < 32; j++)
-                            if (!(key0 + at + e * 32 + j >= lo && key0 + at + e * 32 + j <= pos)) s[e][j] = 0xff800000u;
+                            if (!(there & (1u << j))) s[e][j] = 0xff800000u;
+                    }
                 }
             };
             auto largest = [&] {
@@ -620,6 +626,7 @@ __device__ __forceinline__ float kt_column_sum(uint32_t tmem_s, const float4* co
     for (int e = 0; e < 128; e += 32) {
         uint32_t s[32];
         kp_tmem_ld32(tmem_s + e, s);
+        const uint32_t there = kt_bits(lo - e, hi - e);
         float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
@@ -627,8 +634,8 @@ __device__ __forceinline__ float kt_column_sum(uint32_t tmem_s, const float4* co
             float2 x = kt_fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), k2, make_float2(0.f, 0.f));
             x = make_float2(kv4_exp2(fmaf(x.x, f.x, -f.y)), kv4_exp2(fmaf(x.y, f.z, -f.w)));
             if (MASKED) {
-                if (e + j < lo || e + j > hi) x.x = 0.f;
-                if (e + j + 1 < lo || e + j + 1 > hi) x.y = 0.f;
+                if (!(there & (1u << j))) x.x = 0.f;
+                if (!(there & (2u << j))) x.y = 0.f;
             }
             a[(j >> 1) & 1] = kt_add2(a[(j >> 1) & 1], x);
         }
