@@ -611,7 +611,7 @@ kv4_tiled_kernel(const Kv4Args p) {
         for (int b = 0; b < 4; b++) {
             const int key0 = (t_lo + i) * S::TILE + b * 16;
             if (col1 < col0 || key0 > w_hi || key0 + 15 < w_lo) continue;
-            if (key0 >= max(k_lo, safe_lo) && key0 + 15 <= safe_hi && col0 + 8 * NT <= n_cols)
+            if (key0 >= max(k_lo, safe_lo) && key0 + 15 <= safe_hi)                  // (columns that are not there read along, and are not written)
                 kv4_tile<HD, S::TILE, PARTS, NT, 1, CENTRE, false, false>(A, Q, B, tile, b * 16, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
             else
                 kv4_tile<HD, S::TILE, PARTS, NT, 1, CENTRE, true, false>(A, Q, B, tile, b * 16, key0, C.hi, C.lo, k_lo, k_hi, lane, sc);
