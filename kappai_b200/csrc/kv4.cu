@@ -158,7 +158,7 @@ struct Kv4Args {
     int max_rows;                                          // split form: segments of more rows are not its own
     int min_rows;                                          // tiled form: nor are segments of fewer rows this form's
     int n_seg;
-    int split;                                             // tiled form: CTAs that share the keys of a tile of columns
+    int split;                                             // tiled form: CTAs that share the keys of a tile of columns, or the columns of a tile of keys
 };
 
 // What a warp knows of its columns: column c of a segment stands for row c / R and head kvh R + c % R.
@@ -673,8 +673,8 @@ kv4_tiled_kernel(const Kv4Args p) {
         }
 }
 
-// ---- the tiled form's mass: one CTA per (64 keys, kv head, segment).  Its warps take the columns that read the keys, 8 at a
-// time, compute the scores again and add up 2^(score - lse); the warps' sums are added in their order.
+// ---- the tiled form's mass: a cluster of CTAs per (64 keys, kv head, segment), which share the columns that read the keys.  Their warps take 8 at a
+// time, compute the scores again and add up 2^(score - lse); the warps' sums are added in their order, then the CTAs'.
 template <int HD, int PARTS, typename T>
 __global__ void __launch_bounds__(128)
 kv4_mass_kernel(const Kv4Args p) {
@@ -685,7 +685,8 @@ kv4_mass_kernel(const Kv4Args p) {
     __shared__ float part[4][KEYS];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;      // (the warp's number in a uniform register)
     // the first keys first, of all heads and segments: most rows read them
-    const int kvh = blockIdx.x % p.G, seg = blockIdx.x / p.G % p.n_seg, k0 = blockIdx.x / p.G / p.n_seg * KEYS, R = p.H / p.G;
+    const int n_ctas = p.split, rank = blockIdx.x % n_ctas, place = blockIdx.x / n_ctas;
+    const int kvh = place % p.G, seg = place / p.G % p.n_seg, k0 = place / p.G / p.n_seg * KEYS, R = p.H / p.G;
     const int row0 = p.cu_rows[seg], n_rows = p.cu_rows[seg + 1] - row0, pos0 = p.seg_pos[seg];
     // keys that any row reads (in front of them the pages may be somebody else's by now)
     const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
@@ -710,7 +711,7 @@ kv4_mass_kernel(const Kv4Args p) {
     const Kv4Block<HD, KEYS> B(lane);
     const int c_end = (r_hi + 1) * R, key = F::key_of(lane >> 2);
 #pragma unroll 1
-    for (int col0 = r_lo * R + warp * 8; col0 < c_end; col0 += 32) {
+    for (int col0 = r_lo * R + (rank * 4 + warp) * 8; col0 < c_end; col0 += 32 * n_ctas) {
         Kv4Q<HD, PARTS, 1> Q;
         const int cq = col0 + (lane >> 2);
         const T* const src[1] = {cq < c_end ? (const T*)p.q + (size_t)(row0 + cq / R) * p.ldq + (size_t)(kvh * R + cq % R) * HD : nullptr};
@@ -746,10 +747,15 @@ kv4_mass_kernel(const Kv4Args p) {
         }
     __syncthreads();
     const int k = threadIdx.x;
-    if (k < KEYS && k0 + k <= last && k0 + k >= first) {
+    float all = 0.f;
+    if (k < KEYS) part[0][k] = all = (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
+    if (n_ctas > 1) kv4_cluster_sync();
+    if (rank == 0 && k < KEYS && k0 + k <= last && k0 + k >= first) {
+        for (int i = 1; i < n_ctas; i++) all += kv4_peer(part[0] + k, i);
         const int page = bt[(k0 + k) >> p.ps_log2];
-        p.mass[((size_t)page * p.G + kvh) * p.ps + ((k0 + k) & (p.ps - 1))] += (part[0][k] + part[1][k]) + (part[2][k] + part[3][k]);
+        p.mass[((size_t)page * p.G + kvh) * p.ps + ((k0 + k) & (p.ps - 1))] += all;
     }
+    if (n_ctas > 1) kv4_cluster_sync();                    // (nobody leaves while its sums are read)
 }
 
 // ------------------------------------------------------------------ launchers
@@ -866,7 +872,12 @@ static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_row
         const int e = a.mass ? kv4_run_tiled<HD, PARTS, true, T>(a, tiles, busy, long_keys, st) : kv4_run_tiled<HD, PARTS, (PARTS > 1), T>(a, tiles, busy, long_keys, st);
         if (e) return e;
         if (a.mass) {
-            const cudaError_t c = kp_launch_pdl(kv4_mass_kernel<HD, PARTS, T>, dim3((unsigned)places), dim3(128), 0, st, a);
+            Kv4Args m = a;
+            m.split = 1;
+            for (int n = 8; n > 1 && m.split == 1; n--)
+                if (places <= kv4_fit<kv4_mass_kernel<HD, PARTS, T>>(n, 128, 0) && (long long)long_rows * R >= 64 * n) m.split = n;
+            const Kv4Launch l((unsigned)places, m.split, 128, 0, st);
+            const cudaError_t c = cudaLaunchKernelEx(&l.cfg, kv4_mass_kernel<HD, PARTS, T>, m);
             if (c) return (int)c;
         }
     }
