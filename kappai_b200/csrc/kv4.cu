@@ -673,13 +673,13 @@ kv4_tiled_kernel(const Kv4Args p) {
         }
 }
 
-// ---- the tiled form's mass: a cluster of CTAs per (64 keys, kv head, segment), which share the columns that read the keys.  Their warps take 8 at a
+// ---- the tiled form's mass: a cluster of CTAs per (128 keys or 64, kv head, segment), which share the columns that read the keys.  Their warps take 8 at a
 // time, compute the scores again and add up 2^(score - lse); the warps' sums are added in their order, then the CTAs'.
 template <int HD, int PARTS, typename T>
 __global__ void __launch_bounds__(128)
 kv4_mass_kernel(const Kv4Args p) {
     using F = Kv4<HD>;
-    constexpr int NB = HD <= 128 ? 4 : 2, KEYS = NB * 16;
+    constexpr int NB = HD <= 128 ? 8 : 4, KEYS = NB * 16;
     kp_pdl_begin();
     __shared__ __align__(128) unsigned char smem[F::bytes(KEYS)];
     __shared__ float part[4][KEYS];
@@ -849,7 +849,7 @@ static int kv4_run_split(const Kv4Args& a, long long n_pages, cudaStream_t st) {
 template <int HD, int PARTS, typename T>
 static int kv4_run(const Kv4Args& a, long long n_pages, int n_rows, int long_rows, int long_keys, cudaStream_t st) {
     using S = Kv4Tiled<HD, PARTS>;
-    constexpr int KEYS = HD <= 128 ? 64 : 32;          // of the mass kernel
+    constexpr int KEYS = HD <= 128 ? 128 : 64;         // of the mass kernel
     const int R = a.H / a.G;
     const long long tiles = ((long long)n_rows * R + S::COLS - 1) / S::COLS + a.n_seg, places = (long long)((long_keys + KEYS - 1) / KEYS) * a.G * a.n_seg;
     if (long_rows > 0 && (tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL))) return KP_ERR_UNSUPPORTED;
