@@ -8,6 +8,39 @@
 // A thread takes 8 consecutive values of a group; the lanes of a group (8, or 4) find its range together.
 __device__ __forceinline__ float kv4_min_nan(float a, float b) { float d; asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
 __device__ __forceinline__ float kv4_max_nan(float a, float b) { float d; asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b)); return d; }
+__device__ __forceinline__ float kv4_min_nan(float a, float b, float c) { float d; asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+__device__ __forceinline__ float kv4_max_nan(float a, float b, float c) { float d; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+
+// (a call: inlined, the compiler makes its first steps where nothing is divided)
+__device__ __noinline__ float kv4_divide(float a, float b) { return __fdiv_rn(a, b); }
+// bfloat16(x / 15), x >= 0: the product with the reciprocal is off by a unit or two of float32's last place, which matters only where it lies next to
+// a half of bfloat16's; there (and for the smallest) x is divided.
+__device__ __forceinline__ bf16 kv4_fifteenth(float x) {
+    float q = x * (1.0f / 15.0f);
+    if (q < 1e-30f || ((__float_as_uint(q) & 0xffffu) - 0x7ffcu) < 8u) q = kv4_divide(x, 15.0f);
+    return __float2bfloat16_rn(q);
+}
+// The codes round((x - z) / s) of eight values, halves to even, within 0 .. 15 (s > 0).  One Newton step on the quotient by the reciprocal (Markstein's
+// method): q + (d - q s) / s with the remainder exact.  Where d / s is at a half or rounds to it the step gives that half itself, and elsewhere a
+// unit of the last place changes no code.  Scales whose reciprocal is not to be had are divided by.  Adding 2^23 rounds to the even integer and
+// leaves the code in the low bits, under the same 0x4b000000 for each.
+__device__ __forceinline__ uint32_t kv4_eight_codes(const float (&x)[8], float s, float z) {
+    float inv, q[8];
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float d = x[i] - z, t = d * inv;
+        q[i] = fmaf(fmaf(-t, s, d), inv, t);
+    }
+    if (!(s >= 1e-30f && s <= 1e30f)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[i] = kv4_divide(x[i] - z, s);
+    }
+    uint32_t w = 0u;
+#pragma unroll
+    for (int i = 7; i >= 0; i--) w = w * 16u + __float_as_uint(fminf(fmaxf(q[i], 0.f), 15.f) + 8388608.0f);
+    return w - 0xfb000000u;                                // (0x4b000000 and 16 times it; the others have left the word)
+}
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void kv4_load8(float (&v)[8], const T* p) {
@@ -26,8 +59,9 @@ __device__ __forceinline__ void kv4_load8(float (&v)[8], const T* p) {
 }
 
 // Thread idx of a launch of `n_threads`: place `idx % per_row` of the rows idx / per_row + u (n_threads / per_row), u < U.  With
-// U rows a thread their loads are under way together: one row a thread leaves a CTA waiting for its slot, then for its values
-// (6,007 rows of 8 heads of 128 float32 values written: 29 us with one, 20 with four).
+// U rows a thread their loads are under way together: one row a thread leaves a CTA waiting for its slot, then for its values.
+// 6,007 rows of 8 heads of 128 float32 values written: 18.9 us with one row, 16.6 with two, 15.2 with three, 15.7 with four; 49 MB read and 7
+// written, 3.7 TB/s; 237 instructions a warp and row of 8 values a thread are two thirds of what the SMs could issue in that time.
 struct Kv4Rows { int n, ps_log2, G, hd, gs; long long n_slots; };
 
 template <typename T, bool VEC, int U>
@@ -41,8 +75,12 @@ kv4_write_kernel(const T* __restrict__ k, long long ldk, const T* __restrict__ v
     const bool is_v = place >= half;
     const int within = is_v ? place - half : place, head = within / (p.hd / 8), d8 = within - head * (p.hd / 8);
     const int lanes = p.gs / 8, ng = p.hd / p.gs;          // lanes of a group, groups of a head
-    const T* src = (is_v ? v : k) + within * 8;
-    const long long ld = is_v ? ldv : ldk;
+    const long long ld = is_v ? ldv : ldk, stride = step * ld;
+    const T* src = (is_v ? v : k) + within * 8 + row0 * ld;
+    const int ps = 1 << p.ps_log2;
+    const unsigned rec = kv4_page_bytes(ps, p.hd);
+    unsigned char* codes = pages + ((is_v ? ps : 0) * (p.hd / 2) + d8 * 4);       // of this head's first page, its first slot
+    unsigned char* ranges = pages + (ps * p.hd + ((is_v ? ps : 0) * ng + d8 / lanes) * 4);
     int slot[U];
     float x[U][8];
 #pragma unroll
@@ -55,40 +93,29 @@ kv4_write_kernel(const T* __restrict__ k, long long ldk, const T* __restrict__ v
     for (int u = 0; u < U; u++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[u][i] = 0.f;
-        if (slot[u] >= 0) kv4_load8<T, VEC>(x[u], src + (row0 + u * step) * ld);
+        if (slot[u] >= 0) kv4_load8<T, VEC>(x[u], src + u * stride);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         // a range that holds a NaN, or an infinity, is none: the group reads as NaN
-        float lo = x[u][0], hi = x[u][0];
+        float lo = kv4_min_nan(x[u][0], x[u][1]), hi = kv4_max_nan(x[u][0], x[u][1]);
 #pragma unroll
-        for (int i = 1; i < 8; i++) { lo = kv4_min_nan(lo, x[u][i]); hi = kv4_max_nan(hi, x[u][i]); }
-        for (int d = 1; d < lanes; d <<= 1) {
+        for (int i = 2; i < 8; i += 2) { lo = kv4_min_nan(lo, x[u][i], x[u][i + 1]); hi = kv4_max_nan(hi, x[u][i], x[u][i + 1]); }
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+            if (d == 4 && lanes == 4) break;
             lo = kv4_min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
             hi = kv4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
         if (slot[u] < 0) continue;
-        const bf16 sb = __float2bfloat16_rn(__fdiv_rn(hi - lo, 15.0f)), zb = __float2bfloat16_rn(lo);
+        const bf16 sb = kv4_fifteenth(hi - lo), zb = __float2bfloat16_rn(lo);
         const float s = __bfloat162float(sb), z = __bfloat162float(zb);
-        uint32_t w = 0;
-        if (s > 0.f) {
-            // round((x - z) / s): the quotient by the reciprocal is off by a few units of the last place, which matters only where it lies
-            // at a half; there (and for scales whose reciprocal is too large) it is divided.  Adding 2^23 rounds to the even integer.
-            const float inv = __frcp_rn(s);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float d = x[u][i] - z;
-                float t = fminf(fmaxf(d * inv, 0.f), 15.f), r = t + 8388608.0f;
-                if (s < 1e-30f || fabsf(t - (r - 8388608.0f)) > 0.4999f) r = fminf(fmaxf(__fdiv_rn(d, s), 0.f), 15.f) + 8388608.0f;
-                w |= (__float_as_uint(r) & 15u) << (4 * i);
-            }
-        }
-        const int ps = 1 << p.ps_log2, page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);
-        unsigned char* rec = pages + ((size_t)page * p.G + head) * kv4_page_bytes(ps, p.hd);
-        reinterpret_cast<uint32_t*>(rec + (size_t)((is_v ? ps : 0) + off) * (p.hd / 2))[d8] = w;
+        const uint32_t w = s > 0.f ? kv4_eight_codes(x[u], s, z) : 0u;
+        const unsigned page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);
+        const size_t at = (size_t)(page * p.G + head) * rec;
+        *reinterpret_cast<uint32_t*>(codes + at + off * (p.hd / 2)) = w;
         if (d8 % lanes == 0)
-            reinterpret_cast<uint32_t*>(rec + (size_t)ps * p.hd)[((is_v ? ps : 0) + off) * ng + d8 / lanes] =
-                (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+            *reinterpret_cast<uint32_t*>(ranges + at + off * ng * 4) = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
     }
 }
 
@@ -114,6 +141,10 @@ kv4_read_kernel(const unsigned char* __restrict__ pages, const int* __restrict__
     if (row0 >= step) return;
     const bool is_v = place >= half;
     const int within = is_v ? place - half : place, head = within / (p.hd / 8), d8 = within - head * (p.hd / 8), ng = p.hd / p.gs, g = d8 / (p.gs / 8);
+    const int ps = 1 << p.ps_log2;
+    const unsigned rec = kv4_page_bytes(ps, p.hd);
+    const unsigned char* codes = pages + ((is_v ? ps : 0) * (p.hd / 2) + d8 * 4);
+    const unsigned char* ranges = pages + (ps * p.hd + ((is_v ? ps : 0) * ng + g) * 4);
     int slot[U];
     uint32_t w[U], r[U];
 #pragma unroll
@@ -125,10 +156,10 @@ kv4_read_kernel(const unsigned char* __restrict__ pages, const int* __restrict__
     for (int u = 0; u < U; u++) {
         w[u] = r[u] = 0u;                                  // a row without a slot reads as zeros
         if (slot[u] < 0 || slot[u] >= p.n_slots) continue;
-        const int ps = 1 << p.ps_log2, page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);
-        const unsigned char* rec = pages + ((size_t)page * p.G + head) * kv4_page_bytes(ps, p.hd);
-        w[u] = reinterpret_cast<const uint32_t*>(rec + (size_t)((is_v ? ps : 0) + off) * (p.hd / 2))[d8];
-        r[u] = reinterpret_cast<const uint32_t*>(rec + (size_t)ps * p.hd)[((is_v ? ps : 0) + off) * ng + g];
+        const unsigned page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);
+        const size_t at = (size_t)(page * p.G + head) * rec;
+        w[u] = *reinterpret_cast<const uint32_t*>(codes + at + off * (p.hd / 2));
+        r[u] = *reinterpret_cast<const uint32_t*>(ranges + at + off * ng * 4);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -787,25 +818,20 @@ kv4_mass_kernel(const Kv4Args p) {
 
 static int kv4_log2(int v) { int l = 0; while ((1 << l) < v) l++; return l; }
 
-// CTAs of the writing and reading kernels with one row a thread, and with four
-#define KV4_ONE_ROW (148 * 8)                              // more CTAs than that are more than fit at once: four rows a thread
-static int kv4_row_blocks(const Kv4Rows& p, unsigned (&blocks)[2]) {
+// CTAs of the writing and reading kernels with one row a thread, and with `rows`
+#define KV4_ONE_ROW (148 * 8)                              // more CTAs than that are more than fit at once: several rows a thread
+static int kv4_row_blocks(const Kv4Rows& p, int rows, unsigned (&blocks)[2]) {
     const long long per_row = 2LL * p.G * p.hd / 8;
-    if (p.n * per_row >= (1LL << 32) - 256) return KP_ERR_UNSUPPORTED;
+    if (p.n * per_row >= (1LL << 32) - 256 || (p.n_slots >> p.ps_log2) * p.G >= 1LL << 32 || 2LL * p.hd << p.ps_log2 > 1LL << 30) return KP_ERR_UNSUPPORTED;
     blocks[0] = (unsigned)((p.n * per_row + 255) / 256);
-    blocks[1] = (unsigned)(((p.n + 3) / 4 * per_row + 255) / 256);
+    blocks[1] = (unsigned)((((long long)p.n + rows - 1) / rows * per_row + 255) / 256);
     return 0;
 }
 
 template <int HD, int PARTS, bool CENTRE, typename T>
 static int kv4_run_tiled(Kv4Args a, long long tiles, long long busy, int max_context, cudaStream_t st) {
     using S = Kv4Tiled<HD, PARTS>;
-    static std::atomic<unsigned long long> ready{0};
-    const auto kern = kv4_tiled_kernel<HD, PARTS, CENTRE, T>;
-    if (S::SMEM > 48 * 1024) {
-        const int e = kp_smem_limit(kern, S::SMEM, ready);
-        if (e) return e;
-    }
+    static_assert(S::SMEM <= 48 * 1024, "needs no raised limit of shared memory");
     // A tile's keys over as many CTAs, up to eight, as the GPU holds clusters of, where each has a tile of keys and there are three or more.  Measured
     // with 32 heads over 8, one CTA a tile against the rule's: float32 rows of 64 values, 64 rows behind 4000 keys 139 us against 42, behind
     // 500 26 against 17, 4 x 64 behind 2000 77 against 57; bfloat16 of 256 values 168 against 72, 32 against 22, 133 against 132.
@@ -815,7 +841,7 @@ static int kv4_run_tiled(Kv4Args a, long long tiles, long long busy, int max_con
         if (busy * a.G <= kv4_fit<kv4_tiled_kernel<HD, PARTS, CENTRE, T>>(n, 128, S::SMEM) && (reach + S::TILE - 1) / S::TILE >= max(n, 3)) a.split = n;
     if (tiles * a.G * a.split > 2147483647LL) return KP_ERR_UNSUPPORTED;
     const Kv4Launch l((unsigned)(tiles * a.G), a.split, 128, S::SMEM, st);
-    const cudaError_t c = cudaLaunchKernelEx(&l.cfg, kern, a);
+    const cudaError_t c = cudaLaunchKernelEx(&l.cfg, kv4_tiled_kernel<HD, PARTS, CENTRE, T>, a);
     return c ? (int)c : kp_launch_status();
 }
 
@@ -907,13 +933,13 @@ int kp_kv4_write(const void* k, long long ldk, const void* v, long long ldv, voi
     if (hd < 32 || hd % 32 || ps < 16 || (ps & (ps - 1)) || G < 1 || ((uintptr_t)pages & 15)) return KP_ERR_BAD_ARG;
     const Kv4Rows p = {n, kv4_log2(ps), G, hd, hd % 64 == 0 ? 64 : 32, n_pages * ps};
     unsigned blocks[2];
-    const int e = kv4_row_blocks(p, blocks);
+    const int e = kv4_row_blocks(p, 3, blocks);
     if (e) return e;
     const bool many = blocks[0] > KV4_ONE_ROW;
     KP_DISPATCH_DTYPE(dtype, T, {
         const long long a = 16 / sizeof(T);
         const bool vec = !(((uintptr_t)k | (uintptr_t)v) & 15) && ldk % a == 0 && ldv % a == 0;
-        auto kern = vec ? (many ? kv4_write_kernel<T, true, 4> : kv4_write_kernel<T, true, 1>) : (many ? kv4_write_kernel<T, false, 4> : kv4_write_kernel<T, false, 1>);
+        auto kern = vec ? (many ? kv4_write_kernel<T, true, 3> : kv4_write_kernel<T, true, 1>) : (many ? kv4_write_kernel<T, false, 3> : kv4_write_kernel<T, false, 1>);
         const cudaError_t c = kp_launch_pdl(kern, dim3(blocks[many]), dim3(256), 0, (cudaStream_t)stream, (const T*)k, ldk, (const T*)v, ldv,
                                             (unsigned char*)pages, slot_map, p);
         if (c) return (int)c;
@@ -926,7 +952,7 @@ int kp_kv4_read(const void* pages, long long n_pages, const int* slot_map, void*
     if (hd < 32 || hd % 32 || ps < 16 || (ps & (ps - 1)) || G < 1 || (((uintptr_t)pages | (uintptr_t)k | (uintptr_t)v) & 15)) return KP_ERR_BAD_ARG;
     const Kv4Rows p = {n, kv4_log2(ps), G, hd, hd % 64 == 0 ? 64 : 32, n_pages * ps};
     unsigned blocks[2];
-    const int e = kv4_row_blocks(p, blocks);
+    const int e = kv4_row_blocks(p, 4, blocks);
     if (e) return e;
     const bool many = blocks[0] > KV4_ONE_ROW;
     KP_DISPATCH_DTYPE(dtype, T, {
