@@ -227,8 +227,9 @@ __device__ __forceinline__ void kv4_columns(Kv4Cols<NT>& C, int col0, int n_cols
 // ---- split form: few rows a segment (decode).  One CTA per (chunk of keys, kv head and 8 of its columns, segment).  Its tiles of KEYS
 // keys come by the TMA into a ring of three stages, asked for two tiles ahead by the warps in turn; each of the four warps takes a
 // quarter of a tile, with the softmax and output of its own keys, and the four are joined at the end.  What bounds it is the issue of
-// instructions, 170 a block of 16 keys of 64 values (1,152 bytes; 192 slots would pass while those come at the copy rate): hence the TMA and
-// not cp.async (97 instructions a block), tiles asked for by one warp and not by each (65 against 15), four CTAs an SM.
+// instructions, 174 a block of 16 keys of 64 values and 328 of 128 (142 for the scores, 115 for the values), at half of what the SMs could
+// issue: hence the TMA and not cp.async (410 a block of 128 values), four CTAs an SM, and codes that are operands as they lie.  64 sequences
+// of 1,000 to 2,100 keys, 32 heads over 8 of 128 values: 42 us, 2.7 TB/s; two of 131,072 keys with mass, 16 heads over 8 of 64: 67 us, 2.1 TB/s.
 KP_STATUS_WORD(g_kv4_status, kv4)                     // 0 ok; 1: a bounded wait gave up
 
 template <int HD, int PARTS>
@@ -563,7 +564,8 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
     }
 }
 
-// ---- tiled form: many rows a segment (portions of prompts).  A CTA takes 32 NT columns of a kv head (8 NT a warp) and walks
+// ---- tiled form: many rows a segment (portions of prompts) that the tcgen05 form does not take.  A CTA takes 32 NT columns of a kv head (8 NT a warp,
+// as many as the registers of its output hold: codes become operands once for all of them) and walks
 // their keys in tiles of 64 that its warps bring and share.
 template <int HD, int PARTS>
 struct Kv4Tiled {

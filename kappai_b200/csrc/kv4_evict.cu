@@ -24,7 +24,8 @@ __device__ __forceinline__ uint32_t ke_order(float m) {
 
 // ---- which keys stay: one CTA a (segment, kv head).  A radix selection finds the want-th largest mass, 11, 11 and 10 bits at a time,
 // from masses that were brought to shared memory once (more than fit there are read again each time); then every warp has a stretch
-// of the keys, counts in it and, when it knows what stands in front of it, writes down the ones that stay, in their order.
+// of the keys, counts in it and, when it knows what stands in front of it, writes down the ones that stay, in their order.  16 x 8 lists of up
+// to 16,384 masses: 20 us (a CTA a list, 128 of 148 SMs: the passes over shared memory bound it, not the 8 MB).
 __global__ void __launch_bounds__(KE_THREADS)
 kv4_select_kernel(const KeArgs p) {
     kp_pdl_begin();

@@ -20,6 +20,10 @@
 // (O is rescaled when it does): fp16 then holds whatever bfloat16 did.  P is taken against a reference that follows the row's maximum
 // in steps of at least 2^8 (O is rescaled in tensor memory only then), P <= 2^15.
 // Every mbarrier wait is bounded; one that gives up sets the status word, and the CTA frees its tensor memory and returns.
+//
+// Measured.  A tile (256 columns, 128 keys) takes 1.9 us with heads of 64, whose exponentials alone are 1.04 us of the SM's, and 2.4 us with heads of
+// 128, whose products are 1.1: what bounds it is the chain of S, softmax, P and second product, which two groups cannot hide.  A CTA's start
+// and end take 8 us and 12.  1,024 rows of 32 heads over 8 of 128 values behind 15,360 keys: 326 us, 0.81 PFLOP/s.
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 
@@ -648,7 +652,8 @@ __device__ __forceinline__ float kt_column_sum(uint32_t tmem_s, const float4* co
 // ---- mass.  A cluster of CTAs per (128 keys, kv head, segment): S^T = K Q^T with a thread a key, so that a key's weights add up in its
 // thread.  The operands of Q and the columns' (factor, lse) are those that the kernel above left, brought by bulk copies into a ring; the two groups
 // of 128 threads take the tiles of 128 columns in turn.  The CTAs of a cluster share the columns out (the first keys of a prompt are
-// read by all of it), and their sums are added in order.
+// read by all of it), and their sums are added in order.  2,048 rows of 32 heads over 8 of 64: 38 us, of which the exponentials are 16.  (Two tiles of
+// keys a CTA for each image, to halve their way from L2: slower by 4 to 5 us there, with one CTA's start for twice the keys.)
 template <int HD>
 __global__ void __launch_bounds__(Kt<HD>::MASS_THREADS, 2)
 kv4_tc_mass_kernel(const Kv4TcArgs p) {
