@@ -414,39 +414,56 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
     float* lse = jm;                                       // (the warps' shifts have been read) [column]
     if (p.n_chunks > 1) {
         // the cluster's CTAs are the chunks: each joins its share of the outputs, in the order of the chunks, from all of them
+        float* weight = jo;                                // (so have their results) [column][chunk of 8]
         kv4_cluster_sync();
+        if (threadIdx.x < live) {
+            float m[8], l[8], M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k < p.n_chunks) { m[k] = kv4_peer(cm + threadIdx.x, k); l[k] = kv4_peer(cl + threadIdx.x, k); }
+#pragma unroll
+            for (int k = 0; k < 8; k++) if (k < p.n_chunks) M = fmaxf(M, m[k]);
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k < p.n_chunks) { m[k] = kv4_exp2(m[k] - (M == -INFINITY ? 0.f : M)); L = fmaf(l[k], m[k], L); }
+#pragma unroll
+            for (int k = 0; k < 8; k++) if (k < p.n_chunks) weight[threadIdx.x * 8 + k] = M == -INFINITY ? 0.f : m[k] / L;
+            if (KEEP) lse[threadIdx.x] = M == -INFINITY ? INFINITY : M + log2f(L);
+        }
+        __syncthreads();
         for (int e = chunk * 128 + threadIdx.x; e < live * HD; e += p.n_chunks * 128) {
             const int c = e / HD;
-            float M = -INFINITY, acc = 0.f, L = 0.f;
-            for (int k = 0; k < p.n_chunks; k++) M = fmaxf(M, kv4_peer(cm + c, k));
-            for (int k = 0; k < p.n_chunks; k++) {
-                const float m = kv4_peer(cm + c, k);
-                if (m == -INFINITY) continue;
-                const float f = kv4_exp2(m - M);
-                acc = fmaf(kv4_peer(co + e, k), f, acc);
-                L = fmaf(kv4_peer(cl + c, k), f, L);
-            }
-            write(c, e - c * HD, M == -INFINITY ? 0.f : acc / L);
-        }
-        if (KEEP && threadIdx.x < live) {
-            float M = -INFINITY, L = 0.f;
-            for (int k = 0; k < p.n_chunks; k++) M = fmaxf(M, kv4_peer(cm + threadIdx.x, k));
-            for (int k = 0; k < p.n_chunks; k++) {
-                const float m = kv4_peer(cm + threadIdx.x, k);
-                if (m != -INFINITY) L = fmaf(kv4_peer(cl + threadIdx.x, k), kv4_exp2(m - M), L);
-            }
-            lse[threadIdx.x] = M == -INFINITY ? INFINITY : M + log2f(L);
+            float x[8], acc = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) if (k < p.n_chunks) x[k] = kv4_peer(co + e, k);
+#pragma unroll
+            for (int k = 0; k < 8; k++) if (k < p.n_chunks) acc = fmaf(x[k], weight[c * 8 + k], acc);
+            write(c, e - c * HD, acc);
         }
     }
     if (KEEP) {
-        // the weights of the chunk's keys: a thread a key, columns in order (they are all of the segment's)
+        // the weights of the chunk's keys: a thread a key, columns in order (they are all of the segment's); all loads of four keys at once
         __syncthreads();
         const float* sums = p.n_chunks > 1 ? lse : cm;
-        for (int key = k_lo + threadIdx.x; key <= k_hi; key += 128) {
-            float w = 0.f;
-            for (int c = 0; c < live; c++) w += kv4_exp2(p.scores[place_of(c) * p.ld_scores + key - s_base] - sums[c]);
-            const int pg = bt[key >> p.ps_log2];
-            p.mass[((size_t)pg * p.G + kvh) * p.ps + (key & (p.ps - 1))] += w;
+        constexpr int U = 4;
+        for (int key0 = k_lo + threadIdx.x; key0 <= k_hi; key0 += 128 * U) {
+            float x[U][8], *to[U], had[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int key = min(key0 + u * 128, k_hi);
+                to[u] = p.mass + ((size_t)bt[key >> p.ps_log2] * p.G + kvh) * p.ps + (key & (p.ps - 1));
+#pragma unroll
+                for (int c = 0; c < 8; c++) if (c < live) x[u][c] = p.scores[place_of(c) * p.ld_scores + key - s_base];
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) had[u] = *to[u];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float w = 0.f;
+#pragma unroll
+                for (int c = 0; c < 8; c++) if (c < live) w += kv4_exp2(x[u][c] - sums[c]);
+                if (key0 + u * 128 <= k_hi) *to[u] = had[u] + w;
+            }
         }
     }
     if (p.n_chunks > 1) kv4_cluster_sync();                // (nobody leaves while another reads its shared memory)
