@@ -540,9 +540,33 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
     const int last = min(min(pos0 + n_rows, p.max_blocks * p.ps), base + p.ld_scores) - 1;
     if (n_rows > p.max_rows || k0 > last || k0 + KV4_MASS_KEYS - 1 < first) return;
     constexpr int U = KV4_MASS_KEYS / 128;
-    float sum[U];
+    // what does not wait for the chunks' sums is asked for first: the keys' masses, and the scores of the first two columns
+    float sum[U], had[U], *to[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) sum[u] = 0.f;
+    for (int u = 0; u < U; u++) {
+        const int key = min(max(k0 + u * 128 + (int)threadIdx.x, first), last);
+        to[u] = p.mass + ((size_t)p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)] * p.G + kvh) * p.ps + (key & (p.ps - 1));
+        sum[u] = 0.f;
+    }
+    struct Two { int lo[2], hi[2]; float x[2][U]; };
+    auto fetch = [&](Two& t, int c) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int r = (c + j) / R;
+            t.hi[j] = c + j < n_cols ? min(pos0 + r, last) : -1;
+            t.lo[j] = p.window > 0 ? max(0, pos0 + r - p.window + 1) : 0;
+            const float* sc = p.scores + (((size_t)seg * p.max_rows + r) * p.H + kvh * R + (c + j) % R) * p.ld_scores - base;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int key = k0 + u * 128 + threadIdx.x;
+                t.x[j][u] = key >= t.lo[j] && key <= t.hi[j] ? sc[key] : 0.f;
+            }
+        }
+    };
+    Two now;
+    fetch(now, 0);
+#pragma unroll
+    for (int u = 0; u < U; u++) had[u] = *to[u];
     for (int c0 = 0; c0 < n_cols; c0 += 64) {
         const int n = min(64, n_cols - c0);
         __syncthreads();
@@ -561,23 +585,22 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
             if (lane == 0) lse[i] = v;
         }
         __syncthreads();
-#pragma unroll 2
-        for (int i = 0; i < n; i++) {
-            const int r = (c0 + i) / R, hi = min(pos0 + r, last), lo = p.window > 0 ? max(0, pos0 + r - p.window + 1) : 0;
-            const float* sc = p.scores + (((size_t)seg * p.max_rows + r) * p.H + kvh * R + (c0 + i) % R) * p.ld_scores - base;
+#pragma unroll 1
+        for (int i = 0; i < n; i += 2) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int key = k0 + u * 128 + threadIdx.x;
-                if (key >= lo && key <= hi) sum[u] += kv4_exp2(sc[key] - lse[i]);
-            }
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int key = k0 + u * 128 + threadIdx.x;
+                    if (key >= now.lo[j] && key <= now.hi[j]) sum[u] += kv4_exp2(now.x[j][u] - lse[i + j]);
+                }
+            if (c0 + i + 2 < n_cols) fetch(now, c0 + i + 2);
         }
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int key = k0 + u * 128 + threadIdx.x;
-        if (key < first || key > last) continue;
-        const int page = p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)];
-        p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += sum[u];
+        if (key >= first && key <= last) *to[u] = had[u] + sum[u];
     }
 }
 
