@@ -694,7 +694,8 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     __syncthreads();
     kp_tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    float sum = 0.f;
+    float sum = 0.f, had = 0.f;                        // this key's weight here; its mass before, and where that lies
+    float* to = nullptr;
 
     if (warp == 8) {
         // ---- copies and products
@@ -733,6 +734,10 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
             const int page = there ? p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)] : 0;
             KtRow<HD> x;
             x.load(p.pages + ((size_t)page * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key & (p.ps - 1), p.ps, there, false);
+            if (there && rank == 0) {
+                to = p.mass + ((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1));
+                had = *to;
+            }
             int ek = -100;
 #pragma unroll
             for (int y = 0; y < S::NG; y++) ek = max(ek, kt_exponent(x.r[y]));
@@ -771,14 +776,10 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     float* join = reinterpret_cast<float*>(Ks);        // [group][key]; the cluster's first CTA adds them up, in order
     if (warp < 8) join[threadIdx.x] = sum;
     if (n_ctas > 1) kv4_cluster_sync(); else __syncthreads();
-    if (rank == 0 && warp < 4) {
-        const int key = k0 + threadIdx.x;
-        if (key >= first && key <= last) {
-            float all = join[threadIdx.x] + join[128 + threadIdx.x];
-            for (int r = 1; r < n_ctas; r++) all += kv4_peer(join + threadIdx.x, r) + kv4_peer(join + 128 + threadIdx.x, r);
-            const int page = p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)];
-            p.mass[((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1))] += all;
-        }
+    if (to) {
+        float all = sum + join[128 + threadIdx.x];
+        for (int r = 1; r < n_ctas; r++) all += kv4_peer(join + threadIdx.x, r) + kv4_peer(join + 128 + threadIdx.x, r);
+        *to = had + all;
     }
     if (n_ctas > 1) kv4_cluster_sync();                 // (nobody leaves while its sums are read)
 }
