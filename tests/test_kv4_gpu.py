@@ -190,6 +190,29 @@ def test_written_values_at_the_edges():
     assert bool(torch.isnan(held).all())                                                       # the row without a slot wrote nothing
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("factor", [1.0, 1e-3, 3e4, 1e-20, 1e25, 1e-33, 2e36])
+@pytest.mark.parametrize("kind", ["normal", "halves", "far from zero"])
+def test_codes_are_those_of_the_division(dtype, factor, kind):
+    """The kernel does not divide: its codes are those of the rounded quotient all the same, at halves and at scales without a reciprocal."""
+    n, G, hd, page = 2048, 2, 64, 16
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn((n, G * hd), generator=g, device=DEV)
+    if kind == "halves":
+        x = torch.randint(-40, 40, (n, G * hd), generator=g, device=DEV) / 2.0 ** torch.randint(0, 4, (n, 1), generator=g, device=DEV)
+    k = ((x + 100 if kind == "far from zero" else x) * factor).to(dtype)
+    pages = torch.zeros((n // page, G, kv4.kv4_page_bytes(page, hd)), dtype=torch.uint8, device=DEV)
+    kv4.kv4_write(k, k, pages, torch.arange(n, dtype=torch.int32, device=DEV), page, G, hd)
+    x = k.float().view(n, G, hd)
+    least, most = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
+    s, z = ((most - least) / torch.tensor(15.0, device=DEV)).bfloat16(), least.bfloat16()
+    want = torch.where(s > 0, ((x - z.float()) / s.float()).clamp(0, 15).round(), 0.0).to(torch.uint8)
+    rows = lambda at, size: pages[:, :, at * page:(at + size) * page].view(n // page, G, page, size).permute(0, 2, 1, 3).reshape(n, G, size)  # noqa: E731
+    codes = rows(0, hd // 2)
+    assert torch.equal(torch.stack((codes & 15, codes >> 4), -1).view(n, G, hd), want)
+    assert torch.equal(rows(hd, 4).contiguous().view(torch.int16), torch.cat((s, z), -1).contiguous().view(torch.int16))
+
+
 def test_values_that_are_not_finite_spoil_their_group_only():
     hd, G, page = 128, 2, 16
     x = np.random.default_rng(0).standard_normal((3, G * hd)).astype(np.float32)
