@@ -611,7 +611,7 @@ template <int HD, int PARTS>
 struct Kv4Tiled {
     static constexpr int NT = PARTS == 1 ? (HD <= 64 ? 4 : (HD <= 128 ? 2 : 1)) : (HD <= 64 ? 2 : 1);
     static constexpr int COLS = 32 * NT, TILE = 64, STAGE = Kv4<HD>::bytes(64);
-    static constexpr size_t JOIN = sizeof(float) * kv4_share_floats(COLS, HD), SMEM = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
+    static constexpr size_t JOIN = sizeof(float) * kv4_share_floats(COLS, HD, 8), SMEM = 2 * STAGE > JOIN ? 2 * STAGE : JOIN;
 };
 
 // The tile'th of the tiles that the segments of at least min_rows rows make of `per` columns each: its segment and first column
@@ -727,7 +727,7 @@ kv4_tiled_kernel(const Kv4Args p) {
                 if (lane < 4) kv4_share_sums(part, S::COLS, HD, c, A.shift[nt][i], A.l[nt][i]);
             }
         kv4_cluster_sync();
-        kv4_join_shares<T, HD, S::COLS, 128, false>(
+        kv4_join_shares<T, HD, S::COLS, 128, false, 8>(
             part, p.split, rank, cta_col1 - cta_col0 + 1,
             [&](int col) { return (T*)p.out + (size_t)(row0 + (cta_col0 + col) / R) * p.ldo + (size_t)(kvh * R + (cta_col0 + col) % R) * HD; },
             [&](int col, float top, float sum) {

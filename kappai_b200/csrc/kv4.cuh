@@ -538,15 +538,15 @@ __device__ __forceinline__ float4 kv4_peer4(const float* p, int rank) {
     return v;
 }
 // A CTA's share of a tile of `cols` rows in shared memory: [column][HD] float32, each row divided by its own sum, shift [column], sum of p [column], and
-// room for the weights of the join [column][8].  Four dimensions lie together, eight such places turned by the column.
-__host__ __device__ constexpr int kv4_share_floats(int cols, int hd) { return cols * (hd + 10); }
+// room for the weights of the join [column][most].  Four dimensions lie together, eight such places turned by the column.
+__host__ __device__ constexpr int kv4_share_floats(int cols, int hd, int most) { return cols * (hd + 2 + most); }
 __device__ __forceinline__ int kv4_share_at(int col, int d, int hd) { return col * hd + ((d >> 2 ^ (col & 7)) << 2) + (d & 3); }
 __device__ __forceinline__ void kv4_share_sums(float* part, int cols, int hd, int col, float shift, float sum) {
     part[cols * hd + col] = shift;
     part[cols * (hd + 1) + col] = sum;
 }
 // Rows of this CTA's columns from the shares of the cluster's n CTAs (at most MOST), four dimensions a thread; BATCH loads from each are under way at once
-template <typename T, int HD, int THREADS, bool ALIGNED, int MOST, int BATCH, typename RowOf>
+template <typename T, int HD, int THREADS, bool ALIGNED, int STRIDE, int MOST, int BATCH, typename RowOf>
 __device__ __forceinline__ void kv4_join_rows(const float* part, const float* weight, int rank, int n, int n_cols, RowOf row_of) {
     constexpr int LANES = HD / 4;
     for (int i0 = threadIdx.x; i0 < n_cols * LANES; i0 += THREADS * BATCH) {
@@ -566,7 +566,7 @@ __device__ __forceinline__ void kv4_join_rows(const float* part, const float* we
 #pragma unroll
             for (int j = 0; j < MOST; j++)
                 if (j < n) {
-                    const float y = weight[col * 8 + j];
+                    const float y = weight[col * STRIDE + j];
                     x = make_float4(fmaf(y, v[b][j].x, x.x), fmaf(y, v[b][j].y, x.y), fmaf(y, v[b][j].z, x.z), fmaf(y, v[b][j].w, x.w));
                 }
             T* dst = row_of(col) + i % LANES * 4;
@@ -581,30 +581,31 @@ __device__ __forceinline__ void kv4_join_rows(const float* part, const float* we
 // The rows of n_here columns from the shares of the cluster's n CTAs, each weighted by its part of the sum, added in order, by THREADS threads, between
 // two meetings of the cluster.  The CTAs share the columns out: this one has every n-th.  sums_of gets a column's shift and sum.  ALIGNED: bfloat16 rows
 // on 8-byte boundaries.
-template <typename T, int HD, int COLS, int THREADS, bool ALIGNED, typename RowOf, typename SumsOf>
+template <typename T, int HD, int COLS, int THREADS, bool ALIGNED, int MOST, typename RowOf, typename SumsOf>
 __device__ __forceinline__ void kv4_join_shares(float* part, int n, int rank, int n_here, RowOf row_of, SumsOf sums_of) {
     const float* stat = part + COLS * HD;
     float* weight = part + COLS * (HD + 2);
     const int col = rank + threadIdx.x * n;
     if (col < COLS) {
-        float m[8], l[8], top = -INFINITY, sum = 0.f;
+        float m[MOST], l[MOST], top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++)
+        for (int j = 0; j < MOST; j++)
             if (j < n) { m[j] = kv4_peer(stat + col, j); l[j] = kv4_peer(stat + COLS + col, j); }
 #pragma unroll
-        for (int j = 0; j < 8; j++) if (j < n) top = fmaxf(top, m[j]);
+        for (int j = 0; j < MOST; j++) if (j < n) top = fmaxf(top, m[j]);
 #pragma unroll
-        for (int j = 0; j < 8; j++)
+        for (int j = 0; j < MOST; j++)
             if (j < n) { l[j] *= kv4_exp2(m[j] - (top == -INFINITY ? 0.f : top)); sum += l[j]; }
 #pragma unroll
-        for (int j = 0; j < 8; j++) if (j < n) weight[col * 8 + j] = sum == 0.f ? 0.f : l[j] / sum;
+        for (int j = 0; j < MOST; j++) if (j < n) weight[col * MOST + j] = sum == 0.f ? 0.f : l[j] / sum;
         sums_of(col, top, sum);
     }
     asm volatile("bar.sync 4, %0;" ::"n"(THREADS) : "memory");
     const int n_cta = (n_here + n - 1 - rank) / n;         // this CTA's columns
-    if (n == 2) kv4_join_rows<T, HD, THREADS, ALIGNED, 2, 4>(part, weight, rank, n, n_cta, row_of);
-    else if (n <= 4) kv4_join_rows<T, HD, THREADS, ALIGNED, 4, 2>(part, weight, rank, n, n_cta, row_of);
-    else kv4_join_rows<T, HD, THREADS, ALIGNED, 8, 1>(part, weight, rank, n, n_cta, row_of);
+    if (n == 2) kv4_join_rows<T, HD, THREADS, ALIGNED, MOST, 2, 4>(part, weight, rank, n, n_cta, row_of);
+    else if (n <= 4) kv4_join_rows<T, HD, THREADS, ALIGNED, MOST, 4, 2>(part, weight, rank, n, n_cta, row_of);
+    else if (MOST == 8 || n <= 8) kv4_join_rows<T, HD, THREADS, ALIGNED, MOST, 8, 1>(part, weight, rank, n, n_cta, row_of);
+    else kv4_join_rows<T, HD, THREADS, ALIGNED, MOST, MOST, 1>(part, weight, rank, n, n_cta, row_of);
 }
 
 // ---- launches of `places` clusters of `cluster` CTAs
@@ -625,15 +626,19 @@ struct Kv4Launch {
         cfg.numAttrs = cluster > 1 ? 2 : 1;
     }
 };
-// clusters of n (at most 8) CTAs of a kernel that the GPU holds at once (the kernel's limit of shared memory has been raised)
+// clusters of n (at most 16; above 8 the kernel has to be let) CTAs of a kernel that the GPU holds at once (its limit of shared memory has been raised)
 template <auto KERNEL>
 static int kv4_fit(int n, int threads, size_t smem) {
-    static std::atomic<int> known[64][9];                  // one more than the answer, by device
+    static std::atomic<int> known[64][17];                 // one more than the answer, by device
     int dev = 0, fit = 0;
     if (cudaGetDevice(&dev) || dev >= 64) return 0;
     if (const int k = known[dev][n]) return k - 1;
     const Kv4Launch l(1, n, threads, smem, nullptr);
-    if (cudaOccupancyMaxActiveClusters(&fit, KERNEL, &l.cfg)) { cudaGetLastError(); fit = 0; }
+    if ((n > 8 && cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) ||
+        cudaOccupancyMaxActiveClusters(&fit, KERNEL, &l.cfg)) {
+        cudaGetLastError();
+        fit = 0;
+    }
     known[dev][n] = fit + 1;
     return fit;
 }

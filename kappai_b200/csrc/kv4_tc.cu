@@ -30,6 +30,7 @@
 KP_STATUS_WORD(g_kv4_tc_status, kv4_tc)               // 0 ok; 1: a bounded wait gave up
 
 #define KT_ROWS 128                                    // columns a group, and keys a tile
+#define KT_MOST 16                                     // most CTAs that share a tile's keys
 #define KT_EXT 4096                                    // 128 rows of 16 fp16 beside a tile: the parts of the second term
 
 struct Kv4TcArgs {
@@ -271,8 +272,8 @@ template <int HD>
 __device__ __noinline__ void kt_join_shares(const Kv4TcArgs& p, unsigned char* sm, int rank, int kvh, int tile, int row0, int cta_col0, int n_here) {
     const int R = p.H / p.G;
     float* part = reinterpret_cast<float*>(sm);
-    const float* factor = part + kv4_share_floats(256, HD);
-    kv4_join_shares<bf16, HD, 256, 256, true>(
+    const float* factor = part + kv4_share_floats(256, HD, KT_MOST);
+    kv4_join_shares<bf16, HD, 256, 256, true, KT_MOST>(
         part, p.split, rank, n_here,
         [&](int col) { return p.out + (size_t)(row0 + (cta_col0 + col) / R) * p.ldo + (size_t)(kvh * R + (cta_col0 + col) % R) * HD; },
         [&](int col, float top, float sum) {
@@ -577,7 +578,7 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
                 }
             }
             kv4_share_sums(part, 256, HD, col, m, l);
-            part[kv4_share_floats(256, HD) + col] = f;
+            part[kv4_share_floats(256, HD, KT_MOST) + col] = f;
         } else {
             if (p.mass) {
                 p.col[((size_t)kvh * p.n_tiles + tile) * 256 + g * 128 + r] = make_float2(f, none ? INFINITY : m - 7.0f + log2f(l));
@@ -797,13 +798,15 @@ static int kt_run(Kv4TcArgs a, int max_context, long long busy, cudaStream_t st)
     // 4096 keys 137 against 154, 4 x 1024 behind 1024 223 against 243.
     const int tiles = (max_context + KT_ROWS - 1) / KT_ROWS;
     const long long places = (long long)tiles * a.n_seg * a.G;
-    // A tile's keys over as many CTAs, up to eight, as the GPU holds clusters of, where each has a tile of keys and there are three or more:
+    // A tile's keys over as many CTAs, up to 16 (8 is what clusters may have without being let), as the GPU holds clusters of, where each has a tile of
+    // keys and there are three or more:
     // the join costs less than the second tile.  Measured with 32 heads over 8, one CTA a tile against the rule's: 64 rows behind 16000 keys
-    // 249 us against 45, 300 behind 4096 111 against 47, 512 behind 1024 32 against 24, 64 behind 512 18.5 against 15; 256 rows and no
+    // 249 us against 41 (45 with at most eight; over 2 kv heads 247, 32 and 44), 300 behind 4096 79 against 37, 512 behind 1024 32 against 24, 64 behind
+    // 512 18.5 against 15; 256 rows and no
     // more (two tiles of keys) 13.1 against 14.6, 1024 behind 4096, whose pairs would not all be there at once, 87 against 97.
     const int reach = a.window > 0 && a.window + 256 / (a.H / a.G) < max_context ? a.window + 256 / (a.H / a.G) : max_context;
     a.split = 1;
-    for (int n = 8; n > 1 && a.split == 1; n--)
+    for (int n = KT_MOST; n > 1 && a.split == 1; n--)
         if (busy * a.G <= kv4_fit<kv4_tc_kernel<HD, true>>(n, S::THREADS, S::SMEM) && (reach + KT_ROWS - 1) / KT_ROWS >= max(n, 3)) a.split = n;
     if ((long long)a.n_tiles * a.G > 2147483647LL || (a.mass && places > 2147483647LL)) return KP_ERR_UNSUPPORTED;
     const Kv4Launch l((unsigned)a.n_tiles * a.G, a.split, S::THREADS, S::SMEM, st);

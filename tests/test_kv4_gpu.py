@@ -286,7 +286,7 @@ def test_long_contexts(dtype, hd, lengths, rows):
                                                      ([800], [40], 5, 1, None), ([2050], [130], 8, 2, None), ([600], [300], 32, 32, None),
                                                      ([900, 40, 12, 300], [20, 20, 12, 33], 4, 2, None), ([1500, 1400], [30, 9], 4, 2, 200), ([900], [30], 4, 1, 3)])
 def test_keys_that_a_cluster_shares_out(dtype, hd, lengths, rows, H, G, window):
-    """Few rows over many keys: two to eight CTAs a tile, some of them without a key of a shorter sequence."""
+    """Few rows over many keys: two to sixteen CTAs a tile, some of them without a key of a shorter sequence."""
     run_and_check(lengths, rows, H, G, hd, 32, dtype, window)
     run_and_check(lengths, rows, H, G, hd, 32, dtype, window, mass=False, seed=8, strided=True)
 
