@@ -124,6 +124,8 @@ class Kv4Cache:
         past = [self._length[s] - n for s, n in zip(seqs, rows)]
         if min(past, default=0) < 0:
             raise CacheError("attend: more rows than keys; append them first")
+        if q.dim() != 2 or q.shape[0] != sum(rows):
+            raise CacheError(f"attend: {sum(rows)} rows of queries were announced, got a tensor of shape {tuple(q.shape)}")
         out = torch.empty((q.shape[0], q.shape[1]), dtype=q.dtype, device=q.device) if out is None else out
         if not seqs:
             return out

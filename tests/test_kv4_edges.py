@@ -1,0 +1,24 @@
+"""The 4-bit cache's bookkeeping where a call is wrong, or nothing is there: no device is needed for any of it."""
+import pytest
+import torch
+
+from kappai_b200 import Kv4Cache
+from kappai_b200.cache import CacheError
+from kappai_b200.ops import kv4
+from kappai_b200.ops.kernels import KernelError
+
+
+def held(n, n_pages=8, mass=False):
+    """A cache whose sequence "a" has n keys, nothing of them written."""
+    c = Kv4Cache(2, 64, n_pages, page_size=16, mass=mass, device="cpu")
+    c.add("a")
+    c.pool.extend("a", n)
+    c._length["a"] = n
+    return c
+
+
+@pytest.mark.parametrize("shape", [(3, 256), (5, 256), (0, 256), (4, 4, 64), (1024,)])
+def test_attend_takes_as_many_queries_as_rows(shape):
+    """Fewer would be read, and their outputs written, behind the tensors' ends; more would leave rows of the output as they were."""
+    with pytest.raises(CacheError, match="rows of queries"):
+        held(20).attend(torch.zeros(shape), ["a"], [4], 4, 0.125)
