@@ -174,25 +174,24 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     window = window or 0
     if short or (tiled and not tc):
         n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd, min_rows if short and tiled else None)
-        # one allocation for what the launches hand one another: results of chunks, their (shift, sum), scores, logarithms of sums
+        # one allocation for what the launches hand one another: results of chunks, their (shift, sum), scores, logarithms of sums.  It has a
+        # name until this function returns: another thread would be given memory that is free before the launch that uses it is queued.
         fused = n_chunks <= 8 and (pm is None or short * (H // G) <= 8)
         places, many = n_seg * short * H, n_chunks > 1 and not fused
         sizes = (places * n_chunks * hd if many else 0, places * n_chunks * 2 if many else 0,
                  places * n_chunks * chunk if pm else 0, places if pm and not fused else 0, n * H if pm and tiled and not tc else 0)
         total = sum(sizes)
-        p0 = torch.empty(total, dtype=torch.float32, device=q.device).data_ptr() if total else 0
+        scratch = torch.empty(total, dtype=torch.float32, device=q.device) if total else None
+        p0 = scratch.data_ptr() if total else 0
         p1 = p0 + 4 * sizes[0]
         p2 = p1 + 4 * sizes[1]
         p3 = p2 + 4 * sizes[2]
         _run("kv4_attention", _fn("kp_kv4_attention"), pq, ldq, at, pages.shape[0], table, width, cu, pos, n_seg, po, ldo, scale, window, page_size, H, G,
              hd, n, short, max_rows if tiled and not tc else 0, n_chunks, chunk, fused, max_context, p0, p1, p2, n_chunks * chunk, p3, p3 + 4 * sizes[3], pm, code, STREAM)
     if tc:
-        scratch = None
-        if pm:
-            size = _tc_scratch(n, n_seg, H, G, hd)
-            scratch = torch.empty(size, dtype=torch.uint8, device=q.device).data_ptr()
+        images = torch.empty(_tc_scratch(n, n_seg, H, G, hd), dtype=torch.uint8, device=q.device) if pm else None
         _run("kv4_attention_tc", _fn("kp_kv4_attention_tc"), pq, ldq, at, table, width, cu, pos, n_seg, po, ldo, scale, window, page_size, H, G, hd, n,
-             short + 1, max_rows, max_context, pm, scratch, STREAM)
+             short + 1, max_rows, max_context, pm, images.data_ptr() if pm else None, STREAM)
     return out
 
 

@@ -1,0 +1,72 @@
+"""The 4-bit cache's kernels at the edges of what they promise, against the definition in 64 bits.
+
+The plain implementation and its tolerances are those of test_kv4_gpu.py; where a test has one of its own it says how that was derived.
+"""
+import numpy as np
+import pytest
+import torch
+
+from kappai_b200 import Kv4Cache
+from kappai_b200.ops import kv4
+from kappai_b200.ops.kernels import KernelError, read_status
+from test_kv4_gpu import DEV, Paged, plain_attention, plain_values
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def attend(P, q, rows, H, scale=None, window=None, mass=None, table=None, pos=None, min_rows=None, out=None):
+    """kv4_attention of the last `rows[i]` keys' rows of every sequence."""
+    cu = np.concatenate([[0], np.cumsum(rows)])
+    pos = [n - r for n, r in zip(P.lengths, rows)] if pos is None else pos
+    out = torch.full_like(q, float("nan")) if out is None else out
+    return kv4.kv4_attention(q, P.pages, P.table_d if table is None else table, i32(cu.tolist()), i32(pos), out, P.hd ** -0.5 if scale is None else scale, window,
+                             P.page, H, P.G, P.hd, max(rows), max(1, max(p + r for p, r in zip(pos, rows))), min_rows=min(rows) if min_rows is None else min_rows,
+                             mass=mass)
+
+
+def queries(n, width, dtype, seed=1):
+    return torch.from_numpy(np.random.default_rng(seed).standard_normal((n, width)).astype(np.float32)).to(dtype)
+
+
+def near(have, want, most, dtype):
+    """test_kv4_gpu.py's bounds: 1e-4 for float32 rows, the output's rounding and two of fp16 for bfloat16 ones."""
+    if dtype == torch.float32:
+        np.testing.assert_allclose(have, want, rtol=0, atol=1e-4)
+    else:
+        assert (np.abs(have - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * most).all(), np.abs(have - want).max()
+
+
+# dtype, head size and rows behind 700 keys that take each form: split, its chunks joined, tiled, tcgen05
+FORMS = [(torch.bfloat16, 64, 1), (torch.bfloat16, 128, 3), (torch.float32, 96, 2), (torch.float32, 64, 60), (torch.bfloat16, 96, 60), (torch.bfloat16, 64, 60),
+         (torch.bfloat16, 128, 60), (torch.bfloat16, 128, 300)]
+
+
+@pytest.mark.parametrize("dtype,hd,rows,lengths", [(torch.bfloat16, 64, [1, 1], [9000, 300]), (torch.float32, 64, [60], [700]), (torch.bfloat16, 64, [60], [700]),
+                                                   (torch.bfloat16, 128, [1, 60], [9000, 700])])
+def test_scratch_is_held_until_the_launch_has_returned(dtype, hd, rows, lengths, monkeypatch):
+    """What the allocator gives somebody else while a launcher runs is not what the launcher was handed.  (Nothing is launched here.)"""
+    H, G = 4, 2
+    P = Paged(lengths, G, hd, 16, 3, dtype)
+    q, mass = queries(sum(rows), H * hd, dtype).to(DEV), P.mass()
+    sizes, calls, empty = [], [], torch.empty
+
+    def noted(*a, **kw):
+        t = empty(*a, **kw)
+        sizes.append(t.numel() * t.element_size())
+        return t
+
+    def launcher(what, fn, *args, **kw):
+        theirs = [empty(n, dtype=torch.uint8, device=DEV) for n in sizes for _ in range(2)]
+        calls.append(what)
+        for t in theirs:
+            assert not any(isinstance(a, int) and t.data_ptr() <= a < t.data_ptr() + t.numel() for a in args), f"{what} was handed memory that is free"
+
+    out = torch.empty_like(q)
+    monkeypatch.setattr(kv4, "_run", launcher)
+    monkeypatch.setattr(torch, "empty", noted)
+    attend(P, q, rows, H, mass=mass, out=out)
+    assert calls and sizes
