@@ -10,12 +10,25 @@ before it.
 """
 from __future__ import annotations
 
+from functools import wraps
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from .manager import CacheError, PagePool
+
+
+def _on_its_device(method):
+    """The cache's device is the current one while a method of it runs: launches go to that device's current stream."""
+    @wraps(method)
+    def run(self, *args, **kw):
+        if self.device.type != "cuda":
+            return method(self, *args, **kw)
+        with torch.cuda.device(self.device):
+            return method(self, *args, **kw)
+
+    return run
 
 
 class Kv4Cache:
@@ -28,6 +41,8 @@ class Kv4Cache:
             raise CacheError(f"num_kv_heads={num_kv_heads} must be positive")
         self.G, self.hd, self.page_size = int(num_kv_heads), int(head_dim), int(page_size)
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         record = kv4_page_bytes(self.page_size, self.hd)
         self.pool = PagePool(n_pages, self.page_size)
         self.pages = torch.zeros((n_pages, self.G, record), dtype=torch.uint8, device=self.device)
@@ -87,6 +102,7 @@ class Kv4Cache:
                 raise CacheError(f"{what}: {n} rows of sequence {s!r}")
 
     # -- the three operators
+    @_on_its_device
     def append(self, k: torch.Tensor, v: torch.Tensor, seqs: Sequence[Hashable], rows: Sequence[int]) -> None:
         """The next ``rows[i]`` keys and values of ``seqs[i]``: k and v are [sum of rows, num_kv_heads * head_dim], float32 or bfloat16,
         possibly columns of a wider product.  All sequences get their pages or none does (:class:`~.manager.OutOfPages`)."""
@@ -113,6 +129,7 @@ class Kv4Cache:
         for s, n in zip(seqs, rows):
             self._length[s] += n
 
+    @_on_its_device
     def attend(self, q: torch.Tensor, seqs: Sequence[Hashable], rows: Sequence[int], num_heads: int, scale: float,
                window: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of the last ``rows[i]`` tokens of ``seqs[i]`` (their keys and values have been appended): q is [sum of rows,
@@ -133,6 +150,7 @@ class Kv4Cache:
         return kv4_attention(q, self.pages, table, cu, pos, out, scale, window, self.page_size, num_heads, self.G, self.hd, max(rows),
                              max(p + n for p, n in zip(past, rows)), min_rows=min(rows), mass=self.mass)
 
+    @_on_its_device
     def evict(self, seqs: Sequence[Hashable], keep: int, recent: int = 0, first: int = 0) -> torch.Tensor:
         """Of each sequence every kv head keeps ``keep`` keys: the ``first`` first, the ``recent`` last and those with the most mass of the
         others; a sequence that has no more keeps all.  Returns the indices that the kept keys had, int32 [sequences, kv heads, keep],
@@ -176,6 +194,7 @@ class Kv4Cache:
             kept[torch.tensor([i for i, s in enumerate(seqs) if self._length[s] > 0], device=self.device)] = part
         return kept
 
+    @_on_its_device
     def read(self, seq: Hashable, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
         """The sequence's keys and values as the cache holds them, [length, num_kv_heads * head_dim]."""
         from ..ops.kv4 import kv4_read
@@ -185,6 +204,7 @@ class Kv4Cache:
         slots, = self._upload([self._slots(seq, 0, self._length[seq])])
         return kv4_read(self.pages, slots, self.page_size, self.G, self.hd, dtype)
 
+    @_on_its_device
     def mass_of(self, seq: Hashable) -> torch.Tensor:
         """The weight that the sequence's keys have got, [kv heads, length] (float32)."""
         if self.mass is None:

@@ -2,7 +2,7 @@
 
 Pages are one uint8 tensor ``[n_pages, G, page_bytes]``: of every kv head one record with the codes of ``page_size`` keys,
 those of their values, the keys' ranges and the values' ranges.  Key ``j`` of a sequence lies in page ``block_table[j //
-page_size]`` at place ``j % page_size``, as in the 16-bit cache.  Each function checks its tensors (device, dtype, layout),
+page_size]`` at place ``j % page_size``, as in the 16-bit cache.  Each function checks its tensors (the current device's, dtype, layout),
 launches on the current CUDA stream and raises :class:`~kappai_b200.ops.kernels.KernelError` on any error.
 """
 from __future__ import annotations
@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from .build import load_library
-from .kernels import STREAM, KernelError, _need, _rows_2d, _run, dtype_code
+from .kernels import STREAM, KernelError, _need, _raw_device, _rows_2d, _run, dtype_code
 
 KV4_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 # Segments of few columns (rows times the query heads of a kv head) take the split form, where eight columns share a block of keys.  Measured against
@@ -62,17 +62,28 @@ def kv4_page_bytes(page_size: int, hd: int) -> int:
     return page_size * (hd + 8 * (hd // kv4_group(hd)))
 
 
+_device = _raw_device or torch.cuda.current_device      # number of the current device
+
+
+def _elsewhere(t: torch.Tensor, name: str) -> None:
+    raise KernelError(f"{name}: is on {t.device}, the current device is cuda:{_device()}, to whose stream the launch would go")
+
+
 def _have(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
-    """The address of a contiguous CUDA tensor of that type."""
+    """The address of a contiguous tensor of that type on the current device."""
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
         _need(t, name, dtype)
+    if t.get_device() != _device():
+        _elsewhere(t, name)
     return t.data_ptr()
 
 
 def _have_rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, width: int) -> Tuple[int, int]:
-    """Address and row stride of a CUDA tensor [n, width] with contiguous rows."""
+    """Address and row stride of a tensor [n, width] with contiguous rows on the current device."""
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
         _need(t, name, dtype, contiguous=False)
+    if t.get_device() != _device():
+        _elsewhere(t, name)
     if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
         raise KernelError(f"{name}: expected [{n}, {width}], got {tuple(t.shape)}")
     return t.data_ptr(), _rows_2d(t, name)

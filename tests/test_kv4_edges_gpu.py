@@ -70,3 +70,43 @@ def test_scratch_is_held_until_the_launch_has_returned(dtype, hd, rows, lengths,
     monkeypatch.setattr(torch, "empty", noted)
     attend(P, q, rows, H, mass=mass, out=out)
     assert calls and sizes
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    """The launch goes to the current device's stream.  (A stand-in says that device 1 is current; nothing is launched.)"""
+    P = Paged([40], 2, 64, 16, 0)
+    new, kept, mass = Paged([8], 2, 64, 16, 1), torch.empty((1, 2, 8), dtype=torch.int32, device=DEV), P.mass()
+    q, k, s = torch.zeros((1, 256), device=DEV), torch.zeros((2, 128), device=DEV), i32([0, 1])
+    calls = [lambda: kv4.kv4_write(k, k, P.pages, s, 16, 2, 64), lambda: kv4.kv4_read(P.pages, s, 16, 2, 64), lambda: attend(P, q, [1], 4),
+             lambda: kv4.kv4_evict(P.pages, mass, P.table_d, i32([40]), new.pages, new.mass(), new.table_d, kept, 40, 8, 2, 1, 16, 2, 64)]
+    for call in calls:
+        call()
+    launched = []
+    monkeypatch.setattr(kv4, "_device", lambda: 1, raising=False)
+    monkeypatch.setattr(kv4, "_run", lambda *a, **kw: launched.append(a))
+    for call in calls:
+        with pytest.raises(KernelError, match="current device"):
+            call()
+    assert not launched
+
+
+def test_a_cache_works_on_its_own_device(monkeypatch):
+    """Every operator of a cache runs with the cache's device as the current one, whichever was before."""
+    c = Kv4Cache(2, 64, 16, page_size=16, mass=True, device=DEV)
+    assert c.device.index == torch.cuda.current_device()
+    entered = []
+    real = torch.cuda.device
+
+    class Noted(real):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+    monkeypatch.setattr(torch.cuda, "device", Noted)
+    x = torch.randn((40, 128), device=DEV)
+    c.add("a")
+    for call in (lambda: c.append(x, x, ["a"], [40]), lambda: c.attend(torch.randn((2, 256), device=DEV), ["a"], [2], 4, 0.125), lambda: c.evict(["a"], 20),
+                 lambda: c.read("a"), lambda: c.mass_of("a")):
+        before = len(entered)
+        call()
+        assert entered[before:] and set(entered) == {c.device.index}
