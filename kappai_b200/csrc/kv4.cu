@@ -447,7 +447,7 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
         const float* sums = p.n_chunks > 1 ? lse : cm;
         constexpr int U = 4;
         for (int key0 = k_lo + threadIdx.x; key0 <= k_hi; key0 += 128 * U) {
-            float x[U][8], *to[U], had[U];
+            float x[U][8], *to[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int key = min(key0 + u * 128, k_hi);
@@ -456,13 +456,11 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
                 for (int c = 0; c < 8; c++) if (c < live) x[u][c] = p.scores[place_of(c) * p.ld_scores + key - s_base];
             }
 #pragma unroll
-            for (int u = 0; u < U; u++) had[u] = *to[u];
-#pragma unroll
             for (int u = 0; u < U; u++) {
                 float w = 0.f;
 #pragma unroll
                 for (int c = 0; c < 8; c++) if (c < live) w += kv4_exp2(x[u][c] - sums[c]);
-                if (key0 + u * 128 <= k_hi) *to[u] = had[u] + w;
+                if (key0 + u * 128 <= k_hi) kv4_add_mass(to[u], w);
             }
         }
     }
@@ -540,8 +538,8 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
     const int last = min(min(pos0 + n_rows, p.max_blocks * p.ps), base + p.ld_scores) - 1;
     if (n_rows > p.max_rows || k0 > last || k0 + KV4_MASS_KEYS - 1 < first) return;
     constexpr int U = KV4_MASS_KEYS / 128;
-    // what does not wait for the chunks' sums is asked for first: the keys' masses, and the scores of the first two columns
-    float sum[U], had[U], *to[U];
+    // what does not wait for the chunks' sums is asked for first: where the keys' masses lie, and the scores of the first two columns
+    float sum[U], *to[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int key = min(max(k0 + u * 128 + (int)threadIdx.x, first), last);
@@ -565,8 +563,6 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
     };
     Two now;
     fetch(now, 0);
-#pragma unroll
-    for (int u = 0; u < U; u++) had[u] = *to[u];
     for (int c0 = 0; c0 < n_cols; c0 += 64) {
         const int n = min(64, n_cols - c0);
         __syncthreads();
@@ -600,7 +596,7 @@ kv4_join_kernel(const Kv4Args p, int hd, int n_join, int mass_blocks) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int key = k0 + u * 128 + threadIdx.x;
-        if (key >= first && key <= last) *to[u] = had[u] + sum[u];
+        if (key >= first && key <= last) kv4_add_mass(to[u], sum[u]);
     }
 }
 
@@ -841,7 +837,7 @@ kv4_mass_kernel(const Kv4Args p) {
     if (rank == 0 && k < KEYS && k0 + k <= last && k0 + k >= first) {
         for (int i = 1; i < n_ctas; i++) all += kv4_peer(part[0] + k, i);
         const int page = bt[(k0 + k) >> p.ps_log2];
-        p.mass[((size_t)page * p.G + kvh) * p.ps + ((k0 + k) & (p.ps - 1))] += all;
+        kv4_add_mass(p.mass + ((size_t)page * p.G + kvh) * p.ps + ((k0 + k) & (p.ps - 1)), all);
     }
     if (n_ctas > 1) kv4_cluster_sync();                    // (nobody leaves while its sums are read)
 }

@@ -517,6 +517,12 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
     }
 }
 
+// Adds a sequence's weights to a key's mass.  Each (sequence, kv head) adds once to a key in a launch, so the order of additions is fixed and the result's bits
+// are; where several sequences' tables name the same page each one's weights arrive, in an order that is not.
+__device__ __forceinline__ void kv4_add_mass(float* to, float w) {
+    asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to), "f"(w) : "memory");
+}
+
 // ---- CTAs of a cluster that share the keys of some columns
 __device__ __forceinline__ void kv4_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");

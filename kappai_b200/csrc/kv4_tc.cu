@@ -695,7 +695,7 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     __syncthreads();
     kp_tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    float sum = 0.f, had = 0.f;                        // this key's weight here; its mass before, and where that lies
+    float sum = 0.f;                                   // this key's weight here, and where its mass lies
     float* to = nullptr;
 
     if (warp == 8) {
@@ -735,10 +735,7 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
             const int page = there ? p.block_table[(size_t)seg * p.max_blocks + (key >> p.ps_log2)] : 0;
             KtRow<HD> x;
             x.load(p.pages + ((size_t)page * p.G + kvh) * (size_t)kv4_page_bytes(p.ps, HD), key & (p.ps - 1), p.ps, there, false);
-            if (there && rank == 0) {
-                to = p.mass + ((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1));
-                had = *to;
-            }
+            if (there && rank == 0) to = p.mass + ((size_t)page * p.G + kvh) * p.ps + (key & (p.ps - 1));
             int ek = -100;
 #pragma unroll
             for (int y = 0; y < S::NG; y++) ek = max(ek, kt_exponent(x.r[y]));
@@ -780,7 +777,7 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     if (to) {
         float all = sum + join[128 + threadIdx.x];
         for (int r = 1; r < n_ctas; r++) all += kv4_peer(join + threadIdx.x, r) + kv4_peer(join + 128 + threadIdx.x, r);
-        *to = had + all;
+        kv4_add_mass(to, all);
     }
     if (n_ctas > 1) kv4_cluster_sync();                 // (nobody leaves while its sums are read)
 }

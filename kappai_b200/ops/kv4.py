@@ -160,7 +160,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     the keys up to that one, of which ``window`` (None: all) the last; a row that reads none gives zeros.  ``max_rows`` and
     ``min_rows`` bound the rows of a sequence, ``max_context`` the keys that any row reads (host integers).  ``mass`` (float32
     [n_pages, G, page_size]): the softmax weight of every key, summed over the rows and the query heads of its kv head, is added
-    to the key's entry (in a fixed order: the same call gives the same bits)."""
+    to the key's entry, in a fixed order: the same call gives the same bits.  Sequences whose tables name the same pages each add their
+    weights; only the order in which these sums arrive is then not fixed."""
     if G < 1 or H % G:
         raise KernelError(f"kv4_attention: {H} query heads over {G} kv heads")
     n, n_seg, code = q.shape[0], seg_pos.numel(), dtype_code(q.dtype)

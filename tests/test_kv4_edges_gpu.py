@@ -110,3 +110,19 @@ def test_a_cache_works_on_its_own_device(monkeypatch):
         before = len(entered)
         call()
         assert entered[before:] and set(entered) == {c.device.index}
+
+
+@pytest.mark.parametrize("dtype,hd,rows", FORMS)
+@pytest.mark.parametrize("n", [700, 9000])
+def test_weights_of_keys_that_sequences_share(dtype, hd, rows, n):
+    """Several samples of one prompt: block tables that name the same pages.  Every sequence's weights reach the keys' mass.  (Each of 8 sequences' sums is off by
+    1e-5 of itself, their addition by less: the bounds of test_kv4_gpu.py hold for the whole.)"""
+    H, G, S = 4, 2, 8
+    P = Paged([n], G, hd, 16, 3, dtype)
+    q, mass = queries(S * rows, H * hd, dtype), P.mass(5)
+    m0 = mass.clone()
+    table = P.table_d.expand(S, -1).contiguous()
+    attend(P, q.to(DEV), [rows] * S, H, mass=mass, table=table, pos=[n - rows] * S)
+    want = sum(plain_attention(x.double().numpy().reshape(rows, H, hd), P.k[0], P.v[0], n - rows, hd ** -0.5, None, H)[1] for x in q.split(rows))
+    np.testing.assert_allclose(P.mass_of(mass, 0), P.mass_of(m0, 0) + want, rtol=1e-5, atol=1e-6)
+    assert not any(read_status().values())
