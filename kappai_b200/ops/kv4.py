@@ -65,39 +65,41 @@ def kv4_page_bytes(page_size: int, hd: int) -> int:
 _device = _raw_device or torch.cuda.current_device      # number of the current device
 
 
-def _elsewhere(t: torch.Tensor, name: str) -> None:
-    raise KernelError(f"{name}: is on {t.device}, the current device is cuda:{_device()}, to whose stream the launch would go")
+def _here(t: torch.Tensor) -> int:
+    """The current device's number, asked for once a call; a number that no tensor has where ``t`` is on no device."""
+    return _device() if isinstance(t, torch.Tensor) and t.is_cuda else -2
 
 
-def _have(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
-    """The address of a contiguous tensor of that type on the current device."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
-        _need(t, name, dtype)
-    if t.get_device() != _device():
-        _elsewhere(t, name)
+def _unlike(t: torch.Tensor, name: str, dtype: torch.dtype, contiguous: bool = True) -> None:
+    _need(t, name, dtype, contiguous)
+    raise KernelError(f"{name}: is on {t.device}; all tensors of a call are on the current device, to whose stream its launches go")
+
+
+def _have(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> int:
+    """The address of a contiguous tensor of that type on device ``dev``, the current one."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        _unlike(t, name, dtype)
     return t.data_ptr()
 
 
-def _have_rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, width: int) -> Tuple[int, int]:
-    """Address and row stride of a tensor [n, width] with contiguous rows on the current device."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
-        _need(t, name, dtype, contiguous=False)
-    if t.get_device() != _device():
-        _elsewhere(t, name)
+def _have_rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, width: int, dev: int) -> Tuple[int, int]:
+    """Address and row stride of a tensor [n, width] with contiguous rows on device ``dev``, the current one."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev:
+        _unlike(t, name, dtype, contiguous=False)
     if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
         raise KernelError(f"{name}: expected [{n}, {width}], got {tuple(t.shape)}")
     return t.data_ptr(), _rows_2d(t, name)
 
 
-def _have_pages(t: torch.Tensor, name: str, page_size: int, G: int, hd: int) -> int:
-    at = _have(t, name, torch.uint8)
+def _have_pages(t: torch.Tensor, name: str, page_size: int, G: int, hd: int, dev: int) -> int:
+    at = _have(t, name, torch.uint8, dev)
     if t.dim() != 3 or t.shape[1] != G or t.shape[2] != kv4_page_bytes(page_size, hd):
         raise KernelError(f"{name}: expected [n_pages, {G}, {kv4_page_bytes(page_size, hd)}], got {tuple(t.shape)}")
     return at
 
 
-def _have_mass(t: torch.Tensor, name: str, pages: torch.Tensor, page_size: int, G: int) -> int:
-    at = _have(t, name, torch.float32)
+def _have_mass(t: torch.Tensor, name: str, pages: torch.Tensor, page_size: int, G: int, dev: int) -> int:
+    at = _have(t, name, torch.float32, dev)
     if tuple(t.shape) != (pages.shape[0], G, page_size):
         raise KernelError(f"{name}: expected [{pages.shape[0]}, {G}, {page_size}], got {tuple(t.shape)}")
     return at
@@ -108,18 +110,20 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slot_map: t
     (int32: page * page_size + place; -1: nowhere).  A group is cut into 16 equal steps from its smallest value on, ``s =
     bfloat16((max - min) / 15)``, ``z = bfloat16(min)``, ``c = round((x - z) / s)`` (halves to even, within 0..15; 0 where s is
     0).  A group with a value that is not finite reads as NaN."""
-    slots = _have(slot_map, "slot_map", torch.int32)
-    at, n, code = _have_pages(pages, "pages", page_size, G, hd), slot_map.numel(), dtype_code(k.dtype)
-    pk, ldk = _have_rows(k, "k", k.dtype, n, G * hd)
-    pv, ldv = _have_rows(v, "v", k.dtype, n, G * hd)
+    dev = _here(pages)
+    slots = _have(slot_map, "slot_map", torch.int32, dev)
+    at, n, code = _have_pages(pages, "pages", page_size, G, hd, dev), slot_map.numel(), dtype_code(k.dtype)
+    pk, ldk = _have_rows(k, "k", k.dtype, n, G * hd, dev)
+    pv, ldv = _have_rows(v, "v", k.dtype, n, G * hd, dev)
     _run("kv4_write", _fn("kp_kv4_write"), pk, ldk, pv, ldv, at, pages.shape[0], slots, n, page_size, G, hd, code, STREAM)
 
 
 def kv4_read(pages: torch.Tensor, slot_map: torch.Tensor, page_size: int, G: int, hd: int,
              dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The keys and values in the slots, as rows [n, G hd] of ``dtype`` (a slot of -1 reads as zeros)."""
-    slots = _have(slot_map, "slot_map", torch.int32)
-    at, n, code = _have_pages(pages, "pages", page_size, G, hd), slot_map.numel(), dtype_code(dtype)
+    dev = _here(pages)
+    slots = _have(slot_map, "slot_map", torch.int32, dev)
+    at, n, code = _have_pages(pages, "pages", page_size, G, hd, dev), slot_map.numel(), dtype_code(dtype)
     k, v = torch.empty((2, n, G * hd), dtype=dtype, device=pages.device).unbind(0)
     _run("kv4_read", _fn("kp_kv4_read"), at, pages.shape[0], slots, k.data_ptr(), v.data_ptr(), n, page_size, G, hd, code, STREAM)
     return k, v
@@ -164,11 +168,12 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     weights; only the order in which these sums arrive is then not fixed."""
     if G < 1 or H % G:
         raise KernelError(f"kv4_attention: {H} query heads over {G} kv heads")
+    dev = _here(pages)
     n, n_seg, code = q.shape[0], seg_pos.numel(), dtype_code(q.dtype)
-    pq, ldq = _have_rows(q, "q", q.dtype, n, H * hd)
-    po, ldo = _have_rows(out, "out", q.dtype, n, H * hd)
-    at = _have_pages(pages, "pages", page_size, G, hd)
-    table, cu, pos = _have(block_table, "block_table", torch.int32), _have(cu_rows, "cu_rows", torch.int32), _have(seg_pos, "seg_pos", torch.int32)
+    pq, ldq = _have_rows(q, "q", q.dtype, n, H * hd, dev)
+    po, ldo = _have_rows(out, "out", q.dtype, n, H * hd, dev)
+    at = _have_pages(pages, "pages", page_size, G, hd, dev)
+    table, cu, pos = _have(block_table, "block_table", torch.int32, dev), _have(cu_rows, "cu_rows", torch.int32, dev), _have(seg_pos, "seg_pos", torch.int32, dev)
     if cu_rows.numel() != n_seg + 1 or block_table.dim() != 2 or block_table.shape[0] < n_seg:
         raise KernelError("kv4_attention: cu_rows has one entry more than seg_pos, block_table a row for each of them")
     if window is not None and window < 1:
@@ -176,7 +181,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     width = block_table.shape[1]
     if max_context < 1 or max_context > width * page_size:
         raise KernelError(f"kv4_attention: max_context={max_context} does not lie within the block table's {width} pages")
-    pm = None if mass is None else _have_mass(mass, "mass", pages, page_size, G)
+    pm = None if mass is None else _have_mass(mass, "mass", pages, page_size, G, dev)
     if not n or not n_seg:
         return out
     most = kv4_short_rows(H // G, pm is not None)
@@ -220,10 +225,11 @@ def kv4_evict(pages: torch.Tensor, mass: torch.Tensor, block_table: torch.Tensor
     ``recent`` last and of the others those with the most ``mass`` (equal: the lowest index); all, where there are not more.
     They move with their mass to places 0, 1, ... of ``new_table``'s pages, in their order.  The new pages are none of the
     sequences' old ones.  ``kept`` (int32 [n, G, keep]) gets the old indices, -1 behind the last."""
-    at, new_at = _have_pages(pages, "pages", page_size, G, hd), _have_pages(new_pages, "new_pages", page_size, G, hd)
-    pm, new_pm = _have_mass(mass, "mass", pages, page_size, G), _have_mass(new_mass, "new_mass", new_pages, page_size, G)
-    table, new_t = _have(block_table, "block_table", torch.int32), _have(new_table, "new_table", torch.int32)
-    keys, pk, n = _have(n_keys, "n_keys", torch.int32), _have(kept, "kept", torch.int32), n_keys.numel()
+    dev = _here(pages)
+    at, new_at = _have_pages(pages, "pages", page_size, G, hd, dev), _have_pages(new_pages, "new_pages", page_size, G, hd, dev)
+    pm, new_pm = _have_mass(mass, "mass", pages, page_size, G, dev), _have_mass(new_mass, "new_mass", new_pages, page_size, G, dev)
+    table, new_t = _have(block_table, "block_table", torch.int32, dev), _have(new_table, "new_table", torch.int32, dev)
+    keys, pk, n = _have(n_keys, "n_keys", torch.int32, dev), _have(kept, "kept", torch.int32, dev), n_keys.numel()
     if keep < 1 or min(recent, first) < 0 or first + recent > keep:
         raise KernelError(f"kv4_evict: keep={keep} is positive and not less than first={first} and recent={recent} together")
     if block_table.dim() != 2 or new_table.dim() != 2 or min(block_table.shape[0], new_table.shape[0]) < n or tuple(kept.shape) != (n, G, keep):
