@@ -28,6 +28,7 @@
 #include "mma.cuh"
 
 #define KV4_LOG2E 1.4426950408889634f
+#define KV4_LEAST_SCALE 8.271806125530277e-25f             // 2^-80
 
 template <int HD>
 struct Kv4 {
@@ -316,7 +317,7 @@ struct Kv4Acc {
     float l[NT][2];                                        // and of sum p
     float m[NT][2];                                        // largest score so far (base 2)
     float shift[NT][2];                                    // what p is taken against: p = 2^(score - shift)
-    float top_s;                                           // the values' largest scale so far
+    float top_s;                                           // the values' largest scale so far, or 2^-80 of the largest minimum
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -330,10 +331,11 @@ struct Kv4Acc {
                 for (int i = 0; i < 4; i++) o[nt][j][i] = 0.f;
         }
         // Scales below 2^-90 are taken for that: with p s at most 2^15 the sum of p then stays below 2^105 times the number
-        // of keys.  (Values of 2^-86 and less lose their last bits.)
+        // of keys.  (Values of 2^-86 and less lose their last bits.)  Where a minimum is so much larger than the scales that p z would leave
+        // float32 (a group of equal values has the scale 0), 2^-80 of it counts as a scale: p z stays below 2^95, its sum below 2^125.
         top_s = 8.077935669463161e-28f;
     }
-    // Before a tile's weights: `mx` are the thread's largest scores of it, `ts` its largest scale of a value.  The shift follows
+    // Before a tile's weights: `mx` are the thread's largest scores of it, `ts` its largest scale of a value (see top_s).  The shift follows
     // the maxima in steps: only a score above the last one's by 8, or a larger scale, moves it (and what has been added up).
     __device__ __forceinline__ void follow(float (&mx)[NT][2], float ts) {
         bool above = ts > top_s;
@@ -458,7 +460,7 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
     const int key = F::key_of(lane >> 2);
     float s[TB][NT][4];
     uint32_t ranges[TB][F::NG][2];
-    float mx[NT][2], ts = 0.f;
+    float mx[NT][2], ts = 0.f, tz = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
@@ -474,6 +476,7 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
                 if (!(kb >= k_lo && kb <= k_hi)) ranges[b][y][1] = 0u;
             }
             ts = kv4_max3(ts, kv4_scale(ranges[b][y][0]), kv4_scale(ranges[b][y][1]));
+            tz = kv4_max3(tz, fabsf(kv4_least(ranges[b][y][0])), fabsf(kv4_least(ranges[b][y][1])));
         }
         kv4_scores<HD, KEYS, PARTS, NT, CENTRE>(s[b], tile, at + b * 16, B, Q);
 #pragma unroll
@@ -488,6 +491,7 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
                 mx[nt][i] = kv4_max3(mx[nt][i], s[b][nt][i], s[b][nt][2 + i]);
             }
     }
+    ts = fmaxf(ts, tz * KV4_LEAST_SCALE);
     if (ts == INFINITY) {                                  // (a group that is not finite sets no scale)
         ts = 0.f;
 #pragma unroll
@@ -495,7 +499,10 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
 #pragma unroll
             for (int y = 0; y < F::NG; y++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) ts = fmaxf(ts, kv4_scale(ranges[b][y][i]) < INFINITY ? kv4_scale(ranges[b][y][i]) : 0.f);
+                for (int i = 0; i < 2; i++) {
+                    const float s = kv4_scale(ranges[b][y][i]), z = fabsf(kv4_least(ranges[b][y][i])), t = fmaxf(s, z * KV4_LEAST_SCALE);
+                    if (s < INFINITY && z < INFINITY) ts = fmaxf(ts, t);
+                }
     }
     A.follow(mx, ts);
     float sh[NT][2];

@@ -126,3 +126,38 @@ def test_weights_of_keys_that_sequences_share(dtype, hd, rows, n):
     want = sum(plain_attention(x.double().numpy().reshape(rows, H, hd), P.k[0], P.v[0], n - rows, hd ** -0.5, None, H)[1] for x in q.split(rows))
     np.testing.assert_allclose(P.mass_of(mass, 0), P.mass_of(m0, 0) + want, rtol=1e-5, atol=1e-6)
     assert not any(read_status().values())
+
+
+@pytest.mark.parametrize("dtype,hd,rows", FORMS)
+@pytest.mark.parametrize("value", [0.0, 1e6, 1e10, -1e30, 3e38])
+@pytest.mark.parametrize("n", [1, 20000])
+def test_values_that_are_all_the_same(dtype, hd, rows, value, n):
+    """Groups without a range: scale 0, all of the value in the minimum.  The output is that value: float32 sums of up to 20,000 weights, at most 2,500 of them added
+    one after another (a thread's share of a tile's keys), are off by 2500 x 2^-24 of themselves, the sum of weights above and below the line: 3e-4."""
+    rows = min(rows, n)
+    H, G = 4, 2
+    P = Paged([n], G, hd, 16, 3, dtype)
+    k = torch.randn((n, G * hd), generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    v = torch.full((n, G * hd), value, dtype=dtype, device=DEV)
+    kv4.kv4_write(k, v, P.pages, P.slots(0, n), 16, G, hd)
+    out = attend(P, queries(rows, H * hd, dtype).to(DEV), [rows], H).double().cpu().numpy()
+    want = float(torch.tensor(value).bfloat16())
+    np.testing.assert_allclose(out, want, rtol=3e-4 if dtype == torch.float32 else 2.0 ** -8 + 3e-4, atol=0)
+
+
+@pytest.mark.parametrize("dtype,hd,rows", FORMS)
+@pytest.mark.parametrize("scale", [1.0, 1e10, 1e-12])
+def test_values_without_a_range_before_others(dtype, hd, rows, scale):
+    """The first half of the keys have values without a range, the others have one.  (Bounds as for values of many sizes in test_kv4_gpu.py.)"""
+    H, G, n = 4, 2, 1400
+    P = Paged([n], G, hd, 16, 3, dtype, scale=scale)
+    v = torch.from_numpy((P.v[0] * 1.0).astype(np.float32)).to(dtype)
+    v[:n // 2] = (torch.arange(n // 2)[:, None, None] % 7 - 3.0) * scale
+    kv4.kv4_write(torch.from_numpy(P.k[0].astype(np.float32)).reshape(n, -1).to(dtype).to(DEV), v.reshape(n, -1).to(DEV), P.pages, P.slots(0, n), 16, G, hd)
+    kq, vq = (x.double().cpu().numpy().reshape(n, G, hd) for x in kv4.kv4_read(P.pages, P.slots(0, n), 16, G, hd, torch.float32))
+    q = queries(rows, H * hd, dtype)
+    s = hd ** -0.5 / scale
+    out = attend(P, q.to(DEV), [rows], H, scale=s).double().cpu().numpy().reshape(rows, H, hd)
+    want, _ = plain_attention(q.double().numpy().reshape(rows, H, hd), kq, vq, n - rows, s, None, H)
+    top = np.abs(vq).max()
+    assert (np.abs(out - want) <= (1e-3 if dtype == torch.float32 else 2.0 ** -7) * top).all()
