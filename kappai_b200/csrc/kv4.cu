@@ -20,6 +20,12 @@ __device__ __forceinline__ bf16 kv4_fifteenth(float x) {
     if (q < 1e-30f || ((__float_as_uint(q) & 0xffffu) - 0x7ffcu) < 8u) q = kv4_divide(x, 15.0f);
     return __float2bfloat16_rn(q);
 }
+// A group's scale, bfloat16((hi - lo) / 15).  Where hi - lo is above the largest float32 it is taken of a sixteenth of both, which rounds no differently.
+__device__ __forceinline__ bf16 kv4_group_scale(float lo, float hi) {
+    const float x = hi - lo;
+    if (x != INFINITY) return kv4_fifteenth(x);
+    return __float2bfloat16_rn(kv4_divide(hi * 0.0625f - lo * 0.0625f, 15.0f) * 16.0f);
+}
 // The codes round((x - z) / s) of eight values, halves to even, within 0 .. 15 (s > 0).  One Newton step on the quotient by the reciprocal (Markstein's
 // method): q + (d - q s) / s with the remainder exact.  Where d / s is at a half or rounds to it the step gives that half itself, and elsewhere a
 // unit of the last place changes no code.  Scales whose reciprocal is not to be had are divided by.  Adding 2^23 rounds to the even integer and
@@ -33,8 +39,9 @@ __device__ __forceinline__ uint32_t kv4_eight_codes(const float (&x)[8], float s
         q[i] = fmaf(fmaf(-t, s, d), inv, t);
     }
     if (!(s >= 1e-30f && s <= 1e30f)) {
+        const float f = s > 1.0f ? 0.0625f : 1.0f;         // (a difference of finite values may be above the largest float32)
 #pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = kv4_divide(x[i] - z, s);
+        for (int i = 0; i < 8; i++) q[i] = kv4_divide(x[i] * f - z * f, s * f);
     }
     uint32_t w = 0u;
 #pragma unroll
@@ -108,7 +115,7 @@ kv4_write_kernel(const T* __restrict__ k, long long ldk, const T* __restrict__ v
             hi = kv4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
         if (slot[u] < 0) continue;
-        const bf16 sb = kv4_fifteenth(hi - lo), zb = __float2bfloat16_rn(lo);
+        const bf16 sb = kv4_group_scale(lo, hi), zb = __float2bfloat16_rn(lo);
         const float s = __bfloat162float(sb), z = __bfloat162float(zb);
         const uint32_t w = s > 0.f ? kv4_eight_codes(x[u], s, z) : 0u;
         const unsigned page = slot[u] >> p.ps_log2, off = slot[u] & (ps - 1);

@@ -161,3 +161,27 @@ def test_values_without_a_range_before_others(dtype, hd, rows, scale):
     want, _ = plain_attention(q.double().numpy().reshape(rows, H, hd), kq, vq, n - rows, s, None, H)
     top = np.abs(vq).max()
     assert (np.abs(out - want) <= (1e-3 if dtype == torch.float32 else 2.0 ** -7) * top).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hd", [64, 96])
+def test_groups_whose_range_is_above_float32s(dtype, hd):
+    """Finite values whose difference is not finite in float32.  A power of two changes neither codes nor the rounding of scale and minimum, so what is
+    to be read are the values of the rows divided by 16, times 16."""
+    n, G, page = 12, 2, 16
+    rng = np.random.default_rng(2)
+    x = rng.uniform(-3.2e38, 3.2e38, (n, G * hd)).astype(np.float32)
+    x[0] = np.where(np.arange(G * hd) % 2, 3.2e38, -3.2e38)
+    x[1] = np.linspace(-3e38, 3e38, G * hd)
+    x[2, :hd] = rng.standard_normal(hd)                                       # (a head of ordinary values beside one that is not)
+    x[3] = np.where(np.arange(G * hd) % 5, 1e-30, np.where(np.arange(G * hd) % 2, 2e38, -2e38))
+    x = torch.from_numpy(x).to(dtype)
+    pages = torch.zeros((1, G, kv4.kv4_page_bytes(page, hd)), dtype=torch.uint8, device=DEV)
+    slots = torch.arange(n, dtype=torch.int32, device=DEV)
+    kv4.kv4_write(x.to(DEV), x.to(DEV), pages, slots, page, G, hd)
+    want = (plain_values((x.float().numpy() / np.float32(16.0)).reshape(n, G, hd), hd) * 16.0).reshape(n, G * hd)
+    assert np.isfinite(want).all() and np.abs(want).max() < 3.4e38
+    for have in kv4.kv4_read(pages, slots, page, G, hd, torch.float32):
+        have = have.cpu().numpy()
+        # (the division by 16 leaves of 1e-30 what it was; the read rounds s c + z once, to float32)
+        assert np.array_equal(have, want.astype(np.float32))
