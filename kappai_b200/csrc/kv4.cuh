@@ -12,8 +12,8 @@
 // so the codes themselves enter the matrix instructions and a scale is one multiplication a (key, group), not one a value.
 // A code is an fp16 operand without any arithmetic: the bits 0000 0000 0000 cccc are the subnormal c 2^-24, and
 // 0000 0000 cccc 0000 are c 2^-20, so eight codes of a word need four ANDs and one shift.  Queries enter as fp16 too,
-// scaled by a power of two that brings the largest value of the warp's queries to [2^14, 2^15): a bfloat16 query loses nothing
-// that is above 2^-38 of that value.  float32 queries enter as two fp16 parts (22 bits).  The softmax weights p are
+// each scaled by a power of two that brings its largest value to [2^14, 2^15): what fp16 does not hold of a bfloat16 query
+// is below 2^-35 of that value.  float32 queries enter as two fp16 parts (22 bits).  The softmax weights p are
 // multiplied with the values' scales and enter as fp16 (as two parts in the float32 form), with the running maximum in
 // units that hold p s at or below 2^15 (it follows the maxima in steps of 2^8 and more): at least 31 binary orders of fp16 lie
 // below the largest weight of a row.
@@ -143,8 +143,8 @@ __device__ __forceinline__ W kv4_at(const unsigned char* p) { return *reinterpre
 template <int HD, int PARTS, int NT>
 struct Kv4Q {
     uint32_t b[NT][PARTS][HD / 16][2];
-    float fs;                                              // factor of s (q.c), the same for all columns
-    float fz[NT][Kv4<HD>::NG][2];                          // factor of z for this thread's queries 2t and 2t + 1
+    float fs[NT][2];                                       // factor of s (q.c) for this thread's queries 2t and 2t + 1
+    float fz[NT][Kv4<HD>::NG][2];                          // factor of z for them
 };
 
 // Loads the warp's columns: src[nt] is the query of column 8 nt + lane / 4 (null: none).
@@ -182,27 +182,32 @@ __device__ __forceinline__ void kv4_load_q(Kv4Q<HD, PARTS, NT>& Q, const T* cons
     using F = Kv4<HD>;
     const int t = lane & 3;
     constexpr int W = F::GS / 4;                           // values of a group that a lane holds: 16 or 8 consecutive ones
-    // One power of two for all the columns brings their largest value to [2^14, 2^15): what fp16 cannot hold of a smaller column is
-    // below 2^-39 of that value.  A column that is not finite has no say.
-    float top = 0.f;
+    // A power of two of each column's own brings its largest value to [2^14, 2^15): its neighbours' size has no part in what fp16 holds of it.
+    // (A value that is not finite stays so.)
+    float up[NT], f[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        float mine = 0.f;
+        float top = 0.f;
         if (src[nt]) {
 #pragma unroll
             for (int y = 0; y < F::NG; y++) {
                 float v[W];
                 kv4_values<W>(v, src[nt] + y * F::GS + t * W);
 #pragma unroll
-                for (int i = 0; i < W; i++) mine = fmaxf(mine, fabsf(v[i]));
+                for (int i = 0; i < W; i++) top = fmaxf(top, fabsf(v[i]));
             }
         }
-        top = mine < INFINITY ? fmaxf(top, mine) : top;
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 100) : 0;
+        up[nt] = ldexpf(1.0f, e);
+        f[nt] = ldexpf(scale * KV4_LOG2E, -e);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float theirs = __shfl_sync(0xffffffffu, f[nt], (2 * t + i) * 4);                      // (from a lane whose column this is)
+            Q.fs[nt][i] = CENTRE ? theirs : theirs * 16777216.0f;
+        }
     }
-    top = warp_max(top);
-    const int e = top > 0.f ? min(14 - ilogbf(top), 100) : 0;
-    const float up = ldexpf(1.0f, e), f = ldexpf(scale * KV4_LOG2E, -e);
-    Q.fs = CENTRE ? f : f * 16777216.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -212,7 +217,7 @@ __device__ __forceinline__ void kv4_load_q(Kv4Q<HD, PARTS, NT>& Q, const T* cons
             for (int i = 0; i < W; i++) v[i] = 0.f;
             if (src[nt]) kv4_values<W>(v, src[nt] + y * F::GS + t * W);
 #pragma unroll
-            for (int i = 0; i < W; i++) v[i] *= up;
+            for (int i = 0; i < W; i++) v[i] *= up[nt];
 #pragma unroll
             for (int k = 0; k < F::KS; k++) {              // step k: values (0, 4), (1, 5) of a word, then (2, 6), (3, 7), then the next word
                 const int d = (k >> 1) * 8 + (k & 1) * 2;
@@ -229,7 +234,7 @@ __device__ __forceinline__ void kv4_load_q(Kv4Q<HD, PARTS, NT>& Q, const T* cons
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                Q.fz[nt][y][i] = f * __shfl_sync(0xffffffffu, sum, (2 * t + i) * 4);                // (from a lane whose column this is)
+                Q.fz[nt][y][i] = __shfl_sync(0xffffffffu, f[nt] * sum, (2 * t + i) * 4);
             }
         }
 }
@@ -285,7 +290,6 @@ __device__ __forceinline__ void kv4_scores(float (&s)[NT][4], const unsigned cha
         const uint32_t r0 = kv4_at<uint32_t>(r), r1 = kv4_at<uint32_t>(r + 32 * F::NG);
         float z0 = kv4_least(r0), s0 = kv4_scale(r0), z1 = kv4_least(r1), s1 = kv4_scale(r1);
         if (CENTRE) { z0 = fmaf(8.0f, s0, z0); z1 = fmaf(8.0f, s1, z1); }
-        s0 *= Q.fs; s1 *= Q.fs;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -294,16 +298,11 @@ __device__ __forceinline__ void kv4_scores(float (&s)[NT][4], const unsigned cha
 #pragma unroll
                 for (int k = 0; k < F::KS; k++)
                     mma_f16(acc, a[k][0], a[k][1], a[k][2], a[k][3], Q.b[nt][p][y * F::KS + k][0], Q.b[nt][p][y * F::KS + k][1]);
-            if (y == 0) {
-                s[nt][0] = fmaf(acc[0], s0, z0 * Q.fz[nt][y][0]);
-                s[nt][1] = fmaf(acc[1], s0, z0 * Q.fz[nt][y][1]);
-                s[nt][2] = fmaf(acc[2], s1, z1 * Q.fz[nt][y][0]);
-                s[nt][3] = fmaf(acc[3], s1, z1 * Q.fz[nt][y][1]);
-            } else {
-                s[nt][0] = fmaf(acc[0], s0, fmaf(z0, Q.fz[nt][y][0], s[nt][0]));
-                s[nt][1] = fmaf(acc[1], s0, fmaf(z0, Q.fz[nt][y][1], s[nt][1]));
-                s[nt][2] = fmaf(acc[2], s1, fmaf(z1, Q.fz[nt][y][0], s[nt][2]));
-                s[nt][3] = fmaf(acc[3], s1, fmaf(z1, Q.fz[nt][y][1], s[nt][3]));
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float fs = Q.fs[nt][i], fz = Q.fz[nt][y][i];
+                s[nt][i] = fmaf(acc[i], s0 * fs, y == 0 ? z0 * fz : fmaf(z0, fz, s[nt][i]));
+                s[nt][2 + i] = fmaf(acc[2 + i], s1 * fs, y == 0 ? z1 * fz : fmaf(z1, fz, s[nt][2 + i]));
             }
         }
     }

@@ -185,3 +185,20 @@ def test_groups_whose_range_is_above_float32s(dtype, hd):
         have = have.cpu().numpy()
         # (the division by 16 leaves of 1e-30 what it was; the read rounds s c + z once, to float32)
         assert np.array_equal(have, want.astype(np.float32))
+
+
+@pytest.mark.parametrize("dtype,hd,rows", FORMS + [(torch.bfloat16, 256, 1), (torch.float32, 256, 30), (torch.bfloat16, 32, 30)])
+@pytest.mark.parametrize("factor", [2.0 ** 30, 2.0 ** 45, 2.0 ** -45])
+def test_a_query_does_not_change_its_neighbours(dtype, hd, rows, factor):
+    """Queries of one head, and of one row, that are much larger or smaller than the others beside which they are computed."""
+    H, G, n = 4, 2, 700
+    P = Paged([n], G, hd, 16, 3, dtype)
+    q = queries(rows, H * hd, dtype).view(rows, H, hd)
+    other = torch.zeros((rows, H), dtype=torch.bool)
+    other[:, 1] = other[rows // 2] = True
+    other[:, 3] = False
+    x = torch.where(other[..., None], q * factor, q).to(dtype)
+    out = attend(P, x.reshape(rows, -1).to(DEV), [rows], H).double().cpu().numpy().reshape(rows, H, hd)
+    want, _ = plain_attention(x.double().numpy(), P.k[0], P.v[0], n - rows, hd ** -0.5, None, H)
+    ordinary = ~other.numpy() if factor > 1 else np.ones((rows, H), dtype=bool)      # (scores of 1e10 themselves are off by thousands)
+    near(out[ordinary], want[ordinary], np.abs(P.v[0]).max(), dtype)
