@@ -783,7 +783,7 @@ kv4_mass_kernel(const Kv4Args p) {
     const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
     if (n_rows < p.min_rows || k0 > last || k0 + KEYS - 1 < first) return;
     // rows that read any of the keys
-    const int r_lo = max(0, k0 - pos0), r_hi = p.window > 0 ? min(n_rows - 1, k0 + KEYS - 1 + p.window - 1 - pos0) : n_rows - 1;
+    const int r_lo = max(0, k0 - pos0), r_hi = p.window > 0 ? min(n_rows - 1, k0 - pos0 + KEYS - 2 + p.window) : n_rows - 1;
     if (r_hi < r_lo) return;
     const int* bt = p.block_table + (size_t)seg * p.max_blocks;
     for (int b = warp; b < NB; b += 4) {

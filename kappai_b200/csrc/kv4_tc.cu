@@ -680,7 +680,7 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
     // keys that any row reads, and columns that read any of this CTA's, in tiles of 128 from column 0; this CTA has every n_ctas-th tile
     const int last = min(pos0 + n_rows - 1, p.max_blocks * p.ps - 1), first = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
     const int c_lo = max(0, k0 - pos0) * R;
-    const int c_hi = (p.window > 0 ? min(n_rows - 1, k0 + KT_ROWS - 1 + p.window - 1 - pos0) : n_rows - 1) * R + R - 1;
+    const int c_hi = (p.window > 0 ? min(n_rows - 1, k0 - pos0 + KT_ROWS - 2 + p.window) : n_rows - 1) * R + R - 1;
     if (n_rows < p.min_rows || k0 > last || k0 + KT_ROWS - 1 < first || c_hi < c_lo) return;       // (all of a cluster or none)
     const int j_lo = c_lo / 128 + rank, n_j = max(0, (c_hi / 128 - j_lo + n_ctas) / n_ctas);
     if (threadIdx.x == 0) {
@@ -749,7 +749,7 @@ kv4_tc_mass_kernel(const Kv4TcArgs p) {
         const uint32_t tmem_s = tmem_base + g * 128 + ((uint32_t)(q4 * 32) << 16);
         // columns that read this key
         const int mine_lo = max(0, key - pos0) * R;
-        const int mine_hi = !there ? -1 : (p.window > 0 ? min(n_cols, (key + p.window - pos0) * R) : n_cols) - 1;
+        const int mine_hi = !there ? -1 : (p.window > 0 ? min(n_rows, key - pos0 + p.window) * R : n_cols) - 1;
         bool ok = n_j == 0 || kp_mbar_wait_bounded(k_full, 0);
         const float kappa = kt_pow2(max(max(tops[0], tops[1]), max(tops[2], tops[3])) - 7);
 #pragma unroll 1

@@ -22,6 +22,7 @@ KV4_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 # 67, 88 against 122.  With mass, whose scores it keeps in memory: 32 columns, 8 x 4000 keys 66 against 106, 1 x 500 29 against 20; 64 columns
 # 136 against 106.
 KV4_SHORT_COLS, KV4_SHORT_COLS_MASS, KV4_SHORT_ROWS_MASS = 64, 32, 16
+KV4_MAX_KEYS = 1 << 30     # that a block table has room for: the kernels count keys, and add windows and tiles to them, in 32 bits
 USE_TC_KV4 = True          # longer ones of bfloat16 rows with heads of 64 or 128 run on the tcgen05 tensor cores
 _CTAS = 148 * 4            # CTAs of the split form that an even spread over the SMs wants
 
@@ -162,7 +163,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
 
     Rows ``cu_rows[i] .. cu_rows[i + 1] - 1`` belong to sequence ``i``; the first of them stands at key ``seg_pos[i]`` and reads
     the keys up to that one, of which ``window`` (None: all) the last; a row that reads none gives zeros.  ``max_rows`` and
-    ``min_rows`` bound the rows of a sequence, ``max_context`` the keys that any row reads (host integers).  ``mass`` (float32
+    ``min_rows`` bound the rows of a sequence, ``max_context`` the last key that any row reads, counted from 1 (host integers).  ``mass`` (float32
     [n_pages, G, page_size]): the softmax weight of every key, summed over the rows and the query heads of its kv head, is added
     to the key's entry, in a fixed order: the same call gives the same bits.  Sequences whose tables name the same pages each add their
     weights; only the order in which these sums arrive is then not fixed."""
@@ -179,8 +180,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     if window is not None and window < 1:
         raise KernelError("kv4_attention: the window is a positive number of keys")
     width = block_table.shape[1]
-    if max_context < 1 or max_context > width * page_size:
-        raise KernelError(f"kv4_attention: max_context={max_context} does not lie within the block table's {width} pages")
+    if max_context < 1 or max_context > width * page_size or width * page_size > KV4_MAX_KEYS:
+        raise KernelError(f"kv4_attention: max_context={max_context} does not lie within the block table's {width} pages, or these have more than {KV4_MAX_KEYS} keys")
     pm = None if mass is None else _have_mass(mass, "mass", pages, page_size, G, dev)
     if not n or not n_seg:
         return out
@@ -188,7 +189,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     short = min(max_rows, most) if min_rows <= most else 0
     tiled = max_rows > most
     tc = tiled and kv4_tc_ok(q, out, hd, scale)
-    window = window or 0
+    window = 0 if window is None or window >= max_context else window
     if short or (tiled and not tc):
         n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd, min_rows if short and tiled else None)
         # one allocation for what the launches hand one another: results of chunks, their (shift, sum), scores, logarithms of sums.  It has a
@@ -236,6 +237,8 @@ def kv4_evict(pages: torch.Tensor, mass: torch.Tensor, block_table: torch.Tensor
         raise KernelError("kv4_evict: block tables with a row a sequence and kept of [sequences, kv heads, keep]")
     if max_keys < 1 or max_keys > block_table.shape[1] * page_size or min(keep, max_keys) > new_table.shape[1] * page_size:
         raise KernelError("kv4_evict: the block tables hold max_keys keys, and the ones that stay")
+    if max(block_table.shape[1], new_table.shape[1]) * page_size > KV4_MAX_KEYS:
+        raise KernelError(f"kv4_evict: block tables of at most {KV4_MAX_KEYS} keys")
     _run("kv4_evict", _fn("kp_kv4_evict"), at, pm, table, block_table.shape[1], keys, new_at, new_pm, new_t, new_table.shape[1], pk, n, max_keys, keep,
          recent, first, page_size, G, hd, STREAM)
     return kept

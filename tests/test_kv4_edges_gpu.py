@@ -202,3 +202,28 @@ def test_a_query_does_not_change_its_neighbours(dtype, hd, rows, factor):
     want, _ = plain_attention(x.double().numpy(), P.k[0], P.v[0], n - rows, hd ** -0.5, None, H)
     ordinary = ~other.numpy() if factor > 1 else np.ones((rows, H), dtype=bool)      # (scores of 1e10 themselves are off by thousands)
     near(out[ordinary], want[ordinary], np.abs(P.v[0]).max(), dtype)
+
+
+@pytest.mark.parametrize("dtype,hd,rows", FORMS)
+@pytest.mark.parametrize("window", [701, 2 ** 29, 2 ** 31 - 1, 2 ** 31 + 5, 2 ** 40])
+def test_a_window_that_no_row_exceeds_is_none(dtype, hd, rows, window):
+    H, G, n = 4, 2, 700
+    P = Paged([n], G, hd, 16, 3, dtype)
+    q = queries(rows, H * hd, dtype).to(DEV)
+    m0, m1 = P.mass(), P.mass()
+    a = attend(P, q, [rows], H, mass=m0)
+    b = attend(P, q, [rows], H, mass=m1, window=window)
+    assert torch.equal(a, b) and torch.equal(m0, m1) and abs(float(m1.sum()) - rows * H) < 1e-3 * rows * H
+
+
+def test_block_tables_of_more_keys_than_indices_hold():
+    """Keys are counted in 32 bits, with room for what is added to them."""
+    page, hd = 32768, 32
+    pages = torch.zeros((2, 1, kv4.kv4_page_bytes(page, hd)), dtype=torch.uint8, device=DEV)
+    wide, mass = torch.zeros((1, 32769), dtype=torch.int32, device=DEV), torch.zeros((2, 1, page), device=DEV)
+    q = torch.zeros((1, hd), device=DEV)
+    with pytest.raises(KernelError, match="keys"):
+        kv4.kv4_attention(q, pages, wide, i32([0, 1]), i32([5]), torch.empty_like(q), 0.1, None, page, 1, 1, hd, 1, 6)
+    with pytest.raises(KernelError, match="keys"):
+        kv4.kv4_evict(pages, mass, wide, i32([40]), pages, mass, i32([[1]]), torch.empty((1, 1, 8), dtype=torch.int32, device=DEV), 40, 8, 2, 1, page, 1, hd)
+    kv4.kv4_attention(q, pages, wide[:, :32768].contiguous(), i32([0, 1]), i32([5]), torch.empty_like(q), 0.1, None, page, 1, 1, hd, 1, 6)
