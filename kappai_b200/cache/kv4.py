@@ -44,6 +44,8 @@ class Kv4Cache:
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         record = kv4_page_bytes(self.page_size, self.hd)
+        if n_pages * self.page_size >= 1 << 31:
+            raise CacheError(f"{n_pages} pages of {self.page_size} keys: slots are 32-bit numbers, below 2^31")
         self.pool = PagePool(n_pages, self.page_size)
         self.pages = torch.zeros((n_pages, self.G, record), dtype=torch.uint8, device=self.device)
         self.mass: Optional[torch.Tensor] = None

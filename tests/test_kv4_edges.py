@@ -22,3 +22,10 @@ def test_attend_takes_as_many_queries_as_rows(shape):
     """Fewer would be read, and their outputs written, behind the tensors' ends; more would leave rows of the output as they were."""
     with pytest.raises(CacheError, match="rows of queries"):
         held(20).attend(torch.zeros(shape), ["a"], [4], 4, 0.125)
+
+
+def test_slots_are_32_bit_numbers():
+    """A slot above 2^31 would turn negative, which is the name of no slot: what is written there would be lost."""
+    with pytest.raises(CacheError, match="2\\^31"):
+        Kv4Cache(1, 32, n_pages=2 ** 11, page_size=2 ** 20, device="meta")
+    Kv4Cache(1, 32, n_pages=2 ** 11 - 1, page_size=2 ** 20, device="meta")
