@@ -118,16 +118,20 @@ class Kv4Cache:
             raise OutOfPages(f"need {need} pages, {self.pool.n_free} free")
         if k.shape[0] != sum(rows):
             raise CacheError(f"append: {k.shape[0]} rows of keys, {sum(rows)} were announced")
-        fresh = []
-        for s, n in zip(seqs, rows):
-            held = len(self.pool.table(s))
-            self.pool.extend(s, self._length[s] + n)
-            fresh += self.pool.table(s)[held:]
-        slots = np.concatenate([self._slots(s, self._length[s], self._length[s] + n) for s, n in zip(seqs, rows)])
-        slots_d, fresh_d = self._upload([slots, np.asarray(fresh, dtype=np.int32)])
-        if self.mass is not None and fresh:
-            self.mass.index_fill_(0, fresh_d.long(), 0.0)                        # (a page may have been another sequence's)
-        kv4_write(k, v, self.pages, slots_d, self.page_size, self.G, self.hd)
+        held = [len(self.pool.table(s)) for s in seqs]
+        try:
+            for s, n in zip(seqs, rows):
+                self.pool.extend(s, self._length[s] + n)
+            fresh = [page for s, h in zip(seqs, held) for page in self.pool.table(s)[h:]]
+            slots = np.concatenate([self._slots(s, self._length[s], self._length[s] + n) for s, n in zip(seqs, rows)])
+            slots_d, fresh_d = self._upload([slots, np.asarray(fresh, dtype=np.int32)])
+            if self.mass is not None and fresh:
+                self.mass.index_fill_(0, fresh_d.long(), 0.0)                    # (a page may have been another sequence's)
+            kv4_write(k, v, self.pages, slots_d, self.page_size, self.G, self.hd)
+        except BaseException:
+            for s, h in reversed(list(zip(seqs, held))):
+                self.pool.cut(s, h)
+            raise
         for s, n in zip(seqs, rows):
             self._length[s] += n
 

@@ -129,6 +129,18 @@ class PagePool:
         self._held[req] += need
         self._version[req] = self._stamp()
 
+    def cut(self, req: Hashable, n_pages: int) -> None:
+        """Give the pages behind the table's first ``n_pages`` back, the last one first."""
+        t = self._tables[req]
+        if len(t) <= n_pages:
+            return
+        while len(t) > n_pages:
+            page = t.pop()
+            if page != RELEASED:
+                self._free.append(page)
+                self._held[req] -= 1
+        self._version[req] = self._stamp()
+
     def release_behind(self, req: Hashable, next_pos: int) -> int:
         """Groups with a window or with blocks of positions: give back pages
         whose every key lies before the window of position ``next_pos`` (the

@@ -29,3 +29,30 @@ def test_slots_are_32_bit_numbers():
     with pytest.raises(CacheError, match="2\\^31"):
         Kv4Cache(1, 32, n_pages=2 ** 11, page_size=2 ** 20, device="meta")
     Kv4Cache(1, 32, n_pages=2 ** 11 - 1, page_size=2 ** 20, device="meta")
+
+
+@pytest.mark.parametrize("k,v", [(torch.zeros(20, 128), torch.zeros(20, 128)), (torch.zeros(20, 128), torch.zeros(19, 128)), (torch.zeros(20, 64), torch.zeros(20, 64))])
+def test_an_append_that_fails_takes_no_pages(k, v):
+    c = held(10)
+    free, table = c.pool.n_free, list(c.pool.table("a"))
+    with pytest.raises(KernelError):
+        c.append(k, v, ["a"], [20])
+    assert c.length("a") == 10 and c.pool.n_free == free and c.pool.table("a") == table
+    c.pool.check()
+
+
+def test_a_page_pool_takes_pages_back():
+    from kappai_b200.cache import PagePool
+
+    pool = PagePool(6, 16)
+    pool.open("a")
+    pool.extend("a", 50)
+    stamp, table = pool.version("a"), list(pool.table("a"))
+    pool.cut("a", 4)
+    assert pool.table("a") == table and pool.version("a") == stamp
+    pool.cut("a", 1)
+    pool.check()
+    assert pool.table("a") == table[:1] and pool.n_free == 5 and pool.version("a") != stamp
+    pool.extend("a", 50)
+    assert pool.table("a") == table                 # (in the order in which they were handed out)
+    pool.check()
