@@ -118,6 +118,8 @@ class Kv4Cache:
             raise OutOfPages(f"need {need} pages, {self.pool.n_free} free")
         if k.shape[0] != sum(rows):
             raise CacheError(f"append: {k.shape[0]} rows of keys, {sum(rows)} were announced")
+        if not seqs:
+            return
         held = [len(self.pool.table(s)) for s in seqs]
         try:
             for s, n in zip(seqs, rows):

@@ -56,3 +56,12 @@ def test_a_page_pool_takes_pages_back():
     pool.extend("a", 50)
     assert pool.table("a") == table                 # (in the order in which they were handed out)
     pool.check()
+
+
+def test_calls_for_no_sequence():
+    c, none = held(10, mass=True), torch.zeros(0, 128)
+    c.append(none, none, [], [])
+    assert c.attend(torch.zeros(0, 256), [], [], 4, 0.125).shape == (0, 256) and c.evict([], 4).shape == (0, 2, 4)
+    with pytest.raises(CacheError):
+        c.append(torch.zeros(1, 128), torch.zeros(1, 128), [], [])
+    assert c.length("a") == 10
