@@ -167,8 +167,10 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     [n_pages, G, page_size]): the softmax weight of every key, summed over the rows and the query heads of its kv head, is added
     to the key's entry, in a fixed order: the same call gives the same bits.  Sequences whose tables name the same pages each add their
     weights; only the order in which these sums arrive is then not fixed."""
-    if G < 1 or H % G:
+    if G < 1 or H < 1 or H % G:
         raise KernelError(f"kv4_attention: {H} query heads over {G} kv heads")
+    if max_rows < max(1, min_rows):
+        raise KernelError(f"kv4_attention: a sequence has between min_rows={min_rows} and max_rows={max_rows} rows")
     dev = _here(pages)
     n, n_seg, code = q.shape[0], seg_pos.numel(), dtype_code(q.dtype)
     pq, ldq = _have_rows(q, "q", q.dtype, n, H * hd, dev)

@@ -227,3 +227,14 @@ def test_block_tables_of_more_keys_than_indices_hold():
     with pytest.raises(KernelError, match="keys"):
         kv4.kv4_evict(pages, mass, wide, i32([40]), pages, mass, i32([[1]]), torch.empty((1, 1, 8), dtype=torch.int32, device=DEV), 40, 8, 2, 1, page, 1, hd)
     kv4.kv4_attention(q, pages, wide[:, :32768].contiguous(), i32([0, 1]), i32([5]), torch.empty_like(q), 0.1, None, page, 1, 1, hd, 1, 6)
+
+
+def test_numbers_of_rows_and_heads_that_make_no_sense_are_refused():
+    """None of these is launched: without rows or heads nothing would be written, or a division by zero raised."""
+    P = Paged([40], 2, 64, 16, 0)
+    q = torch.zeros((1, 256), device=DEV)
+    ok = dict(q=q, pages=P.pages, block_table=P.table_d, cu_rows=i32([0, 1]), seg_pos=i32([39]), out=torch.zeros_like(q), scale=0.1, window=None, page_size=16, H=4,
+              G=2, hd=64, max_rows=1, max_context=40)
+    for bad in (dict(max_rows=0), dict(max_rows=-3), dict(min_rows=2), dict(H=0, q=q[:, :0], out=q[:, :0]), dict(H=-2)):
+        with pytest.raises(KernelError):
+            kv4.kv4_attention(**{**ok, **bad})
