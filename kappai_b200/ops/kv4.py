@@ -23,6 +23,9 @@ KV4_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 # 136 against 106.
 KV4_SHORT_COLS, KV4_SHORT_COLS_MASS, KV4_SHORT_ROWS_MASS = 64, 32, 16
 KV4_MAX_KEYS = 1 << 30     # that a block table has room for: the kernels count keys, and add windows and tiles to them, in 32 bits
+# Bytes of scratch up to which the split form takes all the rows that it could.  It is indexed by the most rows that a segment may have, so that beside a
+# prompt 31 decoded rows behind 131,072 keys with mass would ask for 4.3 GB; above the limit segments of several rows go to the other forms.
+KV4_SCRATCH = 1 << 30
 USE_TC_KV4 = True          # longer ones of bfloat16 rows with heads of 64 or 128 run on the tcgen05 tensor cores
 _CTAS = 148 * 4            # CTAs of the split form that an even spread over the SMs wants
 
@@ -87,21 +90,22 @@ def _have_rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, width: in
     """Address and row stride of a tensor [n, width] with contiguous rows on device ``dev``, the current one."""
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev:
         _unlike(t, name, dtype, contiguous=False)
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
+    if t.shape != (n, width):
         raise KernelError(f"{name}: expected [{n}, {width}], got {tuple(t.shape)}")
     return t.data_ptr(), _rows_2d(t, name)
 
 
 def _have_pages(t: torch.Tensor, name: str, page_size: int, G: int, hd: int, dev: int) -> int:
     at = _have(t, name, torch.uint8, dev)
-    if t.dim() != 3 or t.shape[1] != G or t.shape[2] != kv4_page_bytes(page_size, hd):
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != G or shape[2] != kv4_page_bytes(page_size, hd):
         raise KernelError(f"{name}: expected [n_pages, {G}, {kv4_page_bytes(page_size, hd)}], got {tuple(t.shape)}")
     return at
 
 
 def _have_mass(t: torch.Tensor, name: str, pages: torch.Tensor, page_size: int, G: int, dev: int) -> int:
     at = _have(t, name, torch.float32, dev)
-    if tuple(t.shape) != (pages.shape[0], G, page_size):
+    if t.shape != (pages.shape[0], G, page_size):
         raise KernelError(f"{name}: expected [{pages.shape[0]}, {G}, {page_size}], got {tuple(t.shape)}")
     return at
 
@@ -169,7 +173,7 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     weights; only the order in which these sums arrive is then not fixed."""
     if G < 1 or H < 1 or H % G:
         raise KernelError(f"kv4_attention: {H} query heads over {G} kv heads")
-    if max_rows < max(1, min_rows):
+    if max_rows < 1 or max_rows < min_rows:
         raise KernelError(f"kv4_attention: a sequence has between min_rows={min_rows} and max_rows={max_rows} rows")
     dev = _here(pages)
     n, n_seg, code = q.shape[0], seg_pos.numel(), dtype_code(q.dtype)
@@ -177,26 +181,37 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     po, ldo = _have_rows(out, "out", q.dtype, n, H * hd, dev)
     at = _have_pages(pages, "pages", page_size, G, hd, dev)
     table, cu, pos = _have(block_table, "block_table", torch.int32, dev), _have(cu_rows, "cu_rows", torch.int32, dev), _have(seg_pos, "seg_pos", torch.int32, dev)
-    if cu_rows.numel() != n_seg + 1 or block_table.dim() != 2 or block_table.shape[0] < n_seg:
+    shape = block_table.shape
+    if cu_rows.numel() != n_seg + 1 or len(shape) != 2 or shape[0] < n_seg:
         raise KernelError("kv4_attention: cu_rows has one entry more than seg_pos, block_table a row for each of them")
     if window is not None and window < 1:
         raise KernelError("kv4_attention: the window is a positive number of keys")
-    width = block_table.shape[1]
+    width = shape[1]
     if max_context < 1 or max_context > width * page_size or width * page_size > KV4_MAX_KEYS:
         raise KernelError(f"kv4_attention: max_context={max_context} does not lie within the block table's {width} pages, or these have more than {KV4_MAX_KEYS} keys")
     pm = None if mass is None else _have_mass(mass, "mass", pages, page_size, G, dev)
     if not n or not n_seg:
         return out
-    most = kv4_short_rows(H // G, pm is not None)
+    R = H // G
+    most = kv4_short_rows(R, pm is not None)
     short = min(max_rows, most) if min_rows <= most else 0
     tiled = max_rows > most
+    if window is None or window >= max_context:
+        window = 0
+    if short:
+        n_chunks, chunk = kv4_chunks(n_seg, short, max_context, window, H, G, hd, min_rows if tiled else None)
+        if short > 1 and short > min_rows:
+            row_bytes = 4 * n_seg * H * n_chunks * ((hd + 2 if n_chunks > 1 else 0) + (chunk if pm else 0))
+            if short * row_bytes > KV4_SCRATCH:
+                short, tiled = max(min_rows, 1, KV4_SCRATCH // row_bytes), True
+                n_chunks, chunk = kv4_chunks(n_seg, short, max_context, window, H, G, hd, min_rows)
+    else:
+        n_chunks, chunk = kv4_chunks(1, 1, 1, 0, 1, 1, hd)     # (nothing is cut)
     tc = tiled and kv4_tc_ok(q, out, hd, scale)
-    window = 0 if window is None or window >= max_context else window
     if short or (tiled and not tc):
-        n_chunks, chunk = kv4_chunks(n_seg, max(short, 1), max_context, window, H, G, hd, min_rows if short and tiled else None)
         # one allocation for what the launches hand one another: results of chunks, their (shift, sum), scores, logarithms of sums.  It has a
         # name until this function returns: another thread would be given memory that is free before the launch that uses it is queued.
-        fused = n_chunks <= 8 and (pm is None or short * (H // G) <= 8)
+        fused = n_chunks <= 8 and (pm is None or short * R <= 8)
         places, many = n_seg * short * H, n_chunks > 1 and not fused
         sizes = (places * n_chunks * hd if many else 0, places * n_chunks * 2 if many else 0,
                  places * n_chunks * chunk if pm else 0, places if pm and not fused else 0, n * H if pm and tiled and not tc else 0)

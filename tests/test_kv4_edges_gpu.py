@@ -238,3 +238,45 @@ def test_numbers_of_rows_and_heads_that_make_no_sense_are_refused():
     for bad in (dict(max_rows=0), dict(max_rows=-3), dict(min_rows=2), dict(H=0, q=q[:, :0], out=q[:, :0]), dict(H=-2)):
         with pytest.raises(KernelError):
             kv4.kv4_attention(**{**ok, **bad})
+
+
+def test_a_prompt_beside_decoded_rows_asks_for_no_more_scratch_than_it_needs(monkeypatch):
+    """31 sequences decode behind up to 131,072 keys while another's prompt runs: scores for a row a sequence are half a gigabyte, for the eight rows that
+    the split form could take of each they would be four.  (Nothing is launched.)"""
+    H, G, hd, page, n = 32, 8, 64, 128, 131072
+    pages = torch.zeros((2, G, kv4.kv4_page_bytes(page, hd)), dtype=torch.uint8, device=DEV)
+    mass = torch.zeros((2, G, page), device=DEV)
+    table = torch.zeros((32, n // page), dtype=torch.int32, device=DEV)
+    rows = [1] * 31 + [200]
+    q = torch.zeros((sum(rows), H * hd), dtype=torch.bfloat16, device=DEV)
+    calls = []
+    monkeypatch.setattr(kv4, "_run", lambda what, *a, **kw: calls.append(what))
+    out = torch.empty_like(q)
+    cu, pos = i32(np.concatenate([[0], np.cumsum(rows)]).tolist()), i32([n - r for r in rows])
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    kv4.kv4_attention(q, pages, table, cu, pos, out, 0.125, None, page, H, G, hd, max(rows), n, min_rows=1, mass=mass)
+    assert calls == ["kv4_attention", "kv4_attention_tc"]
+    assert torch.cuda.max_memory_allocated() - before <= 1.2 * 2 ** 30
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 96), (torch.float32, 64)])
+@pytest.mark.parametrize("with_mass", [False, True])
+@pytest.mark.parametrize("limit", [0, 300000, 2 ** 30])
+def test_a_mixed_call_with_little_scratch(dtype, hd, with_mass, limit, monkeypatch):
+    """The fewer rows the split form may take, the more go to the others: the results are the same."""
+    monkeypatch.setattr(kv4, "KV4_SCRATCH", limit, raising=False)
+    H, G, lengths, rows = 8, 2, [900, 400, 33, 150, 8, 300], [1, 2, 3, 150, 8, 5]
+    P = Paged(lengths, G, hd, 16, 3, dtype)
+    q, mass = queries(sum(rows), H * hd, dtype), P.mass(5) if with_mass else None
+    m0 = mass.clone() if with_mass else None
+    out = attend(P, q.to(DEV), rows, H, mass=mass).double().cpu().numpy()
+    at = 0
+    for i, r in enumerate(rows):
+        want, got = plain_attention(q[at:at + r].double().numpy().reshape(r, H, hd), P.k[i], P.v[i], lengths[i] - r, hd ** -0.5, None, H)
+        near(out[at:at + r].reshape(r, H, hd), want, np.abs(P.v[i]).max(), dtype)
+        if with_mass:
+            np.testing.assert_allclose(P.mass_of(mass, i), P.mass_of(m0, i) + got, rtol=1e-5, atol=1e-6)
+        at += r
+    assert not any(read_status().values())
