@@ -83,6 +83,7 @@ __device__ __forceinline__ uint32_t pack_f16_part(float& a, float& b) {
 // a range's two halves
 __device__ __forceinline__ float kv4_scale(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float kv4_least(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
+__device__ __forceinline__ bool kv4_finite(uint32_t r) { return (r & 0x7f80u) != 0x7f80u && (r & 0x7f800000u) != 0x7f800000u; }
 
 // ---- a block of 16 keys from its page's record to shared memory by a warp's cp.async: row `at` of a tile of KEYS keys (`rec`:
 // record of (page, kv head), `off`: the block's first key in the page)
@@ -519,6 +520,22 @@ __device__ __forceinline__ void kv4_tile(Kv4Acc<HD, PARTS, NT>& A, const Kv4Q<HD
                 s[b][nt][2 + i] = kv4_exp2(s[b][nt][2 + i] - sh[nt][i]);
                 A.l[nt][i] += s[b][nt][i] + s[b][nt][2 + i];
             }
+        if (MASKED) {                                      // a value that is not finite has no part in a column that does not read its key
+            const int k[2] = {key0 + b * 16 + key, key0 + b * 16 + key + 8};
+#pragma unroll
+            for (int y = 0; y < F::NG; y++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    if (kv4_finite(ranges[b][y][h])) continue;
+                    const float bad = kv4_scale(ranges[b][y][h]) * 0.f + kv4_least(ranges[b][y][h]);
+                    ranges[b][y][h] = 0u;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+                            if (k[h] >= lo[nt][i] && k[h] <= hi[nt][i]) A.z[nt][y][i] += bad;
+                }
+        }
         kv4_add_block<HD, KEYS, PARTS, NT>(A, s[b], tile, at + b * 16, B, ranges[b]);
     }
 }

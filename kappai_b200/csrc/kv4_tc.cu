@@ -287,6 +287,9 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
     using S = Kt<HD>;
     constexpr int ST = S::ST;
     extern __shared__ unsigned char smem_dyn[];
+    // (these at fixed addresses: a pointer to them costs the loop over the keys a register, and 10 % of its time)
+    __shared__ volatile unsigned unsound[4 * S::NG * 4];      // [4 tiles][group][4]: a bit a key, whose value's group is not finite
+    __shared__ volatile unsigned char struck[256];     // groups in which a column reads such a value
     unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)smem_dyn + 1023) & ~(uintptr_t)1023);
     unsigned char* Qs = sm;                            // [2] OPER
     unsigned char* Ks = Qs + 2 * S::OPER;              // [ST] OPER
@@ -299,7 +302,7 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
     uint64_t* p_full = bars + 14; uint64_t* o_done = bars + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* meta = abort_flag + 1;               // [K's scale, V's][4 tiles]: exponents
+    volatile int* meta = abort_flag + 1;               // [K's scale, V's][4 tiles]: exponents; V's twice, plus 1 where a value is not finite
     volatile int* tops = meta + 8;                     // [2][4 warps]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -377,9 +380,22 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
         };
         auto do_value = [&](int i) {
             const int st = i % ST, use = i / ST;
+            // a group that is not finite is zeros in the product, and the columns that read its key are told
+#pragma unroll
+            for (int y = 0; y < S::NG; y++) {
+                const bool fine = kv4_finite(value.r[y]);
+                const unsigned bits = __ballot_sync(0xffffffffu, !fine);
+                if (lane == 0) unsound[((i & 3) * S::NG + y) * 4 + (warp & 3)] = bits;
+                if (!fine) value.r[y] = 0u;
+            }
             ev = exponent(value, ev);
             if (ok && (*abort_flag || !kp_mbar_wait_bounded(&v_empty[st], (use & 1) ^ 1))) ok = false;
-            if (d == 0) meta[4 + (i & 3)] = ev;
+            if (d == 0) {
+                unsigned any = 0u;
+#pragma unroll
+                for (int e = 0; e < 4 * S::NG; e++) any |= unsound[(i & 3) * 4 * S::NG + e];
+                meta[4 + (i & 3)] = ev * 2 + (any ? 1 : 0);
+            }
             const float f = kt_pow2(14 - ev);
 #pragma unroll
             for (int y = 0; y < S::NG; y++) {
@@ -447,6 +463,7 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
         // where column c's row lies in q or in out; -1: nowhere
         auto place_of = [&](int c, long long ld) { return c < n_cols ? (long long)(row0 + c / R) * ld + (kvh * R + c % R) * HD : -1LL; };
         unsigned char* Qg = Qs + g * S::OPER;
+        struck[threadIdx.x] = 0;
         const float f = kt_write_queries<HD>(Qg, q4 * 32, p.q, place_of(c, p.ldq), p.scale, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         kp_mbar_arrive(&q_full[g]);
@@ -525,7 +542,12 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
             // the product of the tile before has read P and added to O (known from S where P lies in it); this tile's values are there
             if (!S::ALIAS && i > 0 && ok && !kp_mbar_wait_bounded(&o_done[g], (i - 1) & 1)) ok = false;
             if (ok && !kp_mbar_wait_bounded(&v_full[i % ST], (i / ST) & 1)) ok = false;
-            const int ev_now = meta[4 + (i & 3)];
+            const int of_v = meta[4 + (i & 3)], ev_now = of_v >> 1;
+            if (__builtin_expect(of_v & 1, 0)) {
+#pragma unroll 1
+                for (int e = 0; e < 4 * S::NG; e++)
+                    if (unsound[(i & 3) * 4 * S::NG + e] & kt_bits(lo - key0 - (e & 3) * 32, pos - key0 - (e & 3) * 32)) struck[threadIdx.x] |= 1 << (e >> 2);
+            }
             const float corr_o = corr_l * kt_pow2(ev - ev_now);
             if (i > 0 && __any_sync(0xffffffffu, corr_o != 1.0f)) {
                 kp_tc_fence_after();
@@ -568,12 +590,13 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
             for (int e = 0; e < HD; e += 32) {
                 uint32_t v[32];
                 if (n_kt > 0) kp_tmem_ld32(tmem_o + e, v);
+                const float by = struck[threadIdx.x] >> (e / 64) & 1 ? __int_as_float(0x7fffffff) : inv;
 #pragma unroll
                 for (int d = 0; d < 32; d += 4) {
                     // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
                     float x[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) x[j] = none ? 0.f : __uint_as_float(v[(d & ~7) + 2 * j + (d >> 2 & 1)]) * inv;
+                    for (int j = 0; j < 4; j++) x[j] = none ? 0.f : __uint_as_float(v[(d & ~7) + 2 * j + (d >> 2 & 1)]) * by;
                     *reinterpret_cast<float4*>(part + kv4_share_at(col, e + d, HD)) = make_float4(x[0], x[1], x[2], x[3]);
                 }
             }
@@ -589,12 +612,13 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
             for (int e = 0; e < HD; e += 32) {
                 uint32_t v[32];
                 if (n_kt > 0) kp_tmem_ld32(tmem_o + e, v);
+                const float by = struck[threadIdx.x] >> (e / 64) & 1 ? __int_as_float(0x7fffffff) : inv;
 #pragma unroll
                 for (int d = 0; d < 32; d += 8) {
                     // places 0..7 hold dimensions 0, 4, 1, 5, 2, 6, 3, 7
                     float x[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) x[(j >> 1) + (j & 1) * 4] = none ? 0.f : __uint_as_float(v[d + j]) * inv;
+                    for (int j = 0; j < 8; j++) x[(j >> 1) + (j & 1) * 4] = none ? 0.f : __uint_as_float(v[d + j]) * by;
                     *reinterpret_cast<uint4*>(Qg + kt_at(r, (e + d) / 8)) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
                 }
             }

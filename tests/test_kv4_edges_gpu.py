@@ -280,3 +280,27 @@ def test_a_mixed_call_with_little_scratch(dtype, hd, with_mass, limit, monkeypat
             np.testing.assert_allclose(P.mass_of(mass, i), P.mass_of(m0, i) + got, rtol=1e-5, atol=1e-6)
         at += r
     assert not any(read_status().values())
+
+
+@pytest.mark.parametrize("dtype,hd,rows", FORMS + [(torch.bfloat16, 256, 30), (torch.bfloat16, 64, 9), (torch.float32, 128, 8)])
+@pytest.mark.parametrize("window", [None, 40])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_values_that_are_not_finite_reach_the_rows_that_read_them_only(dtype, hd, rows, window, bad):
+    """A value that a row's mask hides from it, a later token's or one behind the window, has no part in the row, whatever it is."""
+    H, G, n = 4, 2, 700
+    P = Paged([n], G, hd, 16, 3, dtype)
+    x = torch.from_numpy(P.v[0].astype(np.float32)).to(dtype)
+    first = n - rows
+    x[first + rows // 2, 1, 5] = bad                                          # a row in the middle, one value of kv head 1
+    x[n - 1, 0, hd - 1] = bad                                                 # the last
+    x[max(0, first - 20), 0, 0] = bad                                         # a key that the window hides from the later rows
+    k = torch.from_numpy(P.k[0].astype(np.float32)).to(dtype)
+    kv4.kv4_write(k.reshape(n, -1).to(DEV), x.reshape(n, -1).to(DEV), P.pages, P.slots(0, n), 16, G, hd)
+    kq, vq = (t.double().cpu().numpy().reshape(n, G, hd) for t in kv4.kv4_read(P.pages, P.slots(0, n), 16, G, hd, torch.float32))
+    q = queries(rows, H * hd, dtype)
+    out = attend(P, q.to(DEV), [rows], H, window=window).double().cpu().numpy().reshape(rows, H, hd)
+    with np.errstate(invalid="ignore"):
+        want, _ = plain_attention(q.double().numpy().reshape(rows, H, hd), kq, vq, first, hd ** -0.5, window, H)
+    assert np.array_equal(np.isfinite(out), np.isfinite(want))
+    fine = np.isfinite(want)
+    near(out[fine], want[fine], np.abs(vq[np.isfinite(vq)]).max(), dtype)
