@@ -304,3 +304,22 @@ def test_values_that_are_not_finite_reach_the_rows_that_read_them_only(dtype, hd
     assert np.array_equal(np.isfinite(out), np.isfinite(want))
     fine = np.isfinite(want)
     near(out[fine], want[fine], np.abs(vq[np.isfinite(vq)]).max(), dtype)
+
+
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
+@pytest.mark.parametrize("with_mass", [False, True])
+def test_lengths_that_differ_much(dtype, hd, with_mass):
+    """One long sequence among many short ones, and one without a key: chunks that most sequences have nothing in."""
+    H, G = 8, 2
+    lengths = [30, 1, 12000, 0, 257] + list(range(2, 60))
+    rows = [1] * len(lengths)
+    P = Paged(lengths, G, hd, 16, 3, dtype)
+    q, mass = queries(len(rows), H * hd, dtype), P.mass(5) if with_mass else None
+    m0 = mass.clone() if with_mass else None
+    out = attend(P, q.to(DEV), rows, H, mass=mass).double().cpu().numpy()
+    for i, n in enumerate(lengths):
+        want, got = plain_attention(q[i:i + 1].double().numpy().reshape(1, H, hd), P.k[i], P.v[i], n - 1, hd ** -0.5, None, H)
+        near(out[i:i + 1].reshape(1, H, hd), want, np.abs(P.v[i]).max() if n else 0.0, dtype)
+        if with_mass:
+            np.testing.assert_allclose(P.mass_of(mass, i), P.mass_of(m0, i) + got, rtol=1e-5, atol=1e-6)
+    assert not any(read_status().values())
