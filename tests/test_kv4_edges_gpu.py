@@ -52,24 +52,24 @@ def test_scratch_is_held_until_the_launch_has_returned(dtype, hd, rows, lengths,
     H, G = 4, 2
     P = Paged(lengths, G, hd, 16, 3, dtype)
     q, mass = queries(sum(rows), H * hd, dtype).to(DEV), P.mass()
-    sizes, calls, empty = [], [], torch.empty
+    handed, calls, empty = {}, [], torch.empty
 
     def noted(*a, **kw):
         t = empty(*a, **kw)
-        sizes.append(t.numel() * t.element_size())
+        handed[t.data_ptr()] = t.numel() * t.element_size()
         return t
 
     def launcher(what, fn, *args, **kw):
-        theirs = [empty(n, dtype=torch.uint8, device=DEV) for n in sizes for _ in range(2)]
+        assert set(handed) & {a for a in args if isinstance(a, int)}
+        theirs = [empty(n, dtype=torch.uint8, device=DEV) for n in handed.values() for _ in range(2)]
         calls.append(what)
-        for t in theirs:
-            assert not any(isinstance(a, int) and t.data_ptr() <= a < t.data_ptr() + t.numel() for a in args), f"{what} was handed memory that is free"
+        assert not any(t.data_ptr() in handed for t in theirs), f"{what} was handed memory that is free"
 
     out = torch.empty_like(q)
     monkeypatch.setattr(kv4, "_run", launcher)
     monkeypatch.setattr(torch, "empty", noted)
     attend(P, q, rows, H, mass=mass, out=out)
-    assert calls and sizes
+    assert calls and handed
 
 
 def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
