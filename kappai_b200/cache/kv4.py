@@ -142,7 +142,8 @@ class Kv4Cache:
                window: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of the last ``rows[i]`` tokens of ``seqs[i]`` (their keys and values have been appended): q is [sum of rows,
         num_heads * head_dim], the heads that share a kv head beside one another.  Where the cache keeps ``mass``, the weight that
-        every key gets, summed over the rows and over the heads of its kv head, is added to it."""
+        every key gets, summed over the rows and over the heads of its kv head, is added to it.  ``window`` counts places of the cache: after an
+        eviction these are the keys that stayed, which differ from head to head, and no longer positions of the text."""
         from ..ops.kv4 import kv4_attention
 
         self._check(seqs, rows, "attend")

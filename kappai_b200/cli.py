@@ -59,7 +59,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--max-batch", type=int, default=64, help="requests that run together (default 64)")
     g.add_argument("--max-step-tokens", type=int, default=2048, help="token budget of one step (default 2048)")
     g.add_argument("--page-size", type=int, default=64, help="tokens in a cache page (default 64)")
-    g.add_argument("--kv-bits", type=int, choices=[16, 4], default=16, help="bits of a cached key or value: 16 (default) or 4")
+    g.add_argument("--kv-bits", type=int, choices=[16, 4], default=16,
+                   help="bits of a key or value that attention caches: 16 (default) or 4; other mixers' memories stay as they are")
     g.add_argument("--kv-tokens", type=int, default=0, help="tokens the cache pools hold (0 = max-batch x ctx)")
     g.add_argument("--device", default="cuda:0", help="compute device (default: cuda:0)")
     g.add_argument("--random-weights", metavar="CONFIG", help="write a model folder with random weights from this "

@@ -67,8 +67,9 @@ __device__ __forceinline__ void kv4_load8(float (&v)[8], const T* p) {
 
 // Thread idx of a launch of `n_threads`: place `idx % per_row` of the rows idx / per_row + u (n_threads / per_row), u < U.  With
 // U rows a thread their loads are under way together: one row a thread leaves a CTA waiting for its slot, then for its values.
-// 6,007 rows of 8 heads of 128 float32 values written: 18.9 us with one row, 16.6 with two, 15.2 with three, 15.7 with four; 49 MB read and 7
-// written, 3.7 TB/s; 237 instructions a warp and row of 8 values a thread are two thirds of what the SMs could issue in that time.
+// 6,007 rows of 8 heads of 128 float32 values written: 18.9 us with one row, 16.6 with two, 15.2 with three, 15.7 with four (15.4 with three since
+// ranges above float32's are looked for); 49 MB read and 7 written, 3.7 TB/s.  257 instructions a warp and row of 8 values a thread use 74 % of the
+// issue slots, with 43 % of the warps there: fewer of either would help, no wall is reached.
 struct Kv4Rows { int n, ps_log2, G, hd, gs; long long n_slots; };
 
 template <typename T, bool VEC, int U>
@@ -233,10 +234,13 @@ __device__ __forceinline__ void kv4_columns(Kv4Cols<NT>& C, int col0, int n_cols
 
 // ---- split form: few rows a segment (decode).  One CTA per (chunk of keys, kv head and 8 of its columns, segment).  Its tiles of KEYS
 // keys come by the TMA into a ring of three stages, asked for two tiles ahead by the warps in turn; each of the four warps takes a
-// quarter of a tile, with the softmax and output of its own keys, and the four are joined at the end.  What bounds it is the issue of
-// instructions, 174 a block of 16 keys of 64 values and 328 of 128 (142 for the scores, 115 for the values), at half of what the SMs could
-// issue: hence the TMA and not cp.async (410 a block of 128 values), four CTAs an SM, and codes that are operands as they lie.  64 sequences
-// of 1,000 to 2,100 keys, 32 heads over 8 of 128 values: 42 us, 2.7 TB/s; two of 131,072 keys with mass, 16 heads over 8 of 64: 67 us, 2.1 TB/s.
+// quarter of a tile, with the softmax and output of its own keys, and the four are joined at the end.  A block of 16 keys takes 185 instructions
+// with heads of 64 values and 333 with 128: hence the TMA and not cp.async (80 more), four CTAs an SM, and codes that are operands as they lie.
+// 64 sequences of 1,000 to 2,100 keys, 32 heads over 8 of 128 values: 43 us, 2.7 TB/s; 90,001 and 131,072 keys with mass, 16 heads over 8 of 64: 61 us,
+// 2.3 TB/s, 14 of them the join's.  No one thing bounds it there: 51 and 57 % of the issue slots and 31 % of memory's rate are used, by 11 to 13 of 64
+// warps an SM that wait for their own products and loads; and the chunks are as long as the longest sequence's, so that CTAs with shorter ones (or none: 88
+// of 592) leave SMs idle at the end.  A sequence much longer than the others of its batch pays for that most: 131,072 keys beside 63 x 500 are one
+// chunk, 697 us, where 64 x 2,548, the same bytes, take 36.
 KP_STATUS_WORD(g_kv4_status, kv4)                     // 0 ok; 1: a bounded wait gave up
 
 template <int HD, int PARTS>

@@ -4,9 +4,10 @@
 //     key codes [ps][HD/2] | value codes [ps][HD/2] | key ranges [ps][NG] | value ranges [ps][NG]
 // A row of HD values is cut into NG groups of GS = 64 values (32 where 64 does not divide HD).  A group has a scale s and
 // a minimum z, both bfloat16 (a range in the low and the high half of 4 bytes), and 4-bit codes c (value 2i of the row in
-// the low half of byte i): the value is s c + z.  Codes are integers, so what is read is exact up to that formula; bfloat16
-// has the range of float32, so no key or value is too large for the cache, and the codes are taken against the rounded s
-// and z, so their rounding is not added to the codes'.
+// the low half of byte i): the value is s c + z.  Codes are integers, so what is read is exact up to that formula.  bfloat16
+// has the exponents of float32: values up to its largest, 3.39e38, have their place (larger ones count as infinite).  The codes are taken against
+// the rounded s and z, which makes up for their rounding but at the group's edge: z, the nearest bfloat16 number, can lie up to 2^-8 |min| above the
+// minimum, and values below z read as z.  That is more than half a step where |min| is more than 8.5 times the group's range.
 //
 // The arithmetic.  With q the query and k = s c + z,   q.k = sum over groups  s (q.c) + z (sum of q),
 // so the codes themselves enter the matrix instructions and a scale is one multiplication a (key, group), not one a value.
@@ -16,7 +17,8 @@
 // is below 2^-35 of that value.  float32 queries enter as two fp16 parts (22 bits).  The softmax weights p are
 // multiplied with the values' scales and enter as fp16 (as two parts in the float32 form), with the running maximum in
 // units that hold p s at or below 2^15 (it follows the maxima in steps of 2^8 and more): at least 31 binary orders of fp16 lie
-// below the largest weight of a row.
+// below the largest weight of a row.  (s is the largest scale of the values so far: values 2^30 and more smaller than another of the same
+// kv head lose bits to it.)
 // Scores, maxima, sums and accumulators are float32.
 //
 // Keys are the rows of the score product (m16n8k16: 16 keys x 8 queries), so that no row of the instruction is wasted where

@@ -1,7 +1,7 @@
 // Eviction from a 4-bit cache (kv4.cuh) by the weight that its keys have got.
 //
 // Of the n keys of a (segment, kv head) the first `first`, the last `recent` and, of those between, the ones with the most
-// mass stay, `keep` in all (equal mass: the lowest index); all of them where n <= keep.  They move, in their order, to
+// mass stay, `keep` in all (equal mass: the lowest index; one that is not a number counts as the most); all of them where n <= keep.  They move, in their order, to
 // places 0 .. of the segment's new pages, which are other pages than the old ones: nothing is read that this pass writes.
 #include "kv4.cuh"
 

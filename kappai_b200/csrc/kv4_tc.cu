@@ -15,15 +15,18 @@
 // Exactness.  K's operand is s (c - 8): an 8-bit times a 4-bit number, exact in fp16's 11 bits.  The rest, (z + 8 s) times the
 // query's sum over the group, is 16 more columns of the same product: both factors in two fp16 parts.  So S is off by float32
 // rounding only, and the weights added up as mass are those of the definition to 1e-6.  V's operand s (c - 8) + (z + 8 s) is
-// rounded to fp16 once (2^-12; the output's own rounding to bfloat16 is 2^-9), and so is P.
+// rounded to fp16 once (by up to 2^-11 of it; the output's own rounding to bfloat16 is up to 2^-8), and so is P; further products
+// for what fp16 leaves of them would be lost in the output's rounding.
 // Ranges.  Queries are scaled by a power of two a column, K by one a tile of keys, V by one that only grows from tile to tile
-// (O is rescaled when it does): fp16 then holds whatever bfloat16 did.  P is taken against a reference that follows the row's maximum
+// (O is rescaled when it does).  fp16 then holds a query's values down to 2^-24 of its largest, K's codes of groups whose scale is above 2^-24
+// of the tile's largest key, 11 bits of values down to 2^-28 of the largest so far; what is smaller loses bits, also in columns that do not read the key that
+// is so large.  P is taken against a reference that follows the row's maximum
 // in steps of at least 2^8 (O is rescaled in tensor memory only then), P <= 2^15.
 // Every mbarrier wait is bounded; one that gives up sets the status word, and the CTA frees its tensor memory and returns.
 //
 // Measured.  A tile (256 columns, 128 keys) takes 1.9 us with heads of 64, whose exponentials alone are 1.04 us of the SM's, and 2.4 us with heads of
 // 128, whose products are 1.1: what bounds it is the chain of S, softmax, P and second product, which two groups cannot hide.  A CTA's start
-// and end take 8 us and 12.  1,024 rows of 32 heads over 8 of 128 values behind 15,360 keys: 326 us, 0.81 PFLOP/s.
+// and end take 8 us and 12.  1,024 rows of 32 heads over 8 of 128 values behind 15,360 keys: 326 us on the device, 0.81 PFLOP/s.
 #include "kv4.cuh"
 #include "tcgen05.cuh"
 
@@ -338,8 +341,8 @@ kv4_tc_kernel(const __grid_constant__ Kv4TcArgs p) {
     const int kt_skip = kt_all * rank / n_split, kt_lo = k_lo / KT_ROWS + kt_skip, n_kt = kt_all * (rank + 1) / n_split - kt_skip;
 
     if (warp >= 8 && warp < 12) {
-        // ---- codes to operands: thread d has key d of every tile.  Keys run two tiles ahead of the values' next: with one stage each K's is
-        // free half a tile before V's.
+        // ---- codes to operands: thread d has key d of every tile.  Keys run a tile ahead of the values: K's stage is free once both groups'
+        // scores are there, V's half a tile later.
         const int d = threadIdx.x - 256;
         const int* bt = p.block_table + (size_t)seg * p.max_blocks;
         const size_t rec = (size_t)kv4_page_bytes(p.ps, HD);

@@ -40,7 +40,7 @@ class EngineArgs:
     max_batch: int = 64                # requests that run together (state slots)
     max_step_tokens: int = 2048        # token budget of one step
     page_size: int = 64
-    kv_bits: int = 16                  # 4: attention keeps keys and values in 4 bits (page_size a power of two, at least 16)
+    kv_bits: int = 16                  # 4: attention keeps keys and values in 4 bits (page_size a power of two, at least 16), other mixers theirs as ever
     kv_tokens: int = 0                 # tokens the page pools hold (0: max_batch * ctx_size, or what fits beside the weights)
     device: str = "cuda:0"
     look_ahead: bool = True            # launch the next decode step before the last one's tokens are read

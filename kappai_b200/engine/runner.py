@@ -72,7 +72,8 @@ class ModelRunner:
         ``free_memory``: a function that returns the device's free bytes (for
         tests; by default the device is asked).  ``kv_bits``: 4 keeps the keys and
         values of the attention mixers in 4 bits (``page_size`` is then a power of
-        two, at least 16); a model without such a mixer is refused."""
+        two, at least 16), other mixers keep theirs as ever; a model without such a mixer, or
+        with one whose attention the kernels over 4 bits do not have, is refused."""
         if dtype not in DTYPES:
             raise EngineError(f"dtype '{dtype}': expected bfloat16 or float32")
         self.device = require_cuda(device)

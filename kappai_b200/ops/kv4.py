@@ -114,7 +114,7 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, pages: torch.Tensor, slot_map: t
     """Rows of keys and values [n, G hd] (float32 or bfloat16; columns of wider rows will do) to the slots ``slot_map`` names
     (int32: page * page_size + place; -1: nowhere).  A group is cut into 16 equal steps from its smallest value on, ``s =
     bfloat16((max - min) / 15)``, ``z = bfloat16(min)``, ``c = round((x - z) / s)`` (halves to even, within 0..15; 0 where s is
-    0).  A group with a value that is not finite reads as NaN."""
+    0).  A group with a value that is not finite reads as NaN.  No slot is named twice (which row it then holds, or parts of which, is not fixed)."""
     dev = _here(pages)
     slots = _have(slot_map, "slot_map", torch.int32, dev)
     at, n, code = _have_pages(pages, "pages", page_size, G, hd, dev), slot_map.numel(), dtype_code(k.dtype)
@@ -166,7 +166,8 @@ def kv4_attention(q: torch.Tensor, pages: torch.Tensor, block_table: torch.Tenso
     """Causal attention of the rows q [n, H hd] over their sequences' 4-bit pages (this step's keys and values already in them).
 
     Rows ``cu_rows[i] .. cu_rows[i + 1] - 1`` belong to sequence ``i``; the first of them stands at key ``seg_pos[i]`` and reads
-    the keys up to that one, of which ``window`` (None: all) the last; a row that reads none gives zeros.  ``max_rows`` and
+    the keys up to that one, of which ``window`` (None: all) the last; a row that reads none gives zeros, and what a row does not read has
+    no part in it, finite or not.  ``out`` is other memory than ``q``; ``cu_rows`` ends with at most the rows of ``q``.  ``max_rows`` and
     ``min_rows`` bound the rows of a sequence, ``max_context`` the last key that any row reads, counted from 1 (host integers).  ``mass`` (float32
     [n_pages, G, page_size]): the softmax weight of every key, summed over the rows and the query heads of its kv head, is added
     to the key's entry, in a fixed order: the same call gives the same bits.  Sequences whose tables name the same pages each add their
