@@ -468,9 +468,9 @@ kv4_split_kernel(const __grid_constant__ CUtensorMap codes, const Kv4Args p) {
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                float w = 0.f;
+                float w = 0.f;                             // (a score of -inf: the column does not read the key, whatever its sum is)
 #pragma unroll
-                for (int c = 0; c < 8; c++) if (c < live) w += kv4_exp2(x[u][c] - sums[c]);
+                for (int c = 0; c < 8; c++) if (c < live) w += x[u][c] == -INFINITY ? 0.f : kv4_exp2(x[u][c] - sums[c]);
                 if (key0 + u * 128 <= k_hi) kv4_add_mass(to[u], w);
             }
         }

@@ -323,3 +323,25 @@ def test_lengths_that_differ_much(dtype, hd, with_mass):
         if with_mass:
             np.testing.assert_allclose(P.mass_of(mass, i), P.mass_of(m0, i) + got, rtol=1e-5, atol=1e-6)
     assert not any(read_status().values())
+
+
+@pytest.mark.parametrize("dtype,hd,rows", FORMS + [(torch.bfloat16, 64, 2), (torch.float32, 64, 2), (torch.bfloat16, 64, 9)])
+@pytest.mark.parametrize("window", [None, 40])
+@pytest.mark.parametrize("n", [100, 1500, 9000])
+def test_weights_that_are_no_numbers_reach_the_keys_that_are_read_only(dtype, hd, rows, window, n):
+    """A row with a NaN in its query has weights that are NaN: its keys' masses are, those of keys that it does not read are not."""
+    H, G = 4, 2
+    rows = min(rows, n)
+    P = Paged([n], G, hd, 16, 3, dtype)
+    q, mass = queries(rows, H * hd, dtype), P.mass(5)
+    m0 = mass.clone()
+    x = q.clone()
+    x[rows // 3, hd + 3] = float("nan")                                       # head 1, of kv head 0
+    attend(P, x.to(DEV), [rows], H, window=window, mass=mass)
+    hi = n - rows + rows // 3
+    read = np.arange(n) <= hi if window is None else (np.arange(n) <= hi) & (np.arange(n) > hi - window)
+    have = P.mass_of(mass, 0)
+    assert np.isnan(have[0, read]).all() and not np.isnan(have[0, ~read]).any() and not np.isnan(have[1]).any()
+    _, want = plain_attention(q.double().numpy().reshape(rows, H, hd), P.k[0], P.v[0], n - rows, hd ** -0.5, window, H)
+    ok = ~np.isnan(have)
+    np.testing.assert_allclose(have[ok], (P.mass_of(m0, 0) + want)[ok], rtol=1e-5, atol=1e-6)
