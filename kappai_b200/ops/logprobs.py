@@ -1,0 +1,75 @@
+"""Python face of the log probabilities' kernel (``csrc/logprobs.cu``)."""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from .build import load_library
+from .kernels import STREAM, KernelError, _rows_2d, _run, dtype_code
+from .kv4 import _have, _here, _unlike
+
+MAX_TOP_LOGPROBS = 32      # alternatives of a row
+_CTAS = 148 * 4            # CTAs up to which rows are shared out over clusters
+_LEAST = 2048              # logits below which a CTA has too little to do
+
+_P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+_token_logprobs = None
+
+
+class TokenLogprobs(NamedTuple):
+    """What :func:`token_logprobs` says of each row, on the device."""
+
+    logprob: torch.Tensor          # float32 [n]: the given token's log probability (0 where none is given)
+    entropy: torch.Tensor          # float32 [n]: of the row's distribution, in nats
+    rank: torch.Tensor             # int32 [n]: how many tokens have a larger logit than the given one (-1 where none is given)
+    top_ids: torch.Tensor          # int32 [n, top]: the tokens with the largest logits, equal ones by index
+    top_logprobs: torch.Tensor     # float32 [n, top]: their log probabilities
+
+
+def _launcher():
+    global _token_logprobs
+    if _token_logprobs is None:
+        fn = load_library("logprobs").kp_token_logprobs
+        fn.argtypes = [_P, _L, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P]
+        _token_logprobs = fn
+    return _token_logprobs
+
+
+def logprob_parts(n: int, V: int) -> int:
+    """CTAs that share a row: as many as fill the SMs, none with less than a few thousand logits."""
+    parts = 1
+    while parts < 8 and n * parts * 2 <= _CTAS and V // (parts * 2) >= _LEAST:
+        parts *= 2
+    return parts
+
+
+def token_logprobs(logits: torch.Tensor, ids: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+    """Log probabilities under the softmax of each row of ``logits`` [n, vocab] (float32 or bfloat16; rows may lie any distance apart):
+    of the token ``ids[r]`` (int32; -1, or a number that is no token: none), and of the ``top`` (at most 32) tokens with the largest logits; the row's
+    entropy; and the given token's rank.
+
+    Logits of -inf have no probability; a row of nothing else has log probabilities of -inf and no entropy.  A row with a NaN or +inf gives NaN, and
+    -1 for its alternatives."""
+    dev = _here(logits)
+    if not isinstance(logits, torch.Tensor) or logits.get_device() != dev:
+        _unlike(logits, "logits", logits.dtype if isinstance(logits, torch.Tensor) else torch.float32, contiguous=False)
+    code = dtype_code(logits.dtype)
+    ld = _rows_2d(logits, "logits")
+    n, V = logits.shape
+    if V < 1 or top < 0 or top > min(MAX_TOP_LOGPROBS, V):
+        raise KernelError(f"token_logprobs: top={top} of {V} tokens; at most {MAX_TOP_LOGPROBS}, and no more than there are")
+    pid = None
+    if ids is not None:
+        pid = _have(ids, "ids", torch.int32, dev)
+        if ids.numel() != n:
+            raise KernelError(f"token_logprobs: one token a row, got {ids.numel()} for {n} rows")
+    if n > (2 ** 31 - 1) // 8:
+        raise KernelError(f"token_logprobs: {n} rows are more than a launch takes")
+    f = torch.empty(n * (2 + top), dtype=torch.float32, device=logits.device)
+    i = torch.empty(n * (1 + top), dtype=torch.int32, device=logits.device)
+    pf, pi = f.data_ptr(), i.data_ptr()
+    if n:
+        _run("token_logprobs", _launcher(), logits.data_ptr(), ld, pid, n, V, top, logprob_parts(n, V), pf, pf + 4 * n, pi, pi + 4 * n, pf + 8 * n, code, STREAM)
+    return TokenLogprobs(f[:n], f[n:2 * n], i[:n], i[n:].view(n, top), f[2 * n:].view(n, top))
