@@ -1,0 +1,46 @@
+// Attention of a batch whose sequences share a long prefix: what its kernels have in common.
+//
+// Sequences come in groups.  The block tables of a group's sequences begin alike: the first `prefix_len` keys are the same for all of them (a page in
+// which the prefix ends is each sequence's own copy).  A row at position pos reads the keys 0 .. pos of its sequence,
+//   o = sum_j exp(s_j) v_j / sum_j exp(s_j),   s_j = scale q k_j,
+// and the sum falls in two: the keys below prefix_len, which all rows of the group read, and the sequence's own keys from there on.
+//   The prefix: the rows of a group and the R = H / G query heads that share a kv head are one list of columns, c = row R + head, and a tile of columns
+//   reads a chunk of the prefix's keys once for all of them.  It leaves (m, l, O) of each column: the largest score (in units of log2), sum
+//   2^(s - m) and sum 2^(s - m) v.
+//   The own keys: a tile of columns of one sequence, its keys shared out over the CTAs of a cluster.  The cluster then joins its parts with the
+//   prefix's, M = max m, o = sum 2^(m - M) O / sum 2^(m - M) l, and writes the rows.
+// Two launches: the second runs while the first is still at work and waits for it only before it joins.
+//
+// Scratch: part_o [n_rows][H][n_chunks][hd] and part_ml [n_rows][H][n_chunks][2], float32; chunks that a group's prefix does not reach are neither
+// written nor read.
+#pragma once
+#include "common.cuh"
+
+#define SH_MAX_CHUNKS 64
+#define SH_MAX_CLUSTER 8
+
+struct ShArgs {
+    const void* q; long long ldq; int q_vec;                 // q_vec: rows start on 16-byte boundaries
+    const void* cache; long long n_pages;
+    const int* table; int width;
+    const int* cu_rows; const int* seg_pos; const int* group_seqs; const int* prefix_len;
+    int n, n_seq, n_groups;
+    void* out; long long ldo; int out_vec;
+    float* part_o; float* part_ml;
+    int n_chunks, chunk;                                     // of a prefix; keys a chunk
+    int tiles;                                               // of columns, of a group (first launch) or of a sequence (second)
+    int alone;                                               // second launch: there was no first one
+    float scale; int ps, ps_log2; int H, G, max_prefix;
+};
+
+__device__ __forceinline__ int sh_prefix(const ShArgs& p, int group) {
+    return max(0, min(min(p.prefix_len[group], p.max_prefix), p.width * p.ps));
+}
+__device__ __forceinline__ int sh_row(const ShArgs& p, int seq) { return max(0, min(p.cu_rows[seq], p.n)); }
+__device__ __forceinline__ float sh_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// the page of a key and its place there
+__device__ __forceinline__ int sh_block(const ShArgs& p, int key) { return p.ps_log2 >= 0 ? key >> p.ps_log2 : key / p.ps; }

@@ -1,0 +1,102 @@
+"""Python face of attention behind a shared prefix (``csrc/shared.cuh`` has its formulas and how the work is cut)."""
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import Tuple
+
+import torch
+
+from .build import load_library
+from .kernels import STREAM, KernelError, _run, dtype_code
+from .kv4 import _have, _have_rows, _here
+
+SHARED_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
+SHARED_MAX_KEYS = 1 << 30      # that a block table has room for: the kernels count keys in 32 bits
+_SMS = 148
+_MAX_CHUNKS, _MAX_CLUSTER = 64, 8
+
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_attention_shared = None
+
+
+def _launcher():
+    global _attention_shared
+    if _attention_shared is None:
+        fn = load_library("shared").kp_attention_shared
+        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 13 + [_P]
+        _attention_shared = fn
+    return _attention_shared
+
+
+@lru_cache(maxsize=4096)
+def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int) -> Tuple[int, ...]:
+    """How the work is cut: (columns of a tile of the prefix, tiles a group, chunks of the prefix, keys a chunk, columns of a tile of a sequence's own
+    keys, tiles a sequence, CTAs that share a tile's own keys).  Tiles have 16 columns where that is all there are; keys are shared out until
+    two CTAs an SM have work, none with less than a few tiles of keys."""
+    cols = max_group_rows * R
+    tile = 16 if cols <= 16 else 64
+    tiles = -(-cols // tile)
+    want = -(-2 * _SMS // (n_groups * tiles * G))
+    chunks = max(1, min(want, _MAX_CHUNKS, -(-max_prefix // 256)))
+    chunk = -(-max_prefix // (chunks * 64)) * 64 if max_prefix else 64
+    chunks = -(-max_prefix // chunk)
+    own_cols = max_rows * R
+    own_tile = 16 if own_cols <= 16 else 64
+    own_tiles = -(-own_cols // own_tile)
+    want = -(-2 * _SMS // (n_seq * own_tiles * G))
+    ctas = max(1, min(want, _MAX_CLUSTER, -(-max_own // 128)))
+    return tile, tiles, chunks, chunk, own_tile, own_tiles, ctas
+
+
+def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, cu_rows: torch.Tensor, seg_pos: torch.Tensor, group_seqs: torch.Tensor,
+                     prefix_len: torch.Tensor, out: torch.Tensor, scale: float, page_size: int, H: int, G: int, hd: int, max_rows: int, max_group_rows: int,
+                     max_prefix: int, max_own: int) -> torch.Tensor:
+    """Causal attention of the rows q [n, H hd] over their sequences' pages, where groups of sequences share their first keys: those are read once
+    for all rows of a group.
+
+    ``cache`` [pages, 2, G, page_size, hd] has keys and values (this step's in them already).  Rows ``cu_rows[i] .. cu_rows[i + 1] - 1`` belong to
+    sequence ``i``, the first of them stands at key ``seg_pos[i]`` and reads the keys up to that one; ``block_table[i]`` has all of the sequence's pages,
+    the shared ones in front.  Sequences ``group_seqs[g] .. group_seqs[g + 1] - 1`` are group ``g``: the first ``prefix_len[g]`` keys are the same for all of
+    them (read from the pages of the group's first sequence; a page that the prefix ends in may be each sequence's own copy), and no row stands before
+    their end (``seg_pos[i] >= prefix_len[g]``).  A sequence in no group shares nothing.  All int32 on the device.
+
+    Host bounds: ``max_rows`` rows of a sequence, ``max_group_rows`` rows of a group, ``max_prefix`` shared keys, ``max_own`` keys of a sequence
+    behind them.  ``out`` is other memory than ``q``; rows behind ``cu_rows[-1]`` are left as they were, and a row that reads no key gives zeros.  float32 or bfloat16,
+    accumulated in float32; the sums' order is fixed, so the same call gives the same bits."""
+    if G < 1 or H < 1 or H % G:
+        raise KernelError(f"attention_shared: {H} query heads over {G} kv heads")
+    if hd not in SHARED_HEAD_DIMS or page_size < 1:
+        raise KernelError(f"attention_shared: heads of {SHARED_HEAD_DIMS} values and pages of at least one key, got {hd} and {page_size}")
+    if max_rows < 1 or max_group_rows < 1 or max_prefix < 0 or max_own < 0:
+        raise KernelError(f"attention_shared: max_rows={max_rows} and max_group_rows={max_group_rows} are positive, max_prefix={max_prefix} and max_own={max_own} not negative")
+    dev = _here(cache)
+    at, code = _have(cache, "cache", q.dtype, dev), dtype_code(q.dtype)
+    n, n_seq, n_groups = q.shape[0], seg_pos.numel(), prefix_len.numel()
+    pq, ldq = _have_rows(q, "q", q.dtype, n, H * hd, dev)
+    po, ldo = _have_rows(out, "out", q.dtype, n, H * hd, dev)
+    table, cu, pos = _have(block_table, "block_table", torch.int32, dev), _have(cu_rows, "cu_rows", torch.int32, dev), _have(seg_pos, "seg_pos", torch.int32, dev)
+    seqs, lens = _have(group_seqs, "group_seqs", torch.int32, dev), _have(prefix_len, "prefix_len", torch.int32, dev)
+    shape, pages = block_table.shape, cache.shape
+    if len(pages) != 5 or pages[1:] != (2, G, page_size, hd) or at % 16:
+        raise KernelError(f"attention_shared: cache of [pages, 2, {G}, {page_size}, {hd}] on a 16-byte boundary, got {tuple(pages)}")
+    if cu_rows.numel() != n_seq + 1 or group_seqs.numel() != n_groups + 1 or len(shape) != 2 or shape[0] < n_seq:
+        raise KernelError("attention_shared: cu_rows has one entry more than seg_pos, group_seqs one more than prefix_len, block_table a row for each sequence")
+    if not n or not n_seq:
+        return out
+    width = shape[1]
+    if not pages[0] or width < 1 or width * page_size > SHARED_MAX_KEYS or max_prefix > width * page_size:
+        raise KernelError(f"attention_shared: max_prefix={max_prefix} does not lie within the block table's {width} pages, these have more than {SHARED_MAX_KEYS} keys, "
+                          "or there is no page")
+    if not n_groups:
+        max_prefix = 0
+    tile, tiles, chunks, chunk, own_tile, own_tiles, ctas = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, H // G)
+    if n_groups * tiles > 65535 or n_seq * own_tiles > 65535 or G > 65535:
+        raise KernelError(f"attention_shared: {n_seq} sequences in {n_groups} groups are more than a launch takes")
+    parts, ml = n * H * chunks * hd, None
+    scratch = torch.empty(n * H * chunks * (hd + 2), dtype=torch.float32, device=q.device) if chunks else None    # (has a name until the launches are queued)
+    p0 = scratch.data_ptr() if chunks else None
+    ml = p0 + 4 * parts if chunks else None
+    _run("attention_shared", _launcher(), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, ml, chunks, chunk, scale,
+         page_size, H, G, hd, max_prefix, tile, tiles, own_tile, own_tiles, ctas, int(chunks > 0), 0, code, STREAM)
+    return out
