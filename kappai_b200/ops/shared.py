@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import ctypes
 from functools import lru_cache
-from typing import Tuple
+from typing import NamedTuple
 
 import torch
 
@@ -15,9 +15,21 @@ SHARED_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 SHARED_MAX_KEYS = 1 << 30      # that a block table has room for: the kernels count keys in 32 bits
 _SMS = 148
 _MAX_CHUNKS, _MAX_CLUSTER = 64, 8
+TC_MIN_COLS = 16               # columns of a group above which the tcgen05 form takes its prefix
+
+USE_TC_SHARED = True           # the prefix's part of bfloat16 rows with heads of 64 or 128 runs on the tcgen05 tensor cores
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-_attention_shared = None
+_attention_shared = _prefix_tc = None
+
+
+def _launcher_tc():
+    global _prefix_tc
+    if _prefix_tc is None:
+        fn = load_library("shared_tc").kp_attention_shared_prefix_tc
+        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _F] + [_I] * 7 + [_P]
+        _prefix_tc = fn
+    return _prefix_tc
 
 
 def _launcher():
@@ -29,24 +41,48 @@ def _launcher():
     return _attention_shared
 
 
+class SharedCut(NamedTuple):
+    """How the work of a call is cut."""
+
+    tile: int          # columns of a tile of the prefix (0: none; 128: the tcgen05 form, 256 columns a CTA or 128 with two chunks of keys)
+    split: bool        # the latter
+    tiles: int         # of columns, a group
+    chunks: int        # of the prefix (0: there is none)
+    chunk: int         # keys a chunk
+    own_tile: int      # columns of a tile of a sequence's own keys
+    own_tiles: int     # of those, a sequence
+    ctas: int          # that share a tile's own keys
+
+
 @lru_cache(maxsize=4096)
-def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int) -> Tuple[int, ...]:
-    """How the work is cut: (columns of a tile of the prefix, tiles a group, chunks of the prefix, keys a chunk, columns of a tile of a sequence's own
-    keys, tiles a sequence, CTAs that share a tile's own keys).  Tiles have 16 columns where that is all there are; keys are shared out until
-    two CTAs an SM have work, none with less than a few tiles of keys."""
+def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int, tc: bool) -> SharedCut:
+    """Keys are shared out until the SMs have work, none with less than a few tiles of keys.  Tiles have 16 columns where that is all there are."""
+    own_tile = 16 if max_rows * R <= 16 else 64
+    own_tiles = -(-max_rows * R // own_tile)
+    ctas = max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // 128)))
+    if not max_prefix:
+        return SharedCut(0, False, 1, 0, 64, own_tile, own_tiles, ctas)
     cols = max_group_rows * R
+    if tc and cols > TC_MIN_COLS:
+        rows = 128 // R
+        split = max_group_rows <= rows
+        tiles = -(-max_group_rows // (rows if split else 2 * rows))
+        # one CTA an SM; of groups whose prefixes differ most have fewer chunks than the longest
+        want = max(1, (_SMS if n_groups == 1 else 2 * _SMS) // (n_groups * tiles * G)) * (2 if split else 1)
+        keys = -(-max_prefix // 128)
+        chunk = -(-keys // min(want, keys, _MAX_CHUNKS)) * 128
+        return SharedCut(128, split, tiles, -(-max_prefix // chunk), chunk, own_tile, own_tiles, ctas)
     tile = 16 if cols <= 16 else 64
     tiles = -(-cols // tile)
-    want = -(-2 * _SMS // (n_groups * tiles * G))
-    chunks = max(1, min(want, _MAX_CHUNKS, -(-max_prefix // 256)))
-    chunk = -(-max_prefix // (chunks * 64)) * 64 if max_prefix else 64
-    chunks = -(-max_prefix // chunk)
-    own_cols = max_rows * R
-    own_tile = 16 if own_cols <= 16 else 64
-    own_tiles = -(-own_cols // own_tile)
-    want = -(-2 * _SMS // (n_seq * own_tiles * G))
-    ctas = max(1, min(want, _MAX_CLUSTER, -(-max_own // 128)))
-    return tile, tiles, chunks, chunk, own_tile, own_tiles, ctas
+    chunks = max(1, min(-(-2 * _SMS // (n_groups * tiles * G)), _MAX_CHUNKS, -(-max_prefix // 256)))
+    chunk = -(-max_prefix // (chunks * 64)) * 64
+    return SharedCut(tile, False, tiles, -(-max_prefix // chunk), chunk, own_tile, own_tiles, ctas)
+
+
+def shared_tc_ok(q: torch.Tensor, cache: torch.Tensor, page_size: int, R: int, hd: int) -> bool:
+    """Can the tcgen05 form take the prefix of this call (bfloat16, heads of 64 or 128, rows on 16-byte boundaries, pages of which a tile of 128 keys is made)?"""
+    return (USE_TC_SHARED and q.dtype is torch.bfloat16 and hd in (64, 128) and R <= 128 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+            and page_size % 8 == 0 and (page_size % 128 == 0 or 128 % page_size == 0) and cache.shape[0] * 2 * cache.shape[2] * page_size < 2 ** 31 - 1)
 
 
 def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, cu_rows: torch.Tensor, seg_pos: torch.Tensor, group_seqs: torch.Tensor,
@@ -70,6 +106,8 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         raise KernelError(f"attention_shared: heads of {SHARED_HEAD_DIMS} values and pages of at least one key, got {hd} and {page_size}")
     if max_rows < 1 or max_group_rows < 1 or max_prefix < 0 or max_own < 0:
         raise KernelError(f"attention_shared: max_rows={max_rows} and max_group_rows={max_group_rows} are positive, max_prefix={max_prefix} and max_own={max_own} not negative")
+    if not 0.0 < scale < float("inf"):
+        raise KernelError(f"attention_shared: the scale is a positive number, got {scale}")
     dev = _here(cache)
     at, code = _have(cache, "cache", q.dtype, dev), dtype_code(q.dtype)
     n, n_seq, n_groups = q.shape[0], seg_pos.numel(), prefix_len.numel()
@@ -88,15 +126,21 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     if not pages[0] or width < 1 or width * page_size > SHARED_MAX_KEYS or max_prefix > width * page_size:
         raise KernelError(f"attention_shared: max_prefix={max_prefix} does not lie within the block table's {width} pages, these have more than {SHARED_MAX_KEYS} keys, "
                           "or there is no page")
+    R = H // G
     if not n_groups:
         max_prefix = 0
-    tile, tiles, chunks, chunk, own_tile, own_tiles, ctas = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, H // G)
-    if n_groups * tiles > 65535 or n_seq * own_tiles > 65535 or G > 65535:
+    cut = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, R, shared_tc_ok(q, cache, page_size, R, hd))
+    if n_groups * cut.tiles > 65535 or n_seq * cut.own_tiles > 65535 or G > 65535:
         raise KernelError(f"attention_shared: {n_seq} sequences in {n_groups} groups are more than a launch takes")
-    parts, ml = n * H * chunks * hd, None
-    scratch = torch.empty(n * H * chunks * (hd + 2), dtype=torch.float32, device=q.device) if chunks else None    # (has a name until the launches are queued)
-    p0 = scratch.data_ptr() if chunks else None
-    ml = p0 + 4 * parts if chunks else None
-    _run("attention_shared", _launcher(), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, ml, chunks, chunk, scale,
-         page_size, H, G, hd, max_prefix, tile, tiles, own_tile, own_tiles, ctas, int(chunks > 0), 0, code, STREAM)
+    chunks, tc = cut.chunks, cut.tile == 128
+    p0 = p1 = scratch = None
+    if chunks:
+        scratch = torch.empty(n * H * chunks * (hd + 2), dtype=torch.float32, device=q.device)       # (has a name until the launches are queued)
+        p0 = scratch.data_ptr()
+        p1 = p0 + 4 * n * H * chunks * hd
+    if tc:
+        _run("attention_shared_prefix", _launcher_tc(), pq, ldq, at, pages[0], table, width, cu, seqs, lens, n, n_seq, n_groups, p0, p1, chunks, cut.chunk, scale,
+             page_size, H, G, hd, max_prefix, cut.tiles, cut.split, STREAM)
+    _run("attention_shared", _launcher(), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, p1, chunks, cut.chunk, scale,
+         page_size, H, G, hd, max_prefix, 16 if cut.tile == 16 else 64, cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, bool(chunks) and not tc, tc, code, STREAM)
     return out
