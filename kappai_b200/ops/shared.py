@@ -8,7 +8,7 @@ from typing import NamedTuple
 import torch
 
 from .build import load_library
-from .kernels import STREAM, KernelError, _run, dtype_code
+from .kernels import F32, STREAM, KernelError, _run, dtype_code
 from .kv4 import _have, _have_rows, _here
 
 SHARED_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
@@ -20,7 +20,7 @@ TC_MIN_COLS = 16               # columns of a group above which the tcgen05 form
 USE_TC_SHARED = True           # the prefix's part of bfloat16 rows with heads of 64 or 128 runs on the tcgen05 tensor cores
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
-_attention_shared = _prefix_tc = None
+_attention_shared, _prefix_tc = {}, None
 
 
 def _launcher_tc():
@@ -32,13 +32,14 @@ def _launcher_tc():
     return _prefix_tc
 
 
-def _launcher():
-    global _attention_shared
-    if _attention_shared is None:
-        fn = load_library("shared").kp_attention_shared
-        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 13 + [_P]
-        _attention_shared = fn
-    return _attention_shared
+def _launcher(dtype: torch.dtype):
+    fn = _attention_shared.get(dtype)
+    if fn is None:
+        f32 = dtype_code(dtype) == F32
+        fn = load_library("shared_f32").kp_attention_shared_f32 if f32 else load_library("shared").kp_attention_shared
+        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 12 + [_P]
+        _attention_shared[dtype] = fn
+    return fn
 
 
 class SharedCut(NamedTuple):
@@ -55,9 +56,12 @@ class SharedCut(NamedTuple):
 
 
 @lru_cache(maxsize=4096)
-def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int, tc: bool) -> SharedCut:
-    """Keys are shared out until the SMs have work, none with less than a few tiles of keys.  Tiles have 16 columns where that is all there are."""
-    own_tile = 16 if max_rows * R <= 16 else 64
+def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int, tc: bool, f32: bool = False) -> SharedCut:
+    """Keys are shared out until the SMs have work, none with less than a few tiles of keys.  Tiles are no wider than the columns need."""
+    def columns(n):
+        return 8 if n <= 8 else (16 if n <= 16 else (32 if n <= 32 and f32 else 64))
+
+    own_tile = columns(max_rows * R)
     own_tiles = -(-max_rows * R // own_tile)
     ctas = max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // 128)))
     if not max_prefix:
@@ -72,7 +76,7 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
         keys = -(-max_prefix // 128)
         chunk = -(-keys // min(want, keys, _MAX_CHUNKS)) * 128
         return SharedCut(128, split, tiles, -(-max_prefix // chunk), chunk, own_tile, own_tiles, ctas)
-    tile = 16 if cols <= 16 else 64
+    tile = columns(cols)
     tiles = -(-cols // tile)
     chunks = max(1, min(-(-2 * _SMS // (n_groups * tiles * G)), _MAX_CHUNKS, -(-max_prefix // 256)))
     chunk = -(-max_prefix // (chunks * 64)) * 64
@@ -109,7 +113,8 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention_shared: the scale is a positive number, got {scale}")
     dev = _here(cache)
-    at, code = _have(cache, "cache", q.dtype, dev), dtype_code(q.dtype)
+    dtype_code(q.dtype)
+    at = _have(cache, "cache", q.dtype, dev)
     n, n_seq, n_groups = q.shape[0], seg_pos.numel(), prefix_len.numel()
     pq, ldq = _have_rows(q, "q", q.dtype, n, H * hd, dev)
     po, ldo = _have_rows(out, "out", q.dtype, n, H * hd, dev)
@@ -129,7 +134,7 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     R = H // G
     if not n_groups:
         max_prefix = 0
-    cut = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, R, shared_tc_ok(q, cache, page_size, R, hd))
+    cut = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, R, shared_tc_ok(q, cache, page_size, R, hd), q.dtype is torch.float32)
     if n_groups * cut.tiles > 65535 or n_seq * cut.own_tiles > 65535 or G > 65535:
         raise KernelError(f"attention_shared: {n_seq} sequences in {n_groups} groups are more than a launch takes")
     chunks, tc = cut.chunks, cut.tile == 128
@@ -141,6 +146,6 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     if tc:
         _run("attention_shared_prefix", _launcher_tc(), pq, ldq, at, pages[0], table, width, cu, seqs, lens, n, n_seq, n_groups, p0, p1, chunks, cut.chunk, scale,
              page_size, H, G, hd, max_prefix, cut.tiles, cut.split, STREAM)
-    _run("attention_shared", _launcher(), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, p1, chunks, cut.chunk, scale,
-         page_size, H, G, hd, max_prefix, 16 if cut.tile == 16 else 64, cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, bool(chunks) and not tc, tc, code, STREAM)
+    _run("attention_shared", _launcher(q.dtype), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, p1, chunks, cut.chunk, scale,
+         page_size, H, G, hd, max_prefix, 64 if tc else (cut.tile or 8), cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, bool(chunks) and not tc, tc, STREAM)
     return out
