@@ -189,7 +189,7 @@ def _rows_2d(t: torch.Tensor, name: str) -> int:
 
 _STATUS_LIBS = (("gemm_tc", "tc"), ("gemm_stream", "stream"), ("attention_mma", "attention_mma"),
                 ("attention_tc", "attention_tc"), ("moe", "moe_tc"), ("latent", "latent"), ("kv4", "kv4"), ("kv4_tc", "kv4_tc"),
-                ("shared", "shared"), ("shared_tc", "shared_tc"))
+                ("logprobs", "logprobs"), ("shared", "shared"), ("shared_tc", "shared_tc"))
 
 
 def read_status() -> dict:
