@@ -857,14 +857,18 @@ static int sh_run(ShArgs& a, int tile, int group_tiles, int own_tile, int own_ti
     return sh_run_tma<HD, false>(tm, a, tile, group_tiles, own_tile, own_tiles, own_ctas, with_prefix, st);
 }
 
-// tile, own_tile: columns of a tile, 8, 16, 32 (float32) or 64, of the first and of the second launch; with_prefix: 0 where the prefix's parts come from another
-// launch (prefix_done: it has been queued) or there is none.
+// The first launch in its tcgen05 form (kp_attention_shared_prefix_tc)
+typedef int (*ShPrefixTc)(const void*, long long, const void*, long long, const int*, int, const int*, const int*, const int*, int, int, int, float*, float*, int, int,
+                          float, int, int, int, int, int, int, int, void*);
+
+// tile, own_tile: columns of a tile, 8, 16, 32 (float32) or 64, of the first and of the second launch; n_chunks = 0: there is no prefix.  prefix_tc: the first
+// launch's tcgen05 form, or null; split: its argument.
 extern "C" int SH_ENTRY(const void* q, long long ldq, const void* cache, long long n_pages, const int* table, int width, const int* cu_rows, const int* seg_pos,
                         const int* group_seqs, const int* prefix_len, int n, int n_seq, int n_groups, void* out, long long ldo, float* part_o,
                         float* part_ml, int n_chunks, int chunk, float scale, int ps, int H, int G, int hd, int max_prefix, int tile, int group_tiles,
-                        int own_tile, int own_tiles, int own_ctas, int with_prefix, int prefix_done, void* stream) {
+                        int own_tile, int own_tiles, int own_ctas, void* prefix_tc, int split, void* stream) {
     if (n <= 0 || n_seq <= 0) return 0;
-    const int elt = sizeof(ShT);
+    const int elt = sizeof(ShT), with_prefix = n_chunks > 0 && !prefix_tc, prefix_done = n_chunks > 0 && prefix_tc;
     if (G < 1 || G > 65535 || H < 1 || H % G || ps < 1 || width < 1 || (long long)width * ps > (1 << 30) || n_pages < 1 || n_groups < 0 || chunk < 1 ||
         n_chunks < 0 || n_chunks > SH_MAX_CHUNKS || ((with_prefix || prefix_done) && (n_chunks < 1 || (long long)n_chunks * chunk < max_prefix)) ||
         (tile != 8 && tile != 16 && tile != 32 && tile != 64) || (own_tile != 8 && own_tile != 16 && own_tile != 32 && own_tile != 64) || group_tiles < 1 || own_tiles < 1 || own_ctas < 1 || own_ctas > SH_MAX_CLUSTER ||
@@ -877,6 +881,11 @@ extern "C" int SH_ENTRY(const void* q, long long ldq, const void* cache, long lo
                 out, ldo, ((uintptr_t)out & 15) == 0 && ldo * elt % 16 == 0, part_o, part_ml, n_chunks, chunk, 1, !(with_prefix || prefix_done), scale, ps, ps_log2,
                 H, G, with_prefix || prefix_done ? max_prefix : 0};
     const cudaStream_t st = (cudaStream_t)stream;
+    if (prefix_done) {
+        const int e = ((ShPrefixTc)prefix_tc)(q, ldq, cache, n_pages, table, width, cu_rows, group_seqs, prefix_len, n, n_seq, n_groups, part_o, part_ml, n_chunks, chunk,
+                                              scale, ps, H, G, hd, max_prefix, group_tiles, split, stream);
+        if (e) return e;
+    }
 #define SH_HD(D) case D: return sh_run<D>(a, tile, group_tiles, own_tile, own_tiles, own_ctas, with_prefix, st)
     switch (hd) {
         SH_HD(32);

@@ -23,12 +23,11 @@ _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_floa
 _attention_shared, _prefix_tc = {}, None
 
 
-def _launcher_tc():
+def _tc_address() -> int:
+    """The address of the prefix's tcgen05 form, which the launcher of both calls."""
     global _prefix_tc
     if _prefix_tc is None:
-        fn = load_library("shared_tc").kp_attention_shared_prefix_tc
-        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _I, _I, _F] + [_I] * 7 + [_P]
-        _prefix_tc = fn
+        _prefix_tc = ctypes.cast(load_library("shared_tc").kp_attention_shared_prefix_tc, ctypes.c_void_p).value
     return _prefix_tc
 
 
@@ -37,7 +36,7 @@ def _launcher(dtype: torch.dtype):
     if fn is None:
         f32 = dtype_code(dtype) == F32
         fn = load_library("shared_f32").kp_attention_shared_f32 if f32 else load_library("shared").kp_attention_shared
-        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 12 + [_P]
+        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 10 + [_P, _I, _P]
         _attention_shared[dtype] = fn
     return fn
 
@@ -143,9 +142,6 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         scratch = torch.empty(n * H * chunks * (hd + 2), dtype=torch.float32, device=q.device)       # (has a name until the launches are queued)
         p0 = scratch.data_ptr()
         p1 = p0 + 4 * n * H * chunks * hd
-    if tc:
-        _run("attention_shared_prefix", _launcher_tc(), pq, ldq, at, pages[0], table, width, cu, seqs, lens, n, n_seq, n_groups, p0, p1, chunks, cut.chunk, scale,
-             page_size, H, G, hd, max_prefix, cut.tiles, cut.split, STREAM)
     _run("attention_shared", _launcher(q.dtype), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, p1, chunks, cut.chunk, scale,
-         page_size, H, G, hd, max_prefix, 64 if tc else (cut.tile or 8), cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, bool(chunks) and not tc, tc, STREAM)
+         page_size, H, G, hd, max_prefix, 64 if tc else (cut.tile or 8), cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, _tc_address() if tc else None, cut.split, STREAM)
     return out

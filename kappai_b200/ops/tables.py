@@ -8,7 +8,7 @@ import torch
 
 from .build import load_library
 from .kernels import MAX_STEP_ROWS, STREAM, KernelError, _run
-from .kv4 import _have, _here
+from .kv4 import _here, _unlike
 
 MAX_TABLE_SEQS = 8192      # sequences of a call: their sums lie in shared memory
 
@@ -16,6 +16,7 @@ MAX_TABLE_SEQS = 8192      # sequences of a call: their sums lie in shared memor
 TABLES_NO_PAGES, TABLES_TOO_NARROW, TABLES_NO_ROOM, TABLES_NO_SENSE = 1, 2, 4, 8
 
 _P, _I = ctypes.c_void_p, ctypes.c_int
+_NAMES = ("block_table", "length", "delta", "free_pages", "n_free", "cu_rows", "seg_pos", "row_seg", "positions", "slot_map", "status", "own_from")
 _page_tables = None
 
 
@@ -47,12 +48,12 @@ def page_tables(block_table: torch.Tensor, length: torch.Tensor, delta: torch.Te
 
     ``status`` [1] gets 0, or the sum of what kept the step from being made: 1 too few free pages, 2 a block table too narrow, 4 more rows than
     room for them, 8 lengths or counts that make no sense.  Then nothing changes, and the step has no rows."""
-    dev = _here(block_table)
-    table, lens, change = _have(block_table, "block_table", torch.int32, dev), _have(length, "length", torch.int32, dev), _have(delta, "delta", torch.int32, dev)
-    free, count = _have(free_pages, "free_pages", torch.int32, dev), _have(n_free, "n_free", torch.int32, dev)
-    cu, pos, seg = _have(cu_rows, "cu_rows", torch.int32, dev), _have(seg_pos, "seg_pos", torch.int32, dev), _have(row_seg, "row_seg", torch.int32, dev)
-    at, slots, st = _have(positions, "positions", torch.int32, dev), _have(slot_map, "slot_map", torch.int32, dev), _have(status, "status", torch.int32, dev)
-    own = None if own_from is None else _have(own_from, "own_from", torch.int32, dev)
+    dev, i32 = _here(block_table), torch.int32
+    given = (block_table, length, delta, free_pages, n_free, cu_rows, seg_pos, row_seg, positions, slot_map, status) if own_from is None else (
+        block_table, length, delta, free_pages, n_free, cu_rows, seg_pos, row_seg, positions, slot_map, status, own_from)
+    for i, t in enumerate(given):
+        if not isinstance(t, torch.Tensor) or t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            _unlike(t, _NAMES[i], i32)
     S, cap, P = length.numel(), slot_map.numel(), free_pages.numel()
     if block_table.dim() != 2 or block_table.shape[0] != S or delta.numel() != S or seg_pos.numel() != S or cu_rows.numel() != S + 1 or (
             own_from is not None and own_from.numel() != S):
@@ -64,4 +65,6 @@ def page_tables(block_table: torch.Tensor, length: torch.Tensor, delta: torch.Te
     width = block_table.shape[1]
     if page_size < 1 or S * width >= 2 ** 31 - 1 or max(P, width) * page_size >= 2 ** 31:
         raise KernelError("page_tables: slots and positions are 32-bit numbers, below 2^31")
-    _run("page_tables", _launcher(), table, width, lens, change, own, free, P, count, page_size, S, cap, cu, pos, seg, at, slots, st, STREAM)
+    _run("page_tables", _launcher(), block_table.data_ptr(), width, length.data_ptr(), delta.data_ptr(), None if own_from is None else own_from.data_ptr(),
+         free_pages.data_ptr(), P, n_free.data_ptr(), page_size, S, cap, cu_rows.data_ptr(), seg_pos.data_ptr(), row_seg.data_ptr(), positions.data_ptr(),
+         slot_map.data_ptr(), status.data_ptr(), STREAM)
