@@ -5,7 +5,7 @@ The reference's entry point is ``engine_init(ctx, args, argc, argv)`` ->
 with a table-driven flag parser (src/config.c:403-447).  The same three calls
 exist here; flags keep the reference's names and meanings where it has them
 (-m, -c, -p, -n, -t, -k, -P, -M, --repeat-penalty, --repeat-last-n, -s,
---metrics, --stream, --time, --debug-forward, --debug).  There is no tokenizer in the engine:
+--metrics, --stream, --time, --debug-forward, --debug); --logprobs and --score are its own.  There is no tokenizer in the engine:
 a prompt is a list of token ids ("5,17,3" or "5 17 3") and so is the output.
 
     python -m kappai_b200.cli -m MODEL_DIR -p "5,17,3" -n 16 -t 0
@@ -79,8 +79,10 @@ def build_parser() -> argparse.ArgumentParser:
     b.add_argument("-M", "--min-p", type=float, default=0.10, help="min-p sampling (default 0.10, 0.0 = disabled)")
     b.add_argument("--repeat-penalty", type=float, default=1.0, help="repetition penalty (default 1.0 = disabled)")
     b.add_argument("--repeat-last-n", type=int, default=64, help="last-n tokens considered by repeat penalty (default 64)")
+    b.add_argument("--logprobs", type=int, default=None, metavar="N", help="say each new token's log probability, with N alternatives")
     b.add_argument("-s", "--seed", type=int, default=0, help="RNG seed (0 = random)")
     d = ap.add_argument_group("Tools / debug")
+    d.add_argument("--score", action="store_true", help="generate nothing: print the log probability of each prompt token but the first, given those before it")
     d.add_argument("--time", action="store_true", help="print device time by kernel class after generation")
     d.add_argument("--debug-forward", action="store_true",
                    help="print per-layer activation stats for the first step and the top logits at every sample")
@@ -110,6 +112,12 @@ def engine_init(argv: Optional[Sequence[str]] = None) -> Tuple[Engine, argparse.
     return eng, a
 
 
+def _print_logprobs(who: str, said) -> None:
+    for t in said:
+        print(f"[logprobs] {who} token {t.token} {t.logprob:.6f} rank {t.rank} entropy {t.entropy:.6f}"
+              + "".join(f" [{i}]={v:.6f}" for i, v in t.top), file=sys.stderr)
+
+
 def engine_run(eng: Engine, a: argparse.Namespace) -> int:
     """One-shot generation for the given prompts (src/engine.c:162-196,450-468).
     Returns 0, or ENGINE_EXIT_CONTEXT_FULL if a request ran into the context limit."""
@@ -124,7 +132,13 @@ def engine_run(eng: Engine, a: argparse.Namespace) -> int:
         return ENGINE_EXIT
     sp = SamplingParams(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p,
                         repeat_penalty=a.repeat_penalty, repeat_last_n=a.repeat_last_n, seed=a.seed,
-                        n_predict=a.n_predict)
+                        n_predict=a.n_predict, logprobs=a.logprobs)
+    if a.score:
+        for said in eng.score(prompts, a.logprobs or 0):
+            print(" ".join(f"{t.logprob:.6f}" for t in said))
+            if a.logprobs is not None:
+                _print_logprobs("prompt", said)
+        return 0
     single = len(prompts) == 1
     t0 = time.perf_counter()
     first = [None]
@@ -143,6 +157,9 @@ def engine_run(eng: Engine, a: argparse.Namespace) -> int:
     else:
         for o in outs:
             print(" ".join(str(t) for t in o))
+    if a.logprobs is not None:
+        for rid, r in eng.requests.items():
+            _print_logprobs(f"request {rid!r}", r.logprobs)
     st = eng.stats
     parts = []
     wanted = [m.strip() for m in a.metrics.split(",") if m.strip()]

@@ -17,7 +17,9 @@ from typing import Callable, Dict, Hashable, List, Optional, Sequence
 
 import torch
 
-from ..sampling.params import SamplingParams
+from ..ops.logprobs import token_logprobs
+from ..sampling.logprobs import TokenLogprob, packed, unpacked
+from ..sampling.params import MAX_LOGPROBS, SamplingParams
 from ..sampling.rng import resolve_seed
 from ..sampling.sampler import sample
 from ..ops import kernels as K
@@ -67,6 +69,7 @@ class _Launched:
     tokens: Optional[torch.Tensor]             # their new tokens on the device (int32)
     host: torch.Tensor                         # the pinned buffer the tokens and the status word are copied to
     done: torch.cuda.Event                     # recorded behind that copy
+    logprobs: Optional[torch.Tensor] = None    # pinned: what was said of the tokens, where a request asked for it (see sampling.logprobs)
 
 
 class Engine:
@@ -181,19 +184,26 @@ class Engine:
         n = len(got)
         # the new tokens and, behind them, one word that says whether a kernel of the step gave up a wait
         buf = torch.empty(n + 1, dtype=torch.int32, device=self.runner.device)
-        toks = None
+        toks = logprobs = None
         if got:
             # the token history only where a repeat penalty reads it
             recent = [r.tokens for r in got] if any(r.params.repeat_penalty != 1.0 for r in got) else None
+            tops = [r.params.logprobs for r in got if r.params.logprobs is not None]
+            # (a penalty changes the logits where they lie; a token's log probability is the model's own)
+            own = logits.clone() if tops and recent is not None else logits
             toks = sample(logits, [r.params for r in got], [r.seed for r in got],
                           [len(r.output) + ahead for r in got], recent, out=buf[:n])
+            if tops:
+                said = packed(token_logprobs(own, toks, max(tops)))
+                logprobs = torch.empty(said.shape, dtype=said.dtype, pin_memory=True)
+                logprobs.copy_(said, non_blocking=True)
         self.status.gather(buf[n:])
         host = self._token_staging[self._staging_turn]
         self._staging_turn ^= 1
         host[:n + 1].copy_(buf, non_blocking=True)
         done = torch.cuda.Event()
         done.record()
-        return _Launched(plan, got, toks, host, done)
+        return _Launched(plan, got, toks, host, done, logprobs)
 
     def _launch_ahead(self, cur: _Launched) -> Optional[_Launched]:
         """The step after ``cur``, if it can only be one more token for every request of ``cur``."""
@@ -233,6 +243,10 @@ class Engine:
             self._compute_failed(cur, ahead)
         plan = [e for e in cur.plan if e.request.state == RUNNING]   # without those that ended meanwhile
         sampled = {r.id: t for r, t in zip(cur.got, new)}
+        if cur.logprobs is not None:
+            for i, r in enumerate(cur.got):
+                if r.params.logprobs is not None and r.state == RUNNING:
+                    r.logprobs.append(unpacked(cur.logprobs, i, new[i], r.params.logprobs))
         n_prompt = sum(e.n for e in plan if e.n > 1 or not e.request.output)
         n_decode = sum(1 for e in plan if e.n == 1 and e.request.output and e.sample)
         self.scheduler.update(plan, sampled)
@@ -284,6 +298,70 @@ class Engine:
                 if on_token is not None:
                     on_token(r.id, r.output[-1])
         return [self.requests[i].output for i in ids]
+
+    # -- scores
+    SCORE_ROWS = 512           # logits that a step of a scoring makes at most (256 KB each at a vocabulary of 65,536)
+
+    def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenLogprob]]:
+        """The log probability of every token of each prompt given those before it, with ``top`` alternatives each: for a prompt of n tokens a list of
+        n - 1, the first token having nothing before it.  Nothing is sampled; the engine must have no request under way.  Prompts run in portions beside
+        one another, as requests do."""
+        if self.has_work():
+            raise EngineError("score: requests are under way; let them end first")
+        if not (0 <= top <= min(MAX_LOGPROBS, self.vocab_size)):
+            raise ValueError(f"score: top={top}; at most {min(MAX_LOGPROBS, self.vocab_size)} alternatives")
+        prompts = [[int(t) for t in p] for p in prompts]
+        for p in prompts:
+            if not 1 <= len(p) <= self.runner.max_model_len:
+                raise ValueError(f"score: a prompt of {len(p)} tokens; 1 to {self.runner.max_model_len} can be scored")
+            for t in p:
+                if not (0 <= t < self.vocab_size):
+                    raise ValueError(f"token id {t} outside the vocabulary of {self.vocab_size}")
+        if self._launched is not None:                               # (a step ahead whose requests have all ended meanwhile)
+            self._launched.done.synchronize()
+            self._launched = None
+        out: List[List[TokenLogprob]] = [[] for _ in prompts]
+        waiting = [i for i, p in enumerate(prompts) if len(p) > 1]   # of one token there is nothing to say
+        live: Dict[int, int] = {}                                    # prompt -> tokens that have run
+        name = lambda i: ("score", i)  # noqa: E731
+        budget = min(self.args.max_step_tokens, self.SCORE_ROWS)
+        try:
+            while live or waiting:
+                entries, rows = [], []                               # rows: (prompt, index of the token that a row's logits are for)
+                room = budget
+                for i in list(live) + waiting:
+                    if not room:
+                        break
+                    start = live.get(i, 0)
+                    n = min(len(prompts[i]) - 1 - start, room)       # (nothing follows the last token)
+                    if not self.runner.can_run(name(i), n) or (i not in live and len(live) == self.args.max_batch):
+                        if not entries:
+                            raise EngineError(f"score: no pages for prompt {i} of {len(prompts[i])} tokens")
+                        break
+                    entries.append(StepEntry(name(i), prompts[i][start:start + n], list(range(n))))
+                    rows += [(i, start + j + 1) for j in range(n)]
+                    room -= n
+                    if i not in live:
+                        waiting.remove(i)
+                    live[i] = start + n
+                    if not self.runner.is_live(name(i)):
+                        # (its pages are taken by the step; what comes next must see them as taken)
+                        self.runner.cache.admit(name(i))
+                    self.runner.cache.extend(name(i), start + n)
+                logits = self.runner.step(entries)
+                ids = torch.tensor([prompts[i][j] for i, j in rows], dtype=torch.int32).to(self.runner.device)
+                host = packed(token_logprobs(logits, ids, top)).cpu()
+                for k, (i, j) in enumerate(rows):
+                    out[i].append(unpacked(host, k, prompts[i][j], top))
+                for i in [i for i, at in live.items() if at == len(prompts[i]) - 1]:
+                    del live[i]
+                    self.runner.end(name(i))
+            self.runner.check_status()
+        finally:
+            for i in range(len(prompts)):
+                if self.runner.is_live(name(i)):
+                    self.runner.end(name(i))
+        return out
 
     def finish_reason(self, request_id: Hashable) -> Optional[str]:
         return self.requests[request_id].finish_reason

@@ -32,6 +32,7 @@ from dataclasses import dataclass, field
 from typing import Deque, Dict, Hashable, List, Optional
 
 from ..cache.manager import CacheManager
+from ..sampling.logprobs import TokenLogprob
 from ..sampling.params import SamplingParams
 
 WAITING, RUNNING, FINISHED = "waiting", "running", "finished"
@@ -46,6 +47,7 @@ class Request:
     params: SamplingParams
     seed: int = 1                               # resolved seed (never 0)
     output: List[int] = field(default_factory=list)
+    logprobs: List[TokenLogprob] = field(default_factory=list)     # of ``output``, where the request asked for them
     state: str = WAITING
     n_computed: int = 0                         # tokens whose keys/state are in the cache
     n_preempted: int = 0

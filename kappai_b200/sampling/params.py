@@ -3,8 +3,10 @@ meanings (src/config.c:156-172, help text :119-131)."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from typing import Optional
 
 MAX_TOP_K = 1024     # the device sampler keeps at most this many candidates (src/sampler.c:7)
+MAX_LOGPROBS = 32    # alternatives that a token's log probability can come with
 
 
 @dataclass
@@ -17,6 +19,7 @@ class SamplingParams:
     repeat_last_n: int = 64        # --repeat-last-n
     seed: int = 0                  # -s; 0 = random
     n_predict: int = -1            # -n; -1 = until the context is full or EOS
+    logprobs: Optional[int] = None  # --logprobs; with every new token its log probability and that many alternatives (None: neither)
 
     def validate(self, vocab_size: int) -> None:
         if self.top_k > MAX_TOP_K and self.top_k < vocab_size:
@@ -26,6 +29,8 @@ class SamplingParams:
             raise ValueError("repeat_penalty must be positive")
         if not (0.0 <= self.min_p <= 1.0) or self.top_p < 0.0:
             raise ValueError("top_p and min_p must lie in [0, 1]")
+        if self.logprobs is not None and not (0 <= self.logprobs <= min(MAX_LOGPROBS, vocab_size)):
+            raise ValueError(f"logprobs={self.logprobs}: at most {min(MAX_LOGPROBS, vocab_size)} alternatives")
         if self.repeat_last_n < 0 or self.repeat_last_n > 256:
             raise ValueError("repeat_last_n must lie in 0..256")
 
