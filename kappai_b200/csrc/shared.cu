@@ -708,7 +708,7 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     const ShMem<T, HD, BM, TMA> sm(smem);
     float* ml = sm.ml;
     float* wts = sm.wts;
-    __shared__ int s_group;
+    __shared__ int s_group, s_chunk;
     cg::cluster_group cluster = cg::this_cluster();
     const int n_cl = gridDim.x, part = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = blockIdx.y, seq = blockIdx.z / p.tiles, c0 = blockIdx.z % p.tiles * BM, R = p.H / p.G;
@@ -729,12 +729,16 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         sh_work(p, tm, sm, p.table + (size_t)seq * p.width, g, R, row0, n_cols, c0, k0, k1, min(k1, pos0 + c0 / R + 1),
                 [&](int c) { return min(k1, pos0 + (c0 + c) / R + 1); });
     }
+    if (p.budget) {
+        if (warp == 0) { const int c = sh_chunk(p, lane); if (lane == 0) s_chunk = c; }
+        __syncthreads();
+    }
     KP_TRACE_MARK(1);
     if (!p.alone) pdl_wait();                                // the prefix's parts are there
     pdl_launch_dependents();
     if (!work) return;
     if (n_cl > 1) cluster.sync();
-    const int n_pre = group >= 0 ? (P + p.chunk - 1) / p.chunk : 0, n_parts = n_cl + n_pre, ld_w = n_cl + p.n_chunks;
+    const int chunk = p.budget ? s_chunk : p.chunk, n_pre = group >= 0 ? (P + chunk - 1) / chunk : 0, n_parts = n_cl + n_pre, ld_w = n_cl + p.n_chunks;
     const float* O = reinterpret_cast<const float*>(sm.ring);
     // the parts' weights: 2^(m - M) / sum 2^(m - M) l.  The cluster's CTAs share the columns.
     for (int c = part + warp * n_cl; c < BM && c0 + c < n_cols; c += n_cl * (THREADS / 32)) {
@@ -859,31 +863,31 @@ static int sh_run(ShArgs& a, int tile, int group_tiles, int own_tile, int own_ti
 
 // The first launch in its tcgen05 form (kp_attention_shared_prefix_tc)
 typedef int (*ShPrefixTc)(const void*, long long, const void*, long long, const int*, int, const int*, const int*, const int*, int, int, int, float*, float*, int, int,
-                          float, int, int, int, int, int, int, int, void*);
+                          float, int, int, int, int, int, int, int, int, void*);
 
 // tile, own_tile: columns of a tile, 8, 16, 32 (float32) or 64, of the first and of the second launch; n_chunks = 0: there is no prefix.  prefix_tc: the first
-// launch's tcgen05 form, or null; split: its argument.
+// launch's tcgen05 form, or null; mode, budget: its arguments.
 extern "C" int SH_ENTRY(const void* q, long long ldq, const void* cache, long long n_pages, const int* table, int width, const int* cu_rows, const int* seg_pos,
                         const int* group_seqs, const int* prefix_len, int n, int n_seq, int n_groups, void* out, long long ldo, float* part_o,
                         float* part_ml, int n_chunks, int chunk, float scale, int ps, int H, int G, int hd, int max_prefix, int tile, int group_tiles,
-                        int own_tile, int own_tiles, int own_ctas, void* prefix_tc, int split, void* stream) {
+                        int own_tile, int own_tiles, int own_ctas, void* prefix_tc, int mode, int budget, void* stream) {
     if (n <= 0 || n_seq <= 0) return 0;
     const int elt = sizeof(ShT), with_prefix = n_chunks > 0 && !prefix_tc, prefix_done = n_chunks > 0 && prefix_tc;
     if (G < 1 || G > 65535 || H < 1 || H % G || ps < 1 || width < 1 || (long long)width * ps > (1 << 30) || n_pages < 1 || n_groups < 0 || chunk < 1 ||
         n_chunks < 0 || n_chunks > SH_MAX_CHUNKS || ((with_prefix || prefix_done) && (n_chunks < 1 || (long long)n_chunks * chunk < max_prefix)) ||
         (tile != 8 && tile != 16 && tile != 32 && tile != 64) || (own_tile != 8 && own_tile != 16 && own_tile != 32 && own_tile != 64) || group_tiles < 1 || own_tiles < 1 || own_ctas < 1 || own_ctas > SH_MAX_CLUSTER ||
         (long long)n_groups * group_tiles > 65535 || (long long)n_seq * own_tiles > 65535 || ((uintptr_t)cache & 15) || ((uintptr_t)q & (elt - 1)) ||
-        ((uintptr_t)out & (elt - 1)) || !(scale > 0.f) || (with_prefix && chunk % 64))
+        ((uintptr_t)out & (elt - 1)) || !(scale > 0.f) || (with_prefix && chunk % 64) || budget < 0 || (budget && (n_groups > 32 || (long long)n_groups * group_tiles * G > budget || chunk % 128)))
         return KP_ERR_BAD_ARG;
     int ps_log2 = -1;
     for (int i = 0; i < 31; i++) if (ps == 1 << i) ps_log2 = i;
     ShArgs a = {q, ldq, ((uintptr_t)q & 15) == 0 && ldq * elt % 16 == 0, cache, n_pages, table, width, cu_rows, seg_pos, group_seqs, prefix_len, n, n_seq, n_groups,
-                out, ldo, ((uintptr_t)out & 15) == 0 && ldo * elt % 16 == 0, part_o, part_ml, n_chunks, chunk, 1, !(with_prefix || prefix_done), scale, ps, ps_log2,
+                out, ldo, ((uintptr_t)out & 15) == 0 && ldo * elt % 16 == 0, part_o, part_ml, n_chunks, chunk, prefix_done ? budget : 0, group_tiles, 1, !(with_prefix || prefix_done), scale, ps, ps_log2,
                 H, G, with_prefix || prefix_done ? max_prefix : 0};
     const cudaStream_t st = (cudaStream_t)stream;
     if (prefix_done) {
         const int e = ((ShPrefixTc)prefix_tc)(q, ldq, cache, n_pages, table, width, cu_rows, group_seqs, prefix_len, n, n_seq, n_groups, part_o, part_ml, n_chunks, chunk,
-                                              scale, ps, H, G, hd, max_prefix, group_tiles, split, stream);
+                                              scale, ps, H, G, hd, max_prefix, group_tiles, mode, budget, stream);
         if (e) return e;
     }
 #define SH_HD(D) case D: return sh_run<D>(a, tile, group_tiles, own_tile, own_tiles, own_ctas, with_prefix, st)

@@ -36,7 +36,7 @@ def _launcher(dtype: torch.dtype):
     if fn is None:
         f32 = dtype_code(dtype) == F32
         fn = load_library("shared_f32").kp_attention_shared_f32 if f32 else load_library("shared").kp_attention_shared
-        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 10 + [_P, _I, _P]
+        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 10 + [_P, _I, _I, _P]
         _attention_shared[dtype] = fn
     return fn
 
@@ -44,11 +44,12 @@ def _launcher(dtype: torch.dtype):
 class SharedCut(NamedTuple):
     """How the work of a call is cut."""
 
-    tile: int          # columns of a tile of the prefix (0: none; 128: the tcgen05 form, 256 columns a CTA or 128 with two chunks of keys)
-    split: bool        # the latter
+    tile: int          # columns of a tile of the prefix (0: there is none; 128: the tcgen05 form)
+    mode: int          # of that: 0, 256 columns a CTA; 1, 128, whose tiles of keys two sets of warps take in turn; 2, 64, with half a tile of keys a warp
+    budget: int        # of that: CTAs that the prefixes of all groups are shared out over (0: chunks are of one length)
     tiles: int         # of columns, a group
-    chunks: int        # of the prefix (0: there is none)
-    chunk: int         # keys a chunk
+    chunks: int        # of a prefix, at most (0: there is none)
+    chunk: int         # keys a chunk (with a budget: at least)
     own_tile: int      # columns of a tile of a sequence's own keys
     own_tiles: int     # of those, a sequence
     ctas: int          # that share a tile's own keys
@@ -62,24 +63,25 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
 
     own_tile = columns(max_rows * R)
     own_tiles = -(-max_rows * R // own_tile)
-    ctas = max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // 128)))
+    own = (own_tile, own_tiles, max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // 128))))
     if not max_prefix:
-        return SharedCut(0, False, 1, 0, 64, own_tile, own_tiles, ctas)
+        return SharedCut(0, 0, 0, 1, 0, 64, *own)
     cols = max_group_rows * R
     if tc and cols > TC_MIN_COLS:
-        rows = 128 // R
-        split = max_group_rows <= rows
-        tiles = -(-max_group_rows // (rows if split else 2 * rows))
-        # one CTA an SM; of groups whose prefixes differ most have fewer chunks than the longest
-        want = max(1, (_SMS if n_groups == 1 else 2 * _SMS) // (n_groups * tiles * G)) * (2 if split else 1)
-        keys = -(-max_prefix // 128)
-        chunk = -(-keys // min(want, keys, _MAX_CHUNKS)) * 128
-        return SharedCut(128, split, tiles, -(-max_prefix // chunk), chunk, own_tile, own_tiles, ctas)
+        mode = 2 if max_group_rows <= 64 // R else (1 if max_group_rows <= 128 // R else 0)
+        tiles = 1 if mode else -(-max_group_rows // (128 // R * 2))
+        keys, items = -(-max_prefix // 128), n_groups * tiles * G
+        if 1 < n_groups <= 32 and items <= _SMS:
+            # (a prefix that is all there is has the shortest chunks)
+            least = max(-(-keys * tiles * G // _SMS), -(-keys // _MAX_CHUNKS))
+            return SharedCut(128, mode, _SMS, tiles, -(-keys // least), least * 128, *own)
+        chunk = -(-keys // min(max(1, _SMS // items), -(-keys // (2 if mode else 1)), _MAX_CHUNKS)) * 128
+        return SharedCut(128, mode, 0, tiles, -(-max_prefix // chunk), chunk, *own)
     tile = columns(cols)
     tiles = -(-cols // tile)
     chunks = max(1, min(-(-2 * _SMS // (n_groups * tiles * G)), _MAX_CHUNKS, -(-max_prefix // 256)))
     chunk = -(-max_prefix // (chunks * 64)) * 64
-    return SharedCut(tile, False, tiles, -(-max_prefix // chunk), chunk, own_tile, own_tiles, ctas)
+    return SharedCut(tile, 0, 0, tiles, -(-max_prefix // chunk), chunk, *own)
 
 
 def shared_tc_ok(q: torch.Tensor, cache: torch.Tensor, page_size: int, R: int, hd: int) -> bool:
@@ -143,5 +145,5 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         p0 = scratch.data_ptr()
         p1 = p0 + 4 * n * H * chunks * hd
     _run("attention_shared", _launcher(q.dtype), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, p1, chunks, cut.chunk, scale,
-         page_size, H, G, hd, max_prefix, 64 if tc else (cut.tile or 8), cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, _tc_address() if tc else None, cut.split, STREAM)
+         page_size, H, G, hd, max_prefix, 64 if tc else (cut.tile or 8), cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, _tc_address() if tc else None, cut.mode, cut.budget, STREAM)
     return out

@@ -280,6 +280,6 @@ def test_refusals():
 def test_how_the_work_is_cut(tc):
     for args in ((1, 8, 1, 8, 2048, 150, 8, 4), (5, 80, 4, 40, 12000, 300, 4, 4), (1, 1, 1, 1, 0, 1, 1, 1), (1, 256, 1, 256, 100000, 10, 8, 12), (2, 9, 3, 20, 1, 0, 1, 128)):
         c = shared_cut(*args, tc)
-        per = args[3] if not c.tile else (128 // args[7] * (1 if c.split else 2) if c.tile == 128 else c.tile / args[7])      # rows a tile
+        per = args[3] if not c.tile else ({0: 128 // args[7] * 2, 1: 128 // args[7], 2: 64 // args[7]}[c.mode] if c.tile == 128 else c.tile / args[7])      # rows a tile
         assert per * c.tiles >= args[3] and c.own_tile * c.own_tiles >= args[2] * args[7] and 1 <= c.ctas <= 8
         assert c.chunks <= 64 and c.chunks * c.chunk >= args[4] and c.chunk % (128 if c.tile == 128 else 64) == 0
