@@ -10,7 +10,7 @@
 // More than 128 columns: the two sets are different columns and read the same tiles.  Up to 128: both are the same columns and take turns at the tiles, so
 // that the tensor core and the loads go on for one while the other is at its exponentials.  Up to 64: each set has the columns twice, and the second copy
 // takes the second half of every tile's keys (P is zero in the other half), so that all warps have exponentials to do, half as many each: 24 rows of
-// two heads behind 120001 keys FIG_E.  What a column's copies have is joined through shared memory at the end.
+// two heads behind 120001 keys 62 us, 56 so.  What a column's copies have is joined through shared memory at the end.
 //
 // A column's reference m follows its largest score in steps of at least 2^8 (O is rescaled in tensor memory only then): weights are at most 2^8.  The
 // prefix's last page may hold anything behind the prefix: those scores are set to -inf, and the values' rows to zeros.
@@ -70,6 +70,11 @@ __device__ __forceinline__ void sc_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uin
 // a wait of a warp in step, which gives up as one
 __device__ __forceinline__ bool sc_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, kp_mbar_wait_bounded(bar, parity)); }
 
+// 32 bytes, a whole sector, at a 32-byte boundary
+__device__ __forceinline__ void sc_store32(float* dst, float4 a, float4 b) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(dst), "f"(a.x), "f"(a.y), "f"(a.z), "f"(a.w), "f"(b.x), "f"(b.y), "f"(b.z), "f"(b.w) : "memory");
+}
 __device__ __forceinline__ void sc_sync_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // grid: (chunks of a prefix, kv heads, groups x tiles of columns), or with a budget so many CTAs, which find theirs
@@ -110,9 +115,10 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         tile = at % per / p.G;
         kvh = at % p.G;
     }
-    const int s0 = max(0, min(p.group_seqs[group], p.n_seq)), s1 = max(s0, min(p.group_seqs[group + 1], p.n_seq));
+    const int g0 = p.group_seqs[group], g1 = p.group_seqs[group + 1], P = sh_prefix(p, group);
+    const int s0 = max(0, min(g0, p.n_seq)), s1 = max(s0, min(g1, p.n_seq));
     if (s0 == s1) return;
-    const int P = sh_prefix(p, group), first = sh_row(p, s0), rows = sh_row(p, s1) - first;
+    const int first = sh_row(p, s0), rows = sh_row(p, s1) - first;
     const int tile_row = tile * (MODE ? T : 2 * T);                        // the tile's first row in the group
     const int k_lo = chunk * chunk_keys, k_hi = min(P, k_lo + chunk_keys);
     if (tile_row >= rows || k_lo >= k_hi) return;
@@ -123,12 +129,44 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     auto number = [&](int i, int g) { return MODE ? 2 * i + g : i; };
     auto key_of = [&](int i, int g) { return k_lo + number(i, g) * SC_KEYS; };
 
-    if (threadIdx.x == 0) {
-        kp_mbar_init(q_full, 1);
-        for (int i = 0; i < ST; i++) { kp_mbar_init(&k_full[i], 1); kp_mbar_init(&k_empty[i], 1); kp_mbar_init(&v_full[i], 1); kp_mbar_init(&v_empty[i], 1); }
-        for (int i = 0; i < 2; i++) { kp_mbar_init(&s_full[i], 1); kp_mbar_init(&s_free[i], 128); kp_mbar_init(&p_full[i], 128); kp_mbar_init(&o_done[i], 1); }
-        *abort_flag = 0;
-        kp_mbar_init_fence();
+    // the first loads are under way while tensor memory is allocated
+    const int box = min(p.ps, SC_KEYS), n_box = SC_KEYS / box;
+    const int* bt = p.table + (size_t)s0 * p.width;
+    auto page_of = [&](int i, int g) {                 // of this lane's box of a tile
+        const int key = key_of(i, g) + lane * box;
+        return i < (g ? n1 : n0) && lane < n_box && key < k_hi ? bt[sh_block(p, key)] : -1;
+    };
+    auto load = [&](unsigned char* dst, int page, int i, int g, int kv, uint64_t* bar) {
+        const int key = key_of(i, g) + lane * box;
+        const bool mine = lane < n_box && key < k_hi && (unsigned)page < (unsigned long long)p.n_pages;
+        const int count = __popc(__ballot_sync(0xffffffffu, mine));
+        if (lane == 0) kp_mbar_expect_tx(bar, count * box * C::NB * 128);
+        __syncwarp();
+        if (mine) {
+            const int row = ((page * 2 + kv) * p.G + kvh) * p.ps + key - sh_block(p, key) * p.ps;
+            for (int y = 0; y < C::NB; y++) kp_tma_load_2d(dst + y * 16384 + lane * box * 128, &tmC, y * 64, row, bar);
+        }
+        __syncwarp();
+    };
+    int page[2];
+    if (warp == 9) {
+        page[0] = page_of(0, 0);
+        page[1] = MODE ? page_of(0, 1) : -1;
+        if (lane == 0) {
+            kp_mbar_init(q_full, 1);
+            for (int i = 0; i < ST; i++) { kp_mbar_init(&k_full[i], 1); kp_mbar_init(&k_empty[i], 1); kp_mbar_init(&v_full[i], 1); kp_mbar_init(&v_empty[i], 1); }
+            for (int i = 0; i < 2; i++) { kp_mbar_init(&s_full[i], 1); kp_mbar_init(&s_free[i], 128); kp_mbar_init(&p_full[i], 128); kp_mbar_init(&o_done[i], 1); }
+            *abort_flag = 0;
+            kp_mbar_init_fence();
+            const int q_tiles = MODE ? MODE : sets;    // (MODE 2: the same rows twice, 64 rows of the tile apart)
+            kp_mbar_expect_tx(q_full, q_tiles * C::NB * T * R * 128);
+            for (int g = 0; g < q_tiles; g++)
+                for (int y = 0; y < C::NB; y++)
+                    kp_tma_load_3d(Qs + g * (MODE ? 8192 : C::TILE) + y * 16384, &tmQ, y * 64, kvh * R, first + tile_row + (MODE ? 0 : g * T), q_full);
+        }
+        __syncwarp();
+        load(Ks, page[0], 0, 0, 0, &k_full[0]);
+        load(Vs, page[0], 0, 0, 1, &v_full[0]);
     }
     if (warp == 8) kp_tmem_alloc(tmem_slot, 512);
     kp_tc_fence_before();
@@ -138,38 +176,12 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 
     if (warp == 9) {
         // ---- loads
-        const int box = min(p.ps, SC_KEYS), n_box = SC_KEYS / box;
-        const int* bt = p.table + (size_t)s0 * p.width;
-        if (lane == 0) {
-            const int q_tiles = MODE ? MODE : sets;    // (MODE 2: the same rows twice, 64 rows of the tile apart)
-            kp_mbar_expect_tx(q_full, q_tiles * C::NB * T * R * 128);
-            for (int g = 0; g < q_tiles; g++)
-                for (int y = 0; y < C::NB; y++)
-                    kp_tma_load_3d(Qs + g * (MODE ? 8192 : C::TILE) + y * 16384, &tmQ, y * 64, kvh * R, first + tile_row + (MODE ? 0 : g * T), q_full);
-        }
-        __syncwarp();
         bool ok = true;
-        auto page_of = [&](int i, int g) {             // of this lane's box of a tile
-            const int key = key_of(i, g) + lane * box;
-            return i < (g ? n1 : n0) && lane < n_box && key < k_hi ? bt[key / p.ps] : -1;
-        };
-        auto load = [&](unsigned char* dst, int page, int i, int g, int kv, uint64_t* bar) {
-            const int key = key_of(i, g) + lane * box;
-            const bool mine = lane < n_box && key < k_hi && (unsigned)page < (unsigned long long)p.n_pages;
-            const int count = __popc(__ballot_sync(0xffffffffu, mine));
-            if (lane == 0) kp_mbar_expect_tx(bar, count * box * C::NB * 128);
-            __syncwarp();
-            if (mine) {
-                const int row = ((page * 2 + kv) * p.G + kvh) * p.ps + key % p.ps;
-                for (int y = 0; y < C::NB; y++) kp_tma_load_2d(dst + y * 16384 + lane * box * 128, &tmC, y * 64, row, bar);
-            }
-            __syncwarp();
-        };
-        int page[2] = {page_of(0, 0), MODE ? page_of(0, 1) : -1};
+        page[0] = page_of(1, 0);
         for (int i = 0; i < n0 && ok; i++)
 #pragma unroll
             for (int g = 0; g < (MODE ? 2 : 1); g++) {
-                if (i >= (g ? n1 : n0)) continue;
+                if (i >= (g ? n1 : n0) || (i == 0 && g == 0)) continue;
                 const int u = number(i, g), st = u % ST, par = ((u / ST) & 1) ^ 1;
                 if (*abort_flag || !sc_wait(&k_empty[st], par)) { ok = false; break; }
                 load(Ks + st * C::TILE, page[g], i, g, 0, &k_full[st]);
@@ -325,9 +337,9 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     uint32_t v[32];
                     kp_tmem_ld32(tmem_o + d, v);
                     if (live && ok) {
-                        uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * HD + d);
+                        auto four = [&](int j) { return make_float4(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])); };
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) dst[j >> 2] = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        for (int j = 0; j < 32; j += 8) sc_store32(p.part_o + at * HD + d + j, four(j), four(j + 4));
                     }
                 }
                 if (live && ok) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m, l);
@@ -366,17 +378,17 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     uint32_t v[32];
                     kp_tmem_ld32(tmem_o + d, v);
                     if (live && ok) {
-                        float4* dst = reinterpret_cast<float4*>(p.part_o + at * HD + d);
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
+                        auto four = [&](int j) {
                             float4 x = make_float4(__uint_as_float(v[j]) * f, __uint_as_float(v[j + 1]) * f, __uint_as_float(v[j + 2]) * f, __uint_as_float(v[j + 3]) * f);
 #pragma unroll
                             for (int e = 0; e < C::PARTS - 1; e++) {
                                 const float4 y = *reinterpret_cast<const float4*>(O + (e * C::COLS + c) * C::LDO + d + j);
                                 x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
                             }
-                            dst[j >> 2] = x;
-                        }
+                            return x;
+                        };
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) sc_store32(p.part_o + at * HD + d + j, four(j), four(j + 4));
                     }
                 }
                 if (live && ok) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
@@ -412,7 +424,7 @@ extern "C" int kp_attention_shared_prefix_tc(const void* q, long long ldq, const
     if (G < 1 || G > 65535 || H < 1 || H % G || mode < 0 || mode > 2 || H / G > (mode == 2 ? 64 : 128) || ps < 8 || ps % 8 || !(ps % SC_KEYS == 0 || SC_KEYS % ps == 0) ||
         width < 1 || (long long)width * ps > (1 << 30) || n_pages < 1 || n_pages * 2 * G * ps >= 2147483647LL || chunk < SC_KEYS || chunk % SC_KEYS || n_chunks < 1 ||
         n_chunks > SH_MAX_CHUNKS || (long long)n_chunks * chunk < max_prefix || tiles < 1 || (long long)n_groups * tiles > 65535 || (ldq & 7) || !(scale > 0.f) ||
-        (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)part_o) & 15) || (hd != 64 && hd != 128) || budget < 0 ||
+        (((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)part_o & 31) || (hd != 64 && hd != 128) || budget < 0 ||
         (budget && (n_groups > 32 || (long long)n_groups * tiles * G > budget)))
         return KP_ERR_UNSUPPORTED;
     const int R = H / G, T = (mode == 2 ? 64 : 128) / R;
@@ -431,7 +443,8 @@ extern "C" int kp_attention_shared_prefix_tc(const void* q, long long ldq, const
     ShArgs a = {};
     a.q = q; a.ldq = ldq; a.cache = cache; a.n_pages = n_pages; a.table = table; a.width = width; a.cu_rows = cu_rows; a.group_seqs = group_seqs;
     a.prefix_len = prefix_len; a.n = n; a.n_seq = n_seq; a.n_groups = n_groups; a.part_o = part_o; a.part_ml = part_ml; a.n_chunks = n_chunks; a.chunk = chunk;
-    a.budget = budget; a.group_tiles = tiles; a.tiles = tiles; a.scale = scale; a.ps = ps; a.H = H; a.G = G; a.max_prefix = max_prefix;
+    a.budget = budget; a.group_tiles = tiles; a.tiles = tiles; a.scale = scale; a.ps = ps; a.ps_log2 = -1; a.H = H; a.G = G; a.max_prefix = max_prefix;
+    for (int i = 0; i < 31; i++) if (ps == 1 << i) a.ps_log2 = i;
     const cudaStream_t st = (cudaStream_t)stream;
     switch (mode * 256 + hd) {
         case 64: return sc_launch<64, 0>(a, tq, tc, st);

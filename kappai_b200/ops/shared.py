@@ -63,7 +63,7 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
 
     own_tile = columns(max_rows * R)
     own_tiles = -(-max_rows * R // own_tile)
-    own = (own_tile, own_tiles, max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // 128))))
+    own = (own_tile, own_tiles, max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // 384))))
     if not max_prefix:
         return SharedCut(0, 0, 0, 1, 0, 64, *own)
     cols = max_group_rows * R
