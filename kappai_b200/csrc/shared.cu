@@ -39,13 +39,14 @@ template <typename T, int HD, int BM, bool TMA>
 struct Sh {
     static constexpr bool MMA = sizeof(T) == 2, KEYS = MMA && BM <= 16;     // KEYS: the warps share the keys, not the columns
     static constexpr int THREADS = TMA ? SH_WORKERS + 32 : SH_WORKERS;
-    static constexpr int KT = MMA || HD <= 128 ? 64 : 32;                   // keys a tile
+    static constexpr int KT = MMA ? 64 : 32;                                // keys a tile
     static constexpr int E = 16 / sizeof(T);                                // values of 16 bytes
     static constexpr int LD = HD + E;                                       // a row in shared memory: 16 bytes more, so that rows lie in different banks
     static constexpr int TILE = KT * (TMA ? HD : LD);                       // values of K's tile, or of V's (TMA: 64 values a row, swizzled)
     static constexpr int CH = HD / E, NI = (KT * CH + SH_WORKERS - 1) / SH_WORKERS;
     static constexpr int PAIR = 2 * TILE * (int)sizeof(T);
-    static constexpr int ST = TMA ? (HD == 64 ? 3 : 2) : (4 * PAIR <= 100 * 1024 ? 4 : (3 * PAIR <= 110 * 1024 ? 3 : 2));
+    // (float32: few, so that there is room for three CTAs an SM: with one a warp has a scheduler to itself and issues in one cycle of three)
+    static constexpr int ST = TMA ? (HD == 64 ? 3 : 2) : !MMA ? (HD < 96 ? 3 : 2) : (4 * PAIR <= 100 * 1024 ? 4 : (3 * PAIR <= 110 * 1024 ? 3 : 2));
     static constexpr int MR = BM / 8;                                       // columns of a thread (FMA)
     static constexpr int Q_BYTES = BM * LD * sizeof(T);
     static constexpr int RING = ST * PAIR;
@@ -708,18 +709,20 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     const ShMem<T, HD, BM, TMA> sm(smem);
     float* ml = sm.ml;
     float* wts = sm.wts;
-    __shared__ int s_group, s_chunk;
+    __shared__ int s_group, s_prefix, s_chunk;
     cg::cluster_group cluster = cg::this_cluster();
     const int n_cl = gridDim.x, part = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = blockIdx.y, seq = blockIdx.z / p.tiles, c0 = blockIdx.z % p.tiles * BM, R = p.H / p.G;
     sh_init(sm);
     if (tid == 0) s_group = -1;
     __syncthreads();
-    for (int i = tid; i < p.n_groups; i += THREADS)
-        if (p.group_seqs[i] <= seq && seq < p.group_seqs[i + 1]) s_group = i;
+    for (int i = tid; i < p.n_groups; i += THREADS) {        // (the three loads under way together)
+        const int from = p.group_seqs[i], to = p.group_seqs[i + 1], len = sh_prefix(p, i);
+        if (from <= seq && seq < to) { s_group = i; s_prefix = len; }
+    }
     const int row0 = sh_row(p, seq), n_cols = max(0, sh_row(p, seq + 1) - row0) * R, pos0 = max(-p.n, min(p.seg_pos[seq], p.width * p.ps));
     __syncthreads();
-    const int group = s_group, P = group >= 0 ? sh_prefix(p, group) : 0;
+    const int group = s_group, P = group >= 0 ? s_prefix : 0;
     const bool work = c0 < n_cols;                           // (the same for all CTAs of a cluster)
     if (work) {
         const int last = pos0 + (min(n_cols, c0 + BM) - 1) / R;                     // position of the tile's last row

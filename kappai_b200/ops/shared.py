@@ -63,7 +63,7 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
 
     own_tile = columns(max_rows * R)
     own_tiles = -(-max_rows * R // own_tile)
-    own = (own_tile, own_tiles, max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // 384))))
+    own = (own_tile, own_tiles, max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // (96 if f32 else 384)))))
     if not max_prefix:
         return SharedCut(0, 0, 0, 1, 0, 64, *own)
     cols = max_group_rows * R
@@ -79,7 +79,7 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
         return SharedCut(128, mode, 0, tiles, -(-max_prefix // chunk), chunk, *own)
     tile = columns(cols)
     tiles = -(-cols // tile)
-    chunks = max(1, min(-(-2 * _SMS // (n_groups * tiles * G)), _MAX_CHUNKS, -(-max_prefix // 256)))
+    chunks = max(1, min(-(-(3 if f32 else 2) * _SMS // (n_groups * tiles * G)), _MAX_CHUNKS, -(-max_prefix // (128 if f32 else 256))))
     chunk = -(-max_prefix // (chunks * 64)) * 64
     return SharedCut(tile, 0, 0, tiles, -(-max_prefix // chunk), chunk, *own)
 
