@@ -1,7 +1,7 @@
 // Of each row of logits: the log probability of a given token and how many tokens have a larger logit, the row's entropy, and the `top` tokens
 // with the largest logits (equal ones: the lowest index) with their log probabilities.
 //
-// With a reference r, S = sum 2^y and W = sum 2^y y, y = (x - r) log2 e:  log p = ln 2 (y - log2 S),  entropy = ln 2 (log2 S - W / S).  One pass over the
+// With a reference r, S = sum 2^y and W = sum 2^y y, y = (x - r) log2 e:  log p = x - r - ln S,  entropy = ln S - ln 2 W / S.  One pass over the
 // row carries (r, S, W) a thread in float32, y as one fma of x with r log2 e: whatever that is rounded to, it is the same for all.  r follows the thread's
 // maximum in steps of at least 16: with every new maximum rescaled, some lane of a warp had one at almost every piece.  Pieces with logits so far below
 // r that they have no probability (-inf, or the type's lowest value), and rows of nothing else, take differences x - r, bounded below, instead: 0 * inf does
@@ -100,7 +100,6 @@ __device__ __forceinline__ float lp_exp2(float x) {                 // (with sub
 }
 
 #define LP_LOG2E 1.4426950408889634f
-#define LP_LN2 0.6931471805599453f
 __device__ __forceinline__ float lp_max3(float a, float b, float c) {        // the largest of three (one instruction on this architecture)
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -486,15 +485,13 @@ token_logprobs_kernel(const LpArgs p) {
         z = to;
         rank += *cluster.map_shared_rank(&s_count, i);
     }
-    const float log_s = log2f(S);
+    // The last differences are taken in 64 bits, each rounded once: r, log2 e and y = x log2 e - rl as they were rounded add up to (r log2 e - rl) in y.
+    const double off = z.wild() ? 0.0 : (double)z.rl - (double)z.r * (double)LP_LOG2E, log_s = log((double)S) + off * 0.6931471805599453;
     const bool bad = !(S >= 0.f), none = S == 0.f;                   // a NaN or +inf among the logits; nothing but -inf
-    auto logprob = [&](float f) {
-        if (none) return -INFINITY;
-        return z.wild() || !(fabsf(f) <= 1e6f) ? (f - z.r) - log_s * LP_LN2 : (fmaf(f, LP_LOG2E, -z.rl) - log_s) * LP_LN2;
-    };
+    auto logprob = [&](float f) { return none ? -INFINITY : (float)(((double)f - (double)z.r) - log_s); };
     if (tid == 0) {
         p.logprob[row] = id >= 0 ? (bad ? S : logprob(mine)) : 0.f;
-        p.entropy[row] = none ? 0.f : (log_s - W / S) * LP_LN2;
+        p.entropy[row] = none ? 0.f : (float)(log_s - ((double)W / (double)S + off) / (double)LP_LOG2E);
         p.rank[row] = id >= 0 ? rank : -1;
     }
     if (top) {
