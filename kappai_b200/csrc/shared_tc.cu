@@ -13,7 +13,8 @@
 // two heads behind 120001 keys 62 us, 56 so.  What a column's copies have is joined through shared memory at the end.
 //
 // A column's reference m follows its largest score in steps of at least 2^8 (O is rescaled in tensor memory only then): weights are at most 2^8.  The
-// prefix's last page may hold anything behind the prefix: those scores are set to -inf, and the values' rows to zeros.
+// prefix's last page may hold anything behind the prefix: those scores are set to -inf, and the values' rows to zeros.  (All rows of a group read all of
+// the prefix: a value that is not finite belongs in every one of them.  Up to 64 columns an infinite one comes out as NaN, 0 times infinity.)
 // Every mbarrier wait is bounded; one that gives up sets the status word, and the CTA frees its tensor memory and returns.
 #include "shared.cuh"
 #include "tcgen05.cuh"

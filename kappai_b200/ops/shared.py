@@ -9,12 +9,13 @@ import torch
 
 from .build import load_library
 from .kernels import F32, STREAM, KernelError, _run, dtype_code
-from .kv4 import _have, _have_rows, _here
+from .kv4 import _have, _have_rows, _here, _unlike
 
 SHARED_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 SHARED_MAX_KEYS = 1 << 30      # that a block table has room for: the kernels count keys in 32 bits
 _SMS = 148
 _MAX_CHUNKS, _MAX_CLUSTER = 64, 8
+_SCRATCH = 1 << 28             # values of scratch above which a prefix is cut into fewer chunks
 TC_MIN_COLS = 16               # columns of a group above which the tcgen05 form takes its prefix
 
 USE_TC_SHARED = True           # the prefix's part of bfloat16 rows with heads of 64 or 128 runs on the tcgen05 tensor cores
@@ -31,13 +32,12 @@ def _tc_address() -> int:
     return _prefix_tc
 
 
-def _launcher(dtype: torch.dtype):
-    fn = _attention_shared.get(dtype)
+def _launcher(f32: bool):
+    fn = _attention_shared.get(f32)
     if fn is None:
-        f32 = dtype_code(dtype) == F32
         fn = load_library("shared_f32").kp_attention_shared_f32 if f32 else load_library("shared").kp_attention_shared
         fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 10 + [_P, _I, _I, _P]
-        _attention_shared[dtype] = fn
+        _attention_shared[f32] = fn
     return fn
 
 
@@ -56,8 +56,10 @@ class SharedCut(NamedTuple):
 
 
 @lru_cache(maxsize=4096)
-def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int, tc: bool, f32: bool = False) -> SharedCut:
-    """Keys are shared out until the SMs have work, none with less than a few tiles of keys.  Tiles are no wider than the columns need."""
+def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int, tc: bool, f32: bool = False,
+               most: int = _MAX_CHUNKS) -> SharedCut:
+    """Keys are shared out until the SMs have work, none with less than a few tiles of keys, a prefix over at most ``most`` CTAs a tile of columns.  Tiles are
+    no wider than the columns need."""
     def columns(n):
         return 8 if n <= 8 else (16 if n <= 16 else (32 if n <= 32 and f32 else 64))
 
@@ -73,21 +75,22 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
         keys, items = -(-max_prefix // 128), n_groups * tiles * G
         if 1 < n_groups <= 32 and items <= _SMS:
             # (a prefix that is all there is has the shortest chunks)
-            least = max(-(-keys * tiles * G // _SMS), -(-keys // _MAX_CHUNKS))
+            least = max(-(-keys * tiles * G // _SMS), -(-keys // most))
             return SharedCut(128, mode, _SMS, tiles, -(-keys // least), least * 128, *own)
-        chunk = -(-keys // min(max(1, _SMS // items), -(-keys // (2 if mode else 1)), _MAX_CHUNKS)) * 128
+        chunk = -(-keys // min(max(1, _SMS // items), -(-keys // (2 if mode else 1)), most)) * 128
         return SharedCut(128, mode, 0, tiles, -(-max_prefix // chunk), chunk, *own)
     tile = columns(cols)
     tiles = -(-cols // tile)
-    chunks = max(1, min(-(-(3 if f32 else 2) * _SMS // (n_groups * tiles * G)), _MAX_CHUNKS, -(-max_prefix // (128 if f32 else 256))))
+    chunks = max(1, min(-(-(3 if f32 else 2) * _SMS // (n_groups * tiles * G)), most, -(-max_prefix // (128 if f32 else 256))))
     chunk = -(-max_prefix // (chunks * 64)) * 64
     return SharedCut(tile, 0, 0, tiles, -(-max_prefix // chunk), chunk, *own)
 
 
-def shared_tc_ok(q: torch.Tensor, cache: torch.Tensor, page_size: int, R: int, hd: int) -> bool:
-    """Can the tcgen05 form take the prefix of this call (bfloat16, heads of 64 or 128, rows on 16-byte boundaries, pages of which a tile of 128 keys is made)?"""
-    return (USE_TC_SHARED and q.dtype is torch.bfloat16 and hd in (64, 128) and R <= 128 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
-            and page_size % 8 == 0 and (page_size % 128 == 0 or 128 % page_size == 0) and cache.shape[0] * 2 * cache.shape[2] * page_size < 2 ** 31 - 1)
+def shared_tc_ok(ldq: int, q: int, n_pages: int, page_size: int, G: int, R: int, hd: int) -> bool:
+    """Can the tcgen05 form take the prefix of a call with bfloat16 rows (heads of 64 or 128, rows ``ldq`` values apart on 16-byte boundaries from address ``q`` on, pages of
+    which a tile of 128 keys is made)?"""
+    return (USE_TC_SHARED and (hd == 64 or hd == 128) and R <= 128 and ldq % 8 == 0 and q % 16 == 0
+            and page_size % 8 == 0 and (page_size % 128 == 0 or 128 % page_size == 0) and n_pages * 2 * G * page_size < 2 ** 31 - 1)
 
 
 def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, cu_rows: torch.Tensor, seg_pos: torch.Tensor, group_seqs: torch.Tensor,
@@ -113,14 +116,15 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         raise KernelError(f"attention_shared: max_rows={max_rows} and max_group_rows={max_group_rows} are positive, max_prefix={max_prefix} and max_own={max_own} not negative")
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention_shared: the scale is a positive number, got {scale}")
-    dev = _here(cache)
-    dtype_code(q.dtype)
-    at = _have(cache, "cache", q.dtype, dev)
+    dev, dtype, i32 = _here(cache), q.dtype, torch.int32
+    f32 = dtype_code(dtype) == F32
+    at = _have(cache, "cache", dtype, dev)
+    for i, t in enumerate((block_table, cu_rows, seg_pos, group_seqs, prefix_len)):
+        if not isinstance(t, torch.Tensor) or t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            _unlike(t, ("block_table", "cu_rows", "seg_pos", "group_seqs", "prefix_len")[i], i32)
     n, n_seq, n_groups = q.shape[0], seg_pos.numel(), prefix_len.numel()
-    pq, ldq = _have_rows(q, "q", q.dtype, n, H * hd, dev)
-    po, ldo = _have_rows(out, "out", q.dtype, n, H * hd, dev)
-    table, cu, pos = _have(block_table, "block_table", torch.int32, dev), _have(cu_rows, "cu_rows", torch.int32, dev), _have(seg_pos, "seg_pos", torch.int32, dev)
-    seqs, lens = _have(group_seqs, "group_seqs", torch.int32, dev), _have(prefix_len, "prefix_len", torch.int32, dev)
+    pq, ldq = _have_rows(q, "q", dtype, n, H * hd, dev)
+    po, ldo = _have_rows(out, "out", dtype, n, H * hd, dev)
     shape, pages = block_table.shape, cache.shape
     if len(pages) != 5 or pages[1:] != (2, G, page_size, hd) or at % 16:
         raise KernelError(f"attention_shared: cache of [pages, 2, {G}, {page_size}, {hd}] on a 16-byte boundary, got {tuple(pages)}")
@@ -135,15 +139,18 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     R = H // G
     if not n_groups:
         max_prefix = 0
-    cut = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, R, shared_tc_ok(q, cache, page_size, R, hd), q.dtype is torch.float32)
-    if n_groups * cut.tiles > 65535 or n_seq * cut.own_tiles > 65535 or G > 65535:
+    cut = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, R,
+                     not f32 and shared_tc_ok(ldq, pq, pages[0], page_size, G, R, hd), f32, max(1, min(_MAX_CHUNKS, _SCRATCH // (n * H * (hd + 2)))))
+    tile, mode, budget, tiles, chunks, chunk, own_tile, own_tiles, ctas = cut
+    if n_groups * tiles > 65535 or n_seq * own_tiles > 65535 or G > 65535:
         raise KernelError(f"attention_shared: {n_seq} sequences in {n_groups} groups are more than a launch takes")
-    chunks, tc = cut.chunks, cut.tile == 128
+    tc = tile == 128
     p0 = p1 = scratch = None
     if chunks:
         scratch = torch.empty(n * H * chunks * (hd + 2), dtype=torch.float32, device=q.device)       # (has a name until the launches are queued)
         p0 = scratch.data_ptr()
         p1 = p0 + 4 * n * H * chunks * hd
-    _run("attention_shared", _launcher(q.dtype), pq, ldq, at, pages[0], table, width, cu, pos, seqs, lens, n, n_seq, n_groups, po, ldo, p0, p1, chunks, cut.chunk, scale,
-         page_size, H, G, hd, max_prefix, 64 if tc else (cut.tile or 8), cut.tiles, cut.own_tile, cut.own_tiles, cut.ctas, _tc_address() if tc else None, cut.mode, cut.budget, STREAM)
+    _run("attention_shared", _launcher(f32), pq, ldq, at, pages[0], block_table.data_ptr(), width, cu_rows.data_ptr(), seg_pos.data_ptr(), group_seqs.data_ptr(),
+         prefix_len.data_ptr(), n, n_seq, n_groups, po, ldo, p0, p1, chunks, chunk, scale, page_size, H, G, hd, max_prefix, 64 if tc else (tile or 8), tiles, own_tile,
+         own_tiles, ctas, _tc_address() if tc else None, mode, budget, STREAM)
     return out

@@ -169,6 +169,35 @@ def test_another_stream_and_a_captured_call():
         assert torch.equal(a, b)
 
 
+def test_rows_beyond_32_bit_offsets():
+    n, V = 20000, 110001
+    x = torch.empty((n, V), dtype=torch.bfloat16, device="cuda")
+    part, ids = rows(50, V, "bf16")
+    for r in range(0, n, 50):
+        x[r:r + 50] = part
+    got, want = token_logprobs(x, ids.repeat(n // 50), 3), token_logprobs(part, ids, 3)
+    check(part, ids, 3)
+    # other cuts of a row, other orders of its sums: near, and the same ids
+    assert torch.equal(got.top_ids, want.top_ids.repeat(n // 50, 1)) and torch.equal(got.rank, want.rank.repeat(n // 50))
+    assert (got.logprob - want.logprob.repeat(n // 50)).abs().max() <= 2 * (V / 256 + 40) * 2.0 ** -23 + 2.0 ** -21 * want.logprob.abs().max()
+    del x
+    torch.cuda.empty_cache()
+
+
+def test_two_calls_at_once():
+    a, b = rows(300, 30011, "f32"), rows(5, 65536, "bf16", seed=3)
+    want = [token_logprobs(*a, 9), token_logprobs(*b, 20)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for j, (s, args) in enumerate(zip(streams, ((*a, 9), (*b, 20)))):
+            with torch.cuda.stream(s):
+                got[j].append(token_logprobs(*args))
+    torch.cuda.synchronize()
+    for w, calls in zip(want, got):
+        assert all(torch.equal(s, t) for c in calls for s, t in zip(w, c))
+
+
 def test_refusals():
     x, ids = rows(4, 100, "f32")
     for bad in (lambda: token_logprobs(x.half(), ids), lambda: token_logprobs(x, ids.long()), lambda: token_logprobs(x, ids[:3]), lambda: token_logprobs(x, ids, 33),

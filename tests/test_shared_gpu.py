@@ -263,6 +263,49 @@ def test_the_same_call_gives_the_same_bits_on_another_stream_and_captured(dtype,
         assert torch.equal(want, a["out"])
 
 
+@pytest.mark.parametrize("dtype,hd", [("bf16", 64), ("bf16", 128), ("bf16", 96), ("f32", 64)])
+def test_bounds_may_be_wider_than_what_is_there(dtype, hd):
+    """A captured call has bounds for steps to come."""
+    b = Batch([(700, spread(1, 300, 20)), (30, spread(1, 30, 3, (1, 2)))], 16, 4, hd, 16, dtype, seed=6, wider=400)
+    for kw in ({"max_prefix": 6000}, {"max_own": 5000}, {"max_rows": 9}, {"max_group_rows": 100}, {"max_prefix": 5000, "max_own": 3000, "max_rows": 4, "max_group_rows": 64}):
+        b.check(attention_shared(**b.args(**kw)))
+
+
+@pytest.mark.parametrize("groups,hd", [(31, 64), (33, 64), (40, 128), (70, 128)])
+def test_many_groups(groups, hd):
+    Batch([((37 * i) % 200, spread(1, 9, 3 + i % 7, (1, 2))) for i in range(groups)], 8, 1, hd, 16, "bf16", seed=groups).check()
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, of different sizes, beside one another: each has scratch of its own."""
+    a, b = Batch([(3000, spread(1, 200, 40))], 16, 4, 64, 64, "bf16", seed=1), Batch([(900, spread(1, 90, 9))], 16, 4, 128, 64, "bf16", seed=2)
+    want = [attention_shared(**x.args()) for x in (a, b)]
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    args = [[x.args() for _ in range(8)] for x in (a, b)]
+    torch.cuda.synchronize()
+    for i in range(8):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[j].append(attention_shared(**args[j][i]))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
+
+
+@pytest.mark.parametrize("dtype,ps", [("bf16", 64), ("bf16", 60), ("f32", 64)])
+def test_pages_beyond_32_bit_offsets(dtype, ps):
+    """The last pages of a cache of more than 2^31 values: by TMA, copy by copy, and in float32."""
+    b = Batch([(200, spread(1, 70, 9))], 8, 2, 128, ps, dtype, seed=4)
+    used = b.cache.shape[0]
+    n_pages = (1 << 31) // (2 * 2 * ps * 128) + used + 5
+    far = torch.empty((n_pages, 2, 2, ps, 128), dtype=b.cache.dtype, device="cuda")
+    far[n_pages - used:] = b.cache
+    b.cache, b.table = far, np.where(b.table >= 0, b.table + n_pages - used, 0).astype(np.int32)
+    b.check()
+    del far, b
+    torch.cuda.empty_cache()
+
+
 def test_refusals():
     b = Batch([(40, spread(1, 9, 3))], 8, 2, 64, 16)
     ok = b.args()
