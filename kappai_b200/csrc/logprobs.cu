@@ -5,11 +5,11 @@
 // row carries (r, S, W) a thread in float32, y as one fma of x with r log2 e: whatever that is rounded to, it is the same for all.  r follows the thread's
 // maximum in steps of at least 16: with every new maximum rescaled, some lane of a warp had one at almost every piece.  Pieces with logits so far below
 // r that they have no probability (-inf, or the type's lowest value), and rows of nothing else, take differences x - r, bounded below, instead: 0 * inf does
-// not arise.  2048 rows of 65536 float32 logits: 85 us, 6.3 TB/s; with 5, 20 and 32 alternatives 98, 106 and 122; one row 4.5 us, 9 with alternatives.
+// not arise.  2048 rows of 65536 float32 logits: 85 us, 6.3 TB/s; with 5, 20 and 32 alternatives 99, 108 and 118; one row 4.6 us, 8.5 with alternatives.
 //
 // The alternatives need no second pass over the row.  A thread's values are a subset of the row, 64 bytes of every 16 KB.  The top-th largest of the maxima of
-// four subsets each is a bound below which no alternative lies, so only the subsets that reach it (few more than `top`) are read again, and the values
-// that reach it, few more than `top` again, are put in order by counting, compared together with their index as one 64-bit number: no two are
+// four subsets each is a bound below which no alternative lies, so only the subsets that reach it (few more than `top`) are read again, of these the pieces
+// that reach it a value a thread, and the values that reach it, few more than `top` again, are put in order by counting, compared together with their index as one 64-bit number: no two are
 // equal.  Where many maxima equal the bound (most of the row is masked), they are compared with their indices too, so that equal logits make no more
 // candidates.  Logits that crowd in few subsets can make more than there is room for; then the alternatives are found one after the other.
 // (A list that logits above a bound so far were put on as they came by made the pass half as long again.)
@@ -164,12 +164,13 @@ token_logprobs_kernel(const LpArgs p) {
     __shared__ int redi[LP_THREADS / 32];
     __shared__ float s_sums[3];                                      // of this CTA's part, read by the cluster's first CTA
     __shared__ int s_count;
-    __shared__ u64 s_best[LP_THREADS];                               // the threads' largest
+    __shared__ u64 s_best[LP_THREADS];                               // the threads' largest; then pieces
+    static_assert(LP_CAND * 4 <= sizeof(s_best), "");
     __shared__ u64 s_cand[LP_CAND];
     __shared__ u64 s_sel[LP_MAX_TOP];                                // the part's alternatives in order (0: there are no more)
     __shared__ u64 s_bound;
     __shared__ __align__(16) float s_most[LP_THREADS / 4];           // the largest of four threads
-    __shared__ int s_subset[LP_THREADS], s_n_subset, s_n_cand, s_reach;
+    __shared__ int s_subset[LP_THREADS], s_n_subset, s_n_hit, s_n_cand, s_reach;
     __shared__ float s_tau;
 
     if (tid == 0) {
@@ -315,7 +316,7 @@ token_logprobs_kernel(const LpArgs p) {
         if (lane == 0) { red2[0][warp] = s; red2[1][warp] = w; redi[warp] = c; }
     }
     const bool some = v0 + tid * LP_PIECES < v1 || single >= 0;      // this thread has values
-    if (tid == 0) { s_n_subset = 0; s_n_cand = 0; s_bound = 0; s_tau = -INFINITY; s_reach = 0; }
+    if (tid == 0) { s_n_subset = 0; s_n_hit = 0; s_n_cand = 0; s_bound = 0; s_tau = -INFINITY; s_reach = 0; }
     if (top) {
         // (NaN where four threads have nothing: no comparison counts it)
         const unsigned any = __ballot_sync(0xffffffffu, some);
@@ -391,8 +392,8 @@ token_logprobs_kernel(const LpArgs p) {
         if (reaches && single >= 0) take(to_f32(x[single]), single);
         // the threads' shares that reach it, a piece a thread: place i of them is piece i % 4 of stage (i / 4) % n_stages of share i / 4 / n_stages
         const int n_all = s_n_subset * n_stages * LP_PIECES;
-        const float least = low ? lp_value(low) : -INFINITY;
-        constexpr int U = 8;                                         // pieces under way
+        int* s_hit = reinterpret_cast<int*>(s_best);                 // pieces that may have some
+        constexpr int U = 4;                                         // pieces under way
         if (n_all) {
             const int d_sub = LP_THREADS / LP_PIECES / n_stages, d_stage = LP_THREADS / LP_PIECES - d_sub * n_stages;
             int sub = tid / LP_PIECES / n_stages, stage = tid / LP_PIECES - sub * n_stages;
@@ -409,17 +410,27 @@ token_logprobs_kernel(const LpArgs p) {
                 }
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    if (at[u] >= v1) continue;
                     float f[N];
                     lp_unpack(q[u], f);
                     float m = f[0];
 #pragma unroll
                     for (int j = 1; j < N; j++) m = fmaxf(m, f[j]);
-                    if (m >= least)
-#pragma unroll
-                        for (int j = 0; j < N; j++) take(f[j], head + at[u] * N + j);
+                    // (as if the largest were the piece's first)
+                    if (at[u] < v1 && lp_key(m, head + at[u] * N) >= low) { const int h = atomicAdd(&s_n_hit, 1); if (h < LP_CAND) s_hit[h] = at[u]; }
                 }
             }
+            lp_sync();
+            // ... and those once more, a value a thread: where they were found a place for each of a thread's values made so much code that fetching it took
+            // longest (592 rows of 100003 16-bit logits, 32 alternatives: 68 us, 45 so)
+            const int n_hit = s_n_hit;
+            if (n_hit <= LP_CAND)
+#pragma unroll 1
+                for (int i = tid; i < n_hit * N; i += LP_THREADS) {
+                    const int v = s_hit[i / N];
+                    take(to_f32(held ? *(reinterpret_cast<const T*>(ring + (at0 + (v - v0) / (LP_THREADS * LP_PIECES)) % LP_STAGES * LP_STAGE) + (v - v0) % (LP_THREADS * LP_PIECES) * N + i % N)
+                                     : x[head + v * N + i % N]), head + v * N + i % N);
+                }
+            else if (tid == 0) s_n_cand = LP_CAND + 1;
         }
         lp_sync();
         const int n_cand = s_n_cand;
