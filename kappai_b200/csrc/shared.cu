@@ -5,8 +5,8 @@
 //   their 16 rows and the columns as their 8: the 4 heads of a decoded token fill half of a product, not a quarter.  With up to 64 every warp takes 16 of the
 //   columns.  Scores, weights and output stay in registers.  Weights are rounded to bfloat16 as they enter the product with V, by up to 2^-8 of each, as the
 //   output itself is.
-//   float32 (FMA): a thread has some columns times some keys of the scores, then the same columns times some values of the output; weights pass through shared
-//   memory of their warp.  Nothing is rounded below 32 bits.
+//   float32 (FMA, two at a time: sums over the heads' even and odd places, pairs of values): a thread has some columns times some keys of the scores, then the
+//   same columns times some values of the output; weights pass through shared memory of their warp.  Nothing is rounded below 32 bits.
 // Tiles come by TMA from a warp of its own where the sizes allow it (bfloat16, heads of a multiple of 64 values, pages of which a tile is made): four warps
 // that also copied, 16 bytes a thread with a page to find for each, took twice the time.  Elsewhere by cp.async.
 // A key that a column does not read has no part in it, finite or not: in a tile with such keys the values that are not finite are taken out of the
@@ -83,6 +83,13 @@ __device__ __forceinline__ void sh_sync_workers() { asm volatile("bar.sync 1, 12
 
 // not a number, or infinite
 __device__ __forceinline__ bool sh_odd(float v) { return !(fabsf(v) <= 3.402823466e38f); }
+// two float32 operations at once
+__device__ __forceinline__ float2 sh_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
 // an 8 x 8 matrix of bfloat16, a row four lanes, turned over
 __device__ __forceinline__ uint32_t sh_transposed(uint32_t a) {
     uint32_t d;
@@ -517,13 +524,14 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
         constexpr int MR = C::MR, KJ = KT / 16, DJ = HD / 32;
         const int tr = tid >> 4, tc = tid & 15;
         float* P = reinterpret_cast<float*>(Pbuf);
-        float o[MR][2 * DJ], m[MR], l[MR];
+        float2 o[MR][DJ];
+        float m[MR], l[MR];
         int lm[MR];
 #pragma unroll
         for (int r = 0; r < MR; r++) {
             m[r] = -INFINITY; l[r] = 0.f; lm[r] = lim(tr * MR + r);
 #pragma unroll
-            for (int d = 0; d < 2 * DJ; d++) o[r][d] = 0.f;
+            for (int d = 0; d < DJ; d++) o[r][d] = make_float2(0.f, 0.f);
         }
         for (int t = 0; t < n_tiles; t++) {
             begin(t);
@@ -531,11 +539,11 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
             const float* Vt = Kt + TILE;
             const float* Qf = reinterpret_cast<const float*>(Qs) + tr * MR * LD;
             const int key0 = base + t * KT;
-            float s[MR][KJ];
+            float2 s2[MR][KJ];                                              // even and odd places of the heads
 #pragma unroll
             for (int r = 0; r < MR; r++)
 #pragma unroll
-                for (int j = 0; j < KJ; j++) s[r][j] = 0.f;
+                for (int j = 0; j < KJ; j++) s2[r][j] = make_float2(0.f, 0.f);
 #pragma unroll 4
             for (int d = 0; d < HD; d += 4) {
                 float4 k[KJ];
@@ -545,17 +553,19 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
                 for (int r = 0; r < MR; r++) {
                     const float4 q = *reinterpret_cast<const float4*>(Qf + r * LD + d);
 #pragma unroll
-                    for (int j = 0; j < KJ; j++) s[r][j] = fmaf(q.x, k[j].x, fmaf(q.y, k[j].y, fmaf(q.z, k[j].z, fmaf(q.w, k[j].w, s[r][j]))));
+                    for (int j = 0; j < KJ; j++)
+                        s2[r][j] = sh_fma2(make_float2(q.x, q.y), make_float2(k[j].x, k[j].y), sh_fma2(make_float2(q.z, q.w), make_float2(k[j].z, k[j].w), s2[r][j]));
                 }
             }
             const bool masked = key0 + KT > lim_min || key0 < k0;
 #pragma unroll
             for (int r = 0; r < MR; r++) {
-                float top = -INFINITY;
+                float top = -INFINITY, s[KJ];
 #pragma unroll
                 for (int j = 0; j < KJ; j++) {
-                    if (masked && (key0 + tc + 16 * j >= lm[r] || key0 + tc + 16 * j < k0)) s[r][j] = -INFINITY;
-                    top = fmaxf(top, s[r][j]);
+                    s[j] = s2[r][j].x + s2[r][j].y;
+                    if (masked && (key0 + tc + 16 * j >= lm[r] || key0 + tc + 16 * j < k0)) s[j] = -INFINITY;
+                    top = fmaxf(top, s[j]);
                 }
 #pragma unroll
                 for (int x = 8; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
@@ -564,17 +574,17 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
                 m[r] = n;
                 l[r] *= f;
 #pragma unroll
-                for (int d = 0; d < 2 * DJ; d++) o[r][d] *= f;
+                for (int d = 0; d < DJ; d++) { o[r][d].x *= f; o[r][d].y *= f; }
 #pragma unroll
                 for (int j = 0; j < KJ; j++) {
-                    const float e = exp2f(fmaf(s[r][j], sl2, -u));
+                    const float e = exp2f(fmaf(s[j], sl2, -u));
                     l[r] += e;
                     P[(tr * MR + r) * (KT + 4) + tc + 16 * j] = e;
                 }
             }
             __syncwarp();                                                   // (a column's weights are made and read by one half of a warp)
             if (!masked) {
-#pragma unroll 1
+#pragma unroll 2
                 for (int j = 0; j < KT; j += 4) {
                     float2 v[4][DJ];
 #pragma unroll
@@ -584,11 +594,9 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
 #pragma unroll
                     for (int r = 0; r < MR; r++) {
                         const float4 w = *reinterpret_cast<const float4*>(P + (tr * MR + r) * (KT + 4) + j);
+                        const float2 wx = make_float2(w.x, w.x), wy = make_float2(w.y, w.y), wz = make_float2(w.z, w.z), ww = make_float2(w.w, w.w);
 #pragma unroll
-                        for (int d = 0; d < DJ; d++) {
-                            o[r][2 * d] = fmaf(w.x, v[0][d].x, fmaf(w.y, v[1][d].x, fmaf(w.z, v[2][d].x, fmaf(w.w, v[3][d].x, o[r][2 * d]))));
-                            o[r][2 * d + 1] = fmaf(w.x, v[0][d].y, fmaf(w.y, v[1][d].y, fmaf(w.z, v[2][d].y, fmaf(w.w, v[3][d].y, o[r][2 * d + 1]))));
-                        }
+                        for (int d = 0; d < DJ; d++) o[r][d] = sh_fma2(wx, v[0][d], sh_fma2(wy, v[1][d], sh_fma2(wz, v[2][d], sh_fma2(ww, v[3][d], o[r][d]))));
                     }
                 }
             } else {
@@ -599,11 +607,7 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
                         if (key0 + j < lm[r]) {
                             const float w = P[(tr * MR + r) * (KT + 4) + j];
 #pragma unroll
-                            for (int d = 0; d < DJ; d++) {
-                                const float2 v = *reinterpret_cast<const float2*>(Vt + j * LD + d * 32 + tc * 2);
-                                o[r][2 * d] = fmaf(w, v.x, o[r][2 * d]);
-                                o[r][2 * d + 1] = fmaf(w, v.y, o[r][2 * d + 1]);
-                            }
+                            for (int d = 0; d < DJ; d++) o[r][d] = sh_fma2(make_float2(w, w), *reinterpret_cast<const float2*>(Vt + j * LD + d * 32 + tc * 2), o[r][d]);
                         }
             }
             __syncwarp();
@@ -614,7 +618,7 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
         for (int r = 0; r < MR; r++) {
             const int c = tr * MR + r;
 #pragma unroll
-            for (int d = 0; d < DJ; d++) *reinterpret_cast<float2*>(O + c * C::LDO + d * 32 + tc * 2) = make_float2(o[r][2 * d], o[r][2 * d + 1]);
+            for (int d = 0; d < DJ; d++) *reinterpret_cast<float2*>(O + c * C::LDO + d * 32 + tc * 2) = o[r][d];
 #pragma unroll
             for (int x = 8; x; x >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
             if (!tc) { ml[2 * c] = m[r]; ml[2 * c + 1] = l[r]; }

@@ -41,8 +41,8 @@ def _launcher():
 @lru_cache(maxsize=4096)
 def logprob_parts(n: int, V: int, top: int) -> int:
     """CTAs that share a row: as many as two an SM, none with less than a few thousand logits.  Measured, 64 rows of 65536 float32 logits with twenty
-    alternatives: 1, 2, 4 and 8 CTAs a row 14.1, 12.2, 12.2 and 22.7 us; 120 rows 14.7, 14.4, 23.3 and 34.8; one row 13.2, 10.7, 8.8 and 9.1, without alternatives
-    10.2, 6.7, 4.9 and 4.3."""
+    alternatives: 1, 2, 4 and 8 CTAs a row 14.3, 11.9, 11.6 and 22.1 us; 120 rows 14.8, 14.0, 22.4 and 33.7; one row 13.3, 10.5, 8.5 and 8.9, without alternatives
+    10.3, 7.0, 5.1 and 4.6."""
     parts = 1
     while parts < 4 and n * parts * 2 <= _CTAS and V // (parts * 2) >= _LEAST:
         parts *= 2
