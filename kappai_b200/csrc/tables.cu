@@ -9,7 +9,7 @@
 // Three exclusive sums over the sequences (rows, pages back, pages taken) say where everything goes; every CTA makes them for itself, then the
 // pages and the rows are shared out over all threads, each of which finds its sequence by bisection.  CTAs are one cluster: its barrier stands between
 // reading the lengths and writing them, and between putting pages on the stack and taking them.  Launch and latency bound: a chain of loads,
-// the sums, the bisection and a page's load.  Nothing happens, and `status` says why, where pages are short (1), a table is too
+// the sums, the bisection and a page's load.  64 sequences with a row each 4 us, 2000 with 60000 rows 9.8.  Nothing happens, and `status` says why, where pages are short (1), a table is too
 // narrow (2), the rows have no room (4) or lengths or counts make no sense (8): bits that are added up.
 #include "common.cuh"
 
@@ -18,32 +18,39 @@
 
 struct PtArgs {
     int* table; int width; int* length; const int* delta; const int* own_from;
-    int* free_pages; int n_pages; int* n_free; int ps, S, cap;
+    int* free_pages; int n_pages; int* n_free; int ps, ps_log2, S, cap;
     int* cu_rows; int* seg_pos; int* row_seg; int* positions; int* slots; int* status;
 };
 
 __device__ __forceinline__ void pt_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int pt_blocks(long long tokens, int ps) { return (int)((tokens + ps - 1) / ps); }
+// Division by a page's size, in 32 bits: a shift where it is a power of two.  (In 64 bits it was a
+// tenth of the time.)
+struct PtPages {
+    unsigned ps; int log2;
+    __device__ __forceinline__ unsigned of(unsigned x) const { return log2 >= 0 ? x >> log2 : x / ps; }
+    __device__ __forceinline__ int blocks(int tokens) const { return (int)of((unsigned)tokens + ps - 1); }      // (below 2^32: both are below 2^31)
+};
 
 // what a sequence of length L does with a change d
 struct PtSeq { int rows, back, taken, after; bool ended, wide, bad; };
-__device__ __forceinline__ PtSeq pt_seq(int L, int d, int own, int ps, int width) {
+__device__ __forceinline__ PtSeq pt_seq(int L, int d, int own, const PtPages& pages, int width) {
     PtSeq q = {0, 0, 0, L, false, false, false};
-    if (L < 0 || own < 0 || (L + (long long)ps - 1) / ps > width) { q.bad = true; q.after = 0; return q; }
-    const int b0 = pt_blocks(L, ps);
+    const long long most = (long long)width * pages.ps;      // (below 2^31)
+    if (L < 0 || own < 0 || L > most) { q.bad = true; q.after = 0; return q; }
+    const int b0 = pages.blocks(L);
     own = min(own, b0);
     long long after = (long long)L + d;
     q.ended = after <= 0;
     if (q.ended) after = 0;
-    else if (d < 0) after = min((long long)L, max(after, (long long)own * ps));
-    const long long b1 = (after + ps - 1) / ps;
-    if (b1 > width) { q.wide = true; return q; }
+    else if (d < 0) after = min((long long)L, max(after, (long long)own * pages.ps));
+    if (after > most) { q.wide = true; return q; }
+    const int b1 = pages.blocks((int)after);
     q.rows = min(max(d, 0), PT_MAX_ROWS + 1);               // (more have no room, and their sum stays within 32 bits)
     q.after = (int)after;
-    if (b1 < b0) q.back = b0 - max((int)b1, own);
-    else q.taken = (int)b1 - b0;
+    if (b1 < b0) q.back = b0 - max(b1, own);
+    else q.taken = b1 - b0;
     return q;
 }
 
@@ -61,6 +68,7 @@ __global__ void __launch_bounds__(1024)
 page_tables_kernel(const PtArgs p) {
     kp_pdl_begin();
     extern __shared__ int pt_smem[];
+    const PtPages pages = {(unsigned)p.ps, p.ps_log2};
     const int S = p.S, ps = p.ps, tid = threadIdx.x, T = blockDim.x, lane = tid & 31, warp = tid >> 5;
     int* cu_r = pt_smem;                                     // [S + 1] each
     int* cu_b = cu_r + S + 1;
@@ -73,13 +81,25 @@ page_tables_kernel(const PtArgs p) {
     // ---- the sums: a stretch of sequences a thread
     const int per = (S + T - 1) / T, i0 = min(tid * per, S), i1 = min(i0 + per, S);
     int r = 0, b = 0, t = 0, bad = 0;
-    for (int i = i0; i < i1; i++) {
-        const int L = p.length[i];
-        const PtSeq q = pt_seq(L, p.delta[i], p.own_from ? p.own_from[i] : 0, ps, p.width);
-        cu_r[i] = r; cu_b[i] = b; cu_t[i] = t;
-        len[i] = q.ended ? (int)((unsigned)L | 0x80000000u) : L;
-        r += q.rows; b += q.back; t += q.taken;
-        bad |= (q.wide ? 2 : 0) | (q.bad ? 8 : 0);
+    for (int j = i0; j < i1; j += 4) {
+        int L[4], d[4], own[4];                              // (under way together)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const bool there = j + k < i1;
+            L[k] = there ? p.length[j + k] : 0;
+            d[k] = there ? p.delta[j + k] : 0;
+            own[k] = there && p.own_from ? p.own_from[j + k] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = j + k;
+            if (i >= i1) break;
+            const PtSeq q = pt_seq(L[k], d[k], own[k], pages, p.width);
+            cu_r[i] = r; cu_b[i] = b; cu_t[i] = t;
+            len[i] = q.ended ? (int)((unsigned)L[k] | 0x80000000u) : L[k];
+            r += q.rows; b += q.back; t += q.taken;
+            bad |= (q.wide ? 2 : 0) | (q.bad ? 8 : 0);
+        }
     }
     int xr = r, xb = b, xt = t;                              // inclusive sums over the warp's threads
 #pragma unroll
@@ -91,11 +111,10 @@ page_tables_kernel(const PtArgs p) {
     if (bad) atomicOr(&s_bad, bad);
     const int n_free = p.n_free[0];
     __syncthreads();
-    int fr = xr - r, fb = xb - b, ft = xt - t, rows = 0, back = 0, taken = 0;
-    for (int w = 0; w < (T >> 5); w++) {
-        if (w == warp) { fr += rows; fb += back; ft += taken; }
-        rows += wsum[0][w]; back += wsum[1][w]; taken += wsum[2][w];
-    }
+    const int n_warps = T >> 5, wr = lane < n_warps ? wsum[0][lane] : 0, wb = lane < n_warps ? wsum[1][lane] : 0, wt = lane < n_warps ? wsum[2][lane] : 0;
+    int rows = __reduce_add_sync(0xffffffffu, wr), back = __reduce_add_sync(0xffffffffu, wb), taken = __reduce_add_sync(0xffffffffu, wt);
+    const int fr = xr - r + __reduce_add_sync(0xffffffffu, lane < warp ? wr : 0), fb = xb - b + __reduce_add_sync(0xffffffffu, lane < warp ? wb : 0),
+              ft = xt - t + __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0);
     int status = s_bad;
     // (a count that makes no sense, or more pages back than the stack has places for)
     if (n_free < 0 || n_free > p.n_pages || back > p.n_pages - n_free) status |= 8;
@@ -110,7 +129,7 @@ page_tables_kernel(const PtArgs p) {
     // ---- pages that come back
     for (int a = gt; a < back; a += GT) {
         const int i = pt_find(cu_b, S, a);
-        const int b0 = pt_blocks(len[i] & 0x7fffffff, ps), block = b0 - (cu_b[i + 1] - cu_b[i]) + a - cu_b[i];
+        const int b0 = pages.blocks(len[i] & 0x7fffffff), block = b0 - (cu_b[i + 1] - cu_b[i]) + a - cu_b[i];
         int* entry = p.table + (size_t)i * p.width + block;
         p.free_pages[top - 1 - a] = *entry;
         *entry = -1;
@@ -118,7 +137,7 @@ page_tables_kernel(const PtArgs p) {
     if (!status)
         for (int i = gt >> 5; i < S; i += GT >> 5)           // of a sequence that ends the shared blocks are forgotten too
             if (len[i] < 0) {
-                const int shared = pt_blocks(len[i] & 0x7fffffff, ps) - (cu_b[i + 1] - cu_b[i]);
+                const int shared = pages.blocks(len[i] & 0x7fffffff) - (cu_b[i + 1] - cu_b[i]);
                 for (int block = lane; block < shared; block += 32) p.table[(size_t)i * p.width + block] = -1;
             }
     __threadfence();
@@ -126,16 +145,16 @@ page_tables_kernel(const PtArgs p) {
     // ---- pages that are taken
     for (int k = gt; k < taken; k += GT) {
         const int i = pt_find(cu_t, S, k);
-        p.table[(size_t)i * p.width + pt_blocks(len[i], ps) + k - cu_t[i]] = p.free_pages[top - 1 - k];
+        p.table[(size_t)i * p.width + pages.blocks(len[i]) + k - cu_t[i]] = p.free_pages[top - 1 - k];
     }
     // ---- the rows
     for (int x = gt; x < p.cap; x += GT) {
         int seg = 0, pos = -1, slot = -1;
         if (x < rows) {
             seg = pt_find(cu_r, S, x);
-            const int L = len[seg], b0 = pt_blocks(L, ps);   // (a sequence with rows does not end)
+            const int L = len[seg], b0 = pages.blocks(L);   // (a sequence with rows does not end)
             pos = L + x - cu_r[seg];
-            const int block = pos / ps;
+            const int block = (int)pages.of(pos);
             const int page = block < b0 ? p.table[(size_t)seg * p.width + block] : p.free_pages[top - 1 - (cu_t[seg] + block - b0)];
             slot = page * ps + pos - block * ps;
         }
@@ -152,7 +171,7 @@ page_tables_kernel(const PtArgs p) {
             continue;
         }
         const int n = cu_r[i + 1] - cu_r[i];
-        const PtSeq q = pt_seq(L, p.delta[i], p.own_from ? p.own_from[i] : 0, ps, p.width);
+        const PtSeq q = pt_seq(L, p.delta[i], p.own_from ? p.own_from[i] : 0, pages, p.width);
         p.cu_rows[i + 1] = cu_r[i + 1];
         p.seg_pos[i] = n ? L : q.after;
         p.length[i] = q.after;
@@ -164,6 +183,30 @@ page_tables_kernel(const PtArgs p) {
     }
 }
 
+// CTAs of the largest cluster that the GPU can have, 16 or 8
+static int pt_cluster() {
+    static std::atomic<int> known[64];
+    int dev = 0, fit = 0;
+    if (cudaGetDevice(&dev) || dev >= 64) return 8;
+    if (const int k = known[dev].load(std::memory_order_relaxed)) return k;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = (size_t)(4 * PT_MAX_SEQS + 3) * 4;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 16; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) || cudaOccupancyMaxActiveClusters(&fit, page_tables_kernel, &cfg)) {
+        cudaGetLastError();
+        fit = 0;
+    }
+    const int most = fit > 0 ? 16 : 8;
+    known[dev].store(most, std::memory_order_relaxed);
+    return most;
+}
+
 extern "C" int kp_page_tables(int* table, int width, int* length, const int* delta, const int* own_from, int* free_pages, int n_pages, int* n_free,
                               int ps, int S, int cap, int* cu_rows, int* seg_pos, int* row_seg, int* positions, int* slots, int* status, void* stream) {
     if (S < 0 || S > PT_MAX_SEQS || cap < 0 || cap > PT_MAX_ROWS || ps < 1 || width < 0 || n_pages < 0 ||
@@ -172,12 +215,14 @@ extern "C" int kp_page_tables(int* table, int width, int* length, const int* del
     static std::atomic<unsigned long long> ready{0};
     int e = kp_smem_limit(page_tables_kernel, (size_t)(4 * PT_MAX_SEQS + 3) * 4, ready);
     if (e) return e;
-    // One CTA for a decode step's rows (a cluster's start and barrier cost more than they share out), a cluster of eight above.
+    // Measured (a step and the one that takes it back): 64 sequences with a row each, one CTA 9.5 us, four 8.0, sixteen 7.7; 2000 with 60000 rows, four, eight and
+    // sixteen CTAs 30, 23 and 19.5.  More than eight are for long ones, where the GPU can have such a cluster.
     const int work = cap > S ? cap : S;
-    const int ctas = work <= 2048 ? 1 : 8;
-    int threads = 128;
+    int threads = 128, ps_log2 = -1;
+    for (int i = 0; i < 31; i++) if (ps == 1 << i) ps_log2 = i;
     while (threads < 1024 && threads < work) threads *= 2;
-    PtArgs a = {table, width, length, delta, own_from, free_pages, n_pages, n_free, ps, S, cap, cu_rows, seg_pos, row_seg, positions, slots, status};
+    const int ctas = work <= 2048 ? 4 : pt_cluster();
+    PtArgs a = {table, width, length, delta, own_from, free_pages, n_pages, n_free, ps, ps_log2, S, cap, cu_rows, seg_pos, row_seg, positions, slots, status};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(threads);
