@@ -7,7 +7,7 @@
 //   output itself is.
 //   float32 (FMA, two at a time: sums over the heads' even and odd places, pairs of values): a thread has some columns times some keys of the scores, then the
 //   same columns times some values of the output; weights pass through shared memory of their warp.  Nothing is rounded below 32 bits.
-// Tiles come by TMA from a warp of its own where the sizes allow it (bfloat16, heads of a multiple of 64 values, pages of which a tile is made): four warps
+// Tiles come by TMA from a warp of its own where the sizes allow it (bfloat16, pages of which a tile is made): four warps
 // that also copied, 16 bytes a thread with a page to find for each, took twice the time.  Elsewhere by cp.async.
 // A key that a column does not read has no part in it, finite or not: in a tile with such keys the values that are not finite are taken out of the
 // product and added to the columns that do read them.
@@ -33,6 +33,9 @@ typedef bf16 ShT;
 KP_STATUS_WORD(g_shared_status, shared)                // 0 ok; 1: a bounded wait gave up
 #endif
 
+// Keys of a box of own keys: of a sequence's last keys fewer come for nothing.  1424 tiles of columns with 19 to 34, heads of 256, boxes of 64 keys 77 us, of
+// 16 67.
+#define SH_OWN_BOX 16
 #define SH_WORKERS 128                                 // threads of the four warps that compute
 
 template <typename T, int HD, int BM, bool TMA>
@@ -42,11 +45,12 @@ struct Sh {
     static constexpr int KT = MMA ? 64 : 32;                                // keys a tile
     static constexpr int E = 16 / sizeof(T);                                // values of 16 bytes
     static constexpr int LD = HD + E;                                       // a row in shared memory: 16 bytes more, so that rows lie in different banks
-    static constexpr int TILE = KT * (TMA ? HD : LD);                       // values of K's tile, or of V's (TMA: 64 values a row, swizzled)
+    static constexpr int BW = HD % 64 ? 32 : 64;                            // values of a row of a TMA box
+    static constexpr int TILE = KT * (TMA ? HD : LD);                       // values of K's tile, or of V's (TMA: BW values a row, swizzled)
     static constexpr int CH = HD / E, NI = (KT * CH + SH_WORKERS - 1) / SH_WORKERS;
     static constexpr int PAIR = 2 * TILE * (int)sizeof(T);
     // (float32: few, so that there is room for three CTAs an SM: with one a warp has a scheduler to itself and issues in one cycle of three)
-    static constexpr int ST = TMA ? (HD == 64 ? 3 : 2) : !MMA ? (HD < 96 ? 3 : 2) : (4 * PAIR <= 100 * 1024 ? 4 : (3 * PAIR <= 110 * 1024 ? 3 : 2));
+    static constexpr int ST = TMA ? (HD == 32 ? 4 : (HD <= 96 ? 3 : 2)) : !MMA ? (HD < 96 ? 3 : 2) : (4 * PAIR <= 100 * 1024 ? 4 : (3 * PAIR <= 110 * 1024 ? 3 : 2));
     static constexpr int MR = BM / 8;                                       // columns of a thread (FMA)
     static constexpr int Q_BYTES = BM * LD * sizeof(T);
     static constexpr int RING = ST * PAIR;
@@ -55,7 +59,7 @@ struct Sh {
     static constexpr int LDO = HD + 4;                                      // (columns in different banks)
     static constexpr int O_BYTES = (PARTS > 1 ? PARTS + 1 : 1) * BM * LDO * 4;
     // CTAs an SM that registers are to allow: as many as shared memory does
-    static constexpr int CTAS = !TMA ? 1 : (BM <= 16 ? (HD == 64 ? 4 : (HD == 128 ? 3 : 1)) : (HD <= 128 ? 2 : 1));
+    static constexpr int CTAS = !TMA ? 1 : (BM <= 16 ? (HD <= 64 ? 4 : (HD <= 128 ? (BM == 8 ? 3 : 2) : (BM == 8 ? 2 : 1))) : (HD <= 128 ? 2 : 1));
     static constexpr int ML_BYTES = (PARTS + 1) * BM * 2 * 4;
     static constexpr int MAIN = RING > O_BYTES ? RING : O_BYTES;            // the output takes the ring's place
     static constexpr int PAD = TMA ? 1024 : 0;                              // the ring starts on a multiple of 1024 bytes
@@ -69,9 +73,9 @@ template <typename T, int HD, int BM, bool TMA>
 struct ShMem {
     typedef Sh<T, HD, BM, TMA> C;
     unsigned char* ring; T* Qs; unsigned char* P; float* ml; uint64_t* full; uint64_t* empty; float* wts;
-    __device__ __forceinline__ ShMem(unsigned char* smem) {
+    __device__ __forceinline__ ShMem(unsigned char* smem, int main) {
         ring = TMA ? reinterpret_cast<unsigned char*>(((uintptr_t)smem + 1023) & ~(uintptr_t)1023) : smem;
-        Qs = reinterpret_cast<T*>(ring + C::MAIN);
+        Qs = reinterpret_cast<T*>(ring + main);
         P = reinterpret_cast<unsigned char*>(Qs) + C::Q_BYTES;
         ml = reinterpret_cast<float*>(P + C::P_BYTES);
         full = reinterpret_cast<uint64_t*>(ml + C::ML_BYTES / 4);
@@ -102,43 +106,44 @@ __device__ __forceinline__ uint32_t sh_finite2(uint32_t r) {                // a
     return r;
 }
 
-// The loads of the keys k0 .. k1 - 1 of a block-table row, by a warp of their own: a box a page.  Tiles start at multiples of KT.
+// The loads of the keys k0 .. k1 - 1 of a block-table row, by a warp of their own: a box of p.box keys a lane, those that have any of them.  Tiles start at multiples of KT.
 template <typename T, int HD, int BM>
 __device__ __forceinline__ bool sh_load(const ShArgs& p, const CUtensorMap& tm, const ShMem<T, HD, BM, true>& sm, const int* bt, int g, int k0, int k1) {
     typedef Sh<T, HD, BM, true> C;
-    constexpr int KT = C::KT, ST = C::ST;
-    const int lane = threadIdx.x & 31, box = min(p.ps, KT), n_box = KT / box, t0 = k0 / KT, t1 = k1 > k0 ? (k1 + KT - 1) / KT : t0;
+    constexpr int KT = C::KT;
+    const int lane = threadIdx.x & 31, box = p.box, n_box = KT / box, t0 = k0 / KT, t1 = k1 > k0 ? (k1 + KT - 1) / KT : t0;
     auto page_of = [&](int t) {
         const int key = t * KT + lane * box;
         return t < t1 && lane < n_box && key < k1 && key + box > k0 ? __ldg(bt + sh_block(p, key)) : -1;
     };
-    int page = page_of(t0);
+    int page = page_of(t0), st = 0, round = 0;
     for (int t = t0; t < t1; t++) {
-        const int u = t - t0, st = u % ST, key = t * KT + lane * box;
-        if (!__all_sync(0xffffffffu, kp_mbar_wait_bounded(&sm.empty[st], ((u / ST) & 1) ^ 1))) return false;
+        const int key = t * KT + lane * box;
+        if (!__all_sync(0xffffffffu, kp_mbar_wait_bounded(&sm.empty[st], (round & 1) ^ 1))) return false;
         const bool mine = (unsigned)page < (unsigned long long)p.n_pages;  // (-1: not this lane's)
         const int count = __popc(__ballot_sync(0xffffffffu, mine));
         if (lane == 0) kp_mbar_expect_tx(&sm.full[st], 2 * count * box * HD * 2);
         __syncwarp();
         if (mine) {
             const int row = (page * 2 * p.G + g) * p.ps + (key - sh_block(p, key) * p.ps);
-            unsigned char* dst = sm.ring + st * C::PAIR + lane * box * 128;
+            unsigned char* dst = sm.ring + st * C::PAIR + lane * box * C::BW * 2;
 #pragma unroll
-            for (int y = 0; y < HD / 64; y++) {
-                kp_tma_load_2d(dst + y * KT * 128, &tm, y * 64, row, &sm.full[st]);
-                kp_tma_load_2d(dst + C::PAIR / 2 + y * KT * 128, &tm, y * 64, row + p.G * p.ps, &sm.full[st]);
+            for (int y = 0; y < HD / C::BW; y++) {
+                kp_tma_load_2d(dst + y * KT * C::BW * 2, &tm, y * C::BW, row, &sm.full[st]);
+                kp_tma_load_2d(dst + C::PAIR / 2 + y * KT * C::BW * 2, &tm, y * C::BW, row + p.G * p.ps, &sm.full[st]);
             }
         }
         __syncwarp();
+        if (++st == p.stages) { st = 0; round++; }
         page = page_of(t + 1);
     }
     return true;
 }
 
 // One tile of BM columns, of which `live` are there, through the keys k0 .. k1 - 1 of the block-table row bt, by the four warps; column c reads those below
-// lim(c) <= k1.  Leaves
+// lim(c) <= k1 (all of them those below k1 unless OWN).  Leaves
 // O [BM][HD] at the ring's place and (m, l) [BM] in ml.  False if a wait gave up.
-template <typename T, int HD, int BM, bool TMA, typename Lim>
+template <typename T, int HD, int BM, bool TMA, bool OWN, typename Lim>
 __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, TMA>& sm, const int* bt, int g, int live, int k0, int k1, int lim_min, Lim lim) {
     typedef Sh<T, HD, BM, TMA> C;
     constexpr int KT = C::KT, LD = C::LD, TILE = C::TILE, CH = C::CH, NI = C::NI, ST = C::ST, E = C::E;
@@ -181,9 +186,10 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
             cp_async_commit();
         }
     }
+    int st = 0, round = 0;                                                  // the tile's stage, and how often it has been used
     auto begin = [&](int t) {                                               // tile t is there
         if constexpr (TMA) {
-            if (ok && !kp_mbar_wait_bounded(&sm.full[t % ST], (t / ST) & 1)) ok = false;
+            if (ok && !kp_mbar_wait_bounded(&sm.full[st], round & 1)) ok = false;
         } else {
             cp_async_wait<ST - 2>();
             __syncthreads();
@@ -191,19 +197,21 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
             cp_async_commit();
         }
     };
-    auto end = [&](int t) {                                                 // and has been read
+    auto end = [&] {                                                        // and has been read
         if constexpr (TMA) {
             __syncwarp();
-            if (lane == 0) kp_mbar_arrive(&sm.empty[t % ST]);
+            if (lane == 0) kp_mbar_arrive(&sm.empty[st]);
         }
+        if (++st == (TMA ? p.stages : ST)) { st = 0; round++; }
     };
     auto finish = [&] {                                                     // the ring has been read: the output takes its place
         if constexpr (!TMA) cp_async_wait<0>();
         sh_sync_workers();
     };
-    // a value's place in a tile (TMA: rows of 64 values, 16-byte pieces in the order that the swizzle gives them)
+    // a value's place in a tile (TMA: rows of 64 or 32 values, 16-byte pieces in the order that the swizzle gives them)
     auto at_ = [&](const T* tile, int row, int col) {
-        return TMA ? tile + (col >> 6) * KT * 64 + row * 64 + ((((col & 63) >> 3) ^ (row & 7)) << 3) + (col & 7) : tile + row * LD + col;
+        if constexpr (!TMA) return tile + row * LD + col;
+        else return tile + col / C::BW * (KT * C::BW) + row * C::BW + ((col % C::BW / 8 ^ (C::BW == 64 ? row & 7 : (row >> 1) & 3)) << 3) + (col & 7);
     };
     const float sl2 = p.scale * 1.4426950408889634f;                        // scores in units of log2
 
@@ -236,7 +244,7 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
         }
         for (int t = 0; t < n_tiles; t++) {
             begin(t);
-            const T* Kt = ring + (t % ST) * 2 * TILE;
+            const T* Kt = ring + st * 2 * TILE;
             const T* Vt = Kt + TILE;
             const int key0 = base + t * KT + kw;
             float s[NT][4];
@@ -305,14 +313,16 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         a[e] &= keep[e >> 1];
-                        const uint32_t g_ = sh_finite2(a[e]);
-                        odd |= g_ != a[e];
-                        a[e] = g_;
+                        if constexpr (OWN) {
+                            const uint32_t g_ = sh_finite2(a[e]);
+                            odd |= g_ != a[e];
+                            a[e] = g_;
+                        }
                     }
 #pragma unroll
                 for (int n = 0; n < NT; n++) mma_bf16(o[d][n], a[0], a[1], a[2], a[3], b[n][0], b[n][1]);
             }
-            if (masked && __any_sync(0xffffffffu, odd)) {
+            if (OWN && masked && __any_sync(0xffffffffu, odd)) {
                 // values that are not finite, key by key, to the columns that read them
                 float* P = reinterpret_cast<float*>(Pbuf) + warp * 256;     // [column][16 keys]
 #pragma unroll
@@ -336,7 +346,7 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
                         }
                 __syncwarp();
             }
-            end(t);
+            end();
         }
         finish();
         constexpr int LDO = C::LDO;
@@ -393,7 +403,7 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
             for (int e = 0; e < 4; e++) o[d][e] = 0.f;
         for (int t = 0; t < n_tiles; t++) {
             begin(t);
-            const T* Kt = ring + (t % ST) * 2 * TILE;
+            const T* Kt = ring + st * 2 * TILE;
             const T* Vt = Kt + TILE;
             const int key0 = base + t * KT;
             float s[NK / 8][4];
@@ -417,6 +427,7 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
                 }
             }
             const bool masked = key0 + NK > lim_min || key0 < k0;
+            unsigned odd = 0;                                               // stretches of 16 keys that have values that are not finite
             float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NK / 8; j++)
@@ -462,7 +473,6 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
                         if (key < k0 || key >= k1) keep[h] &= 0xffff0000u;
                         if (key + 1 < k0 || key + 1 >= k1) keep[h] &= 0x0000ffffu;
                     }
-                bool odd = false;
 #pragma unroll
                 for (int d = 0; d < HD / 16; d++) {
                     uint32_t b[4];
@@ -471,22 +481,31 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             b[e] &= keep[e & 1];
-                            const uint32_t f = sh_finite2(b[e]);
-                            odd |= f != b[e];
-                            b[e] = f;
+                            if constexpr (OWN) {
+                                const uint32_t f = sh_finite2(b[e]);
+                                odd |= (unsigned)(f != b[e]) << j;
+                                b[e] = f;
+                            }
                         }
                     mma_bf16(o[2 * d], a[0], a[1], a[2], a[3], b[0], b[1]);
                     mma_bf16(o[2 * d + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
                 }
-                if (masked && __any_sync(0xffffffffu, odd)) {
-                    // values that are not finite, key by key, to the columns that read them
-                    float* P = reinterpret_cast<float*>(Pbuf) + warp * 256;
+            }
+            if constexpr (OWN) {
+                // values that are not finite, key by key, to the columns that read them
+                odd = __reduce_or_sync(0xffffffffu, odd);
+                float* P = reinterpret_cast<float*>(Pbuf) + warp * 256;
+#pragma unroll 1
+                for (int j = 0; odd >> j; j++) {
+                    if (!((odd >> j) & 1)) continue;
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            P[(lane >> 2) * 16 + h * 8 + (lane & 3) * 2 + e] = s[2 * j + h][e];
-                            P[((lane >> 2) + 8) * 16 + h * 8 + (lane & 3) * 2 + e] = s[2 * j + h][2 + e];
+                        for (int e = 0; e < 4; e++) {
+                            float w = s[h][e];
+#pragma unroll
+                            for (int i = 1; i < NK / 16; i++) w = i == j ? s[2 * i + h][e] : w;
+                            P[((lane >> 2) + (e >> 1) * 8) * 16 + h * 8 + (lane & 3) * 2 + (e & 1)] = w;
                         }
                     __syncwarp();
 #pragma unroll 1
@@ -507,7 +526,7 @@ __device__ __forceinline__ bool sh_tile(const ShArgs& p, const ShMem<T, HD, BM, 
                     __syncwarp();
                 }
             }
-            end(t);
+            end();
         }
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
@@ -657,7 +676,7 @@ __device__ __forceinline__ void sh_init(const ShMem<T, HD, BM, TMA>& sm) {
     }
 }
 // queries, loads and the tile by the warps whose work they are; then everyone has the output
-template <typename T, int HD, int BM, bool TMA, typename Lim>
+template <typename T, int HD, int BM, bool TMA, bool OWN, typename Lim>
 __device__ __forceinline__ void sh_work(const ShArgs& p, const CUtensorMap& tm, const ShMem<T, HD, BM, TMA>& sm, const int* bt, int g, int R, int row0, int n_cols, int c0,
                                         int k0, int k1, int lim_min, Lim lim) {
     bool ok = true;
@@ -665,7 +684,7 @@ __device__ __forceinline__ void sh_work(const ShArgs& p, const CUtensorMap& tm, 
         if constexpr (TMA) ok = sh_load(p, tm, sm, bt, g, k0, k1);
     } else {
         sh_queries<T, HD, BM, TMA>(p, sm.Qs, row0, n_cols, c0, g, R);
-        ok = sh_tile<T, HD, BM, TMA>(p, sm, bt, g, min(BM, n_cols - c0), k0, k1, lim_min, lim);
+        ok = sh_tile<T, HD, BM, TMA, OWN>(p, sm, bt, g, min(BM, n_cols - c0), k0, k1, lim_min, lim);
     }
     if (__builtin_expect(!ok, 0)) {
         atomicExch(&g_shared_status, 1);
@@ -680,7 +699,7 @@ __global__ void __launch_bounds__(Sh<T, HD, BM, TMA>::THREADS, Sh<T, HD, BM, TMA
 shared_prefix_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ ShArgs p) {
     kp_pdl_begin();
     extern __shared__ __align__(16) unsigned char smem[];
-    const ShMem<T, HD, BM, TMA> sm(smem);
+    const ShMem<T, HD, BM, TMA> sm(smem, p.main);
     const int chunk = blockIdx.x, g = blockIdx.y, group = blockIdx.z / p.tiles, c0 = blockIdx.z % p.tiles * BM, R = p.H / p.G;
     const int s0 = max(0, min(p.group_seqs[group], p.n_seq)), s1 = max(s0, min(p.group_seqs[group + 1], p.n_seq));
     const int P = sh_prefix(p, group), k0 = chunk * p.chunk, k1 = min(P, k0 + p.chunk);
@@ -689,7 +708,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm, const __grid_consta
     if (c0 >= n_cols) return;
     sh_init(sm);
     __syncthreads();
-    sh_work(p, tm, sm, p.table + (size_t)s0 * p.width, g, R, row0, n_cols, c0, k0, k1, k1, [&](int) { return k1; });
+    sh_work<T, HD, BM, TMA, false>(p, tm, sm, p.table + (size_t)s0 * p.width, g, R, row0, n_cols, c0, k0, k1, k1, [&](int) { return k1; });
     const float* O = reinterpret_cast<const float*>(sm.ring);
     for (int i = threadIdx.x; i < BM * HD / 4; i += Sh<T, HD, BM, TMA>::THREADS) {
         const int c = i / (HD / 4), d = i % (HD / 4) * 4, col = c0 + c;
@@ -710,7 +729,7 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     typedef Sh<T, HD, BM, TMA> C;
     constexpr int KT = C::KT, THREADS = C::THREADS;
     extern __shared__ __align__(16) unsigned char smem[];
-    const ShMem<T, HD, BM, TMA> sm(smem);
+    const ShMem<T, HD, BM, TMA> sm(smem, p.main);
     float* ml = sm.ml;
     float* wts = sm.wts;
     __shared__ int s_group, s_prefix, s_chunk;
@@ -733,7 +752,7 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
         const int end = max(P, (int)min((long long)last + 1, (long long)p.width * p.ps));
         const int t0 = P / KT, per = ((end + KT - 1) / KT - t0 + n_cl - 1) / n_cl;  // whole tiles of keys, and a CTA's
         const int k0 = min(end, max(P, (t0 + part * per) * KT)), k1 = min(end, (t0 + (part + 1) * per) * KT);
-        sh_work(p, tm, sm, p.table + (size_t)seq * p.width, g, R, row0, n_cols, c0, k0, k1, min(k1, pos0 + c0 / R + 1),
+        sh_work<T, HD, BM, TMA, true>(p, tm, sm, p.table + (size_t)seq * p.width, g, R, row0, n_cols, c0, k0, k1, min(k1, pos0 + c0 / R + 1),
                 [&](int c) { return min(k1, pos0 + (c0 + c) / R + 1); });
     }
     if (p.budget) {
@@ -804,8 +823,11 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
 }
 
 template <int HD, int BM, bool TMA>
-static int sh_prefix_launch(const CUtensorMap& tm, const ShArgs& a, cudaStream_t st) {
+static int sh_prefix_launch(const CUtensorMap& tm, ShArgs a, cudaStream_t st) {
     typedef Sh<ShT, HD, BM, TMA> C;
+    a.stages = C::ST;
+    a.main = C::MAIN;
+    a.box = min(a.ps, C::KT);
     static std::atomic<unsigned long long> ready{0};
     int e = kp_smem_limit(shared_prefix_kernel<ShT, HD, BM, TMA>, C::SMEM, ready, true);
     if (e) return e;
@@ -813,15 +835,20 @@ static int sh_prefix_launch(const CUtensorMap& tm, const ShArgs& a, cudaStream_t
     return c ? (int)c : kp_launch_status();
 }
 template <int HD, int BM, bool TMA>
-static int sh_own_launch(const CUtensorMap& tm, const ShArgs& a, int ctas, cudaStream_t st) {
+static int sh_own_launch(const CUtensorMap& tm, ShArgs a, int ctas, int own_keys, cudaStream_t st) {
     typedef Sh<ShT, HD, BM, TMA> C;
+    // No more stages than a CTA has tiles, so that more CTAs fit an SM: 1424 tiles of columns with 19 to 34 own keys, heads of 256, 102 us with two
+    // stages, 77 with one.
+    a.stages = TMA ? max(1, min(C::ST, (own_keys / ctas + C::KT - 1) / C::KT)) : C::ST;
+    a.main = max(a.stages * C::PAIR, C::O_BYTES);
+    a.box = min(a.ps, SH_OWN_BOX);
     static std::atomic<unsigned long long> ready{0};
     int e = kp_smem_limit(shared_own_kernel<ShT, HD, BM, TMA>, C::MOST, ready, true);
     if (e) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, a.G, a.n_seq * a.tiles);
     cfg.blockDim = dim3(C::THREADS);
-    cfg.dynamicSmemBytes = C::SMEM + (size_t)BM * (ctas + a.n_chunks) * 4;
+    cfg.dynamicSmemBytes = C::SMEM - C::MAIN + a.main + (size_t)BM * (ctas + a.n_chunks) * 4;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -834,7 +861,7 @@ static int sh_own_launch(const CUtensorMap& tm, const ShArgs& a, int ctas, cudaS
     return c ? (int)c : kp_launch_status();
 }
 template <int HD, bool TMA>
-static int sh_run_tma(const CUtensorMap& tm, ShArgs& a, int tile, int group_tiles, int own_tile, int own_tiles, int own_ctas, int with_prefix, cudaStream_t st) {
+static int sh_run_tma(const CUtensorMap& tm, const CUtensorMap& own, ShArgs& a, int tile, int group_tiles, int own_tile, int own_tiles, int own_ctas, int own_keys, int with_prefix, cudaStream_t st) {
     if (with_prefix) {
         a.tiles = group_tiles;
         int e;
@@ -848,41 +875,55 @@ static int sh_run_tma(const CUtensorMap& tm, ShArgs& a, int tile, int group_tile
     }
     a.tiles = own_tiles;
     switch (own_tile) {
-        case 8: return sh_own_launch<HD, 8, TMA>(tm, a, own_ctas, st);
-        case 16: return sh_own_launch<HD, 16, TMA>(tm, a, own_ctas, st);
-        case 32: return SH_32(sh_own_launch, tm, a, own_ctas, st);
-        default: return sh_own_launch<HD, 64, TMA>(tm, a, own_ctas, st);
+        case 8: return sh_own_launch<HD, 8, TMA>(own, a, own_ctas, own_keys, st);
+        case 16: return sh_own_launch<HD, 16, TMA>(own, a, own_ctas, own_keys, st);
+        case 32: return SH_32(sh_own_launch, own, a, own_ctas, own_keys, st);
+        default: return sh_own_launch<HD, 64, TMA>(own, a, own_ctas, own_keys, st);
     }
 }
+// the cache as rows of a key's (or value's) hd numbers of a head, in boxes of bw of them (32 or 64: swizzled over 64 or 128 bytes) by the keys of a page, `most` at
+// most
+static int sh_make_map(CUtensorMap* map, const ShArgs& a, int hd, int bw, int most) {
+    KpEncodeTiledFn fn = kp_encode_tiled_fn();
+    if (!fn) return KP_ERR_UNSUPPORTED;
+    cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)a.n_pages * 2 * a.G * a.ps}, strides[1] = {(cuuint64_t)hd * 2};
+    cuuint32_t box[2] = {(cuuint32_t)bw, (cuuint32_t)(a.ps < most ? a.ps : most)}, steps[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.cache), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              bw == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0 : KP_ERR_UNSUPPORTED;
+}
 template <int HD>
-static int sh_run(ShArgs& a, int tile, int group_tiles, int own_tile, int own_tiles, int own_ctas, int with_prefix, cudaStream_t st) {
+static int sh_run(ShArgs& a, int tile, int group_tiles, int own_tile, int own_tiles, int own_ctas, int own_keys, int with_prefix, cudaStream_t st) {
     alignas(64) CUtensorMap tm = {};
-    if constexpr (sizeof(ShT) == 2 && HD % 64 == 0) {
+    if constexpr (sizeof(ShT) == 2) {
         typedef Sh<ShT, HD, 16, true> C;
         if (a.ps % 8 == 0 && (a.ps % C::KT == 0 || C::KT % a.ps == 0) && a.n_pages * 2 * a.G * a.ps < 2147483647LL) {
-            const int e = kp_make_map_bf16_2d(&tm, a.cache, (unsigned long long)a.n_pages * 2 * a.G * a.ps, HD, HD, 64, a.ps < C::KT ? a.ps : C::KT);
+            alignas(64) CUtensorMap own;
+            int e = with_prefix ? sh_make_map(&tm, a, HD, C::BW, C::KT) : 0;
+            if (!e) e = sh_make_map(&own, a, HD, C::BW, SH_OWN_BOX);
             if (e) return e;
-            return sh_run_tma<HD, true>(tm, a, tile, group_tiles, own_tile, own_tiles, own_ctas, with_prefix, st);
+            return sh_run_tma<HD, true>(tm, own, a, tile, group_tiles, own_tile, own_tiles, own_ctas, own_keys, with_prefix, st);
         }
     }
-    return sh_run_tma<HD, false>(tm, a, tile, group_tiles, own_tile, own_tiles, own_ctas, with_prefix, st);
+    return sh_run_tma<HD, false>(tm, tm, a, tile, group_tiles, own_tile, own_tiles, own_ctas, own_keys, with_prefix, st);
 }
 
 // The first launch in its tcgen05 form (kp_attention_shared_prefix_tc)
 typedef int (*ShPrefixTc)(const void*, long long, const void*, long long, const int*, int, const int*, const int*, const int*, int, int, int, float*, float*, int, int,
                           float, int, int, int, int, int, int, int, int, void*);
 
-// tile, own_tile: columns of a tile, 8, 16, 32 (float32) or 64, of the first and of the second launch; n_chunks = 0: there is no prefix.  prefix_tc: the first
+// tile, own_tile: columns of a tile, 8, 16, 32 (float32) or 64, of the first and of the second launch; n_chunks = 0: there is no prefix; own_keys: a
+// sequence's own keys, about.  prefix_tc: the first
 // launch's tcgen05 form, or null; mode, budget: its arguments.
 extern "C" int SH_ENTRY(const void* q, long long ldq, const void* cache, long long n_pages, const int* table, int width, const int* cu_rows, const int* seg_pos,
                         const int* group_seqs, const int* prefix_len, int n, int n_seq, int n_groups, void* out, long long ldo, float* part_o,
                         float* part_ml, int n_chunks, int chunk, float scale, int ps, int H, int G, int hd, int max_prefix, int tile, int group_tiles,
-                        int own_tile, int own_tiles, int own_ctas, void* prefix_tc, int mode, int budget, void* stream) {
+                        int own_tile, int own_tiles, int own_ctas, int own_keys, void* prefix_tc, int mode, int budget, void* stream) {
     if (n <= 0 || n_seq <= 0) return 0;
     const int elt = sizeof(ShT), with_prefix = n_chunks > 0 && !prefix_tc, prefix_done = n_chunks > 0 && prefix_tc;
     if (G < 1 || G > 65535 || H < 1 || H % G || ps < 1 || width < 1 || (long long)width * ps > (1 << 30) || n_pages < 1 || n_groups < 0 || chunk < 1 ||
         n_chunks < 0 || n_chunks > SH_MAX_CHUNKS || ((with_prefix || prefix_done) && (n_chunks < 1 || (long long)n_chunks * chunk < max_prefix)) ||
-        (tile != 8 && tile != 16 && tile != 32 && tile != 64) || (own_tile != 8 && own_tile != 16 && own_tile != 32 && own_tile != 64) || group_tiles < 1 || own_tiles < 1 || own_ctas < 1 || own_ctas > SH_MAX_CLUSTER ||
+        (tile != 8 && tile != 16 && tile != 32 && tile != 64) || (own_tile != 8 && own_tile != 16 && own_tile != 32 && own_tile != 64) || group_tiles < 1 || own_tiles < 1 || own_ctas < 1 || own_ctas > SH_MAX_CLUSTER || own_keys < 0 ||
         (long long)n_groups * group_tiles > 65535 || (long long)n_seq * own_tiles > 65535 || ((uintptr_t)cache & 15) || ((uintptr_t)q & (elt - 1)) ||
         ((uintptr_t)out & (elt - 1)) || !(scale > 0.f) || (with_prefix && chunk % 64) || budget < 0 || (budget && (n_groups > 32 || (long long)n_groups * group_tiles * G > budget || chunk % 128)))
         return KP_ERR_BAD_ARG;
@@ -890,14 +931,14 @@ extern "C" int SH_ENTRY(const void* q, long long ldq, const void* cache, long lo
     for (int i = 0; i < 31; i++) if (ps == 1 << i) ps_log2 = i;
     ShArgs a = {q, ldq, ((uintptr_t)q & 15) == 0 && ldq * elt % 16 == 0, cache, n_pages, table, width, cu_rows, seg_pos, group_seqs, prefix_len, n, n_seq, n_groups,
                 out, ldo, ((uintptr_t)out & 15) == 0 && ldo * elt % 16 == 0, part_o, part_ml, n_chunks, chunk, prefix_done ? budget : 0, group_tiles, 1, !(with_prefix || prefix_done), scale, ps, ps_log2,
-                H, G, with_prefix || prefix_done ? max_prefix : 0};
+                H, G, with_prefix || prefix_done ? max_prefix : 0, 0, 0, 0};
     const cudaStream_t st = (cudaStream_t)stream;
     if (prefix_done) {
         const int e = ((ShPrefixTc)prefix_tc)(q, ldq, cache, n_pages, table, width, cu_rows, group_seqs, prefix_len, n, n_seq, n_groups, part_o, part_ml, n_chunks, chunk,
                                               scale, ps, H, G, hd, max_prefix, group_tiles, mode, budget, stream);
         if (e) return e;
     }
-#define SH_HD(D) case D: return sh_run<D>(a, tile, group_tiles, own_tile, own_tiles, own_ctas, with_prefix, st)
+#define SH_HD(D) case D: return sh_run<D>(a, tile, group_tiles, own_tile, own_tiles, own_ctas, own_keys, with_prefix, st)
     switch (hd) {
         SH_HD(32);
         SH_HD(64);

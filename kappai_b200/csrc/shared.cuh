@@ -33,6 +33,8 @@ struct ShArgs {
     int tiles;                                               // of columns, of a group (first launch) or of a sequence (second)
     int alone;                                               // second launch: there was no first one
     float scale; int ps, ps_log2; int H, G, max_prefix;
+    int box;                                                 // shared.cu: keys that a TMA load brings
+    int stages, main;                                        // and stages of the ring that there is room for, and the bytes that it (and later the output) has
 };
 
 __device__ __forceinline__ int sh_prefix(const ShArgs& p, int group) {

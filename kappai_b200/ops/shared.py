@@ -36,7 +36,7 @@ def _launcher(f32: bool):
     fn = _attention_shared.get(f32)
     if fn is None:
         fn = load_library("shared_f32").kp_attention_shared_f32 if f32 else load_library("shared").kp_attention_shared
-        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 10 + [_P, _I, _I, _P]
+        fn.argtypes = [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P, _I, _I, _F] + [_I] * 11 + [_P, _I, _I, _P]
         _attention_shared[f32] = fn
     return fn
 
@@ -57,17 +57,22 @@ class SharedCut(NamedTuple):
 
 @lru_cache(maxsize=4096)
 def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, max_prefix: int, max_own: int, G: int, R: int, tc: bool, f32: bool = False,
-               most: int = _MAX_CHUNKS) -> SharedCut:
+               most: int = _MAX_CHUNKS, hd: int = 64) -> SharedCut:
     """Keys are shared out until the SMs have work, none with less than a few tiles of keys, a prefix over at most ``most`` CTAs a tile of columns.  Tiles are
     no wider than the columns need."""
     def columns(n):
         return 8 if n <= 8 else (16 if n <= 16 else (32 if n <= 32 and f32 else 64))
 
-    own_tile = columns(max_rows * R)
-    own_tiles = -(-max_rows * R // own_tile)
-    own = (own_tile, own_tiles, max(1, min(-(-2 * _SMS // (n_seq * own_tiles * G)), _MAX_CLUSTER, -(-max_own // (96 if f32 else 384)))))
+    def own(chunks):
+        # (a cluster shares the join of its columns' parts as well as the keys; 64 columns take twice as long for a tile of keys as 8, and with wide heads want
+        # an SM for themselves beside the prefix's)
+        cols = max_rows * R
+        tile = columns(cols)
+        tiles, least = -(-cols // tile), 96 if f32 else (128 if tile == 64 else 384)
+        return tile, tiles, max(1, min(_SMS // (2 * n_seq * tiles * G) if tile == 64 and hd > 128 else -(-2 * _SMS // (n_seq * tiles * G)), _MAX_CLUSTER, max(-(-max_own // least), -(-chunks * min(cols, tile) // 256))))
+
     if not max_prefix:
-        return SharedCut(0, 0, 0, 1, 0, 64, *own)
+        return SharedCut(0, 0, 0, 1, 0, 64, *own(0))
     cols = max_group_rows * R
     if tc and cols > TC_MIN_COLS:
         mode = 2 if max_group_rows <= 64 // R else (1 if max_group_rows <= 128 // R else 0)
@@ -76,14 +81,14 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
         if 1 < n_groups <= 32 and items <= _SMS:
             # (a prefix that is all there is has the shortest chunks)
             least = max(-(-keys * tiles * G // _SMS), -(-keys // most))
-            return SharedCut(128, mode, _SMS, tiles, -(-keys // least), least * 128, *own)
+            return SharedCut(128, mode, _SMS, tiles, -(-keys // least), least * 128, *own(-(-keys // least)))
         chunk = -(-keys // min(max(1, _SMS // items), -(-keys // (2 if mode else 1)), most)) * 128
-        return SharedCut(128, mode, 0, tiles, -(-max_prefix // chunk), chunk, *own)
+        return SharedCut(128, mode, 0, tiles, -(-max_prefix // chunk), chunk, *own(-(-max_prefix // chunk)))
     tile = columns(cols)
     tiles = -(-cols // tile)
     chunks = max(1, min(-(-(3 if f32 else 2) * _SMS // (n_groups * tiles * G)), most, -(-max_prefix // (128 if f32 else 256))))
     chunk = -(-max_prefix // (chunks * 64)) * 64
-    return SharedCut(tile, 0, 0, tiles, -(-max_prefix // chunk), chunk, *own)
+    return SharedCut(tile, 0, 0, tiles, -(-max_prefix // chunk), chunk, *own(-(-max_prefix // chunk)))
 
 
 def shared_tc_ok(ldq: int, q: int, n_pages: int, page_size: int, G: int, R: int, hd: int) -> bool:
@@ -140,7 +145,7 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     if not n_groups:
         max_prefix = 0
     cut = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, R,
-                     not f32 and shared_tc_ok(ldq, pq, pages[0], page_size, G, R, hd), f32, max(1, min(_MAX_CHUNKS, _SCRATCH // (n * H * (hd + 2)))))
+                     not f32 and shared_tc_ok(ldq, pq, pages[0], page_size, G, R, hd), f32, max(1, min(_MAX_CHUNKS, _SCRATCH // (n * H * (hd + 2)))), hd)
     tile, mode, budget, tiles, chunks, chunk, own_tile, own_tiles, ctas = cut
     if n_groups * tiles > 65535 or n_seq * own_tiles > 65535 or G > 65535:
         raise KernelError(f"attention_shared: {n_seq} sequences in {n_groups} groups are more than a launch takes")
@@ -152,5 +157,5 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
         p1 = p0 + 4 * n * H * chunks * hd
     _run("attention_shared", _launcher(f32), pq, ldq, at, pages[0], block_table.data_ptr(), width, cu_rows.data_ptr(), seg_pos.data_ptr(), group_seqs.data_ptr(),
          prefix_len.data_ptr(), n, n_seq, n_groups, po, ldo, p0, p1, chunks, chunk, scale, page_size, H, G, hd, max_prefix, 64 if tc else (tile or 8), tiles, own_tile,
-         own_tiles, ctas, _tc_address() if tc else None, mode, budget, STREAM)
+         own_tiles, ctas, max_own, _tc_address() if tc else None, mode, budget, STREAM)
     return out
