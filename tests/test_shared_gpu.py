@@ -306,6 +306,21 @@ def test_pages_beyond_32_bit_offsets(dtype, ps):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("hd", SHARED_HEAD_DIMS)
+@pytest.mark.parametrize("ps", [8, 24, 64, 128])
+def test_heads_and_pages(hd, ps):
+    """Tiles by boxes of 32 and of 64 values, and copy by copy; few columns, more and many; own keys that end in their first tile of keys, or cross into a second."""
+    Batch([(100, spread(1, 60, 5))], 8, 2, hd, ps, "bf16", seed=hd + ps).check()
+    Batch([(333, spread(1, 3, 2, (1, 2))), (64, spread(30, 64, 9))], 6, 2, hd, ps, "bf16", seed=hd + ps).check()
+    Batch([(190, spread(5, 140, 3, (5, 1, 3)))], 16, 2, hd, ps, "bf16", seed=hd + ps).check()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_joins_of_many_parts(hd):
+    """Few sequences with many columns behind a long prefix: a cluster shares the join."""
+    Batch([(5000, spread(4, 20, 2, (4, 3)))], 16, 2, hd, 64, "bf16", seed=hd).check()
+
+
 def test_refusals():
     b = Batch([(40, spread(1, 9, 3))], 8, 2, 64, 16)
     ok = b.args()
