@@ -12,6 +12,9 @@
 // takes the second half of every tile's keys (P is zero in the other half), so that all warps have exponentials to do, half as many each: 24 rows of
 // two heads behind 120001 keys 62 us, 56 so.  What a column's copies have is joined through shared memory at the end.
 //
+// Bound by its loads with few columns (24 rows of two heads of 64 behind 120001 keys: 53 us in all, 6.2 TB/s while its tiles run), by the chain of a tile with many
+// (256 columns with heads of 128: 3 to 3.5 us a tile of 128 keys, of which products are 1.5).
+//
 // A column's reference m follows its largest score in steps of at least 2^8 (O is rescaled in tensor memory only then): weights are at most 2^8.  The
 // prefix's last page may hold anything behind the prefix: those scores are set to -inf, and the values' rows to zeros.  (All rows of a group read all of
 // the prefix: a value that is not finite belongs in every one of them.  Up to 64 columns an infinite one comes out as NaN, 0 times infinity.)
