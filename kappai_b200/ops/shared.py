@@ -85,6 +85,8 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
         chunk = -(-keys // min(max(1, _SMS // items), -(-keys // (2 if mode else 1)), most)) * 128
         return SharedCut(128, mode, 0, tiles, -(-max_prefix // chunk), chunk, *own(-(-max_prefix // chunk)))
     tile = columns(cols)
+    while f32 and tile > 16 and n_groups * -(-cols // tile) * G * -(-max_prefix // 128) < _SMS:
+        tile //= 2             # (few CTAs have narrower tiles: 20 rows of 6 heads of 256 behind 274 keys, 64 columns a tile 95 us, 16 62)
     tiles = -(-cols // tile)
     chunks = max(1, min(-(-(3 if f32 else 2) * _SMS // (n_groups * tiles * G)), most, -(-max_prefix // (128 if f32 else 256))))
     chunk = -(-max_prefix // (chunks * 64)) * 64
