@@ -51,7 +51,6 @@ class SharedCache:
         # the host's count
         self._length, self._own, self._prompt = [0] * max_seqs, [0] * max_seqs, [-1] * max_seqs       # (a sequence's prompt; its own number: it is one)
         self._groups: Dict[int, List[int]] = {}                     # prompt -> its live continuations
-        self._group_seqs = self._prefix = None
         self._free = self.n_pages
 
     # -- questions
@@ -79,30 +78,29 @@ class SharedCache:
         return -(-n // self.page_size)
 
     # -- changes
-    def _move(self, change: Dict[int, int], n_rows: int):
-        """The lengths' step on the device, and the same on the host: (positions, slots) of its rows."""
+    def _move(self, change: Dict[int, int], n_rows: int, beside: Sequence[int] = ()):
+        """The lengths' step on the device, and the same on the host: (positions, slots) of its rows, and the numbers ``beside``, which go to the
+        device in the same copy."""
         from ..ops.tables import page_tables
 
-        delta = np.zeros(len(self._length), dtype=np.int32)
+        n_seq = len(self._length)
+        numbers = np.zeros(n_seq + len(beside), dtype=np.int32)
         for s, d in change.items():
-            delta[s] = d
-        delta_d = self._upload(delta)
+            numbers[s] = d
+        numbers[n_seq:] = beside
+        numbers = self._upload(numbers)
+        delta_d = numbers[:n_seq]
         row_seg, positions, slots = torch.empty((3, n_rows), dtype=torch.int32, device=self.device).unbind(0)
         page_tables(self.block_table, self.lengths, delta_d, self.free_pages, self.n_free, self.page_size, self._cu, self._pos, row_seg, positions, slots,
                     self.status, own_from=self.own_from)
         for s, d in change.items():
             before, self._length[s] = self._blocks(self._length[s]), self._length[s] + d
             self._free -= max(self._blocks(self._length[s]), self._own[s]) - max(before, self._own[s])
-        return positions, slots
+        return positions, slots, numbers[n_seq:]
 
     def _upload(self, a) -> torch.Tensor:
         t = torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32))
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
-
-    def _regroup(self) -> None:
-        starts = sorted(self._groups)
-        both = self._upload(np.asarray(starts + [len(self._length)] + [self._length[p] for p in starts]))
-        self._group_seqs, self._prefix = both[:len(starts) + 1], both[len(starts) + 1:]
 
     def _room(self, pages: int) -> None:
         if pages > self._free:
@@ -155,7 +153,7 @@ class SharedCache:
         if at < 0:
             raise OutOfSlots(f"no {n + 1} sequences in a row are free")
         seqs = list(range(at + 1, at + 1 + n))
-        positions, slots = self._move({at: P}, P)
+        positions, slots, _ = self._move({at: P}, P)
         none = self._upload(np.zeros(1))
         out = self._attend(qkv, positions, slots, scale, group_seqs=none, prefix_len=none[:0], max_rows=P, max_group_rows=P,
                            max_prefix=0, max_own=P)
@@ -173,7 +171,6 @@ class SharedCache:
                 self._move({s: tail for s in part}, len(part) * tail)
             self.pages[self.block_table[rows, whole].long(), :, :, :tail] = self.pages[self.block_table[at, whole].long(), :, :, :tail]
         self._groups[at] = seqs
-        self._regroup()
         return out, list(seqs)
 
     @_on_its_device
@@ -194,13 +191,20 @@ class SharedCache:
         if max(after) > self.max_len:
             raise CacheError(f"step: a continuation of {max(after)} tokens, max_len={self.max_len}")
         self._room(sum(self._blocks(a) - max(self._blocks(self._length[s]), self._own[s]) for a, s in zip(after, seqs)))
-        positions, slots = self._move(dict(zip(seqs, rows)), sum(rows))
-        of: Dict[int, int] = {}
-        for s, r in zip(seqs, rows):
-            of[self._prompt[s]] = of.get(self._prompt[s], 0) + r
-        return self._attend(qkv, positions, slots, scale, group_seqs=self._group_seqs, prefix_len=self._prefix,
-                            max_rows=max(rows), max_group_rows=max(of.values()), max_prefix=max(self._length[p] for p in self._groups),
-                            max_own=max(a - self._length[self._prompt[s]] for a, s in zip(after, seqs)))
+        # Groups: stretches of these continuations that are of one prompt.  (A prompt that was forked into the places which ended continuations left stands
+        # among another's; what lies between a stretch's members, and up to the next stretch, has no rows.)
+        prompts = [self._prompt[s] for s in seqs]
+        starts, group_rows = [], []
+        for i, r in enumerate(rows):
+            if not i or prompts[i] != prompts[i - 1]:
+                starts.append(i)
+                group_rows.append(0)
+            group_rows[-1] += r
+        prefix = [self._length[prompts[i]] for i in starts]
+        positions, slots, groups = self._move(dict(zip(seqs, rows)), sum(rows), [seqs[i] for i in starts] + [len(self._length)] + prefix)
+        return self._attend(qkv, positions, slots, scale, group_seqs=groups[:len(starts) + 1], prefix_len=groups[len(starts) + 1:],
+                            max_rows=max(rows), max_group_rows=max(group_rows), max_prefix=max(prefix),
+                            max_own=max(a - self._length[p] for a, p in zip(after, prompts)))
 
     @_on_its_device
     def take_back(self, seqs: Sequence[int], tokens: Sequence[int]) -> None:
@@ -232,10 +236,6 @@ class SharedCache:
         for s in over:
             self._own[s], self._prompt[s] = 0, -1
         self._groups = kept
-        if kept:
-            self._regroup()
-        else:
-            self._group_seqs = self._prefix = None
 
     def check(self) -> None:
         """The device's count is the host's, and no page is lost or held twice (synchronises; for tests and doubts)."""

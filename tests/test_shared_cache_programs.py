@@ -1,0 +1,45 @@
+"""Programs over a SharedCache whose device calls are stand-ins on the CPU that do what their documentation says: which keys a continuation reads, and what a call
+leaves behind."""
+import pytest
+import torch
+
+import shared_fakes
+from shared_fakes import Program
+
+
+@pytest.fixture(autouse=True)
+def on_the_cpu(monkeypatch):
+    shared_fakes.install(monkeypatch)
+
+
+def near(got, want, off):
+    # the stand-in's sums are of 64 bits and rounded once, to float32 (2^-24 of a value)
+    assert (((got.double() - want).abs()) <= 1e-10 + 2.0 ** -24 * want.abs()).all()
+
+
+def program(seed=0, **kw):
+    a = dict(n_pages=200, max_seqs=16, max_len=400, page_size=8, dtype=torch.float32)
+    a.update(kw)
+    return Program(4, 2, 32, near, seed, **a)
+
+
+def test_a_fork_into_the_gap_that_ended_continuations_left():
+    """A second prompt among the first one's continuations: those behind it still read their own prompt."""
+    p = program()
+    a = p.fork(160, 8)
+    p.step()
+    p.end(a[1:5])
+    b = p.fork(32, 2)
+    assert a[0] < b[0] < a[5]
+    p.step()
+    p.step([a[0], b[1], a[5], a[7]], [1, 3, 2, 1])
+    p.end(b[:1])
+    p.step()
+    p.end(a[:1])
+    p.step()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_programs(seed):
+    p = program(seed, page_size=(8, 5, 16)[seed % 3], max_seqs=(12, 24)[seed % 2])
+    p.random(seed, 60, 90, 5)

@@ -1,0 +1,45 @@
+"""Random programs over a SharedCache on the device, against lists of keys and values and attention in 64 bits.
+
+Tolerances as in the attention's own tests: 1e-4 for float32; for bfloat16 2^-8 of the weighted mean of |v| and of the output beside it."""
+import pytest
+import torch
+
+from kappai_b200.ops import kernels as K
+from shared_fakes import Program
+
+pytestmark = pytest.mark.gpu
+
+
+def program(H, G, hd, seed=0, **kw):
+    a = dict(n_pages=300, max_seqs=16, max_len=700, page_size=16, dtype=torch.bfloat16)
+    a.update(kw)
+
+    def near(got, want, off):
+        assert ((got.double().cpu() - want).abs() <= 1e-4 + (2.0 ** -8 * off if got.dtype == torch.bfloat16 else 0.0 * off)).all()
+
+    return Program(H, G, hd, near, seed, device="cuda", **a)
+
+
+@pytest.mark.parametrize("dtype,H,G,hd", [(torch.bfloat16, 8, 2, 64), (torch.bfloat16, 16, 1, 128), (torch.float32, 4, 2, 64)])
+def test_a_fork_into_the_gap_that_ended_continuations_left(dtype, H, G, hd):
+    p = program(H, G, hd, dtype=dtype)
+    a = p.fork(160, 8)
+    p.step()
+    p.end(a[1:5])
+    b = p.fork(32, 2)
+    assert a[0] < b[0] < a[5]
+    p.step()
+    p.step([a[0], b[1], a[5], a[7]], [1, 3, 2, 1])
+    p.end(b[:1])
+    p.step()
+    p.end(a[:1])
+    p.step()
+
+
+@pytest.mark.parametrize("seed,dtype,H,G,hd,page", [(0, torch.bfloat16, 8, 2, 64, 16), (1, torch.bfloat16, 16, 1, 128, 64), (2, torch.float32, 4, 2, 64, 7),
+                                                    (3, torch.bfloat16, 6, 2, 96, 24), (4, torch.bfloat16, 32, 2, 64, 32)])
+def test_random_programs(seed, dtype, H, G, hd, page):
+    p = program(H, G, hd, seed, dtype=dtype, page_size=page, max_seqs=14)
+    p.random(seed, 70, 300, 6)
+    torch.cuda.synchronize()
+    assert not any(K.read_status().values())
