@@ -512,7 +512,7 @@ token_logprobs_kernel(const LpArgs p) {
             p.top_ids[at] = bad ? -1 : lp_index(k);
             p.top_logprobs[at] = bad ? S : logprob(lp_value(k));
         };
-        if (C == 1) {
+        if (C == 1 || bad) {                                         // (of numbers there may be fewer than alternatives then)
             if (tid < top) put(tid, s_sel[tid]);
         } else {
             for (int i = tid; i < n_all; i += LP_THREADS) s_cand[i] = *cluster.map_shared_rank(&s_sel[i % top], i / top);
