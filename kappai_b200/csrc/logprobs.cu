@@ -4,8 +4,8 @@
 // With a reference r, S = sum 2^y and W = sum 2^y y, y = (x - r) log2 e:  log p = x - r - ln S,  entropy = ln S - ln 2 W / S.  One pass over the
 // row carries (r, S, W) a thread in float32, y as one fma of x with r log2 e: whatever that is rounded to, it is the same for all.  r follows the thread's
 // maximum in steps of at least 16: with every new maximum rescaled, some lane of a warp had one at almost every piece.  Pieces with logits so far below
-// r that they have no probability (-inf, or the type's lowest value), and rows of nothing else, take differences x - r, bounded below, instead: 0 * inf does
-// not arise.  2048 rows of 65536 float32 logits: 85 us, 6.3 TB/s; with 5, 20 and 32 alternatives 99, 108 and 118; one row 4.6 us, 8.5 with alternatives.
+// r that they have no probability (-inf, or the type's lowest value) have y bounded below: 0 * inf does not arise.  References beyond +-1e6, those of rows of
+// nothing else among them, take differences x - r instead.  2048 rows of 65536 float32 logits: 85 us, 6.3 TB/s; with 5, 20 and 32 alternatives 99, 108 and 118; one row 4.6 us, 8.5 with alternatives.
 //
 // The alternatives need no second pass over the row.  A thread's values are a subset of the row, 64 bytes of every 16 KB.  The top-th largest of the maxima of
 // four subsets each is a bound below which no alternative lies, so only the subsets that reach it (few more than `top`) are read again, of these the pieces
@@ -112,14 +112,17 @@ __device__ __forceinline__ float lp_min3(float a, float b, float c) {
 }
 
 // A reference: r, and r log2 e as the fma takes it.  Beyond +-1e6 (`wild`) what that is rounded by would no longer be small beside the differences, and these
-// are taken themselves instead.
+// are taken themselves instead.  All terms of a sum are of one kind: what r log2 e was rounded by (`off`, up to 0.06) is put right for the sum as a whole.
 struct LpRef {
     float r, rl;
     __device__ __forceinline__ LpRef(float x) { r = x; rl = x * LP_LOG2E; }
     __device__ __forceinline__ bool wild() const { return !(fabsf(r) <= 1e6f); }
-    __device__ __forceinline__ float y(float x) const { return lp_max_nan(x - r, LP_LEAST) * LP_LOG2E; }     // by the difference
+    __device__ __forceinline__ float y(float x) const { return lp_max_nan(wild() ? (x - r) * LP_LOG2E : fmaf(x, LP_LOG2E, -rl), LP_LEAST); }
+    __device__ __forceinline__ float off() const { return wild() ? 0.f : fmaf(-r, LP_LOG2E, rl); }       // (exact: what a rounding leaves is a float32)
     // by how much less (a power of two) sums count that were relative to `o`, o.r <= r
-    __device__ __forceinline__ float from(const LpRef& o) const { return fmaxf(wild() || o.wild() ? (o.r - r) * LP_LOG2E : o.rl - rl, LP_LEAST); }
+    __device__ __forceinline__ float from(const LpRef& o) const {
+        return fmaxf(wild() || o.wild() ? (o.r - r) * LP_LOG2E + (o.off() - off()) : o.rl - rl, LP_LEAST);
+    }
 };
 // sums, and what becomes of them when their reference moves by y <= 0
 __device__ __forceinline__ void lp_move(float& s, float& w, float y) {
@@ -497,7 +500,7 @@ token_logprobs_kernel(const LpArgs p) {
         rank += *cluster.map_shared_rank(&s_count, i);
     }
     // The last differences are taken in 64 bits, each rounded once: r, log2 e and y = x log2 e - rl as they were rounded add up to (r log2 e - rl) in y.
-    const double off = z.wild() ? 0.0 : (double)z.rl - (double)z.r * (double)LP_LOG2E, log_s = log((double)S) + off * 0.6931471805599453;
+    const double off = (double)z.off(), log_s = log((double)S) + off * 0.6931471805599453;
     const bool bad = !(S >= 0.f), none = S == 0.f;                   // a NaN or +inf among the logits; nothing but -inf
     auto logprob = [&](float f) { return none ? -INFINITY : (float)(((double)f - (double)z.r) - log_s); };
     if (tid == 0) {
