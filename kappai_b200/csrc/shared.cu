@@ -702,7 +702,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm, const __grid_consta
     kp_pdl_begin();
     extern __shared__ __align__(16) unsigned char smem[];
     const ShMem<T, HD, BM, TMA> sm(smem, p.main);
-    const int chunk = blockIdx.x, g = blockIdx.y, group = blockIdx.z / p.tiles, c0 = blockIdx.z % p.tiles * BM, R = p.H / p.G;
+    const ShPlace at(p);
+    const int chunk = blockIdx.x, g = at.g, group = at.i / p.tiles, c0 = at.i % p.tiles * BM, R = p.H / p.G;
+    if (group >= p.n_groups) return;
     const int s0 = max(0, min(p.group_seqs[group], p.n_seq)), s1 = max(s0, min(p.group_seqs[group + 1], p.n_seq));
     const int P = sh_prefix(p, group), k0 = chunk * p.chunk, k1 = min(P, k0 + p.chunk);
     if (s0 == s1 || k0 >= k1) return;
@@ -715,9 +717,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tm, const __grid_consta
     for (int i = threadIdx.x; i < BM * HD / 4; i += Sh<T, HD, BM, TMA>::THREADS) {
         const int c = i / (HD / 4), d = i % (HD / 4) * 4, col = c0 + c;
         if (col >= n_cols) break;
-        const size_t at = ((size_t)(row0 + col / R) * p.H + g * R + col % R) * p.n_chunks + chunk;
-        *reinterpret_cast<float4*>(p.part_o + at * HD + d) = *reinterpret_cast<const float4*>(O + c * Sh<T, HD, BM, TMA>::LDO + d);
-        if (!d) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(sm.ml[2 * c], sm.ml[2 * c + 1]);
+        const size_t to = ((size_t)(row0 + col / R) * p.H + g * R + col % R) * p.n_chunks + chunk;
+        *reinterpret_cast<float4*>(p.part_o + to * HD + d) = *reinterpret_cast<const float4*>(O + c * Sh<T, HD, BM, TMA>::LDO + d);
+        if (!d) *reinterpret_cast<float2*>(p.part_ml + to * 2) = make_float2(sm.ml[2 * c], sm.ml[2 * c + 1]);
     }
 }
 
@@ -738,7 +740,9 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     __shared__ int s_group, s_prefix, s_chunk;
     cg::cluster_group cluster = cg::this_cluster();
     const int n_cl = gridDim.x, part = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int g = blockIdx.y, seq = blockIdx.z / p.tiles, c0 = blockIdx.z % p.tiles * BM, R = p.H / p.G;
+    const ShPlace at(p);
+    const int g = at.g, seq = at.i / p.tiles, c0 = at.i % p.tiles * BM, R = p.H / p.G;
+    if (seq >= p.n_seq) return;                              // (a whole cluster; the first place's CTAs wait for the first launch as all with rows do)
     sh_init(sm);
     if (tid == 0) s_group = -1;
     __syncthreads();
@@ -834,7 +838,7 @@ static int sh_prefix_launch(const CUtensorMap& tm, ShArgs a, cudaStream_t st) {
     static std::atomic<unsigned long long> ready{0};
     int e = kp_smem_limit(shared_prefix_kernel<ShT, HD, BM, TMA>, C::SMEM, ready, true);
     if (e) return e;
-    cudaError_t c = kp_launch_pdl(shared_prefix_kernel<ShT, HD, BM, TMA>, dim3(a.n_chunks, a.G, a.n_groups * a.tiles), dim3(C::THREADS), C::SMEM, st, tm, a);
+    cudaError_t c = kp_launch_pdl(shared_prefix_kernel<ShT, HD, BM, TMA>, sh_grid(a.n_chunks, a.G, a.n_groups * a.tiles), dim3(C::THREADS), C::SMEM, st, tm, a);
     return c ? (int)c : kp_launch_status();
 }
 template <int HD, int BM, bool TMA>
@@ -849,7 +853,7 @@ static int sh_own_launch(const CUtensorMap& tm, ShArgs a, int ctas, int own_keys
     int e = kp_smem_limit(shared_own_kernel<ShT, HD, BM, TMA>, C::MOST, ready, true);
     if (e) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, a.G, a.n_seq * a.tiles);
+    cfg.gridDim = sh_grid(ctas, a.G, a.n_seq * a.tiles);
     cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM - C::MAIN + a.main + (size_t)BM * (ctas + a.n_chunks) * 4;
     cfg.stream = st;
@@ -924,10 +928,10 @@ extern "C" int SH_ENTRY(const void* q, long long ldq, const void* cache, long lo
                         int own_tile, int own_tiles, int own_ctas, int own_keys, void* prefix_tc, int mode, int budget, void* stream) {
     if (n <= 0 || n_seq <= 0) return 0;
     const int elt = sizeof(ShT), with_prefix = n_chunks > 0 && !prefix_tc, prefix_done = n_chunks > 0 && prefix_tc;
-    if (G < 1 || G > 65535 || H < 1 || H % G || ps < 1 || width < 1 || (long long)width * ps > (1 << 30) || n_pages < 1 || n_groups < 0 || chunk < 1 ||
+    if (G < 1 || H < 1 || H % G || ps < 1 || width < 1 || (long long)width * ps > (1 << 30) || n_pages < 1 || n_groups < 0 || chunk < 1 ||
         n_chunks < 0 || n_chunks > SH_MAX_CHUNKS || ((with_prefix || prefix_done) && (n_chunks < 1 || (long long)n_chunks * chunk < max_prefix)) ||
         (tile != 8 && tile != 16 && tile != 32 && tile != 64) || (own_tile != 8 && own_tile != 16 && own_tile != 32 && own_tile != 64) || group_tiles < 1 || own_tiles < 1 || own_ctas < 1 || own_ctas > SH_MAX_CLUSTER || own_keys < 0 ||
-        (long long)n_groups * group_tiles > 65535 || (long long)n_seq * own_tiles > 65535 || ((uintptr_t)cache & 15) || ((uintptr_t)q & (elt - 1)) ||
+        !sh_grid_ok(n_groups, group_tiles, G) || !sh_grid_ok(n_seq, own_tiles, G) || ((uintptr_t)cache & 15) || ((uintptr_t)q & (elt - 1)) ||
         ((uintptr_t)out & (elt - 1)) || !(scale > 0.f) || (with_prefix && chunk % 64) || budget < 0 || (budget && (n_groups > 32 || (long long)n_groups * group_tiles * G > budget || chunk % 128)))
         return KP_ERR_BAD_ARG;
     int ps_log2 = -1;

@@ -19,6 +19,15 @@
 #define SH_MAX_CHUNKS 64
 #define SH_MAX_CLUSTER 8
 
+// The grid of a launch: x, kv heads, and places (a group's or a sequence's tiles of columns).  The third axis ends at 65535: places beyond that stand beside
+// the others on the second one, the last of them perhaps too many.
+#define SH_AXIS 65535
+static inline dim3 sh_grid(int x, int G, int places) { return places <= SH_AXIS ? dim3(x, G, places) : dim3(x, G * ((places + SH_AXIS - 1) / SH_AXIS), SH_AXIS); }
+static inline bool sh_grid_ok(int n, int tiles, int G) {
+    const long long places = (long long)n * tiles;
+    return places < 2147483647LL - SH_AXIS && (places + SH_AXIS - 1) / SH_AXIS * G <= SH_AXIS;
+}
+
 struct ShArgs {
     const void* q; long long ldq; int q_vec;                 // q_vec: rows start on 16-byte boundaries
     const void* cache; long long n_pages;
@@ -37,6 +46,14 @@ struct ShArgs {
     int stages, main;                                        // and stages of the ring that there is room for, and the bytes that it (and later the output) has
 };
 
+struct ShPlace {                                             // a CTA's kv head and place
+    int g, i;
+    __device__ __forceinline__ ShPlace(const ShArgs& p) {
+        g = blockIdx.y;
+        i = blockIdx.z;
+        if (gridDim.y != p.G) { i += g / p.G * SH_AXIS; g %= p.G; }
+    }
+};
 __device__ __forceinline__ int sh_prefix(const ShArgs& p, int group) {
     return max(0, min(min(p.prefix_len[group], p.max_prefix), p.width * p.ps));
 }

@@ -81,7 +81,7 @@ __device__ __forceinline__ void sc_store32(float* dst, float4 a, float4 b) {
 }
 __device__ __forceinline__ void sc_sync_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// grid: (chunks of a prefix, kv heads, groups x tiles of columns), or with a budget so many CTAs, which find theirs
+// grid: chunks of a prefix, kv heads, groups x tiles of columns (sh_grid), or with a budget so many CTAs, which find theirs
 template <int HD, int MODE>
 __global__ void __launch_bounds__(SC_THREADS, 1)
 shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ ShArgs p) {
@@ -103,7 +103,8 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     kp_pdl_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int R = p.H / p.G, T = C::COLS / R;
-    int chunk = blockIdx.x, kvh = blockIdx.y, group = blockIdx.z / p.tiles, tile = blockIdx.z % p.tiles;
+    const ShPlace place(p);
+    int chunk = blockIdx.x, kvh = place.g, group = place.i / p.tiles, tile = place.i % p.tiles;
     const int chunk_keys = sh_chunk(p, lane);
     if (p.budget) {
         // this CTA's place in the list of (group, chunk, tile, kv head)
@@ -118,7 +119,7 @@ shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         chunk = at / per;
         tile = at % per / p.G;
         kvh = at % p.G;
-    }
+    } else if (group >= p.n_groups) return;
     const int g0 = p.group_seqs[group], g1 = p.group_seqs[group + 1], P = sh_prefix(p, group);
     const int s0 = max(0, min(g0, p.n_seq)), s1 = max(s0, min(g1, p.n_seq));
     if (s0 == s1) return;
@@ -414,7 +415,7 @@ static int sc_launch(const ShArgs& a, const CUtensorMap& tq, const CUtensorMap& 
     static std::atomic<unsigned long long> ready{0};
     int e = kp_smem_limit(shared_prefix_tc_kernel<HD, MODE>, Sc<HD, MODE>::SMEM, ready);
     if (e) return e;
-    const dim3 grid = a.budget ? dim3(a.budget) : dim3(a.n_chunks, a.G, a.n_groups * a.tiles);
+    const dim3 grid = a.budget ? dim3(a.budget) : sh_grid(a.n_chunks, a.G, a.n_groups * a.tiles);
     cudaError_t c = kp_launch_pdl(shared_prefix_tc_kernel<HD, MODE>, grid, dim3(SC_THREADS), Sc<HD, MODE>::SMEM, st, tq, tc, a);
     return c ? (int)c : kp_launch_status();
 }
@@ -425,9 +426,9 @@ extern "C" int kp_attention_shared_prefix_tc(const void* q, long long ldq, const
                                              const int* group_seqs, const int* prefix_len, int n, int n_seq, int n_groups, float* part_o, float* part_ml, int n_chunks,
                                              int chunk, float scale, int ps, int H, int G, int hd, int max_prefix, int tiles, int mode, int budget, void* stream) {
     if (n <= 0 || n_seq <= 0 || n_groups <= 0 || max_prefix <= 0) return 0;
-    if (G < 1 || G > 65535 || H < 1 || H % G || mode < 0 || mode > 2 || H / G > (mode == 2 ? 64 : 128) || ps < 8 || ps % 8 || !(ps % SC_KEYS == 0 || SC_KEYS % ps == 0) ||
+    if (G < 1 || H < 1 || H % G || mode < 0 || mode > 2 || H / G > (mode == 2 ? 64 : 128) || ps < 8 || ps % 8 || !(ps % SC_KEYS == 0 || SC_KEYS % ps == 0) ||
         width < 1 || (long long)width * ps > (1 << 30) || n_pages < 1 || n_pages * 2 * G * ps >= 2147483647LL || chunk < SC_KEYS || chunk % SC_KEYS || n_chunks < 1 ||
-        n_chunks > SH_MAX_CHUNKS || (long long)n_chunks * chunk < max_prefix || tiles < 1 || (long long)n_groups * tiles > 65535 || (ldq & 7) || !(scale > 0.f) ||
+        n_chunks > SH_MAX_CHUNKS || (long long)n_chunks * chunk < max_prefix || tiles < 1 || !sh_grid_ok(n_groups, tiles, G) || (ldq & 7) || !(scale > 0.f) ||
         (((uintptr_t)q | (uintptr_t)cache) & 15) || ((uintptr_t)part_o & 31) || (hd != 64 && hd != 128) || budget < 0 ||
         (budget && (n_groups > 32 || (long long)n_groups * tiles * G > budget)))
         return KP_ERR_UNSUPPORTED;

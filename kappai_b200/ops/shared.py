@@ -15,6 +15,7 @@ SHARED_HEAD_DIMS = (32, 64, 96, 128, 192, 256)
 SHARED_MAX_KEYS = 1 << 30      # that a block table has room for: the kernels count keys in 32 bits
 _SMS = 148
 _MAX_CHUNKS, _MAX_CLUSTER = 64, 8
+_AXIS = 65535                  # a grid's second and third axis
 _SCRATCH = 1 << 28             # values of scratch above which a prefix is cut into fewer chunks
 TC_MIN_COLS = 16               # columns of a group above which the tcgen05 form takes its prefix
 
@@ -149,7 +150,7 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     cut = shared_cut(max(1, n_groups), n_seq, min(max_rows, n), min(max_group_rows, n), max_prefix, max_own, G, R,
                      not f32 and shared_tc_ok(ldq, pq, pages[0], page_size, G, R, hd), f32, max(1, min(_MAX_CHUNKS, _SCRATCH // (n * H * (hd + 2)))), hd)
     tile, mode, budget, tiles, chunks, chunk, own_tile, own_tiles, ctas = cut
-    if n_groups * tiles > 65535 or n_seq * own_tiles > 65535 or G > 65535:
+    if -(-max(n_groups * tiles, n_seq * own_tiles) // _AXIS) * G > _AXIS or max(n_groups * tiles, n_seq * own_tiles) >= 2 ** 31 - 2 ** 16:
         raise KernelError(f"attention_shared: {n_seq} sequences in {n_groups} groups are more than a launch takes")
     tc = tile == 128
     p0 = p1 = scratch = None
