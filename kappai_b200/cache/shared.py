@@ -106,15 +106,16 @@ class SharedCache:
         if pages > self._free:
             raise OutOfPages(f"need {pages} pages, {self._free} free")
 
-    def _attend(self, qkv, positions, slots, scale, **bounds) -> torch.Tensor:
+    def _attend(self, qkv, positions, slots, scale, lo: int, hi: int, **bounds) -> torch.Tensor:
+        """The rows' attention; ``lo`` to ``hi`` - 1 are the sequences that may have any, and groups count from ``lo``."""
         from ..ops.kernels import qk_norm_rope_kv
         from ..ops.shared import attention_shared
 
         H, G, hd = self.H, self.G, self.hd
         q = torch.empty((qkv.shape[0], H * hd), dtype=qkv.dtype, device=qkv.device)
         qk_norm_rope_kv(qkv, None, None, 0.0, None, None, 0, False, positions, slots, q, self.pages, self.page_size, H, G, hd)
-        return attention_shared(q, self.pages, self.block_table, self._cu, self._pos, out=torch.empty_like(q), scale=scale, page_size=self.page_size, H=H, G=G, hd=hd,
-                                **bounds)
+        return attention_shared(q, self.pages, self.block_table[lo:hi], self._cu[lo:hi + 1], self._pos[lo:hi], out=torch.empty_like(q), scale=scale,
+                                page_size=self.page_size, H=H, G=G, hd=hd, **bounds)
 
     def _scale(self, scale: Optional[float], what: str) -> float:
         if scale is None:
@@ -155,7 +156,7 @@ class SharedCache:
         seqs = list(range(at + 1, at + 1 + n))
         positions, slots, _ = self._move({at: P}, P)
         none = self._upload(np.zeros(1))
-        out = self._attend(qkv, positions, slots, scale, group_seqs=none, prefix_len=none[:0], max_rows=P, max_group_rows=P,
+        out = self._attend(qkv, positions, slots, scale, at, at + 1, group_seqs=none, prefix_len=none[:0], max_rows=P, max_group_rows=P,
                            max_prefix=0, max_own=P)
         # the continuations' tables begin with the prompt's whole pages; a page that it ends in each has for itself
         rows = slice(at + 1, at + 1 + n)
@@ -200,9 +201,9 @@ class SharedCache:
                 starts.append(i)
                 group_rows.append(0)
             group_rows[-1] += r
-        prefix = [self._length[prompts[i]] for i in starts]
-        positions, slots, groups = self._move(dict(zip(seqs, rows)), sum(rows), [seqs[i] for i in starts] + [len(self._length)] + prefix)
-        return self._attend(qkv, positions, slots, scale, group_seqs=groups[:len(starts) + 1], prefix_len=groups[len(starts) + 1:],
+        prefix, lo, hi = [self._length[prompts[i]] for i in starts], seqs[0], seqs[-1] + 1
+        positions, slots, groups = self._move(dict(zip(seqs, rows)), sum(rows), [seqs[i] - lo for i in starts] + [hi - lo] + prefix)
+        return self._attend(qkv, positions, slots, scale, lo, hi, group_seqs=groups[:len(starts) + 1], prefix_len=groups[len(starts) + 1:],
                             max_rows=max(rows), max_group_rows=max(group_rows), max_prefix=max(prefix),
                             max_own=max(a - self._length[p] for a, p in zip(after, prompts)))
 

@@ -43,3 +43,24 @@ def test_a_fork_into_the_gap_that_ended_continuations_left():
 def test_random_programs(seed):
     p = program(seed, page_size=(8, 5, 16)[seed % 3], max_seqs=(12, 24)[seed % 2])
     p.random(seed, 60, 90, 5)
+
+
+def test_a_call_takes_no_more_sequences_than_may_have_rows(monkeypatch):
+    """Spare places of the cache are not in the attention's way, and its work is cut for those that are."""
+    from kappai_b200.ops import shared
+
+    took = []
+
+    def attention_shared(q, cache, block_table, cu_rows, seg_pos, *args, **kw):
+        took.append(seg_pos.numel())
+        return shared_fakes.attention_shared(q, cache, block_table, cu_rows, seg_pos, *args, **kw)
+
+    monkeypatch.setattr(shared, "attention_shared", attention_shared)
+    p = program(max_seqs=257)
+    a = p.fork(40, 8)
+    b = p.fork(9, 20)
+    p.step()
+    p.step(a)
+    p.step([a[2], a[5]], [2, 1])
+    p.step(b[-1:])
+    assert took == [1, 1, b[-1] - a[0] + 1, 8, a[5] - a[2] + 1, 1]

@@ -43,3 +43,27 @@ def test_random_programs(seed, dtype, H, G, hd, page):
     p.random(seed, 70, 300, 6)
     torch.cuda.synchronize()
     assert not any(K.read_status().values())
+
+
+@pytest.mark.parametrize("P,n,H,G,hd", [(4096, 256, 32, 8, 128), (8000, 256, 32, 8, 64), (3001, 8000, 16, 2, 64)])
+def test_long_prompts_in_caches_of_many_places(P, n, H, G, hd):
+    """The prompt's rows, and a step of all of its continuations, whatever the cache has room for besides."""
+    p = program(H, G, hd, page_size=64, max_len=P + 64, n_pages=P // 64 + 2 * n + 10, max_seqs=min(8192, 2 * n))
+    x, some = p.make(P), [0, 1, 63, 64, 1000, P - 2, P - 1]
+    out, seqs = p.c.fork(x, n)
+    want, off, whole = p.attend(None, x, some)
+    p.near(out[some], want, off)
+    y = p.make(n)
+    out = p.c.step(y)
+    for i in (0, 1, n // 2, n - 1):
+        want, off, _ = p.attend(whole, y[i:i + 1])
+        p.near(out[i:i + 1], want, off)
+    p.c.end(seqs[:n // 2])
+    p.kv = {s: torch.cat([whole, y[i:i + 1, H * hd:].double().cpu().reshape(1, 2, G, hd)]) for i, s in enumerate(seqs) if i in (n // 2, n - 1)}
+    p.prompt_of = dict.fromkeys(p.kv)
+    z = p.make(3)
+    out = p.c.step(z, [seqs[n // 2], seqs[n - 1]], [1, 2])
+    for s, a, b in ((seqs[n // 2], 0, 1), (seqs[n - 1], 1, 3)):
+        want, off, _ = p.attend(p.kv[s], z[a:b])
+        p.near(out[a:b], want, off)
+    p.c.check()
