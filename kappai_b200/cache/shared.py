@@ -98,6 +98,14 @@ class SharedCache:
             self._free -= max(self._blocks(self._length[s]), self._own[s]) - max(before, self._own[s])
         return positions, slots, numbers[n_seq:]
 
+    def _forget(self, over: Sequence[int]) -> None:
+        """These sequences are no more, whatever they had got."""
+        index = self._upload(np.asarray(over)).long()
+        self._move({s: -self._length[s] for s in over if self._length[s]}, 0)
+        self.own_from.index_fill_(0, index, 0)
+        for s in over:
+            self._own[s], self._prompt[s] = 0, -1
+
     def _upload(self, a) -> torch.Tensor:
         t = torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32))
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
@@ -137,7 +145,7 @@ class SharedCache:
     def fork(self, qkv: torch.Tensor, n: int, scale: Optional[float] = None) -> Tuple[torch.Tensor, List[int]]:
         """A prompt's rows [tokens, (num_heads + 2 num_kv_heads) * head_dim] (queries, keys, values), and ``n`` continuations of it: the rows'
         causal attention [tokens, num_heads * head_dim], and the continuations' numbers.  ``scale``: head_dim ** -0.5 unless given.  Nothing is taken
-        where the pages do not suffice (:class:`~.manager.OutOfPages`) or no ``n + 1`` sequences in a row are free (:class:`~.manager.OutOfSlots`)."""
+        by a call that fails, for instance where the pages do not suffice (:class:`~.manager.OutOfPages`) or no ``n + 1`` sequences in a row are free (:class:`~.manager.OutOfSlots`)."""
         P = qkv.shape[0] if isinstance(qkv, torch.Tensor) and qkv.dim() == 2 else 0
         if P < 1 or n < 1 or P > self.max_len:
             raise CacheError(f"fork: a prompt of {P} tokens (at most {self.max_len}) with {n} continuations")
@@ -154,23 +162,28 @@ class SharedCache:
         if at < 0:
             raise OutOfSlots(f"no {n + 1} sequences in a row are free")
         seqs = list(range(at + 1, at + 1 + n))
-        positions, slots, _ = self._move({at: P}, P)
-        none = self._upload(np.zeros(1))
-        out = self._attend(qkv, positions, slots, scale, at, at + 1, group_seqs=none, prefix_len=none[:0], max_rows=P, max_group_rows=P,
-                           max_prefix=0, max_own=P)
-        # the continuations' tables begin with the prompt's whole pages; a page that it ends in each has for itself
-        rows = slice(at + 1, at + 1 + n)
-        self.block_table[rows, :whole] = self.block_table[at, :whole]
-        self.own_from[rows] = whole
-        self.lengths[rows] = whole * self.page_size
-        for s in seqs:
-            self._length[s], self._own[s], self._prompt[s] = whole * self.page_size, whole, at
-        self._prompt[at] = at
-        if tail:
-            for a in range(0, n, self._most // tail):               # (as many rows as a call takes)
-                part = seqs[a:a + self._most // tail]
-                self._move({s: tail for s in part}, len(part) * tail)
-            self.pages[self.block_table[rows, whole].long(), :, :, :tail] = self.pages[self.block_table[at, whole].long(), :, :, :tail]
+        try:
+            positions, slots, _ = self._move({at: P}, P)
+            none = self._upload(np.zeros(1))
+            out = self._attend(qkv, positions, slots, scale, at, at + 1, group_seqs=none, prefix_len=none[:0], max_rows=P, max_group_rows=P,
+                               max_prefix=0, max_own=P)
+            # the continuations' tables begin with the prompt's whole pages; a page that it ends in each has for itself
+            rows = slice(at + 1, at + 1 + n)
+            self.block_table[rows, :whole] = self.block_table[at, :whole]
+            self.own_from[rows] = whole
+            self.lengths[rows] = whole * self.page_size
+            for s in seqs:
+                self._length[s], self._own[s] = whole * self.page_size, whole
+            if tail:
+                for a in range(0, n, self._most // tail):           # (as many rows as a call takes)
+                    part = seqs[a:a + self._most // tail]
+                    self._move({s: tail for s in part}, len(part) * tail)
+                self.pages[self.block_table[rows, whole].long(), :, :, :tail] = self.pages[self.block_table[at, whole].long(), :, :, :tail]
+        except BaseException:
+            self._forget([at] + seqs)
+            raise
+        for s in [at] + seqs:
+            self._prompt[s] = at
         self._groups[at] = seqs
         return out, list(seqs)
 
@@ -178,7 +191,7 @@ class SharedCache:
     def step(self, qkv: torch.Tensor, seqs: Optional[Sequence[int]] = None, rows: Optional[Sequence[int]] = None, scale: Optional[float] = None) -> torch.Tensor:
         """The next ``rows[i]`` (None: one each) tokens of ``seqs[i]`` (None: all that are live; ascending): their keys and values join the cache, and what is
         returned is each row's causal attention over its prompt and its own continuation, [rows, num_heads * head_dim].  All get their pages or
-        none does."""
+        none does, and a call that fails leaves everything as it was."""
         seqs = self.live() if seqs is None else list(seqs)
         self._check(seqs, "step")
         rows = [1] * len(seqs) if rows is None else [int(r) for r in rows]
@@ -203,9 +216,13 @@ class SharedCache:
             group_rows[-1] += r
         prefix, lo, hi = [self._length[prompts[i]] for i in starts], seqs[0], seqs[-1] + 1
         positions, slots, groups = self._move(dict(zip(seqs, rows)), sum(rows), [seqs[i] - lo for i in starts] + [hi - lo] + prefix)
-        return self._attend(qkv, positions, slots, scale, lo, hi, group_seqs=groups[:len(starts) + 1], prefix_len=groups[len(starts) + 1:],
-                            max_rows=max(rows), max_group_rows=max(group_rows), max_prefix=max(prefix),
-                            max_own=max(a - self._length[p] for a, p in zip(after, prompts)))
+        try:
+            return self._attend(qkv, positions, slots, scale, lo, hi, group_seqs=groups[:len(starts) + 1], prefix_len=groups[len(starts) + 1:],
+                                max_rows=max(rows), max_group_rows=max(group_rows), max_prefix=max(prefix),
+                                max_own=max(a - self._length[p] for a, p in zip(after, prompts)))
+        except BaseException:
+            self._move({s: -r for s, r in zip(seqs, rows)}, 0)
+            raise
 
     @_on_its_device
     def take_back(self, seqs: Sequence[int], tokens: Sequence[int]) -> None:
@@ -230,12 +247,7 @@ class SharedCache:
         if not over:
             return
         kept = {p: [s for s in c if s not in gone] for p, c in self._groups.items() if p not in prompts}
-        change = {s: -self._length[s] for s in over}
-        self._move(change, 0)
-        index = self._upload(np.asarray(over)).long()
-        self.own_from[index] = 0
-        for s in over:
-            self._own[s], self._prompt[s] = 0, -1
+        self._forget(over)
         self._groups = kept
 
     def check(self) -> None:

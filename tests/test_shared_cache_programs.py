@@ -64,3 +64,54 @@ def test_a_call_takes_no_more_sequences_than_may_have_rows(monkeypatch):
     p.step([a[2], a[5]], [2, 1])
     p.step(b[-1:])
     assert took == [1, 1, b[-1] - a[0] + 1, 8, a[5] - a[2] + 1, 1]
+
+
+class Refused(Exception):
+    pass
+
+
+@pytest.mark.parametrize("P", [24, 29])                  # whole pages, and a page that each continuation has a copy of
+@pytest.mark.parametrize("what,call", [("page_tables", 1), ("page_tables", 2), ("qk_norm_rope_kv", 1), ("attention_shared", 1), ("copy", 1)])
+def test_a_call_that_fails_leaves_everything_as_it_was(what, call, P, monkeypatch):
+    """Whatever of a fork's or a step's calls refuses: pages, lengths and places are those of before, and what comes next is right."""
+    from kappai_b200.ops import kernels, shared, tables
+
+    p = program()
+    a, c, armed = p.fork(21, 3), p.c, [0]
+    p.step()
+
+    def refusing(run):
+        def counted(*args, **kw):
+            armed[0] -= 1
+            if armed[0] == 0:
+                raise Refused
+            return run(*args, **kw)
+        return counted
+
+    def state():
+        return c.pages_free, list(c._length), list(c._own), list(c._prompt), c.live(), sorted(c.free_pages[:c._free].tolist())
+
+    kept = state()
+    if what == "copy":                                   # (the keys' own writing is the first one to the pages)
+        plain, copy = torch.Tensor.__setitem__, refusing(torch.Tensor.__setitem__)
+        monkeypatch.setattr(torch.Tensor, "__setitem__", lambda self, *args: (copy if self is c.pages else plain)(self, *args))
+        call = 2
+    else:
+        monkeypatch.setattr({"qk_norm_rope_kv": kernels, "attention_shared": shared, "page_tables": tables}[what], what, refusing(getattr(shared_fakes, what)))
+    if P % c.page_size or call == 1:
+        armed[0] = call
+        with pytest.raises(Refused):
+            c.fork(p.make(P), 4)
+        assert state() == kept
+        p.check()
+    if call == 1:
+        armed[0] = 1
+        with pytest.raises(Refused):
+            c.step(p.make(9), a, [5, 3, 1])
+        assert state() == kept
+        p.check()
+    armed[0] = 0
+    p.fork(P, 4)
+    p.step()
+    p.end(a)
+    p.step()
