@@ -114,15 +114,15 @@ class SharedCache:
         if pages > self._free:
             raise OutOfPages(f"need {pages} pages, {self._free} free")
 
-    def _attend(self, qkv, positions, slots, scale, lo: int, hi: int, **bounds) -> torch.Tensor:
-        """The rows' attention; ``lo`` to ``hi`` - 1 are the sequences that may have any, and groups count from ``lo``."""
+    def _attend(self, qkv, out, positions, slots, scale, lo: int, hi: int, **bounds) -> torch.Tensor:
+        """The rows' attention into ``out``; ``lo`` to ``hi`` - 1 are the sequences that may have any, and groups count from ``lo``."""
         from ..ops.kernels import qk_norm_rope_kv
         from ..ops.shared import attention_shared
 
         H, G, hd = self.H, self.G, self.hd
-        q = torch.empty((qkv.shape[0], H * hd), dtype=qkv.dtype, device=qkv.device)
+        q = self._out(qkv)
         qk_norm_rope_kv(qkv, None, None, 0.0, None, None, 0, False, positions, slots, q, self.pages, self.page_size, H, G, hd)
-        return attention_shared(q, self.pages, self.block_table[lo:hi], self._cu[lo:hi + 1], self._pos[lo:hi], out=torch.empty_like(q), scale=scale,
+        return attention_shared(q, self.pages, self.block_table[lo:hi], self._cu[lo:hi + 1], self._pos[lo:hi], out=out, scale=scale,
                                 page_size=self.page_size, H=H, G=G, hd=hd, **bounds)
 
     def _scale(self, scale: Optional[float], what: str) -> float:
@@ -137,13 +137,14 @@ class SharedCache:
         if not isinstance(qkv, torch.Tensor) or qkv.device != self.device or qkv.dtype != self.pages.dtype or tuple(qkv.shape) != (n, w) or qkv.stride(1) != 1:
             raise CacheError(f"{what}: rows [{n}, {w}] of queries, keys and values in {self.pages.dtype} on {self.device} were announced, got "
                              f"{tuple(qkv.shape) if isinstance(qkv, torch.Tensor) else qkv!r}")
-        if n > self._most:
-            raise CacheError(f"{what}: {n} rows, a call takes {self._most}")
+
+    def _out(self, qkv: torch.Tensor) -> torch.Tensor:
+        return torch.empty((qkv.shape[0], self.H * self.hd), dtype=qkv.dtype, device=qkv.device)
 
     # -- the operators
     @_on_its_device
     def fork(self, qkv: torch.Tensor, n: int, scale: Optional[float] = None) -> Tuple[torch.Tensor, List[int]]:
-        """A prompt's rows [tokens, (num_heads + 2 num_kv_heads) * head_dim] (queries, keys, values), and ``n`` continuations of it: the rows'
+        """A prompt's rows [tokens, (num_heads + 2 num_kv_heads) * head_dim] (queries, keys, values; as many as there are), and ``n`` continuations of it: the rows'
         causal attention [tokens, num_heads * head_dim], and the continuations' numbers.  ``scale``: head_dim ** -0.5 unless given.  Nothing is taken
         by a call that fails, for instance where the pages do not suffice (:class:`~.manager.OutOfPages`) or no ``n + 1`` sequences in a row are free (:class:`~.manager.OutOfSlots`)."""
         P = qkv.shape[0] if isinstance(qkv, torch.Tensor) and qkv.dim() == 2 else 0
@@ -163,10 +164,12 @@ class SharedCache:
             raise OutOfSlots(f"no {n + 1} sequences in a row are free")
         seqs = list(range(at + 1, at + 1 + n))
         try:
-            positions, slots, _ = self._move({at: P}, P)
-            none = self._upload(np.zeros(1))
-            out = self._attend(qkv, positions, slots, scale, at, at + 1, group_seqs=none, prefix_len=none[:0], max_rows=P, max_group_rows=P,
-                               max_prefix=0, max_own=P)
+            none, out = self._upload(np.zeros(1)), self._out(qkv)
+            for a in range(0, P, self._most):                       # (as many rows as a call takes)
+                b = min(P, a + self._most)
+                positions, slots, _ = self._move({at: b - a}, b - a)
+                self._attend(qkv[a:b], out[a:b], positions, slots, scale, at, at + 1, group_seqs=none, prefix_len=none[:0], max_rows=b - a,
+                             max_group_rows=b - a, max_prefix=0, max_own=b)
             # the continuations' tables begin with the prompt's whole pages; a page that it ends in each has for itself
             rows = slice(at + 1, at + 1 + n)
             self.block_table[rows, :whole] = self.block_table[at, :whole]
@@ -175,9 +178,11 @@ class SharedCache:
             for s in seqs:
                 self._length[s], self._own[s] = whole * self.page_size, whole
             if tail:
-                for a in range(0, n, self._most // tail):           # (as many rows as a call takes)
-                    part = seqs[a:a + self._most // tail]
-                    self._move({s: tail for s in part}, len(part) * tail)
+                for a in range(0, tail, self._most):
+                    rows_each = min(tail - a, self._most)
+                    for i in range(0, n, self._most // rows_each):
+                        part = seqs[i:i + self._most // rows_each]
+                        self._move({s: rows_each for s in part}, len(part) * rows_each)
                 self.pages[self.block_table[rows, whole].long(), :, :, :tail] = self.pages[self.block_table[at, whole].long(), :, :, :tail]
         except BaseException:
             self._forget([at] + seqs)
@@ -198,6 +203,8 @@ class SharedCache:
         if len(rows) != len(seqs) or min(rows, default=1) < 1:
             raise CacheError("step: a positive number of rows for every continuation")
         self._rows(qkv, sum(rows), "step")
+        if sum(rows) > self._most:
+            raise CacheError(f"step: {sum(rows)} rows, a call takes {self._most}")
         scale = self._scale(scale, "step")
         if not seqs:
             return qkv[:, :self.H * self.hd].clone()
@@ -217,7 +224,7 @@ class SharedCache:
         prefix, lo, hi = [self._length[prompts[i]] for i in starts], seqs[0], seqs[-1] + 1
         positions, slots, groups = self._move(dict(zip(seqs, rows)), sum(rows), [seqs[i] - lo for i in starts] + [hi - lo] + prefix)
         try:
-            return self._attend(qkv, positions, slots, scale, lo, hi, group_seqs=groups[:len(starts) + 1], prefix_len=groups[len(starts) + 1:],
+            return self._attend(qkv, self._out(qkv), positions, slots, scale, lo, hi, group_seqs=groups[:len(starts) + 1], prefix_len=groups[len(starts) + 1:],
                                 max_rows=max(rows), max_group_rows=max(group_rows), max_prefix=max(prefix),
                                 max_own=max(a - self._length[p] for a, p in zip(after, prompts)))
         except BaseException:

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import shared_fakes
+from kappai_b200.cache import CacheError
 from shared_fakes import Program
 
 
@@ -115,3 +116,18 @@ def test_a_call_that_fails_leaves_everything_as_it_was(what, call, P, monkeypatc
     p.step()
     p.end(a)
     p.step()
+
+
+@pytest.mark.parametrize("page_size", [8, 150])
+def test_a_prompt_of_more_rows_than_a_call_takes(page_size):
+    """... runs in portions, as do the copies of the page that it ends in."""
+    p = program(page_size=page_size)
+    p.c._most = 40
+    p.fork(133, 5)
+    p.fork(40, 2)
+    p.fork(41, 3)
+    p.step()
+    p.step(None, [3] * 10)
+    with pytest.raises(CacheError):
+        p.c.step(p.make(50), None, [5] * 10)
+    p.check()

@@ -67,3 +67,19 @@ def test_long_prompts_in_caches_of_many_places(P, n, H, G, hd):
         want, off, _ = p.attend(p.kv[s], z[a:b])
         p.near(out[a:b], want, off)
     p.c.check()
+
+
+def test_a_prompt_of_more_rows_than_a_call_takes():
+    """A very long text and questions about it: the text runs in portions."""
+    P, n, H, G, hd = 120001, 24, 16, 8, 64
+    p = program(H, G, hd, page_size=64, max_len=P + 1000, n_pages=P // 64 + 2 * n + 10, max_seqs=n + 1)
+    x, some = p.make(P), [0, 65534, 65535, 65536, P - 1]
+    out, seqs = p.c.fork(x, n)
+    want, off, whole = p.attend(None, x, some)
+    p.near(out[some], want, off)
+    y = p.make(n)
+    out = p.c.step(y)
+    for i in (0, 11, n - 1):
+        want, off, _ = p.attend(whole, y[i:i + 1])
+        p.near(out[i:i + 1], want, off)
+    p.c.check()
