@@ -146,7 +146,8 @@ class SharedCache:
     def fork(self, qkv: torch.Tensor, n: int, scale: Optional[float] = None) -> Tuple[torch.Tensor, List[int]]:
         """A prompt's rows [tokens, (num_heads + 2 num_kv_heads) * head_dim] (queries, keys, values; as many as there are), and ``n`` continuations of it: the rows'
         causal attention [tokens, num_heads * head_dim], and the continuations' numbers.  ``scale``: head_dim ** -0.5 unless given.  Nothing is taken
-        by a call that fails, for instance where the pages do not suffice (:class:`~.manager.OutOfPages`) or no ``n + 1`` sequences in a row are free (:class:`~.manager.OutOfSlots`)."""
+        by a call that fails, for instance where the pages do not suffice (:class:`~.manager.OutOfPages`) or fewer than ``n + 1`` sequences are free
+        (:class:`~.manager.OutOfSlots`)."""
         P = qkv.shape[0] if isinstance(qkv, torch.Tensor) and qkv.dim() == 2 else 0
         if P < 1 or n < 1 or P > self.max_len:
             raise CacheError(f"fork: a prompt of {P} tokens (at most {self.max_len}) with {n} continuations")
@@ -154,15 +155,12 @@ class SharedCache:
         scale = self._scale(scale, "fork")
         whole, tail = divmod(P, self.page_size)
         self._room(self._blocks(P) + (n if tail else 0))
-        run, at = 0, -1
-        for s, p in enumerate(self._prompt):
-            run = run + 1 if p < 0 else 0
-            if run == n + 1:
-                at = s - n
-                break
-        if at < 0:
-            raise OutOfSlots(f"no {n + 1} sequences in a row are free")
-        seqs = list(range(at + 1, at + 1 + n))
+        free = [s for s, p in enumerate(self._prompt) if p < 0]
+        if len(free) <= n:
+            raise OutOfSlots(f"need {n + 1} sequences, {len(free)} are free")
+        # (in a row where there are so many: a step reads a prompt once for each stretch of its continuations)
+        first = next((i for i in range(len(free) - n) if free[i + n] - free[i] == n), 0)
+        at, seqs = free[first], free[first + 1:first + 1 + n]
         try:
             none, out = self._upload(np.zeros(1)), self._out(qkv)
             for a in range(0, P, self._most):                       # (as many rows as a call takes)
@@ -171,10 +169,10 @@ class SharedCache:
                 self._attend(qkv[a:b], out[a:b], positions, slots, scale, at, at + 1, group_seqs=none, prefix_len=none[:0], max_rows=b - a,
                              max_group_rows=b - a, max_prefix=0, max_own=b)
             # the continuations' tables begin with the prompt's whole pages; a page that it ends in each has for itself
-            rows = slice(at + 1, at + 1 + n)
+            rows = self._upload(np.asarray(seqs)).long()
             self.block_table[rows, :whole] = self.block_table[at, :whole]
-            self.own_from[rows] = whole
-            self.lengths[rows] = whole * self.page_size
+            self.own_from.index_fill_(0, rows, whole)
+            self.lengths.index_fill_(0, rows, whole * self.page_size)
             for s in seqs:
                 self._length[s], self._own[s] = whole * self.page_size, whole
             if tail:

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import shared_fakes
-from kappai_b200.cache import CacheError
+from kappai_b200.cache import CacheError, OutOfSlots
 from shared_fakes import Program
 
 
@@ -131,3 +131,20 @@ def test_a_prompt_of_more_rows_than_a_call_takes(page_size):
     with pytest.raises(CacheError):
         p.c.step(p.make(50), None, [5] * 10)
     p.check()
+
+
+def test_a_fork_into_scattered_places():
+    """Places that are free suffice, in a row or not."""
+    p = program(max_seqs=9)
+    a, b, c = p.fork(20, 2), p.fork(16, 1), p.fork(9, 3)
+    p.step()
+    p.end(a)
+    p.end(c[1:])
+    d = p.fork(30, 4)                                    # a prompt and four, where three and two are free
+    p.step()
+    p.step(sorted([d[0], b[0], c[0], d[3]]), [2, 1, 3, 1])
+    with pytest.raises(OutOfSlots):
+        p.c.fork(p.make(3), 1)
+    p.end(d[1:])
+    p.fork(5, 2)
+    p.step()
