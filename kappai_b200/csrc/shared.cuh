@@ -68,9 +68,23 @@ __device__ __forceinline__ float sh_exp2(float x) {
 __device__ __forceinline__ int sh_chunk(const ShArgs& p, int lane) {
     if (!p.budget) return p.chunk;
     const int n = lane < p.n_groups ? (sh_prefix(p, lane) + 127) / 128 : 0, per = p.group_tiles * p.G;
-    int c = (int)max((long long)p.chunk / 128, ((long long)__reduce_add_sync(0xffffffffu, n) * per + p.budget - 1) / p.budget);
-    while ((long long)__reduce_add_sync(0xffffffffu, (n + c - 1) / c) * per > p.budget) c++;        // (ends: a chunk a prefix fits)
-    return c * 128;
+    // The least length with which the chunks are within the budget (a chunk a prefix always is), in doubled steps and then by bisection.  Mostly it is one of
+    // the first (bisection alone takes 1.2 us longer then); with one prefix much longer than the others it is the hundredth: one of 200000 keys and 15 of
+    // 300, 4 kv heads, counted up in ones 76 us, 71.5 so.
+    auto fits = [&](int c) { return (long long)__reduce_add_sync(0xffffffffu, (n + c - 1) / c) * per <= p.budget; };
+    int lo = (int)max((long long)p.chunk / 128, ((long long)__reduce_add_sync(0xffffffffu, n) * per + p.budget - 1) / p.budget);
+    if (!fits(lo)) {
+        int hi = lo + 1;
+#pragma unroll 1
+        for (int step = 2; !fits(hi); step *= 2) { lo = hi; hi += step; }       // (fits at the longest prefix at last)
+#pragma unroll 1
+        while (hi - lo > 1) {                                // (lo: does not fit; hi: does)
+            const int mid = (lo + hi) >> 1;
+            if (fits(mid)) hi = mid; else lo = mid;
+        }
+        lo = hi;
+    }
+    return lo * 128;
 }
 // the page of a key and its place there
 __device__ __forceinline__ int sh_block(const ShArgs& p, int key) { return p.ps_log2 >= 0 ? key >> p.ps_log2 : key / p.ps; }
