@@ -742,18 +742,25 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant_
     const int n_cl = gridDim.x, part = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const ShPlace at(p);
     const int g = at.g, seq = at.i / p.tiles, c0 = at.i % p.tiles * BM, R = p.H / p.G;
-    if (seq >= p.n_seq) return;                              // (a whole cluster; the first place's CTAs wait for the first launch as all with rows do)
+    if (seq >= p.n_seq) return;
+    // (all of these loads under way together)
+    const bool look = tid < p.n_groups;
+    int from = look ? p.group_seqs[tid] : 0, to = look ? p.group_seqs[tid + 1] : 0, len = look ? sh_prefix(p, tid) : 0;
+    const int row0 = sh_row(p, seq), n_cols = max(0, sh_row(p, seq + 1) - row0) * R, pos0 = max(-p.n, min(p.seg_pos[seq], p.width * p.ps));
+    // Clusters without rows make room for those that have some.  The first place's stay: they wait for the first launch as all with rows do, so that this one
+    // ends behind it, which what comes next relies on.
+    const bool work = c0 < n_cols;                           // (the same for all CTAs of a cluster)
+    if (!work && at.i) return;
     sh_init(sm);
     if (tid == 0) s_group = -1;
     __syncthreads();
-    for (int i = tid; i < p.n_groups; i += THREADS) {        // (the three loads under way together)
-        const int from = p.group_seqs[i], to = p.group_seqs[i + 1], len = sh_prefix(p, i);
+    for (int i = tid;;) {
         if (from <= seq && seq < to) { s_group = i; s_prefix = len; }
+        if ((i += THREADS) >= p.n_groups) break;
+        from = p.group_seqs[i]; to = p.group_seqs[i + 1]; len = sh_prefix(p, i);
     }
-    const int row0 = sh_row(p, seq), n_cols = max(0, sh_row(p, seq + 1) - row0) * R, pos0 = max(-p.n, min(p.seg_pos[seq], p.width * p.ps));
     __syncthreads();
     const int group = s_group, P = group >= 0 ? s_prefix : 0;
-    const bool work = c0 < n_cols;                           // (the same for all CTAs of a cluster)
     if (work) {
         const int last = pos0 + (min(n_cols, c0 + BM) - 1) / R;                     // position of the tile's last row
         const int end = max(P, (int)min((long long)last + 1, (long long)p.width * p.ps));

@@ -1,8 +1,9 @@
 """Attention behind a shared prefix at its edges: more places for sequences, groups and tiles of columns than a grid's second and third axis count.  Tolerances are those of
 test_shared_gpu.py."""
 import pytest
+import torch
 
-from kappai_b200.ops.shared import shared_cut
+from kappai_b200.ops.shared import attention_shared, shared_cut
 from test_shared_gpu import DT, Batch, spread
 
 pytestmark = pytest.mark.gpu
@@ -25,3 +26,23 @@ def test_many_groups_of_which_one_has_many_rows(hd, dtype):
 def test_prefixes_of_which_one_is_much_longer(hd, G):
     """The chunks' length is found among hundreds."""
     Batch([(17, spread(1, 5, 5))] * 15 + [(50001, spread(1, 9, 5))] + [(300, spread(1, 5, 5))] * 12, 4 * G, G, hd, 64, "bf16", seed=hd).check()
+
+
+@pytest.mark.parametrize("hd,dtype", [(64, "bf16"), (128, "bf16"), (96, "bf16"), (64, "f32")])
+def test_calls_one_behind_another_in_which_few_places_have_rows(hd, dtype):
+    """Calls that follow one another use the same scratch: each ends before the next one's kernels write there, whichever of its places have rows, or none."""
+    last = Batch([(3000, [(9, 0)] * 60 + [(40, 3)])], 8, 2, hd, 64, dtype, seed=1)
+    first = Batch([(2500, [(30, 3)] + [(9, 0)] * 60)], 8, 2, hd, 64, dtype, seed=2)
+    none = Batch([(2500, [(9, 1)] * 40)], 8, 2, hd, 64, dtype, seed=3)
+    want, out = [b.check() for b in (last, first)], []
+    a = none.args()
+    a["cu_rows"].zero_()
+    for i in range(30):
+        for j, b in enumerate((last, first)):
+            out.append((j, b.args()))
+    torch.cuda.synchronize()
+    for j, args in out:
+        attention_shared(**args)
+        attention_shared(**a)
+    torch.cuda.synchronize()
+    assert all(torch.equal(args["out"], want[j]) for j, args in out) and (a["out"] == 7).all()
