@@ -95,9 +95,9 @@ def shared_cut(n_groups: int, n_seq: int, max_rows: int, max_group_rows: int, ma
 
 
 def shared_tc_ok(ldq: int, q: int, n_pages: int, page_size: int, G: int, R: int, hd: int) -> bool:
-    """Can the tcgen05 form take the prefix of a call with bfloat16 rows (heads of 64 or 128, rows ``ldq`` values apart on 16-byte boundaries from address ``q`` on, pages of
-    which a tile of 128 keys is made)?"""
-    return (USE_TC_SHARED and (hd == 64 or hd == 128) and R <= 128 and ldq % 8 == 0 and q % 16 == 0
+    """Can the tcgen05 form take the prefix of a call with bfloat16 rows (heads of 64 or 128, rows ``ldq`` values apart, one behind the other, on 16-byte boundaries from address ``q``
+    on, pages of which a tile of 128 keys is made)?"""
+    return (USE_TC_SHARED and (hd == 64 or hd == 128) and R <= 128 and ldq % 8 == 0 and ldq >= G * R * hd and q % 16 == 0
             and page_size % 8 == 0 and (page_size % 128 == 0 or 128 % page_size == 0) and n_pages * 2 * G * page_size < 2 ** 31 - 1)
 
 

@@ -46,3 +46,15 @@ def test_calls_one_behind_another_in_which_few_places_have_rows(hd, dtype):
         attention_shared(**a)
     torch.cuda.synchronize()
     assert all(torch.equal(args["out"], want[j]) for j, args in out) and (a["out"] == 7).all()
+
+
+@pytest.mark.parametrize("hd,dtype", [(64, "bf16"), (128, "bf16"), (64, "f32")])
+@pytest.mark.parametrize("step", [0, 8])
+def test_rows_that_lie_in_one_another(step, hd, dtype):
+    """One row for all, and rows that begin within the one before."""
+    b = Batch([(333, spread(1, 90, 20))], 8, 2, hd, 16, dtype, seed=5)
+    n, w = b.q.shape
+    flat = torch.randn(w + n * step, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(b.q.dtype)
+    q = flat.as_strided((n, w), (step, 1))
+    b.q = q.contiguous()
+    b.check(attention_shared(**b.args(q=q)))
