@@ -10,7 +10,8 @@
 // pages and the rows are shared out over all threads, each of which finds its sequence by bisection.  CTAs are one cluster: its barrier stands between
 // reading the lengths and writing them, and between putting pages on the stack and taking them.  Launch and latency bound: a chain of loads,
 // the sums, the bisection and a page's load.  64 sequences with a row each 4 us, 2000 with 60000 rows 9.8.  Nothing happens, and `status` says why, where pages are short (1), a table is too
-// narrow (2), the rows have no room (4) or lengths or counts make no sense (8): bits that are added up.
+// narrow (2), the rows have no room (4) or lengths or counts make no sense (8): bits that are added up (the rows and
+// pages of a sequence with 2 or 8 are not counted for the others).
 #include "common.cuh"
 
 #define PT_MAX_SEQS 8192

@@ -114,7 +114,8 @@ def attention_shared(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Te
     their end (``seg_pos[i] >= prefix_len[g]``).  A sequence in no group shares nothing.  All int32 on the device.
 
     Host bounds: ``max_rows`` rows of a sequence, ``max_group_rows`` rows of a group, ``max_prefix`` shared keys, ``max_own`` keys of a sequence
-    behind them.  ``out`` is other memory than ``q``; rows behind ``cu_rows[-1]`` are left as they were, and a row that reads no key gives zeros.  float32 or bfloat16,
+    behind them.  ``out`` is other memory than ``q``; rows behind ``cu_rows[-1]`` are left as they were, and a row that reads no key gives zeros.  Keys and values
+    that a row does not read may be anything; where it reads an infinite value the output is infinite or NaN.  float32 or bfloat16,
     accumulated in float32; the sums' order is fixed, so the same call gives the same bits."""
     if G < 1 or H < 1 or H % G:
         raise KernelError(f"attention_shared: {H} query heads over {G} kv heads")

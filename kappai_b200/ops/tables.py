@@ -47,7 +47,8 @@ def page_tables(block_table: torch.Tensor, length: torch.Tensor, delta: torch.Te
     and slot (page * page_size + place); behind the last row these hold 0, -1 and -1.
 
     ``status`` [1] gets 0, or the sum of what kept the step from being made: 1 too few free pages, 2 a block table too narrow, 4 more rows than
-    room for them, 8 lengths or counts that make no sense.  Then nothing changes, and the step has no rows."""
+    room for them, 8 lengths or counts that make no sense.  A sequence that adds 2 or 8 asks for no rows and pages: 1 and 4 are about the others.
+    Then nothing changes, and the step has no rows."""
     dev, i32 = _here(block_table), torch.int32
     given = (block_table, length, delta, free_pages, n_free, cu_rows, seg_pos, row_seg, positions, slot_map, status) if own_from is None else (
         block_table, length, delta, free_pages, n_free, cu_rows, seg_pos, row_seg, positions, slot_map, status, own_from)

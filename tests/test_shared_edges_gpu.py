@@ -58,3 +58,15 @@ def test_rows_that_lie_in_one_another(step, hd, dtype):
     q = flat.as_strided((n, w), (step, 1))
     b.q = q.contiguous()
     b.check(attention_shared(**b.args(q=q)))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("seqs", [3, 12, 30, 60])
+@pytest.mark.parametrize("hd", [64, 128, 96])
+def test_values_of_the_prefix_that_are_not_finite(hd, seqs, bad):
+    """They reach every row, in their place and no other, and nothing there is finite (NaN perhaps where the definition gives an infinite one)."""
+    b = Batch([(300, spread(1, 40, seqs)), (50, spread(1, 9, 3))], 8, 2, hd, 64, "bf16", seed=3)
+    for i in range(seqs):
+        b.v[i][17, 1, 5] = bad
+    b.cache[int(b.table[0, 0]), 1, 1, 17, 5] = bad
+    b.check()
