@@ -111,18 +111,21 @@ __device__ __forceinline__ float lp_min3(float a, float b, float c) {
     return d;
 }
 
-// A reference: r, and r log2 e as the fma takes it.  Beyond +-1e6 (`wild`) what that is rounded by would no longer be small beside the differences, and these
-// are taken themselves instead.  All terms of a sum are of one kind: what r log2 e was rounded by (`off`, up to 0.06) is put right for the sum as a whole.
+// A reference r: what sums are relative to is 2^(r log2 e), with r log2 e as the fma takes it, `rl`.  Beyond +-1e6 (`wild`) what that is rounded by would no longer
+// be small beside the differences, and these are taken themselves instead: r is `sub`, and rl is 0.  All terms of a sum are of one kind: what rl is off by,
+// up to 0.06, is put right for the sum as a whole.
 struct LpRef {
-    float r, rl;
-    __device__ __forceinline__ LpRef(float x) { r = x; rl = x * LP_LOG2E; }
-    __device__ __forceinline__ bool wild() const { return !(fabsf(r) <= 1e6f); }
-    __device__ __forceinline__ float y(float x) const { return lp_max_nan(wild() ? (x - r) * LP_LOG2E : fmaf(x, LP_LOG2E, -rl), LP_LEAST); }
-    __device__ __forceinline__ float off() const { return wild() ? 0.f : fmaf(-r, LP_LOG2E, rl); }       // (exact: what a rounding leaves is a float32)
-    // by how much less (a power of two) sums count that were relative to `o`, o.r <= r
-    __device__ __forceinline__ float from(const LpRef& o) const {
-        return fmaxf(wild() || o.wild() ? (o.r - r) * LP_LOG2E + (o.off() - off()) : o.rl - rl, LP_LEAST);
+    float r, sub, rl;
+    __device__ __forceinline__ LpRef(float x) {
+        const bool wild = !(fabsf(x) <= 1e6f);
+        r = x;
+        sub = wild ? x : 0.f;
+        rl = wild ? 0.f : x * LP_LOG2E;
     }
+    __device__ __forceinline__ bool wild() const { return sub != 0.f; }
+    __device__ __forceinline__ float y(float x) const { return lp_max_nan(fmaf(x - sub, LP_LOG2E, -rl), LP_LEAST); }
+    // by how much less (a power of two) sums count that were relative to `o`, o.r <= r (of either kind: one rounding, of the result)
+    __device__ __forceinline__ float from(const LpRef& o) const { return fmaxf(fmaf(o.sub - sub, LP_LOG2E, o.rl - rl), LP_LEAST); }
 };
 // sums, and what becomes of them when their reference moves by y <= 0
 __device__ __forceinline__ void lp_move(float& s, float& w, float y) {
@@ -500,7 +503,7 @@ token_logprobs_kernel(const LpArgs p) {
         rank += *cluster.map_shared_rank(&s_count, i);
     }
     // The last differences are taken in 64 bits, each rounded once: r, log2 e and y = x log2 e - rl as they were rounded add up to (r log2 e - rl) in y.
-    const double off = (double)z.off(), log_s = log((double)S) + off * 0.6931471805599453;
+    const double off = z.wild() ? 0.0 : (double)z.rl - (double)z.r * (double)LP_LOG2E, log_s = log((double)S) + off * 0.6931471805599453;
     const bool bad = !(S >= 0.f), none = S == 0.f;                   // a NaN or +inf among the logits; nothing but -inf
     auto logprob = [&](float f) { return none ? -INFINITY : (float)(((double)f - (double)z.r) - log_s); };
     if (tid == 0) {
